@@ -53,7 +53,10 @@ enum {
 };
 
 /* Element type codes for activation inputs. */
-enum { H3B_BF16 = 0, H3B_F16 = 1 };
+enum { H3B_BF16 = 0, H3B_F16 = 1, H3B_F32 = 2 /* h3b_kv8_read's output only */ };
+
+/* Code types of the 8-bit key/value cache. */
+enum { H3B_KV_INT8 = 0, H3B_KV_E4M3 = 1 };
 
 /* GEMM epilogue modes (applied in fp32 before the single bf16 rounding). */
 enum {
@@ -250,6 +253,99 @@ H3B_API int h3b_attention_fwd(const void* q, const void* k, const void* v, void*
 H3B_API int h3b_qk_rmsnorm_rope(void* q, void* k, int64_t s, int64_t heads, int64_t seq_stride, int64_t head_stride,
                         const void* q_weight, const void* k_weight, float eps, const float* pos,
                         int64_t pos_offset, const float* inv_freq, int n_t, int n_h, h3b_stream_t stream);
+
+/* --------------------------------------------------------- cross attention */
+
+/*
+ * Attention of query tokens to an encoder's states of another length, for a
+ * batch of samples:
+ *   o[b,i,h,:] = sum_j p_j v[b,j,g,:],  p = softmax over the kept keys j of
+ *   scale * q[b,i,h,:].k[b,j,g,:],  g = h / (heads / kv_heads)
+ * q, o: [batch, s_q, heads, head_dim], k, v: [batch, s_kv, kv_heads,
+ * head_dim], bf16 or f16 (dtype: H3B_BF16 / H3B_F16, one type for all), fp32
+ * scores, softmax and sums; head_dim 64 or 128.  Element (b, s, h, d) of q
+ * lies at q + b*q_batch_stride + s*q_seq_stride + h*q_head_stride + d; k and
+ * v share strides (the halves of one projection do).
+ * Kept keys: j < kv_lens[b] (int32 [batch], device, clamped to 0..s_kv; NULL:
+ * all) and key_mask[b*mask_stride + j] != 0 (bytes, device; NULL: all).  What
+ * a left-out key or value holds is never used, NaN included.  A row without
+ * any kept key gives o = 0 and lse = -inf.  lse (optional, fp32 [batch,
+ * heads, s_q], natural log) is what the backward pass needs.  No reference
+ * counterpart: its block attends over one joint sequence (model/dit.py:
+ * 156-289).
+ * Strides % 8 == 0 and > 0 (any value along an axis of extent 1), pointers
+ * 16-byte aligned.  workspace: h3b_cross_attention_workspace() bytes (may be
+ * 0), 16-byte aligned, free to reuse when the call's work is done.
+ */
+H3B_API int h3b_cross_attention_workspace(int64_t batch, int64_t heads, int64_t kv_heads, int64_t head_dim,
+                                          int64_t s_q, int64_t s_kv, int64_t* bytes);
+H3B_API int h3b_cross_attention_fwd(const void* q, const void* k, const void* v, void* o, float* lse, int dtype,
+                                    int64_t batch, int64_t heads, int64_t kv_heads, int64_t head_dim, int64_t s_q,
+                                    int64_t s_kv, int64_t q_batch_stride, int64_t q_seq_stride,
+                                    int64_t q_head_stride, int64_t kv_batch_stride, int64_t kv_seq_stride,
+                                    int64_t kv_head_stride, int64_t o_batch_stride, int64_t o_seq_stride,
+                                    int64_t o_head_stride, const int32_t* kv_lens, const uint8_t* key_mask,
+                                    int64_t mask_stride, float scale, void* workspace, int64_t workspace_bytes,
+                                    h3b_stream_t stream);
+
+/* --------------------------------------------- 8-bit key/value cache */
+
+/*
+ * The cache: for K and for V, codes [num_blocks, kv_heads, block_tokens,
+ * head_dim] (code_type H3B_KV_INT8: int8, H3B_KV_E4M3: e4m3) and scales fp32
+ * [num_blocks, kv_heads]; a value is code * scale.  table (int32 [batch,
+ * max_blocks], device) gives the block of tokens j*block_tokens .. of each
+ * sequence; an entry outside 0..num_blocks-1 means no block (its tokens are
+ * neither written nor attended, and read as 0).  block_tokens 32, 64 or 128,
+ * head_dim 64 or 128.  The reference keeps no such cache.
+ */
+
+/*
+ * Quantises k, v [batch, n, kv_heads, head_dim] (x_dtype bf16 / f16, shared
+ * strides, % 8 == 0) into positions start[b] .. start[b] + count[b] - 1 of
+ * each sequence (count NULL: n each; at most n).  Per touched (block, head),
+ * K and V apart: s' = max(amax of the new rows, 1e-12) / top (127 or 448);
+ * scale = max(old scale, s') if the block holds tokens before start[b], else
+ * s'; new codes round(x / scale), codes held before round(code * old / scale),
+ * half to even, in IEEE fp32, int8 clamped to +-127, e4m3 saturating; rows of
+ * the block behind the last token are zeroed.  Values are expected finite.
+ * A block belongs to one sequence.
+ */
+H3B_API int h3b_kv8_append(const void* k, const void* v, int x_dtype, int64_t batch, int64_t n, int64_t kv_heads,
+                           int64_t head_dim, int64_t batch_stride, int64_t seq_stride, int64_t head_stride,
+                           uint8_t* k_codes, uint8_t* v_codes, float* k_scale, float* v_scale, int code_type,
+                           int64_t num_blocks, int64_t block_tokens, const int32_t* table, int64_t max_blocks,
+                           const int32_t* start, const int32_t* count, h3b_stream_t stream);
+
+/*
+ * The cache's values in the order of the tokens: k_out, v_out dense [batch,
+ * max_len, kv_heads, head_dim] in out_dtype (H3B_BF16, H3B_F16, H3B_F32),
+ * code * scale rounded once, 0 behind lens[b].
+ */
+H3B_API int h3b_kv8_read(const uint8_t* k_codes, const uint8_t* v_codes, const float* k_scale, const float* v_scale,
+                         int code_type, int64_t num_blocks, int64_t kv_heads, int64_t block_tokens,
+                         int64_t head_dim, const int32_t* table, int64_t max_blocks, const int32_t* lens,
+                         int64_t batch, int64_t max_len, void* k_out, void* v_out, int out_dtype,
+                         h3b_stream_t stream);
+
+/*
+ * Attention of q [batch, s_q, heads, head_dim] (dtype, strides, o and lse as
+ * h3b_cross_attention_fwd) over the lens[b] tokens of each sequence's cache.
+ * causal != 0: the queries are the sequence's last s_q tokens (their keys
+ * already appended), query i sees keys j <= lens[b] - s_q + i.  A row that
+ * sees no key gives o = 0, lse = -inf.  The codes enter the products exactly;
+ * the scales are applied to scores and weights in fp32.
+ */
+H3B_API int h3b_kv8_attention_workspace(int64_t batch, int64_t heads, int64_t kv_heads, int64_t head_dim,
+                                        int64_t s_q, int64_t block_tokens, int64_t max_blocks, int64_t* bytes);
+H3B_API int h3b_kv8_attention(const void* q, void* o, float* lse, int dtype, int64_t batch, int64_t heads,
+                              int64_t kv_heads, int64_t head_dim, int64_t s_q, int64_t q_batch_stride,
+                              int64_t q_seq_stride, int64_t q_head_stride, int64_t o_batch_stride,
+                              int64_t o_seq_stride, int64_t o_head_stride, const uint8_t* k_codes,
+                              const uint8_t* v_codes, const float* k_scale, const float* v_scale, int code_type,
+                              int64_t num_blocks, int64_t block_tokens, const int32_t* table, int64_t max_blocks,
+                              const int32_t* lens, int causal, float scale, void* workspace,
+                              int64_t workspace_bytes, h3b_stream_t stream);
 
 /* ------------------------------------------------------- block elementwise */
 

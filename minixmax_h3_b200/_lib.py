@@ -48,6 +48,15 @@ SIGNATURES: dict[str, list] = {
                                       c_ptr, c_ptr, c_ptr],
     "h3b_rmsnorm_modulate_quant_nvfp4_noalloc": [c_ptr, c_i64, c_i64, c_i64, c_ptr, c_ptr, c_ptr, c_i64, c_ptr,
                                                  c_f32, c_ptr, c_ptr, c_ptr, c_int, c_ptr],
+    "h3b_cross_attention_workspace": [c_i64] * 6 + [c_ptr],
+    "h3b_cross_attention_fwd": [c_ptr] * 5 + [c_int] + [c_i64] * 15 + [c_ptr, c_ptr, c_i64, c_f32, c_ptr, c_i64, c_ptr],
+    "h3b_kv8_append": [c_ptr, c_ptr, c_int] + [c_i64] * 7 + [c_ptr] * 4 + [c_int, c_i64, c_i64, c_ptr, c_i64, c_ptr,
+                                                                           c_ptr, c_ptr],
+    "h3b_kv8_read": [c_ptr] * 4 + [c_int] + [c_i64] * 4 + [c_ptr, c_i64, c_ptr, c_i64, c_i64, c_ptr, c_ptr, c_int,
+                                                           c_ptr],
+    "h3b_kv8_attention_workspace": [c_i64] * 7 + [c_ptr],
+    "h3b_kv8_attention": [c_ptr] * 3 + [c_int] + [c_i64] * 11 + [c_ptr] * 4 + [c_int, c_i64, c_i64, c_ptr, c_i64, c_ptr,
+                                                                               c_int, c_f32, c_ptr, c_i64, c_ptr],
     "h3b_selftest_wait_timeout": [c_ptr] * 7 + [c_i64] * 3 + [c_ptr],
     "h3b_attention_merge_lse": [c_ptr, c_ptr, c_ptr, c_ptr, c_i64, c_i64, c_int, c_ptr, c_ptr, c_ptr],
 }
@@ -96,7 +105,7 @@ def lib() -> ctypes.CDLL:
 
 
 # Entry points that launch no kernel of this library.
-_NO_LAUNCH = {"h3b_version", "h3b_device_status"}
+_NO_LAUNCH = {"h3b_version", "h3b_device_status", "h3b_cross_attention_workspace", "h3b_kv8_attention_workspace"}
 LAUNCHES = [0]  # kernels this process has launched through the ABI
 
 

@@ -74,6 +74,24 @@ int encode_3d(CUtensorMap* map, CUtensorMapDataType dtype, const void* base, uin
   return r == CUDA_SUCCESS ? H3B_OK : H3B_ERR_TMAP;
 }
 
+int encode_4d(CUtensorMap* map, CUtensorMapDataType dtype, const void* base, const uint64_t (&dims)[4],
+              const uint64_t (&strides_bytes)[3], const uint32_t (&box)[4], CUtensorMapSwizzle swizzle) {
+  auto fn = encode_fn();
+  if (fn == nullptr) return H3B_ERR_LAUNCH;
+  cuuint64_t d[4];
+  cuuint64_t st[3];
+  cuuint32_t b[4];
+  cuuint32_t estr[4] = {1, 1, 1, 1};
+  for (int i = 0; i < 4; ++i) {
+    d[i] = dims[i];
+    b[i] = box[i];
+    if (i > 0) st[i - 1] = strides_bytes[i - 1];
+  }
+  CUresult r = fn(map, dtype, 4, const_cast<void*>(base), d, st, b, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle,
+                  CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  return r == CUDA_SUCCESS ? H3B_OK : H3B_ERR_TMAP;
+}
+
 }  // namespace h3b
 
 extern "C" int h3b_version(void) { return 100; }

@@ -28,6 +28,10 @@ int encode_3d(CUtensorMap* map, CUtensorMapDataType dtype, const void* base, uin
               uint64_t d2, uint64_t s1_bytes, uint64_t s2_bytes, uint32_t box_inner, uint32_t box_d1,
               uint32_t box_d2, CUtensorMapSwizzle swizzle);
 
+// 4D variant: dims (inner, d1, d2, d3), byte strides of d1..d3.
+int encode_4d(CUtensorMap* map, CUtensorMapDataType dtype, const void* base, const uint64_t (&dims)[4],
+              const uint64_t (&strides_bytes)[3], const uint32_t (&box)[4], CUtensorMapSwizzle swizzle);
+
 inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
 inline int launch_status() {

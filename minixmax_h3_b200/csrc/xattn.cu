@@ -1,0 +1,154 @@
+// Entry points of cross attention and of attention over the 8-bit cache:
+// argument checks, the choice of kernel and of splits, workspace sizes.
+#include "h3b_host.hpp"
+#include "xattn.hpp"
+
+namespace {
+
+using h3b::XAttn;
+
+// A tensor of extent 1 along an axis may carry any stride there.
+bool fix_strides(int64_t (&st)[3], int64_t batch, int64_t seq, int64_t heads, int64_t d) {
+  const int64_t ext[3] = {batch, seq, heads};
+  for (int i = 0; i < 3; ++i) {
+    if (ext[i] <= 1) st[i] = d;
+    if (st[i] <= 0 || st[i] % 8 != 0 || st[i] > (1ll << 38)) return false;
+  }
+  return true;
+}
+
+int check_sizes(int dtype, int64_t batch, int64_t heads, int64_t kv_heads, int64_t head_dim, int64_t s_q,
+                int64_t s_kv) {
+  if (dtype != H3B_BF16 && dtype != H3B_F16) return H3B_ERR_DTYPE;
+  if (batch < 0 || heads <= 0 || kv_heads <= 0 || heads % kv_heads != 0 || s_q < 0 || s_kv < 0 ||
+      (head_dim != 64 && head_dim != 128) || batch > 65535 || heads > 65535 || s_q > (1ll << 30) ||
+      s_kv > (1ll << 30) || s_q * (heads / kv_heads) > (1ll << 30) || batch * heads * s_q > (1ll << 40))
+    return H3B_ERR_SHAPE;
+  return H3B_OK;
+}
+
+int64_t rows_of(const XAttn& a) { return static_cast<int64_t>(a.batch) * a.heads * a.s_q; }
+
+void plan(XAttn& a) { a.splits = h3b::xattn_rows_splits(a); }
+
+int64_t workspace_of(const XAttn& a) {
+  return a.splits > 1 ? rows_of(a) * a.splits * (a.head_dim + 2) * static_cast<int64_t>(sizeof(float)) : 0;
+}
+
+int run(XAttn& a, void* workspace, int64_t workspace_bytes, cudaStream_t stream) {
+  plan(a);
+  const int64_t need = workspace_of(a);
+  if (need > 0) {
+    if (workspace == nullptr) return H3B_ERR_ARG;
+    if (workspace_bytes < need) return H3B_ERR_SHAPE;
+    if (!h3b::aligned16(workspace)) return H3B_ERR_ALIGN;
+    a.part_o = static_cast<float*>(workspace);
+    a.part_ml = reinterpret_cast<float2*>(a.part_o + rows_of(a) * a.splits * a.head_dim);
+  }
+  return h3b::xattn_rows_launch(a, stream);
+}
+
+XAttn sizes(int dtype, h3b::KvKind kind, int64_t batch, int64_t heads, int64_t kv_heads, int64_t head_dim, int64_t s_q,
+            int64_t s_kv) {
+  XAttn a{};
+  a.dtype = dtype;
+  a.kind = kind;
+  a.batch = static_cast<int>(batch);
+  a.heads = static_cast<int>(heads);
+  a.kv_heads = static_cast<int>(kv_heads);
+  a.head_dim = static_cast<int>(head_dim);
+  a.s_q = static_cast<int>(s_q);
+  a.s_kv = static_cast<int>(s_kv);
+  a.splits = 1;
+  return a;
+}
+
+}  // namespace
+
+extern "C" int h3b_cross_attention_workspace(int64_t batch, int64_t heads, int64_t kv_heads, int64_t head_dim,
+                                             int64_t s_q, int64_t s_kv, int64_t* bytes) {
+  if (bytes == nullptr) return H3B_ERR_ARG;
+  const int rc = check_sizes(H3B_BF16, batch, heads, kv_heads, head_dim, s_q, s_kv);
+  if (rc != H3B_OK) return rc;
+  XAttn a = sizes(H3B_BF16, h3b::KV_DENSE, batch, heads, kv_heads, head_dim, s_q, s_kv);
+  plan(a);
+  *bytes = workspace_of(a);
+  return H3B_OK;
+}
+
+extern "C" int h3b_cross_attention_fwd(const void* q, const void* k, const void* v, void* o, float* lse, int dtype,
+                                       int64_t batch, int64_t heads, int64_t kv_heads, int64_t head_dim, int64_t s_q,
+                                       int64_t s_kv, int64_t q_batch_stride, int64_t q_seq_stride,
+                                       int64_t q_head_stride, int64_t kv_batch_stride, int64_t kv_seq_stride,
+                                       int64_t kv_head_stride, int64_t o_batch_stride, int64_t o_seq_stride,
+                                       int64_t o_head_stride, const int32_t* kv_lens, const uint8_t* key_mask,
+                                       int64_t mask_stride, float scale, void* workspace, int64_t workspace_bytes,
+                                       h3b_stream_t stream) {
+  const int rc = check_sizes(dtype, batch, heads, kv_heads, head_dim, s_q, s_kv);
+  if (rc != H3B_OK) return rc;
+  if (!(scale > 0.0f) || mask_stride < 0) return H3B_ERR_ARG;
+  if (batch == 0 || s_q == 0) return H3B_OK;
+  XAttn a = sizes(dtype, h3b::KV_DENSE, batch, heads, kv_heads, head_dim, s_q, s_kv);
+  a.q = q, a.k = s_kv > 0 ? k : q, a.v = s_kv > 0 ? v : q, a.o = o, a.lse = lse;
+  if (a.q == nullptr || a.k == nullptr || a.v == nullptr || o == nullptr) return H3B_ERR_ARG;
+  a.q_stride[0] = q_batch_stride, a.q_stride[1] = q_seq_stride, a.q_stride[2] = q_head_stride;
+  a.kv_stride[0] = kv_batch_stride, a.kv_stride[1] = kv_seq_stride, a.kv_stride[2] = kv_head_stride;
+  a.o_stride[0] = o_batch_stride, a.o_stride[1] = o_seq_stride, a.o_stride[2] = o_head_stride;
+  if (!fix_strides(a.q_stride, batch, s_q, heads, head_dim) ||
+      !fix_strides(a.kv_stride, s_kv > 0 ? batch : 1, s_kv, s_kv > 0 ? kv_heads : 1, head_dim) ||
+      !fix_strides(a.o_stride, batch, s_q, heads, head_dim))
+    return H3B_ERR_ALIGN;
+  for (const void* p : {a.q, a.k, a.v, static_cast<const void*>(o)})
+    if (!h3b::aligned16(p)) return H3B_ERR_ALIGN;
+  a.kv_lens = kv_lens;
+  a.key_mask = s_kv > 0 ? key_mask : nullptr;
+  a.mask_stride = mask_stride;
+  a.scale = scale;
+  return run(a, workspace, workspace_bytes, reinterpret_cast<cudaStream_t>(stream));
+}
+
+extern "C" int h3b_kv8_attention_workspace(int64_t batch, int64_t heads, int64_t kv_heads, int64_t head_dim,
+                                           int64_t s_q, int64_t block_tokens, int64_t max_blocks, int64_t* bytes) {
+  if (bytes == nullptr) return H3B_ERR_ARG;
+  const int rc = check_sizes(H3B_BF16, batch, heads, kv_heads, head_dim, s_q, 0);
+  if (rc != H3B_OK) return rc;
+  if (max_blocks <= 0 || block_tokens <= 0 || max_blocks * block_tokens > (1ll << 30)) return H3B_ERR_SHAPE;
+  XAttn a = sizes(H3B_BF16, h3b::KV_INT8, batch, heads, kv_heads, head_dim, s_q, max_blocks * block_tokens);
+  plan(a);
+  *bytes = workspace_of(a);
+  return H3B_OK;
+}
+
+extern "C" int h3b_kv8_attention(const void* q, void* o, float* lse, int dtype, int64_t batch, int64_t heads,
+                                 int64_t kv_heads, int64_t head_dim, int64_t s_q, int64_t q_batch_stride,
+                                 int64_t q_seq_stride, int64_t q_head_stride, int64_t o_batch_stride,
+                                 int64_t o_seq_stride, int64_t o_head_stride, const uint8_t* k_codes,
+                                 const uint8_t* v_codes, const float* k_scale, const float* v_scale, int code_type,
+                                 int64_t num_blocks, int64_t block_tokens, const int32_t* table, int64_t max_blocks,
+                                 const int32_t* lens, int causal, float scale, void* workspace,
+                                 int64_t workspace_bytes, h3b_stream_t stream) {
+  const int rc = check_sizes(dtype, batch, heads, kv_heads, head_dim, s_q, 0);
+  if (rc != H3B_OK) return rc;
+  if (code_type != H3B_KV_INT8 && code_type != H3B_KV_E4M3) return H3B_ERR_DTYPE;
+  if ((block_tokens != 32 && block_tokens != 64 && block_tokens != 128) || num_blocks <= 0 || max_blocks <= 0 ||
+      num_blocks * kv_heads > 0x7fffffffll || max_blocks * block_tokens > (1ll << 30))
+    return H3B_ERR_SHAPE;
+  if (!(scale > 0.0f)) return H3B_ERR_ARG;
+  if (batch == 0 || s_q == 0) return H3B_OK;
+  if (!q || !o || !k_codes || !v_codes || !k_scale || !v_scale || !table || !lens) return H3B_ERR_ARG;
+  XAttn a = sizes(dtype, code_type == H3B_KV_INT8 ? h3b::KV_INT8 : h3b::KV_E4M3, batch, heads, kv_heads, head_dim, s_q,
+                  max_blocks * block_tokens);
+  a.q = q, a.k = k_codes, a.v = v_codes, a.o = o, a.lse = lse;
+  a.q_stride[0] = q_batch_stride, a.q_stride[1] = q_seq_stride, a.q_stride[2] = q_head_stride;
+  a.o_stride[0] = o_batch_stride, a.o_stride[1] = o_seq_stride, a.o_stride[2] = o_head_stride;
+  if (!fix_strides(a.q_stride, batch, s_q, heads, head_dim) || !fix_strides(a.o_stride, batch, s_q, heads, head_dim))
+    return H3B_ERR_ALIGN;
+  for (const void* p : {q, static_cast<const void*>(o), a.k, a.v})
+    if (!h3b::aligned16(p)) return H3B_ERR_ALIGN;
+  a.table = table, a.max_blocks = static_cast<int>(max_blocks), a.block_tokens = static_cast<int>(block_tokens);
+  a.num_blocks = static_cast<int>(num_blocks), a.k_scale = k_scale, a.v_scale = v_scale;
+  a.kv_lens = lens;
+  a.causal = causal != 0;
+  a.scale = scale;
+  return run(a, workspace, workspace_bytes, reinterpret_cast<cudaStream_t>(stream));
+}

@@ -1,0 +1,57 @@
+// What the kernels behind h3b_cross_attention_fwd / _bwd and h3b_kv8_attention
+// share: the call's sizes and pointers, and the entry of each kernel family.
+#pragma once
+
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+#include "../../include/h3b.h"
+
+namespace h3b {
+
+// Where keys and values come from: a dense 16-bit tensor of q's type, or the
+// 8-bit cache (codes int8 or e4m3, one scale per block of tokens and head).
+enum KvKind { KV_DENSE = 0, KV_INT8 = 1, KV_E4M3 = 2 };
+
+// One attention call.  Strides are in elements, in the order (batch, token,
+// head); o_* as q_*.  Element (b, s, h, d) of q lies at q + b*q_stride[0] +
+// s*q_stride[1] + h*q_stride[2] + d.
+struct XAttn {
+  const void* q;
+  const void* k;
+  const void* v;
+  void* o;
+  float* lse;  // [batch, heads, s_q] or null
+  int dtype;   // H3B_BF16 / H3B_F16: q, o (and dense k, v)
+  KvKind kind;
+  int64_t q_stride[3];
+  int64_t kv_stride[3];  // dense only
+  int64_t o_stride[3];
+  int batch, heads, kv_heads, head_dim, s_q;
+  int s_kv;                  // dense: keys per sample; cache: max_blocks * block_tokens
+  const int32_t* kv_lens;    // [batch] or null (all s_kv keys)
+  const uint8_t* key_mask;   // dense: [batch, s_kv] bytes, 0 = left out; or null
+  int64_t mask_stride;
+  // cache
+  const int32_t* table;  // [batch, max_blocks]
+  int max_blocks, block_tokens, num_blocks;
+  const float* k_scale;  // [num_blocks, kv_heads]
+  const float* v_scale;
+  int causal;  // query i of s_q sees keys < kv_len - s_q + i + 1
+  float scale;
+  // split calls: partial results of `splits` key ranges per row
+  int splits;
+  float* part_o;   // [splits, batch*heads*s_q, head_dim], unnormalised
+  float2* part_ml; // [splits, batch*heads*s_q]: running max (log2 domain), sum
+};
+
+// Keys split over so many ranges by the row kernel / the tile kernel.
+int xattn_rows_splits(const XAttn& a);
+int xattn_tile_splits(const XAttn& a);
+
+int xattn_rows_launch(const XAttn& a, cudaStream_t stream);
+int xattn_tile_launch(const XAttn& a, cudaStream_t stream);
+// Joins the ranges of a split call into o and lse.
+int xattn_combine_launch(const XAttn& a, cudaStream_t stream);
+
+}  // namespace h3b

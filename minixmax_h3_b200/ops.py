@@ -7,6 +7,7 @@ non-CUDA tensors raise.
 from __future__ import annotations
 
 import ctypes
+import functools
 from dataclasses import dataclass
 from typing import Optional, Sequence
 
@@ -375,6 +376,241 @@ def qk_rmsnorm_rope(q: torch.Tensor, k: Optional[torch.Tensor], q_weight: torch.
     s, heads, d = q.shape
     call("h3b_qk_rmsnorm_rope", q.data_ptr(), _ptr(k), s, heads, q.stride(0), q.stride(1), q_weight.data_ptr(),
          _ptr(k_weight), eps, pos.data_ptr(), pos_offset, inv_freq.data_ptr(), n_t, n_h, _stream(q))
+
+
+# ----------------------------------------------------------------------------- cross attention
+
+_FLOAT16 = {torch.bfloat16: 0, torch.float16: 1}
+
+
+def _fits(t: torch.Tensor) -> bool:
+    """Whether a [B, S, H, D] tensor can be read in place: unit last stride,
+    the others positive multiples of 8 elements (any along an axis of extent
+    1), 16-byte aligned."""
+    st = t.stride()
+    if st[3] != 1 or t.data_ptr() & 15:
+        return False
+    for n, s in zip(t.shape, st[:3]):
+        if n > 1 and (s <= 0 or s & 7):
+            return False
+    return True
+
+
+def _check_qkv(name: str, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor) -> None:
+    if q.dtype not in _FLOAT16 or k.dtype != q.dtype or v.dtype != q.dtype:
+        raise TypeError(f"{name} expects q, k and v of one type, bf16 or fp16")
+    if q.dim() != 4 or k.dim() != 4 or k.shape != v.shape or k.shape[0] != q.shape[0] or k.shape[3] != q.shape[3]:
+        raise ValueError(f"{name} expects q [B, Sq, H, D], k and v [B, Skv, Hkv, D]")
+    if q.shape[3] not in (64, 128):
+        raise ValueError(f"{name}: head dim {q.shape[3]}: the kernels are built for 64 and 128")
+    if k.shape[2] == 0 or q.shape[2] % k.shape[2]:
+        raise ValueError(f"{name}: {q.shape[2]} query heads cannot share {k.shape[2]} key heads")
+
+
+def _kv_in_place(k: torch.Tensor, v: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
+    if not (_fits(k) and _fits(v) and k.stride() == v.stride()):
+        k, v = k.contiguous(), v.contiguous()
+    return k, v
+
+
+def _kept_keys(name: str, k: torch.Tensor, kv_lens: Optional[torch.Tensor],
+               key_mask: Optional[torch.Tensor]) -> Optional[torch.Tensor]:
+    """Checks kv_lens / key_mask; returns the mask with unit key stride."""
+    if kv_lens is not None and (kv_lens.dtype != torch.int32 or kv_lens.shape != k.shape[:1]
+                                or not kv_lens.is_contiguous()):
+        raise ValueError(f"{name}: kv_lens is an int32 tensor of one length per sample")
+    if key_mask is not None:
+        if key_mask.dtype != torch.bool or key_mask.shape != k.shape[:2]:
+            raise ValueError(f"{name}: key_mask is a bool [B, Skv] tensor (True: attended)")
+        if key_mask.stride(1) != 1 or key_mask.stride(0) < 0:
+            key_mask = key_mask.contiguous()
+    return key_mask
+
+
+def _scale(scale: Optional[float], d: int) -> float:
+    scale = d ** -0.5 if scale is None else float(scale)
+    if not 0.0 < scale < float("inf"):
+        raise ValueError("the softmax scale must be positive and finite")
+    return scale
+
+
+@functools.lru_cache(maxsize=512)
+def _workspace_bytes(fn: str, device: int, *sizes: int) -> int:
+    n = ctypes.c_int64(0)
+    call(fn, *sizes, ctypes.addressof(n))
+    return n.value
+
+
+def _workspace(fn: str, t: torch.Tensor, *sizes: int) -> Optional[torch.Tensor]:
+    n = _workspace_bytes(fn, t.device.index, *sizes)
+    return torch.empty((n,), dtype=torch.uint8, device=t.device) if n else None
+
+
+def _check_lse(name: str, lse: Optional[torch.Tensor], q: torch.Tensor) -> None:
+    if lse is not None and (lse.dtype != torch.float32 or lse.shape != (q.shape[0], q.shape[2], q.shape[1])
+                            or not lse.is_contiguous()):
+        raise ValueError(f"{name}: lse is a contiguous fp32 [B, H, Sq] tensor")
+
+
+def _check_out(name: str, out: Optional[torch.Tensor], q: torch.Tensor) -> torch.Tensor:
+    if out is None:
+        return torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    if out.shape != q.shape or out.dtype != q.dtype or not _fits(out):
+        raise ValueError(f"{name}: out has q's shape and type, unit last stride, strides of multiples of 8 and "
+                         "16-byte alignment")
+    return out
+
+
+def cross_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, kv_lens: Optional[torch.Tensor] = None,
+                    key_mask: Optional[torch.Tensor] = None, scale: Optional[float] = None,
+                    out: Optional[torch.Tensor] = None, lse: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Attention of q [B, Sq, H, D] to an encoder's k, v [B, Skv, Hkv, D]
+    (bf16 or fp16, D 64 or 128, H a multiple of Hkv): o [B, Sq, H, D].
+
+    kv_lens (int32 [B], device) keeps the first keys of each sample, key_mask
+    (bool [B, Skv], True: attended) any of them; with both, the keys that both
+    keep.  Left-out keys and values are never used, whatever they hold.  A
+    row without a kept key gives zeros (lse -inf).  lse, if given (fp32
+    [B, H, Sq]), receives the log-sum-exps that cross_attention_bwd needs.
+    Strided q, k and v are read in place (unit last stride, the others
+    multiples of 8, k and v alike, as the halves of one projection); other
+    layouts are copied first.  For gradients by autograd see
+    ``attention.cross_attention``."""
+    _cuda(q, k, v, kv_lens, key_mask, out, lse)
+    _check_qkv("cross_attention", q, k, v)
+    b, s_q, heads, d = q.shape
+    s_kv, kv_heads = k.shape[1], k.shape[2]
+    key_mask = _kept_keys("cross_attention", k, kv_lens, key_mask)
+    _check_lse("cross_attention", lse, q)
+    out = _check_out("cross_attention", out, q)
+    if not _fits(q):
+        q = q.contiguous()
+    k, v = _kv_in_place(k, v)
+    ws = _workspace("h3b_cross_attention_workspace", q, b, heads, kv_heads, d, s_q, s_kv)
+    call("h3b_cross_attention_fwd", q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), _ptr(lse),
+         _FLOAT16[q.dtype], b, heads, kv_heads, d, s_q, s_kv, *q.stride()[:3], *k.stride()[:3], *out.stride()[:3],
+         _ptr(kv_lens), _ptr(key_mask), 0 if key_mask is None else key_mask.stride(0), _scale(scale, d), _ptr(ws),
+         0 if ws is None else ws.numel(), _stream(q))
+    return out
+
+
+# ----------------------------------------------------------------------------- 8-bit key/value cache
+
+_KV8_CODES = {torch.int8: 0, torch.float8_e4m3fn: 1}
+
+
+@dataclass
+class KV8Cache:
+    """Keys and values held in 8 bits: codes k, v [num_blocks, Hkv,
+    block_tokens, D] (int8 or float8_e4m3fn) and one fp32 scale per block of
+    tokens and head, [num_blocks, Hkv]; a value is code * scale.  The blocks
+    of a sequence are named by a block table (int32 [B, max_blocks]), which
+    the caller keeps beside the sequences' lengths (int32 [B])."""
+
+    k: torch.Tensor
+    v: torch.Tensor
+    k_scale: torch.Tensor
+    v_scale: torch.Tensor
+
+    @classmethod
+    def empty(cls, num_blocks: int, kv_heads: int, head_dim: int, *, block_tokens: int = 64,
+              dtype: torch.dtype = torch.int8, device=None) -> "KV8Cache":
+        if dtype not in _KV8_CODES:
+            raise TypeError("KV8Cache holds int8 or float8_e4m3fn codes")
+        if block_tokens not in (32, 64, 128) or head_dim not in (64, 128):
+            raise ValueError("KV8Cache: blocks of 32, 64 or 128 tokens, head dim 64 or 128")
+        k, v = (torch.zeros((num_blocks, kv_heads, block_tokens, head_dim), dtype=torch.uint8, device=device).view(dtype)
+                for _ in range(2))
+        ks, vs = (torch.zeros((num_blocks, kv_heads), dtype=torch.float32, device=device) for _ in range(2))
+        return cls(k, v, ks, vs)
+
+    @property
+    def block_tokens(self) -> int:
+        return self.k.shape[2]
+
+
+def _check_cache(name: str, c: KV8Cache, table: torch.Tensor, lens: torch.Tensor) -> None:
+    _cuda(c.k, c.v, c.k_scale, c.v_scale, table, lens)
+    k, v, ks, vs = c.k, c.v, c.k_scale, c.v_scale
+    if k.dtype not in _KV8_CODES or v.dtype != k.dtype or ks.dtype != torch.float32 or vs.dtype != torch.float32:
+        raise TypeError(f"{name}: the cache holds int8 or float8_e4m3fn codes and fp32 scales")
+    if k.dim() != 4 or v.shape != k.shape or ks.shape != k.shape[:2] or vs.shape != k.shape[:2]:
+        raise ValueError(f"{name}: codes [num_blocks, Hkv, block_tokens, D], scales [num_blocks, Hkv]")
+    if not (k.is_contiguous() and v.is_contiguous() and ks.is_contiguous() and vs.is_contiguous()):
+        raise ValueError(f"{name}: the cache's tensors are contiguous")
+    if table.dtype != torch.int32 or table.dim() != 2 or not table.is_contiguous():
+        raise ValueError(f"{name}: the block table is a contiguous int32 [B, max_blocks] tensor")
+    if lens.dtype != torch.int32 or lens.shape != table.shape[:1] or not lens.is_contiguous():
+        raise ValueError(f"{name}: lengths are an int32 tensor of one per sequence of the table")
+
+
+def kv8_append(cache: KV8Cache, k: torch.Tensor, v: torch.Tensor, block_table: torch.Tensor, lens: torch.Tensor, *,
+               new_lens: Optional[torch.Tensor] = None) -> None:
+    """Quantises k, v [B, T, Hkv, D] (bf16 or fp16) into the cache behind the
+    lens[b] tokens that each sequence holds (int32 [B], device; not updated
+    here).  new_lens (int32 [B]) appends the first new_lens[b] rows of a
+    ragged batch.  A block that held tokens keeps the larger of its scale and
+    the new rows' one, and its codes are rounded again if it grew."""
+    _check_cache("kv8_append", cache, block_table, lens)
+    _cuda(k, v, new_lens)
+    nb, kv_heads, bt, d = cache.k.shape
+    if k.dtype not in _FLOAT16 or v.dtype != k.dtype:
+        raise TypeError("kv8_append expects bf16 or fp16 keys and values")
+    if k.dim() != 4 or v.shape != k.shape or k.shape[0] != lens.shape[0] or k.shape[2] != kv_heads or k.shape[3] != d:
+        raise ValueError("kv8_append: k and v [B, T, Hkv, D] of the cache's heads")
+    if new_lens is not None and (new_lens.dtype != torch.int32 or new_lens.shape != lens.shape
+                                 or not new_lens.is_contiguous()):
+        raise ValueError("kv8_append: new_lens is an int32 [B] tensor")
+    k, v = _kv_in_place(k, v)
+    call("h3b_kv8_append", k.data_ptr(), v.data_ptr(), _FLOAT16[k.dtype], k.shape[0], k.shape[1], kv_heads, d,
+         *k.stride()[:3], cache.k.data_ptr(), cache.v.data_ptr(), cache.k_scale.data_ptr(), cache.v_scale.data_ptr(),
+         _KV8_CODES[cache.k.dtype], nb, bt, block_table.data_ptr(), block_table.shape[1], lens.data_ptr(),
+         _ptr(new_lens), _stream(k))
+
+
+def kv8_read(cache: KV8Cache, block_table: torch.Tensor, lens: torch.Tensor, max_len: int, *,
+             dtype: torch.dtype = torch.bfloat16) -> tuple[torch.Tensor, torch.Tensor]:
+    """The cache's values in the order of the tokens: k, v [B, max_len, Hkv,
+    D] in dtype (bf16, fp16 or fp32), zero behind lens[b]."""
+    _check_cache("kv8_read", cache, block_table, lens)
+    nb, kv_heads, bt, d = cache.k.shape
+    codes = {**_FLOAT16, torch.float32: 2}
+    if dtype not in codes:
+        raise TypeError("kv8_read writes bf16, fp16 or fp32")
+    k, v = (torch.empty((lens.shape[0], max_len, kv_heads, d), dtype=dtype, device=cache.k.device) for _ in range(2))
+    call("h3b_kv8_read", cache.k.data_ptr(), cache.v.data_ptr(), cache.k_scale.data_ptr(), cache.v_scale.data_ptr(),
+         _KV8_CODES[cache.k.dtype], nb, kv_heads, bt, d, block_table.data_ptr(), block_table.shape[1],
+         lens.data_ptr(), lens.shape[0], max_len, k.data_ptr(), v.data_ptr(), codes[dtype], _stream(cache.k))
+    return k, v
+
+
+def kv8_attention(q: torch.Tensor, cache: KV8Cache, block_table: torch.Tensor, lens: torch.Tensor, *,
+                  causal: bool = False, scale: Optional[float] = None, out: Optional[torch.Tensor] = None,
+                  lse: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Attention of q [B, Sq, H, D] (bf16 or fp16, H a multiple of the
+    cache's heads) over the lens[b] tokens that each sequence's cache holds:
+    o [B, Sq, H, D].  causal: the queries are the sequence's last Sq tokens
+    (already appended), each sees the tokens up to its own.  Tokens of a block
+    that the table does not name (an entry outside the pool) are left out.  A
+    row that sees no token gives zeros (lse, fp32 [B, H, Sq] if given: -inf)."""
+    _check_cache("kv8_attention", cache, block_table, lens)
+    _cuda(q, out, lse)
+    nb, kv_heads, bt, d = cache.k.shape
+    if q.dtype not in _FLOAT16:
+        raise TypeError("kv8_attention expects bf16 or fp16 queries")
+    if q.dim() != 4 or q.shape[0] != lens.shape[0] or q.shape[3] != d or q.shape[2] % kv_heads:
+        raise ValueError("kv8_attention expects q [B, Sq, H, D], H a multiple of the cache's heads")
+    b, s_q, heads, _ = q.shape
+    _check_lse("kv8_attention", lse, q)
+    out = _check_out("kv8_attention", out, q)
+    if not _fits(q):
+        q = q.contiguous()
+    ws = _workspace("h3b_kv8_attention_workspace", q, b, heads, kv_heads, d, s_q, bt, block_table.shape[1])
+    call("h3b_kv8_attention", q.data_ptr(), out.data_ptr(), _ptr(lse), _FLOAT16[q.dtype], b, heads, kv_heads, d, s_q,
+         *q.stride()[:3], *out.stride()[:3], cache.k.data_ptr(), cache.v.data_ptr(), cache.k_scale.data_ptr(),
+         cache.v_scale.data_ptr(), _KV8_CODES[cache.k.dtype], nb, bt, block_table.data_ptr(), block_table.shape[1],
+         lens.data_ptr(), 1 if causal else 0, _scale(scale, d), _ptr(ws), 0 if ws is None else ws.numel(), _stream(q))
+    return out
 
 
 # ----------------------------------------------------------------------------- block elementwise
