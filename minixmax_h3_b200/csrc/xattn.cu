@@ -29,7 +29,11 @@ int check_sizes(int dtype, int64_t batch, int64_t heads, int64_t kv_heads, int64
 
 int64_t rows_of(const XAttn& a) { return static_cast<int64_t>(a.batch) * a.heads * a.s_q; }
 
-void plan(XAttn& a) { a.splits = h3b::xattn_rows_splits(a); }
+// Which kernel: the tile kernel works on 128 rows of one head whether they
+// exist or not; the row kernel on 32 rows of the heads that share a key head.
+bool by_tiles(const XAttn& a) { return a.kind == h3b::KV_DENSE && a.s_q >= 64; }
+
+void plan(XAttn& a) { a.splits = by_tiles(a) ? h3b::xattn_tile_splits(a) : h3b::xattn_rows_splits(a); }
 
 int64_t workspace_of(const XAttn& a) {
   return a.splits > 1 ? rows_of(a) * a.splits * (a.head_dim + 2) * static_cast<int64_t>(sizeof(float)) : 0;
@@ -45,7 +49,7 @@ int run(XAttn& a, void* workspace, int64_t workspace_bytes, cudaStream_t stream)
     a.part_o = static_cast<float*>(workspace);
     a.part_ml = reinterpret_cast<float2*>(a.part_o + rows_of(a) * a.splits * a.head_dim);
   }
-  return h3b::xattn_rows_launch(a, stream);
+  return by_tiles(a) ? h3b::xattn_tile_launch(a, stream) : h3b::xattn_rows_launch(a, stream);
 }
 
 XAttn sizes(int dtype, h3b::KvKind kind, int64_t batch, int64_t heads, int64_t kv_heads, int64_t head_dim, int64_t s_q,

@@ -112,11 +112,6 @@ H3B_DEV uint2 lds64(uint32_t addr) {
   return v;
 }
 
-H3B_DEV uint32_t pack_f16x2(float lo, float hi) {
-  const __half2 h = __floats2half2_rn(lo, hi);
-  return *reinterpret_cast<const uint32_t*>(&h);
-}
-
 // Two codes -> f16x2.  int8 (bytes biased by 128 by the caller): 0x6400 | u is
 // 1024 + u in f16, minus 1152 leaves u - 128.
 H3B_DEV uint32_t i8_pair(uint32_t biased, uint32_t sel) {

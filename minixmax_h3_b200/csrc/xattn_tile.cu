@@ -1,0 +1,654 @@
+// Attention of many query rows on tcgen05 (h3b_cross_attention_fwd): 256 query
+// rows of one head at a time, in 128-key tiles.
+//
+//   S = Q K^T;  P = 2^(scale log2e S - M);  O = O 2^(M_old - M) + P V;  o = O / l
+//
+// An encoder's states are few (77 to some thousand keys), so a call is many
+// short pieces of work: 256 rows x 512 keys are 4 tiles, ~8 us of which a
+// launch-per-piece scheme would spend a third on barriers, TMEM allocation,
+// the first loads and the last stores.  So the kernel is persistent: one CTA
+// per SM runs through units (sample, head, 256 rows, range of keys) with one
+// continuous pipeline of matrix instructions; the next unit's Q and first K
+// are loaded, and its first scores computed, while the last one's softmax and
+// stores are under way.
+//   warps 0-3   softmax and stores of rows 0-127 (thread = row = TMEM lane)
+//   warps 4-7   the same for rows 128-255
+//   warp 8      TMA: Q through a ring of 3 tiles, K and V through one of 4
+//   warp 9      TMEM allocation and matrix instructions
+//   warps 10-11 idle (complete the third warpgroup for setmaxnreg)
+// TMEM: S0 | S1 | O0 | O1, 128 columns each (O: D).  P goes back to TMEM as
+// 16-bit values over the S it came from and is the A operand of P V.  One
+// warp issues, per tile j of a unit:
+//   S0(j)  P V1(j-1)  S1(j)  P V0(j)
+// across the units' borders too, so the tensor pipe has one 128-row tile's
+// products while the other's softmax runs.  The stream executes in order:
+// S_i(j) cannot overwrite P_i(j-1) before P V_i(j-1) has read it, and the
+// commit behind S_i(j) says that O_i is settled as well.  O_i of the next unit
+// starts only when P_i of its first tile is there, which the softmax warps
+// write after they have read the last unit's O_i.
+// The running maximum is raised lazily, by steps of more than 2^8, so P <=
+// 2^8: exact in fp32 sums, inside f16's range.
+// Left-out keys: a score column is replaced (-inf) whatever it holds, and the
+// row of V is zeroed in shared memory before P V reads it (0 * NaN is NaN).
+#include "h3b_common.cuh"
+#include "h3b_host.hpp"
+#include "xattn.hpp"
+
+H3B_DECLARE_STATUS();
+H3B_REGISTER_STATUS_READER(xattn_tile);
+
+namespace {
+
+using h3b::XAttn;
+
+constexpr int BQ = 128, BKV = 128;
+constexpr int QST = 3;   // Q ring (128-row tiles)
+constexpr int KVST = 4;  // K/V ring (K_s in slots 0, 2, V_s in 1, 3)
+constexpr int THREADS = 384;
+constexpr int REGS_LAUNCH = 168;
+constexpr int REGS_CONTROL = 88;
+constexpr int REGS_SOFTMAX = 208;
+static_assert(128 * (REGS_CONTROL + 2 * REGS_SOFTMAX) <= THREADS * REGS_LAUNCH, "register split exceeds launch");
+constexpr float RESCALE_THRESHOLD = 8.0f;
+constexpr float LOG2E = 1.4426950408889634f;
+constexpr float LN2 = 0.69314718055994531f;
+
+template <int D>
+struct Cfg {
+  static constexpr int HALVES = D / 64;            // 64-column TMA boxes of a tile
+  static constexpr int TILE_BYTES = 128 * D * 2;   // Q, K or V
+  static constexpr int HALF_BYTES = 128 * 64 * 2;  // 16 KB
+};
+
+struct __align__(8) Bars {
+  uint64_t q_full[QST];
+  uint64_t q_free[QST];
+  uint64_t kv_full[KVST];
+  uint64_t kv_free[KVST];
+  uint64_t s_full[2];
+  uint64_t p_half[2][2];  // one arrival per softmax warp
+  uint64_t o_full[2];
+  uint64_t drain;
+  uint32_t tmem_base;
+  int abort_flag;
+};
+
+template <int D>
+constexpr size_t smem_bytes() {
+  return 1024 + (QST + KVST) * Cfg<D>::TILE_BYTES + sizeof(Bars);
+}
+
+struct TileArgs {
+  XAttn a;
+  int q_tiles;  // units of 256 rows per (sample, head)
+  int units;
+  int group;
+  int o_wide;   // 32-byte stores of o allowed
+  float scale_log2;
+};
+
+// One unit of work.
+struct Unit {
+  int b, head, q0, split;
+  int len;   // the sample's kept prefix
+  int j0, n; // first tile, tiles
+  bool two;  // rows 128-255 exist
+};
+
+H3B_DEV Unit unit_of(const TileArgs& args, int u) {
+  const XAttn& a = args.a;
+  Unit x;
+  const int qt = u % args.q_tiles;  // fastest: units that run together share K and V in L2
+  u /= args.q_tiles;
+  x.split = u % a.splits;
+  u /= a.splits;
+  x.head = u % a.heads;
+  x.b = u / a.heads;
+  x.q0 = qt * 2 * BQ;
+  x.len = a.s_kv;
+  if (a.kv_lens != nullptr) x.len = max(0, min(x.len, __ldg(a.kv_lens + x.b)));
+  int end = x.len;
+  if (a.causal) end = max(0, min(end, x.len - a.s_q + min(x.q0 + 2 * BQ, a.s_q)));
+  const int per = ((x.len + BKV - 1) / BKV + a.splits - 1) / a.splits;
+  x.j0 = x.split * per;
+  x.n = max(0, min((end + BKV - 1) / BKV, x.j0 + per) - x.j0);
+  x.two = x.q0 + BQ < a.s_q;
+  return x;
+}
+
+template <bool SPIN = false>
+H3B_DEV bool warp_wait(uint64_t* bar, uint32_t parity, int site, volatile int* abort_flag) {
+  const bool ok = mbar_wait<SPIN>(bar, parity, &g_status, site, abort_flag);
+  return __all_sync(0xffffffffu, ok);
+}
+
+H3B_DEV float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// Which keys of a tile are kept, one bit each: first the bytes (or 1s), then
+// the words, so that a wait can stand between the load and its use.
+H3B_DEV uint32_t mask_bytes(const XAttn& a, int b, int key0, int len, int lane) {
+  uint32_t m = 0;
+#pragma unroll
+  for (int c = 0; c < 4; ++c) {
+    const int key = key0 + c * 32 + lane;
+    if (key < len && __ldg(a.key_mask + b * a.mask_stride + key) != 0) m |= 1u << c;
+  }
+  return m;
+}
+H3B_DEV void keep_words(bool masked, uint32_t bytes, int valid, uint32_t (&w)[4]) {
+#pragma unroll
+  for (int c = 0; c < 4; ++c) {
+    const int v = valid - 32 * c;
+    w[c] = v >= 32 ? 0xffffffffu : (v <= 0 ? 0u : (1u << v) - 1u);
+    if (masked) w[c] = __ballot_sync(0xffffffffu, (bytes >> c) & 1u);
+  }
+}
+
+H3B_DEV float row_max64(const uint32_t* r) {
+  float mx[8];
+#pragma unroll
+  for (int c = 0; c < 8; ++c)
+    mx[c] = fmax3(__uint_as_float(r[c]), __uint_as_float(r[c + 8]), __uint_as_float(r[c + 16]));
+#pragma unroll
+  for (int e = 24; e < 56; e += 16)
+#pragma unroll
+    for (int c = 0; c < 8; ++c) mx[c] = fmax3(mx[c], __uint_as_float(r[e + c]), __uint_as_float(r[e + 8 + c]));
+#pragma unroll
+  for (int c = 0; c < 8; ++c) mx[c] = fmaxf(mx[c], __uint_as_float(r[56 + c]));
+  return fmax3(fmax3(mx[0], mx[1], mx[2]), fmax3(mx[3], mx[4], mx[5]), fmaxf(mx[6], mx[7]));
+}
+
+// 64 scores r[0..63] -> weights 2^(s * scale + neg_m), packed into dst[0..31];
+// returns their sum and, with MAX, the largest of the 128 scores r[0..127].
+template <bool F16, bool MAX>
+H3B_DEV float2 exp_pack64(uint32_t* r, uint32_t* dst, float scale_log2, float neg_m) {
+  const float2 sc = make_float2(scale_log2, scale_log2);
+  const float2 nm = make_float2(neg_m, neg_m);
+  float mx[8];
+  if constexpr (MAX) {
+#pragma unroll
+    for (int c = 0; c < 8; ++c) mx[c] = -INFINITY;
+  }
+#pragma unroll
+  for (int e = 0; e < 32; ++e) {
+    const float sa = __uint_as_float(r[2 * e]), sb = __uint_as_float(r[2 * e + 1]);
+    if constexpr (MAX) {
+      mx[e & 7] = fmax3(mx[e & 7], sa, sb);
+      mx[e & 7] = fmax3(mx[e & 7], __uint_as_float(r[64 + 2 * e]), __uint_as_float(r[64 + 2 * e + 1]));
+    }
+    const float2 x = fma2(make_float2(sa, sb), sc, nm);
+    r[2 * e] = __float_as_uint(ex2(x.x));
+    r[2 * e + 1] = __float_as_uint(ex2(x.y));
+  }
+  float2 acc[4] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f), make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+#pragma unroll
+  for (int e = 0; e < 32; ++e) {
+    const float2 p = make_float2(__uint_as_float(r[2 * e]), __uint_as_float(r[2 * e + 1]));
+    acc[e & 3] = add2(acc[e & 3], p);
+    dst[e] = pack16x2<F16>(p.x, p.y);
+  }
+  const float2 t = add2(add2(acc[0], acc[1]), add2(acc[2], acc[3]));
+  float m = 0.0f;
+  if constexpr (MAX) m = fmax3(fmax3(mx[0], mx[1], mx[2]), fmax3(mx[3], mx[4], mx[5]), fmaxf(mx[6], mx[7]));
+  return make_float2(t.x + t.y, m);
+}
+
+template <int D, bool F16>
+__global__ void __launch_bounds__(THREADS, 1)
+    xattn_tile_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
+                      const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ TileArgs args) {
+  using C = Cfg<D>;
+  constexpr uint32_t IDESC_S = F16 ? idesc_f16_f32(128, BKV, 0, 0) : idesc_bf16_f32(128, BKV, 0, 0);
+  constexpr uint32_t IDESC_O = F16 ? idesc_f16_f32(128, D, 0, 1) : idesc_bf16_f32(128, D, 0, 1);
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint8_t* sQ = smem;
+  uint8_t* sKV = sQ + QST * C::TILE_BYTES;
+  Bars* bars = reinterpret_cast<Bars*>(sKV + KVST * C::TILE_BYTES);
+  const XAttn& a = args.a;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  volatile int* abort_flag = &bars->abort_flag;
+  const bool masked = a.key_mask != nullptr;
+
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < QST; ++i) {
+      mbar_init(&bars->q_full[i], 1);
+      mbar_init(&bars->q_free[i], 1);
+    }
+    for (int i = 0; i < KVST; ++i) {
+      mbar_init(&bars->kv_full[i], 1);
+      mbar_init(&bars->kv_free[i], 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&bars->s_full[i], 1);
+      mbar_init(&bars->p_half[i][0], 4);
+      mbar_init(&bars->p_half[i][1], 4);
+      mbar_init(&bars->o_full[i], 1);
+    }
+    mbar_init(&bars->drain, 1);
+    bars->abort_flag = 0;
+    fence_barrier_init();
+  }
+  if (warp == 9) {
+    tmem_alloc(&bars->tmem_base, 512);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = bars->tmem_base;
+  auto s_col = [](int i) { return static_cast<uint32_t>(i * 128); };
+  auto o_col = [](int i) { return static_cast<uint32_t>(256 + i * 128); };
+
+  if (warp >= 8) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(REGS_CONTROL));
+    if (warp == 8 && lane == 0) {
+      // ------------------------------------------------------------ TMA
+      // Slot of the c-th Q (K/V) tile: c % ring; its free barrier has
+      // completed phase (c / ring) - 1 when the tile before it is read, and
+      // its next phase needs this very load: a parity wait is one phase behind.
+      prefetch_tmap(&tm_q);
+      prefetch_tmap(&tm_k);
+      prefetch_tmap(&tm_v);
+      int qc = 0, kvc = 0;
+      bool ok = true;
+      auto load_q = [&](const Unit& u, int i) {
+        const int s = qc % QST;
+        if (qc >= QST && !mbar_wait(&bars->q_free[s], (qc / QST - 1) & 1, &g_status, 1, abort_flag)) return false;
+        mbar_arrive_expect_tx(&bars->q_full[s], C::TILE_BYTES);
+        for (int h = 0; h < C::HALVES; ++h)
+          tma_load_4d(sQ + s * C::TILE_BYTES + h * C::HALF_BYTES, &tm_q, h * 64, u.q0 + i * BQ, u.head, u.b,
+                      &bars->q_full[s]);
+        ++qc;
+        return true;
+      };
+      auto load_kv = [&](const CUtensorMap* tm, const Unit& u, int j) {
+        const int s = kvc % KVST;
+        if (kvc >= KVST && !mbar_wait(&bars->kv_free[s], (kvc / KVST - 1) & 1, &g_status, 2, abort_flag)) return false;
+        mbar_arrive_expect_tx(&bars->kv_full[s], C::TILE_BYTES);
+        for (int h = 0; h < C::HALVES; ++h)
+          tma_load_4d(sKV + s * C::TILE_BYTES + h * C::HALF_BYTES, tm, h * 64, (u.j0 + j) * BKV, u.head / args.group,
+                      u.b, &bars->kv_full[s]);
+        ++kvc;
+        return true;
+      };
+      for (int x = blockIdx.x; x < args.units && ok; x += gridDim.x) {
+        const Unit u = unit_of(args, x);
+        for (int j = 0; j < u.n && ok; ++j) {
+          if (j == 0) ok = ok && load_q(u, 0);
+          ok = ok && load_kv(&tm_k, u, j);
+          if (j == 0 && u.two) ok = ok && load_q(u, 1);
+          ok = ok && load_kv(&tm_v, u, j);
+        }
+      }
+      if (!ok || *abort_flag) {
+        // let the copies in flight land (bounded) before the CTA goes
+        for (int c = max(0, qc - QST); c < qc; ++c)
+          mbar_wait(&bars->q_full[c % QST], (c / QST) & 1, &g_status, 10, nullptr);
+        for (int c = max(0, kvc - KVST); c < kvc; ++c)
+          mbar_wait(&bars->kv_full[c % KVST], (c / KVST) & 1, &g_status, 11, nullptr);
+      }
+    } else if (warp == 9) {
+      // ------------------------------------------------------------ MMA
+      // The warp runs the schedule converged: all lanes poll, one elected
+      // lane issues.  Every barrier waited on here completes once per use and
+      // its next use depends on what this warp issues after the wait.
+      int qc = 0, step = 0;
+      uint32_t pc[2] = {0, 0};  // P tiles consumed, per row tile
+      bool ok = true;
+      auto commit = [&](uint64_t* bar) {
+        if (elect_one()) tc_commit(bar);
+        __syncwarp();
+      };
+      auto wait = [&](uint64_t* bar, uint32_t parity, int site) {
+        if (!warp_wait<true>(bar, parity, site, abort_flag)) return false;
+        tc_fence_after();
+        return true;
+      };
+      auto wait_kv = [&](int c) { return wait(&bars->kv_full[c % KVST], (c / KVST) & 1, 4); };
+      auto issue_s = [&](int i, int qslot, int kslot) {
+        const uint64_t qd = sdesc_kmajor_sw128(smem_u32(sQ + qslot * C::TILE_BYTES));
+        const uint64_t kd = sdesc_kmajor_sw128(smem_u32(sKV + kslot * C::TILE_BYTES));
+        if (elect_one()) {
+#pragma unroll
+          for (int kk = 0; kk < D / 16; ++kk) {
+            const uint32_t at = static_cast<uint32_t>((kk >> 2) * (C::HALF_BYTES >> 4) + (kk & 3) * 2);
+            mma_f16_ss(tmem + s_col(i), desc_add_lo(qd, at), desc_add_lo(kd, at), IDESC_S, kk > 0);
+          }
+          tc_commit(&bars->s_full[i]);
+        }
+        __syncwarp();
+      };
+      // O_i (+)= P_i V, in two halves of 64 keys as the softmax delivers them
+      auto issue_pv = [&](int i, int vslot, bool first) -> bool {
+        const uint64_t vd = sdesc_mnmajor_sw128(smem_u32(sKV + vslot * C::TILE_BYTES), C::HALF_BYTES, 1024);
+        for (int h = 0; h < 2; ++h) {
+          if (!wait(&bars->p_half[i][h], pc[i] & 1, 5)) return false;
+          if (elect_one()) {
+#pragma unroll
+            for (int kk = 4 * h; kk < 4 * h + 4; ++kk)
+              mma_f16_ts(tmem + o_col(i), tmem + s_col(i) + kk * 8, desc_add_lo(vd, static_cast<uint32_t>(kk * (2048 >> 4))),
+                         IDESC_O, (first && kk == 0) ? 0u : 1u);
+          }
+          __syncwarp();
+        }
+        ++pc[i];
+        return true;
+      };
+      bool pend = false, pend_first = false, pend_last = false;  // P V1 of the step before
+      int pend_slot = 0;
+      auto flush = [&]() -> bool {
+        if (!pend) return true;
+        if (!issue_pv(1, pend_slot, pend_first)) return false;
+        if (pend_last) commit(&bars->o_full[1]);
+        commit(&bars->kv_free[pend_slot]);
+        pend = false;
+        return true;
+      };
+      for (int x = blockIdx.x; x < args.units && ok; x += gridDim.x) {
+        const Unit u = unit_of(args, x);
+        if (u.n == 0) continue;
+        const int q0c = qc, q1c = qc + 1;
+        qc += u.two ? 2 : 1;
+        for (int j = 0; j < u.n && ok; ++j, ++step) {
+          const int kc = 2 * step, vc = 2 * step + 1;
+          const int key0 = (u.j0 + j) * BKV;
+          const uint32_t mb = masked ? mask_bytes(a, u.b, key0, u.len, lane) : 0u;
+          ok = wait_kv(kc) && (j > 0 || wait(&bars->q_full[q0c % QST], (q0c / QST) & 1, 3));
+          if (!ok) break;
+          issue_s(0, q0c % QST, kc % KVST);
+          const bool last = j == u.n - 1;
+          if (last) commit(&bars->q_free[q0c % QST]);
+          ok = flush() && (j > 0 || !u.two || wait(&bars->q_full[q1c % QST], (q1c / QST) & 1, 3));
+          if (!ok) break;
+          if (u.two) issue_s(1, q1c % QST, kc % KVST);
+          commit(&bars->kv_free[kc % KVST]);
+          if (last && u.two) commit(&bars->q_free[q1c % QST]);
+          ok = wait_kv(vc);
+          if (!ok) break;
+          uint32_t w[4];
+          keep_words(masked, mb, u.len - key0, w);
+          if ((w[0] & w[1] & w[2] & w[3]) != 0xffffffffu) {
+            // rows of V that are left out: zeros (a row's 16-byte pieces keep
+            // their row under the swizzle, so the order does not matter)
+            const uint32_t v = smem_u32(sKV + (vc % KVST) * C::TILE_BYTES);
+            const int piece = lane & 7;
+            for (int r = lane >> 3; r < BKV; r += 4) {
+              if (((w[r >> 5] >> (r & 31)) & 1u) == 0) {
+#pragma unroll
+                for (int h = 0; h < C::HALVES; ++h)
+                  asm volatile("st.shared.v4.u32 [%0], {%1,%1,%1,%1};" ::"r"(v + h * C::HALF_BYTES + r * 128 + piece * 16),
+                               "r"(0u)
+                               : "memory");
+              }
+            }
+            fence_proxy_async_smem();
+            __syncwarp();
+          }
+          ok = issue_pv(0, vc % KVST, j == 0);
+          if (!ok) break;
+          if (last) commit(&bars->o_full[0]);
+          if (u.two) {
+            pend = true;
+            pend_first = j == 0;
+            pend_last = last;
+            pend_slot = vc % KVST;
+          } else {
+            commit(&bars->kv_free[vc % KVST]);
+          }
+        }
+      }
+      if (ok) flush();
+      commit(&bars->drain);
+      warp_wait(&bars->drain, 0, 8, nullptr);
+    }
+  } else {
+    // ------------------------------------------------------------ softmax, stores
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(REGS_SOFTMAX));
+    const int wg = warp >> 2;
+    const int row = (warp & 3) * 32 + lane;
+    const uint32_t lane_off = static_cast<uint32_t>((warp & 3) * 32) << 16;
+    const uint32_t s_tmem = tmem + s_col(wg) + lane_off;
+    const uint32_t o_tmem = tmem + o_col(wg) + lane_off;
+    const int64_t total_rows = static_cast<int64_t>(a.batch) * a.heads * a.s_q;
+    uint32_t sc = 0, oc = 0;  // S tiles, O tiles seen
+    bool ok = true;
+    for (int x = blockIdx.x; x < args.units && ok; x += gridDim.x) {
+      const Unit u = unit_of(args, x);
+      if (wg == 1 && !u.two) continue;
+      const int q_row = u.q0 + wg * BQ + row;
+      float m_run = -INFINITY;  // running max, log2 domain
+      float l_run = 0.0f;
+      for (int j = 0; j < u.n; ++j, ++sc) {
+        const int key0 = (u.j0 + j) * BKV;
+        const uint32_t mb = masked ? mask_bytes(a, u.b, key0, u.len, lane) : 0u;
+        // S_i of the next tile is published only after this tile's P_i
+        if (!warp_wait<true>(&bars->s_full[wg], sc & 1, 20, abort_flag)) {
+          ok = false;
+          break;
+        }
+        tc_fence_after();
+        uint32_t w[4];
+        keep_words(masked, mb, u.len - key0, w);
+        bool whole = (w[0] & w[1] & w[2] & w[3]) == 0xffffffffu;
+        if (a.causal && u.len - a.s_q + u.q0 + wg * BQ + 1 < key0 + BKV) {
+          const int valid = u.len - a.s_q + q_row + 1 - key0;
+#pragma unroll
+          for (int c = 0; c < 4; ++c) {
+            const int v = valid - 32 * c;
+            w[c] &= v >= 32 ? 0xffffffffu : (v <= 0 ? 0u : (1u << v) - 1u);
+          }
+          whole = false;
+        }
+        uint32_t r[128];
+        auto load_s = [&]() {
+#pragma unroll
+          for (int c = 0; c < 4; ++c) tmem_ld32p(s_tmem + c * 32, r + 32 * c);
+          tmem_wait_fence<4>(r);
+          if (!whole) {
+#pragma unroll
+            for (int e = 0; e < 128; ++e)
+              if ((w[e >> 5] & (1u << (e & 31))) == 0) r[e] = __float_as_uint(-INFINITY);
+          }
+        };
+        load_s();
+        // After the first tile half 0 is exponentiated against the running
+        // maximum while the tile's is found; only where that outgrew it by
+        // more than the threshold the warp reloads S (P is not written yet).
+        float m_use = m_run;
+        float sum = 0.0f;
+        bool slow = j == 0;
+        if (!slow) {
+          const float2 sm = exp_pack64<F16, true>(r, r, args.scale_log2, m_run == -INFINITY ? 0.0f : -m_run);
+          slow = __any_sync(0xffffffffu, sm.y * args.scale_log2 > m_run + RESCALE_THRESHOLD);
+          if (slow) {
+            load_s();
+          } else {
+            sum = sm.x;
+          }
+        }
+        if (slow) {
+          const float m_tile = fmaxf(row_max64(r), row_max64(r + 64)) * args.scale_log2;
+          const bool rescale = m_tile > m_run + RESCALE_THRESHOLD;
+          if (rescale) m_use = m_tile;
+          if (__any_sync(0xffffffffu, rescale)) {
+            const float factor = rescale ? ex2(m_run - m_use) : 1.0f;
+            l_run *= factor;
+            if (j > 0) {
+#pragma unroll
+              for (int c = 0; c < D / 32; ++c) {
+                uint32_t o[32];
+                tmem_ld32p(o_tmem + c * 32, o);
+                tmem_wait_fence<1>(o);
+#pragma unroll
+                for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * factor);
+                tmem_st32(o_tmem + c * 32, o);
+              }
+            }
+            if (rescale) m_run = m_use;
+          }
+          sum = exp_pack64<F16, false>(r, r, args.scale_log2, m_use == -INFINITY ? 0.0f : -m_use).x;
+        }
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          if (h == 1)
+            sum += exp_pack64<F16, false>(r + 64, r + 32, args.scale_log2, m_use == -INFINITY ? 0.0f : -m_use).x;
+          tmem_st32(s_tmem + 32 * h, *reinterpret_cast<uint32_t(*)[32]>(r + 32 * h));
+          tc_wait_st();
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&bars->p_half[wg][h]);
+        }
+        l_run += sum;
+      }
+      if (!ok) break;
+      // ---- the unit's rows
+      if (u.n > 0) {
+        if (!warp_wait(&bars->o_full[wg], oc & 1, 23, abort_flag)) {
+          ok = false;
+          break;
+        }
+        ++oc;
+        tc_fence_after();
+      }
+      const bool in = q_row < a.s_q;
+      const int64_t lse_row = (static_cast<int64_t>(u.b) * a.heads + u.head) * a.s_q + q_row;
+      const float inv_l = l_run > 0.0f ? 1.0f / l_run : 0.0f;
+      uint16_t* orow = static_cast<uint16_t*>(a.o) + u.b * a.o_stride[0] + q_row * a.o_stride[1] + u.head * a.o_stride[2];
+      float* prow = a.part_o + (u.split * total_rows + lse_row) * D;
+#pragma unroll
+      for (int c = 0; c < D / 32; ++c) {
+        uint32_t r[32];
+        if (u.n > 0) {
+          tmem_ld32p(o_tmem + c * 32, r);
+          tmem_wait_fence<1>(r);
+        } else {
+#pragma unroll
+          for (int e = 0; e < 32; ++e) r[e] = 0u;
+        }
+        if (!in) continue;
+        if (a.splits > 1) {
+#pragma unroll
+          for (int e = 0; e < 32; e += 8) {
+            uint32_t v[8];
+#pragma unroll
+            for (int t = 0; t < 8; ++t) v[t] = r[e + t];
+            st_global_v8(prow + c * 32 + e, v);
+          }
+        } else {
+          uint32_t p[16];
+#pragma unroll
+          for (int e = 0; e < 16; ++e)
+            p[e] = pack16x2<F16>(__uint_as_float(r[2 * e]) * inv_l, __uint_as_float(r[2 * e + 1]) * inv_l);
+          if (args.o_wide) {
+#pragma unroll
+            for (int e = 0; e < 16; e += 8) {
+              uint32_t v[8];
+#pragma unroll
+              for (int t = 0; t < 8; ++t) v[t] = p[e + t];
+              st_global_v8(orow + c * 32 + 2 * e, v);
+            }
+          } else {
+#pragma unroll
+            for (int e = 0; e < 16; e += 4)
+              *reinterpret_cast<uint4*>(orow + c * 32 + 2 * e) = make_uint4(p[e], p[e + 1], p[e + 2], p[e + 3]);
+          }
+        }
+      }
+      if (in) {
+        if (a.splits > 1) {
+          a.part_ml[u.split * total_rows + lse_row] = make_float2(m_run, l_run);
+        } else if (a.lse != nullptr) {
+          a.lse[lse_row] = l_run > 0.0f ? (m_run + __log2f(l_run)) * LN2 : -INFINITY;
+        }
+      }
+    }
+  }
+
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 9) {
+    tc_fence_after();
+    tmem_dealloc(tmem, 512);
+  }
+}
+
+template <int D, bool F16>
+int launch(const XAttn& a, cudaStream_t stream) {
+  const CUtensorMapDataType dt = F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+  CUtensorMap tq, tk, tv;
+  auto encode = [&](CUtensorMap* m, const void* p, const int64_t (&st)[3], int seq, int heads) {
+    const uint64_t dims[4] = {D, static_cast<uint64_t>(seq > 0 ? seq : 1), static_cast<uint64_t>(heads),
+                              static_cast<uint64_t>(a.batch)};
+    const uint64_t sb[3] = {static_cast<uint64_t>(st[1]) * 2, static_cast<uint64_t>(st[2]) * 2,
+                            static_cast<uint64_t>(st[0]) * 2};
+    const uint32_t box[4] = {64, 128, 1, 1};
+    return h3b::encode_4d(m, dt, p, dims, sb, box, CU_TENSOR_MAP_SWIZZLE_128B);
+  };
+  int rc = encode(&tq, a.q, a.q_stride, a.s_q, a.heads);
+  if (rc == H3B_OK) rc = encode(&tk, a.k, a.kv_stride, a.s_kv, a.kv_heads);
+  if (rc == H3B_OK) rc = encode(&tv, a.v, a.kv_stride, a.s_kv, a.kv_heads);
+  if (rc != H3B_OK) return rc;
+  auto kernel = xattn_tile_kernel<D, F16>;
+  static bool attr = false;
+  if (!attr) {
+    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem_bytes<D>())) !=
+        cudaSuccess)
+      return H3B_ERR_LAUNCH;
+    attr = true;
+  }
+  TileArgs args{};
+  args.a = a;
+  args.group = a.heads / a.kv_heads;
+  args.q_tiles = (a.s_q + 2 * BQ - 1) / (2 * BQ);
+  const int64_t units = static_cast<int64_t>(a.batch) * a.heads * a.splits * args.q_tiles;
+  if (units > 0x3fffffff) return H3B_ERR_SHAPE;
+  args.units = static_cast<int>(units);
+  args.scale_log2 = a.scale * LOG2E;
+  args.o_wide = (reinterpret_cast<uintptr_t>(a.o) & 31u) == 0 && a.o_stride[0] % 16 == 0 && a.o_stride[1] % 16 == 0 &&
+                a.o_stride[2] % 16 == 0;
+  const int sms = h3b::num_sms();
+  kernel<<<static_cast<unsigned>(units < sms ? units : sms), THREADS, smem_bytes<D>(), stream>>>(tq, tk, tv, args);
+  return h3b::launch_status();
+}
+
+}  // namespace
+
+namespace h3b {
+
+int xattn_tile_splits(const XAttn& a) {
+  // Ranges of keys per row tile: units run in rounds of one per SM, so the
+  // call takes about ceil(units / SMs) / splits of a whole unit; a split
+  // costs the write and the second read of its fp32 rows, about as much as
+  // half a tile of 128 keys of work.
+  const int64_t tiles = (static_cast<int64_t>(a.s_kv) + BKV - 1) / BKV;
+  const int64_t base = static_cast<int64_t>(a.batch) * a.heads * ((a.s_q + 2 * BQ - 1) / (2 * BQ));
+  const int sms = num_sms();
+  int best = 1;
+  double cost = 1e30;
+  for (int s = 1; s <= 32 && s <= tiles; ++s) {
+    const double per = static_cast<double>((tiles + s - 1) / s) + 1.0 + (s > 1 ? 2.0 : 0.0);
+    const double c = static_cast<double>((base * s + sms - 1) / sms) * per;
+    if (c < cost * 0.97) {
+      cost = c;
+      best = s;
+    }
+  }
+  return best;
+}
+
+int xattn_tile_launch(const XAttn& a, cudaStream_t stream) {
+  int rc;
+  if (a.head_dim == 128) {
+    rc = a.dtype == H3B_F16 ? launch<128, true>(a, stream) : launch<128, false>(a, stream);
+  } else {
+    rc = a.dtype == H3B_F16 ? launch<64, true>(a, stream) : launch<64, false>(a, stream);
+  }
+  return rc != H3B_OK || a.splits == 1 ? rc : xattn_combine_launch(a, stream);
+}
+
+}  // namespace h3b
