@@ -275,7 +275,7 @@ H3B_API int h3b_qk_rmsnorm_rope(void* q, void* k, int64_t s, int64_t heads, int6
  * 156-289).
  * Strides % 8 == 0 and > 0 (any value along an axis of extent 1), pointers
  * 16-byte aligned.  workspace: h3b_cross_attention_workspace() bytes (may be
- * 0), 16-byte aligned, free to reuse when the call's work is done.
+ * 0), 32-byte aligned, free to reuse when the call's work is done.
  */
 H3B_API int h3b_cross_attention_workspace(int64_t batch, int64_t heads, int64_t kv_heads, int64_t head_dim,
                                           int64_t s_q, int64_t s_kv, int64_t* bytes);
@@ -287,6 +287,28 @@ H3B_API int h3b_cross_attention_fwd(const void* q, const void* k, const void* v,
                                     int64_t o_head_stride, const int32_t* kv_lens, const uint8_t* key_mask,
                                     int64_t mask_stride, float scale, void* workspace, int64_t workspace_bytes,
                                     h3b_stream_t stream);
+
+/*
+ * Gradients of h3b_cross_attention_fwd for d_o, the gradient of o: dq dense
+ * [batch, s_q, heads, head_dim], dk, dv dense [batch, s_kv, kv_heads,
+ * head_dim] (the heads that share a key head summed), in dtype, 32-byte
+ * aligned.  q, k, v, o, lse, kv_lens, key_mask and scale as in the forward
+ * call; d_o has strides of its own.  Left-out keys get zero gradients, rows
+ * without kept keys too.  fp32 sums in a fixed order: the same inputs give
+ * the same bits.  workspace: h3b_cross_attention_bwd_workspace() bytes,
+ * 32-byte aligned.
+ */
+H3B_API int h3b_cross_attention_bwd_workspace(int64_t batch, int64_t heads, int64_t kv_heads, int64_t head_dim,
+                                              int64_t s_q, int64_t s_kv, int64_t* bytes);
+H3B_API int h3b_cross_attention_bwd(const void* d_o, const void* q, const void* k, const void* v, const void* o,
+                                    const float* lse, void* dq, void* dk, void* dv, int dtype, int64_t batch,
+                                    int64_t heads, int64_t kv_heads, int64_t head_dim, int64_t s_q, int64_t s_kv,
+                                    int64_t do_batch_stride, int64_t do_seq_stride, int64_t do_head_stride,
+                                    int64_t q_batch_stride, int64_t q_seq_stride, int64_t q_head_stride,
+                                    int64_t kv_batch_stride, int64_t kv_seq_stride, int64_t kv_head_stride,
+                                    int64_t o_batch_stride, int64_t o_seq_stride, int64_t o_head_stride,
+                                    const int32_t* kv_lens, const uint8_t* key_mask, int64_t mask_stride,
+                                    float scale, void* workspace, int64_t workspace_bytes, h3b_stream_t stream);
 
 /* --------------------------------------------- 8-bit key/value cache */
 

@@ -50,6 +50,8 @@ SIGNATURES: dict[str, list] = {
                                                  c_f32, c_ptr, c_ptr, c_ptr, c_int, c_ptr],
     "h3b_cross_attention_workspace": [c_i64] * 6 + [c_ptr],
     "h3b_cross_attention_fwd": [c_ptr] * 5 + [c_int] + [c_i64] * 15 + [c_ptr, c_ptr, c_i64, c_f32, c_ptr, c_i64, c_ptr],
+    "h3b_cross_attention_bwd_workspace": [c_i64] * 6 + [c_ptr],
+    "h3b_cross_attention_bwd": [c_ptr] * 9 + [c_int] + [c_i64] * 18 + [c_ptr, c_ptr, c_i64, c_f32, c_ptr, c_i64, c_ptr],
     "h3b_kv8_append": [c_ptr, c_ptr, c_int] + [c_i64] * 7 + [c_ptr] * 4 + [c_int, c_i64, c_i64, c_ptr, c_i64, c_ptr,
                                                                            c_ptr, c_ptr],
     "h3b_kv8_read": [c_ptr] * 4 + [c_int] + [c_i64] * 4 + [c_ptr, c_i64, c_ptr, c_i64, c_i64, c_ptr, c_ptr, c_int,
@@ -105,7 +107,8 @@ def lib() -> ctypes.CDLL:
 
 
 # Entry points that launch no kernel of this library.
-_NO_LAUNCH = {"h3b_version", "h3b_device_status", "h3b_cross_attention_workspace", "h3b_kv8_attention_workspace"}
+_NO_LAUNCH = {"h3b_version", "h3b_device_status", "h3b_cross_attention_workspace",
+              "h3b_cross_attention_bwd_workspace", "h3b_kv8_attention_workspace"}
 LAUNCHES = [0]  # kernels this process has launched through the ABI
 
 

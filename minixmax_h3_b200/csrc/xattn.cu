@@ -45,7 +45,7 @@ int run(XAttn& a, void* workspace, int64_t workspace_bytes, cudaStream_t stream)
   if (need > 0) {
     if (workspace == nullptr) return H3B_ERR_ARG;
     if (workspace_bytes < need) return H3B_ERR_SHAPE;
-    if (!h3b::aligned16(workspace)) return H3B_ERR_ALIGN;
+    if ((reinterpret_cast<uintptr_t>(workspace) & 31u) != 0) return H3B_ERR_ALIGN;
     a.part_o = static_cast<float*>(workspace);
     a.part_ml = reinterpret_cast<float2*>(a.part_o + rows_of(a) * a.splits * a.head_dim);
   }
@@ -109,6 +109,95 @@ extern "C" int h3b_cross_attention_fwd(const void* q, const void* k, const void*
   a.mask_stride = mask_stride;
   a.scale = scale;
   return run(a, workspace, workspace_bytes, reinterpret_cast<cudaStream_t>(stream));
+}
+
+namespace {
+
+// Workspace of a backward call: the ranges' sums (16-byte pieces), then delta.
+int64_t grad_part_floats(const h3b::XAttnGrad& a) {
+  return a.splits > 1 ? 2ll * a.splits * a.batch * a.s_kv * a.kv_heads * a.head_dim : 0;
+}
+int64_t grad_workspace(const h3b::XAttnGrad& a) {
+  return (grad_part_floats(a) + static_cast<int64_t>(a.batch) * a.heads * a.s_q) * static_cast<int64_t>(sizeof(float));
+}
+h3b::XAttnGrad grad_sizes(int dtype, int64_t batch, int64_t heads, int64_t kv_heads, int64_t head_dim, int64_t s_q,
+                          int64_t s_kv) {
+  h3b::XAttnGrad a{};
+  a.dtype = dtype;
+  a.batch = static_cast<int>(batch);
+  a.heads = static_cast<int>(heads);
+  a.kv_heads = static_cast<int>(kv_heads);
+  a.head_dim = static_cast<int>(head_dim);
+  a.s_q = static_cast<int>(s_q);
+  a.s_kv = static_cast<int>(s_kv);
+  a.splits = h3b::xattn_bwd_splits(a);
+  return a;
+}
+
+}  // namespace
+
+extern "C" int h3b_cross_attention_bwd_workspace(int64_t batch, int64_t heads, int64_t kv_heads, int64_t head_dim,
+                                                 int64_t s_q, int64_t s_kv, int64_t* bytes) {
+  if (bytes == nullptr) return H3B_ERR_ARG;
+  const int rc = check_sizes(H3B_BF16, batch, heads, kv_heads, head_dim, s_q, s_kv);
+  if (rc != H3B_OK) return rc;
+  *bytes = grad_workspace(grad_sizes(H3B_BF16, batch, heads, kv_heads, head_dim, s_q, s_kv));
+  return H3B_OK;
+}
+
+extern "C" int h3b_cross_attention_bwd(const void* d_o, const void* q, const void* k, const void* v, const void* o,
+                                       const float* lse, void* dq, void* dk, void* dv, int dtype, int64_t batch,
+                                       int64_t heads, int64_t kv_heads, int64_t head_dim, int64_t s_q, int64_t s_kv,
+                                       int64_t do_batch_stride, int64_t do_seq_stride, int64_t do_head_stride,
+                                       int64_t q_batch_stride, int64_t q_seq_stride, int64_t q_head_stride,
+                                       int64_t kv_batch_stride, int64_t kv_seq_stride, int64_t kv_head_stride,
+                                       int64_t o_batch_stride, int64_t o_seq_stride, int64_t o_head_stride,
+                                       const int32_t* kv_lens, const uint8_t* key_mask, int64_t mask_stride,
+                                       float scale, void* workspace, int64_t workspace_bytes, h3b_stream_t stream) {
+  const int rc = check_sizes(dtype, batch, heads, kv_heads, head_dim, s_q, s_kv);
+  if (rc != H3B_OK) return rc;
+  if (!(scale > 0.0f) || mask_stride < 0) return H3B_ERR_ARG;
+  if (batch == 0) return H3B_OK;
+  cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+  if (s_kv > 0 && (dk == nullptr || dv == nullptr)) return H3B_ERR_ARG;
+  if (s_q == 0) {  // no query: the sums over queries are zero
+    const size_t n = static_cast<size_t>(batch * s_kv * kv_heads * head_dim) * 2;
+    if (n == 0) return H3B_OK;
+    return cudaMemsetAsync(dk, 0, n, st) == cudaSuccess && cudaMemsetAsync(dv, 0, n, st) == cudaSuccess
+               ? H3B_OK
+               : H3B_ERR_LAUNCH;
+  }
+  h3b::XAttnGrad a = grad_sizes(dtype, batch, heads, kv_heads, head_dim, s_q, s_kv);
+  a.q = q, a.k = s_kv > 0 ? k : q, a.v = s_kv > 0 ? v : q, a.o = o, a.d_o = d_o, a.lse = lse;
+  a.dq = dq, a.dk = dk, a.dv = dv;
+  if (!a.q || !a.k || !a.v || !o || !d_o || !lse || !dq || !workspace) return H3B_ERR_ARG;
+  const int64_t st4[4][3] = {{q_batch_stride, q_seq_stride, q_head_stride},
+                             {kv_batch_stride, kv_seq_stride, kv_head_stride},
+                             {o_batch_stride, o_seq_stride, o_head_stride},
+                             {do_batch_stride, do_seq_stride, do_head_stride}};
+  for (int i = 0; i < 3; ++i) {
+    a.q_stride[i] = st4[0][i];
+    a.kv_stride[i] = st4[1][i];
+    a.o_stride[i] = st4[2][i];
+    a.do_stride[i] = st4[3][i];
+  }
+  if (!fix_strides(a.q_stride, batch, s_q, heads, head_dim) ||
+      !fix_strides(a.kv_stride, s_kv > 0 ? batch : 1, s_kv, s_kv > 0 ? kv_heads : 1, head_dim) ||
+      !fix_strides(a.o_stride, batch, s_q, heads, head_dim) || !fix_strides(a.do_stride, batch, s_q, heads, head_dim))
+    return H3B_ERR_ALIGN;
+  for (const void* p : {a.q, a.k, a.v, o, d_o})
+    if (!h3b::aligned16(p)) return H3B_ERR_ALIGN;
+  for (const void* p : {static_cast<const void*>(dq), static_cast<const void*>(dk), static_cast<const void*>(dv),
+                        static_cast<const void*>(workspace)})
+    if ((reinterpret_cast<uintptr_t>(p) & 31u) != 0) return H3B_ERR_ALIGN;
+  if (workspace_bytes < grad_workspace(a)) return H3B_ERR_SHAPE;
+  a.part = static_cast<float*>(workspace);
+  a.delta = a.part + grad_part_floats(a);
+  a.kv_lens = kv_lens;
+  a.key_mask = s_kv > 0 ? key_mask : nullptr;
+  a.mask_stride = mask_stride;
+  a.scale = scale;
+  return h3b::xattn_bwd_launch(a, st);
 }
 
 extern "C" int h3b_kv8_attention_workspace(int64_t batch, int64_t heads, int64_t kv_heads, int64_t head_dim,

@@ -45,6 +45,31 @@ struct XAttn {
   float2* part_ml; // [splits, batch*heads*s_q]: running max (log2 domain), sum
 };
 
+// A backward call.  Outputs dq, dk, dv are dense [batch, tokens, heads, D].
+struct XAttnGrad {
+  const void* q;
+  const void* k;
+  const void* v;
+  const void* o;
+  const void* d_o;
+  const float* lse;  // [batch, heads, s_q]
+  void* dq;
+  void* dk;
+  void* dv;
+  int dtype;
+  int64_t q_stride[3], kv_stride[3], o_stride[3], do_stride[3];
+  int batch, heads, kv_heads, head_dim, s_q, s_kv;
+  const int32_t* kv_lens;
+  const uint8_t* key_mask;
+  int64_t mask_stride;
+  float scale;
+  float* delta;  // workspace [batch, heads, s_q]
+  int splits;
+  float* part;   // workspace [dv | dk][splits, batch, s_kv, kv_heads, D], if splits > 1
+};
+int xattn_bwd_splits(const XAttnGrad& a);
+int xattn_bwd_launch(const XAttnGrad& a, cudaStream_t stream);
+
 // Keys split over so many ranges by the row kernel / the tile kernel.
 int xattn_rows_splits(const XAttn& a);
 int xattn_tile_splits(const XAttn& a);

@@ -1,0 +1,1051 @@
+// Gradients of cross attention (h3b_cross_attention_bwd) on tcgen05.
+//
+//   P = 2^(scale log2e S - lse log2e),  delta_i = do_i . o_i
+//   dP = dO V^T,  dS = P (dP - delta)
+//   dQ = scale dS K,  dK = scale dS^T Q,  dV = P^T dO   (a key head's query heads summed)
+//
+// Two kernels, each the owner of what it sums, so no sum crosses CTAs through
+// atomics and the result does not depend on scheduling:
+//   xattn_dq_kernel   a unit is 128 query rows of one head; it runs over the
+//                     key tiles (three products a tile) and also finds delta.
+//   xattn_dkv_kernel  a unit is 128 keys of one key head and a range of the
+//                     query tiles of all heads that share it (four products a
+//                     tile), in the transposed form: TMEM lanes are keys.
+//                     Ranges exist because an encoder's keys are few (512 keys
+//                     x 24 heads are 96 units for 148 SMs); their fp32 sums
+//                     are joined in order by xattn_dkv_join_kernel.
+// That is seven products where five would do if dQ were summed across key
+// tiles in memory; the five-product form needs fp32 atomics on dQ (one 64 KB
+// tile per 128 x 128 block) or a cluster exchange of them.
+// P and dS go back to TMEM as 16-bit values and are the A operands; Q, dO and
+// K tiles are read from shared memory both ways (K-major for S and dP,
+// MN-major for the sums) through two descriptors of the same bytes.
+// Work of a 128 x 128 block on the other pipes: 16384 exponentials and ~10
+// fp32 operations a value, two warpgroups of 64 columns each.
+// In f16, P is held times 2^8 (P <= 1), which lowers the point where small
+// weights lose bits; dS is not scaled (its size is the caller's loss scale).
+#include "h3b_common.cuh"
+#include "h3b_host.hpp"
+#include "xattn.hpp"
+
+H3B_DECLARE_STATUS();
+H3B_REGISTER_STATUS_READER(xattn_bwd);
+
+namespace {
+
+using h3b::XAttnGrad;
+
+constexpr int THREADS = 384;  // two compute warpgroups; TMA, MMA, statistics, idle
+constexpr int REGS_LAUNCH = 168;
+constexpr int REGS_CONTROL = 88;
+constexpr int REGS_COMPUTE = 208;
+static_assert(128 * (REGS_CONTROL + 2 * REGS_COMPUTE) <= THREADS * REGS_LAUNCH, "register split exceeds launch");
+constexpr float LOG2E = 1.4426950408889634f;
+
+template <int D>
+struct Cfg {
+  static constexpr int HALVES = D / 64;
+  static constexpr int TILE_BYTES = 128 * D * 2;
+  static constexpr int HALF_BYTES = 128 * 64 * 2;
+};
+
+H3B_DEV float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+template <bool SPIN = false>
+H3B_DEV bool warp_wait(uint64_t* bar, uint32_t parity, int site, volatile int* abort_flag) {
+  const bool ok = mbar_wait<SPIN>(bar, parity, &g_status, site, abort_flag);
+  return __all_sync(0xffffffffu, ok);
+}
+
+// The tiles need 1024-byte alignment; the same answer for the whole CTA,
+// before it has started anything.
+H3B_DEV bool misaligned(const uint8_t* smem) {
+  if ((smem_u32(smem) & 1023u) == 0) return false;
+  if (threadIdx.x == 0 && atomicCAS(&g_status.code, 0, H3B_ERR_DEVICE) == 0) g_status.site = 30;
+  return true;
+}
+
+// log2-domain row statistic; a row without kept keys (-inf) gives +inf, so
+// that all its weights are 2^-inf = 0.
+H3B_DEV float lse2_of(float lse) { return lse == -INFINITY ? INFINITY : lse * LOG2E; }
+
+// Products of one 128-row tile: D (+)= A B^T with both operands K-major in
+// shared memory (contraction over the head dim), and D (+)= A B with A in
+// TMEM (two pieces of 64 columns' worth, at a0 and a1) and B MN-major.
+template <int D>
+H3B_DEV void issue_ss(uint32_t d, uint32_t a_s, uint32_t b_s, uint32_t idesc) {
+  const uint64_t ad = sdesc_kmajor_sw128(a_s), bd = sdesc_kmajor_sw128(b_s);
+#pragma unroll
+  for (int kk = 0; kk < D / 16; ++kk) {
+    const uint32_t at = static_cast<uint32_t>((kk >> 2) * (Cfg<D>::HALF_BYTES >> 4) + (kk & 3) * 2);
+    mma_f16_ss(d, desc_add_lo(ad, at), desc_add_lo(bd, at), idesc, kk > 0);
+  }
+}
+template <int D>
+H3B_DEV void issue_ts_half(uint32_t d, uint32_t a_tmem, uint32_t b_s, int half, uint32_t idesc, bool fresh) {
+  const uint64_t bd = sdesc_mnmajor_sw128(b_s, Cfg<D>::HALF_BYTES, 1024);
+#pragma unroll
+  for (int kk = 0; kk < 4; ++kk)
+    mma_f16_ts(d, a_tmem + kk * 8, desc_add_lo(bd, static_cast<uint32_t>((4 * half + kk) * (2048 >> 4))), idesc,
+               (fresh && kk == 0) ? 0u : 1u);
+}
+
+struct GradArgs {
+  XAttnGrad a;
+  int q_tiles;   // of 128 rows
+  int k_tiles;   // of 128 keys
+  int group;
+  int units;
+  float scale_log2;
+};
+
+// Kept-key words of a tile (see xattn_tile.cu).
+H3B_DEV uint32_t mask_bytes(const XAttnGrad& a, int b, int key0, int len, int lane) {
+  uint32_t m = 0;
+#pragma unroll
+  for (int c = 0; c < 4; ++c) {
+    const int key = key0 + c * 32 + lane;
+    if (key < len && __ldg(a.key_mask + b * a.mask_stride + key) != 0) m |= 1u << c;
+  }
+  return m;
+}
+H3B_DEV void keep_words(bool masked, uint32_t bytes, int valid, uint32_t (&w)[4]) {
+#pragma unroll
+  for (int c = 0; c < 4; ++c) {
+    const int v = valid - 32 * c;
+    w[c] = v >= 32 ? 0xffffffffu : (v <= 0 ? 0u : (1u << v) - 1u);
+    if (masked) w[c] = __ballot_sync(0xffffffffu, (bytes >> c) & 1u);
+  }
+}
+H3B_DEV int len_of(const XAttnGrad& a, int b) {
+  return a.kv_lens == nullptr ? a.s_kv : max(0, min(a.s_kv, __ldg(a.kv_lens + b)));
+}
+
+// ============================================================== dQ (and delta)
+// TMEM: SA | SB | dP | dQ.  S of tile j goes to SA or SB by turns, dS(j) over
+// it.  Issue order a tile: S(j+1); dP(j+1) when dP(j) has been read; dQ += dS(j) K(j).
+constexpr int XST = 3;  // ring of Q and dO tiles, by turns
+constexpr int KST = 2, VST = 2;
+
+struct __align__(8) DqBars {
+  uint64_t x_full[XST], x_free[XST];
+  uint64_t k_full[KST], k_free[KST];
+  uint64_t v_full[VST], v_free[VST];
+  uint64_t s_full[2];   // by step parity
+  uint64_t dp_full;
+  uint64_t dp_free;     // 8 warps have read dP
+  // [step parity][warpgroup], 4 warps each.  By parity, because S and dP run
+  // a tile ahead of dQ: a fast warp may deliver tile j + 1 before a slow one
+  // of its warpgroup has delivered tile j (but not j + 2, which waits for dQ(j)).
+  uint64_t ds_half[2][2];
+  uint64_t dq_full;
+  uint64_t delta_ready; // 8 warps
+  uint64_t drain;
+  uint32_t tmem_base;
+  int abort_flag;
+};
+
+// No slack for alignment: seven tiles and the statistics fill the shared
+// memory, whose start is aligned (checked by the kernels).
+template <int D>
+constexpr size_t dq_smem() {
+  return (XST + KST + VST) * Cfg<D>::TILE_BYTES + 2 * 256 * sizeof(float) + sizeof(DqBars);
+}
+
+static_assert(dq_smem<128>() <= 232448, "shared memory of a CTA");
+
+struct DqUnit {
+  int b, head, q0, len, n;
+};
+H3B_DEV DqUnit dq_unit(const GradArgs& args, int u) {
+  DqUnit x;
+  x.q0 = (u % args.q_tiles) * 128;
+  u /= args.q_tiles;
+  x.head = u % args.a.heads;
+  x.b = u / args.a.heads;
+  x.len = len_of(args.a, x.b);
+  x.n = (x.len + 127) / 128;
+  return x;
+}
+
+template <int D, bool F16>
+__global__ void __launch_bounds__(THREADS, 1)
+    xattn_dq_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_do,
+                    const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v,
+                    const __grid_constant__ GradArgs args) {
+  using C = Cfg<D>;
+  constexpr uint32_t IDESC_S = F16 ? idesc_f16_f32(128, 128, 0, 0) : idesc_bf16_f32(128, 128, 0, 0);
+  constexpr uint32_t IDESC_G = F16 ? idesc_f16_f32(128, D, 0, 1) : idesc_bf16_f32(128, D, 0, 1);
+  extern __shared__ __align__(1024) uint8_t smem_tiles[];
+  uint8_t* smem = smem_tiles;
+  if (misaligned(smem)) return;
+  uint8_t* sX = smem;
+  uint8_t* sK = sX + XST * C::TILE_BYTES;
+  uint8_t* sV = sK + KST * C::TILE_BYTES;
+  float* s_delta = reinterpret_cast<float*>(sV + VST * C::TILE_BYTES);  // [unit parity][256]
+  DqBars* bars = reinterpret_cast<DqBars*>(s_delta + 2 * 256);
+  const XAttnGrad& a = args.a;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  volatile int* abort_flag = &bars->abort_flag;
+  const bool masked = a.key_mask != nullptr;
+
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < XST; ++i) mbar_init(&bars->x_full[i], 1), mbar_init(&bars->x_free[i], 1);
+    for (int i = 0; i < KST; ++i) mbar_init(&bars->k_full[i], 1), mbar_init(&bars->k_free[i], 1);
+    for (int i = 0; i < VST; ++i) mbar_init(&bars->v_full[i], 1), mbar_init(&bars->v_free[i], 1);
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&bars->s_full[i], 1);
+      mbar_init(&bars->ds_half[i][0], 4);
+      mbar_init(&bars->ds_half[i][1], 4);
+    }
+    mbar_init(&bars->dp_full, 1);
+    mbar_init(&bars->dp_free, 8);
+    mbar_init(&bars->dq_full, 1);
+    mbar_init(&bars->delta_ready, 8);
+    mbar_init(&bars->drain, 1);
+    bars->abort_flag = 0;
+    fence_barrier_init();
+  }
+  if (warp == 9) {
+    tmem_alloc(&bars->tmem_base, 512);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = bars->tmem_base;
+  constexpr uint32_t DP_COL = 256, DQ_COL = 384;
+
+  if (warp >= 8) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(REGS_CONTROL));
+    if (warp == 8 && lane == 0) {
+      // ---------------------------------------------------------- TMA
+      // A slot's free barrier completed phase (c / ring) - 1 when the tile
+      // before it was read, and its next phase needs this load.
+      prefetch_tmap(&tm_q);
+      prefetch_tmap(&tm_do);
+      prefetch_tmap(&tm_k);
+      prefetch_tmap(&tm_v);
+      int xc = 0, kc = 0, vc = 0;
+      bool ok = true;
+      auto load = [&](const CUtensorMap* tm, uint8_t* ring, uint64_t* full, uint64_t* free_, int stages, int& c, int row,
+                      int head, int b) {
+        const int s = c % stages;
+        if (c >= stages && !mbar_wait(&free_[s], (c / stages - 1) & 1, &g_status, 1, abort_flag)) return false;
+        mbar_arrive_expect_tx(&full[s], C::TILE_BYTES);
+        for (int h = 0; h < C::HALVES; ++h)
+          tma_load_4d(ring + s * C::TILE_BYTES + h * C::HALF_BYTES, tm, h * 64, row, head, b, &full[s]);
+        ++c;
+        return true;
+      };
+      for (int x = blockIdx.x; x < args.units && ok; x += gridDim.x) {
+        const DqUnit u = dq_unit(args, x);
+        for (int j = 0; j < u.n && ok; ++j) {
+          const int kvh = u.head / args.group;
+          if (j == 0) ok = ok && load(&tm_q, sX, bars->x_full, bars->x_free, XST, xc, u.q0, u.head, u.b);
+          ok = ok && load(&tm_k, sK, bars->k_full, bars->k_free, KST, kc, j * 128, kvh, u.b);
+          if (j == 0) ok = ok && load(&tm_do, sX, bars->x_full, bars->x_free, XST, xc, u.q0, u.head, u.b);
+          ok = ok && load(&tm_v, sV, bars->v_full, bars->v_free, VST, vc, j * 128, kvh, u.b);
+        }
+      }
+      if (!ok || *abort_flag) {
+        for (int c = max(0, xc - XST); c < xc; ++c)
+          mbar_wait(&bars->x_full[c % XST], (c / XST) & 1, &g_status, 10, nullptr);
+        for (int c = max(0, kc - KST); c < kc; ++c)
+          mbar_wait(&bars->k_full[c % KST], (c / KST) & 1, &g_status, 11, nullptr);
+        for (int c = max(0, vc - VST); c < vc; ++c)
+          mbar_wait(&bars->v_full[c % VST], (c / VST) & 1, &g_status, 12, nullptr);
+      }
+    } else if (warp == 9) {
+      // ---------------------------------------------------------- MMA
+      // Two cursors run over the same tiles: `f` one tile ahead issues S and
+      // dP, `c` issues dQ.
+      bool ok = true;
+      auto commit = [&](uint64_t* bar) {
+        if (elect_one()) tc_commit(bar);
+        __syncwarp();
+      };
+      auto wait = [&](uint64_t* bar, uint32_t parity, int site) {
+        if (!warp_wait<true>(bar, parity, site, abort_flag)) return false;
+        tc_fence_after();
+        return true;
+      };
+      struct Cursor {
+        int x, j, step, xc;  // unit index, tile, steps done, index of the unit's Q tile in its ring
+        DqUnit u;
+      };
+      auto settle = [&](Cursor& c) {  // to the next unit that has tiles
+        while (c.x < args.units) {
+          c.u = dq_unit(args, c.x);
+          if (c.u.n > 0) break;
+          c.x += gridDim.x;
+        }
+      };
+      auto advance = [&](Cursor& c) {
+        ++c.step;
+        if (++c.j == c.u.n) {
+          c.j = 0;
+          c.xc += 2;
+          c.x += gridDim.x;
+          settle(c);
+        }
+      };
+      auto issue_s = [&](const Cursor& f) -> bool {
+        const int key0 = f.j * 128;
+        const uint32_t mb = masked ? mask_bytes(a, f.u.b, key0, f.u.len, lane) : 0u;
+        if (f.j == 0 && !wait(&bars->x_full[f.xc % XST], (f.xc / XST) & 1, 3)) return false;
+        if (!wait(&bars->k_full[f.step % KST], (f.step / KST) & 1, 4)) return false;
+        uint32_t w[4];
+        keep_words(masked, mb, f.u.len - key0, w);
+        const uint32_t k_s = smem_u32(sK + (f.step % KST) * C::TILE_BYTES);
+        if ((w[0] & w[1] & w[2] & w[3]) != 0xffffffffu) {
+          // left-out rows of K are zeroed: dS is 0 there, but 0 * NaN is not
+          const int piece = lane & 7;
+          for (int r = lane >> 3; r < 128; r += 4)
+            if (((w[r >> 5] >> (r & 31)) & 1u) == 0) {
+#pragma unroll
+              for (int h = 0; h < C::HALVES; ++h)
+                asm volatile("st.shared.v4.u32 [%0], {%1,%1,%1,%1};" ::"r"(k_s + h * C::HALF_BYTES + r * 128 + piece * 16),
+                             "r"(0u)
+                             : "memory");
+            }
+          fence_proxy_async_smem();
+          __syncwarp();
+        }
+        if (elect_one()) {
+          issue_ss<D>(tmem + (f.step & 1) * 128, smem_u32(sX + (f.xc % XST) * C::TILE_BYTES), k_s, IDESC_S);
+          tc_commit(&bars->s_full[f.step & 1]);
+          if (f.j == f.u.n - 1) tc_commit(&bars->x_free[f.xc % XST]);
+        }
+        __syncwarp();
+        return true;
+      };
+      auto issue_dp = [&](const Cursor& f) -> bool {
+        const int dc = f.xc + 1;
+        if (f.j == 0 && !wait(&bars->x_full[dc % XST], (dc / XST) & 1, 5)) return false;
+        if (!wait(&bars->v_full[f.step % VST], (f.step / VST) & 1, 6)) return false;
+        // dP(step - 1) has been read: the barrier's next phase follows this dP
+        if (f.step > 0 && !wait(&bars->dp_free, (f.step - 1) & 1, 7)) return false;
+        if (elect_one()) {
+          issue_ss<D>(tmem + DP_COL, smem_u32(sX + (dc % XST) * C::TILE_BYTES),
+                      smem_u32(sV + (f.step % VST) * C::TILE_BYTES), IDESC_S);
+          tc_commit(&bars->dp_full);
+          tc_commit(&bars->v_free[f.step % VST]);
+          if (f.j == f.u.n - 1) tc_commit(&bars->x_free[dc % XST]);
+        }
+        __syncwarp();
+        return true;
+      };
+      auto issue_dq = [&](const Cursor& c) -> bool {
+        const uint32_t k_s = smem_u32(sK + (c.step % KST) * C::TILE_BYTES);
+        uint64_t* ds = bars->ds_half[c.step & 1];
+        const uint32_t phase = (c.step >> 1) & 1;
+        for (int h = 0; h < 2; ++h) {
+          if (!wait(&ds[h], phase, 8)) return false;
+          // The first product of a unit overwrites dQ, half of which each
+          // warpgroup reads: both have to be past the last unit's stores.
+          if (c.j == 0 && h == 0 && !wait(&ds[1], phase, 8)) return false;
+          if (elect_one())
+            issue_ts_half<D>(tmem + DQ_COL, tmem + (c.step & 1) * 128 + h * 64, k_s, h, IDESC_G, c.j == 0 && h == 0);
+          __syncwarp();
+        }
+        if (elect_one()) {
+          tc_commit(&bars->k_free[c.step % KST]);
+          if (c.j == c.u.n - 1) tc_commit(&bars->dq_full);
+        }
+        __syncwarp();
+        return true;
+      };
+      Cursor f{static_cast<int>(blockIdx.x), 0, 0, 0, {}};
+      settle(f);
+      Cursor c = f;
+      if (f.x < args.units) {
+        ok = issue_s(f) && issue_dp(f);
+        advance(f);
+      }
+      while (ok && c.x < args.units) {
+        if (f.x < args.units) {
+          ok = issue_s(f) && issue_dp(f);
+          advance(f);
+        }
+        ok = ok && issue_dq(c);
+        advance(c);
+      }
+      commit(&bars->drain);
+      warp_wait(&bars->drain, 0, 9, nullptr);
+    }
+  } else {
+    // ------------------------------------------------------------ compute
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(REGS_COMPUTE));
+    const int wg = warp >> 2;
+    const int row = (warp & 3) * 32 + lane;
+    const uint32_t lane_off = static_cast<uint32_t>((warp & 3) * 32) << 16;
+    uint32_t step = 0, uc = 0, qc = 0;
+    bool ok = true;
+    for (int x = blockIdx.x; x < args.units && ok; x += gridDim.x, ++uc) {
+      const DqUnit u = dq_unit(args, x);
+      const int q_row = u.q0 + row;
+      const int64_t stat = (static_cast<int64_t>(u.b) * a.heads + u.head) * a.s_q;
+      // ---- delta = do . o of the unit's rows: warp w takes rows 16 w .. 16 w + 15,
+      // D / 8 lanes a row.  Where one tile holds all keys it is summed from
+      // P and dP instead (below): with few keys dP is close to delta, and the
+      // 16-bit rounding of o would cost dS bits (measured: 1.6 to 2.3 times
+      // the error of dq and dk at 2 to 26 keys).
+      if (u.n != 1) {
+        constexpr int LPR = D / 8, RPI = 32 / LPR;  // lanes a row, rows an instruction
+        float part[16 / RPI];
+        const uint16_t* op = static_cast<const uint16_t*>(a.o) + u.b * a.o_stride[0] + u.head * a.o_stride[2];
+        const uint16_t* gp = static_cast<const uint16_t*>(a.d_o) + u.b * a.do_stride[0] + u.head * a.do_stride[2];
+        const int col = (lane % LPR) * 8;
+#pragma unroll
+        for (int i = 0; i < 16 / RPI; ++i) {
+          const int r = u.q0 + warp * 16 + i * RPI + lane / LPR;
+          float s = 0.0f;
+          if (r < a.s_q) {
+            const uint4 ov = __ldg(reinterpret_cast<const uint4*>(op + r * a.o_stride[1] + col));
+            const uint4 gv = __ldg(reinterpret_cast<const uint4*>(gp + r * a.do_stride[1] + col));
+            const uint32_t ow[4] = {ov.x, ov.y, ov.z, ov.w}, gw[4] = {gv.x, gv.y, gv.z, gv.w};
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              if constexpr (F16) {
+                const float2 of = __half22float2(*reinterpret_cast<const __half2*>(&ow[k]));
+                const float2 gf = __half22float2(*reinterpret_cast<const __half2*>(&gw[k]));
+                s = fmaf(of.x, gf.x, fmaf(of.y, gf.y, s));
+              } else {
+                s = fmaf(bf16lo_to_f32(ow[k]), bf16lo_to_f32(gw[k]), s);
+                s = fmaf(bf16hi_to_f32(ow[k]), bf16hi_to_f32(gw[k]), s);
+              }
+            }
+          }
+          part[i] = s;
+        }
+#pragma unroll
+        for (int i = 0; i < 16 / RPI; ++i) {
+#pragma unroll
+          for (int o = LPR / 2; o > 0; o >>= 1) part[i] += __shfl_xor_sync(0xffffffffu, part[i], o);
+          const int r = warp * 16 + i * RPI + lane / LPR;
+          if (lane % LPR == 0) {
+            s_delta[(uc & 1) * 256 + r] = part[i];
+            if (u.q0 + r < a.s_q) a.delta[stat + u.q0 + r] = part[i];
+          }
+        }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&bars->delta_ready);
+        // (completes once a unit; no warp can be a unit ahead of another)
+        if (!warp_wait(&bars->delta_ready, uc & 1, 20, abort_flag)) {
+          ok = false;
+          break;
+        }
+      }
+      float delta = u.n != 1 ? s_delta[(uc & 1) * 256 + row] : 0.0f;
+      const float neg_lse2 = q_row < a.s_q ? -lse2_of(__ldg(a.lse + stat + q_row)) : -INFINITY;
+      for (int j = 0; j < u.n; ++j, ++step) {
+        const int key0 = j * 128;
+        const uint32_t mb = masked ? mask_bytes(a, u.b, key0, u.len, lane) : 0u;
+        const uint32_t s_tmem = tmem + (step & 1) * 128 + wg * 64 + lane_off;
+        // S of this parity again only after this tile's dS has been read
+        if (!warp_wait<true>(&bars->s_full[step & 1], (step >> 1) & 1, 21, abort_flag)) {
+          ok = false;
+          break;
+        }
+        tc_fence_after();
+        uint32_t w[4];
+        keep_words(masked, mb, u.len - key0, w);
+        const uint32_t w0 = wg ? w[2] : w[0], w1 = wg ? w[3] : w[1];
+        uint32_t s[64], d[64];
+        tmem_ld32p(s_tmem, s);
+        tmem_ld32p(s_tmem + 32, s + 32);
+        tmem_wait_fence<2>(s);
+#pragma unroll
+        for (int e = 0; e < 64; e += 2) {
+          const float2 t = fma2(make_float2(__uint_as_float(s[e]), __uint_as_float(s[e + 1])),
+                                make_float2(args.scale_log2, args.scale_log2), make_float2(neg_lse2, neg_lse2));
+          s[e] = __float_as_uint(ex2(t.x));
+          s[e + 1] = __float_as_uint(ex2(t.y));
+        }
+        if (!warp_wait<true>(&bars->dp_full, step & 1, 22, abort_flag)) {
+          ok = false;
+          break;
+        }
+        tc_fence_after();
+        tmem_ld32p(tmem + DP_COL + wg * 64 + lane_off, d);
+        tmem_ld32p(tmem + DP_COL + wg * 64 + lane_off + 32, d + 32);
+        tmem_wait_fence<2>(d);
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&bars->dp_free);
+        if ((w0 & w1) != 0xffffffffu) {  // left-out keys: no weight, whatever they hold
+#pragma unroll
+          for (int e = 0; e < 64; ++e)
+            if (((e < 32 ? w0 : w1) & (1u << (e & 31))) == 0) s[e] = d[e] = 0u;
+        }
+        if (u.n == 1) {
+          // One tile holds all keys: delta = sum_j P_j dP_j, both halves
+          float2 acc[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+#pragma unroll
+          for (int e = 0; e < 64; e += 2)
+            acc[(e >> 1) & 1] = fma2(make_float2(__uint_as_float(s[e]), __uint_as_float(s[e + 1])),
+                                     make_float2(__uint_as_float(d[e]), __uint_as_float(d[e + 1])), acc[(e >> 1) & 1]);
+          const float2 t = add2(acc[0], acc[1]);
+          float* part = s_delta + (uc & 1) * 256;
+          part[wg * 128 + row] = t.x + t.y;
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&bars->delta_ready);
+          if (!warp_wait(&bars->delta_ready, uc & 1, 24, abort_flag)) {
+            ok = false;
+            break;
+          }
+          delta = part[row] + part[128 + row];
+          if (wg == 0 && q_row < a.s_q) a.delta[stat + q_row] = delta;
+        }
+        const float2 nd = make_float2(-delta, -delta);
+#pragma unroll
+        for (int e = 0; e < 64; e += 2) {
+          float2 t = add2(make_float2(__uint_as_float(d[e]), __uint_as_float(d[e + 1])), nd);
+          t = mul2(t, make_float2(__uint_as_float(s[e]), __uint_as_float(s[e + 1])));
+          d[e] = __float_as_uint(t.x);
+          d[e + 1] = __float_as_uint(t.y);
+        }
+#pragma unroll
+        for (int e = 0; e < 32; ++e)
+          d[e] = pack16x2<F16>(__uint_as_float(d[2 * e]), __uint_as_float(d[2 * e + 1]));
+        tmem_st32(s_tmem, *reinterpret_cast<uint32_t(*)[32]>(d));
+        tc_wait_st();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&bars->ds_half[step & 1][wg]);
+      }
+      if (!ok) break;
+      // ---- dQ: this warpgroup's D / 2 columns
+      if (u.n > 0) {
+        if (!warp_wait(&bars->dq_full, qc & 1, 23, abort_flag)) {
+          ok = false;
+          break;
+        }
+        ++qc;
+        tc_fence_after();
+      }
+      uint16_t* out = static_cast<uint16_t*>(a.dq) +
+                      ((static_cast<int64_t>(u.b) * a.s_q + q_row) * a.heads + u.head) * D + wg * (D / 2);
+#pragma unroll
+      for (int c = 0; c < D / 64; ++c) {
+        uint32_t r[32];
+        if (u.n > 0) {
+          tmem_ld32p(tmem + DQ_COL + wg * (D / 2) + c * 32 + lane_off, r);
+          tmem_wait_fence<1>(r);
+        } else {
+#pragma unroll
+          for (int e = 0; e < 32; ++e) r[e] = 0u;
+        }
+        if (q_row < a.s_q) {
+#pragma unroll
+          for (int e = 0; e < 32; e += 16) {
+            uint32_t v[8];
+#pragma unroll
+            for (int t = 0; t < 8; ++t)
+              v[t] = pack16x2<F16>(__uint_as_float(r[e + 2 * t]) * a.scale, __uint_as_float(r[e + 2 * t + 1]) * a.scale);
+            st_global_v8(out + c * 32 + e, v);
+          }
+        }
+      }
+      tc_fence_before();
+    }
+  }
+
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 9) {
+    tc_fence_after();
+    tmem_dealloc(tmem, 512);
+  }
+}
+
+// ============================================================== dK and dV
+// TMEM lanes are keys: S^T | dP^T | dV | dK.  P^T goes over S^T, dS^T over
+// dP^T.  Issue order a tile: dV += P^T(j) dO(j), S^T(j+1); dK += dS^T(j) Q(j), dP^T(j+1).
+constexpr int RST = 5;    // ring of Q and dO tiles, by turns
+constexpr int STATS = 2;  // ring of the rows' lse and delta
+
+struct __align__(8) DkvBars {
+  uint64_t r_full[RST], r_free[RST];
+  uint64_t k_full, v_full, k_free, v_free;
+  uint64_t stat_full[STATS], stat_free[STATS];
+  uint64_t s_full, dp_full;
+  uint64_t p_half[2], ds_half[2];
+  uint64_t out_full;
+  uint64_t drain;
+  uint32_t tmem_base;
+  int abort_flag;
+};
+
+template <int D>
+constexpr size_t dkv_smem() {
+  return (RST + 2) * Cfg<D>::TILE_BYTES + STATS * 2 * 128 * sizeof(float) + sizeof(DkvBars);
+}
+
+static_assert(dkv_smem<128>() <= 232448, "shared memory of a CTA");
+
+struct DkvUnit {
+  int b, kvh, key0, split, len;
+  int t0, n;  // first (head of the group, query tile), tiles
+};
+H3B_DEV DkvUnit dkv_unit(const GradArgs& args, int u) {
+  DkvUnit x;
+  x.key0 = (u % args.k_tiles) * 128;  // fastest: units that run together share Q and dO in L2
+  u /= args.k_tiles;
+  x.split = u % args.a.splits;
+  u /= args.a.splits;
+  x.kvh = u % args.a.kv_heads;
+  x.b = u / args.a.kv_heads;
+  x.len = len_of(args.a, x.b);
+  const int all = args.group * args.q_tiles;
+  const int per = (all + args.a.splits - 1) / args.a.splits;
+  x.t0 = x.split * per;
+  x.n = x.key0 < x.len ? max(0, min(all, x.t0 + per) - x.t0) : 0;
+  return x;
+}
+
+template <int D, bool F16>
+__global__ void __launch_bounds__(THREADS, 1)
+    xattn_dkv_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_do,
+                     const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v,
+                     const __grid_constant__ GradArgs args) {
+  using C = Cfg<D>;
+  constexpr uint32_t IDESC_S = F16 ? idesc_f16_f32(128, 128, 0, 0) : idesc_bf16_f32(128, 128, 0, 0);
+  constexpr uint32_t IDESC_G = F16 ? idesc_f16_f32(128, D, 0, 1) : idesc_bf16_f32(128, D, 0, 1);
+  constexpr float P_SHIFT = F16 ? 8.0f : 0.0f;             // P held times 2^P_SHIFT
+  constexpr float P_UNIT = F16 ? 0.00390625f : 1.0f;       // 2^-P_SHIFT
+  extern __shared__ __align__(1024) uint8_t smem_tiles[];
+  uint8_t* smem = smem_tiles;
+  if (misaligned(smem)) return;
+  uint8_t* sR = smem;
+  uint8_t* sK = sR + RST * C::TILE_BYTES;
+  uint8_t* sV = sK + C::TILE_BYTES;
+  float* s_stat = reinterpret_cast<float*>(sV + C::TILE_BYTES);  // [STATS][shift - lse2 | delta scaled][128]
+  DkvBars* bars = reinterpret_cast<DkvBars*>(s_stat + STATS * 2 * 128);
+  const XAttnGrad& a = args.a;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  volatile int* abort_flag = &bars->abort_flag;
+
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < RST; ++i) mbar_init(&bars->r_full[i], 1), mbar_init(&bars->r_free[i], 1);
+    for (int i = 0; i < STATS; ++i) mbar_init(&bars->stat_full[i], 1), mbar_init(&bars->stat_free[i], 8);
+    mbar_init(&bars->k_full, 1);
+    mbar_init(&bars->v_full, 1);
+    mbar_init(&bars->k_free, 1);
+    mbar_init(&bars->v_free, 1);
+    mbar_init(&bars->s_full, 1);
+    mbar_init(&bars->dp_full, 1);
+    for (int i = 0; i < 2; ++i) mbar_init(&bars->p_half[i], 4), mbar_init(&bars->ds_half[i], 4);
+    mbar_init(&bars->out_full, 1);
+    mbar_init(&bars->drain, 1);
+    bars->abort_flag = 0;
+    fence_barrier_init();
+  }
+  if (warp == 9) {
+    tmem_alloc(&bars->tmem_base, 512);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = bars->tmem_base;
+  constexpr uint32_t DP_COL = 128, DV_COL = 256, DK_COL = 384;
+
+  if (warp >= 8) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(REGS_CONTROL));
+    if (warp == 8 && lane == 0) {
+      // ---------------------------------------------------------- TMA
+      prefetch_tmap(&tm_q);
+      prefetch_tmap(&tm_do);
+      prefetch_tmap(&tm_k);
+      prefetch_tmap(&tm_v);
+      int rc = 0, uc = 0;
+      bool ok = true;
+      auto tile = [&](const CUtensorMap* tm, uint8_t* dst, uint64_t* full, int row, int head, int b) {
+        mbar_arrive_expect_tx(full, C::TILE_BYTES);
+        for (int h = 0; h < C::HALVES; ++h) tma_load_4d(dst + h * C::HALF_BYTES, tm, h * 64, row, head, b, full);
+      };
+      auto load_r = [&](const CUtensorMap* tm, int row, int head, int b) {
+        const int s = rc % RST;
+        if (rc >= RST && !mbar_wait(&bars->r_free[s], (rc / RST - 1) & 1, &g_status, 1, abort_flag)) return false;
+        tile(tm, sR + s * C::TILE_BYTES, &bars->r_full[s], row, head, b);
+        ++rc;
+        return true;
+      };
+      for (int x = blockIdx.x; x < args.units && ok; x += gridDim.x) {
+        const DkvUnit u = dkv_unit(args, x);
+        if (u.n == 0) continue;
+        // K and V are held for the unit; the unit before releases them (one
+        // phase a unit)
+        if (uc > 0 && !mbar_wait(&bars->k_free, (uc - 1) & 1, &g_status, 2, abort_flag)) ok = false;
+        if (ok) tile(&tm_k, sK, &bars->k_full, u.key0, u.kvh, u.b);
+        for (int i = 0; i < u.n && ok; ++i) {
+          const int head = u.kvh * args.group + (u.t0 + i) / args.q_tiles;
+          const int q0 = ((u.t0 + i) % args.q_tiles) * 128;
+          ok = load_r(&tm_q, q0, head, u.b);
+          if (ok && i == 0) {
+            if (uc > 0 && !mbar_wait(&bars->v_free, (uc - 1) & 1, &g_status, 3, abort_flag)) ok = false;
+            if (ok) {
+              tile(&tm_v, sV, &bars->v_full, u.key0, u.kvh, u.b);
+              ++uc;
+            }
+          }
+          ok = ok && load_r(&tm_do, q0, head, u.b);
+        }
+      }
+      if (!ok || *abort_flag) {
+        for (int c = max(0, rc - RST); c < rc; ++c)
+          mbar_wait(&bars->r_full[c % RST], (c / RST) & 1, &g_status, 10, nullptr);
+        if (uc > 0) {
+          mbar_wait(&bars->k_full, (uc - 1) & 1, &g_status, 11, nullptr);
+          mbar_wait(&bars->v_full, (uc - 1) & 1, &g_status, 12, nullptr);
+        }
+      }
+    } else if (warp == 9) {
+      // ---------------------------------------------------------- MMA
+      bool ok = true;
+      int step = 0, uc = 0;
+      auto commit = [&](uint64_t* bar) {
+        if (elect_one()) tc_commit(bar);
+        __syncwarp();
+      };
+      auto wait = [&](uint64_t* bar, uint32_t parity, int site) {
+        if (!warp_wait<true>(bar, parity, site, abort_flag)) return false;
+        tc_fence_after();
+        return true;
+      };
+      auto ring = [&](int c) { return smem_u32(sR + (c % RST) * C::TILE_BYTES); };
+      auto issue_s = [&](int t) -> bool {  // S^T(t) = K Q^T
+        if (!wait(&bars->r_full[(2 * t) % RST], (2 * t / RST) & 1, 4)) return false;
+        if (elect_one()) {
+          issue_ss<D>(tmem, smem_u32(sK), ring(2 * t), IDESC_S);
+          tc_commit(&bars->s_full);
+        }
+        __syncwarp();
+        return true;
+      };
+      auto issue_dp = [&](int t) -> bool {  // dP^T(t) = V dO^T
+        if (!wait(&bars->r_full[(2 * t + 1) % RST], ((2 * t + 1) / RST) & 1, 5)) return false;
+        if (elect_one()) {
+          issue_ss<D>(tmem + DP_COL, smem_u32(sV), ring(2 * t + 1), IDESC_S);
+          tc_commit(&bars->dp_full);
+        }
+        __syncwarp();
+        return true;
+      };
+      for (int x = blockIdx.x; x < args.units && ok; x += gridDim.x) {
+        const DkvUnit u = dkv_unit(args, x);
+        if (u.n == 0) continue;
+        ok = wait(&bars->k_full, uc & 1, 6) && issue_s(step) && wait(&bars->v_full, uc & 1, 7) && issue_dp(step);
+        for (int i = 0; i < u.n && ok; ++i, ++step) {
+          const bool last = i == u.n - 1;
+          for (int h = 0; h < 2 && ok; ++h) {  // dV += P^T dO
+            ok = wait(&bars->p_half[h], step & 1, 8);
+            if (ok && elect_one())
+              issue_ts_half<D>(tmem + DV_COL, tmem + h * 64, ring(2 * step + 1), h, IDESC_G, i == 0 && h == 0);
+            __syncwarp();
+          }
+          if (!ok) break;
+          commit(&bars->r_free[(2 * step + 1) % RST]);
+          if (last) {
+            commit(&bars->k_free);  // every S^T of the unit is behind this
+          } else {
+            ok = issue_s(step + 1);
+          }
+          for (int h = 0; h < 2 && ok; ++h) {  // dK += dS^T Q
+            ok = wait(&bars->ds_half[h], step & 1, 9);
+            if (ok && elect_one())
+              issue_ts_half<D>(tmem + DK_COL, tmem + DP_COL + h * 64, ring(2 * step), h, IDESC_G, i == 0 && h == 0);
+            __syncwarp();
+          }
+          if (!ok) break;
+          commit(&bars->r_free[(2 * step) % RST]);
+          if (last) {
+            commit(&bars->v_free);
+            commit(&bars->out_full);
+          } else {
+            ok = issue_dp(step + 1);
+          }
+        }
+        ++uc;
+      }
+      commit(&bars->drain);
+      warp_wait(&bars->drain, 0, 13, nullptr);
+    } else if (warp == 10) {
+      // ---------------------------------------------------------- row statistics
+      int step = 0;
+      bool ok = true;
+      for (int x = blockIdx.x; x < args.units && ok; x += gridDim.x) {
+        const DkvUnit u = dkv_unit(args, x);
+        for (int i = 0; i < u.n; ++i, ++step) {
+          const int head = u.kvh * args.group + (u.t0 + i) / args.q_tiles;
+          const int q0 = ((u.t0 + i) % args.q_tiles) * 128;
+          const int64_t at = (static_cast<int64_t>(u.b) * a.heads + head) * a.s_q;
+          float lse[4], del[4];
+#pragma unroll
+          for (int c = 0; c < 4; ++c) {
+            const int r = q0 + c * 32 + lane;
+            const bool in = r < a.s_q;
+            lse[c] = in ? P_SHIFT - lse2_of(__ldg(a.lse + at + r)) : -INFINITY;
+            del[c] = in ? -a.delta[at + r] * P_UNIT : 0.0f;
+          }
+          const int s = step % STATS;
+          if (step >= STATS && !warp_wait(&bars->stat_free[s], (step / STATS - 1) & 1, 14, abort_flag)) {
+            ok = false;
+            break;
+          }
+#pragma unroll
+          for (int c = 0; c < 4; ++c) {
+            s_stat[s * 256 + c * 32 + lane] = lse[c];
+            s_stat[s * 256 + 128 + c * 32 + lane] = del[c];
+          }
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&bars->stat_full[s]);
+        }
+      }
+    }
+  } else {
+    // ------------------------------------------------------------ compute
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(REGS_COMPUTE));
+    const int wg = warp >> 2;
+    const int row = (warp & 3) * 32 + lane;
+    const uint32_t lane_off = static_cast<uint32_t>((warp & 3) * 32) << 16;
+    const uint32_t s_tmem = tmem + wg * 64 + lane_off;
+    const uint32_t dp_tmem = tmem + DP_COL + wg * 64 + lane_off;
+    uint32_t step = 0, oc = 0;
+    bool ok = true;
+    for (int x = blockIdx.x; x < args.units && ok; x += gridDim.x) {
+      const DkvUnit u = dkv_unit(args, x);
+      const int key = u.key0 + row;
+      const bool kept = key < u.len && (a.key_mask == nullptr || __ldg(a.key_mask + u.b * a.mask_stride + key) != 0);
+      for (int i = 0; i < u.n; ++i, ++step) {
+        const int slot = step % STATS;
+        const float4* lse = reinterpret_cast<const float4*>(s_stat + slot * 256 + wg * 64);
+        const float4* del = reinterpret_cast<const float4*>(s_stat + slot * 256 + 128 + wg * 64);
+        if (!warp_wait(&bars->stat_full[slot], (step / STATS) & 1, 20, abort_flag) ||
+            !warp_wait<true>(&bars->s_full, step & 1, 21, abort_flag)) {
+          ok = false;
+          break;
+        }
+        tc_fence_after();
+        uint32_t s[64], d[64];
+        tmem_ld32p(s_tmem, s);
+        tmem_ld32p(s_tmem + 32, s + 32);
+        tmem_wait_fence<2>(s);
+        const float2 sc = make_float2(args.scale_log2, args.scale_log2);
+#pragma unroll
+        for (int e = 0; e < 64; e += 4) {
+          const float4 l = lse[e / 4];
+          const float2 t0 = fma2(make_float2(__uint_as_float(s[e]), __uint_as_float(s[e + 1])), sc, make_float2(l.x, l.y));
+          const float2 t1 = fma2(make_float2(__uint_as_float(s[e + 2]), __uint_as_float(s[e + 3])), sc, make_float2(l.z, l.w));
+          s[e] = __float_as_uint(kept ? ex2(t0.x) : 0.0f);
+          s[e + 1] = __float_as_uint(kept ? ex2(t0.y) : 0.0f);
+          s[e + 2] = __float_as_uint(kept ? ex2(t1.x) : 0.0f);
+          s[e + 3] = __float_as_uint(kept ? ex2(t1.y) : 0.0f);
+        }
+#pragma unroll
+        for (int e = 0; e < 32; ++e) d[e] = pack16x2<F16>(__uint_as_float(s[2 * e]), __uint_as_float(s[2 * e + 1]));
+        tmem_st32(s_tmem, *reinterpret_cast<uint32_t(*)[32]>(d));
+        tc_wait_st();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&bars->p_half[wg]);
+        if (!warp_wait<true>(&bars->dp_full, step & 1, 22, abort_flag)) {
+          ok = false;
+          break;
+        }
+        tc_fence_after();
+        tmem_ld32p(dp_tmem, d);
+        tmem_ld32p(dp_tmem + 32, d + 32);
+        tmem_wait_fence<2>(d);
+        const float2 pu = make_float2(P_UNIT, P_UNIT);
+#pragma unroll
+        for (int e = 0; e < 64; e += 4) {
+          const float4 l = del[e / 4];
+          float2 t0 = make_float2(__uint_as_float(d[e]), __uint_as_float(d[e + 1]));
+          float2 t1 = make_float2(__uint_as_float(d[e + 2]), __uint_as_float(d[e + 3]));
+          if constexpr (F16) {
+            t0 = fma2(t0, pu, make_float2(l.x, l.y));
+            t1 = fma2(t1, pu, make_float2(l.z, l.w));
+          } else {
+            t0 = add2(t0, make_float2(l.x, l.y));
+            t1 = add2(t1, make_float2(l.z, l.w));
+          }
+          t0 = mul2(t0, make_float2(__uint_as_float(s[e]), __uint_as_float(s[e + 1])));
+          t1 = mul2(t1, make_float2(__uint_as_float(s[e + 2]), __uint_as_float(s[e + 3])));
+          d[e / 2] = kept ? pack16x2<F16>(t0.x, t0.y) : 0u;
+          d[e / 2 + 1] = kept ? pack16x2<F16>(t1.x, t1.y) : 0u;
+        }
+        tmem_st32(dp_tmem, *reinterpret_cast<uint32_t(*)[32]>(d));
+        tc_wait_st();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) {
+          mbar_arrive(&bars->ds_half[wg]);
+          mbar_arrive(&bars->stat_free[slot]);
+        }
+      }
+      if (!ok) break;
+      // ---- warpgroup 0 writes dV, warpgroup 1 dK
+      if (u.n > 0) {
+        if (!warp_wait(&bars->out_full, oc & 1, 23, abort_flag)) {
+          ok = false;
+          break;
+        }
+        ++oc;
+        tc_fence_after();
+      }
+      const float f = wg ? a.scale : P_UNIT;
+      const int64_t key_row = (static_cast<int64_t>(u.b) * a.s_kv + key) * a.kv_heads + u.kvh;
+      const int64_t per_split = static_cast<int64_t>(a.batch) * a.s_kv * a.kv_heads;
+#pragma unroll
+      for (int c = 0; c < D / 32; ++c) {
+        uint32_t r[32];
+        if (u.n > 0) {
+          tmem_ld32p(tmem + (wg ? DK_COL : DV_COL) + c * 32 + lane_off, r);
+          tmem_wait_fence<1>(r);
+        } else {
+#pragma unroll
+          for (int e = 0; e < 32; ++e) r[e] = 0u;
+        }
+        if (key >= a.s_kv) continue;
+        if (a.splits > 1) {
+          float* dst = a.part + ((wg * static_cast<int64_t>(a.splits) + u.split) * per_split + key_row) * D + c * 32;
+#pragma unroll
+          for (int e = 0; e < 32; e += 8) {
+            uint32_t v[8];
+#pragma unroll
+            for (int t = 0; t < 8; ++t) v[t] = __float_as_uint(__uint_as_float(r[e + t]) * f);
+            st_global_v8(dst + e, v);
+          }
+        } else {
+          uint16_t* dst = static_cast<uint16_t*>(wg ? a.dk : a.dv) + key_row * D + c * 32;
+#pragma unroll
+          for (int e = 0; e < 32; e += 16) {
+            uint32_t v[8];
+#pragma unroll
+            for (int t = 0; t < 8; ++t)
+              v[t] = pack16x2<F16>(__uint_as_float(r[e + 2 * t]) * f, __uint_as_float(r[e + 2 * t + 1]) * f);
+            st_global_v8(dst + e, v);
+          }
+        }
+      }
+      tc_fence_before();
+    }
+  }
+
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 9) {
+    tc_fence_after();
+    tmem_dealloc(tmem, 512);
+  }
+}
+
+// dv (blockIdx.y 0) and dk (1): the ranges' fp32 sums added in order, rounded
+// once.  One thread = 8 values.
+template <bool F16>
+__global__ void __launch_bounds__(256) xattn_dkv_join_kernel(const float* part, uint16_t* dv, uint16_t* dk, int splits,
+                                                             int64_t n) {
+  const int64_t i = (static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x) * 8;
+  if (i >= n) return;
+  const float* p = part + blockIdx.y * splits * n + i;
+  float s[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+  for (int k = 0; k < splits; ++k) {
+    const float4 x = *reinterpret_cast<const float4*>(p + k * n), y = *reinterpret_cast<const float4*>(p + k * n + 4);
+    s[0] += x.x, s[1] += x.y, s[2] += x.z, s[3] += x.w;
+    s[4] += y.x, s[5] += y.y, s[6] += y.z, s[7] += y.w;
+  }
+  *reinterpret_cast<uint4*>((blockIdx.y ? dk : dv) + i) =
+      make_uint4(pack16x2<F16>(s[0], s[1]), pack16x2<F16>(s[2], s[3]), pack16x2<F16>(s[4], s[5]), pack16x2<F16>(s[6], s[7]));
+}
+
+int encode_tiles(CUtensorMap* m, const void* p, bool f16, int d, const int64_t (&st)[3], int seq, int heads, int batch) {
+  const uint64_t dims[4] = {static_cast<uint64_t>(d), static_cast<uint64_t>(seq > 0 ? seq : 1),
+                            static_cast<uint64_t>(heads), static_cast<uint64_t>(batch)};
+  const uint64_t sb[3] = {static_cast<uint64_t>(st[1]) * 2, static_cast<uint64_t>(st[2]) * 2,
+                          static_cast<uint64_t>(st[0]) * 2};
+  const uint32_t box[4] = {64, 128, 1, 1};
+  return h3b::encode_4d(m, f16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, p, dims, sb, box,
+                        CU_TENSOR_MAP_SWIZZLE_128B);
+}
+
+template <int D, bool F16>
+int launch(const XAttnGrad& a, cudaStream_t stream) {
+  CUtensorMap tq, tdo, tk, tv;
+  int rc = encode_tiles(&tq, a.q, F16, D, a.q_stride, a.s_q, a.heads, a.batch);
+  if (rc == H3B_OK) rc = encode_tiles(&tdo, a.d_o, F16, D, a.do_stride, a.s_q, a.heads, a.batch);
+  if (rc == H3B_OK) rc = encode_tiles(&tk, a.k, F16, D, a.kv_stride, a.s_kv, a.kv_heads, a.batch);
+  if (rc == H3B_OK) rc = encode_tiles(&tv, a.v, F16, D, a.kv_stride, a.s_kv, a.kv_heads, a.batch);
+  if (rc != H3B_OK) return rc;
+  auto dq = xattn_dq_kernel<D, F16>;
+  auto dkv = xattn_dkv_kernel<D, F16>;
+  static bool attr = false;
+  if (!attr) {
+    if (cudaFuncSetAttribute(dq, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(dq_smem<D>())) !=
+            cudaSuccess ||
+        cudaFuncSetAttribute(dkv, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(dkv_smem<D>())) !=
+            cudaSuccess)
+      return H3B_ERR_LAUNCH;
+    attr = true;
+  }
+  GradArgs args{};
+  args.a = a;
+  args.group = a.heads / a.kv_heads;
+  args.q_tiles = (a.s_q + 127) / 128;
+  args.k_tiles = (a.s_kv + 127) / 128;
+  args.scale_log2 = a.scale * LOG2E;
+  const int sms = h3b::num_sms();
+  const int64_t qu = static_cast<int64_t>(a.batch) * a.heads * args.q_tiles;
+  const int64_t ku = static_cast<int64_t>(a.batch) * a.kv_heads * args.k_tiles * a.splits;
+  if (qu > 0x3fffffff || ku > 0x3fffffff) return H3B_ERR_SHAPE;
+  args.units = static_cast<int>(qu);
+  dq<<<static_cast<unsigned>(qu < sms ? qu : sms), THREADS, dq_smem<D>(), stream>>>(tq, tdo, tk, tv, args);
+  rc = h3b::launch_status();
+  if (rc != H3B_OK || ku == 0) return rc;
+  args.units = static_cast<int>(ku);
+  dkv<<<static_cast<unsigned>(ku < sms ? ku : sms), THREADS, dkv_smem<D>(), stream>>>(tq, tdo, tk, tv, args);
+  rc = h3b::launch_status();
+  if (rc != H3B_OK || a.splits == 1) return rc;
+  const int64_t n = static_cast<int64_t>(a.batch) * a.s_kv * a.kv_heads * D;
+  const dim3 grid(static_cast<unsigned>((n / 8 + 255) / 256), 2);
+  xattn_dkv_join_kernel<F16><<<grid, 256, 0, stream>>>(a.part, static_cast<uint16_t*>(a.dv),
+                                                       static_cast<uint16_t*>(a.dk), a.splits, n);
+  return h3b::launch_status();
+}
+
+}  // namespace
+
+namespace h3b {
+
+int xattn_bwd_splits(const XAttnGrad& a) {
+  // Ranges of the query tiles: rounds of units over the SMs times the tiles
+  // of a unit, a unit's own start and end counted as three tiles.
+  const int64_t base = static_cast<int64_t>(a.batch) * a.kv_heads * ((a.s_kv + 127) / 128);
+  const int64_t tiles = static_cast<int64_t>(a.heads / a.kv_heads) * ((a.s_q + 127) / 128);
+  const int sms = num_sms();
+  int best = 1;
+  double cost = 1e30;
+  for (int s = 1; s <= 64 && s <= tiles; ++s) {
+    const double c = static_cast<double>((base * s + sms - 1) / sms) *
+                     (static_cast<double>((tiles + s - 1) / s) + 3.0 + (s > 1 ? 1.0 : 0.0));
+    if (c < cost * 0.98) {
+      cost = c;
+      best = s;
+    }
+  }
+  return best;
+}
+
+int xattn_bwd_launch(const XAttnGrad& a, cudaStream_t stream) {
+  if (a.head_dim == 128) return a.dtype == H3B_F16 ? launch<128, true>(a, stream) : launch<128, false>(a, stream);
+  return a.dtype == H3B_F16 ? launch<64, true>(a, stream) : launch<64, false>(a, stream);
+}
+
+}  // namespace h3b

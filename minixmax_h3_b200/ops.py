@@ -494,6 +494,35 @@ def cross_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, kv_len
     return out
 
 
+def cross_attention_bwd(dout: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, out: torch.Tensor,
+                        lse: torch.Tensor, *, kv_lens: Optional[torch.Tensor] = None,
+                        key_mask: Optional[torch.Tensor] = None, scale: Optional[float] = None
+                        ) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """Gradients (dq, dk, dv) of cross_attention for the gradient dout of its
+    result out; lse and the other arguments as the forward call had them.
+    Heads that share a key head add into its dk and dv; left-out keys get
+    zeros.  Sums are fp32 in a fixed order (bit-reproducible)."""
+    _cuda(dout, q, k, v, out, lse, kv_lens, key_mask)
+    _check_qkv("cross_attention_bwd", q, k, v)
+    if out.shape != q.shape or dout.shape != q.shape or out.dtype != q.dtype or dout.dtype != q.dtype:
+        raise ValueError("cross_attention_bwd: out and dout have q's shape and type")
+    b, s_q, heads, d = q.shape
+    s_kv, kv_heads = k.shape[1], k.shape[2]
+    key_mask = _kept_keys("cross_attention_bwd", k, kv_lens, key_mask)
+    _check_lse("cross_attention_bwd", lse, q)
+    q, out, dout = (t if _fits(t) else t.contiguous() for t in (q, out, dout))
+    k, v = _kv_in_place(k, v)
+    dq = torch.empty((b, s_q, heads, d), dtype=q.dtype, device=q.device)
+    dk, dv = (torch.empty((b, s_kv, kv_heads, d), dtype=q.dtype, device=q.device) for _ in range(2))
+    ws = _workspace("h3b_cross_attention_bwd_workspace", q, b, heads, kv_heads, d, s_q, s_kv)
+    call("h3b_cross_attention_bwd", dout.data_ptr(), q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(),
+         lse.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), _FLOAT16[q.dtype], b, heads, kv_heads, d, s_q,
+         s_kv, *dout.stride()[:3], *q.stride()[:3], *k.stride()[:3], *out.stride()[:3], _ptr(kv_lens),
+         _ptr(key_mask), 0 if key_mask is None else key_mask.stride(0), _scale(scale, d), _ptr(ws),
+         0 if ws is None else ws.numel(), _stream(q))
+    return dq, dk, dv
+
+
 # ----------------------------------------------------------------------------- 8-bit key/value cache
 
 _KV8_CODES = {torch.int8: 0, torch.float8_e4m3fn: 1}
