@@ -19,7 +19,9 @@ EPI_STORE, EPI_GELU, EPI_GATE_RES, EPI_SWIGLU, EPI_STORE_POSMAX = 0, 1, 2, 3, 4
 
 
 def _stream(t: torch.Tensor) -> int:
-    return torch.cuda.current_stream(t.device).cuda_stream
+    # The raw handle of the current stream: 0.15 us against 2.3 us for a
+    # torch.cuda.Stream object, on calls of 5 to 10 us.
+    return torch._C._cuda_getCurrentRawStream(t.get_device())
 
 
 def _ptr(t: Optional[torch.Tensor]) -> Optional[int]:
@@ -396,19 +398,26 @@ def _fits(t: torch.Tensor) -> bool:
     return True
 
 
-def _check_qkv(name: str, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor) -> None:
-    if q.dtype not in _FLOAT16 or k.dtype != q.dtype or v.dtype != q.dtype:
+def _check_qkv(name: str, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor) -> tuple[int, int, int, int, int, int]:
+    """Checks q [B, Sq, H, D] and k, v [B, Skv, Hkv, D]; returns (B, H, Hkv,
+    D, Sq, Skv), the sizes as the C ABI takes them."""
+    dtype = q.dtype
+    if dtype not in _FLOAT16 or k.dtype != dtype or v.dtype != dtype:
         raise TypeError(f"{name} expects q, k and v of one type, bf16 or fp16")
-    if q.dim() != 4 or k.dim() != 4 or k.shape != v.shape or k.shape[0] != q.shape[0] or k.shape[3] != q.shape[3]:
+    qs, ks = q.shape, k.shape
+    if len(qs) != 4 or len(ks) != 4 or ks != v.shape or ks[0] != qs[0] or ks[3] != qs[3]:
         raise ValueError(f"{name} expects q [B, Sq, H, D], k and v [B, Skv, Hkv, D]")
-    if q.shape[3] not in (64, 128):
-        raise ValueError(f"{name}: head dim {q.shape[3]}: the kernels are built for 64 and 128")
-    if k.shape[2] == 0 or q.shape[2] % k.shape[2]:
-        raise ValueError(f"{name}: {q.shape[2]} query heads cannot share {k.shape[2]} key heads")
+    b, s_q, heads, d = qs
+    _, s_kv, kv_heads, _ = ks
+    if d not in (64, 128):
+        raise ValueError(f"{name}: head dim {d}: the kernels are built for 64 and 128")
+    if kv_heads == 0 or heads % kv_heads:
+        raise ValueError(f"{name}: {heads} query heads cannot share {kv_heads} key heads")
+    return b, heads, kv_heads, d, s_q, s_kv
 
 
 def _kv_in_place(k: torch.Tensor, v: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
-    if not (_fits(k) and _fits(v) and k.stride() == v.stride()):
+    if k.stride() != v.stride() or v.data_ptr() & 15 or not _fits(k):
         k, v = k.contiguous(), v.contiguous()
     return k, v
 
@@ -442,8 +451,8 @@ def _workspace_bytes(fn: str, device: int, *sizes: int) -> int:
 
 
 def _workspace(fn: str, t: torch.Tensor, *sizes: int) -> Optional[torch.Tensor]:
-    n = _workspace_bytes(fn, t.device.index, *sizes)
-    return torch.empty((n,), dtype=torch.uint8, device=t.device) if n else None
+    n = _workspace_bytes(fn, t.get_device(), *sizes)
+    return t.new_empty(n, dtype=torch.uint8) if n else None
 
 
 def _check_lse(name: str, lse: Optional[torch.Tensor], q: torch.Tensor) -> None:
@@ -454,7 +463,7 @@ def _check_lse(name: str, lse: Optional[torch.Tensor], q: torch.Tensor) -> None:
 
 def _check_out(name: str, out: Optional[torch.Tensor], q: torch.Tensor) -> torch.Tensor:
     if out is None:
-        return torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        return torch.empty_like(q, memory_format=torch.contiguous_format)
     if out.shape != q.shape or out.dtype != q.dtype or not _fits(out):
         raise ValueError(f"{name}: out has q's shape and type, unit last stride, strides of multiples of 8 and "
                          "16-byte alignment")
@@ -477,20 +486,18 @@ def cross_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, kv_len
     layouts are copied first.  For gradients by autograd see
     ``attention.cross_attention``."""
     _cuda(q, k, v, kv_lens, key_mask, out, lse)
-    _check_qkv("cross_attention", q, k, v)
-    b, s_q, heads, d = q.shape
-    s_kv, kv_heads = k.shape[1], k.shape[2]
+    sizes = _check_qkv("cross_attention", q, k, v)
     key_mask = _kept_keys("cross_attention", k, kv_lens, key_mask)
     _check_lse("cross_attention", lse, q)
     out = _check_out("cross_attention", out, q)
     if not _fits(q):
         q = q.contiguous()
     k, v = _kv_in_place(k, v)
-    ws = _workspace("h3b_cross_attention_workspace", q, b, heads, kv_heads, d, s_q, s_kv)
+    ws = _workspace("h3b_cross_attention_workspace", q, *sizes)
     call("h3b_cross_attention_fwd", q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), _ptr(lse),
-         _FLOAT16[q.dtype], b, heads, kv_heads, d, s_q, s_kv, *q.stride()[:3], *k.stride()[:3], *out.stride()[:3],
-         _ptr(kv_lens), _ptr(key_mask), 0 if key_mask is None else key_mask.stride(0), _scale(scale, d), _ptr(ws),
-         0 if ws is None else ws.numel(), _stream(q))
+         _FLOAT16[q.dtype], *sizes, *q.stride()[:3], *k.stride()[:3], *out.stride()[:3],
+         _ptr(kv_lens), _ptr(key_mask), 0 if key_mask is None else key_mask.stride(0), _scale(scale, sizes[3]),
+         _ptr(ws), 0 if ws is None else ws.numel(), _stream(q))
     return out
 
 
@@ -503,22 +510,19 @@ def cross_attention_bwd(dout: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v:
     Heads that share a key head add into its dk and dv; left-out keys get
     zeros.  Sums are fp32 in a fixed order (bit-reproducible)."""
     _cuda(dout, q, k, v, out, lse, kv_lens, key_mask)
-    _check_qkv("cross_attention_bwd", q, k, v)
+    sizes = _check_qkv("cross_attention_bwd", q, k, v)
     if out.shape != q.shape or dout.shape != q.shape or out.dtype != q.dtype or dout.dtype != q.dtype:
         raise ValueError("cross_attention_bwd: out and dout have q's shape and type")
-    b, s_q, heads, d = q.shape
-    s_kv, kv_heads = k.shape[1], k.shape[2]
     key_mask = _kept_keys("cross_attention_bwd", k, kv_lens, key_mask)
     _check_lse("cross_attention_bwd", lse, q)
     q, out, dout = (t if _fits(t) else t.contiguous() for t in (q, out, dout))
     k, v = _kv_in_place(k, v)
-    dq = torch.empty((b, s_q, heads, d), dtype=q.dtype, device=q.device)
-    dk, dv = (torch.empty((b, s_kv, kv_heads, d), dtype=q.dtype, device=q.device) for _ in range(2))
-    ws = _workspace("h3b_cross_attention_bwd_workspace", q, b, heads, kv_heads, d, s_q, s_kv)
+    dq, dk, dv = (torch.empty_like(t, memory_format=torch.contiguous_format) for t in (q, k, v))
+    ws = _workspace("h3b_cross_attention_bwd_workspace", q, *sizes)
     call("h3b_cross_attention_bwd", dout.data_ptr(), q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(),
-         lse.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), _FLOAT16[q.dtype], b, heads, kv_heads, d, s_q,
-         s_kv, *dout.stride()[:3], *q.stride()[:3], *k.stride()[:3], *out.stride()[:3], _ptr(kv_lens),
-         _ptr(key_mask), 0 if key_mask is None else key_mask.stride(0), _scale(scale, d), _ptr(ws),
+         lse.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), _FLOAT16[q.dtype], *sizes,
+         *dout.stride()[:3], *q.stride()[:3], *k.stride()[:3], *out.stride()[:3], _ptr(kv_lens), _ptr(key_mask),
+         0 if key_mask is None else key_mask.stride(0), _scale(scale, sizes[3]), _ptr(ws),
          0 if ws is None else ws.numel(), _stream(q))
     return dq, dk, dv
 
@@ -563,7 +567,8 @@ def _check_cache(name: str, c: KV8Cache, table: torch.Tensor, lens: torch.Tensor
     k, v, ks, vs = c.k, c.v, c.k_scale, c.v_scale
     if k.dtype not in _KV8_CODES or v.dtype != k.dtype or ks.dtype != torch.float32 or vs.dtype != torch.float32:
         raise TypeError(f"{name}: the cache holds int8 or float8_e4m3fn codes and fp32 scales")
-    if k.dim() != 4 or v.shape != k.shape or ks.shape != k.shape[:2] or vs.shape != k.shape[:2]:
+    shape = k.shape
+    if len(shape) != 4 or v.shape != shape or ks.shape != shape[:2] or vs.shape != ks.shape:
         raise ValueError(f"{name}: codes [num_blocks, Hkv, block_tokens, D], scales [num_blocks, Hkv]")
     if not (k.is_contiguous() and v.is_contiguous() and ks.is_contiguous() and vs.is_contiguous()):
         raise ValueError(f"{name}: the cache's tensors are contiguous")
@@ -606,7 +611,8 @@ def kv8_read(cache: KV8Cache, block_table: torch.Tensor, lens: torch.Tensor, max
     codes = {**_FLOAT16, torch.float32: 2}
     if dtype not in codes:
         raise TypeError("kv8_read writes bf16, fp16 or fp32")
-    k, v = (torch.empty((lens.shape[0], max_len, kv_heads, d), dtype=dtype, device=cache.k.device) for _ in range(2))
+    shape = (lens.shape[0], max_len, kv_heads, d)
+    k, v = cache.k_scale.new_empty(shape, dtype=dtype), cache.k_scale.new_empty(shape, dtype=dtype)
     call("h3b_kv8_read", cache.k.data_ptr(), cache.v.data_ptr(), cache.k_scale.data_ptr(), cache.v_scale.data_ptr(),
          _KV8_CODES[cache.k.dtype], nb, kv_heads, bt, d, block_table.data_ptr(), block_table.shape[1],
          lens.data_ptr(), lens.shape[0], max_len, k.data_ptr(), v.data_ptr(), codes[dtype], _stream(cache.k))
