@@ -118,11 +118,31 @@ H3B_DEV bool mbar_try_wait_cluster(uint32_t bar_addr, uint32_t parity) {
   return ok != 0;
 }
 
+// Out-of-line part of a compact wait: `t0` 0 starts the clock; returns 0 when
+// the wait is to be given up (budget spent, reported; or another warp of the
+// CTA has given up), else the start time.
+static __device__ __noinline__ uint64_t mbar_overdue(uint64_t t0, H3bDeviceStatus* st, int site, int parity,
+                                                     volatile int* abort_flag) {
+  if (abort_flag != nullptr && *abort_flag) return 0;
+  const uint64_t now = globaltimer_ns();
+  if (t0 == 0) return now;
+  if (now - t0 <= H3B_WAIT_NS) return t0;
+  if (atomicCAS(&st->code, 0, H3B_ERR_DEVICE_TIMEOUT) == 0) {
+    st->site = site;
+    st->info = parity;
+    st->block = static_cast<int>(blockIdx.x);
+  }
+  if (abort_flag != nullptr) *abort_flag = 1;
+  return 0;
+}
+
 // Wait for phase `parity` of `bar` to complete.  Returns false (and records
 // `site` in *st, raising *abort_flag) when the budget runs out or when another
 // warp of the CTA already aborted.  SPIN: poll without a suspend hint;
-// CLUSTER: cluster-scope acquire (polls too).
-template <bool SPIN = false, bool CLUSTER = false>
+// CLUSTER: cluster-scope acquire (polls too).  COMPACT: the clock and the
+// report stay out of line (~1 KB less code a wait, for kernels whose warps
+// run different code from one instruction cache).
+template <bool SPIN = false, bool CLUSTER = false, bool COMPACT = false>
 H3B_DEV bool mbar_wait(uint64_t* bar, uint32_t parity, H3bDeviceStatus* st, int site,
                        volatile int* abort_flag) {
   const uint32_t addr = smem_u32(bar);
@@ -131,11 +151,16 @@ H3B_DEV bool mbar_wait(uint64_t* bar, uint32_t parity, H3bDeviceStatus* st, int 
                    : (SPIN ? mbar_try_wait_spin(addr, parity) : mbar_try_wait(addr, parity));
   };
   if (poll()) return true;
-  const uint64_t t0 = globaltimer_ns();
+  uint64_t t0 = COMPACT ? 0 : globaltimer_ns();
   uint32_t spins = 0;
   while (true) {
     if (poll()) return true;
     if ((++spins & 255u) == 0) {
+      if constexpr (COMPACT) {
+        t0 = mbar_overdue(t0, st, site, static_cast<int>(parity), abort_flag);
+        if (t0 == 0) return false;
+        continue;
+      }
       if (abort_flag != nullptr && *abort_flag) return false;
       if (globaltimer_ns() - t0 > H3B_WAIT_NS) {
         if (atomicCAS(&st->code, 0, H3B_ERR_DEVICE_TIMEOUT) == 0) {

@@ -57,7 +57,7 @@ H3B_DEV float ex2(float x) {
 
 template <bool SPIN = false>
 H3B_DEV bool warp_wait(uint64_t* bar, uint32_t parity, int site, volatile int* abort_flag) {
-  const bool ok = mbar_wait<SPIN>(bar, parity, &g_status, site, abort_flag);
+  const bool ok = mbar_wait<SPIN, false, true>(bar, parity, &g_status, site, abort_flag);
   return __all_sync(0xffffffffu, ok);
 }
 
@@ -235,7 +235,7 @@ __global__ void __launch_bounds__(THREADS, 1)
       auto load = [&](const CUtensorMap* tm, uint8_t* ring, uint64_t* full, uint64_t* free_, int stages, int& c, int row,
                       int head, int b) {
         const int s = c % stages;
-        if (c >= stages && !mbar_wait(&free_[s], (c / stages - 1) & 1, &g_status, 1, abort_flag)) return false;
+        if (c >= stages && !mbar_wait<false, false, true>(&free_[s], (c / stages - 1) & 1, &g_status, 1, abort_flag)) return false;
         mbar_arrive_expect_tx(&full[s], C::TILE_BYTES);
         for (int h = 0; h < C::HALVES; ++h)
           tma_load_4d(ring + s * C::TILE_BYTES + h * C::HALF_BYTES, tm, h * 64, row, head, b, &full[s]);
@@ -254,11 +254,11 @@ __global__ void __launch_bounds__(THREADS, 1)
       }
       if (!ok || *abort_flag) {
         for (int c = max(0, xc - XST); c < xc; ++c)
-          mbar_wait(&bars->x_full[c % XST], (c / XST) & 1, &g_status, 10, nullptr);
+          mbar_wait<false, false, true>(&bars->x_full[c % XST], (c / XST) & 1, &g_status, 10, nullptr);
         for (int c = max(0, kc - KST); c < kc; ++c)
-          mbar_wait(&bars->k_full[c % KST], (c / KST) & 1, &g_status, 11, nullptr);
+          mbar_wait<false, false, true>(&bars->k_full[c % KST], (c / KST) & 1, &g_status, 11, nullptr);
         for (int c = max(0, vc - VST); c < vc; ++c)
-          mbar_wait(&bars->v_full[c % VST], (c / VST) & 1, &g_status, 12, nullptr);
+          mbar_wait<false, false, true>(&bars->v_full[c % VST], (c / VST) & 1, &g_status, 12, nullptr);
       }
     } else if (warp == 9) {
       // ---------------------------------------------------------- MMA
@@ -672,7 +672,7 @@ __global__ void __launch_bounds__(THREADS, 1)
       };
       auto load_r = [&](const CUtensorMap* tm, int row, int head, int b) {
         const int s = rc % RST;
-        if (rc >= RST && !mbar_wait(&bars->r_free[s], (rc / RST - 1) & 1, &g_status, 1, abort_flag)) return false;
+        if (rc >= RST && !mbar_wait<false, false, true>(&bars->r_free[s], (rc / RST - 1) & 1, &g_status, 1, abort_flag)) return false;
         tile(tm, sR + s * C::TILE_BYTES, &bars->r_full[s], row, head, b);
         ++rc;
         return true;
@@ -682,14 +682,14 @@ __global__ void __launch_bounds__(THREADS, 1)
         if (u.n == 0) continue;
         // K and V are held for the unit; the unit before releases them (one
         // phase a unit)
-        if (uc > 0 && !mbar_wait(&bars->k_free, (uc - 1) & 1, &g_status, 2, abort_flag)) ok = false;
+        if (uc > 0 && !mbar_wait<false, false, true>(&bars->k_free, (uc - 1) & 1, &g_status, 2, abort_flag)) ok = false;
         if (ok) tile(&tm_k, sK, &bars->k_full, u.key0, u.kvh, u.b);
         for (int i = 0; i < u.n && ok; ++i) {
           const int head = u.kvh * args.group + (u.t0 + i) / args.q_tiles;
           const int q0 = ((u.t0 + i) % args.q_tiles) * 128;
           ok = load_r(&tm_q, q0, head, u.b);
           if (ok && i == 0) {
-            if (uc > 0 && !mbar_wait(&bars->v_free, (uc - 1) & 1, &g_status, 3, abort_flag)) ok = false;
+            if (uc > 0 && !mbar_wait<false, false, true>(&bars->v_free, (uc - 1) & 1, &g_status, 3, abort_flag)) ok = false;
             if (ok) {
               tile(&tm_v, sV, &bars->v_full, u.key0, u.kvh, u.b);
               ++uc;
@@ -700,10 +700,10 @@ __global__ void __launch_bounds__(THREADS, 1)
       }
       if (!ok || *abort_flag) {
         for (int c = max(0, rc - RST); c < rc; ++c)
-          mbar_wait(&bars->r_full[c % RST], (c / RST) & 1, &g_status, 10, nullptr);
+          mbar_wait<false, false, true>(&bars->r_full[c % RST], (c / RST) & 1, &g_status, 10, nullptr);
         if (uc > 0) {
-          mbar_wait(&bars->k_full, (uc - 1) & 1, &g_status, 11, nullptr);
-          mbar_wait(&bars->v_full, (uc - 1) & 1, &g_status, 12, nullptr);
+          mbar_wait<false, false, true>(&bars->k_full, (uc - 1) & 1, &g_status, 11, nullptr);
+          mbar_wait<false, false, true>(&bars->v_full, (uc - 1) & 1, &g_status, 12, nullptr);
         }
       }
     } else if (warp == 9) {

@@ -11,21 +11,22 @@
 // continuous pipeline of matrix instructions; the next unit's Q and first K
 // are loaded, and its first scores computed, while the last one's softmax and
 // stores are under way.
-//   warps 0-3   softmax and stores of rows 0-127 (thread = row = TMEM lane)
-//   warps 4-7   the same for rows 128-255
+//   warps 0-3   softmax of rows 0-127 (thread = row = TMEM lane)
+//   warps 4-7   softmax of rows 128-255
 //   warp 8      TMA: Q through a ring of 3 tiles, K and V through one of 4
 //   warp 9      TMEM allocation and matrix instructions
-//   warps 10-11 idle (complete the third warpgroup for setmaxnreg)
+//   warp 10     zeroes the left-out rows of V tiles
+//   warp 11     idle
+//   warps 12-15 stores: O / l of a finished unit, while the softmax warps are
+//               at the next one
 // TMEM: S0 | S1 | O0 | O1, 128 columns each (O: D).  P goes back to TMEM as
 // 16-bit values over the S it came from and is the A operand of P V.  One
-// warp issues, per tile j of a unit:
-//   S0(j)  P V1(j-1)  S1(j)  P V0(j)
-// across the units' borders too, so the tensor pipe has one 128-row tile's
-// products while the other's softmax runs.  The stream executes in order:
-// S_i(j) cannot overwrite P_i(j-1) before P V_i(j-1) has read it, and the
-// commit behind S_i(j) says that O_i is settled as well.  O_i of the next unit
-// starts only when P_i of its first tile is there, which the softmax warps
-// write after they have read the last unit's O_i.
+// warp issues round after round, across the units' borders too:
+//   P V0(t-1)  S0(t)  P V1(t-1)  S1(t)
+// so the tensor pipe has one 128-row tile's products while the other's softmax
+// runs.  The stream executes in order: S_i(t) cannot overwrite P_i(t-1) before
+// P V_i has read it, and the commit behind S_i(t) says that O_i is settled as
+// well.
 // The running maximum is raised lazily, by steps of more than 2^8, so P <=
 // 2^8: exact in fp32 sums, inside f16's range.
 // Left-out keys: a score column is replaced (-inf) whatever it holds, and the
@@ -44,11 +45,13 @@ using h3b::XAttn;
 constexpr int BQ = 128, BKV = 128;
 constexpr int QST = 3;   // Q ring (128-row tiles)
 constexpr int KVST = 4;  // K/V ring (K_s in slots 0, 2, V_s in 1, 3)
-constexpr int THREADS = 384;
-constexpr int REGS_LAUNCH = 168;
+constexpr int THREADS = 512;
+constexpr int REGS_LAUNCH = 128;
 constexpr int REGS_CONTROL = 88;
-constexpr int REGS_SOFTMAX = 208;
-static_assert(128 * (REGS_CONTROL + 2 * REGS_SOFTMAX) <= THREADS * REGS_LAUNCH, "register split exceeds launch");
+constexpr int REGS_STORE = 72;
+constexpr int REGS_SOFTMAX = 176;
+static_assert(128 * (REGS_CONTROL + REGS_STORE + 2 * REGS_SOFTMAX) <= THREADS * REGS_LAUNCH,
+              "register split exceeds launch");
 constexpr float RESCALE_THRESHOLD = 8.0f;
 constexpr float LOG2E = 1.4426950408889634f;
 constexpr float LN2 = 0.69314718055994531f;
@@ -64,10 +67,14 @@ struct __align__(8) Bars {
   uint64_t q_full[QST];
   uint64_t q_free[QST];
   uint64_t kv_full[KVST];
-  uint64_t kv_free[KVST];
+  uint64_t kv_free[2];    // by round parity: round t of the products has read V_{t-1} and K_t
   uint64_t s_full[2];
   uint64_t p_half[2][2];  // one arrival per softmax warp
   uint64_t o_full[2];
+  uint64_t o_free[2];     // the 4 storing warps have read O_i
+  uint64_t ml_full[2];    // the row statistics of O_i: one arrival per softmax warp
+  uint64_t ml_free[2];    // read by the 4 storing warps
+  uint64_t v_ready[2];    // a V tile (by turns) is loaded and its left-out rows are zeroed
   uint64_t drain;
   uint32_t tmem_base;
   int abort_flag;
@@ -75,8 +82,9 @@ struct __align__(8) Bars {
 
 template <int D>
 constexpr size_t smem_bytes() {
-  return 1024 + (QST + KVST) * Cfg<D>::TILE_BYTES + sizeof(Bars);
+  return (QST + KVST) * Cfg<D>::TILE_BYTES + 2 * 128 * sizeof(float2) + sizeof(Bars);
 }
+static_assert(smem_bytes<128>() <= 232448, "shared memory of a CTA");
 
 struct TileArgs {
   XAttn a;
@@ -84,41 +92,62 @@ struct TileArgs {
   int units;
   int group;
   int o_wide;   // 32-byte stores of o allowed
+  int step_q, step_split, step_head, step_b;  // gridDim.x units further, digit by digit
   float scale_log2;
 };
 
-// One unit of work.
+// The units of one CTA, x = blockIdx.x, + gridDim.x, ...  x counts query tile
+// (fastest: units that run together share K and V in L2), split, head, sample.
+// The digits are carried from unit to unit: four divisions cost the issuing
+// warp and the softmax warps ~2000 cycles a unit.
 struct Unit {
-  int b, head, q0, split;
-  int len;   // the sample's kept prefix
-  int j0, n; // first tile, tiles
-  bool two;  // rows 128-255 exist
-};
+  int x;
+  int qt, split, head, b;
+  int q0;
+  int len;    // the sample's kept prefix
+  int j0, n;  // first tile, tiles
+  bool two;   // rows 128-255 exist
 
-H3B_DEV Unit unit_of(const TileArgs& args, int u) {
-  const XAttn& a = args.a;
-  Unit x;
-  const int qt = u % args.q_tiles;  // fastest: units that run together share K and V in L2
-  u /= args.q_tiles;
-  x.split = u % a.splits;
-  u /= a.splits;
-  x.head = u % a.heads;
-  x.b = u / a.heads;
-  x.q0 = qt * 2 * BQ;
-  x.len = a.s_kv;
-  if (a.kv_lens != nullptr) x.len = max(0, min(x.len, __ldg(a.kv_lens + x.b)));
-  int end = x.len;
-  if (a.causal) end = max(0, min(end, x.len - a.s_q + min(x.q0 + 2 * BQ, a.s_q)));
-  const int per = ((x.len + BKV - 1) / BKV + a.splits - 1) / a.splits;
-  x.j0 = x.split * per;
-  x.n = max(0, min((end + BKV - 1) / BKV, x.j0 + per) - x.j0);
-  x.two = x.q0 + BQ < a.s_q;
-  return x;
-}
+  H3B_DEV void settle(const TileArgs& args) {
+    const XAttn& a = args.a;
+    q0 = qt * 2 * BQ;
+    two = q0 + BQ < a.s_q;
+    len = a.s_kv;
+    if (a.kv_lens != nullptr && x < args.units) len = max(0, min(len, __ldg(a.kv_lens + b)));
+    int end = len;
+    if (a.causal) end = max(0, min(end, len - a.s_q + min(q0 + 2 * BQ, a.s_q)));
+    const int tiles = (len + BKV - 1) / BKV;
+    const int per = a.splits == 1 ? tiles : (tiles + a.splits - 1) / a.splits;
+    j0 = split * per;
+    n = max(0, min((end + BKV - 1) / BKV, j0 + per) - j0);
+  }
+  H3B_DEV void first(const TileArgs& args) {
+    x = blockIdx.x;
+    int u = x;
+    qt = u % args.q_tiles;
+    u /= args.q_tiles;
+    split = u % args.a.splits;
+    u /= args.a.splits;
+    head = u % args.a.heads;
+    b = u / args.a.heads;
+    settle(args);
+  }
+  H3B_DEV void next(const TileArgs& args) {
+    x += gridDim.x;
+    qt += args.step_q;
+    split += args.step_split;
+    head += args.step_head;
+    b += args.step_b;
+    if (qt >= args.q_tiles) qt -= args.q_tiles, ++split;
+    if (split >= args.a.splits) split -= args.a.splits, ++head;
+    if (head >= args.a.heads) head -= args.a.heads, ++b;
+    settle(args);
+  }
+};
 
 template <bool SPIN = false>
 H3B_DEV bool warp_wait(uint64_t* bar, uint32_t parity, int site, volatile int* abort_flag) {
-  const bool ok = mbar_wait<SPIN>(bar, parity, &g_status, site, abort_flag);
+  const bool ok = mbar_wait<SPIN, false, true>(bar, parity, &g_status, site, abort_flag);
   return __all_sync(0xffffffffu, ok);
 }
 
@@ -146,6 +175,17 @@ H3B_DEV void keep_words(bool masked, uint32_t bytes, int valid, uint32_t (&w)[4]
     w[c] = v >= 32 ? 0xffffffffu : (v <= 0 ? 0u : (1u << v) - 1u);
     if (masked) w[c] = __ballot_sync(0xffffffffu, (bytes >> c) & 1u);
   }
+}
+
+H3B_DEV void tmem_ld8(uint32_t taddr, uint32_t (&r)[8]) {
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
+               : "r"(taddr));
+}
+H3B_DEV void tmem_st8(uint32_t taddr, const uint32_t (&r)[8]) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"r"(taddr), "r"(r[0]),
+               "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
+               : "memory");
 }
 
 H3B_DEV float row_max64(const uint32_t* r) {
@@ -204,11 +244,15 @@ __global__ void __launch_bounds__(THREADS, 1)
   using C = Cfg<D>;
   constexpr uint32_t IDESC_S = F16 ? idesc_f16_f32(128, BKV, 0, 0) : idesc_bf16_f32(128, BKV, 0, 0);
   constexpr uint32_t IDESC_O = F16 ? idesc_f16_f32(128, D, 0, 1) : idesc_bf16_f32(128, D, 0, 1);
-  extern __shared__ uint8_t smem_raw[];
-  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  uint8_t* sQ = smem;
+  extern __shared__ __align__(1024) uint8_t smem_tiles[];
+  if ((smem_u32(smem_tiles) & 1023u) != 0) {  // the same for the whole CTA; nothing has been started
+    if (threadIdx.x == 0 && atomicCAS(&g_status.code, 0, H3B_ERR_DEVICE) == 0) g_status.site = 30;
+    return;
+  }
+  uint8_t* sQ = smem_tiles;
   uint8_t* sKV = sQ + QST * C::TILE_BYTES;
-  Bars* bars = reinterpret_cast<Bars*>(sKV + KVST * C::TILE_BYTES);
+  float2* s_ml = reinterpret_cast<float2*>(sKV + KVST * C::TILE_BYTES);  // [2][128]
+  Bars* bars = reinterpret_cast<Bars*>(s_ml + 2 * 128);
   const XAttn& a = args.a;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   volatile int* abort_flag = &bars->abort_flag;
@@ -219,16 +263,19 @@ __global__ void __launch_bounds__(THREADS, 1)
       mbar_init(&bars->q_full[i], 1);
       mbar_init(&bars->q_free[i], 1);
     }
-    for (int i = 0; i < KVST; ++i) {
-      mbar_init(&bars->kv_full[i], 1);
-      mbar_init(&bars->kv_free[i], 1);
-    }
+    for (int i = 0; i < KVST; ++i) mbar_init(&bars->kv_full[i], 1);
     for (int i = 0; i < 2; ++i) {
+      mbar_init(&bars->kv_free[i], 1);
       mbar_init(&bars->s_full[i], 1);
       mbar_init(&bars->p_half[i][0], 4);
       mbar_init(&bars->p_half[i][1], 4);
       mbar_init(&bars->o_full[i], 1);
+      mbar_init(&bars->o_free[i], 4);
+      mbar_init(&bars->ml_full[i], 4);
+      mbar_init(&bars->ml_free[i], 4);
     }
+    mbar_init(&bars->v_ready[0], 1);
+    mbar_init(&bars->v_ready[1], 1);
     mbar_init(&bars->drain, 1);
     bars->abort_flag = 0;
     fence_barrier_init();
@@ -244,21 +291,25 @@ __global__ void __launch_bounds__(THREADS, 1)
   auto s_col = [](int i) { return static_cast<uint32_t>(i * 128); };
   auto o_col = [](int i) { return static_cast<uint32_t>(256 + i * 128); };
 
-  if (warp >= 8) {
+  Unit u;  // each role walks the CTA's units on its own
+  u.first(args);
+
+  if (warp >= 8 && warp < 12) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(REGS_CONTROL));
     if (warp == 8 && lane == 0) {
       // ------------------------------------------------------------ TMA
-      // Slot of the c-th Q (K/V) tile: c % ring; its free barrier has
-      // completed phase (c / ring) - 1 when the tile before it is read, and
-      // its next phase needs this very load: a parity wait is one phase behind.
+      // Slot of the c-th Q tile: c % ring; its free barrier has completed
+      // phase (c / ring) - 1 when the tile before it is read, and its next
+      // phase needs this very load: a parity wait is one phase behind.  So it
+      // is for K and V: round t + 1 of the products needs V_t, round t needs K_t.
       prefetch_tmap(&tm_q);
       prefetch_tmap(&tm_k);
       prefetch_tmap(&tm_v);
-      int qc = 0, kvc = 0;
+      int qc = 0;
       bool ok = true;
       auto load_q = [&](const Unit& u, int i) {
         const int s = qc % QST;
-        if (qc >= QST && !mbar_wait(&bars->q_free[s], (qc / QST - 1) & 1, &g_status, 1, abort_flag)) return false;
+        if (qc >= QST && !mbar_wait<false, false, true>(&bars->q_free[s], (qc / QST - 1) & 1, &g_status, 1, abort_flag)) return false;
         mbar_arrive_expect_tx(&bars->q_full[s], C::TILE_BYTES);
         for (int h = 0; h < C::HALVES; ++h)
           tma_load_4d(sQ + s * C::TILE_BYTES + h * C::HALF_BYTES, &tm_q, h * 64, u.q0 + i * BQ, u.head, u.b,
@@ -266,177 +317,203 @@ __global__ void __launch_bounds__(THREADS, 1)
         ++qc;
         return true;
       };
-      auto load_kv = [&](const CUtensorMap* tm, const Unit& u, int j) {
-        const int s = kvc % KVST;
-        if (kvc >= KVST && !mbar_wait(&bars->kv_free[s], (kvc / KVST - 1) & 1, &g_status, 2, abort_flag)) return false;
+      // K_t overwrites K_{t-2}, released with round t - 2 of the products; V_t
+      // overwrites V_{t-2}, released with round t - 1 (see the matrix warp).
+      auto load_kv = [&](const CUtensorMap* tm, const Unit& u, int j, int s, int round) {
+        if (round >= 0 &&
+            !mbar_wait<false, false, true>(&bars->kv_free[round & 1], (round >> 1) & 1, &g_status, 2, abort_flag))
+          return false;
         mbar_arrive_expect_tx(&bars->kv_full[s], C::TILE_BYTES);
         for (int h = 0; h < C::HALVES; ++h)
-          tma_load_4d(sKV + s * C::TILE_BYTES + h * C::HALF_BYTES, tm, h * 64, (u.j0 + j) * BKV, u.head / args.group,
-                      u.b, &bars->kv_full[s]);
-        ++kvc;
+          tma_load_4d(sKV + s * C::TILE_BYTES + h * C::HALF_BYTES, tm, h * 64, (u.j0 + j) * BKV,
+                      args.group == 1 ? u.head : u.head / args.group, u.b, &bars->kv_full[s]);
         return true;
       };
-      for (int x = blockIdx.x; x < args.units && ok; x += gridDim.x) {
-        const Unit u = unit_of(args, x);
-        for (int j = 0; j < u.n && ok; ++j) {
-          if (j == 0) ok = ok && load_q(u, 0);
-          ok = ok && load_kv(&tm_k, u, j);
-          if (j == 0 && u.two) ok = ok && load_q(u, 1);
-          ok = ok && load_kv(&tm_v, u, j);
+      int t = 0, loaded = 0;
+#pragma unroll 1
+      for (; u.x < args.units && ok; u.next(args)) {
+#pragma unroll 1
+        for (int j = 0; j < u.n && ok; ++j, ++t) {
+          if (j == 0) ok = load_q(u, 0);
+          if (ok && (ok = load_kv(&tm_k, u, j, 2 * (t & 1), t - 2))) loaded = 2 * t + 1;
+          if (ok && j == 0 && u.two) ok = load_q(u, 1);
+          if (ok && (ok = load_kv(&tm_v, u, j, 2 * (t & 1) + 1, t < 2 ? -1 : t - 1))) loaded = 2 * t + 2;
         }
       }
       if (!ok || *abort_flag) {
         // let the copies in flight land (bounded) before the CTA goes
         for (int c = max(0, qc - QST); c < qc; ++c)
-          mbar_wait(&bars->q_full[c % QST], (c / QST) & 1, &g_status, 10, nullptr);
-        for (int c = max(0, kvc - KVST); c < kvc; ++c)
-          mbar_wait(&bars->kv_full[c % KVST], (c / KVST) & 1, &g_status, 11, nullptr);
+          mbar_wait<false, false, true>(&bars->q_full[c % QST], (c / QST) & 1, &g_status, 10, nullptr);
+        for (int c = max(0, loaded - KVST); c < loaded; ++c)
+          mbar_wait<false, false, true>(&bars->kv_full[c % KVST], (c / KVST) & 1, &g_status, 11, nullptr);
       }
     } else if (warp == 9) {
       // ------------------------------------------------------------ MMA
       // The warp runs the schedule converged: all lanes poll, one elected
-      // lane issues.  Every barrier waited on here completes once per use and
-      // its next use depends on what this warp issues after the wait.
-      int qc = 0, step = 0;
-      uint32_t pc[2] = {0, 0};  // P tiles consumed, per row tile
+      // lane issues.  Round t of the products is
+      //   P V_0(t-1)  S_0(t)  P V_1(t-1)  S_1(t)
+      // and everything that can be waited for or worked out before a P tile
+      // is there (V, K, Q, descriptors, the next unit) comes before the wait
+      // for P: what stands between P and the products behind it is on every
+      // tile's critical path (softmax -> P V -> S -> softmax).  Measured with
+      // those waits behind P V: 5000 cycles a round, 3000 of them with the
+      // softmax warps idle.
+      // Every barrier waited on completes once per use and its next use
+      // depends on what this warp issues after the wait.
+      int qc = 0, j = 0;
+      uint32_t phases = 0;  // bit i: parity of row tile i's P; bit 2 + i: of its O; bit 4 + i: O begun once
       bool ok = true;
-      auto commit = [&](uint64_t* bar) {
-        if (elect_one()) tc_commit(bar);
-        __syncwarp();
-      };
       auto wait = [&](uint64_t* bar, uint32_t parity, int site) {
-        if (!warp_wait<true>(bar, parity, site, abort_flag)) return false;
-        tc_fence_after();
-        return true;
+        ok = mbar_wait<true, false, true>(bar, parity, &g_status, site, abort_flag) && ok;
       };
-      auto wait_kv = [&](int c) { return wait(&bars->kv_full[c % KVST], (c / KVST) & 1, 4); };
-      auto issue_s = [&](int i, int qslot, int kslot) {
-        const uint64_t qd = sdesc_kmajor_sw128(smem_u32(sQ + qslot * C::TILE_BYTES));
-        const uint64_t kd = sdesc_kmajor_sw128(smem_u32(sKV + kslot * C::TILE_BYTES));
-        if (elect_one()) {
+      // of the step whose P V comes in this round
+      bool pv = false, pv_two = false, pv_first = false, pv_last = false;
+      while (u.x < args.units && u.n == 0) u.next(args);
+      bool more = u.x < args.units;
+#pragma unroll 1
+      for (int t = 0; more || pv; ++t) {
+        const bool first = j == 0, last = j == u.n - 1, two = u.two;
+        const uint32_t k_s = smem_u32(sKV + 2 * (t & 1) * C::TILE_BYTES);
+        const uint32_t v_s = smem_u32(sKV + (2 * ((t + 1) & 1) + 1) * C::TILE_BYTES);
+        const uint64_t kd = sdesc_kmajor_sw128(k_s);
+        const uint64_t vd = sdesc_mnmajor_sw128(v_s, C::HALF_BYTES, 1024);
+        if (pv) wait(&bars->v_ready[(t + 1) & 1], ((t - 1) >> 1) & 1, 7);
+        if (more) wait(&bars->kv_full[2 * (t & 1)], (t >> 1) & 1, 4);
 #pragma unroll
-          for (int kk = 0; kk < D / 16; ++kk) {
-            const uint32_t at = static_cast<uint32_t>((kk >> 2) * (C::HALF_BYTES >> 4) + (kk & 3) * 2);
-            mma_f16_ss(tmem + s_col(i), desc_add_lo(qd, at), desc_add_lo(kd, at), IDESC_S, kk > 0);
+        for (int i = 0; i < 2; ++i) {
+          const bool do_pv = pv && (i == 0 || pv_two), do_s = more && (i == 0 || two);
+          const int qs = (qc + i) % QST;
+          const uint64_t qd = sdesc_kmajor_sw128(smem_u32(sQ + qs * C::TILE_BYTES));
+          const uint32_t s_tmem = tmem + s_col(i), o_tmem = tmem + o_col(i);
+          if (do_s && first) wait(&bars->q_full[qs], ((qc + i) / QST) & 1, 3);
+          if (do_pv) {
+            if (pv_first) {  // O_i of the unit before has been read (its phase: one a unit)
+              if ((phases >> (4 + i)) & 1) {
+                wait(&bars->o_free[i], (phases >> (2 + i)) & 1, 6);
+                phases ^= 4u << i;
+              }
+              phases |= 16u << i;
+            }
+            // as the softmax delivers: 64 keys a half
+            wait(&bars->p_half[i][0], (phases >> i) & 1, 5);
+            __syncwarp();
+            tc_fence_after();
+            if (elect_one()) {
+#pragma unroll
+              for (int kk = 0; kk < 4; ++kk)
+                mma_f16_ts(o_tmem, s_tmem + kk * 8, desc_add_lo(vd, static_cast<uint32_t>(kk * (2048 >> 4))), IDESC_O,
+                           (pv_first && kk == 0) ? 0u : 1u);
+            }
+            wait(&bars->p_half[i][1], (phases >> i) & 1, 5);
+            phases ^= 1u << i;
           }
-          tc_commit(&bars->s_full[i]);
-        }
-        __syncwarp();
-      };
-      // O_i (+)= P_i V, in two halves of 64 keys as the softmax delivers them
-      auto issue_pv = [&](int i, int vslot, bool first) -> bool {
-        const uint64_t vd = sdesc_mnmajor_sw128(smem_u32(sKV + vslot * C::TILE_BYTES), C::HALF_BYTES, 1024);
-        for (int h = 0; h < 2; ++h) {
-          if (!wait(&bars->p_half[i][h], pc[i] & 1, 5)) return false;
+          __syncwarp();
+          tc_fence_after();
           if (elect_one()) {
+            if (do_pv) {
 #pragma unroll
-            for (int kk = 4 * h; kk < 4 * h + 4; ++kk)
-              mma_f16_ts(tmem + o_col(i), tmem + s_col(i) + kk * 8, desc_add_lo(vd, static_cast<uint32_t>(kk * (2048 >> 4))),
-                         IDESC_O, (first && kk == 0) ? 0u : 1u);
+              for (int kk = 4; kk < 8; ++kk)
+                mma_f16_ts(o_tmem, s_tmem + kk * 8, desc_add_lo(vd, static_cast<uint32_t>(kk * (2048 >> 4))), IDESC_O, 1u);
+              if (pv_last) tc_commit(&bars->o_full[i]);
+            }
+            if (do_s) {
+#pragma unroll
+              for (int kk = 0; kk < D / 16; ++kk) {
+                const uint32_t at = static_cast<uint32_t>((kk >> 2) * (C::HALF_BYTES >> 4) + (kk & 3) * 2);
+                mma_f16_ss(s_tmem, desc_add_lo(qd, at), desc_add_lo(kd, at), IDESC_S, kk > 0);
+              }
+              tc_commit(&bars->s_full[i]);
+              if (last) tc_commit(&bars->q_free[qs]);
+            }
+            if (i == 1) tc_commit(&bars->kv_free[t & 1]);
           }
           __syncwarp();
         }
-        ++pc[i];
-        return true;
-      };
-      bool pend = false, pend_first = false, pend_last = false;  // P V1 of the step before
-      int pend_slot = 0;
-      auto flush = [&]() -> bool {
-        if (!pend) return true;
-        if (!issue_pv(1, pend_slot, pend_first)) return false;
-        if (pend_last) commit(&bars->o_full[1]);
-        commit(&bars->kv_free[pend_slot]);
-        pend = false;
-        return true;
-      };
-      for (int x = blockIdx.x; x < args.units && ok; x += gridDim.x) {
-        const Unit u = unit_of(args, x);
-        if (u.n == 0) continue;
-        const int q0c = qc, q1c = qc + 1;
-        qc += u.two ? 2 : 1;
-        for (int j = 0; j < u.n && ok; ++j, ++step) {
-          const int kc = 2 * step, vc = 2 * step + 1;
+        if (!__all_sync(0xffffffffu, ok)) break;
+        pv = more;
+        pv_two = two;
+        pv_first = first;
+        pv_last = last;
+        if (more && ++j == u.n) {
+          j = 0;
+          qc += two ? 2 : 1;
+          do {
+            u.next(args);
+          } while (u.x < args.units && u.n == 0);
+          more = u.x < args.units;
+        }
+      }
+      if (elect_one()) tc_commit(&bars->drain);
+      __syncwarp();
+      warp_wait(&bars->drain, 0, 8, nullptr);
+    } else if (warp == 10) {
+      // ------------------------------------------------------------ left-out rows of V
+      // Every V tile passes through here, so that this warp is never more than
+      // a phase behind: V_{t+2} is loaded over V_t after P V(t), which waits
+      // for v_ready.  (V is there well before it is needed.)
+      int step = 0;
+      bool ok = true;
+      #pragma unroll 1
+      for (; u.x < args.units && ok; u.next(args)) {
+#pragma unroll 1
+        for (int j = 0; j < u.n; ++j, ++step) {
           const int key0 = (u.j0 + j) * BKV;
+          const int slot = 2 * (step & 1) + 1;
           const uint32_t mb = masked ? mask_bytes(a, u.b, key0, u.len, lane) : 0u;
-          ok = wait_kv(kc) && (j > 0 || wait(&bars->q_full[q0c % QST], (q0c / QST) & 1, 3));
-          if (!ok) break;
-          issue_s(0, q0c % QST, kc % KVST);
-          const bool last = j == u.n - 1;
-          if (last) commit(&bars->q_free[q0c % QST]);
-          ok = flush() && (j > 0 || !u.two || wait(&bars->q_full[q1c % QST], (q1c / QST) & 1, 3));
-          if (!ok) break;
-          if (u.two) issue_s(1, q1c % QST, kc % KVST);
-          commit(&bars->kv_free[kc % KVST]);
-          if (last && u.two) commit(&bars->q_free[q1c % QST]);
-          ok = wait_kv(vc);
-          if (!ok) break;
-          uint32_t w[4];
-          keep_words(masked, mb, u.len - key0, w);
-          if ((w[0] & w[1] & w[2] & w[3]) != 0xffffffffu) {
-            // rows of V that are left out: zeros (a row's 16-byte pieces keep
-            // their row under the swizzle, so the order does not matter)
-            const uint32_t v = smem_u32(sKV + (vc % KVST) * C::TILE_BYTES);
+          if (!warp_wait(&bars->kv_full[slot], (step >> 1) & 1, 9, abort_flag)) {
+            ok = false;
+            break;
+          }
+          if (masked || key0 + BKV > u.len) {
+            uint32_t w[4];
+            keep_words(masked, mb, u.len - key0, w);
+            // (a row's 16-byte pieces keep their row under the swizzle)
+            const uint32_t v = smem_u32(sKV + slot * C::TILE_BYTES);
             const int piece = lane & 7;
-            for (int r = lane >> 3; r < BKV; r += 4) {
-              if (((w[r >> 5] >> (r & 31)) & 1u) == 0) {
 #pragma unroll
-                for (int h = 0; h < C::HALVES; ++h)
-                  asm volatile("st.shared.v4.u32 [%0], {%1,%1,%1,%1};" ::"r"(v + h * C::HALF_BYTES + r * 128 + piece * 16),
-                               "r"(0u)
-                               : "memory");
-              }
+            for (int c = 0; c < 4; ++c) {
+              if (w[c] == 0xffffffffu) continue;
+              for (int r = lane >> 3; r < 32; r += 4)
+                if (((w[c] >> r) & 1u) == 0) {
+#pragma unroll
+                  for (int h = 0; h < C::HALVES; ++h)
+                    asm volatile("st.shared.v4.u32 [%0], {%1,%1,%1,%1};" ::"r"(v + h * C::HALF_BYTES + (c * 32 + r) * 128 +
+                                                                               piece * 16),
+                                 "r"(0u)
+                                 : "memory");
+                }
             }
             fence_proxy_async_smem();
             __syncwarp();
           }
-          ok = issue_pv(0, vc % KVST, j == 0);
-          if (!ok) break;
-          if (last) commit(&bars->o_full[0]);
-          if (u.two) {
-            pend = true;
-            pend_first = j == 0;
-            pend_last = last;
-            pend_slot = vc % KVST;
-          } else {
-            commit(&bars->kv_free[vc % KVST]);
-          }
+          if (lane == 0) mbar_arrive(&bars->v_ready[step & 1]);
         }
       }
-      if (ok) flush();
-      commit(&bars->drain);
-      warp_wait(&bars->drain, 0, 8, nullptr);
     }
-  } else {
-    // ------------------------------------------------------------ softmax, stores
+  } else if (warp < 8) {
+    // ------------------------------------------------------------ softmax
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(REGS_SOFTMAX));
     const int wg = warp >> 2;
     const int row = (warp & 3) * 32 + lane;
     const uint32_t lane_off = static_cast<uint32_t>((warp & 3) * 32) << 16;
     const uint32_t s_tmem = tmem + s_col(wg) + lane_off;
     const uint32_t o_tmem = tmem + o_col(wg) + lane_off;
-    const int64_t total_rows = static_cast<int64_t>(a.batch) * a.heads * a.s_q;
-    uint32_t sc = 0, oc = 0;  // S tiles, O tiles seen
+    uint32_t sc = 0, oc = 0;  // S tiles, units seen
     bool ok = true;
-    for (int x = blockIdx.x; x < args.units && ok; x += gridDim.x) {
-      const Unit u = unit_of(args, x);
-      if (wg == 1 && !u.two) continue;
-      const int q_row = u.q0 + wg * BQ + row;
+    #pragma unroll 1
+    for (; u.x < args.units && ok; u.next(args)) {
+      if (u.n == 0 || (wg == 1 && !u.two)) continue;
       float m_run = -INFINITY;  // running max, log2 domain
       float l_run = 0.0f;
+#pragma unroll 1
       for (int j = 0; j < u.n; ++j, ++sc) {
         const int key0 = (u.j0 + j) * BKV;
-        const uint32_t mb = masked ? mask_bytes(a, u.b, key0, u.len, lane) : 0u;
-        // S_i of the next tile is published only after this tile's P_i
-        if (!warp_wait<true>(&bars->s_full[wg], sc & 1, 20, abort_flag)) {
-          ok = false;
-          break;
-        }
-        tc_fence_after();
+        // which columns are kept: known before S is
         uint32_t w[4];
-        keep_words(masked, mb, u.len - key0, w);
+        keep_words(masked, masked ? mask_bytes(a, u.b, key0, u.len, lane) : 0u, u.len - key0, w);
         bool whole = (w[0] & w[1] & w[2] & w[3]) == 0xffffffffu;
         if (a.causal && u.len - a.s_q + u.q0 + wg * BQ + 1 < key0 + BKV) {
-          const int valid = u.len - a.s_q + q_row + 1 - key0;
+          const int valid = u.len - a.s_q + u.q0 + wg * BQ + row + 1 - key0;
 #pragma unroll
           for (int c = 0; c < 4; ++c) {
             const int v = valid - 32 * c;
@@ -444,54 +521,72 @@ __global__ void __launch_bounds__(THREADS, 1)
           }
           whole = false;
         }
-        uint32_t r[128];
-        auto load_s = [&]() {
+        // S_i of the next tile is published only after this tile's P_i
+        if (!warp_wait<true>(&bars->s_full[wg], sc & 1, 20, abort_flag)) {
+          ok = false;
+          break;
+        }
+        tc_fence_after();
+        if (!whole) {
+          // Left-out columns become -inf in TMEM, 32 at a time in a loop that
+          // stays out of the instruction cache of whole tiles.
+#pragma unroll 1
+          for (int c = 0; c < 4; ++c) {
+            const uint32_t keep = c < 2 ? (c == 0 ? w[0] : w[1]) : (c == 2 ? w[2] : w[3]);
+            if (__all_sync(0xffffffffu, keep == 0xffffffffu)) continue;
+            uint32_t o[32];
+            tmem_ld32p(s_tmem + c * 32, o);
+            tmem_wait_fence<1>(o);
 #pragma unroll
-          for (int c = 0; c < 4; ++c) tmem_ld32p(s_tmem + c * 32, r + 32 * c);
-          tmem_wait_fence<4>(r);
-          if (!whole) {
-#pragma unroll
-            for (int e = 0; e < 128; ++e)
-              if ((w[e >> 5] & (1u << (e & 31))) == 0) r[e] = __float_as_uint(-INFINITY);
+            for (int e = 0; e < 32; ++e)
+              if ((keep & (1u << e)) == 0) o[e] = __float_as_uint(-INFINITY);
+            __syncwarp();
+            tmem_st32(s_tmem + c * 32, o);
           }
-        };
-        load_s();
-        // After the first tile half 0 is exponentiated against the running
-        // maximum while the tile's is found; only where that outgrew it by
-        // more than the threshold the warp reloads S (P is not written yet).
+          tc_wait_st();
+        }
+        // The first tile looks for its maximum first.  After it, half 0 is
+        // exponentiated against the running maximum while the tile's is found;
+        // only where that outgrew it by more than the threshold the warp goes
+        // round again (P is not written over S yet).
+        uint32_t r[128];
         float m_use = m_run;
         float sum = 0.0f;
         bool slow = j == 0;
-        if (!slow) {
-          const float2 sm = exp_pack64<F16, true>(r, r, args.scale_log2, m_run == -INFINITY ? 0.0f : -m_run);
-          slow = __any_sync(0xffffffffu, sm.y * args.scale_log2 > m_run + RESCALE_THRESHOLD);
+#pragma unroll 1
+        for (int round = 0; round < 2; ++round) {
+#pragma unroll
+          for (int c = 0; c < 4; ++c) tmem_ld32p(s_tmem + c * 32, r + 32 * c);
+          tmem_wait_fence<4>(r);
           if (slow) {
-            load_s();
-          } else {
-            sum = sm.x;
-          }
-        }
-        if (slow) {
-          const float m_tile = fmaxf(row_max64(r), row_max64(r + 64)) * args.scale_log2;
-          const bool rescale = m_tile > m_run + RESCALE_THRESHOLD;
-          if (rescale) m_use = m_tile;
-          if (__any_sync(0xffffffffu, rescale)) {
-            const float factor = rescale ? ex2(m_run - m_use) : 1.0f;
-            l_run *= factor;
-            if (j > 0) {
+            const float m_tile = fmaxf(row_max64(r), row_max64(r + 64)) * args.scale_log2;
+            const bool rescale = m_tile > m_run + RESCALE_THRESHOLD;
+            if (rescale) m_use = m_tile;
+            if (__any_sync(0xffffffffu, rescale)) {
+              const float factor = rescale ? ex2(m_run - m_use) : 1.0f;
+              l_run *= factor;
+              if (j > 0) {
+#pragma unroll 1
+                for (int c = 0; c < D / 8; ++c) {  // (few registers: the tile's scores stay live)
+                  uint32_t o[8];
+                  tmem_ld8(o_tmem + c * 8, o);
+                  tc_wait_ld();
 #pragma unroll
-              for (int c = 0; c < D / 32; ++c) {
-                uint32_t o[32];
-                tmem_ld32p(o_tmem + c * 32, o);
-                tmem_wait_fence<1>(o);
-#pragma unroll
-                for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * factor);
-                tmem_st32(o_tmem + c * 32, o);
+                  for (int e = 0; e < 8; ++e) {
+                    asm volatile("" : "+r"(o[e]));
+                    o[e] = __float_as_uint(__uint_as_float(o[e]) * factor);
+                  }
+                  tmem_st8(o_tmem + c * 8, o);
+                }
               }
+              if (rescale) m_run = m_use;
             }
-            if (rescale) m_run = m_use;
           }
-          sum = exp_pack64<F16, false>(r, r, args.scale_log2, m_use == -INFINITY ? 0.0f : -m_use).x;
+          const float2 sm = exp_pack64<F16, true>(r, r, args.scale_log2, m_use == -INFINITY ? 0.0f : -m_use);
+          sum = sm.x;
+          if (slow) break;
+          slow = __any_sync(0xffffffffu, sm.y * args.scale_log2 > m_run + RESCALE_THRESHOLD);
+          if (!slow) break;
         }
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
@@ -506,64 +601,99 @@ __global__ void __launch_bounds__(THREADS, 1)
         l_run += sum;
       }
       if (!ok) break;
-      // ---- the unit's rows
-      if (u.n > 0) {
-        if (!warp_wait(&bars->o_full[wg], oc & 1, 23, abort_flag)) {
-          ok = false;
-          break;
-        }
-        ++oc;
-        tc_fence_after();
+      // ---- the row statistics, to the storing warps
+      if (oc > 0 && !warp_wait(&bars->ml_free[wg], (oc - 1) & 1, 22, abort_flag)) {
+        ok = false;
+        break;
       }
-      const bool in = q_row < a.s_q;
-      const int64_t lse_row = (static_cast<int64_t>(u.b) * a.heads + u.head) * a.s_q + q_row;
-      const float inv_l = l_run > 0.0f ? 1.0f / l_run : 0.0f;
-      uint16_t* orow = static_cast<uint16_t*>(a.o) + u.b * a.o_stride[0] + q_row * a.o_stride[1] + u.head * a.o_stride[2];
-      float* prow = a.part_o + (u.split * total_rows + lse_row) * D;
-#pragma unroll
-      for (int c = 0; c < D / 32; ++c) {
-        uint32_t r[32];
+      ++oc;
+      s_ml[wg * 128 + row] = make_float2(m_run, l_run);
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&bars->ml_full[wg]);
+    }
+  } else {
+    // ------------------------------------------------------------ stores
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(REGS_STORE));
+    const int row = (warp & 3) * 32 + lane;
+    const uint32_t lane_off = static_cast<uint32_t>((warp & 3) * 32) << 16;
+    const int64_t total_rows = static_cast<int64_t>(a.batch) * a.heads * a.s_q;
+    uint32_t oc0 = 0, oc1 = 0;
+    bool ok = true;
+    #pragma unroll 1
+    for (; u.x < args.units && ok; u.next(args)) {
+#pragma unroll 1
+      for (int i = 0; i < 2; ++i) {
+        if (!ok || (i == 1 && !u.two)) continue;
+        float2 ml = make_float2(-INFINITY, 0.0f);
+        const uint32_t phase = (i ? oc1 : oc0) & 1;
         if (u.n > 0) {
-          tmem_ld32p(o_tmem + c * 32, r);
-          tmem_wait_fence<1>(r);
-        } else {
-#pragma unroll
-          for (int e = 0; e < 32; ++e) r[e] = 0u;
+          // both complete once a unit, and again only after this warp's arrivals below
+          ok = warp_wait(&bars->ml_full[i], phase, 23, abort_flag) &&
+               warp_wait(&bars->o_full[i], phase, 24, abort_flag);
+          if (!ok) continue;
+          if (i) ++oc1; else ++oc0;
+          tc_fence_after();
+          ml = s_ml[i * 128 + row];
         }
-        if (!in) continue;
-        if (a.splits > 1) {
-#pragma unroll
-          for (int e = 0; e < 32; e += 8) {
-            uint32_t v[8];
-#pragma unroll
-            for (int t = 0; t < 8; ++t) v[t] = r[e + t];
-            st_global_v8(prow + c * 32 + e, v);
-          }
-        } else {
-          uint32_t p[16];
-#pragma unroll
-          for (int e = 0; e < 16; ++e)
-            p[e] = pack16x2<F16>(__uint_as_float(r[2 * e]) * inv_l, __uint_as_float(r[2 * e + 1]) * inv_l);
-          if (args.o_wide) {
-#pragma unroll
-            for (int e = 0; e < 16; e += 8) {
-              uint32_t v[8];
-#pragma unroll
-              for (int t = 0; t < 8; ++t) v[t] = p[e + t];
-              st_global_v8(orow + c * 32 + 2 * e, v);
+        const int q_row = u.q0 + i * BQ + row;
+        const bool in = q_row < a.s_q;
+        const int64_t lse_row = (static_cast<int64_t>(u.b) * a.heads + u.head) * a.s_q + q_row;
+        const float inv_l = ml.y > 0.0f ? 1.0f / ml.y : 0.0f;
+        uint16_t* orow =
+            static_cast<uint16_t*>(a.o) + u.b * a.o_stride[0] + q_row * a.o_stride[1] + u.head * a.o_stride[2];
+        float* prow = a.part_o + (u.split * total_rows + lse_row) * D;
+#pragma unroll 1
+        for (int c = 0; c < D / 32; ++c) {
+          uint32_t r[32];
+          if (u.n > 0) {
+            tmem_ld32p(tmem + o_col(i) + c * 32 + lane_off, r);
+            tmem_wait_fence<1>(r);
+            if (c == D / 32 - 1) {  // O_i and the statistics are read
+              tc_fence_before();
+              __syncwarp();
+              if (lane == 0) {
+                mbar_arrive(&bars->o_free[i]);
+                mbar_arrive(&bars->ml_free[i]);
+              }
             }
           } else {
 #pragma unroll
-            for (int e = 0; e < 16; e += 4)
-              *reinterpret_cast<uint4*>(orow + c * 32 + 2 * e) = make_uint4(p[e], p[e + 1], p[e + 2], p[e + 3]);
+            for (int e = 0; e < 32; ++e) r[e] = 0u;
           }
+          if (in && a.splits > 1) {
+#pragma unroll
+            for (int e = 0; e < 32; e += 8) {
+              uint32_t v[8];
+#pragma unroll
+              for (int t = 0; t < 8; ++t) v[t] = r[e + t];
+              st_global_v8(prow + c * 32 + e, v);
+            }
+          } else if (in) {
+#pragma unroll
+            for (int e = 0; e < 16; ++e)
+              r[e] = pack16x2<F16>(__uint_as_float(r[2 * e]) * inv_l, __uint_as_float(r[2 * e + 1]) * inv_l);
+            if (args.o_wide) {
+#pragma unroll
+              for (int e = 0; e < 16; e += 8) {
+                uint32_t v[8];
+#pragma unroll
+                for (int t = 0; t < 8; ++t) v[t] = r[e + t];
+                st_global_v8(orow + c * 32 + 2 * e, v);
+              }
+            } else {
+#pragma unroll
+              for (int e = 0; e < 16; e += 4)
+                *reinterpret_cast<uint4*>(orow + c * 32 + 2 * e) = make_uint4(r[e], r[e + 1], r[e + 2], r[e + 3]);
+            }
+          }
+          __syncwarp();  // the next tcgen05.ld is for the whole warp
         }
-      }
-      if (in) {
-        if (a.splits > 1) {
-          a.part_ml[u.split * total_rows + lse_row] = make_float2(m_run, l_run);
-        } else if (a.lse != nullptr) {
-          a.lse[lse_row] = l_run > 0.0f ? (m_run + __log2f(l_run)) * LN2 : -INFINITY;
+        if (in) {
+          if (a.splits > 1) {
+            a.part_ml[u.split * total_rows + lse_row] = ml;
+          } else if (a.lse != nullptr) {
+            a.lse[lse_row] = ml.y > 0.0f ? (ml.x + __log2f(ml.y)) * LN2 : -INFINITY;
+          }
         }
       }
     }
@@ -612,6 +742,13 @@ int launch(const XAttn& a, cudaStream_t stream) {
   args.o_wide = (reinterpret_cast<uintptr_t>(a.o) & 31u) == 0 && a.o_stride[0] % 16 == 0 && a.o_stride[1] % 16 == 0 &&
                 a.o_stride[2] % 16 == 0;
   const int sms = h3b::num_sms();
+  int step = static_cast<int>(units < sms ? units : sms);
+  args.step_q = step % args.q_tiles;
+  step /= args.q_tiles;
+  args.step_split = step % a.splits;
+  step /= a.splits;
+  args.step_head = step % a.heads;
+  args.step_b = step / a.heads;
   kernel<<<static_cast<unsigned>(units < sms ? units : sms), THREADS, smem_bytes<D>(), stream>>>(tq, tk, tv, args);
   return h3b::launch_status();
 }
