@@ -15,7 +15,8 @@
 //   warps 4-7   softmax of rows 128-255
 //   warp 8      TMA: Q through a ring of 3 tiles, K and V through one of 4
 //   warp 9      TMEM allocation and matrix instructions
-//   warp 10     zeroes the left-out rows of V tiles
+//   warp 10     what the next round of products consists of, and that its
+//               tiles are there; zeroes the left-out rows of V
 //   warp 11     idle
 //   warps 12-15 stores: O / l of a finished unit, while the softmax warps are
 //               at the next one
@@ -63,6 +64,20 @@ struct Cfg {
   static constexpr int HALF_BYTES = 128 * 64 * 2;  // 16 KB
 };
 
+// What a round of products consists of, written by warp 10 for the issuing warp.
+enum : uint32_t {
+  R_S0 = 1,        // S_0, S_1 of a tile
+  R_S1 = 2,
+  R_S_LAST = 4,    // the unit's last: Q is free after it
+  R_PV0 = 8,       // P V of the tile before
+  R_PV1 = 16,
+  R_PV_FIRST = 32, // of its unit: O starts anew
+  R_PV_LAST = 64,  // O is complete after it
+  R_END = 128,     // the last round
+  R_Q0_SHIFT = 8,  // Q slots of S_0, S_1
+  R_Q1_SHIFT = 10
+};
+
 struct __align__(8) Bars {
   uint64_t q_full[QST];
   uint64_t q_free[QST];
@@ -74,8 +89,9 @@ struct __align__(8) Bars {
   uint64_t o_free[2];     // the 4 storing warps have read O_i
   uint64_t ml_full[2];    // the row statistics of O_i: one arrival per softmax warp
   uint64_t ml_free[2];    // read by the 4 storing warps
-  uint64_t v_ready[2];    // a V tile (by turns) is loaded and its left-out rows are zeroed
+  uint64_t ready[2];      // by round parity: what round t reads is in shared memory, and todo[] says what to do
   uint64_t drain;
+  uint32_t todo[2];       // by round parity: R_* bits and Q slots
   uint32_t tmem_base;
   int abort_flag;
 };
@@ -108,12 +124,19 @@ struct Unit {
   int j0, n;  // first tile, tiles
   bool two;   // rows 128-255 exist
 
+  // WARP: called by whole warps; a reduction tells the compiler that the
+  // length, and with it all control flow, is the same for the warp (uniform
+  // registers, no convergence code: the issuing warp's rounds need it).
+  template <bool WARP>
   H3B_DEV void settle(const TileArgs& args) {
     const XAttn& a = args.a;
     q0 = qt * 2 * BQ;
     two = q0 + BQ < a.s_q;
     len = a.s_kv;
-    if (a.kv_lens != nullptr && x < args.units) len = max(0, min(len, __ldg(a.kv_lens + b)));
+    if (a.kv_lens != nullptr && x < args.units) {
+      len = max(0, min(len, __ldg(a.kv_lens + b)));
+      if constexpr (WARP) len = __reduce_max_sync(0xffffffffu, len);
+    }
     int end = len;
     if (a.causal) end = max(0, min(end, len - a.s_q + min(q0 + 2 * BQ, a.s_q)));
     const int tiles = (len + BKV - 1) / BKV;
@@ -130,8 +153,9 @@ struct Unit {
     u /= args.a.splits;
     head = u % args.a.heads;
     b = u / args.a.heads;
-    settle(args);
+    settle<true>(args);
   }
+  template <bool WARP = true>
   H3B_DEV void next(const TileArgs& args) {
     x += gridDim.x;
     qt += args.step_q;
@@ -141,14 +165,18 @@ struct Unit {
     if (qt >= args.q_tiles) qt -= args.q_tiles, ++split;
     if (split >= args.a.splits) split -= args.a.splits, ++head;
     if (head >= args.a.heads) head -= args.a.heads, ++b;
-    settle(args);
+    settle<WARP>(args);
   }
 };
 
+// (compact: the roles share instruction caches)
+template <bool SPIN>
+H3B_DEV bool lane_wait(uint64_t* bar, uint32_t parity, int site, volatile int* abort_flag) {
+  return mbar_wait<SPIN, false, true>(bar, parity, &g_status, site, abort_flag);
+}
 template <bool SPIN = false>
 H3B_DEV bool warp_wait(uint64_t* bar, uint32_t parity, int site, volatile int* abort_flag) {
-  const bool ok = mbar_wait<SPIN, false, true>(bar, parity, &g_status, site, abort_flag);
-  return __all_sync(0xffffffffu, ok);
+  return __all_sync(0xffffffffu, lane_wait<SPIN>(bar, parity, site, abort_flag));
 }
 
 H3B_DEV float ex2(float x) {
@@ -274,8 +302,8 @@ __global__ void __launch_bounds__(THREADS, 1)
       mbar_init(&bars->ml_full[i], 4);
       mbar_init(&bars->ml_free[i], 4);
     }
-    mbar_init(&bars->v_ready[0], 1);
-    mbar_init(&bars->v_ready[1], 1);
+    mbar_init(&bars->ready[0], 1);
+    mbar_init(&bars->ready[1], 1);
     mbar_init(&bars->drain, 1);
     bars->abort_flag = 0;
     fence_barrier_init();
@@ -287,7 +315,14 @@ __global__ void __launch_bounds__(THREADS, 1)
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const uint32_t tmem = bars->tmem_base;
+  // All 512 columns are this CTA's, so they start at 0: a constant, which
+  // keeps the products' operands in uniform registers.
+  constexpr uint32_t tmem = 0;
+  if (bars->tmem_base != 0) {  // (cannot happen; the same for the whole CTA)
+    if (threadIdx.x == 0 && atomicCAS(&g_status.code, 0, H3B_ERR_DEVICE) == 0) g_status.site = 31;
+    if (warp == 9) tmem_dealloc(bars->tmem_base, 512);
+    return;
+  }
   auto s_col = [](int i) { return static_cast<uint32_t>(i * 128); };
   auto o_col = [](int i) { return static_cast<uint32_t>(256 + i * 128); };
 
@@ -309,7 +344,7 @@ __global__ void __launch_bounds__(THREADS, 1)
       bool ok = true;
       auto load_q = [&](const Unit& u, int i) {
         const int s = qc % QST;
-        if (qc >= QST && !mbar_wait<false, false, true>(&bars->q_free[s], (qc / QST - 1) & 1, &g_status, 1, abort_flag)) return false;
+        if (qc >= QST && !lane_wait<false>(&bars->q_free[s], (qc / QST - 1) & 1, 1, abort_flag)) return false;
         mbar_arrive_expect_tx(&bars->q_full[s], C::TILE_BYTES);
         for (int h = 0; h < C::HALVES; ++h)
           tma_load_4d(sQ + s * C::TILE_BYTES + h * C::HALF_BYTES, &tm_q, h * 64, u.q0 + i * BQ, u.head, u.b,
@@ -321,7 +356,7 @@ __global__ void __launch_bounds__(THREADS, 1)
       // overwrites V_{t-2}, released with round t - 1 (see the matrix warp).
       auto load_kv = [&](const CUtensorMap* tm, const Unit& u, int j, int s, int round) {
         if (round >= 0 &&
-            !mbar_wait<false, false, true>(&bars->kv_free[round & 1], (round >> 1) & 1, &g_status, 2, abort_flag))
+            !lane_wait<false>(&bars->kv_free[round & 1], (round >> 1) & 1, 2, abort_flag))
           return false;
         mbar_arrive_expect_tx(&bars->kv_full[s], C::TILE_BYTES);
         for (int h = 0; h < C::HALVES; ++h)
@@ -331,7 +366,7 @@ __global__ void __launch_bounds__(THREADS, 1)
       };
       int t = 0, loaded = 0;
 #pragma unroll 1
-      for (; u.x < args.units && ok; u.next(args)) {
+      for (; u.x < args.units && ok; u.next<false>(args)) {
 #pragma unroll 1
         for (int j = 0; j < u.n && ok; ++j, ++t) {
           if (j == 0) ok = load_q(u, 0);
@@ -343,68 +378,60 @@ __global__ void __launch_bounds__(THREADS, 1)
       if (!ok || *abort_flag) {
         // let the copies in flight land (bounded) before the CTA goes
         for (int c = max(0, qc - QST); c < qc; ++c)
-          mbar_wait<false, false, true>(&bars->q_full[c % QST], (c / QST) & 1, &g_status, 10, nullptr);
+          lane_wait<false>(&bars->q_full[c % QST], (c / QST) & 1, 10, nullptr);
         for (int c = max(0, loaded - KVST); c < loaded; ++c)
-          mbar_wait<false, false, true>(&bars->kv_full[c % KVST], (c / KVST) & 1, &g_status, 11, nullptr);
+          lane_wait<false>(&bars->kv_full[c % KVST], (c / KVST) & 1, 11, nullptr);
       }
     } else if (warp == 9) {
       // ------------------------------------------------------------ MMA
       // The warp runs the schedule converged: all lanes poll, one elected
       // lane issues.  Round t of the products is
       //   P V_0(t-1)  S_0(t)  P V_1(t-1)  S_1(t)
-      // and everything that can be waited for or worked out before a P tile
-      // is there (V, K, Q, descriptors, the next unit) comes before the wait
-      // for P: what stands between P and the products behind it is on every
-      // tile's critical path (softmax -> P V -> S -> softmax).  Measured with
-      // those waits behind P V: 5000 cycles a round, 3000 of them with the
-      // softmax warps idle.
+      // What stands between a P tile and the products behind it is on every
+      // tile's critical path (softmax -> P V -> S -> softmax), and this warp
+      // shares its scheduler and instruction cache with softmax warps that
+      // stream through 10 KB of code a tile.  So it only waits for `ready` and
+      // for P, and issues; warp 10 does everything else ahead of it.  (With
+      // the bookkeeping here a round took 5000 cycles, 3000 of them with the
+      // softmax warps idle.)
       // Every barrier waited on completes once per use and its next use
       // depends on what this warp issues after the wait.
-      int qc = 0, j = 0;
       uint32_t phases = 0;  // bit i: parity of row tile i's P; bit 2 + i: of its O; bit 4 + i: O begun once
       bool ok = true;
-      auto wait = [&](uint64_t* bar, uint32_t parity, int site) {
-        ok = mbar_wait<true, false, true>(bar, parity, &g_status, site, abort_flag) && ok;
-      };
-      // of the step whose P V comes in this round
-      bool pv = false, pv_two = false, pv_first = false, pv_last = false;
-      while (u.x < args.units && u.n == 0) u.next(args);
-      bool more = u.x < args.units;
 #pragma unroll 1
-      for (int t = 0; more || pv; ++t) {
-        const bool first = j == 0, last = j == u.n - 1, two = u.two;
-        const uint32_t k_s = smem_u32(sKV + 2 * (t & 1) * C::TILE_BYTES);
-        const uint32_t v_s = smem_u32(sKV + (2 * ((t + 1) & 1) + 1) * C::TILE_BYTES);
-        const uint64_t kd = sdesc_kmajor_sw128(k_s);
-        const uint64_t vd = sdesc_mnmajor_sw128(v_s, C::HALF_BYTES, 1024);
-        if (pv) wait(&bars->v_ready[(t + 1) & 1], ((t - 1) >> 1) & 1, 7);
-        if (more) wait(&bars->kv_full[2 * (t & 1)], (t >> 1) & 1, 4);
+      for (int t = 0; ok; ++t) {
+        ok = lane_wait<true>(&bars->ready[t & 1], (t >> 1) & 1, 4, abort_flag);
+        // (the reduction makes the word uniform for the compiler too)
+        const uint32_t todo = ok ? *const_cast<volatile uint32_t*>(&bars->todo[t & 1]) : static_cast<uint32_t>(R_END);
+        const uint32_t r = __reduce_or_sync(0xffffffffu, todo);
+        const uint64_t kd = sdesc_kmajor_sw128(smem_u32(sKV + 2 * (t & 1) * C::TILE_BYTES));
+        const uint64_t vd =
+            sdesc_mnmajor_sw128(smem_u32(sKV + (2 * ((t + 1) & 1) + 1) * C::TILE_BYTES), C::HALF_BYTES, 1024);
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-          const bool do_pv = pv && (i == 0 || pv_two), do_s = more && (i == 0 || two);
-          const int qs = (qc + i) % QST;
+          const bool do_pv = (r & (i ? R_PV1 : R_PV0)) != 0, do_s = (r & (i ? R_S1 : R_S0)) != 0;
+          const uint32_t qs = (r >> (i ? R_Q1_SHIFT : R_Q0_SHIFT)) & 3u;
           const uint64_t qd = sdesc_kmajor_sw128(smem_u32(sQ + qs * C::TILE_BYTES));
           const uint32_t s_tmem = tmem + s_col(i), o_tmem = tmem + o_col(i);
-          if (do_s && first) wait(&bars->q_full[qs], ((qc + i) / QST) & 1, 3);
           if (do_pv) {
-            if (pv_first) {  // O_i of the unit before has been read (its phase: one a unit)
+            if (r & R_PV_FIRST) {  // O_i of the unit before has been read (its phase: one a unit)
               if ((phases >> (4 + i)) & 1) {
-                wait(&bars->o_free[i], (phases >> (2 + i)) & 1, 6);
+                ok = lane_wait<true>(&bars->o_free[i], (phases >> (2 + i)) & 1, 6, abort_flag) && ok;
                 phases ^= 4u << i;
               }
               phases |= 16u << i;
             }
             // as the softmax delivers: 64 keys a half
-            wait(&bars->p_half[i][0], (phases >> i) & 1, 5);
+            ok = lane_wait<true>(&bars->p_half[i][0], (phases >> i) & 1, 5, abort_flag) && ok;
             __syncwarp();
             tc_fence_after();
             if (elect_one()) {
 #pragma unroll
               for (int kk = 0; kk < 4; ++kk)
                 mma_f16_ts(o_tmem, s_tmem + kk * 8, desc_add_lo(vd, static_cast<uint32_t>(kk * (2048 >> 4))), IDESC_O,
-                           (pv_first && kk == 0) ? 0u : 1u);
+                           kk == 0 ? (~r & R_PV_FIRST) : 1u);
             }
-            wait(&bars->p_half[i][1], (phases >> i) & 1, 5);
+            ok = lane_wait<true>(&bars->p_half[i][1], (phases >> i) & 1, 5, abort_flag) && ok;
             phases ^= 1u << i;
           }
           __syncwarp();
@@ -414,7 +441,7 @@ __global__ void __launch_bounds__(THREADS, 1)
 #pragma unroll
               for (int kk = 4; kk < 8; ++kk)
                 mma_f16_ts(o_tmem, s_tmem + kk * 8, desc_add_lo(vd, static_cast<uint32_t>(kk * (2048 >> 4))), IDESC_O, 1u);
-              if (pv_last) tc_commit(&bars->o_full[i]);
+              if (r & R_PV_LAST) tc_commit(&bars->o_full[i]);
             }
             if (do_s) {
 #pragma unroll
@@ -423,71 +450,88 @@ __global__ void __launch_bounds__(THREADS, 1)
                 mma_f16_ss(s_tmem, desc_add_lo(qd, at), desc_add_lo(kd, at), IDESC_S, kk > 0);
               }
               tc_commit(&bars->s_full[i]);
-              if (last) tc_commit(&bars->q_free[qs]);
+              if (r & R_S_LAST) tc_commit(&bars->q_free[qs]);
             }
             if (i == 1) tc_commit(&bars->kv_free[t & 1]);
           }
           __syncwarp();
         }
-        if (!__all_sync(0xffffffffu, ok)) break;
-        pv = more;
-        pv_two = two;
-        pv_first = first;
-        pv_last = last;
-        if (more && ++j == u.n) {
-          j = 0;
-          qc += two ? 2 : 1;
-          do {
-            u.next(args);
-          } while (u.x < args.units && u.n == 0);
-          more = u.x < args.units;
-        }
+        ok = __all_sync(0xffffffffu, ok) && (r & R_END) == 0;
       }
       if (elect_one()) tc_commit(&bars->drain);
       __syncwarp();
       warp_wait(&bars->drain, 0, 8, nullptr);
     } else if (warp == 10) {
-      // ------------------------------------------------------------ left-out rows of V
-      // Every V tile passes through here, so that this warp is never more than
-      // a phase behind: V_{t+2} is loaded over V_t after P V(t), which waits
-      // for v_ready.  (V is there well before it is needed.)
-      int step = 0;
+      // ------------------------------------------------------------ rounds
+      // Ahead of the issuing warp: says what round t consists of, waits for
+      // K_t, V_{t-1} and at a unit's start its Q tiles, and zeroes the rows of
+      // V_{t-1} that are left out.  It is at most two rounds ahead (K_t
+      // overwrites K_{t-2}, released with round t - 2), so todo[] and ready[]
+      // of that parity are free again, and every tile's barrier is waited for
+      // once: one phase behind.
+      int qc = 0;
+      uint32_t pv = 0;               // R_PV* of the tile before
+      int v_key0 = 0, v_len = 0, v_b = 0;
       bool ok = true;
-      #pragma unroll 1
-      for (; u.x < args.units && ok; u.next(args)) {
+      while (u.x < args.units && u.n == 0) u.next(args);
+      int j = 0;
+      bool end = false;
 #pragma unroll 1
-        for (int j = 0; j < u.n; ++j, ++step) {
-          const int key0 = (u.j0 + j) * BKV;
-          const int slot = 2 * (step & 1) + 1;
-          const uint32_t mb = masked ? mask_bytes(a, u.b, key0, u.len, lane) : 0u;
-          if (!warp_wait(&bars->kv_full[slot], (step >> 1) & 1, 9, abort_flag)) {
-            ok = false;
-            break;
+      for (int t = 0; !end; ++t) {
+        const bool more = u.x < args.units;
+        uint32_t r = pv;
+        if (more) {
+          r |= R_S0 | (u.two ? R_S1 : 0u) | (j == u.n - 1 ? R_S_LAST : 0u) | ((qc % QST) << R_Q0_SHIFT) |
+               (((qc + 1) % QST) << R_Q1_SHIFT);
+          ok = warp_wait(&bars->kv_full[2 * (t & 1)], (t >> 1) & 1, 9, abort_flag);
+          if (j == 0) {
+            ok = ok && warp_wait(&bars->q_full[qc % QST], (qc / QST) & 1, 3, abort_flag);
+            if (u.two) ok = ok && warp_wait(&bars->q_full[(qc + 1) % QST], ((qc + 1) / QST) & 1, 3, abort_flag);
           }
-          if (masked || key0 + BKV > u.len) {
+        }
+        if (pv != 0) {
+          const uint32_t mb = masked ? mask_bytes(a, v_b, v_key0, v_len, lane) : 0u;
+          ok = ok && warp_wait(&bars->kv_full[2 * ((t + 1) & 1) + 1], ((t - 1) >> 1) & 1, 7, abort_flag);
+          if (ok && (masked || v_key0 + BKV > v_len)) {
             uint32_t w[4];
-            keep_words(masked, mb, u.len - key0, w);
+            keep_words(masked, mb, v_len - v_key0, w);
             // (a row's 16-byte pieces keep their row under the swizzle)
-            const uint32_t v = smem_u32(sKV + slot * C::TILE_BYTES);
+            const uint32_t v = smem_u32(sKV + (2 * ((t + 1) & 1) + 1) * C::TILE_BYTES);
             const int piece = lane & 7;
+#pragma unroll 1
+            for (int r4 = 0; r4 < BKV; r4 += 4) {
+              const int row = r4 + (lane >> 3);
+              const uint32_t keep = r4 < 64 ? (r4 < 32 ? w[0] : w[1]) : (r4 < 96 ? w[2] : w[3]);
+              if (((keep >> (row & 31)) & 1u) == 0) {
 #pragma unroll
-            for (int c = 0; c < 4; ++c) {
-              if (w[c] == 0xffffffffu) continue;
-              for (int r = lane >> 3; r < 32; r += 4)
-                if (((w[c] >> r) & 1u) == 0) {
-#pragma unroll
-                  for (int h = 0; h < C::HALVES; ++h)
-                    asm volatile("st.shared.v4.u32 [%0], {%1,%1,%1,%1};" ::"r"(v + h * C::HALF_BYTES + (c * 32 + r) * 128 +
-                                                                               piece * 16),
-                                 "r"(0u)
-                                 : "memory");
-                }
+                for (int h = 0; h < C::HALVES; ++h)
+                  asm volatile("st.shared.v4.u32 [%0], {%1,%1,%1,%1};" ::"r"(v + h * C::HALF_BYTES + row * 128 + piece * 16),
+                               "r"(0u)
+                               : "memory");
+              }
             }
             fence_proxy_async_smem();
-            __syncwarp();
           }
-          if (lane == 0) mbar_arrive(&bars->v_ready[step & 1]);
         }
+        if (!ok) break;
+        pv = 0;
+        if (more) {
+          pv = R_PV0 | (u.two ? R_PV1 : 0u) | (j == 0 ? R_PV_FIRST : 0u) | (j == u.n - 1 ? R_PV_LAST : 0u);
+          v_key0 = (u.j0 + j) * BKV;
+          v_len = u.len;
+          v_b = u.b;
+          if (++j == u.n) {
+            j = 0;
+            qc += u.two ? 2 : 1;
+            do {
+              u.next(args);
+            } while (u.x < args.units && u.n == 0);
+          }
+        }
+        end = pv == 0;
+        if (lane == 0) *const_cast<volatile uint32_t*>(&bars->todo[t & 1]) = r | (end ? R_END : 0u);
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&bars->ready[t & 1]);
       }
     }
   } else if (warp < 8) {
@@ -602,7 +646,7 @@ __global__ void __launch_bounds__(THREADS, 1)
       }
       if (!ok) break;
       // ---- the row statistics, to the storing warps
-      if (oc > 0 && !warp_wait(&bars->ml_free[wg], (oc - 1) & 1, 22, abort_flag)) {
+      if (oc > 0 && !warp_wait<true>(&bars->ml_free[wg], (oc - 1) & 1, 22, abort_flag)) {
         ok = false;
         break;
       }
