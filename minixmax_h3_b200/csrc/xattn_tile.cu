@@ -48,9 +48,9 @@ constexpr int QST = 3;   // Q ring (128-row tiles)
 constexpr int KVST = 4;  // K/V ring (K_s in slots 0, 2, V_s in 1, 3)
 constexpr int THREADS = 512;
 constexpr int REGS_LAUNCH = 128;
-constexpr int REGS_CONTROL = 88;
-constexpr int REGS_STORE = 72;
-constexpr int REGS_SOFTMAX = 176;
+constexpr int REGS_CONTROL = 64;
+constexpr int REGS_STORE = 112;
+constexpr int REGS_SOFTMAX = 168;
 static_assert(128 * (REGS_CONTROL + REGS_STORE + 2 * REGS_SOFTMAX) <= THREADS * REGS_LAUNCH,
               "register split exceeds launch");
 constexpr float RESCALE_THRESHOLD = 8.0f;
@@ -78,7 +78,18 @@ enum : uint32_t {
   R_Q1_SHIFT = 10
 };
 
-struct __align__(8) Bars {
+// What the softmax warps of a row tile have to know of a tile, by warp 10.
+struct __align__(16) TileInfo {
+  uint32_t keep[4];  // kept columns
+  uint32_t flags;    // T_*
+  int causal;        // row 0 of the 128 sees columns < causal (T_CAUSAL)
+  uint32_t pad[2];
+};
+enum : uint32_t { T_FIRST = 1, T_LAST = 2, T_WHOLE = 4, T_CAUSAL = 8, T_END = 16 };
+constexpr int INFOS = 4;  // ring: entry s + 4 is written after round s + 2, so after P(s + 1)
+
+struct __align__(16) Bars {
+  TileInfo info[2][INFOS];
   uint64_t q_full[QST];
   uint64_t q_free[QST];
   uint64_t kv_full[KVST];
@@ -452,6 +463,7 @@ __global__ void __launch_bounds__(THREADS, 1)
               tc_commit(&bars->s_full[i]);
               if (r & R_S_LAST) tc_commit(&bars->q_free[qs]);
             }
+            if (r & R_END) tc_commit(&bars->s_full[i]);  // info says that there is no tile
             if (i == 1) tc_commit(&bars->kv_free[t & 1]);
           }
           __syncwarp();
@@ -470,8 +482,9 @@ __global__ void __launch_bounds__(THREADS, 1)
       // of that parity are free again, and every tile's barrier is waited for
       // once: one phase behind.
       int qc = 0;
-      uint32_t pv = 0;               // R_PV* of the tile before
-      int v_key0 = 0, v_len = 0, v_b = 0;
+      uint32_t pv = 0;                  // R_PV* of the tile before
+      uint32_t vw[4] = {0, 0, 0, 0};    // its kept columns
+      uint32_t ic[2] = {0, 0};          // infos written, per row tile
       bool ok = true;
       while (u.x < args.units && u.n == 0) u.next(args);
       int j = 0;
@@ -479,8 +492,11 @@ __global__ void __launch_bounds__(THREADS, 1)
 #pragma unroll 1
       for (int t = 0; !end; ++t) {
         const bool more = u.x < args.units;
+        const int key0 = (u.j0 + j) * BKV;
         uint32_t r = pv;
+        uint32_t w[4] = {~0u, ~0u, ~0u, ~0u};
         if (more) {
+          const uint32_t mb = masked ? mask_bytes(a, u.b, key0, u.len, lane) : 0u;
           r |= R_S0 | (u.two ? R_S1 : 0u) | (j == u.n - 1 ? R_S_LAST : 0u) | ((qc % QST) << R_Q0_SHIFT) |
                (((qc + 1) % QST) << R_Q1_SHIFT);
           ok = warp_wait(&bars->kv_full[2 * (t & 1)], (t >> 1) & 1, 9, abort_flag);
@@ -488,20 +504,18 @@ __global__ void __launch_bounds__(THREADS, 1)
             ok = ok && warp_wait(&bars->q_full[qc % QST], (qc / QST) & 1, 3, abort_flag);
             if (u.two) ok = ok && warp_wait(&bars->q_full[(qc + 1) % QST], ((qc + 1) / QST) & 1, 3, abort_flag);
           }
+          keep_words(masked, mb, u.len - key0, w);
         }
         if (pv != 0) {
-          const uint32_t mb = masked ? mask_bytes(a, v_b, v_key0, v_len, lane) : 0u;
           ok = ok && warp_wait(&bars->kv_full[2 * ((t + 1) & 1) + 1], ((t - 1) >> 1) & 1, 7, abort_flag);
-          if (ok && (masked || v_key0 + BKV > v_len)) {
-            uint32_t w[4];
-            keep_words(masked, mb, v_len - v_key0, w);
+          if (ok && (vw[0] & vw[1] & vw[2] & vw[3]) != ~0u) {
             // (a row's 16-byte pieces keep their row under the swizzle)
             const uint32_t v = smem_u32(sKV + (2 * ((t + 1) & 1) + 1) * C::TILE_BYTES);
             const int piece = lane & 7;
 #pragma unroll 1
             for (int r4 = 0; r4 < BKV; r4 += 4) {
               const int row = r4 + (lane >> 3);
-              const uint32_t keep = r4 < 64 ? (r4 < 32 ? w[0] : w[1]) : (r4 < 96 ? w[2] : w[3]);
+              const uint32_t keep = r4 < 64 ? (r4 < 32 ? vw[0] : vw[1]) : (r4 < 96 ? vw[2] : vw[3]);
               if (((keep >> (row & 31)) & 1u) == 0) {
 #pragma unroll
                 for (int h = 0; h < C::HALVES; ++h)
@@ -514,22 +528,37 @@ __global__ void __launch_bounds__(THREADS, 1)
           }
         }
         if (!ok) break;
+        const int causal = a.causal ? u.len - a.s_q + u.q0 + 1 - key0 : BKV;
+        const uint32_t flags = (j == 0 ? T_FIRST : 0u) | (j == u.n - 1 ? T_LAST : 0u) |
+                               ((w[0] & w[1] & w[2] & w[3]) == ~0u ? T_WHOLE : 0u);
         pv = 0;
+        const bool two = u.two;
         if (more) {
-          pv = R_PV0 | (u.two ? R_PV1 : 0u) | (j == 0 ? R_PV_FIRST : 0u) | (j == u.n - 1 ? R_PV_LAST : 0u);
-          v_key0 = (u.j0 + j) * BKV;
-          v_len = u.len;
-          v_b = u.b;
+          pv = R_PV0 | (two ? R_PV1 : 0u) | (j == 0 ? R_PV_FIRST : 0u) | (j == u.n - 1 ? R_PV_LAST : 0u);
           if (++j == u.n) {
             j = 0;
-            qc += u.two ? 2 : 1;
+            qc += two ? 2 : 1;
             do {
               u.next(args);
             } while (u.x < args.units && u.n == 0);
           }
         }
         end = pv == 0;
+        if (lane < 2 && (lane == 0 || two || end)) {
+          volatile TileInfo* info = &bars->info[lane][(lane ? ic[1] : ic[0]) % INFOS];
+          const int sees = causal + lane * BQ;
+          info->keep[0] = w[0];
+          info->keep[1] = w[1];
+          info->keep[2] = w[2];
+          info->keep[3] = w[3];
+          info->causal = sees;
+          info->flags = end ? static_cast<uint32_t>(T_END) : sees < BKV ? (flags & ~T_WHOLE) | T_CAUSAL : flags;
+        }
+        ++ic[0];
+        if (two) ++ic[1];
         if (lane == 0) *const_cast<volatile uint32_t*>(&bars->todo[t & 1]) = r | (end ? R_END : 0u);
+#pragma unroll
+        for (int c = 0; c < 4; ++c) vw[c] = w[c];
         __syncwarp();
         if (lane == 0) mbar_arrive(&bars->ready[t & 1]);
       }
@@ -542,41 +571,33 @@ __global__ void __launch_bounds__(THREADS, 1)
     const uint32_t lane_off = static_cast<uint32_t>((warp & 3) * 32) << 16;
     const uint32_t s_tmem = tmem + s_col(wg) + lane_off;
     const uint32_t o_tmem = tmem + o_col(wg) + lane_off;
-    uint32_t sc = 0, oc = 0;  // S tiles, units seen
-    bool ok = true;
-    #pragma unroll 1
-    for (; u.x < args.units && ok; u.next(args)) {
-      if (u.n == 0 || (wg == 1 && !u.two)) continue;
-      float m_run = -INFINITY;  // running max, log2 domain
-      float l_run = 0.0f;
+    float m_run = -INFINITY;  // running max, log2 domain
+    float l_run = 0.0f;
+    uint32_t oc = 0;  // units seen
 #pragma unroll 1
-      for (int j = 0; j < u.n; ++j, ++sc) {
-        const int key0 = (u.j0 + j) * BKV;
-        // which columns are kept: known before S is
-        uint32_t w[4];
-        keep_words(masked, masked ? mask_bytes(a, u.b, key0, u.len, lane) : 0u, u.len - key0, w);
-        bool whole = (w[0] & w[1] & w[2] & w[3]) == 0xffffffffu;
-        if (a.causal && u.len - a.s_q + u.q0 + wg * BQ + 1 < key0 + BKV) {
-          const int valid = u.len - a.s_q + u.q0 + wg * BQ + row + 1 - key0;
-#pragma unroll
-          for (int c = 0; c < 4; ++c) {
-            const int v = valid - 32 * c;
-            w[c] &= v >= 32 ? 0xffffffffu : (v <= 0 ? 0u : (1u << v) - 1u);
-          }
-          whole = false;
-        }
+    for (uint32_t sc = 0;; ++sc) {
+      {
         // S_i of the next tile is published only after this tile's P_i
-        if (!warp_wait<true>(&bars->s_full[wg], sc & 1, 20, abort_flag)) {
-          ok = false;
-          break;
-        }
+        if (!warp_wait<true>(&bars->s_full[wg], sc & 1, 20, abort_flag)) break;
         tc_fence_after();
-        if (!whole) {
+        const volatile TileInfo* info = &bars->info[wg][sc % INFOS];
+        const uint32_t flags = info->flags;
+        if (flags & T_END) break;
+        const bool first = (flags & T_FIRST) != 0;
+        if (first) {
+          m_run = -INFINITY;
+          l_run = 0.0f;
+        }
+        if ((flags & T_WHOLE) == 0) {
           // Left-out columns become -inf in TMEM, 32 at a time in a loop that
           // stays out of the instruction cache of whole tiles.
 #pragma unroll 1
           for (int c = 0; c < 4; ++c) {
-            const uint32_t keep = c < 2 ? (c == 0 ? w[0] : w[1]) : (c == 2 ? w[2] : w[3]);
+            uint32_t keep = info->keep[c];
+            if (flags & T_CAUSAL) {
+              const int v = info->causal + row - 32 * c;
+              keep &= v >= 32 ? 0xffffffffu : (v <= 0 ? 0u : (1u << v) - 1u);
+            }
             if (__all_sync(0xffffffffu, keep == 0xffffffffu)) continue;
             uint32_t o[32];
             tmem_ld32p(s_tmem + c * 32, o);
@@ -596,7 +617,7 @@ __global__ void __launch_bounds__(THREADS, 1)
         uint32_t r[128];
         float m_use = m_run;
         float sum = 0.0f;
-        bool slow = j == 0;
+        bool slow = first;
 #pragma unroll 1
         for (int round = 0; round < 2; ++round) {
 #pragma unroll
@@ -609,7 +630,7 @@ __global__ void __launch_bounds__(THREADS, 1)
             if (__any_sync(0xffffffffu, rescale)) {
               const float factor = rescale ? ex2(m_run - m_use) : 1.0f;
               l_run *= factor;
-              if (j > 0) {
+              if (!first) {
 #pragma unroll 1
                 for (int c = 0; c < D / 8; ++c) {  // (few registers: the tile's scores stay live)
                   uint32_t o[8];
@@ -643,17 +664,15 @@ __global__ void __launch_bounds__(THREADS, 1)
           if (lane == 0) mbar_arrive(&bars->p_half[wg][h]);
         }
         l_run += sum;
+        if (flags & T_LAST) {
+          // ---- the row statistics, to the storing warps
+          if (oc > 0 && !warp_wait<true>(&bars->ml_free[wg], (oc - 1) & 1, 22, abort_flag)) break;
+          ++oc;
+          s_ml[wg * 128 + row] = make_float2(m_run, l_run);
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&bars->ml_full[wg]);
+        }
       }
-      if (!ok) break;
-      // ---- the row statistics, to the storing warps
-      if (oc > 0 && !warp_wait<true>(&bars->ml_free[wg], (oc - 1) & 1, 22, abort_flag)) {
-        ok = false;
-        break;
-      }
-      ++oc;
-      s_ml[wg * 128 + row] = make_float2(m_run, l_run);
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&bars->ml_full[wg]);
     }
   } else {
     // ------------------------------------------------------------ stores
@@ -662,6 +681,16 @@ __global__ void __launch_bounds__(THREADS, 1)
     const uint32_t lane_off = static_cast<uint32_t>((warp & 3) * 32) << 16;
     const int64_t total_rows = static_cast<int64_t>(a.batch) * a.heads * a.s_q;
     uint32_t oc0 = 0, oc1 = 0;
+    auto release = [&](int i, int n) {  // O_i and the statistics are read
+      if (n > 0) {
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) {
+          mbar_arrive(&bars->o_free[i]);
+          mbar_arrive(&bars->ml_free[i]);
+        }
+      }
+    };
     bool ok = true;
     #pragma unroll 1
     for (; u.x < args.units && ok; u.next(args)) {
@@ -671,7 +700,7 @@ __global__ void __launch_bounds__(THREADS, 1)
         float2 ml = make_float2(-INFINITY, 0.0f);
         const uint32_t phase = (i ? oc1 : oc0) & 1;
         if (u.n > 0) {
-          // both complete once a unit, and again only after this warp's arrivals below
+          // both complete once a unit, and again only after this warp's release
           ok = warp_wait(&bars->ml_full[i], phase, 23, abort_flag) &&
                warp_wait(&bars->o_full[i], phase, 24, abort_flag);
           if (!ok) continue;
@@ -683,54 +712,64 @@ __global__ void __launch_bounds__(THREADS, 1)
         const bool in = q_row < a.s_q;
         const int64_t lse_row = (static_cast<int64_t>(u.b) * a.heads + u.head) * a.s_q + q_row;
         const float inv_l = ml.y > 0.0f ? 1.0f / ml.y : 0.0f;
-        uint16_t* orow =
-            static_cast<uint16_t*>(a.o) + u.b * a.o_stride[0] + q_row * a.o_stride[1] + u.head * a.o_stride[2];
-        float* prow = a.part_o + (u.split * total_rows + lse_row) * D;
+        if (a.splits > 1) {
+          float* prow = a.part_o + (u.split * total_rows + lse_row) * D;
 #pragma unroll 1
-        for (int c = 0; c < D / 32; ++c) {
-          uint32_t r[32];
-          if (u.n > 0) {
-            tmem_ld32p(tmem + o_col(i) + c * 32 + lane_off, r);
-            tmem_wait_fence<1>(r);
-            if (c == D / 32 - 1) {  // O_i and the statistics are read
-              tc_fence_before();
-              __syncwarp();
-              if (lane == 0) {
-                mbar_arrive(&bars->o_free[i]);
-                mbar_arrive(&bars->ml_free[i]);
-              }
+          for (int c = 0; c < D / 32; ++c) {
+            uint32_t r[32];
+            if (u.n > 0) {
+              tmem_ld32p(tmem + o_col(i) + c * 32 + lane_off, r);
+              tmem_wait_fence<1>(r);
+            } else {
+#pragma unroll
+              for (int e = 0; e < 32; ++e) r[e] = 0u;
             }
-          } else {
+            if (in) {
 #pragma unroll
-            for (int e = 0; e < 32; ++e) r[e] = 0u;
-          }
-          if (in && a.splits > 1) {
-#pragma unroll
-            for (int e = 0; e < 32; e += 8) {
-              uint32_t v[8];
-#pragma unroll
-              for (int t = 0; t < 8; ++t) v[t] = r[e + t];
-              st_global_v8(prow + c * 32 + e, v);
-            }
-          } else if (in) {
-#pragma unroll
-            for (int e = 0; e < 16; ++e)
-              r[e] = pack16x2<F16>(__uint_as_float(r[2 * e]) * inv_l, __uint_as_float(r[2 * e + 1]) * inv_l);
-            if (args.o_wide) {
-#pragma unroll
-              for (int e = 0; e < 16; e += 8) {
+              for (int e = 0; e < 32; e += 8) {
                 uint32_t v[8];
 #pragma unroll
                 for (int t = 0; t < 8; ++t) v[t] = r[e + t];
-                st_global_v8(orow + c * 32 + 2 * e, v);
+                st_global_v8(prow + c * 32 + e, v);
               }
-            } else {
-#pragma unroll
-              for (int e = 0; e < 16; e += 4)
-                *reinterpret_cast<uint4*>(orow + c * 32 + 2 * e) = make_uint4(r[e], r[e + 1], r[e + 2], r[e + 3]);
             }
+            __syncwarp();  // the next tcgen05.ld is for the whole warp
           }
-          __syncwarp();  // the next tcgen05.ld is for the whole warp
+          release(i, u.n);
+        } else {
+          // O is read and rounded into half the registers, given back, and
+          // only then stored: the next unit's first P V waits for it.
+          uint32_t p[D / 2];
+          if (u.n > 0) {
+#pragma unroll
+            for (int c = 0; c < D / 32; ++c) {
+              uint32_t r[32];
+              tmem_ld32p(tmem + o_col(i) + c * 32 + lane_off, r);
+              tmem_wait_fence<1>(r);
+#pragma unroll
+              for (int e = 0; e < 16; ++e)
+                p[16 * c + e] = pack16x2<F16>(__uint_as_float(r[2 * e]) * inv_l, __uint_as_float(r[2 * e + 1]) * inv_l);
+            }
+          } else {
+#pragma unroll
+            for (int e = 0; e < D / 2; ++e) p[e] = 0u;
+          }
+          release(i, u.n);
+          uint16_t* orow =
+              static_cast<uint16_t*>(a.o) + u.b * a.o_stride[0] + q_row * a.o_stride[1] + u.head * a.o_stride[2];
+          if (in && args.o_wide) {
+#pragma unroll
+            for (int e = 0; e < D / 2; e += 8) {
+              uint32_t v[8];
+#pragma unroll
+              for (int t = 0; t < 8; ++t) v[t] = p[e + t];
+              st_global_v8(orow + 2 * e, v);
+            }
+          } else if (in) {
+#pragma unroll
+            for (int e = 0; e < D / 2; e += 4)
+              *reinterpret_cast<uint4*>(orow + 2 * e) = make_uint4(p[e], p[e + 1], p[e + 2], p[e + 3]);
+          }
         }
         if (in) {
           if (a.splits > 1) {
