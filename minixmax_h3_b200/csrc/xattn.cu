@@ -31,7 +31,7 @@ int64_t rows_of(const XAttn& a) { return static_cast<int64_t>(a.batch) * a.heads
 
 // Which kernel: the tile kernel works on 128 rows of one head whether they
 // exist or not; the row kernel on 32 rows of the heads that share a key head.
-bool by_tiles(const XAttn& a) { return a.kind == h3b::KV_DENSE && a.s_q >= 64; }
+bool by_tiles(const XAttn& a) { return a.s_q >= 64; }
 
 void plan(XAttn& a) { a.splits = by_tiles(a) ? h3b::xattn_tile_splits(a) : h3b::xattn_rows_splits(a); }
 

@@ -41,10 +41,13 @@ H3B_REGISTER_STATUS_READER(xattn_tile);
 
 namespace {
 
+using h3b::KV_DENSE;
+using h3b::KV_E4M3;
+using h3b::KV_INT8;
+using h3b::KvKind;
 using h3b::XAttn;
 
 constexpr int BQ = 128, BKV = 128;
-constexpr int QST = 3;   // Q ring (128-row tiles)
 constexpr int KVST = 4;  // K/V ring (K_s in slots 0, 2, V_s in 1, 3)
 constexpr int THREADS = 512;
 constexpr int REGS_LAUNCH = 128;
@@ -57,8 +60,13 @@ constexpr float RESCALE_THRESHOLD = 8.0f;
 constexpr float LOG2E = 1.4426950408889634f;
 constexpr float LN2 = 0.69314718055994531f;
 
-template <int D>
+template <int D, KvKind KIND>
 struct Cfg {
+  static constexpr bool CODES = KIND != KV_DENSE;
+  // Q ring (128-row tiles).  Over a cache a unit is long, and the codes' own
+  // two tiles take the room of the third slot.
+  static constexpr int QST = CODES ? 2 : 3;
+  static constexpr int RAW_BYTES = CODES ? 128 * D : 0;  // codes of a K or V tile
   static constexpr int HALVES = D / 64;            // 64-column TMA boxes of a tile
   static constexpr int TILE_BYTES = 128 * D * 2;   // Q, K or V
   static constexpr int HALF_BYTES = 128 * 64 * 2;  // 16 KB
@@ -84,14 +92,19 @@ struct __align__(16) TileInfo {
   uint32_t flags;    // T_*
   int causal;        // row 0 of the 128 sees columns < causal (T_CAUSAL)
   uint32_t pad[2];
+  // cache, by 32 columns: score factor (log2 domain), log2 and reciprocal of
+  // the values' scale
+  float k_factor[4], v_log2[4], v_inv[4];
 };
 enum : uint32_t { T_FIRST = 1, T_LAST = 2, T_WHOLE = 4, T_CAUSAL = 8, T_END = 16 };
 constexpr int INFOS = 4;  // ring: entry s + 4 is written after round s + 2, so after P(s + 1)
 
 struct __align__(16) Bars {
   TileInfo info[2][INFOS];
-  uint64_t q_full[QST];
-  uint64_t q_free[QST];
+  uint64_t q_full[3];
+  uint64_t q_free[3];
+  uint64_t raw_full[2];   // codes of K, of V
+  uint64_t raw_free[2];   // converted (4 warps)
   uint64_t kv_full[KVST];
   uint64_t kv_free[2];    // by round parity: round t of the products has read V_{t-1} and K_t
   uint64_t s_full[2];
@@ -107,11 +120,12 @@ struct __align__(16) Bars {
   int abort_flag;
 };
 
-template <int D>
+template <int D, KvKind KIND>
 constexpr size_t smem_bytes() {
-  return (QST + KVST) * Cfg<D>::TILE_BYTES + 2 * 128 * sizeof(float2) + sizeof(Bars);
+  using C = Cfg<D, KIND>;
+  return (C::QST + KVST) * C::TILE_BYTES + 2 * C::RAW_BYTES + 2 * 128 * sizeof(float2) + sizeof(Bars);
 }
-static_assert(smem_bytes<128>() <= 232448, "shared memory of a CTA");
+static_assert(smem_bytes<128, KV_DENSE>() <= 232448 && smem_bytes<128, KV_INT8>() <= 232448, "shared memory of a CTA");
 
 struct TileArgs {
   XAttn a;
@@ -227,6 +241,18 @@ H3B_DEV void tmem_st8(uint32_t taddr, const uint32_t (&r)[8]) {
                : "memory");
 }
 
+H3B_DEV float row_max32(const uint32_t* r) {
+  float mx[4];
+#pragma unroll
+  for (int c = 0; c < 4; ++c) mx[c] = __uint_as_float(r[c]);
+#pragma unroll
+  for (int e = 4; e < 28; e += 8)
+#pragma unroll
+    for (int c = 0; c < 4; ++c) mx[c] = fmax3(mx[c], __uint_as_float(r[e + c]), __uint_as_float(r[e + 4 + c]));
+#pragma unroll
+  for (int c = 0; c < 4; ++c) mx[c] = fmaxf(mx[c], __uint_as_float(r[28 + c]));
+  return fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+}
 H3B_DEV float row_max64(const uint32_t* r) {
   float mx[8];
 #pragma unroll
@@ -276,11 +302,122 @@ H3B_DEV float2 exp_pack64(uint32_t* r, uint32_t* dst, float scale_log2, float ne
   return make_float2(t.x + t.y, m);
 }
 
-template <int D, bool F16>
+// The same for a cache's columns, whose factor and exponent offset change
+// every 32: sc and nm are those of the two groups of r[0..63], the sum is
+// weighted by inv.  With MAX the largest exponent of the 128 scores is found
+// (factors fx, offsets ox of the four groups).
+template <bool F16, bool MAX>
+H3B_DEV float2 exp_codes64(uint32_t* r, uint32_t* dst, float2 sc, float2 nm, float2 inv, const float (&fx)[4],
+                           const float (&ox)[4]) {
+  float top = -INFINITY;
+  if constexpr (MAX) {
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+      for (int e = 0; e < 32; e += 2)
+        mx[(e >> 1) & 3] = fmax3(mx[(e >> 1) & 3], __uint_as_float(r[32 * g + e]), __uint_as_float(r[32 * g + e + 1]));
+      top = fmaxf(top, fmaf(fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])), fx[g], ox[g]));
+    }
+  }
+  float sum = 0.0f;
+#pragma unroll
+  for (int g = 0; g < 2; ++g) {
+    const float f = g ? sc.y : sc.x, o = g ? nm.y : nm.x;
+    float2 acc[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+#pragma unroll
+    for (int e = 16 * g; e < 16 * g + 16; ++e) {
+      const float2 x = fma2(make_float2(__uint_as_float(r[2 * e]), __uint_as_float(r[2 * e + 1])), make_float2(f, f),
+                            make_float2(o, o));
+      const float2 w = make_float2(ex2(x.x), ex2(x.y));
+      acc[e & 1] = add2(acc[e & 1], w);
+      dst[e] = pack16x2<F16>(w.x, w.y);
+    }
+    const float2 t = add2(acc[0], acc[1]);
+    sum = fmaf(t.x + t.y, g ? inv.y : inv.x, sum);
+  }
+  return make_float2(sum, top);
+}
+
+// Four codes -> two packed pairs of the operands' type, exactly.
+template <KvKind KIND, bool F16>
+H3B_DEV void codes4(uint32_t w, uint32_t& lo, uint32_t& hi) {
+  if constexpr (KIND == KV_INT8) {
+    w ^= 0x80808080u;
+    if constexpr (F16) {  // 0x6400 | u is 1024 + u in f16
+      const uint32_t a = __byte_perm(w, 0x64646464u, 0x5140), b = __byte_perm(w, 0x64646464u, 0x5342);
+      const __half2 c = __half2half2(__ushort_as_half(0x6480));  // 1152
+      const __half2 x = __hsub2(*reinterpret_cast<const __half2*>(&a), c);
+      const __half2 y = __hsub2(*reinterpret_cast<const __half2*>(&b), c);
+      lo = *reinterpret_cast<const uint32_t*>(&x);
+      hi = *reinterpret_cast<const uint32_t*>(&y);
+    } else {  // 0x4B000000 | u is 2^23 + u in fp32
+      const float2 c = make_float2(-8388736.0f, -8388736.0f);
+      const float2 x = add2(make_float2(__uint_as_float(__byte_perm(w, 0x4B000000u, 0x7440)),
+                                        __uint_as_float(__byte_perm(w, 0x4B000000u, 0x7441))), c);
+      const float2 y = add2(make_float2(__uint_as_float(__byte_perm(w, 0x4B000000u, 0x7442)),
+                                        __uint_as_float(__byte_perm(w, 0x4B000000u, 0x7443))), c);
+      lo = pack_bf16x2(x.x, x.y);
+      hi = pack_bf16x2(y.x, y.y);
+    }
+  } else {
+    uint32_t a, b;
+    asm("{\n\t.reg .b16 l, h;\n\tmov.b32 {l, h}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, l;\n\tcvt.rn.f16x2.e4m3x2 %1, h;\n\t}"
+        : "=r"(a), "=r"(b)
+        : "r"(w));
+    if constexpr (F16) {
+      lo = a;
+      hi = b;
+    } else {
+      const float2 x = __half22float2(*reinterpret_cast<const __half2*>(&a));
+      const float2 y = __half22float2(*reinterpret_cast<const __half2*>(&b));
+      lo = pack_bf16x2(x.x, x.y);
+      hi = pack_bf16x2(y.x, y.y);
+    }
+  }
+}
+
+// One row of a tile of codes (128 rows, TMA swizzle) as 16-bit operands in
+// the two 64-column halves that the products read (128-byte swizzle).
+template <int D, KvKind KIND, bool F16>
+H3B_DEV void convert_row(uint32_t raw, uint32_t dst, int row, bool keep) {
+#pragma unroll 2
+  for (int c = 0; c < D / 16; ++c) {
+    const uint32_t at = D == 128 ? row * 128 + ((c ^ (row & 7)) << 4) : row * 64 + ((c ^ ((row >> 1) & 3)) << 4);
+    uint32_t w[4];
+    asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "r"(raw + at) : "memory");
+    uint32_t v[8];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) codes4<KIND, F16>(w[k], v[2 * k], v[2 * k + 1]);
+    if (!keep) {
+#pragma unroll
+      for (int k = 0; k < 8; ++k) v[k] = 0u;
+    }
+    const uint32_t half = dst + (c >> 2) * (128 * 128) + row * 128;
+    const int p = 2 * (c & 3);
+#pragma unroll
+    for (int k = 0; k < 2; ++k)
+      asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(half + (((p + k) ^ (row & 7)) << 4)), "r"(v[4 * k]),
+                   "r"(v[4 * k + 1]), "r"(v[4 * k + 2]), "r"(v[4 * k + 3])
+                   : "memory");
+  }
+}
+
+// The cache's block of a key, -1 if there is none.
+H3B_DEV int block_of(const XAttn& a, int b, int key) {
+  const int j = key / a.block_tokens;
+  if (j >= a.max_blocks) return -1;
+  const int id = __ldg(a.table + static_cast<int64_t>(b) * a.max_blocks + j);
+  return id >= 0 && id < a.num_blocks ? id : -1;
+}
+
+template <int D, bool F16, KvKind KIND>
 __global__ void __launch_bounds__(THREADS, 1)
     xattn_tile_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
                       const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ TileArgs args) {
-  using C = Cfg<D>;
+  using C = Cfg<D, KIND>;
+  constexpr bool CODES = C::CODES;
+  constexpr int QST = C::QST;
   constexpr uint32_t IDESC_S = F16 ? idesc_f16_f32(128, BKV, 0, 0) : idesc_bf16_f32(128, BKV, 0, 0);
   constexpr uint32_t IDESC_O = F16 ? idesc_f16_f32(128, D, 0, 1) : idesc_bf16_f32(128, D, 0, 1);
   extern __shared__ __align__(1024) uint8_t smem_tiles[];
@@ -290,7 +427,8 @@ __global__ void __launch_bounds__(THREADS, 1)
   }
   uint8_t* sQ = smem_tiles;
   uint8_t* sKV = sQ + QST * C::TILE_BYTES;
-  float2* s_ml = reinterpret_cast<float2*>(sKV + KVST * C::TILE_BYTES);  // [2][128]
+  uint8_t* sRaw = sKV + KVST * C::TILE_BYTES;  // codes of K | V
+  float2* s_ml = reinterpret_cast<float2*>(sRaw + 2 * C::RAW_BYTES);  // [2][128]
   Bars* bars = reinterpret_cast<Bars*>(s_ml + 2 * 128);
   const XAttn& a = args.a;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -302,7 +440,11 @@ __global__ void __launch_bounds__(THREADS, 1)
       mbar_init(&bars->q_full[i], 1);
       mbar_init(&bars->q_free[i], 1);
     }
-    for (int i = 0; i < KVST; ++i) mbar_init(&bars->kv_full[i], 1);
+    for (int i = 0; i < KVST; ++i) mbar_init(&bars->kv_full[i], CODES ? 4 : 1);  // 4 converting warps, or TMA
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&bars->raw_full[i], 1);
+      mbar_init(&bars->raw_free[i], 4);
+    }
     for (int i = 0; i < 2; ++i) {
       mbar_init(&bars->kv_free[i], 1);
       mbar_init(&bars->s_full[i], 1);
@@ -365,14 +507,26 @@ __global__ void __launch_bounds__(THREADS, 1)
       };
       // K_t overwrites K_{t-2}, released with round t - 2 of the products; V_t
       // overwrites V_{t-2}, released with round t - 1 (see the matrix warp).
-      auto load_kv = [&](const CUtensorMap* tm, const Unit& u, int j, int s, int round) {
-        if (round >= 0 &&
-            !lane_wait<false>(&bars->kv_free[round & 1], (round >> 1) & 1, 2, abort_flag))
-          return false;
-        mbar_arrive_expect_tx(&bars->kv_full[s], C::TILE_BYTES);
-        for (int h = 0; h < C::HALVES; ++h)
-          tma_load_4d(sKV + s * C::TILE_BYTES + h * C::HALF_BYTES, tm, h * 64, (u.j0 + j) * BKV,
-                      args.group == 1 ? u.head : u.head / args.group, u.b, &bars->kv_full[s]);
+      auto load_kv = [&](const CUtensorMap* tm, const Unit& u, int j, int t, int v) {
+        const int kvh = args.group == 1 ? u.head : u.head / args.group;
+        const int key0 = (u.j0 + j) * BKV;
+        if constexpr (CODES) {
+          // codes: slot v, converted once a tile
+          if (t > 0 && !lane_wait<false>(&bars->raw_free[v], (t - 1) & 1, 2, abort_flag)) return false;
+          mbar_arrive_expect_tx(&bars->raw_full[v], C::RAW_BYTES);
+          const int rows = min(a.block_tokens, BKV);
+          for (int r = 0; r < BKV; r += rows) {
+            // (an absent block loads block 0: it may hold anything, see warp 10)
+            const int id = max(block_of(a, u.b, key0 + r), 0);
+            tma_load_3d(sRaw + v * C::RAW_BYTES + r * D, tm, 0, 0, id * a.kv_heads + kvh, &bars->raw_full[v]);
+          }
+        } else {
+          const int s = 2 * (t & 1) + v, round = t < 2 ? -1 : t - 2 + v;
+          if (round >= 0 && !lane_wait<false>(&bars->kv_free[round & 1], (round >> 1) & 1, 2, abort_flag)) return false;
+          mbar_arrive_expect_tx(&bars->kv_full[s], C::TILE_BYTES);
+          for (int h = 0; h < C::HALVES; ++h)
+            tma_load_4d(sKV + s * C::TILE_BYTES + h * C::HALF_BYTES, tm, h * 64, key0, kvh, u.b, &bars->kv_full[s]);
+        }
         return true;
       };
       int t = 0, loaded = 0;
@@ -381,16 +535,18 @@ __global__ void __launch_bounds__(THREADS, 1)
 #pragma unroll 1
         for (int j = 0; j < u.n && ok; ++j, ++t) {
           if (j == 0) ok = load_q(u, 0);
-          if (ok && (ok = load_kv(&tm_k, u, j, 2 * (t & 1), t - 2))) loaded = 2 * t + 1;
+          if (ok && (ok = load_kv(&tm_k, u, j, t, 0))) loaded = 2 * t + 1;
           if (ok && j == 0 && u.two) ok = load_q(u, 1);
-          if (ok && (ok = load_kv(&tm_v, u, j, 2 * (t & 1) + 1, t < 2 ? -1 : t - 1))) loaded = 2 * t + 2;
+          if (ok && (ok = load_kv(&tm_v, u, j, t, 1))) loaded = 2 * t + 2;
         }
       }
       if (!ok || *abort_flag) {
         // let the copies in flight land (bounded) before the CTA goes
         for (int c = max(0, qc - QST); c < qc; ++c)
           lane_wait<false>(&bars->q_full[c % QST], (c / QST) & 1, 10, nullptr);
-        for (int c = max(0, loaded - KVST); c < loaded; ++c)
+        for (int c = max(0, loaded - 2); CODES && c < loaded; ++c)
+          lane_wait<false>(&bars->raw_full[c & 1], (c >> 1) & 1, 12, nullptr);
+        for (int c = max(0, loaded - KVST); !CODES && c < loaded; ++c)
           lane_wait<false>(&bars->kv_full[c % KVST], (c / KVST) & 1, 11, nullptr);
       }
     } else if (warp == 9) {
@@ -506,9 +662,28 @@ __global__ void __launch_bounds__(THREADS, 1)
           }
           keep_words(masked, mb, u.len - key0, w);
         }
+        float kf = 1.0f, vs = 1.0f;
+        if constexpr (CODES) {
+          // lane g (of four): the block of columns 32 g .., its scales
+          int id = 0;
+          if (more && lane < 4) {
+            id = block_of(a, u.b, key0 + 32 * lane);
+            if (id >= 0) {
+              const int64_t at = static_cast<int64_t>(id) * a.kv_heads + (args.group == 1 ? u.head : u.head / args.group);
+              kf = __ldg(a.k_scale + at);
+              vs = __ldg(a.v_scale + at);
+            }
+          }
+          const uint32_t there = __ballot_sync(0xffffffffu, id >= 0);
+#pragma unroll
+          for (int c = 0; c < 4; ++c)
+            if (((there >> c) & 1u) == 0) w[c] = 0u;
+          kf = fmaxf(kf * args.scale_log2, 1e-37f);  // (a factor of 0 would make NaN of -inf)
+          vs = fmaxf(vs, 1e-37f);
+        }
         if (pv != 0) {
           ok = ok && warp_wait(&bars->kv_full[2 * ((t + 1) & 1) + 1], ((t - 1) >> 1) & 1, 7, abort_flag);
-          if (ok && (vw[0] & vw[1] & vw[2] & vw[3]) != ~0u) {
+          if (!CODES && ok && (vw[0] & vw[1] & vw[2] & vw[3]) != ~0u) {
             // (a row's 16-byte pieces keep their row under the swizzle)
             const uint32_t v = smem_u32(sKV + (2 * ((t + 1) & 1) + 1) * C::TILE_BYTES);
             const int piece = lane & 7;
@@ -553,6 +728,17 @@ __global__ void __launch_bounds__(THREADS, 1)
           info->keep[3] = w[3];
           info->causal = sees;
           info->flags = end ? static_cast<uint32_t>(T_END) : sees < BKV ? (flags & ~T_WHOLE) | T_CAUSAL : flags;
+        }
+        if constexpr (CODES) {
+          if (lane < 4) {
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+              volatile TileInfo* info = &bars->info[i][ic[i] % INFOS];
+              info->k_factor[lane] = kf;
+              info->v_log2[lane] = __log2f(vs);
+              info->v_inv[lane] = 1.0f / vs;
+            }
+          }
         }
         ++ic[0];
         if (two) ++ic[1];
@@ -623,8 +809,23 @@ __global__ void __launch_bounds__(THREADS, 1)
 #pragma unroll
           for (int c = 0; c < 4; ++c) tmem_ld32p(s_tmem + c * 32, r + 32 * c);
           tmem_wait_fence<4>(r);
+          float fx[4], ox[4];
+          if constexpr (CODES) {
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {
+              fx[g] = info->k_factor[g];
+              ox[g] = info->v_log2[g];
+            }
+          }
           if (slow) {
-            const float m_tile = fmaxf(row_max64(r), row_max64(r + 64)) * args.scale_log2;
+            float m_tile;
+            if constexpr (CODES) {
+              m_tile = -INFINITY;
+#pragma unroll
+              for (int g = 0; g < 4; ++g) m_tile = fmaxf(m_tile, fmaf(row_max32(r + 32 * g), fx[g], ox[g]));
+            } else {
+              m_tile = fmaxf(row_max64(r), row_max64(r + 64)) * args.scale_log2;
+            }
             const bool rescale = m_tile > m_run + RESCALE_THRESHOLD;
             if (rescale) m_use = m_tile;
             if (__any_sync(0xffffffffu, rescale)) {
@@ -647,16 +848,33 @@ __global__ void __launch_bounds__(THREADS, 1)
               if (rescale) m_run = m_use;
             }
           }
-          const float2 sm = exp_pack64<F16, true>(r, r, args.scale_log2, m_use == -INFINITY ? 0.0f : -m_use);
+          const float neg_m = m_use == -INFINITY ? 0.0f : -m_use;
+          float2 sm;
+          if constexpr (CODES) {
+            sm = exp_codes64<F16, true>(r, r, make_float2(fx[0], fx[1]), make_float2(ox[0] + neg_m, ox[1] + neg_m),
+                                        make_float2(info->v_inv[0], info->v_inv[1]), fx, ox);
+          } else {
+            sm = exp_pack64<F16, true>(r, r, args.scale_log2, neg_m);
+            sm.y *= args.scale_log2;
+          }
           sum = sm.x;
           if (slow) break;
-          slow = __any_sync(0xffffffffu, sm.y * args.scale_log2 > m_run + RESCALE_THRESHOLD);
+          slow = __any_sync(0xffffffffu, sm.y > m_run + RESCALE_THRESHOLD);
           if (!slow) break;
         }
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-          if (h == 1)
-            sum += exp_pack64<F16, false>(r + 64, r + 32, args.scale_log2, m_use == -INFINITY ? 0.0f : -m_use).x;
+          if (h == 1) {
+            const float neg_m = m_use == -INFINITY ? 0.0f : -m_use;
+            if constexpr (CODES) {
+              const float f[4] = {0.f, 0.f, 0.f, 0.f};
+              sum += exp_codes64<F16, false>(r + 64, r + 32, make_float2(info->k_factor[2], info->k_factor[3]),
+                                             make_float2(info->v_log2[2] + neg_m, info->v_log2[3] + neg_m),
+                                             make_float2(info->v_inv[2], info->v_inv[3]), f, f).x;
+            } else {
+              sum += exp_pack64<F16, false>(r + 64, r + 32, args.scale_log2, neg_m).x;
+            }
+          }
           tmem_st32(s_tmem + 32 * h, *reinterpret_cast<uint32_t(*)[32]>(r + 32 * h));
           tc_wait_st();
           tc_fence_before();
@@ -692,8 +910,7 @@ __global__ void __launch_bounds__(THREADS, 1)
       }
     };
     bool ok = true;
-    #pragma unroll 1
-    for (; u.x < args.units && ok; u.next(args)) {
+    auto store = [&](const Unit& u) {  // a unit's rows
 #pragma unroll 1
       for (int i = 0; i < 2; ++i) {
         if (!ok || (i == 1 && !u.two)) continue;
@@ -779,6 +996,49 @@ __global__ void __launch_bounds__(THREADS, 1)
           }
         }
       }
+    };
+    if constexpr (CODES) {
+      // These warps also turn the codes into operands: K_t, then V_t, row
+      // `row` each thread.  A finished unit is stored between the next one's
+      // first K and first V: its last P V runs in the round that has that K.
+      int t = 0;
+      Unit done = u;
+      bool have = false;
+      auto convert = [&](int v, int j) {
+        const int key = (u.j0 + j) * BKV + row;
+        const bool keep = v == 0 || (key < u.len && block_of(a, u.b, key) >= 0);
+        const int round = t < 2 ? -1 : t - 2 + v;  // K_t overwrites K_{t-2}, V_t V_{t-2}
+        ok = ok && warp_wait(&bars->raw_full[v], t & 1, 25, abort_flag) &&
+             (round < 0 || warp_wait(&bars->kv_free[round & 1], (round >> 1) & 1, 26, abort_flag));
+        if (!ok) return;
+        const int slot = 2 * (t & 1) + v;
+        convert_row<D, KIND, F16>(smem_u32(sRaw + v * C::RAW_BYTES), smem_u32(sKV + slot * C::TILE_BYTES), row, keep);
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) {
+          mbar_arrive(&bars->kv_full[slot]);
+          mbar_arrive(&bars->raw_free[v]);
+        }
+      };
+#pragma unroll 1
+      for (; u.x < args.units && ok; u.next(args)) {
+        if (u.n == 0) {
+          store(u);
+          continue;
+        }
+#pragma unroll 1
+        for (int j = 0; j < u.n && ok; ++j, ++t) {
+          convert(0, j);
+          if (j == 0 && have && ok) store(done);
+          convert(1, j);
+        }
+        done = u;
+        have = true;
+      }
+      if (have && ok) store(done);
+    } else {
+#pragma unroll 1
+      for (; u.x < args.units && ok; u.next(args)) store(u);
     }
   }
 
@@ -790,7 +1050,7 @@ __global__ void __launch_bounds__(THREADS, 1)
   }
 }
 
-template <int D, bool F16>
+template <int D, bool F16, KvKind KIND>
 int launch(const XAttn& a, cudaStream_t stream) {
   const CUtensorMapDataType dt = F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
   CUtensorMap tq, tk, tv;
@@ -803,13 +1063,23 @@ int launch(const XAttn& a, cudaStream_t stream) {
     return h3b::encode_4d(m, dt, p, dims, sb, box, CU_TENSOR_MAP_SWIZZLE_128B);
   };
   int rc = encode(&tq, a.q, a.q_stride, a.s_q, a.heads);
-  if (rc == H3B_OK) rc = encode(&tk, a.k, a.kv_stride, a.s_kv, a.kv_heads);
-  if (rc == H3B_OK) rc = encode(&tv, a.v, a.kv_stride, a.s_kv, a.kv_heads);
+  if constexpr (KIND == KV_DENSE) {
+    if (rc == H3B_OK) rc = encode(&tk, a.k, a.kv_stride, a.s_kv, a.kv_heads);
+    if (rc == H3B_OK) rc = encode(&tv, a.v, a.kv_stride, a.s_kv, a.kv_heads);
+  } else {
+    const uint64_t slabs = static_cast<uint64_t>(a.num_blocks) * a.kv_heads;
+    const uint64_t slab = static_cast<uint64_t>(a.block_tokens) * D;
+    const uint32_t rows = static_cast<uint32_t>(a.block_tokens < BKV ? a.block_tokens : BKV);
+    constexpr CUtensorMapSwizzle sw = D == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B;
+    for (int i = 0; i < 2 && rc == H3B_OK; ++i)
+      rc = h3b::encode_3d(i ? &tv : &tk, CU_TENSOR_MAP_DATA_TYPE_UINT8, i ? a.v : a.k, D, a.block_tokens, slabs, D, slab,
+                          D, rows, 1, sw);
+  }
   if (rc != H3B_OK) return rc;
-  auto kernel = xattn_tile_kernel<D, F16>;
+  auto kernel = xattn_tile_kernel<D, F16, KIND>;
   static bool attr = false;
   if (!attr) {
-    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem_bytes<D>())) !=
+    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem_bytes<D, KIND>())) !=
         cudaSuccess)
       return H3B_ERR_LAUNCH;
     attr = true;
@@ -832,7 +1102,7 @@ int launch(const XAttn& a, cudaStream_t stream) {
   step /= a.splits;
   args.step_head = step % a.heads;
   args.step_b = step / a.heads;
-  kernel<<<static_cast<unsigned>(units < sms ? units : sms), THREADS, smem_bytes<D>(), stream>>>(tq, tk, tv, args);
+  kernel<<<static_cast<unsigned>(units < sms ? units : sms), THREADS, smem_bytes<D, KIND>(), stream>>>(tq, tk, tv, args);
   return h3b::launch_status();
 }
 
@@ -861,12 +1131,23 @@ int xattn_tile_splits(const XAttn& a) {
   return best;
 }
 
+namespace {
+template <int D, bool F16>
+int launch_kind(const XAttn& a, cudaStream_t stream) {
+  switch (a.kind) {
+    case KV_INT8: return launch<D, F16, KV_INT8>(a, stream);
+    case KV_E4M3: return launch<D, F16, KV_E4M3>(a, stream);
+    default: return launch<D, F16, KV_DENSE>(a, stream);
+  }
+}
+}  // namespace
+
 int xattn_tile_launch(const XAttn& a, cudaStream_t stream) {
   int rc;
   if (a.head_dim == 128) {
-    rc = a.dtype == H3B_F16 ? launch<128, true>(a, stream) : launch<128, false>(a, stream);
+    rc = a.dtype == H3B_F16 ? launch_kind<128, true>(a, stream) : launch_kind<128, false>(a, stream);
   } else {
-    rc = a.dtype == H3B_F16 ? launch<64, true>(a, stream) : launch<64, false>(a, stream);
+    rc = a.dtype == H3B_F16 ? launch_kind<64, true>(a, stream) : launch_kind<64, false>(a, stream);
   }
   return rc != H3B_OK || a.splits == 1 ? rc : xattn_combine_launch(a, stream);
 }
