@@ -405,7 +405,7 @@ H3B_DEV void convert_row(uint32_t raw, uint32_t dst, int row, bool keep) {
 
 // The cache's block of a key, -1 if there is none.
 H3B_DEV int block_of(const XAttn& a, int b, int key) {
-  const int j = key / a.block_tokens;
+  const int j = key >> (a.block_tokens == 32 ? 5 : (a.block_tokens == 64 ? 6 : 7));
   if (j >= a.max_blocks) return -1;
   const int id = __ldg(a.table + static_cast<int64_t>(b) * a.max_blocks + j);
   return id >= 0 && id < a.num_blocks ? id : -1;
@@ -507,6 +507,14 @@ __global__ void __launch_bounds__(THREADS, 1)
       };
       // K_t overwrites K_{t-2}, released with round t - 2 of the products; V_t
       // overwrites V_{t-2}, released with round t - 1 (see the matrix warp).
+      // Cache: the blocks of a tile, looked up a tile ahead (an absent block
+      // loads block 0: it may hold anything, see warp 10).
+      int ids[4] = {0, 0, 0, 0};
+      auto look_up = [&](const Unit& u, int j) {
+#pragma unroll
+        for (int g = 0; g < 4; ++g)
+          if (g * a.block_tokens < BKV) ids[g] = max(block_of(a, u.b, (u.j0 + j) * BKV + g * a.block_tokens), 0);
+      };
       auto load_kv = [&](const CUtensorMap* tm, const Unit& u, int j, int t, int v) {
         const int kvh = args.group == 1 ? u.head : u.head / args.group;
         const int key0 = (u.j0 + j) * BKV;
@@ -514,12 +522,11 @@ __global__ void __launch_bounds__(THREADS, 1)
           // codes: slot v, converted once a tile
           if (t > 0 && !lane_wait<false>(&bars->raw_free[v], (t - 1) & 1, 2, abort_flag)) return false;
           mbar_arrive_expect_tx(&bars->raw_full[v], C::RAW_BYTES);
-          const int rows = min(a.block_tokens, BKV);
-          for (int r = 0; r < BKV; r += rows) {
-            // (an absent block loads block 0: it may hold anything, see warp 10)
-            const int id = max(block_of(a, u.b, key0 + r), 0);
-            tma_load_3d(sRaw + v * C::RAW_BYTES + r * D, tm, 0, 0, id * a.kv_heads + kvh, &bars->raw_full[v]);
-          }
+          const int rows = a.block_tokens;
+#pragma unroll
+          for (int g = 0; g < 4; ++g)
+            if (g * rows < BKV)
+              tma_load_3d(sRaw + v * C::RAW_BYTES + g * rows * D, tm, 0, 0, ids[g] * a.kv_heads + kvh, &bars->raw_full[v]);
         } else {
           const int s = 2 * (t & 1) + v, round = t < 2 ? -1 : t - 2 + v;
           if (round >= 0 && !lane_wait<false>(&bars->kv_free[round & 1], (round >> 1) & 1, 2, abort_flag)) return false;
@@ -534,10 +541,12 @@ __global__ void __launch_bounds__(THREADS, 1)
       for (; u.x < args.units && ok; u.next<false>(args)) {
 #pragma unroll 1
         for (int j = 0; j < u.n && ok; ++j, ++t) {
+          if (CODES && j == 0) look_up(u, 0);
           if (j == 0) ok = load_q(u, 0);
           if (ok && (ok = load_kv(&tm_k, u, j, t, 0))) loaded = 2 * t + 1;
           if (ok && j == 0 && u.two) ok = load_q(u, 1);
           if (ok && (ok = load_kv(&tm_v, u, j, t, 1))) loaded = 2 * t + 2;
+          if (CODES && j + 1 < u.n) look_up(u, j + 1);
         }
       }
       if (!ok || *abort_flag) {
@@ -1004,9 +1013,7 @@ __global__ void __launch_bounds__(THREADS, 1)
       int t = 0;
       Unit done = u;
       bool have = false;
-      auto convert = [&](int v, int j) {
-        const int key = (u.j0 + j) * BKV + row;
-        const bool keep = v == 0 || (key < u.len && block_of(a, u.b, key) >= 0);
+      auto convert = [&](int v, bool keep) {
         const int round = t < 2 ? -1 : t - 2 + v;  // K_t overwrites K_{t-2}, V_t V_{t-2}
         ok = ok && warp_wait(&bars->raw_full[v], t & 1, 25, abort_flag) &&
              (round < 0 || warp_wait(&bars->kv_free[round & 1], (round >> 1) & 1, 26, abort_flag));
@@ -1028,9 +1035,11 @@ __global__ void __launch_bounds__(THREADS, 1)
         }
 #pragma unroll 1
         for (int j = 0; j < u.n && ok; ++j, ++t) {
-          convert(0, j);
+          const int key = (u.j0 + j) * BKV + row;
+          const bool keep = key < u.len && block_of(a, u.b, key) >= 0;  // (needed after K)
+          convert(0, true);
           if (j == 0 && have && ok) store(done);
-          convert(1, j);
+          convert(1, keep);
         }
         done = u;
         have = true;
