@@ -378,29 +378,43 @@ H3B_DEV void codes4(uint32_t w, uint32_t& lo, uint32_t& hi) {
 }
 
 // One row of a tile of codes (128 rows, TMA swizzle) as 16-bit operands in
-// the two 64-column halves that the products read (128-byte swizzle).
+// the two 64-column halves that the products read (128-byte swizzle), 64
+// codes at a time: four loads in flight, then the conversions.
 template <int D, KvKind KIND, bool F16>
-H3B_DEV void convert_row(uint32_t raw, uint32_t dst, int row, bool keep) {
-#pragma unroll 2
-  for (int c = 0; c < D / 16; ++c) {
-    const uint32_t at = D == 128 ? row * 128 + ((c ^ (row & 7)) << 4) : row * 64 + ((c ^ ((row >> 1) & 3)) << 4);
-    uint32_t w[4];
-    asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "r"(raw + at) : "memory");
-    uint32_t v[8];
+H3B_DEV void convert_row(uint32_t raw, uint32_t dst, int row) {
+#pragma unroll 1
+  for (int h = 0; h < D / 64; ++h) {
+    uint32_t w[4][4];
 #pragma unroll
-    for (int k = 0; k < 4; ++k) codes4<KIND, F16>(w[k], v[2 * k], v[2 * k + 1]);
-    if (!keep) {
-#pragma unroll
-      for (int k = 0; k < 8; ++k) v[k] = 0u;
-    }
-    const uint32_t half = dst + (c >> 2) * (128 * 128) + row * 128;
-    const int p = 2 * (c & 3);
-#pragma unroll
-    for (int k = 0; k < 2; ++k)
-      asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(half + (((p + k) ^ (row & 7)) << 4)), "r"(v[4 * k]),
-                   "r"(v[4 * k + 1]), "r"(v[4 * k + 2]), "r"(v[4 * k + 3])
+    for (int c = 0; c < 4; ++c) {
+      const int x = 4 * h + c;
+      const uint32_t at = D == 128 ? row * 128 + ((x ^ (row & 7)) << 4) : row * 64 + ((x ^ ((row >> 1) & 3)) << 4);
+      asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];"
+                   : "=r"(w[c][0]), "=r"(w[c][1]), "=r"(w[c][2]), "=r"(w[c][3])
+                   : "r"(raw + at)
                    : "memory");
+    }
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+      uint32_t v[8];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) codes4<KIND, F16>(w[c][k], v[2 * k], v[2 * k + 1]);
+#pragma unroll
+      for (int k = 0; k < 2; ++k)
+        asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(dst + h * (128 * 128) + row * 128 +
+                                                                   (((2 * c + k) ^ (row & 7)) << 4)),
+                     "r"(v[4 * k]), "r"(v[4 * k + 1]), "r"(v[4 * k + 2]), "r"(v[4 * k + 3])
+                     : "memory");
+    }
   }
+}
+template <int D>
+H3B_DEV void zero_row(uint32_t dst, int row) {
+#pragma unroll 1
+  for (int c = 0; c < D / 8; ++c)
+    asm volatile("st.shared.v4.u32 [%0], {%1,%1,%1,%1};" ::"r"(dst + (c >> 3) * (128 * 128) + row * 128 + (c & 7) * 16),
+                 "r"(0u)
+                 : "memory");
 }
 
 // The cache's block of a key, -1 if there is none.
@@ -650,6 +664,8 @@ __global__ void __launch_bounds__(THREADS, 1)
       uint32_t pv = 0;                  // R_PV* of the tile before
       uint32_t vw[4] = {0, 0, 0, 0};    // its kept columns
       uint32_t ic[2] = {0, 0};          // infos written, per row tile
+      int id_here = 0, id_ahead = 0;    // cache: blocks of this tile and the next, scales of this
+      float k_here = 1.0f, v_here = 1.0f;
       bool ok = true;
       while (u.x < args.units && u.n == 0) u.next(args);
       int j = 0;
@@ -664,6 +680,17 @@ __global__ void __launch_bounds__(THREADS, 1)
           const uint32_t mb = masked ? mask_bytes(a, u.b, key0, u.len, lane) : 0u;
           r |= R_S0 | (u.two ? R_S1 : 0u) | (j == u.n - 1 ? R_S_LAST : 0u) | ((qc % QST) << R_Q0_SHIFT) |
                (((qc + 1) % QST) << R_Q1_SHIFT);
+          if constexpr (CODES) {
+            if (lane < 4) {
+              if (j == 0) id_ahead = block_of(a, u.b, key0 + 32 * lane);
+              id_here = id_ahead;
+              if (j + 1 < u.n) id_ahead = block_of(a, u.b, key0 + BKV + 32 * lane);
+              const int64_t at = static_cast<int64_t>(max(id_here, 0)) * a.kv_heads +
+                                 (args.group == 1 ? u.head : u.head / args.group);
+              k_here = __ldg(a.k_scale + at);
+              v_here = __ldg(a.v_scale + at);
+            }
+          }
           ok = warp_wait(&bars->kv_full[2 * (t & 1)], (t >> 1) & 1, 9, abort_flag);
           if (j == 0) {
             ok = ok && warp_wait(&bars->q_full[qc % QST], (qc / QST) & 1, 3, abort_flag);
@@ -673,15 +700,13 @@ __global__ void __launch_bounds__(THREADS, 1)
         }
         float kf = 1.0f, vs = 1.0f;
         if constexpr (CODES) {
-          // lane g (of four): the block of columns 32 g .., its scales
+          // lane g (of four): the block of columns 32 g .., its scales, looked
+          // up while the tile was awaited (the block of the next one, too)
           int id = 0;
           if (more && lane < 4) {
-            id = block_of(a, u.b, key0 + 32 * lane);
-            if (id >= 0) {
-              const int64_t at = static_cast<int64_t>(id) * a.kv_heads + (args.group == 1 ? u.head : u.head / args.group);
-              kf = __ldg(a.k_scale + at);
-              vs = __ldg(a.v_scale + at);
-            }
+            id = id_here;
+            kf = k_here;
+            vs = v_here;
           }
           const uint32_t there = __ballot_sync(0xffffffffu, id >= 0);
 #pragma unroll
@@ -1013,19 +1038,11 @@ __global__ void __launch_bounds__(THREADS, 1)
       int t = 0;
       Unit done = u;
       bool have = false;
-      auto convert = [&](int v, bool keep) {
-        const int round = t < 2 ? -1 : t - 2 + v;  // K_t overwrites K_{t-2}, V_t V_{t-2}
-        ok = ok && warp_wait(&bars->raw_full[v], t & 1, 25, abort_flag) &&
-             (round < 0 || warp_wait(&bars->kv_free[round & 1], (round >> 1) & 1, 26, abort_flag));
-        if (!ok) return;
-        const int slot = 2 * (t & 1) + v;
-        convert_row<D, KIND, F16>(smem_u32(sRaw + v * C::RAW_BYTES), smem_u32(sKV + slot * C::TILE_BYTES), row, keep);
-        fence_proxy_async_smem();
-        __syncwarp();
-        if (lane == 0) {
-          mbar_arrive(&bars->kv_full[slot]);
-          mbar_arrive(&bars->raw_free[v]);
-        }
+      const int shift = a.block_tokens == 32 ? 5 : (a.block_tokens == 64 ? 6 : 7);
+      // table entry of the thread's row of tile j, fetched a tile ahead of its use
+      auto entry = [&](int j) -> int {
+        const int x = ((u.j0 + j) * BKV + row) >> shift;
+        return j < u.n && x < a.max_blocks ? __ldg(a.table + static_cast<int64_t>(u.b) * a.max_blocks + x) : -1;
       };
 #pragma unroll 1
       for (; u.x < args.units && ok; u.next(args)) {
@@ -1033,13 +1050,29 @@ __global__ void __launch_bounds__(THREADS, 1)
           store(u);
           continue;
         }
+        int id = entry(0);
 #pragma unroll 1
         for (int j = 0; j < u.n && ok; ++j, ++t) {
-          const int key = (u.j0 + j) * BKV + row;
-          const bool keep = key < u.len && block_of(a, u.b, key) >= 0;  // (needed after K)
-          convert(0, true);
-          if (j == 0 && have && ok) store(done);
-          convert(1, keep);
+          const int id_next = entry(j + 1);
+#pragma unroll 1
+          for (int v = 0; v < 2 && ok; ++v) {
+            if (v == 1 && j == 0 && have) store(done);
+            const int round = t < 2 ? -1 : t - 2 + v;  // K_t overwrites K_{t-2}, V_t V_{t-2}
+            ok = ok && (round < 0 || warp_wait(&bars->kv_free[round & 1], (round >> 1) & 1, 26, abort_flag)) &&
+                 warp_wait(&bars->raw_full[v], t & 1, 25, abort_flag);
+            if (!ok) break;
+            const int slot = 2 * (t & 1) + v;
+            const uint32_t dst = smem_u32(sKV + slot * C::TILE_BYTES);
+            convert_row<D, KIND, F16>(smem_u32(sRaw + v * C::RAW_BYTES), dst, row);
+            if (v == 1 && !((u.j0 + j) * BKV + row < u.len && id >= 0 && id < a.num_blocks)) zero_row<D>(dst, row);
+            fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0) {
+              mbar_arrive(&bars->kv_full[slot]);
+              mbar_arrive(&bars->raw_free[v]);
+            }
+          }
+          id = id_next;
         }
         done = u;
         have = true;
