@@ -46,12 +46,12 @@ using h3b::KvKind;
 using h3b::XAttn;
 
 constexpr int WARPS = 4;
-constexpr int RING_BYTES = 24 * 1024;  // per warp
 constexpr float LOG2E = 1.4426950408889634f;
 constexpr float LN2 = 0.69314718055994531f;
 
-template <int D, KvKind KIND>
+template <int D, KvKind KIND, int MT>
 struct Tile {
+  static constexpr int RING_BYTES = (MT == 1 ? 16 : 24) * 1024;  // per warp
   static constexpr int KEYS = KIND == KV_DENSE ? 16 : 32;
   static constexpr int ELT = KIND == KV_DENSE ? 2 : 1;
   static constexpr int ROW = D * ELT < 128 ? D * ELT : 128;  // bytes of a row inside one TMA box
@@ -154,15 +154,15 @@ H3B_DEV uint32_t code_off(int r, int c) {
 }
 
 template <int D, KvKind KIND, bool QF16, int MT>
-__global__ void __launch_bounds__(WARPS * 32, 2)
+__global__ void __launch_bounds__(WARPS * 32, MT == 1 ? 3 : 2)
     xattn_rows_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v,
                       const __grid_constant__ RowsArgs args) {
-  using T = Tile<D, KIND>;
+  using T = Tile<D, KIND, MT>;
   constexpr bool CODES = KIND != KV_DENSE;
   constexpr bool F16 = CODES || QF16;  // operand type of the matrix instructions
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + WARPS * RING_BYTES);
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + WARPS * T::RING_BYTES);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(bars + WARPS * T::STAGES);
   float2* s_ml = reinterpret_cast<float2*>(bars + WARPS * T::STAGES + 2);  // [WARPS][16 MT]
 
@@ -193,7 +193,7 @@ __global__ void __launch_bounds__(WARPS * 32, 2)
   const int tile0 = split * per, tile1 = min(n_tiles, tile0 + per);
   const int mine = tile1 - tile0 > warp ? (tile1 - tile0 - warp + WARPS - 1) / WARPS : 0;  // tiles of this warp
 
-  uint8_t* ring = smem + warp * RING_BYTES;
+  uint8_t* ring = smem + warp * T::RING_BYTES;
   uint64_t* full = bars + warp * T::STAGES;
   // Cache: the block of a tile, -1 if the table has none (its keys are left out).
   auto block_of = [&](int tile) -> int {
@@ -275,6 +275,9 @@ __global__ void __launch_bounds__(WARPS * 32, 2)
       mult[m][hf] = a.scale * LOG2E * e;
     }
   }
+
+  // Keys that every row of the CTA sees (rows past the last one are never stored).
+  const int full_to = a.causal ? len - a.s_q + (row_tile * 16 * MT) / args.group + 1 : len;
 
   float acc[MT][D / 8][4];
   float M[MT][2], L[MT][2];
@@ -385,28 +388,34 @@ __global__ void __launch_bounds__(WARPS * 32, 2)
     // ---- running softmax; x = score * mult * sk + log2 sv
     const float lsv = CODES ? __log2f(fmaxf(sv, 1e-37f)) : 0.0f;
     const float inv_sv = CODES ? 1.0f / fmaxf(sv, 1e-37f) : 1.0f;
+    const float ksk = CODES ? fmaxf(sk, 1e-37f) : 1.0f;  // (a factor of 0 would make NaN of -inf)
+    if (keep != all || key0 + T::KEYS > full_to) {
+#pragma unroll
+      for (int m = 0; m < MT; ++m)
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const int col = 2 * t + (e & 1);
+            const int key = 8 * n + (CODES ? perm<D>(col) : col);
+            if (((keep >> key) & 1u) == 0 || key0 + key >= limit[m][e >> 1]) sc[m][n][e] = -INFINITY;
+          }
+    }
 #pragma unroll
     for (int m = 0; m < MT; ++m) {
-      float top[2] = {-INFINITY, -INFINITY};
-#pragma unroll
-      for (int n = 0; n < NT; ++n)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const int col = 2 * t + (e & 1);
-          const int key = 8 * n + (CODES ? perm<D>(col) : col);
-          const bool in = ((keep >> key) & 1u) != 0 && key0 + key < limit[m][e >> 1];
-          const float x = in ? fmaf(sc[m][n][e], mult[m][e >> 1] * sk, lsv) : -INFINITY;
-          sc[m][n][e] = x;
-          top[e >> 1] = fmaxf(top[e >> 1], x);
-        }
-      float base[2], corr[2];
+      float f[2], off[2], corr[2];
 #pragma unroll
       for (int hf = 0; hf < 2; ++hf) {
-        top[hf] = fmaxf(top[hf], __shfl_xor_sync(0xffffffffu, top[hf], 1));
-        top[hf] = fmaxf(top[hf], __shfl_xor_sync(0xffffffffu, top[hf], 2));
-        const float mn = fmaxf(M[m][hf], top[hf]);
-        base[hf] = mn == -INFINITY ? 0.0f : mn;  // nothing kept so far: every weight is 2^-inf = 0
-        corr[hf] = ex2(M[m][hf] - base[hf]);
+        float top = fmaxf(sc[m][0][2 * hf], sc[m][0][2 * hf + 1]);
+#pragma unroll
+        for (int n = 1; n < NT; ++n) top = fmax3(top, sc[m][n][2 * hf], sc[m][n][2 * hf + 1]);
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+        f[hf] = mult[m][hf] * ksk;
+        const float mn = fmaxf(M[m][hf], fmaf(top, f[hf], lsv));
+        const float base = mn == -INFINITY ? 0.0f : mn;  // nothing kept so far: every weight is 2^-inf = 0
+        corr[hf] = ex2(M[m][hf] - base);
+        off[hf] = lsv - base;
         M[m][hf] = mn;
       }
       if (__any_sync(0xffffffffu, corr[0] != 1.0f || corr[1] != 1.0f)) {
@@ -423,7 +432,7 @@ __global__ void __launch_bounds__(WARPS * 32, 2)
       for (int n = 0; n < NT; ++n)
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          const float w = ex2(sc[m][n][e] - base[e >> 1]);
+          const float w = ex2(fmaf(sc[m][n][e], f[e >> 1], off[e >> 1]));
           sc[m][n][e] = w;
           sum[e >> 1] += w;
         }
@@ -510,7 +519,7 @@ __global__ void __launch_bounds__(WARPS * 32, 2)
   __syncthreads();  // rings are free: every warp has read its last tile
   constexpr int PAD = D + 4;
   float* s_o = reinterpret_cast<float*>(smem);  // [WARPS][16 MT][PAD]
-  static_assert(WARPS * 16 * MT * PAD * 4 <= WARPS * RING_BYTES, "join buffer");
+  static_assert(WARPS * 16 * MT * PAD * 4 <= WARPS * T::RING_BYTES, "join buffer");
 #pragma unroll
   for (int m = 0; m < MT; ++m)
 #pragma unroll
@@ -617,7 +626,7 @@ __global__ void __launch_bounds__(128) xattn_combine_kernel(const __grid_constan
 
 template <int D, KvKind KIND, bool QF16, int MT>
 int launch(const XAttn& a, cudaStream_t stream) {
-  using T = Tile<D, KIND>;
+  using T = Tile<D, KIND, MT>;
   CUtensorMap tk, tv;
   int rc;
   if constexpr (KIND == KV_DENSE) {
@@ -638,7 +647,7 @@ int launch(const XAttn& a, cudaStream_t stream) {
       rc = h3b::encode_3d(&tv, CU_TENSOR_MAP_DATA_TYPE_UINT8, a.v, D, a.block_tokens, slabs, D, slab, D, T::KEYS, 1, sw);
   }
   if (rc != H3B_OK) return rc;
-  constexpr size_t smem = 1024 + WARPS * RING_BYTES + (WARPS * T::STAGES + 2) * 8 + WARPS * 16 * MT * sizeof(float2);
+  constexpr size_t smem = 1024 + WARPS * T::RING_BYTES + (WARPS * T::STAGES + 2) * 8 + WARPS * 16 * MT * sizeof(float2);
   auto kernel = xattn_rows_kernel<D, KIND, QF16, MT>;
   static bool attr = false;
   if (!attr) {
@@ -685,10 +694,23 @@ namespace h3b {
 int xattn_rows_splits(const XAttn& a) {
   const int64_t rows = static_cast<int64_t>(a.s_q) * (a.heads / a.kv_heads);
   const int64_t ctas = (rows <= 16 ? 1 : (rows + 31) / 32) * a.kv_heads * a.batch;
-  const int64_t want = static_cast<int64_t>(num_sms()) * 4 / (ctas > 0 ? ctas : 1);  // two rounds of two CTAs per SM
-  const int64_t most = (static_cast<int64_t>(a.s_kv) + 127) / 128;                   // a tile or more per warp
-  const int64_t n = want < most ? want : most;
-  return static_cast<int>(n < 1 ? 1 : (n > 128 ? 128 : n));
+  // Rounds of CTAs (two or three fit an SM) times the steps of one (its four
+  // warps' tiles), its own start and end counted as two steps.  131072 int8
+  // keys x 24 heads: 18 splits (one round) 179 us, 37 (two) 183, 74 (four)
+  // 202; 32 x 16384 e4m3 keys x 8 heads: 1 split 253, 3 231, 6 220.
+  const int64_t slots = static_cast<int64_t>(num_sms()) * (rows <= 16 ? 3 : 2);
+  const int64_t keys = WARPS * (a.kind == KV_DENSE ? 16 : 32);
+  const int64_t steps = (static_cast<int64_t>(a.s_kv) + keys - 1) / keys;
+  int best = 1;
+  int64_t cost = INT64_MAX;
+  for (int64_t s = 1; s <= 128 && (s == 1 || s <= steps); ++s) {
+    const int64_t c = ((ctas * s + slots - 1) / slots) * ((steps + s - 1) / s + 2);
+    if (c < cost) {
+      cost = c;
+      best = static_cast<int>(s);
+    }
+  }
+  return best;
 }
 
 int xattn_rows_launch(const XAttn& a, cudaStream_t stream) {
