@@ -7,6 +7,9 @@ strides in place.  There is one backend and no SDPA fallback: unsupported
 inputs raise.  The reference's sequence-parallel entries are here too:
 ``gather_fa_bnsd`` / ``sp_gather_fa`` (K/V all-gathered, then attention) and
 ``ring_attention_bnsd`` (the K/V ring with log-sum-exp merges).
+
+``cross_attention`` (no reference counterpart) is the differentiable form of
+``ops.cross_attention``: a batch of query tokens against an encoder's states.
 """
 from __future__ import annotations
 
@@ -41,6 +44,34 @@ def h3_attention_bnsd(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, scal
     only matters to the reference's ring backend and is accepted for parity."""
     del gathered
     return fusion_attention_bnsd(q, k, v, scale=scale)
+
+
+class _CrossAttention(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, v, kv_lens, key_mask, scale):
+        lse = torch.empty((q.shape[0], q.shape[2], q.shape[1]), dtype=torch.float32, device=q.device)
+        o = ops.cross_attention(q, k, v, kv_lens=kv_lens, key_mask=key_mask, scale=scale, lse=lse)
+        ctx.save_for_backward(q, k, v, o, lse, kv_lens, key_mask)
+        ctx.scale = scale
+        return o
+
+    @staticmethod
+    def backward(ctx, do):
+        q, k, v, o, lse, kv_lens, key_mask = ctx.saved_tensors
+        dq, dk, dv = ops.cross_attention_bwd(do, q, k, v, o, lse, kv_lens=kv_lens, key_mask=key_mask,
+                                             scale=ctx.scale)
+        return dq, dk, dv, None, None, None
+
+
+def cross_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, kv_lens: Optional[torch.Tensor] = None,
+                    key_mask: Optional[torch.Tensor] = None, scale: Optional[float] = None) -> torch.Tensor:
+    """ops.cross_attention (q [B, Sq, H, D], k and v [B, Skv, Hkv, D]; see
+    there for kv_lens and key_mask), differentiable by autograd in q, k and v.
+    The backward pass is one call of ops.cross_attention_bwd; it keeps q, k,
+    v, the result and a log-sum-exp per row, and is bit-reproducible."""
+    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
+        return _CrossAttention.apply(q, k, v, kv_lens, key_mask, scale)
+    return ops.cross_attention(q, k, v, kv_lens=kv_lens, key_mask=key_mask, scale=scale)
 
 
 def _tokens(t: torch.Tensor) -> torch.Tensor:

@@ -237,6 +237,68 @@ class Attention(nn.Module):
         return self.out_proj.forward_fused(o, amax=amax_o)
 
 
+class CrossAttention(nn.Module):
+    """Cross attention of video tokens to a text encoder's states, beside the
+    joint-sequence ``Attention``: quantised query, key/value and output
+    projections around ops.cross_attention, with ``kv_heads`` shared key heads
+    (default: as many as query heads).
+
+    A prompt's states are the same at every denoising step, so their keys and
+    values can be projected once: ``encode`` gives them as tensors for the
+    ``kv`` argument, ``fill`` writes them into an 8-bit cache (half the bytes),
+    which ``forward`` then attends through ``cache``."""
+
+    def __init__(self, hidden, heads, head_dim, cond_dim, kv_heads: Optional[int] = None, dtype=None, device=None,
+                 operations=None):
+        super().__init__()
+        operations = operations or Ops
+        self.heads, self.head_dim = heads, head_dim
+        self.kv_heads = heads if kv_heads is None else kv_heads
+        if head_dim not in (64, 128) or heads % self.kv_heads:
+            raise ValueError("CrossAttention: head_dim 64 or 128, heads a multiple of kv_heads")
+        self.q_proj = operations.QuantLinear(hidden, heads * head_dim, bias=False, dtype=dtype, device=device)
+        self.kv_proj = operations.QuantLinear(cond_dim, 2 * self.kv_heads * head_dim, bias=False, dtype=dtype,
+                                              device=device)
+        self.out_proj = operations.QuantLinear(heads * head_dim, hidden, bias=False, dtype=dtype, device=device)
+
+    def encode(self, cond: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
+        """cond [B, n, cond_dim] -> k, v [B, n, kv_heads, head_dim], the two
+        halves of one projection (read in place by the attention)."""
+        b, n, _ = cond.shape
+        kv = self.kv_proj(cond.reshape(b * n, -1)).view(b, n, 2, self.kv_heads, self.head_dim)
+        return kv[:, :, 0], kv[:, :, 1]
+
+    def fill(self, cache: "ops.KV8Cache", cond: torch.Tensor, block_table: torch.Tensor, lens: torch.Tensor, *,
+             new_lens: Optional[torch.Tensor] = None) -> None:
+        """Appends the keys and values of cond [B, n, cond_dim] to the
+        sequences' blocks behind lens[b] tokens (ops.kv8_append)."""
+        k, v = self.encode(cond)
+        ops.kv8_append(cache, k, v, block_table, lens, new_lens=new_lens)
+
+    def forward(self, x: torch.Tensor, cond: Optional[torch.Tensor] = None, *,
+                kv: Optional[tuple[torch.Tensor, torch.Tensor]] = None, cond_lens: Optional[torch.Tensor] = None,
+                key_mask: Optional[torch.Tensor] = None, cache: Optional["ops.KV8Cache"] = None,
+                block_table: Optional[torch.Tensor] = None) -> torch.Tensor:
+        """x [B, S, hidden] bf16 attends to cond (or to kv, or to the
+        cond_lens[b] tokens of a cache): [B, S, hidden].  cond_lens (int32
+        [B]) and key_mask (bool [B, n]) leave padding and dropped tokens out;
+        a sample without any token gets zeros from the attention."""
+        if sum(a is not None for a in (cond, kv, cache)) != 1:
+            raise ValueError("CrossAttention.forward takes one of cond, kv and cache")
+        b, s, _ = x.shape
+        q = self.q_proj(x.reshape(b * s, -1)).view(b, s, self.heads, self.head_dim)
+        if cache is not None:
+            if block_table is None or cond_lens is None or key_mask is not None:
+                raise ValueError("a cache is attended through block_table and cond_lens, without key_mask")
+            with TIMER.span("cross_attention"):
+                o = ops.kv8_attention(q, cache, block_table, cond_lens)
+        else:
+            k, v = self.encode(cond) if kv is None else kv
+            with TIMER.span("cross_attention"):
+                o = ops.cross_attention(q, k, v, kv_lens=cond_lens, key_mask=key_mask)
+        return self.out_proj(o.view(b * s, self.heads * self.head_dim)).view(b, s, -1)
+
+
 class MLP(nn.Module):
     """fc1 -> activation -> fc2 (model/dit.py:291-301).  act="swiglu" is the
     reference MLP (fc1: hidden -> 2*ffn, silu(gate)*up, fused into fc1's

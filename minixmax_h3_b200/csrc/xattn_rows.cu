@@ -630,7 +630,7 @@ int launch(const XAttn& a, cudaStream_t stream) {
   CUtensorMap tk, tv;
   int rc;
   if constexpr (KIND == KV_DENSE) {
-    const uint64_t dims[4] = {D, static_cast<uint64_t>(a.s_kv), static_cast<uint64_t>(a.kv_heads),
+    const uint64_t dims[4] = {D, static_cast<uint64_t>(a.s_kv > 0 ? a.s_kv : 1), static_cast<uint64_t>(a.kv_heads),
                               static_cast<uint64_t>(a.batch)};
     const uint64_t st[3] = {static_cast<uint64_t>(a.kv_stride[1]) * 2, static_cast<uint64_t>(a.kv_stride[2]) * 2,
                             static_cast<uint64_t>(a.kv_stride[0]) * 2};

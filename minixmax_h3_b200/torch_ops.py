@@ -17,13 +17,18 @@ kernel of the path:
     h3b::rmsnorm_modulate(x, weight, shift, scale, eps, row_sel) -> h bf16 [m, hidden]
     h3b::rmsnorm_modulate_quant_i8(x, weight, shift, scale, eps, row_sel, convrot_group)
         -> (q int8 [m, hidden], scale fp32 [m])
+    h3b::cross_attention(q, k, v, kv_lens, key_mask, scale)
+        -> (o [B, Sq, H, D], lse fp32 [B, H, Sq]); differentiable in q, k, v
+    h3b::cross_attention_bwd(dout, q, k, v, out, lse, kv_lens, key_mask, scale) -> (dq, dk, dv)
+    h3b::kv8_append(k, v, codes and scales of K and V, block_table, lens, new_lens) -> None  (updates the cache)
+    h3b::kv8_attention(q, codes and scales, block_table, lens, causal, scale) -> o [B, Sq, H, D]
 
 Each is registered for CUDA tensors only, so tensors on any other device raise
 (there is no CPU fallback).  Each forwards to the ``ops`` function of the same
 name, where a failing status code becomes a RuntimeError.  Each has a fake
 implementation giving the output shapes and dtypes without running anything.
 The operators write only fresh outputs (``mutates_args=()``; gelu_amax_scan
-declares the one fp32 pair it updates), so the epilogue
+declares the one fp32 pair it updates, kv8_append the cache's four tensors), so the epilogue
 that updates a residual in place (EPI_GATE_RES) is refused here; the modules
 use it through ``ops`` directly.  NVFP4 operands are in the tensor cores'
 nibble order (``ops.quant_nvfp4(hi_first=False)``, ``QuantLinear.prepare_cube``).
@@ -114,6 +119,33 @@ def _rmsnorm_modulate_quant_i8(x: torch.Tensor, weight: torch.Tensor, shift: tor
     return ops.rmsnorm_modulate_quant_i8(x, weight, shift, scale, eps, row_sel=row_sel, convrot_group=convrot_group)
 
 
+def _cross_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, kv_lens: Optional[torch.Tensor] = None,
+                     key_mask: Optional[torch.Tensor] = None,
+                     scale: Optional[float] = None) -> tuple[torch.Tensor, torch.Tensor]:
+    lse = torch.empty((q.shape[0], q.shape[2], q.shape[1]), dtype=torch.float32, device=q.device)
+    return ops.cross_attention(q, k, v, kv_lens=kv_lens, key_mask=key_mask, scale=scale, lse=lse), lse
+
+
+def _cross_attention_bwd(dout: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, out: torch.Tensor,
+                         lse: torch.Tensor, kv_lens: Optional[torch.Tensor] = None,
+                         key_mask: Optional[torch.Tensor] = None, scale: Optional[float] = None
+                         ) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    return ops.cross_attention_bwd(dout, q, k, v, out, lse, kv_lens=kv_lens, key_mask=key_mask, scale=scale)
+
+
+def _kv8_append(k: torch.Tensor, v: torch.Tensor, k_codes: torch.Tensor, v_codes: torch.Tensor,
+                k_scale: torch.Tensor, v_scale: torch.Tensor, block_table: torch.Tensor, lens: torch.Tensor,
+                new_lens: Optional[torch.Tensor] = None) -> None:
+    ops.kv8_append(ops.KV8Cache(k_codes, v_codes, k_scale, v_scale), k, v, block_table, lens, new_lens=new_lens)
+
+
+def _kv8_attention(q: torch.Tensor, k_codes: torch.Tensor, v_codes: torch.Tensor, k_scale: torch.Tensor,
+                   v_scale: torch.Tensor, block_table: torch.Tensor, lens: torch.Tensor, causal: bool = False,
+                   scale: Optional[float] = None) -> torch.Tensor:
+    return ops.kv8_attention(q, ops.KV8Cache(k_codes, v_codes, k_scale, v_scale), block_table, lens, causal=causal,
+                             scale=scale)
+
+
 # ----------------------------------------------------------------------------- registration
 
 quant_i8_rows = torch.library.custom_op("h3b::quant_i8_rows", mutates_args=(), device_types="cuda")(_quant_i8_rows)
@@ -131,6 +163,14 @@ rmsnorm_modulate = torch.library.custom_op("h3b::rmsnorm_modulate", mutates_args
                                            device_types="cuda")(_rmsnorm_modulate)
 rmsnorm_modulate_quant_i8 = torch.library.custom_op("h3b::rmsnorm_modulate_quant_i8", mutates_args=(),
                                                     device_types="cuda")(_rmsnorm_modulate_quant_i8)
+
+cross_attention = torch.library.custom_op("h3b::cross_attention", mutates_args=(),
+                                          device_types="cuda")(_cross_attention)
+cross_attention_bwd = torch.library.custom_op("h3b::cross_attention_bwd", mutates_args=(),
+                                              device_types="cuda")(_cross_attention_bwd)
+kv8_append = torch.library.custom_op("h3b::kv8_append", mutates_args=("k_codes", "v_codes", "k_scale", "v_scale"),
+                                     device_types="cuda")(_kv8_append)
+kv8_attention = torch.library.custom_op("h3b::kv8_attention", mutates_args=(), device_types="cuda")(_kv8_attention)
 
 
 @quant_i8_rows.register_fake
@@ -188,3 +228,39 @@ def _(x, weight, shift, scale, eps, row_sel=None):
 def _(x, weight, shift, scale, eps, row_sel=None, convrot_group=0):
     m, hidden = _rows_of(x), x.shape[-1]
     return x.new_empty((m, hidden), dtype=torch.int8), x.new_empty((m,), dtype=torch.float32)
+
+
+@cross_attention.register_fake
+def _(q, k, v, kv_lens=None, key_mask=None, scale=None):
+    return q.new_empty(tuple(q.shape)), q.new_empty((q.shape[0], q.shape[2], q.shape[1]), dtype=torch.float32)
+
+
+@cross_attention_bwd.register_fake
+def _(dout, q, k, v, out, lse, kv_lens=None, key_mask=None, scale=None):
+    return q.new_empty(tuple(q.shape)), k.new_empty(tuple(k.shape)), v.new_empty(tuple(v.shape))
+
+
+def _cross_attention_setup(ctx, inputs, output):
+    q, k, v, kv_lens, key_mask, scale = inputs
+    ctx.save_for_backward(q, k, v, *output, kv_lens, key_mask)
+    ctx.scale = scale
+
+
+def _cross_attention_grad(ctx, dout, dlse):
+    del dlse  # the log-sum-exps are for the backward pass only
+    q, k, v, out, lse, kv_lens, key_mask = ctx.saved_tensors
+    grads = torch.ops.h3b.cross_attention_bwd(dout, q, k, v, out, lse, kv_lens, key_mask, ctx.scale)
+    return (*grads, None, None, None)
+
+
+cross_attention.register_autograd(_cross_attention_grad, setup_context=_cross_attention_setup)
+
+
+@kv8_append.register_fake
+def _(k, v, k_codes, v_codes, k_scale, v_scale, block_table, lens, new_lens=None):
+    return None
+
+
+@kv8_attention.register_fake
+def _(q, k_codes, v_codes, k_scale, v_scale, block_table, lens, causal=False, scale=None):
+    return q.new_empty(tuple(q.shape))
