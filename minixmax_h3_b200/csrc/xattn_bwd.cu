@@ -100,6 +100,7 @@ struct GradArgs {
   int k_tiles;   // of 128 keys
   int group;
   int units;
+  int step_q, step_head, step_b;  // gridDim.x units of the dq kernel further, digit by digit
   float scale_log2;
 };
 
@@ -127,12 +128,26 @@ H3B_DEV int len_of(const XAttnGrad& a, int b) {
 
 // ============================================================== dQ (and delta)
 // TMEM: SA | SB | dP | dQ.  S of tile j goes to SA or SB by turns, dS(j) over
-// it.  Issue order a tile: S(j+1); dP(j+1) when dP(j) has been read; dQ += dS(j) K(j).
-constexpr int XST = 3;  // ring of Q and dO tiles, by turns
-constexpr int KST = 2, VST = 2;
+// it.  Issue order: dP(j+1) when dP(j) has been read; dQ += dS(j) K(j); S(j+2)
+// over dS(j).  So S is two tiles ahead and dP one, and the compute warps find
+// both when they come to a tile.  (With S one tile ahead, K in a ring of two
+// and the walk over the units in the issuing warp a tile took 8000 cycles,
+// its products 1536: the next K was loaded only after dQ.)
+// Warp 10 walks the units ahead of the issuing warp: what tile j is of its
+// unit, which of its keys are kept, and that K, V and Q are there.
+constexpr int KST = 3, VST = 2;
+constexpr int INFOS = 4;  // entry j + 4 is written after dQ(j + 1), so after every warp has read entry j
+enum : uint32_t { T_FIRST = 1, T_LAST = 2, T_WHOLE = 4, T_END = 8 };
+struct __align__(16) TileInfo {
+  uint32_t keep[4];
+  uint32_t flags;
+  uint32_t pad[3];
+};
 
-struct __align__(8) DqBars {
-  uint64_t x_full[XST], x_free[XST];
+struct __align__(16) DqBars {
+  TileInfo info[INFOS];
+  uint64_t ready[INFOS];
+  uint64_t x_full[2], x_free[2];  // Q, dO
   uint64_t k_full[KST], k_free[KST];
   uint64_t v_full[VST], v_free[VST];
   uint64_t s_full[2];   // by step parity
@@ -153,24 +168,47 @@ struct __align__(8) DqBars {
 // memory, whose start is aligned (checked by the kernels).
 template <int D>
 constexpr size_t dq_smem() {
-  return (XST + KST + VST) * Cfg<D>::TILE_BYTES + 2 * 256 * sizeof(float) + sizeof(DqBars);
+  return (2 + KST + VST) * Cfg<D>::TILE_BYTES + 2 * 256 * sizeof(float) + sizeof(DqBars);
 }
 
 static_assert(dq_smem<128>() <= 232448, "shared memory of a CTA");
 
+// The units of one CTA (sample, head, 128 rows; rows fastest), the digits
+// carried from unit to unit.  WARP: called by whole warps (the reduction makes
+// the length uniform for the compiler).
 struct DqUnit {
-  int b, head, q0, len, n;
+  int x, qt, head, b;
+  int q0, len, n;
+
+  template <bool WARP>
+  H3B_DEV void settle(const GradArgs& args) {
+    q0 = qt * 128;
+    len = args.a.s_kv;
+    if (args.a.kv_lens != nullptr && x < args.units) {
+      len = len_of(args.a, b);
+      if constexpr (WARP) len = __reduce_max_sync(0xffffffffu, len);
+    }
+    n = (len + 127) / 128;
+  }
+  H3B_DEV void first(const GradArgs& args) {
+    x = blockIdx.x;
+    qt = x % args.q_tiles;
+    const int u = x / args.q_tiles;
+    head = u % args.a.heads;
+    b = u / args.a.heads;
+    settle<true>(args);
+  }
+  template <bool WARP = true>
+  H3B_DEV void next(const GradArgs& args) {
+    x += gridDim.x;
+    qt += args.step_q;
+    head += args.step_head;
+    b += args.step_b;
+    if (qt >= args.q_tiles) qt -= args.q_tiles, ++head;
+    if (head >= args.a.heads) head -= args.a.heads, ++b;
+    settle<WARP>(args);
+  }
 };
-H3B_DEV DqUnit dq_unit(const GradArgs& args, int u) {
-  DqUnit x;
-  x.q0 = (u % args.q_tiles) * 128;
-  u /= args.q_tiles;
-  x.head = u % args.a.heads;
-  x.b = u / args.a.heads;
-  x.len = len_of(args.a, x.b);
-  x.n = (x.len + 127) / 128;
-  return x;
-}
 
 template <int D, bool F16>
 __global__ void __launch_bounds__(THREADS, 1)
@@ -183,8 +221,8 @@ __global__ void __launch_bounds__(THREADS, 1)
   extern __shared__ __align__(1024) uint8_t smem_tiles[];
   uint8_t* smem = smem_tiles;
   if (misaligned(smem)) return;
-  uint8_t* sX = smem;
-  uint8_t* sK = sX + XST * C::TILE_BYTES;
+  uint8_t* sX = smem;  // Q | dO
+  uint8_t* sK = sX + 2 * C::TILE_BYTES;
   uint8_t* sV = sK + KST * C::TILE_BYTES;
   float* s_delta = reinterpret_cast<float*>(sV + VST * C::TILE_BYTES);  // [unit parity][256]
   DqBars* bars = reinterpret_cast<DqBars*>(s_delta + 2 * 256);
@@ -194,7 +232,8 @@ __global__ void __launch_bounds__(THREADS, 1)
   const bool masked = a.key_mask != nullptr;
 
   if (threadIdx.x == 0) {
-    for (int i = 0; i < XST; ++i) mbar_init(&bars->x_full[i], 1), mbar_init(&bars->x_free[i], 1);
+    for (int i = 0; i < INFOS; ++i) mbar_init(&bars->ready[i], 1);
+    for (int i = 0; i < 2; ++i) mbar_init(&bars->x_full[i], 1), mbar_init(&bars->x_free[i], 1);
     for (int i = 0; i < KST; ++i) mbar_init(&bars->k_full[i], 1), mbar_init(&bars->k_free[i], 1);
     for (int i = 0; i < VST; ++i) mbar_init(&bars->v_full[i], 1), mbar_init(&bars->v_free[i], 1);
     for (int i = 0; i < 2; ++i) {
@@ -217,8 +256,15 @@ __global__ void __launch_bounds__(THREADS, 1)
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const uint32_t tmem = bars->tmem_base;
+  constexpr uint32_t tmem = 0;  // all 512 columns are this CTA's (a constant keeps operands in uniform registers)
+  if (bars->tmem_base != 0) {   // (cannot happen; the same for the whole CTA)
+    if (threadIdx.x == 0 && atomicCAS(&g_status.code, 0, H3B_ERR_DEVICE) == 0) g_status.site = 31;
+    if (warp == 9) tmem_dealloc(bars->tmem_base, 512);
+    return;
+  }
   constexpr uint32_t DP_COL = 256, DQ_COL = 384;
+  DqUnit u;  // each role walks the CTA's units on its own
+  u.first(args);
 
   if (warp >= 8) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(REGS_CONTROL));
@@ -230,153 +276,180 @@ __global__ void __launch_bounds__(THREADS, 1)
       prefetch_tmap(&tm_do);
       prefetch_tmap(&tm_k);
       prefetch_tmap(&tm_v);
-      int xc = 0, kc = 0, vc = 0;
+      int xc = 0, t = 0, loaded = 0;
       bool ok = true;
-      auto load = [&](const CUtensorMap* tm, uint8_t* ring, uint64_t* full, uint64_t* free_, int stages, int& c, int row,
+      // c-th tile of a ring of `stages`
+      auto load = [&](const CUtensorMap* tm, uint8_t* ring, uint64_t* full, uint64_t* free_, int stages, int c, int row,
                       int head, int b) {
         const int s = c % stages;
-        if (c >= stages && !mbar_wait<false, false, true>(&free_[s], (c / stages - 1) & 1, &g_status, 1, abort_flag)) return false;
+        if (c >= stages && !mbar_wait<false, false, true>(&free_[s], (c / stages - 1) & 1, &g_status, 1, abort_flag))
+          return false;
         mbar_arrive_expect_tx(&full[s], C::TILE_BYTES);
         for (int h = 0; h < C::HALVES; ++h)
           tma_load_4d(ring + s * C::TILE_BYTES + h * C::HALF_BYTES, tm, h * 64, row, head, b, &full[s]);
-        ++c;
         return true;
       };
-      for (int x = blockIdx.x; x < args.units && ok; x += gridDim.x) {
-        const DqUnit u = dq_unit(args, x);
-        for (int j = 0; j < u.n && ok; ++j) {
-          const int kvh = u.head / args.group;
-          if (j == 0) ok = ok && load(&tm_q, sX, bars->x_full, bars->x_free, XST, xc, u.q0, u.head, u.b);
-          ok = ok && load(&tm_k, sK, bars->k_full, bars->k_free, KST, kc, j * 128, kvh, u.b);
-          if (j == 0) ok = ok && load(&tm_do, sX, bars->x_full, bars->x_free, XST, xc, u.q0, u.head, u.b);
-          ok = ok && load(&tm_v, sV, bars->v_full, bars->v_free, VST, vc, j * 128, kvh, u.b);
+#pragma unroll 1
+      for (; u.x < args.units && ok; u.next<false>(args)) {
+        const int kvh = args.group == 1 ? u.head : u.head / args.group;
+#pragma unroll 1
+        for (int j = 0; j < u.n && ok; ++j, ++t) {
+          // (Q and dO: rings of one, so the c-th use is the unit's)
+          if (j == 0) ok = load(&tm_q, sX, &bars->x_full[0], &bars->x_free[0], 1, xc, u.q0, u.head, u.b);
+          if (ok && (ok = load(&tm_k, sK, bars->k_full, bars->k_free, KST, t, j * 128, kvh, u.b))) loaded = 2 * t + 1;
+          if (ok && j == 0) {
+            ok = load(&tm_do, sX + C::TILE_BYTES, &bars->x_full[1], &bars->x_free[1], 1, xc, u.q0, u.head, u.b);
+            ++xc;
+          }
+          if (ok && (ok = load(&tm_v, sV, bars->v_full, bars->v_free, VST, t, j * 128, kvh, u.b))) loaded = 2 * t + 2;
         }
       }
       if (!ok || *abort_flag) {
-        for (int c = max(0, xc - XST); c < xc; ++c)
-          mbar_wait<false, false, true>(&bars->x_full[c % XST], (c / XST) & 1, &g_status, 10, nullptr);
-        for (int c = max(0, kc - KST); c < kc; ++c)
+        // let the copies in flight land (bounded) before the CTA goes
+        for (int c = max(0, (loaded + 1) / 2 - KST); c < (loaded + 1) / 2; ++c)
           mbar_wait<false, false, true>(&bars->k_full[c % KST], (c / KST) & 1, &g_status, 11, nullptr);
-        for (int c = max(0, vc - VST); c < vc; ++c)
+        for (int c = max(0, loaded / 2 - VST); c < loaded / 2; ++c)
           mbar_wait<false, false, true>(&bars->v_full[c % VST], (c / VST) & 1, &g_status, 12, nullptr);
+        for (int i = 0; i < 2; ++i)
+          if (xc > 0) mbar_wait<false, false, true>(&bars->x_full[i], (xc - 1) & 1, &g_status, 10, nullptr);
       }
     } else if (warp == 9) {
       // ---------------------------------------------------------- MMA
-      // Two cursors run over the same tiles: `f` one tile ahead issues S and
-      // dP, `c` issues dQ.
+      // The warp runs the schedule converged: all lanes poll, one elected lane
+      // issues.  Every barrier waited on here completes once per use and its
+      // next use depends on what this warp issues after the wait.
       bool ok = true;
-      auto commit = [&](uint64_t* bar) {
-        if (elect_one()) tc_commit(bar);
-        __syncwarp();
-      };
+      uint32_t uc = 0;  // units whose dO has been waited for
       auto wait = [&](uint64_t* bar, uint32_t parity, int site) {
-        if (!warp_wait<true>(bar, parity, site, abort_flag)) return false;
+        ok = mbar_wait<true, false, true>(bar, parity, &g_status, site, abort_flag) && ok;
+      };
+      auto next_tile = [&](int j) -> uint32_t {  // flags of tile j, once it is there
+        wait(&bars->ready[j % INFOS], (j / INFOS) & 1, 4);
+        const uint32_t f = ok ? *const_cast<volatile uint32_t*>(&bars->info[j % INFOS].flags) : static_cast<uint32_t>(T_END);
+        return __reduce_or_sync(0xffffffffu, f);
+      };
+      auto issue_s = [&](int j, uint32_t f) {
+        __syncwarp();
         tc_fence_after();
-        return true;
-      };
-      struct Cursor {
-        int x, j, step, xc;  // unit index, tile, steps done, index of the unit's Q tile in its ring
-        DqUnit u;
-      };
-      auto settle = [&](Cursor& c) {  // to the next unit that has tiles
-        while (c.x < args.units) {
-          c.u = dq_unit(args, c.x);
-          if (c.u.n > 0) break;
-          c.x += gridDim.x;
-        }
-      };
-      auto advance = [&](Cursor& c) {
-        ++c.step;
-        if (++c.j == c.u.n) {
-          c.j = 0;
-          c.xc += 2;
-          c.x += gridDim.x;
-          settle(c);
-        }
-      };
-      auto issue_s = [&](const Cursor& f) -> bool {
-        const int key0 = f.j * 128;
-        const uint32_t mb = masked ? mask_bytes(a, f.u.b, key0, f.u.len, lane) : 0u;
-        if (f.j == 0 && !wait(&bars->x_full[f.xc % XST], (f.xc / XST) & 1, 3)) return false;
-        if (!wait(&bars->k_full[f.step % KST], (f.step / KST) & 1, 4)) return false;
-        uint32_t w[4];
-        keep_words(masked, mb, f.u.len - key0, w);
-        const uint32_t k_s = smem_u32(sK + (f.step % KST) * C::TILE_BYTES);
-        if ((w[0] & w[1] & w[2] & w[3]) != 0xffffffffu) {
-          // left-out rows of K are zeroed: dS is 0 there, but 0 * NaN is not
-          const int piece = lane & 7;
-          for (int r = lane >> 3; r < 128; r += 4)
-            if (((w[r >> 5] >> (r & 31)) & 1u) == 0) {
-#pragma unroll
-              for (int h = 0; h < C::HALVES; ++h)
-                asm volatile("st.shared.v4.u32 [%0], {%1,%1,%1,%1};" ::"r"(k_s + h * C::HALF_BYTES + r * 128 + piece * 16),
-                             "r"(0u)
-                             : "memory");
-            }
-          fence_proxy_async_smem();
-          __syncwarp();
-        }
         if (elect_one()) {
-          issue_ss<D>(tmem + (f.step & 1) * 128, smem_u32(sX + (f.xc % XST) * C::TILE_BYTES), k_s, IDESC_S);
-          tc_commit(&bars->s_full[f.step & 1]);
-          if (f.j == f.u.n - 1) tc_commit(&bars->x_free[f.xc % XST]);
+          issue_ss<D>(tmem + (j & 1) * 128, smem_u32(sX), smem_u32(sK + (j % KST) * C::TILE_BYTES), IDESC_S);
+          tc_commit(&bars->s_full[j & 1]);
+          if (f & T_LAST) tc_commit(&bars->x_free[0]);
         }
         __syncwarp();
-        return true;
       };
-      auto issue_dp = [&](const Cursor& f) -> bool {
-        const int dc = f.xc + 1;
-        if (f.j == 0 && !wait(&bars->x_full[dc % XST], (dc / XST) & 1, 5)) return false;
-        if (!wait(&bars->v_full[f.step % VST], (f.step / VST) & 1, 6)) return false;
-        // dP(step - 1) has been read: the barrier's next phase follows this dP
-        if (f.step > 0 && !wait(&bars->dp_free, (f.step - 1) & 1, 7)) return false;
+      auto issue_dp = [&](int j, uint32_t f) {
+        if (f & T_FIRST) {
+          wait(&bars->x_full[1], uc & 1, 5);
+          ++uc;
+        }
+        // dP(j - 1) has been read: the barrier's next phase follows this dP
+        if (j > 0) wait(&bars->dp_free, (j - 1) & 1, 7);
+        __syncwarp();
+        tc_fence_after();
         if (elect_one()) {
-          issue_ss<D>(tmem + DP_COL, smem_u32(sX + (dc % XST) * C::TILE_BYTES),
-                      smem_u32(sV + (f.step % VST) * C::TILE_BYTES), IDESC_S);
+          issue_ss<D>(tmem + DP_COL, smem_u32(sX + C::TILE_BYTES), smem_u32(sV + (j % VST) * C::TILE_BYTES), IDESC_S);
           tc_commit(&bars->dp_full);
-          tc_commit(&bars->v_free[f.step % VST]);
-          if (f.j == f.u.n - 1) tc_commit(&bars->x_free[dc % XST]);
+          tc_commit(&bars->v_free[j % VST]);
+          if (f & T_LAST) tc_commit(&bars->x_free[1]);
         }
         __syncwarp();
-        return true;
       };
-      auto issue_dq = [&](const Cursor& c) -> bool {
-        const uint32_t k_s = smem_u32(sK + (c.step % KST) * C::TILE_BYTES);
-        uint64_t* ds = bars->ds_half[c.step & 1];
-        const uint32_t phase = (c.step >> 1) & 1;
-        for (int h = 0; h < 2; ++h) {
-          if (!wait(&ds[h], phase, 8)) return false;
-          // The first product of a unit overwrites dQ, half of which each
-          // warpgroup reads: both have to be past the last unit's stores.
-          if (c.j == 0 && h == 0 && !wait(&ds[1], phase, 8)) return false;
-          if (elect_one())
-            issue_ts_half<D>(tmem + DQ_COL, tmem + (c.step & 1) * 128 + h * 64, k_s, h, IDESC_G, c.j == 0 && h == 0);
-          __syncwarp();
-        }
+      uint32_t f0 = next_tile(0), f1 = T_END, f2;  // tiles j, j + 1, j + 2
+      if (!(f0 & T_END)) {
+        issue_s(0, f0);
+        issue_dp(0, f0);
+        f1 = next_tile(1);
+        if (!(f1 & T_END)) issue_s(1, f1);
+      }
+#pragma unroll 1
+      for (int j = 0; !(f0 & T_END); ++j) {
+        if (!(f1 & T_END)) issue_dp(j + 1, f1);
+        // dQ (+)= dS K, the first of a unit after both warpgroups are past
+        // the last unit's stores of it
+        uint64_t* ds = bars->ds_half[j & 1];
+        wait(&ds[0], (j >> 1) & 1, 8);
+        wait(&ds[1], (j >> 1) & 1, 8);
+        __syncwarp();
+        tc_fence_after();
         if (elect_one()) {
-          tc_commit(&bars->k_free[c.step % KST]);
-          if (c.j == c.u.n - 1) tc_commit(&bars->dq_full);
+          const uint32_t k_s = smem_u32(sK + (j % KST) * C::TILE_BYTES);
+#pragma unroll
+          for (int h = 0; h < 2; ++h)
+            issue_ts_half<D>(tmem + DQ_COL, tmem + (j & 1) * 128 + h * 64, k_s, h, IDESC_G, (f0 & T_FIRST) != 0 && h == 0);
+          tc_commit(&bars->k_free[j % KST]);
+          if (f0 & T_LAST) tc_commit(&bars->dq_full);
         }
         __syncwarp();
-        return true;
-      };
-      Cursor f{static_cast<int>(blockIdx.x), 0, 0, 0, {}};
-      settle(f);
-      Cursor c = f;
-      if (f.x < args.units) {
-        ok = issue_s(f) && issue_dp(f);
-        advance(f);
-      }
-      while (ok && c.x < args.units) {
-        if (f.x < args.units) {
-          ok = issue_s(f) && issue_dp(f);
-          advance(f);
+        f2 = T_END;
+        if (!(f1 & T_END)) {
+          f2 = next_tile(j + 2);
+          if (!(f2 & T_END)) issue_s(j + 2, f2);
         }
-        ok = ok && issue_dq(c);
-        advance(c);
+        if (!__all_sync(0xffffffffu, ok)) break;
+        f0 = f1;
+        f1 = f2;
       }
-      commit(&bars->drain);
+      if (elect_one()) tc_commit(&bars->drain);
+      __syncwarp();
       warp_wait(&bars->drain, 0, 9, nullptr);
+    } else if (warp == 10) {
+      // ---------------------------------------------------------- tiles
+      // Ahead of the issuing warp by the K ring; every barrier is waited for
+      // once per use, so the parity waits are one phase behind.
+      bool ok = true;
+      int t = 0;
+      uint32_t uc = 0;
+#pragma unroll 1
+      for (; u.x < args.units && ok; u.next(args)) {
+#pragma unroll 1
+        for (int j = 0; j < u.n; ++j, ++t) {
+          const int key0 = j * 128;
+          const uint32_t mb = masked ? mask_bytes(a, u.b, key0, u.len, lane) : 0u;
+          ok = (j > 0 || warp_wait(&bars->x_full[0], uc & 1, 3, abort_flag)) &&
+               warp_wait(&bars->k_full[t % KST], (t / KST) & 1, 14, abort_flag) &&
+               warp_wait(&bars->v_full[t % VST], (t / VST) & 1, 15, abort_flag);
+          if (!ok) break;
+          uint32_t w[4];
+          keep_words(masked, mb, u.len - key0, w);
+          const bool whole = (w[0] & w[1] & w[2] & w[3]) == ~0u;
+          if (!whole) {
+            // left-out rows of K are zeroed: dS is 0 there, but 0 * NaN is not
+            const uint32_t k_s = smem_u32(sK + (t % KST) * C::TILE_BYTES);
+            const int piece = lane & 7;
+#pragma unroll 1
+            for (int r4 = 0; r4 < 128; r4 += 4) {
+              const int r = r4 + (lane >> 3);
+              const uint32_t keep = r4 < 64 ? (r4 < 32 ? w[0] : w[1]) : (r4 < 96 ? w[2] : w[3]);
+              if (((keep >> (r & 31)) & 1u) == 0) {
+#pragma unroll
+                for (int h = 0; h < C::HALVES; ++h)
+                  asm volatile("st.shared.v4.u32 [%0], {%1,%1,%1,%1};" ::"r"(k_s + h * C::HALF_BYTES + r * 128 + piece * 16),
+                               "r"(0u)
+                               : "memory");
+              }
+            }
+            fence_proxy_async_smem();
+          }
+          volatile TileInfo* info = &bars->info[t % INFOS];
+          if (lane == 0) {
+#pragma unroll
+            for (int c = 0; c < 4; ++c) info->keep[c] = w[c];
+            info->flags = (j == 0 ? T_FIRST : 0u) | (j == u.n - 1 ? T_LAST : 0u) | (whole ? T_WHOLE : 0u);
+          }
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&bars->ready[t % INFOS]);
+        }
+        if (u.n > 0) ++uc;
+      }
+      if (ok) {
+        // entry t - INFOS has been read by all: this wait ends after dQ(t - INFOS)
+        if (t >= INFOS) ok = warp_wait(&bars->k_free[(t - INFOS) % KST], ((t - INFOS) / KST) & 1, 16, abort_flag);
+        if (lane == 0 && ok) {
+          *const_cast<volatile uint32_t*>(&bars->info[t % INFOS].flags) = T_END;
+          mbar_arrive(&bars->ready[t % INFOS]);
+        }
+      }
     }
   } else {
     // ------------------------------------------------------------ compute
@@ -386,8 +459,8 @@ __global__ void __launch_bounds__(THREADS, 1)
     const uint32_t lane_off = static_cast<uint32_t>((warp & 3) * 32) << 16;
     uint32_t step = 0, uc = 0, qc = 0;
     bool ok = true;
-    for (int x = blockIdx.x; x < args.units && ok; x += gridDim.x, ++uc) {
-      const DqUnit u = dq_unit(args, x);
+#pragma unroll 1
+    for (; u.x < args.units && ok; u.next(args), ++uc) {
       const int q_row = u.q0 + row;
       const int64_t stat = (static_cast<int64_t>(u.b) * a.heads + u.head) * a.s_q;
       // ---- delta = do . o of the unit's rows: warp w takes rows 16 w .. 16 w + 15,
@@ -443,9 +516,8 @@ __global__ void __launch_bounds__(THREADS, 1)
       }
       float delta = u.n != 1 ? s_delta[(uc & 1) * 256 + row] : 0.0f;
       const float neg_lse2 = q_row < a.s_q ? -lse2_of(__ldg(a.lse + stat + q_row)) : -INFINITY;
+#pragma unroll 1
       for (int j = 0; j < u.n; ++j, ++step) {
-        const int key0 = j * 128;
-        const uint32_t mb = masked ? mask_bytes(a, u.b, key0, u.len, lane) : 0u;
         const uint32_t s_tmem = tmem + (step & 1) * 128 + wg * 64 + lane_off;
         // S of this parity again only after this tile's dS has been read
         if (!warp_wait<true>(&bars->s_full[step & 1], (step >> 1) & 1, 21, abort_flag)) {
@@ -453,9 +525,8 @@ __global__ void __launch_bounds__(THREADS, 1)
           break;
         }
         tc_fence_after();
-        uint32_t w[4];
-        keep_words(masked, mb, u.len - key0, w);
-        const uint32_t w0 = wg ? w[2] : w[0], w1 = wg ? w[3] : w[1];
+        const volatile TileInfo* info = &bars->info[step % INFOS];
+        const bool whole = (info->flags & T_WHOLE) != 0;
         uint32_t s[64], d[64];
         tmem_ld32p(s_tmem, s);
         tmem_ld32p(s_tmem + 32, s + 32);
@@ -478,7 +549,9 @@ __global__ void __launch_bounds__(THREADS, 1)
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(&bars->dp_free);
-        if ((w0 & w1) != 0xffffffffu) {  // left-out keys: no weight, whatever they hold
+        if (!whole) {  // left-out keys: no weight, whatever they hold
+          asm volatile("// a branch, not selects on every tile");
+          const uint32_t w0 = info->keep[2 * wg], w1 = info->keep[2 * wg + 1];
 #pragma unroll
           for (int e = 0; e < 64; ++e)
             if (((e < 32 ? w0 : w1) & (1u << (e & 31))) == 0) s[e] = d[e] = 0u;
@@ -1006,6 +1079,11 @@ int launch(const XAttnGrad& a, cudaStream_t stream) {
   const int64_t ku = static_cast<int64_t>(a.batch) * a.kv_heads * args.k_tiles * a.splits;
   if (qu > 0x3fffffff || ku > 0x3fffffff) return H3B_ERR_SHAPE;
   args.units = static_cast<int>(qu);
+  int step = static_cast<int>(qu < sms ? qu : sms);
+  args.step_q = step % args.q_tiles;
+  step /= args.q_tiles;
+  args.step_head = step % a.heads;
+  args.step_b = step / a.heads;
   dq<<<static_cast<unsigned>(qu < sms ? qu : sms), THREADS, dq_smem<D>(), stream>>>(tq, tdo, tk, tv, args);
   rc = h3b::launch_status();
   if (rc != H3B_OK || ku == 0) return rc;
