@@ -7,7 +7,7 @@
 // Two kernels, each the owner of what it sums, so no sum crosses CTAs through
 // atomics and the result does not depend on scheduling:
 //   xattn_dq_kernel   a unit is 128 query rows of one head; it runs over the
-//                     key tiles (three products a tile) and also finds delta.
+//                     key tiles (three products a tile).
 //   xattn_dkv_kernel  a unit is 128 keys of one key head and a range of the
 //                     query tiles of all heads that share it (four products a
 //                     tile), in the transposed form: TMEM lanes are keys.
@@ -457,65 +457,32 @@ __global__ void __launch_bounds__(THREADS, 1)
     const int wg = warp >> 2;
     const int row = (warp & 3) * 32 + lane;
     const uint32_t lane_off = static_cast<uint32_t>((warp & 3) * 32) << 16;
-    uint32_t step = 0, uc = 0, qc = 0;
+    uint32_t step = 0, dc = 0, qc = 0;
     bool ok = true;
+    float lse_next = -INFINITY, delta_next = 0.0f;
+    auto fetch = [&](const DqUnit& v) {
+      const int r = v.q0 + row;
+      lse_next = -INFINITY;
+      delta_next = 0.0f;
+      if (v.x < args.units && r < a.s_q) {
+        const int64_t at = (static_cast<int64_t>(v.b) * a.heads + v.head) * a.s_q + r;
+        lse_next = __ldg(a.lse + at);
+        if (args.k_tiles > 1) delta_next = a.delta[at];
+      }
+    };
+    fetch(u);
 #pragma unroll 1
-    for (; u.x < args.units && ok; u.next(args), ++uc) {
+    for (; u.x < args.units && ok; u.next(args)) {
       const int q_row = u.q0 + row;
       const int64_t stat = (static_cast<int64_t>(u.b) * a.heads + u.head) * a.s_q;
-      // ---- delta = do . o of the unit's rows: warp w takes rows 16 w .. 16 w + 15,
-      // D / 8 lanes a row.  Where one tile holds all keys it is summed from
-      // P and dP instead (below): with few keys dP is close to delta, and the
-      // 16-bit rounding of o would cost dS bits (measured: 1.6 to 2.3 times
-      // the error of dq and dk at 2 to 26 keys).
-      if (u.n != 1) {
-        constexpr int LPR = D / 8, RPI = 32 / LPR;  // lanes a row, rows an instruction
-        float part[16 / RPI];
-        const uint16_t* op = static_cast<const uint16_t*>(a.o) + u.b * a.o_stride[0] + u.head * a.o_stride[2];
-        const uint16_t* gp = static_cast<const uint16_t*>(a.d_o) + u.b * a.do_stride[0] + u.head * a.do_stride[2];
-        const int col = (lane % LPR) * 8;
-#pragma unroll
-        for (int i = 0; i < 16 / RPI; ++i) {
-          const int r = u.q0 + warp * 16 + i * RPI + lane / LPR;
-          float s = 0.0f;
-          if (r < a.s_q) {
-            const uint4 ov = __ldg(reinterpret_cast<const uint4*>(op + r * a.o_stride[1] + col));
-            const uint4 gv = __ldg(reinterpret_cast<const uint4*>(gp + r * a.do_stride[1] + col));
-            const uint32_t ow[4] = {ov.x, ov.y, ov.z, ov.w}, gw[4] = {gv.x, gv.y, gv.z, gv.w};
-#pragma unroll
-            for (int k = 0; k < 4; ++k) {
-              if constexpr (F16) {
-                const float2 of = __half22float2(*reinterpret_cast<const __half2*>(&ow[k]));
-                const float2 gf = __half22float2(*reinterpret_cast<const __half2*>(&gw[k]));
-                s = fmaf(of.x, gf.x, fmaf(of.y, gf.y, s));
-              } else {
-                s = fmaf(bf16lo_to_f32(ow[k]), bf16lo_to_f32(gw[k]), s);
-                s = fmaf(bf16hi_to_f32(ow[k]), bf16hi_to_f32(gw[k]), s);
-              }
-            }
-          }
-          part[i] = s;
-        }
-#pragma unroll
-        for (int i = 0; i < 16 / RPI; ++i) {
-#pragma unroll
-          for (int o = LPR / 2; o > 0; o >>= 1) part[i] += __shfl_xor_sync(0xffffffffu, part[i], o);
-          const int r = warp * 16 + i * RPI + lane / LPR;
-          if (lane % LPR == 0) {
-            s_delta[(uc & 1) * 256 + r] = part[i];
-            if (u.q0 + r < a.s_q) a.delta[stat + u.q0 + r] = part[i];
-          }
-        }
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&bars->delta_ready);
-        // (completes once a unit; no warp can be a unit ahead of another)
-        if (!warp_wait(&bars->delta_ready, uc & 1, 20, abort_flag)) {
-          ok = false;
-          break;
-        }
+      // The rows' statistics, fetched a unit ahead.
+      const float neg_lse2 = -lse2_of(lse_next);
+      float delta = delta_next;
+      {
+        DqUnit v = u;
+        v.next(args);
+        fetch(v);
       }
-      float delta = u.n != 1 ? s_delta[(uc & 1) * 256 + row] : 0.0f;
-      const float neg_lse2 = q_row < a.s_q ? -lse2_of(__ldg(a.lse + stat + q_row)) : -INFINITY;
 #pragma unroll 1
       for (int j = 0; j < u.n; ++j, ++step) {
         const uint32_t s_tmem = tmem + (step & 1) * 128 + wg * 64 + lane_off;
@@ -557,21 +524,25 @@ __global__ void __launch_bounds__(THREADS, 1)
             if (((e < 32 ? w0 : w1) & (1u << (e & 31))) == 0) s[e] = d[e] = 0u;
         }
         if (u.n == 1) {
-          // One tile holds all keys: delta = sum_j P_j dP_j, both halves
+          // One tile holds all keys: delta = sum_j P_j dP_j, both halves.  With
+          // few keys dP is close to delta, and the 16-bit rounding of o would
+          // cost dS bits (1.6 to 2.3 times the error of dq and dk at 2 to 26 keys).
           float2 acc[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
 #pragma unroll
           for (int e = 0; e < 64; e += 2)
             acc[(e >> 1) & 1] = fma2(make_float2(__uint_as_float(s[e]), __uint_as_float(s[e + 1])),
                                      make_float2(__uint_as_float(d[e]), __uint_as_float(d[e + 1])), acc[(e >> 1) & 1]);
           const float2 t = add2(acc[0], acc[1]);
-          float* part = s_delta + (uc & 1) * 256;
+          float* part = s_delta + (dc & 1) * 256;
           part[wg * 128 + row] = t.x + t.y;
           __syncwarp();
           if (lane == 0) mbar_arrive(&bars->delta_ready);
-          if (!warp_wait(&bars->delta_ready, uc & 1, 24, abort_flag)) {
+          // (completes once a unit of one tile; no warp can be two such units ahead)
+          if (!warp_wait(&bars->delta_ready, dc & 1, 24, abort_flag)) {
             ok = false;
             break;
           }
+          ++dc;
           delta = part[row] + part[128 + row];
           if (wg == 0 && q_row < a.s_q) a.delta[stat + q_row] = delta;
         }
@@ -635,6 +606,43 @@ __global__ void __launch_bounds__(THREADS, 1)
     tc_fence_after();
     tmem_dealloc(tmem, 512);
   }
+}
+
+// delta = do . o of every row, where the keys take more than one tile: one
+// pass over o and do at memory rate.  (In the dq kernel, at the start of each
+// unit, its loads were waited for: 7 us a unit of 128 rows x 512 keys, whose
+// tiles take 8.)  D / 8 lanes a row.
+template <int D, bool F16>
+__global__ void __launch_bounds__(256) xattn_delta_kernel(const __grid_constant__ XAttnGrad a) {
+  constexpr int LPR = D / 8;
+  const int64_t i = (static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x) / LPR;  // (b, token, head)
+  const int col = (threadIdx.x % LPR) * 8;
+  const int64_t rows = static_cast<int64_t>(a.batch) * a.s_q * a.heads;
+  float s = 0.0f;
+  const int head = static_cast<int>(i % a.heads);
+  const int64_t bt = i / a.heads;
+  const int64_t tok = bt % a.s_q, b = bt / a.s_q;
+  if (i < rows) {
+    const uint4 ov = __ldg(reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(a.o) + b * a.o_stride[0] +
+                                                          tok * a.o_stride[1] + head * a.o_stride[2] + col));
+    const uint4 gv = __ldg(reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(a.d_o) + b * a.do_stride[0] +
+                                                          tok * a.do_stride[1] + head * a.do_stride[2] + col));
+    const uint32_t ow[4] = {ov.x, ov.y, ov.z, ov.w}, gw[4] = {gv.x, gv.y, gv.z, gv.w};
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      if constexpr (F16) {
+        const float2 of = __half22float2(*reinterpret_cast<const __half2*>(&ow[k]));
+        const float2 gf = __half22float2(*reinterpret_cast<const __half2*>(&gw[k]));
+        s = fmaf(of.x, gf.x, fmaf(of.y, gf.y, s));
+      } else {
+        s = fmaf(bf16lo_to_f32(ow[k]), bf16lo_to_f32(gw[k]), s);
+        s = fmaf(bf16hi_to_f32(ow[k]), bf16hi_to_f32(gw[k]), s);
+      }
+    }
+  }
+#pragma unroll
+  for (int o = LPR / 2; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+  if (i < rows && threadIdx.x % LPR == 0) a.delta[(b * a.heads + head) * a.s_q + tok] = s;
 }
 
 // ============================================================== dK and dV
@@ -1078,6 +1086,13 @@ int launch(const XAttnGrad& a, cudaStream_t stream) {
   const int64_t qu = static_cast<int64_t>(a.batch) * a.heads * args.q_tiles;
   const int64_t ku = static_cast<int64_t>(a.batch) * a.kv_heads * args.k_tiles * a.splits;
   if (qu > 0x3fffffff || ku > 0x3fffffff) return H3B_ERR_SHAPE;
+  if (args.k_tiles > 1) {
+    const int64_t blocks = (static_cast<int64_t>(a.batch) * a.s_q * a.heads * (D / 8) + 255) / 256;
+    if (blocks > 0x7fffffff) return H3B_ERR_SHAPE;
+    xattn_delta_kernel<D, F16><<<static_cast<unsigned>(blocks), 256, 0, stream>>>(a);
+    rc = h3b::launch_status();
+    if (rc != H3B_OK) return rc;
+  }
   args.units = static_cast<int>(qu);
   int step = static_cast<int>(qu < sms ? qu : sms);
   args.step_q = step % args.q_tiles;
