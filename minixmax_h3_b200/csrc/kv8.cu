@@ -54,6 +54,17 @@ H3B_DEV void unpack8(const uint4& w, float (&x)[8]) {
   }
 }
 
+// x / s, correctly rounded: from the correctly rounded reciprocal r of s,
+// q = x r is within an ulp or so, the FMA gives its residual exactly, and one
+// more FMA rounds the corrected quotient (Markstein's division; bits as
+// __fdiv_rn for results that are not subnormal, and smaller ones are code 0
+// either way).  s lies between 1e-12 / 448 and 3.4e38 / 127, so r is normal.
+// Three operations against some ten of a division: append of 65 MB 52 us with it.
+H3B_DEV float quotient(float x, float s, float r) {
+  const float q = __fmul_rn(x, r);
+  return __fmaf_rn(__fmaf_rn(-q, s, x), r, q);
+}
+
 // Four values -> four codes of one register, and back.
 template <bool E4M3>
 H3B_DEV uint32_t to_codes4(float a, float b, float c, float d) {
@@ -136,6 +147,7 @@ __global__ void __launch_bounds__(THREADS) kv8_append_kernel(const __grid_consta
   for (int w = 0; w < THREADS / 32; ++w) mx = fmaxf(mx, s_max[w]);
   const float scale = fmaxf(held, __fdiv_rn(fmaxf(mx, 1e-12f), TOP));
   if (threadIdx.x == 0) args.scale[which][slab] = scale;
+  const float recip = __frcp_rn(scale);
 #pragma unroll
   for (int p = 0; p < PASSES; ++p) {
     const int r = p * RPP + row0;
@@ -146,7 +158,7 @@ __global__ void __launch_bounds__(THREADS) kv8_append_kernel(const __grid_consta
       float x[8];
       unpack8<F16>(raw[p], x);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) x[e] = __fdiv_rn(x[e], scale);
+      for (int e = 0; e < 8; ++e) x[e] = quotient(x[e], scale, recip);
       w.x = to_codes4<E4M3>(x[0], x[1], x[2], x[3]);
       w.y = to_codes4<E4M3>(x[4], x[5], x[6], x[7]);
     } else if (r < first) {
@@ -155,10 +167,10 @@ __global__ void __launch_bounds__(THREADS) kv8_append_kernel(const __grid_consta
       float x[8], y[4];
       from_codes4<E4M3>(w.x, y);
 #pragma unroll
-      for (int e = 0; e < 4; ++e) x[e] = __fdiv_rn(__fmul_rn(y[e], held), scale);
+      for (int e = 0; e < 4; ++e) x[e] = quotient(__fmul_rn(y[e], held), scale, recip);
       from_codes4<E4M3>(w.y, y);
 #pragma unroll
-      for (int e = 0; e < 4; ++e) x[4 + e] = __fdiv_rn(__fmul_rn(y[e], held), scale);
+      for (int e = 0; e < 4; ++e) x[4 + e] = quotient(__fmul_rn(y[e], held), scale, recip);
       w.x = to_codes4<E4M3>(x[0], x[1], x[2], x[3]);
       w.y = to_codes4<E4M3>(x[4], x[5], x[6], x[7]);
     }

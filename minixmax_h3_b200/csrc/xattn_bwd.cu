@@ -134,18 +134,13 @@ H3B_DEV int len_of(const XAttnGrad& a, int b) {
 // and the walk over the units in the issuing warp a tile took 8000 cycles,
 // its products 1536: the next K was loaded only after dQ.)
 // Warp 10 walks the units ahead of the issuing warp: what tile j is of its
-// unit, which of its keys are kept, and that K, V and Q are there.
+// unit, and that K, V and Q are there; it zeroes the left-out rows of K and V.
 constexpr int KST = 3, VST = 2;
-constexpr int INFOS = 4;  // entry j + 4 is written after dQ(j + 1), so after every warp has read entry j
-enum : uint32_t { T_FIRST = 1, T_LAST = 2, T_WHOLE = 4, T_END = 8 };
-struct __align__(16) TileInfo {
-  uint32_t keep[4];
-  uint32_t flags;
-  uint32_t pad[3];
-};
+constexpr int INFOS = 4;  // entry j + 4 is written after dQ(j + 1), so after entry j has been read
+enum : uint32_t { T_FIRST = 1, T_LAST = 2, T_END = 4 };
 
 struct __align__(16) DqBars {
-  TileInfo info[INFOS];
+  uint32_t flags[INFOS];  // T_* of a tile
   uint64_t ready[INFOS];
   uint64_t x_full[2], x_free[2];  // Q, dO
   uint64_t k_full[KST], k_free[KST];
@@ -325,7 +320,7 @@ __global__ void __launch_bounds__(THREADS, 1)
       };
       auto next_tile = [&](int j) -> uint32_t {  // flags of tile j, once it is there
         wait(&bars->ready[j % INFOS], (j / INFOS) & 1, 4);
-        const uint32_t f = ok ? *const_cast<volatile uint32_t*>(&bars->info[j % INFOS].flags) : static_cast<uint32_t>(T_END);
+        const uint32_t f = ok ? *const_cast<volatile uint32_t*>(&bars->flags[j % INFOS]) : static_cast<uint32_t>(T_END);
         return __reduce_or_sync(0xffffffffu, f);
       };
       auto issue_s = [&](int j, uint32_t f) {
@@ -412,10 +407,10 @@ __global__ void __launch_bounds__(THREADS, 1)
           if (!ok) break;
           uint32_t w[4];
           keep_words(masked, mb, u.len - key0, w);
-          const bool whole = (w[0] & w[1] & w[2] & w[3]) == ~0u;
-          if (!whole) {
-            // left-out rows of K are zeroed: dS is 0 there, but 0 * NaN is not
-            const uint32_t k_s = smem_u32(sK + (t % KST) * C::TILE_BYTES);
+          if ((w[0] & w[1] & w[2] & w[3]) != ~0u) {
+            // Left-out rows of K and V are zeroed: S and dP are 0 there, so P
+            // (held to 1) and dS are finite, and dS K adds nothing.
+            const uint32_t k_s = smem_u32(sK + (t % KST) * C::TILE_BYTES), v_s = smem_u32(sV + (t % VST) * C::TILE_BYTES);
             const int piece = lane & 7;
 #pragma unroll 1
             for (int r4 = 0; r4 < 128; r4 += 4) {
@@ -423,20 +418,17 @@ __global__ void __launch_bounds__(THREADS, 1)
               const uint32_t keep = r4 < 64 ? (r4 < 32 ? w[0] : w[1]) : (r4 < 96 ? w[2] : w[3]);
               if (((keep >> (r & 31)) & 1u) == 0) {
 #pragma unroll
-                for (int h = 0; h < C::HALVES; ++h)
-                  asm volatile("st.shared.v4.u32 [%0], {%1,%1,%1,%1};" ::"r"(k_s + h * C::HALF_BYTES + r * 128 + piece * 16),
+                for (int h = 0; h < 2 * C::HALVES; ++h)
+                  asm volatile("st.shared.v4.u32 [%0], {%1,%1,%1,%1};" ::"r"((h < C::HALVES ? k_s : v_s) +
+                                                                             (h % C::HALVES) * C::HALF_BYTES + r * 128 + piece * 16),
                                "r"(0u)
                                : "memory");
               }
             }
             fence_proxy_async_smem();
           }
-          volatile TileInfo* info = &bars->info[t % INFOS];
-          if (lane == 0) {
-#pragma unroll
-            for (int c = 0; c < 4; ++c) info->keep[c] = w[c];
-            info->flags = (j == 0 ? T_FIRST : 0u) | (j == u.n - 1 ? T_LAST : 0u) | (whole ? T_WHOLE : 0u);
-          }
+          if (lane == 0)
+            *const_cast<volatile uint32_t*>(&bars->flags[t % INFOS]) = (j == 0 ? T_FIRST : 0u) | (j == u.n - 1 ? T_LAST : 0u);
           __syncwarp();
           if (lane == 0) mbar_arrive(&bars->ready[t % INFOS]);
         }
@@ -446,7 +438,7 @@ __global__ void __launch_bounds__(THREADS, 1)
         // entry t - INFOS has been read by all: this wait ends after dQ(t - INFOS)
         if (t >= INFOS) ok = warp_wait(&bars->k_free[(t - INFOS) % KST], ((t - INFOS) / KST) & 1, 16, abort_flag);
         if (lane == 0 && ok) {
-          *const_cast<volatile uint32_t*>(&bars->info[t % INFOS].flags) = T_END;
+          *const_cast<volatile uint32_t*>(&bars->flags[t % INFOS]) = T_END;
           mbar_arrive(&bars->ready[t % INFOS]);
         }
       }
@@ -492,8 +484,6 @@ __global__ void __launch_bounds__(THREADS, 1)
           break;
         }
         tc_fence_after();
-        const volatile TileInfo* info = &bars->info[step % INFOS];
-        const bool whole = (info->flags & T_WHOLE) != 0;
         uint32_t s[64], d[64];
         tmem_ld32p(s_tmem, s);
         tmem_ld32p(s_tmem + 32, s + 32);
@@ -502,8 +492,9 @@ __global__ void __launch_bounds__(THREADS, 1)
         for (int e = 0; e < 64; e += 2) {
           const float2 t = fma2(make_float2(__uint_as_float(s[e]), __uint_as_float(s[e + 1])),
                                 make_float2(args.scale_log2, args.scale_log2), make_float2(neg_lse2, neg_lse2));
-          s[e] = __float_as_uint(ex2(t.x));
-          s[e + 1] = __float_as_uint(ex2(t.y));
+          // (P <= 1 but for rounding; a left-out key's score of 0 may be far above lse)
+          s[e] = __float_as_uint(ex2(fminf(t.x, 0.0f)));
+          s[e + 1] = __float_as_uint(ex2(fminf(t.y, 0.0f)));
         }
         if (!warp_wait<true>(&bars->dp_full, step & 1, 22, abort_flag)) {
           ok = false;
@@ -516,13 +507,6 @@ __global__ void __launch_bounds__(THREADS, 1)
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(&bars->dp_free);
-        if (!whole) {  // left-out keys: no weight, whatever they hold
-          asm volatile("// a branch, not selects on every tile");
-          const uint32_t w0 = info->keep[2 * wg], w1 = info->keep[2 * wg + 1];
-#pragma unroll
-          for (int e = 0; e < 64; ++e)
-            if (((e < 32 ? w0 : w1) & (1u << (e & 31))) == 0) s[e] = d[e] = 0u;
-        }
         if (u.n == 1) {
           // One tile holds all keys: delta = sum_j P_j dP_j, both halves.  With
           // few keys dP is close to delta, and the 16-bit rounding of o would

@@ -425,7 +425,7 @@ H3B_DEV int block_of(const XAttn& a, int b, int key) {
   return id >= 0 && id < a.num_blocks ? id : -1;
 }
 
-template <int D, bool F16, KvKind KIND>
+template <int D, bool F16, KvKind KIND, bool MASKED>
 __global__ void __launch_bounds__(THREADS, 1)
     xattn_tile_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
                       const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ TileArgs args) {
@@ -447,7 +447,7 @@ __global__ void __launch_bounds__(THREADS, 1)
   const XAttn& a = args.a;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   volatile int* abort_flag = &bars->abort_flag;
-  const bool masked = a.key_mask != nullptr;
+  constexpr bool masked = MASKED;  // a.key_mask is given
 
   if (threadIdx.x == 0) {
     for (int i = 0; i < QST; ++i) {
@@ -808,9 +808,10 @@ __global__ void __launch_bounds__(THREADS, 1)
           m_run = -INFINITY;
           l_run = 0.0f;
         }
-        if ((flags & T_WHOLE) == 0) {
+        if (!MASKED && (flags & T_WHOLE) == 0) {
           // Left-out columns become -inf in TMEM, 32 at a time in a loop that
-          // stays out of the instruction cache of whole tiles.
+          // stays out of the instruction cache of whole tiles.  (With a mask
+          // every tile has some: there they are replaced in registers below.)
 #pragma unroll 1
           for (int c = 0; c < 4; ++c) {
             uint32_t keep = info->keep[c];
@@ -843,6 +844,15 @@ __global__ void __launch_bounds__(THREADS, 1)
 #pragma unroll
           for (int c = 0; c < 4; ++c) tmem_ld32p(s_tmem + c * 32, r + 32 * c);
           tmem_wait_fence<4>(r);
+          if constexpr (MASKED) {
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+              const uint32_t keep = info->keep[c];
+#pragma unroll
+              for (int e = 0; e < 32; ++e)
+                if ((keep & (1u << e)) == 0) r[32 * c + e] = __float_as_uint(-INFINITY);
+            }
+          }
           float fx[4], ox[4];
           if constexpr (CODES) {
 #pragma unroll
@@ -1092,7 +1102,7 @@ __global__ void __launch_bounds__(THREADS, 1)
   }
 }
 
-template <int D, bool F16, KvKind KIND>
+template <int D, bool F16, KvKind KIND, bool MASKED = false>
 int launch(const XAttn& a, cudaStream_t stream) {
   const CUtensorMapDataType dt = F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
   CUtensorMap tq, tk, tv;
@@ -1118,7 +1128,7 @@ int launch(const XAttn& a, cudaStream_t stream) {
                           D, rows, 1, sw);
   }
   if (rc != H3B_OK) return rc;
-  auto kernel = xattn_tile_kernel<D, F16, KIND>;
+  auto kernel = xattn_tile_kernel<D, F16, KIND, MASKED>;
   static bool attr = false;
   if (!attr) {
     if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem_bytes<D, KIND>())) !=
@@ -1179,7 +1189,8 @@ int launch_kind(const XAttn& a, cudaStream_t stream) {
   switch (a.kind) {
     case KV_INT8: return launch<D, F16, KV_INT8>(a, stream);
     case KV_E4M3: return launch<D, F16, KV_E4M3>(a, stream);
-    default: return launch<D, F16, KV_DENSE>(a, stream);
+    default:
+      return a.key_mask != nullptr ? launch<D, F16, KV_DENSE, true>(a, stream) : launch<D, F16, KV_DENSE>(a, stream);
   }
 }
 }  // namespace
