@@ -598,6 +598,25 @@ H3B_DEV float fmax3(float a, float b, float c) {
   return r;
 }
 
+// Zeroes the left-out rows (bit r & 31 of keep[r >> 5] clear) of a 128-row tile
+// of 128-byte rows, HALVES such tiles 16 KB apart; one warp, lane = row of 32.
+// A row's 16-byte pieces keep their row under the swizzle; the lanes start at
+// different pieces, so their stores meet different banks.
+template <int HALVES>
+H3B_DEV void zero_left_out(uint32_t tile, const uint32_t (&keep)[4], int lane) {
+#pragma unroll
+  for (int c = 0; c < 4; ++c) {
+    if (((keep[c] >> lane) & 1u) == 0) {
+      const uint32_t row = tile + static_cast<uint32_t>(c * 32 + lane) * 128;
+#pragma unroll
+      for (int h = 0; h < HALVES; ++h)
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+          asm volatile("st.shared.v4.u32 [%0], {%1,%1,%1,%1};" ::"r"(row + h * 16384 + ((i + lane) & 7) * 16), "r"(0u) : "memory");
+    }
+  }
+}
+
 H3B_DEV float warp_max(float v) {
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));

@@ -410,21 +410,8 @@ __global__ void __launch_bounds__(THREADS, 1)
           if ((w[0] & w[1] & w[2] & w[3]) != ~0u) {
             // Left-out rows of K and V are zeroed: S and dP are 0 there, so P
             // (held to 1) and dS are finite, and dS K adds nothing.
-            const uint32_t k_s = smem_u32(sK + (t % KST) * C::TILE_BYTES), v_s = smem_u32(sV + (t % VST) * C::TILE_BYTES);
-            const int piece = lane & 7;
-#pragma unroll 1
-            for (int r4 = 0; r4 < 128; r4 += 4) {
-              const int r = r4 + (lane >> 3);
-              const uint32_t keep = r4 < 64 ? (r4 < 32 ? w[0] : w[1]) : (r4 < 96 ? w[2] : w[3]);
-              if (((keep >> (r & 31)) & 1u) == 0) {
-#pragma unroll
-                for (int h = 0; h < 2 * C::HALVES; ++h)
-                  asm volatile("st.shared.v4.u32 [%0], {%1,%1,%1,%1};" ::"r"((h < C::HALVES ? k_s : v_s) +
-                                                                             (h % C::HALVES) * C::HALF_BYTES + r * 128 + piece * 16),
-                               "r"(0u)
-                               : "memory");
-              }
-            }
+            zero_left_out<C::HALVES>(smem_u32(sK + (t % KST) * C::TILE_BYTES), w, lane);
+            zero_left_out<C::HALVES>(smem_u32(sV + (t % VST) * C::TILE_BYTES), w, lane);
             fence_proxy_async_smem();
           }
           if (lane == 0)

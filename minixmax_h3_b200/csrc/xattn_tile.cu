@@ -718,21 +718,7 @@ __global__ void __launch_bounds__(THREADS, 1)
         if (pv != 0) {
           ok = ok && warp_wait(&bars->kv_full[2 * ((t + 1) & 1) + 1], ((t - 1) >> 1) & 1, 7, abort_flag);
           if (!CODES && ok && (vw[0] & vw[1] & vw[2] & vw[3]) != ~0u) {
-            // (a row's 16-byte pieces keep their row under the swizzle)
-            const uint32_t v = smem_u32(sKV + (2 * ((t + 1) & 1) + 1) * C::TILE_BYTES);
-            const int piece = lane & 7;
-#pragma unroll 1
-            for (int r4 = 0; r4 < BKV; r4 += 4) {
-              const int row = r4 + (lane >> 3);
-              const uint32_t keep = r4 < 64 ? (r4 < 32 ? vw[0] : vw[1]) : (r4 < 96 ? vw[2] : vw[3]);
-              if (((keep >> (row & 31)) & 1u) == 0) {
-#pragma unroll
-                for (int h = 0; h < C::HALVES; ++h)
-                  asm volatile("st.shared.v4.u32 [%0], {%1,%1,%1,%1};" ::"r"(v + h * C::HALF_BYTES + row * 128 + piece * 16),
-                               "r"(0u)
-                               : "memory");
-              }
-            }
+            zero_left_out<C::HALVES>(smem_u32(sKV + (2 * ((t + 1) & 1) + 1) * C::TILE_BYTES), vw, lane);
             fence_proxy_async_smem();
           }
         }
