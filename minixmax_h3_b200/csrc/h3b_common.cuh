@@ -204,6 +204,14 @@ H3B_DEV void tma_load_4d(void* smem_dst, const CUtensorMap* map, int32_t x, int3
       : "memory");
 }
 
+// The tile into L2 only, ahead of its load.
+H3B_DEV void tma_prefetch_4d(const CUtensorMap* map, int32_t x, int32_t y, int32_t z, int32_t w) {
+  asm volatile("cp.async.bulk.prefetch.tensor.4d.L2.global.tile [%0, {%1, %2, %3, %4}];" ::"l"(
+                   reinterpret_cast<uint64_t>(map)),
+               "r"(x), "r"(y), "r"(z), "r"(w)
+               : "memory");
+}
+
 H3B_DEV void bulk_load(void* smem_dst, const void* gmem_src, uint32_t bytes, uint64_t* bar) {
   asm volatile(
       "cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(

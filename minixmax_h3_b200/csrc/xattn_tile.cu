@@ -65,7 +65,7 @@ struct Cfg {
   static constexpr bool CODES = KIND != KV_DENSE;
   // Q ring (128-row tiles).  Over a cache a unit is long, and the codes' own
   // two tiles take the room of the third slot.
-  static constexpr int QST = CODES ? 2 : 3;
+  static constexpr int QST = CODES ? 2 : (D == 128 ? 3 : 6);
   static constexpr int RAW_BYTES = CODES ? 128 * D : 0;  // codes of a K or V tile
   static constexpr int HALVES = D / 64;            // 64-column TMA boxes of a tile
   static constexpr int TILE_BYTES = 128 * D * 2;   // Q, K or V
@@ -82,8 +82,10 @@ enum : uint32_t {
   R_PV_FIRST = 32, // of its unit: O starts anew
   R_PV_LAST = 64,  // O is complete after it
   R_END = 128,     // the last round
-  R_Q0_SHIFT = 8,  // Q slots of S_0, S_1
-  R_Q1_SHIFT = 10
+  R_S_FIRST = 256, // of its unit: Q_1 has to be waited for, at
+  R_Q1_PHASE = 512,  // this parity
+  R_Q0_SHIFT = 10, // Q slots of S_0, S_1
+  R_Q1_SHIFT = 13
 };
 
 // What the softmax warps of a row tile have to know of a tile, by warp 10.
@@ -101,8 +103,8 @@ constexpr int INFOS = 4;  // ring: entry s + 4 is written after round s + 2, so 
 
 struct __align__(16) Bars {
   TileInfo info[2][INFOS];
-  uint64_t q_full[3];
-  uint64_t q_free[3];
+  uint64_t q_full[6];
+  uint64_t q_free[6];
   uint64_t raw_full[2];   // codes of K, of V
   uint64_t raw_free[2];   // converted (4 warps)
   uint64_t kv_full[KVST];
@@ -556,6 +558,16 @@ __global__ void __launch_bounds__(THREADS, 1)
 #pragma unroll 1
         for (int j = 0; j < u.n && ok; ++j, ++t) {
           if (CODES && j == 0) look_up(u, 0);
+          if (!CODES && j == 0) {  // the next unit's Q into L2: its slots come free late
+            Unit v = u;
+            v.next<false>(args);
+            if (v.x < args.units && v.n > 0) {
+              for (int h = 0; h < C::HALVES; ++h) {
+                tma_prefetch_4d(&tm_q, h * 64, v.q0, v.head, v.b);
+                if (v.two) tma_prefetch_4d(&tm_q, h * 64, v.q0 + BQ, v.head, v.b);
+              }
+            }
+          }
           if (j == 0) ok = load_q(u, 0);
           if (ok && (ok = load_kv(&tm_k, u, j, t, 0))) loaded = 2 * t + 1;
           if (ok && j == 0 && u.two) ok = load_q(u, 1);
@@ -600,7 +612,7 @@ __global__ void __launch_bounds__(THREADS, 1)
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
           const bool do_pv = (r & (i ? R_PV1 : R_PV0)) != 0, do_s = (r & (i ? R_S1 : R_S0)) != 0;
-          const uint32_t qs = (r >> (i ? R_Q1_SHIFT : R_Q0_SHIFT)) & 3u;
+          const uint32_t qs = (r >> (i ? R_Q1_SHIFT : R_Q0_SHIFT)) & 7u;
           const uint64_t qd = sdesc_kmajor_sw128(smem_u32(sQ + qs * C::TILE_BYTES));
           const uint32_t s_tmem = tmem + s_col(i), o_tmem = tmem + o_col(i);
           if (do_pv) {
@@ -624,6 +636,9 @@ __global__ void __launch_bounds__(THREADS, 1)
             ok = lane_wait<true>(&bars->p_half[i][1], (phases >> i) & 1, 5, abort_flag) && ok;
             phases ^= 1u << i;
           }
+          // (Q_1 is loaded half a round later than Q_0: its slot is Q_0's of the unit before)
+          if (i == 1 && do_s && (r & R_S_FIRST))
+            ok = lane_wait<true>(&bars->q_full[qs], (r & R_Q1_PHASE) ? 1u : 0u, 3, abort_flag) && ok;
           __syncwarp();
           tc_fence_after();
           if (elect_one()) {
@@ -655,7 +670,7 @@ __global__ void __launch_bounds__(THREADS, 1)
     } else if (warp == 10) {
       // ------------------------------------------------------------ rounds
       // Ahead of the issuing warp: says what round t consists of, waits for
-      // K_t, V_{t-1} and at a unit's start its Q tiles, and zeroes the rows of
+      // K_t, V_{t-1} and at a unit's start its Q_0, and zeroes the rows of
       // V_{t-1} that are left out.  It is at most two rounds ahead (K_t
       // overwrites K_{t-2}, released with round t - 2), so todo[] and ready[]
       // of that parity are free again, and every tile's barrier is waited for
@@ -679,7 +694,8 @@ __global__ void __launch_bounds__(THREADS, 1)
         if (more) {
           const uint32_t mb = masked ? mask_bytes(a, u.b, key0, u.len, lane) : 0u;
           r |= R_S0 | (u.two ? R_S1 : 0u) | (j == u.n - 1 ? R_S_LAST : 0u) | ((qc % QST) << R_Q0_SHIFT) |
-               (((qc + 1) % QST) << R_Q1_SHIFT);
+               (((qc + 1) % QST) << R_Q1_SHIFT) | (j == 0 ? R_S_FIRST : 0u) |
+               ((((qc + 1) / QST) & 1) ? R_Q1_PHASE : 0u);
           if constexpr (CODES) {
             if (lane < 4) {
               if (j == 0) id_ahead = block_of(a, u.b, key0 + 32 * lane);
@@ -692,10 +708,7 @@ __global__ void __launch_bounds__(THREADS, 1)
             }
           }
           ok = warp_wait(&bars->kv_full[2 * (t & 1)], (t >> 1) & 1, 9, abort_flag);
-          if (j == 0) {
-            ok = ok && warp_wait(&bars->q_full[qc % QST], (qc / QST) & 1, 3, abort_flag);
-            if (u.two) ok = ok && warp_wait(&bars->q_full[(qc + 1) % QST], ((qc + 1) / QST) & 1, 3, abort_flag);
-          }
+          if (j == 0) ok = ok && warp_wait(&bars->q_full[qc % QST], (qc / QST) & 1, 3, abort_flag);
           keep_words(masked, mb, u.len - key0, w);
         }
         float kf = 1.0f, vs = 1.0f;
@@ -730,13 +743,6 @@ __global__ void __launch_bounds__(THREADS, 1)
         const bool two = u.two;
         if (more) {
           pv = R_PV0 | (two ? R_PV1 : 0u) | (j == 0 ? R_PV_FIRST : 0u) | (j == u.n - 1 ? R_PV_LAST : 0u);
-          if (++j == u.n) {
-            j = 0;
-            qc += two ? 2 : 1;
-            do {
-              u.next(args);
-            } while (u.x < args.units && u.n == 0);
-          }
         }
         end = pv == 0;
         if (lane < 2 && (lane == 0 || two || end)) {
@@ -767,6 +773,13 @@ __global__ void __launch_bounds__(THREADS, 1)
         for (int c = 0; c < 4; ++c) vw[c] = w[c];
         __syncwarp();
         if (lane == 0) mbar_arrive(&bars->ready[t & 1]);
+        if (more && ++j == u.n) {
+          j = 0;
+          qc += two ? 2 : 1;
+          do {
+            u.next(args);
+          } while (u.x < args.units && u.n == 0);
+        }
       }
     }
   } else if (warp < 8) {
@@ -929,16 +942,6 @@ __global__ void __launch_bounds__(THREADS, 1)
     const uint32_t lane_off = static_cast<uint32_t>((warp & 3) * 32) << 16;
     const int64_t total_rows = static_cast<int64_t>(a.batch) * a.heads * a.s_q;
     uint32_t oc0 = 0, oc1 = 0;
-    auto release = [&](int i, int n) {  // O_i and the statistics are read
-      if (n > 0) {
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) {
-          mbar_arrive(&bars->o_free[i]);
-          mbar_arrive(&bars->ml_free[i]);
-        }
-      }
-    };
     bool ok = true;
     auto store = [&](const Unit& u) {  // a unit's rows
 #pragma unroll 1
@@ -947,7 +950,7 @@ __global__ void __launch_bounds__(THREADS, 1)
         float2 ml = make_float2(-INFINITY, 0.0f);
         const uint32_t phase = (i ? oc1 : oc0) & 1;
         if (u.n > 0) {
-          // both complete once a unit, and again only after this warp's release
+          // both complete once a unit, and again only after this warp's arrivals below
           ok = warp_wait(&bars->ml_full[i], phase, 23, abort_flag) &&
                warp_wait(&bars->o_full[i], phase, 24, abort_flag);
           if (!ok) continue;
@@ -959,18 +962,31 @@ __global__ void __launch_bounds__(THREADS, 1)
         const bool in = q_row < a.s_q;
         const int64_t lse_row = (static_cast<int64_t>(u.b) * a.heads + u.head) * a.s_q + q_row;
         const float inv_l = ml.y > 0.0f ? 1.0f / ml.y : 0.0f;
-        if (a.splits > 1) {
-          float* prow = a.part_o + (u.split * total_rows + lse_row) * D;
+        // 32 columns at a time in a rolled loop: this code runs once a unit, so
+        // it is fetched anew each time (unrolled, a 128-row tile took 4500
+        // cycles).  O is given back before its last columns are stored.
+        uint16_t* orow =
+            static_cast<uint16_t*>(a.o) + u.b * a.o_stride[0] + q_row * a.o_stride[1] + u.head * a.o_stride[2];
+        float* prow = a.part_o + (u.split * total_rows + lse_row) * D;
 #pragma unroll 1
-          for (int c = 0; c < D / 32; ++c) {
-            uint32_t r[32];
-            if (u.n > 0) {
-              tmem_ld32p(tmem + o_col(i) + c * 32 + lane_off, r);
-              tmem_wait_fence<1>(r);
-            } else {
-#pragma unroll
-              for (int e = 0; e < 32; ++e) r[e] = 0u;
+        for (int c = 0; c < D / 32; ++c) {
+          uint32_t r[32];
+          if (u.n > 0) {
+            tmem_ld32p(tmem + o_col(i) + c * 32 + lane_off, r);
+            tmem_wait_fence<1>(r);
+            if (c == D / 32 - 1) {  // O_i and the statistics are read
+              tc_fence_before();
+              __syncwarp();
+              if (lane == 0) {
+                mbar_arrive(&bars->o_free[i]);
+                mbar_arrive(&bars->ml_free[i]);
+              }
             }
+          } else {
+#pragma unroll
+            for (int e = 0; e < 32; ++e) r[e] = 0u;
+          }
+          if (a.splits > 1) {
             if (in) {
 #pragma unroll
               for (int e = 0; e < 32; e += 8) {
@@ -980,43 +996,28 @@ __global__ void __launch_bounds__(THREADS, 1)
                 st_global_v8(prow + c * 32 + e, v);
               }
             }
-            __syncwarp();  // the next tcgen05.ld is for the whole warp
-          }
-          release(i, u.n);
-        } else {
-          // O is read and rounded into half the registers, given back, and
-          // only then stored: the next unit's first P V waits for it.
-          uint32_t p[D / 2];
-          if (u.n > 0) {
-#pragma unroll
-            for (int c = 0; c < D / 32; ++c) {
-              uint32_t r[32];
-              tmem_ld32p(tmem + o_col(i) + c * 32 + lane_off, r);
-              tmem_wait_fence<1>(r);
-#pragma unroll
-              for (int e = 0; e < 16; ++e)
-                p[16 * c + e] = pack16x2<F16>(__uint_as_float(r[2 * e]) * inv_l, __uint_as_float(r[2 * e + 1]) * inv_l);
-            }
           } else {
 #pragma unroll
-            for (int e = 0; e < D / 2; ++e) p[e] = 0u;
-          }
-          release(i, u.n);
-          uint16_t* orow =
-              static_cast<uint16_t*>(a.o) + u.b * a.o_stride[0] + q_row * a.o_stride[1] + u.head * a.o_stride[2];
-          if (in && args.o_wide) {
-#pragma unroll
-            for (int e = 0; e < D / 2; e += 8) {
-              uint32_t v[8];
-#pragma unroll
-              for (int t = 0; t < 8; ++t) v[t] = p[e + t];
-              st_global_v8(orow + 2 * e, v);
+            for (int e = 0; e < 16; ++e) {
+              const float2 x = mul2(make_float2(__uint_as_float(r[2 * e]), __uint_as_float(r[2 * e + 1])),
+                                    make_float2(inv_l, inv_l));
+              r[e] = pack16x2<F16>(x.x, x.y);
             }
-          } else if (in) {
+            if (in && args.o_wide) {
 #pragma unroll
-            for (int e = 0; e < D / 2; e += 4)
-              *reinterpret_cast<uint4*>(orow + 2 * e) = make_uint4(p[e], p[e + 1], p[e + 2], p[e + 3]);
+              for (int e = 0; e < 16; e += 8) {
+                uint32_t v[8];
+#pragma unroll
+                for (int t = 0; t < 8; ++t) v[t] = r[e + t];
+                st_global_v8(orow + c * 32 + 2 * e, v);
+              }
+            } else if (in) {
+#pragma unroll
+              for (int e = 0; e < 16; e += 4)
+                *reinterpret_cast<uint4*>(orow + c * 32 + 2 * e) = make_uint4(r[e], r[e + 1], r[e + 2], r[e + 3]);
+            }
           }
+          __syncwarp();  // the next tcgen05.ld is for the whole warp
         }
         if (in) {
           if (a.splits > 1) {
