@@ -33,7 +33,26 @@ int64_t rows_of(const XAttn& a) { return static_cast<int64_t>(a.batch) * a.heads
 // exist or not; the row kernel on 32 rows of the heads that share a key head.
 bool by_tiles(const XAttn& a) { return a.s_q >= 64; }
 
-void plan(XAttn& a) { a.splits = by_tiles(a) ? h3b::xattn_tile_splits(a) : h3b::xattn_rows_splits(a); }
+// (The last call's plan is kept by its sizes: a model's layers repeat them,
+// and the search is 2 us of divisions on calls of 10.)
+void plan(XAttn& a) {
+  struct Sizes {
+    int kind, batch, heads, kv_heads, head_dim, s_q, s_kv, sms;
+    bool operator==(const Sizes& o) const {
+      return kind == o.kind && batch == o.batch && heads == o.heads && kv_heads == o.kv_heads &&
+             head_dim == o.head_dim && s_q == o.s_q && s_kv == o.s_kv && sms == o.sms;
+    }
+  };
+  static thread_local Sizes last{};
+  static thread_local int splits = 0;
+  const Sizes now{a.kind == h3b::KV_DENSE ? 0 : 1, a.batch, a.heads, a.kv_heads, a.head_dim, a.s_q, a.s_kv,
+                  h3b::num_sms()};
+  if (splits == 0 || !(now == last)) {
+    splits = by_tiles(a) ? h3b::xattn_tile_splits(a) : h3b::xattn_rows_splits(a);
+    last = now;
+  }
+  a.splits = splits;
+}
 
 int64_t workspace_of(const XAttn& a) {
   return a.splits > 1 ? rows_of(a) * a.splits * (a.head_dim + 2) * static_cast<int64_t>(sizeof(float)) : 0;

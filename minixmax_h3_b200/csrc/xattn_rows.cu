@@ -704,8 +704,9 @@ int xattn_rows_splits(const XAttn& a) {
   int best = 1;
   int64_t cost = INT64_MAX;
   for (int64_t s = 1; s <= 128 && (s == 1 || s <= steps); ++s) {
-    // (joining splits is a second launch, about five steps)
-    const int64_t c = ((ctas * s + slots - 1) / slots) * ((steps + s - 1) / s + 2) + (s > 1 ? 5 : 0);
+    // (joining splits is a second launch: 2 us on the host, 4 on the GPU, or
+    // about eight steps)
+    const int64_t c = ((ctas * s + slots - 1) / slots) * ((steps + s - 1) / s + 2) + (s > 1 ? 8 : 0);
     if (c < cost) {
       cost = c;
       best = static_cast<int>(s);
