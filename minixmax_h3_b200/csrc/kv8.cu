@@ -243,9 +243,62 @@ __global__ void __launch_bounds__(THREADS) kv8_read_kernel(const __grid_constant
   }
 }
 
+// The codes themselves (no scale) as 16-bit numbers in the order of the
+// tokens, heads first: each is exact.  Tokens up to the next 128 behind a
+// sequence's length, and absent blocks, are 0; what lies further is not written.
+template <int D, bool E4M3, bool F16>
+__global__ void __launch_bounds__(THREADS) kv8_expand_kernel(const __grid_constant__ h3b::XAttn a) {
+  constexpr int VPR = D / 16;
+  const int64_t i = static_cast<int64_t>(blockIdx.x) * THREADS + threadIdx.x;
+  const int col = static_cast<int>(i % VPR) * 16;
+  const int64_t row = i / VPR;  // (b, head, token)
+  const int tok = static_cast<int>(row % a.s_kv);
+  const int64_t bh = row / a.s_kv;
+  const int head = static_cast<int>(bh % a.kv_heads);
+  const int64_t b = bh / a.kv_heads;
+  if (b >= a.batch) return;
+  const int len = max(0, min(a.s_kv, a.kv_lens[b]));
+  if (tok >= (len + 127) / 128 * 128) return;
+  const int id = a.table[b * a.max_blocks + tok / a.block_tokens];
+  uint32_t w[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+  if (tok < len && id >= 0 && id < a.num_blocks) {
+    const int64_t slab = static_cast<int64_t>(id) * a.kv_heads + head;
+    const uint4 c = __ldcs(reinterpret_cast<const uint4*>(static_cast<const uint8_t*>(blockIdx.y ? a.v : a.k) +
+                                                          (slab * a.block_tokens + tok % a.block_tokens) * D + col));
+    const uint32_t u[4] = {c.x, c.y, c.z, c.w};
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      float y[4];
+      from_codes4<E4M3>(u[k], y);
+      w[2 * k] = pack16x2<F16>(y[0], y[1]);
+      w[2 * k + 1] = pack16x2<F16>(y[2], y[3]);
+    }
+  }
+  st_global_v8(static_cast<uint16_t*>(blockIdx.y ? a.pre_v : a.pre_k) + row * D + col, w);
+}
+
 bool block_ok(int64_t bt) { return bt == 32 || bt == 64 || bt == 128; }
 
 }  // namespace
+
+namespace h3b {
+
+int kv8_expand_launch(const XAttn& a, cudaStream_t stream) {
+  const int64_t gx = (static_cast<int64_t>(a.batch) * a.kv_heads * a.s_kv * (a.head_dim / 16) + THREADS - 1) / THREADS;
+  if (gx > 0x7fffffffll) return H3B_ERR_SHAPE;
+  const dim3 grid(static_cast<unsigned>(gx), 2);
+  const bool f16 = a.dtype == H3B_F16, e4 = a.kind == KV_E4M3;
+#define H3B_EXPAND(DD)                                                                       \
+  (e4 ? (f16 ? kv8_expand_kernel<DD, true, true><<<grid, THREADS, 0, stream>>>(a)            \
+             : kv8_expand_kernel<DD, true, false><<<grid, THREADS, 0, stream>>>(a))          \
+      : (f16 ? kv8_expand_kernel<DD, false, true><<<grid, THREADS, 0, stream>>>(a)           \
+             : kv8_expand_kernel<DD, false, false><<<grid, THREADS, 0, stream>>>(a)))
+  if (a.head_dim == 128) H3B_EXPAND(128); else H3B_EXPAND(64);
+#undef H3B_EXPAND
+  return launch_status();
+}
+
+}  // namespace h3b
 
 extern "C" int h3b_kv8_append(const void* k, const void* v, int x_dtype, int64_t batch, int64_t n, int64_t kv_heads,
                               int64_t head_dim, int64_t batch_stride, int64_t seq_stride, int64_t head_stride,

@@ -54,9 +54,23 @@ void plan(XAttn& a) {
   a.splits = splits;
 }
 
-int64_t workspace_of(const XAttn& a) {
+// Whether a cache's codes are written out as 16-bit operands first; else each
+// 256-row tile of each query head converts them anew.  32768 int8 tokens x 24
+// heads, bf16, us with and without: 256 rows 229 / 177, 512 rows 314 / 329, 768
+// rows 404 / 475, 1560 rows 853 / 1279.  At most 8 GB of workspace.
+int64_t expand_bytes(const XAttn& a) {
+  const int64_t times = static_cast<int64_t>(a.heads / a.kv_heads) * ((a.s_q + 255) / 256);
+  if (a.kind == h3b::KV_DENSE || !by_tiles(a) || times < 2) return 0;
+  const int64_t n = 2ll * a.batch * a.kv_heads * a.s_kv * a.head_dim * 2;
+  return n <= (8ll << 30) ? n : 0;
+}
+
+int64_t part_bytes(const XAttn& a) {
   return a.splits > 1 ? rows_of(a) * a.splits * (a.head_dim + 2) * static_cast<int64_t>(sizeof(float)) : 0;
 }
+
+// Workspace: 16-bit operands of K and V, then the splits' partial rows.
+int64_t workspace_of(const XAttn& a) { return expand_bytes(a) + part_bytes(a); }
 
 int run(XAttn& a, void* workspace, int64_t workspace_bytes, cudaStream_t stream) {
   plan(a);
@@ -65,7 +79,12 @@ int run(XAttn& a, void* workspace, int64_t workspace_bytes, cudaStream_t stream)
     if (workspace == nullptr) return H3B_ERR_ARG;
     if (workspace_bytes < need) return H3B_ERR_SHAPE;
     if ((reinterpret_cast<uintptr_t>(workspace) & 31u) != 0) return H3B_ERR_ALIGN;
-    a.part_o = static_cast<float*>(workspace);
+    const int64_t pre = expand_bytes(a);
+    if (pre > 0) {
+      a.pre_k = workspace;
+      a.pre_v = static_cast<uint8_t*>(workspace) + pre / 2;
+    }
+    a.part_o = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + pre);
     a.part_ml = reinterpret_cast<float2*>(a.part_o + rows_of(a) * a.splits * a.head_dim);
   }
   return by_tiles(a) ? h3b::xattn_tile_launch(a, stream) : h3b::xattn_rows_launch(a, stream);

@@ -37,6 +37,8 @@ struct XAttn {
   int max_blocks, block_tokens, num_blocks;
   const float* k_scale;  // [num_blocks, kv_heads]
   const float* v_scale;
+  void* pre_k;  // workspace [batch, kv_heads, s_kv, head_dim] of 16-bit operands, or null: see xattn_tile.cu
+  void* pre_v;
   int causal;  // query i of s_q sees keys < kv_len - s_q + i + 1
   float scale;
   // split calls: partial results of `splits` key ranges per row
@@ -76,6 +78,8 @@ int xattn_tile_splits(const XAttn& a);
 
 int xattn_rows_launch(const XAttn& a, cudaStream_t stream);
 int xattn_tile_launch(const XAttn& a, cudaStream_t stream);
+// Writes a cache's codes out as 16-bit numbers of q's type into pre_k, pre_v.
+int kv8_expand_launch(const XAttn& a, cudaStream_t stream);
 // Joins the ranges of a split call into o and lse.
 int xattn_combine_launch(const XAttn& a, cudaStream_t stream);
 

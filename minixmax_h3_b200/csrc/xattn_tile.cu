@@ -60,9 +60,13 @@ constexpr float RESCALE_THRESHOLD = 8.0f;
 constexpr float LOG2E = 1.4426950408889634f;
 constexpr float LN2 = 0.69314718055994531f;
 
-template <int D, KvKind KIND>
+// PRE: a cache whose codes a kernel before this one has written out as 16-bit
+// operands (kv8.cu), for calls of many query tiles; else its codes are
+// converted here, once a tile and unit.
+template <int D, KvKind KIND, bool PRE>
 struct Cfg {
-  static constexpr bool CODES = KIND != KV_DENSE;
+  static constexpr bool SCALED = KIND != KV_DENSE;
+  static constexpr bool CODES = SCALED && !PRE;  // converted here
   // Q ring (128-row tiles).  Over a cache a unit is long, and the codes' own
   // two tiles take the room of the third slot.
   static constexpr int QST = CODES ? 2 : (D == 128 ? 3 : 6);
@@ -122,12 +126,12 @@ struct __align__(16) Bars {
   int abort_flag;
 };
 
-template <int D, KvKind KIND>
+template <int D, KvKind KIND, bool PRE>
 constexpr size_t smem_bytes() {
-  using C = Cfg<D, KIND>;
+  using C = Cfg<D, KIND, PRE>;
   return (C::QST + KVST) * C::TILE_BYTES + 2 * C::RAW_BYTES + 2 * 128 * sizeof(float2) + sizeof(Bars);
 }
-static_assert(smem_bytes<128, KV_DENSE>() <= 232448 && smem_bytes<128, KV_INT8>() <= 232448, "shared memory of a CTA");
+static_assert(smem_bytes<128, KV_DENSE, false>() <= 232448 && smem_bytes<128, KV_INT8, false>() <= 232448, "shared memory of a CTA");
 
 struct TileArgs {
   XAttn a;
@@ -427,12 +431,12 @@ H3B_DEV int block_of(const XAttn& a, int b, int key) {
   return id >= 0 && id < a.num_blocks ? id : -1;
 }
 
-template <int D, bool F16, KvKind KIND, bool MASKED>
+template <int D, bool F16, KvKind KIND, bool MASKED, bool PRE>
 __global__ void __launch_bounds__(THREADS, 1)
     xattn_tile_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
                       const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ TileArgs args) {
-  using C = Cfg<D, KIND>;
-  constexpr bool CODES = C::CODES;
+  using C = Cfg<D, KIND, PRE>;
+  constexpr bool CODES = C::CODES, SCALED = C::SCALED;
   constexpr int QST = C::QST;
   constexpr uint32_t IDESC_S = F16 ? idesc_f16_f32(128, BKV, 0, 0) : idesc_bf16_f32(128, BKV, 0, 0);
   constexpr uint32_t IDESC_O = F16 ? idesc_f16_f32(128, D, 0, 1) : idesc_bf16_f32(128, D, 0, 1);
@@ -696,7 +700,7 @@ __global__ void __launch_bounds__(THREADS, 1)
           r |= R_S0 | (u.two ? R_S1 : 0u) | (j == u.n - 1 ? R_S_LAST : 0u) | ((qc % QST) << R_Q0_SHIFT) |
                (((qc + 1) % QST) << R_Q1_SHIFT) | (j == 0 ? R_S_FIRST : 0u) |
                ((((qc + 1) / QST) & 1) ? R_Q1_PHASE : 0u);
-          if constexpr (CODES) {
+          if constexpr (SCALED) {
             if (lane < 4) {
               if (j == 0) id_ahead = block_of(a, u.b, key0 + 32 * lane);
               id_here = id_ahead;
@@ -712,7 +716,7 @@ __global__ void __launch_bounds__(THREADS, 1)
           keep_words(masked, mb, u.len - key0, w);
         }
         float kf = 1.0f, vs = 1.0f;
-        if constexpr (CODES) {
+        if constexpr (SCALED) {
           // lane g (of four): the block of columns 32 g .., its scales, looked
           // up while the tile was awaited (the block of the next one, too)
           int id = 0;
@@ -755,7 +759,7 @@ __global__ void __launch_bounds__(THREADS, 1)
           info->causal = sees;
           info->flags = end ? static_cast<uint32_t>(T_END) : sees < BKV ? (flags & ~T_WHOLE) | T_CAUSAL : flags;
         }
-        if constexpr (CODES) {
+        if constexpr (SCALED) {
           if (lane < 4) {
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
@@ -853,7 +857,7 @@ __global__ void __launch_bounds__(THREADS, 1)
             }
           }
           float fx[4], ox[4];
-          if constexpr (CODES) {
+          if constexpr (SCALED) {
 #pragma unroll
             for (int g = 0; g < 4; ++g) {
               fx[g] = info->k_factor[g];
@@ -862,7 +866,7 @@ __global__ void __launch_bounds__(THREADS, 1)
           }
           if (slow) {
             float m_tile;
-            if constexpr (CODES) {
+            if constexpr (SCALED) {
               m_tile = -INFINITY;
 #pragma unroll
               for (int g = 0; g < 4; ++g) m_tile = fmaxf(m_tile, fmaf(row_max32(r + 32 * g), fx[g], ox[g]));
@@ -893,7 +897,7 @@ __global__ void __launch_bounds__(THREADS, 1)
           }
           const float neg_m = m_use == -INFINITY ? 0.0f : -m_use;
           float2 sm;
-          if constexpr (CODES) {
+          if constexpr (SCALED) {
             sm = exp_codes64<F16, true>(r, r, make_float2(fx[0], fx[1]), make_float2(ox[0] + neg_m, ox[1] + neg_m),
                                         make_float2(info->v_inv[0], info->v_inv[1]), fx, ox);
           } else {
@@ -909,7 +913,7 @@ __global__ void __launch_bounds__(THREADS, 1)
         for (int h = 0; h < 2; ++h) {
           if (h == 1) {
             const float neg_m = m_use == -INFINITY ? 0.0f : -m_use;
-            if constexpr (CODES) {
+            if constexpr (SCALED) {
               const float f[4] = {0.f, 0.f, 0.f, 0.f};
               sum += exp_codes64<F16, false>(r + 64, r + 32, make_float2(info->k_factor[2], info->k_factor[3]),
                                              make_float2(info->v_log2[2] + neg_m, info->v_log2[3] + neg_m),
@@ -1089,7 +1093,7 @@ __global__ void __launch_bounds__(THREADS, 1)
   }
 }
 
-template <int D, bool F16, KvKind KIND, bool MASKED = false>
+template <int D, bool F16, KvKind KIND, bool MASKED = false, bool PRE = false>
 int launch(const XAttn& a, cudaStream_t stream) {
   const CUtensorMapDataType dt = F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
   CUtensorMap tq, tk, tv;
@@ -1102,7 +1106,11 @@ int launch(const XAttn& a, cudaStream_t stream) {
     return h3b::encode_4d(m, dt, p, dims, sb, box, CU_TENSOR_MAP_SWIZZLE_128B);
   };
   int rc = encode(&tq, a.q, a.q_stride, a.s_q, a.heads);
-  if constexpr (KIND == KV_DENSE) {
+  if constexpr (PRE) {  // [batch, kv_heads, s_kv, D]
+    const int64_t st[3] = {static_cast<int64_t>(a.kv_heads) * a.s_kv * D, D, static_cast<int64_t>(a.s_kv) * D};
+    if (rc == H3B_OK) rc = encode(&tk, a.pre_k, st, a.s_kv, a.kv_heads);
+    if (rc == H3B_OK) rc = encode(&tv, a.pre_v, st, a.s_kv, a.kv_heads);
+  } else if constexpr (KIND == KV_DENSE) {
     if (rc == H3B_OK) rc = encode(&tk, a.k, a.kv_stride, a.s_kv, a.kv_heads);
     if (rc == H3B_OK) rc = encode(&tv, a.v, a.kv_stride, a.s_kv, a.kv_heads);
   } else {
@@ -1115,10 +1123,10 @@ int launch(const XAttn& a, cudaStream_t stream) {
                           D, rows, 1, sw);
   }
   if (rc != H3B_OK) return rc;
-  auto kernel = xattn_tile_kernel<D, F16, KIND, MASKED>;
+  auto kernel = xattn_tile_kernel<D, F16, KIND, MASKED, PRE>;
   static bool attr = false;
   if (!attr) {
-    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem_bytes<D, KIND>())) !=
+    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem_bytes<D, KIND, PRE>())) !=
         cudaSuccess)
       return H3B_ERR_LAUNCH;
     attr = true;
@@ -1141,7 +1149,7 @@ int launch(const XAttn& a, cudaStream_t stream) {
   step /= a.splits;
   args.step_head = step % a.heads;
   args.step_b = step / a.heads;
-  kernel<<<static_cast<unsigned>(units < sms ? units : sms), THREADS, smem_bytes<D, KIND>(), stream>>>(tq, tk, tv, args);
+  kernel<<<static_cast<unsigned>(units < sms ? units : sms), THREADS, smem_bytes<D, KIND, PRE>(), stream>>>(tq, tk, tv, args);
   return h3b::launch_status();
 }
 
@@ -1174,8 +1182,13 @@ namespace {
 template <int D, bool F16>
 int launch_kind(const XAttn& a, cudaStream_t stream) {
   switch (a.kind) {
-    case KV_INT8: return launch<D, F16, KV_INT8>(a, stream);
-    case KV_E4M3: return launch<D, F16, KV_E4M3>(a, stream);
+    case KV_INT8:
+    case KV_E4M3:
+      if (a.pre_k != nullptr) {  // written out: the kinds are the same then
+        const int rc = kv8_expand_launch(a, stream);
+        return rc == H3B_OK ? launch<D, F16, KV_INT8, false, true>(a, stream) : rc;
+      }
+      return a.kind == KV_INT8 ? launch<D, F16, KV_INT8>(a, stream) : launch<D, F16, KV_E4M3>(a, stream);
     default:
       return a.key_mask != nullptr ? launch<D, F16, KV_DENSE, true>(a, stream) : launch<D, F16, KV_DENSE>(a, stream);
   }
