@@ -566,6 +566,7 @@ __global__ void __launch_bounds__(THREADS, 1)
             st_global_v8(out + c * 32 + e, v);
           }
         }
+        __syncwarp();  // the next tcgen05.ld is for the whole warp
       }
       tc_fence_before();
     }
@@ -965,8 +966,7 @@ __global__ void __launch_bounds__(THREADS, 1)
 #pragma unroll
           for (int e = 0; e < 32; ++e) r[e] = 0u;
         }
-        if (key >= a.s_kv) continue;
-        if (a.splits > 1) {
+        if (key < a.s_kv && a.splits > 1) {
           float* dst = a.part + ((wg * static_cast<int64_t>(a.splits) + u.split) * per_split + key_row) * D + c * 32;
 #pragma unroll
           for (int e = 0; e < 32; e += 8) {
@@ -975,7 +975,7 @@ __global__ void __launch_bounds__(THREADS, 1)
             for (int t = 0; t < 8; ++t) v[t] = __float_as_uint(__uint_as_float(r[e + t]) * f);
             st_global_v8(dst + e, v);
           }
-        } else {
+        } else if (key < a.s_kv) {
           uint16_t* dst = static_cast<uint16_t*>(wg ? a.dk : a.dv) + key_row * D + c * 32;
 #pragma unroll
           for (int e = 0; e < 32; e += 16) {
@@ -986,6 +986,7 @@ __global__ void __launch_bounds__(THREADS, 1)
             st_global_v8(dst + e, v);
           }
         }
+        __syncwarp();  // the next tcgen05.ld is for the whole warp
       }
       tc_fence_before();
     }
