@@ -205,6 +205,7 @@ extern "C" int h3b_cross_attention_bwd(const void* d_o, const void* q, const voi
                ? H3B_OK
                : H3B_ERR_LAUNCH;
   }
+  if (batch * heads * s_q > 0x7fffffffll) return H3B_ERR_SHAPE;
   h3b::XAttnGrad a = grad_sizes(dtype, batch, heads, kv_heads, head_dim, s_q, s_kv);
   a.q = q, a.k = s_kv > 0 ? k : q, a.v = s_kv > 0 ? v : q, a.o = o, a.d_o = d_o, a.lse = lse;
   a.dq = dq, a.dk = dk, a.dv = dv;

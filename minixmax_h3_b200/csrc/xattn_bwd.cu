@@ -587,34 +587,49 @@ __global__ void __launch_bounds__(THREADS, 1)
 template <int D, bool F16>
 __global__ void __launch_bounds__(256) xattn_delta_kernel(const __grid_constant__ XAttnGrad a) {
   constexpr int LPR = D / 8;
-  const int64_t i = (static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x) / LPR;  // (b, token, head)
+  constexpr int ROWS = 4;  // a thread's loads in flight
+  // (32-bit row numbers: 2^31 rows would be 274 GB of q)
+  const uint32_t first = blockIdx.x * (256 / LPR) * ROWS + threadIdx.x / LPR;
   const int col = (threadIdx.x % LPR) * 8;
-  const int64_t rows = static_cast<int64_t>(a.batch) * a.s_q * a.heads;
-  float s = 0.0f;
-  const int head = static_cast<int>(i % a.heads);
-  const int64_t bt = i / a.heads;
-  const int64_t tok = bt % a.s_q, b = bt / a.s_q;
-  if (i < rows) {
-    const uint4 ov = __ldg(reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(a.o) + b * a.o_stride[0] +
-                                                          tok * a.o_stride[1] + head * a.o_stride[2] + col));
-    const uint4 gv = __ldg(reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(a.d_o) + b * a.do_stride[0] +
-                                                          tok * a.do_stride[1] + head * a.do_stride[2] + col));
-    const uint32_t ow[4] = {ov.x, ov.y, ov.z, ov.w}, gw[4] = {gv.x, gv.y, gv.z, gv.w};
+  const uint32_t rows = static_cast<uint32_t>(a.batch) * a.s_q * a.heads;
+  uint4 ov[ROWS], gv[ROWS];
+  int64_t at[ROWS];
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      if constexpr (F16) {
-        const float2 of = __half22float2(*reinterpret_cast<const __half2*>(&ow[k]));
-        const float2 gf = __half22float2(*reinterpret_cast<const __half2*>(&gw[k]));
-        s = fmaf(of.x, gf.x, fmaf(of.y, gf.y, s));
-      } else {
-        s = fmaf(bf16lo_to_f32(ow[k]), bf16lo_to_f32(gw[k]), s);
-        s = fmaf(bf16hi_to_f32(ow[k]), bf16hi_to_f32(gw[k]), s);
-      }
+  for (int k = 0; k < ROWS; ++k) {
+    const uint32_t i = first + k * (256 / LPR);  // (b, token, head)
+    at[k] = -1;
+    ov[k] = gv[k] = make_uint4(0, 0, 0, 0);
+    if (i < rows) {
+      const uint32_t bt = i / static_cast<uint32_t>(a.heads);
+      const int64_t head = i - bt * a.heads;
+      const uint32_t b32 = bt / static_cast<uint32_t>(a.s_q);
+      const int64_t b = b32, tok = bt - b32 * a.s_q;
+      ov[k] = __ldg(reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(a.o) + b * a.o_stride[0] +
+                                                   tok * a.o_stride[1] + head * a.o_stride[2] + col));
+      gv[k] = __ldg(reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(a.d_o) + b * a.do_stride[0] +
+                                                   tok * a.do_stride[1] + head * a.do_stride[2] + col));
+      at[k] = (b * a.heads + head) * a.s_q + tok;
     }
   }
 #pragma unroll
-  for (int o = LPR / 2; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-  if (i < rows && threadIdx.x % LPR == 0) a.delta[(b * a.heads + head) * a.s_q + tok] = s;
+  for (int k = 0; k < ROWS; ++k) {
+    const uint32_t ow[4] = {ov[k].x, ov[k].y, ov[k].z, ov[k].w}, gw[4] = {gv[k].x, gv[k].y, gv[k].z, gv[k].w};
+    float s = 0.0f;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      if constexpr (F16) {
+        const float2 of = __half22float2(*reinterpret_cast<const __half2*>(&ow[e]));
+        const float2 gf = __half22float2(*reinterpret_cast<const __half2*>(&gw[e]));
+        s = fmaf(of.x, gf.x, fmaf(of.y, gf.y, s));
+      } else {
+        s = fmaf(bf16lo_to_f32(ow[e]), bf16lo_to_f32(gw[e]), s);
+        s = fmaf(bf16hi_to_f32(ow[e]), bf16hi_to_f32(gw[e]), s);
+      }
+    }
+#pragma unroll
+    for (int o = LPR / 2; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+    if (at[k] >= 0 && threadIdx.x % LPR == 0) a.delta[at[k]] = s;
+  }
 }
 
 // ============================================================== dK and dV
@@ -1059,7 +1074,8 @@ int launch(const XAttnGrad& a, cudaStream_t stream) {
   const int64_t ku = static_cast<int64_t>(a.batch) * a.kv_heads * args.k_tiles * a.splits;
   if (qu > 0x3fffffff || ku > 0x3fffffff) return H3B_ERR_SHAPE;
   if (args.k_tiles > 1) {
-    const int64_t blocks = (static_cast<int64_t>(a.batch) * a.s_q * a.heads * (D / 8) + 255) / 256;
+    const int64_t per = 4 * 256 / (D / 8);  // rows of a block
+    const int64_t blocks = (static_cast<int64_t>(a.batch) * a.s_q * a.heads + per - 1) / per;
     if (blocks > 0x7fffffff) return H3B_ERR_SHAPE;
     xattn_delta_kernel<D, F16><<<static_cast<unsigned>(blocks), 256, 0, stream>>>(a);
     rc = h3b::launch_status();
