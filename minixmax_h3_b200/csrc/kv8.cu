@@ -27,6 +27,11 @@ namespace {
 
 constexpr int THREADS = 256;
 
+// log2 of a block's tokens (32, 64 or 128)
+__host__ __device__ constexpr int shift_of(int block_tokens) {
+  return block_tokens == 32 ? 5 : (block_tokens == 64 ? 6 : 7);
+}
+
 struct AppendArgs {
   const void* src[2];      // new K, new V: [batch, n, kv_heads, D]
   int64_t src_stride[3];   // batch, token, head (elements)
@@ -184,7 +189,7 @@ struct ReadArgs {
   void* dst[2];  // [batch, max_len, kv_heads, D] dense
   const int32_t* table;
   const int32_t* lens;
-  int batch, max_len, kv_heads, max_blocks, num_blocks, block_tokens;
+  int batch, max_len, kv_heads, max_blocks, num_blocks, block_shift;
 };
 
 // OUT: 0 bf16, 1 f16, 2 f32.  One thread = 16 codes of one token's head.
@@ -192,25 +197,26 @@ template <int D, bool E4M3, int OUT>
 __global__ void __launch_bounds__(THREADS) kv8_read_kernel(const __grid_constant__ ReadArgs args) {
   constexpr int VPR = D / 16;
   const int which = blockIdx.y;
-  const int64_t i = static_cast<int64_t>(blockIdx.x) * THREADS + threadIdx.x;
-  const int col = static_cast<int>(i % VPR) * 16;
-  const int64_t row = i / VPR;  // (b, token, head)
-  const int head = static_cast<int>(row % args.kv_heads);
-  const int64_t bt_row = row / args.kv_heads;
-  const int tok = static_cast<int>(bt_row % args.max_len);
-  const int64_t b = bt_row / args.max_len;
+  const int col = static_cast<int>(threadIdx.x % VPR) * 16;
+  // (32-bit row numbers: 2^31 rows of 64 values are 274 GB)
+  const uint32_t row = blockIdx.x * (THREADS / VPR) + threadIdx.x / VPR;  // (b, token, head)
+  const uint32_t bt_row = row / static_cast<uint32_t>(args.kv_heads);
+  const int head = static_cast<int>(row - bt_row * args.kv_heads);
+  const uint32_t b32 = bt_row / static_cast<uint32_t>(args.max_len);
+  const int tok = static_cast<int>(bt_row - b32 * args.max_len);
+  const int64_t b = b32;
   if (b >= args.batch) return;
   float x[16];
 #pragma unroll
   for (int e = 0; e < 16; ++e) x[e] = 0.0f;
-  const int blk = tok / args.block_tokens;
+  const int blk = tok >> args.block_shift;
   if (tok < args.lens[b] && blk < args.max_blocks) {
     const int id = args.table[b * args.max_blocks + blk];
     if (id >= 0 && id < args.num_blocks) {
       const int64_t slab = static_cast<int64_t>(id) * args.kv_heads + head;
       const float s = args.scale[which][slab];
       const uint4 w = __ldcs(reinterpret_cast<const uint4*>(
-          args.codes[which] + (slab * args.block_tokens + tok % args.block_tokens) * D + col));
+          args.codes[which] + ((slab << args.block_shift) + tok - (blk << args.block_shift)) * D + col));
       const uint32_t u[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
@@ -221,7 +227,7 @@ __global__ void __launch_bounds__(THREADS) kv8_read_kernel(const __grid_constant
       }
     }
   }
-  const int64_t at = row * D + col;
+  const int64_t at = static_cast<int64_t>(row) * D + col;
   if constexpr (OUT == 2) {
     float4* dst = reinterpret_cast<float4*>(static_cast<float*>(args.dst[which]) + at);
 #pragma unroll
@@ -249,22 +255,22 @@ __global__ void __launch_bounds__(THREADS) kv8_read_kernel(const __grid_constant
 template <int D, bool E4M3, bool F16>
 __global__ void __launch_bounds__(THREADS) kv8_expand_kernel(const __grid_constant__ h3b::XAttn a) {
   constexpr int VPR = D / 16;
-  const int64_t i = static_cast<int64_t>(blockIdx.x) * THREADS + threadIdx.x;
-  const int col = static_cast<int>(i % VPR) * 16;
-  const int64_t row = i / VPR;  // (b, head, token)
-  const int tok = static_cast<int>(row % a.s_kv);
-  const int64_t bh = row / a.s_kv;
-  const int head = static_cast<int>(bh % a.kv_heads);
-  const int64_t b = bh / a.kv_heads;
-  if (b >= a.batch) return;
+  const int col = static_cast<int>(threadIdx.x % VPR) * 16;
+  const int tok = static_cast<int>(blockIdx.x * (THREADS / VPR) + threadIdx.x / VPR);
+  const int head = blockIdx.y >> 1;
+  const int64_t b = blockIdx.z;
+  const bool values = (blockIdx.y & 1) != 0;
+  if (tok >= a.s_kv) return;
+  const int64_t row = (b * a.kv_heads + head) * static_cast<int64_t>(a.s_kv) + tok;
+  const int shift = shift_of(a.block_tokens);
   const int len = max(0, min(a.s_kv, a.kv_lens[b]));
   if (tok >= (len + 127) / 128 * 128) return;
-  const int id = a.table[b * a.max_blocks + tok / a.block_tokens];
+  const int id = a.table[b * a.max_blocks + (tok >> shift)];
   uint32_t w[8] = {0, 0, 0, 0, 0, 0, 0, 0};
   if (tok < len && id >= 0 && id < a.num_blocks) {
     const int64_t slab = static_cast<int64_t>(id) * a.kv_heads + head;
-    const uint4 c = __ldcs(reinterpret_cast<const uint4*>(static_cast<const uint8_t*>(blockIdx.y ? a.v : a.k) +
-                                                          (slab * a.block_tokens + tok % a.block_tokens) * D + col));
+    const uint4 c = __ldcs(reinterpret_cast<const uint4*>(static_cast<const uint8_t*>(values ? a.v : a.k) +
+                                                          ((slab << shift) + (tok & (a.block_tokens - 1))) * D + col));
     const uint32_t u[4] = {c.x, c.y, c.z, c.w};
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
@@ -274,7 +280,7 @@ __global__ void __launch_bounds__(THREADS) kv8_expand_kernel(const __grid_consta
       w[2 * k + 1] = pack16x2<F16>(y[2], y[3]);
     }
   }
-  st_global_v8(static_cast<uint16_t*>(blockIdx.y ? a.pre_v : a.pre_k) + row * D + col, w);
+  st_global_v8(static_cast<uint16_t*>(values ? a.pre_v : a.pre_k) + row * D + col, w);
 }
 
 bool block_ok(int64_t bt) { return bt == 32 || bt == 64 || bt == 128; }
@@ -284,9 +290,10 @@ bool block_ok(int64_t bt) { return bt == 32 || bt == 64 || bt == 128; }
 namespace h3b {
 
 int kv8_expand_launch(const XAttn& a, cudaStream_t stream) {
-  const int64_t gx = (static_cast<int64_t>(a.batch) * a.kv_heads * a.s_kv * (a.head_dim / 16) + THREADS - 1) / THREADS;
-  if (gx > 0x7fffffffll) return H3B_ERR_SHAPE;
-  const dim3 grid(static_cast<unsigned>(gx), 2);
+  const int per = THREADS / (a.head_dim / 16);
+  if (a.kv_heads > 32767) return H3B_ERR_SHAPE;
+  const dim3 grid(static_cast<unsigned>((a.s_kv + per - 1) / per), static_cast<unsigned>(2 * a.kv_heads),
+                  static_cast<unsigned>(a.batch));
   const bool f16 = a.dtype == H3B_F16, e4 = a.kind == KV_E4M3;
 #define H3B_EXPAND(DD)                                                                       \
   (e4 ? (f16 ? kv8_expand_kernel<DD, true, true><<<grid, THREADS, 0, stream>>>(a)            \
@@ -365,10 +372,10 @@ extern "C" int h3b_kv8_read(const uint8_t* k_codes, const uint8_t* v_codes, cons
   a.table = table, a.lens = lens;
   a.batch = static_cast<int>(batch), a.max_len = static_cast<int>(max_len), a.kv_heads = static_cast<int>(kv_heads);
   a.max_blocks = static_cast<int>(max_blocks), a.num_blocks = static_cast<int>(num_blocks);
-  a.block_tokens = static_cast<int>(block_tokens);
-  const int64_t pieces = batch * max_len * kv_heads * (head_dim / 16);
-  const int64_t gx = (pieces + THREADS - 1) / THREADS;
-  if (gx > 0x7fffffffll) return H3B_ERR_SHAPE;
+  a.block_shift = shift_of(static_cast<int>(block_tokens));
+  const int64_t rows = batch * max_len * kv_heads, per = THREADS / (head_dim / 16);
+  if (rows > 0x7fffffffll) return H3B_ERR_SHAPE;
+  const int64_t gx = (rows + per - 1) / per;
   const dim3 grid(static_cast<unsigned>(gx), 2);
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   const bool e4 = code_type == H3B_KV_E4M3;
