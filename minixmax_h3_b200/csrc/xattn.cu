@@ -33,25 +33,31 @@ int64_t rows_of(const XAttn& a) { return static_cast<int64_t>(a.batch) * a.heads
 // exist or not; the row kernel on 32 rows of the heads that share a key head.
 bool by_tiles(const XAttn& a) { return a.s_q >= 64; }
 
-// (The last call's plan is kept by its sizes: a model's layers repeat them,
-// and the search is 2 us of divisions on calls of 10.)
-void plan(XAttn& a) {
-  struct Sizes {
-    int kind, batch, heads, kv_heads, head_dim, s_q, s_kv, sms;
-    bool operator==(const Sizes& o) const {
-      return kind == o.kind && batch == o.batch && heads == o.heads && kv_heads == o.kv_heads &&
-             head_dim == o.head_dim && s_q == o.s_q && s_kv == o.s_kv && sms == o.sms;
-    }
-  };
-  static thread_local Sizes last{};
-  static thread_local int splits = 0;
-  const Sizes now{a.kind == h3b::KV_DENSE ? 0 : 1, a.batch, a.heads, a.kv_heads, a.head_dim, a.s_q, a.s_kv,
-                  h3b::num_sms()};
+// The last call's splits are kept by its sizes: a model's layers repeat them,
+// and the search is 2 us of divisions on calls of 10.
+struct Sizes {
+  int kind, batch, heads, kv_heads, head_dim, s_q, s_kv, sms;
+  bool operator==(const Sizes& o) const {
+    return kind == o.kind && batch == o.batch && heads == o.heads && kv_heads == o.kv_heads && head_dim == o.head_dim &&
+           s_q == o.s_q && s_kv == o.s_kv && sms == o.sms;
+  }
+};
+template <class A, class F>
+int kept_splits(const A& a, int kind, Sizes& last, int& splits, F search) {
+  const Sizes now{kind, a.batch, a.heads, a.kv_heads, a.head_dim, a.s_q, a.s_kv, h3b::num_sms()};
   if (splits == 0 || !(now == last)) {
-    splits = by_tiles(a) ? h3b::xattn_tile_splits(a) : h3b::xattn_rows_splits(a);
+    splits = search(a);
     last = now;
   }
-  a.splits = splits;
+  return splits;
+}
+
+void plan(XAttn& a) {
+  static thread_local Sizes last{};
+  static thread_local int splits = 0;
+  a.splits = kept_splits(a, a.kind == h3b::KV_DENSE ? 0 : 1, last, splits, [](const XAttn& x) {
+    return by_tiles(x) ? h3b::xattn_tile_splits(x) : h3b::xattn_rows_splits(x);
+  });
 }
 
 // Whether a cache's codes are written out as 16-bit operands first; else each
@@ -168,7 +174,9 @@ h3b::XAttnGrad grad_sizes(int dtype, int64_t batch, int64_t heads, int64_t kv_he
   a.head_dim = static_cast<int>(head_dim);
   a.s_q = static_cast<int>(s_q);
   a.s_kv = static_cast<int>(s_kv);
-  a.splits = h3b::xattn_bwd_splits(a);
+  static thread_local Sizes last{};
+  static thread_local int splits = 0;
+  a.splits = kept_splits(a, 2, last, splits, h3b::xattn_bwd_splits);
   return a;
 }
 
