@@ -30,8 +30,13 @@ int check_sizes(int dtype, int64_t batch, int64_t heads, int64_t kv_heads, int64
 int64_t rows_of(const XAttn& a) { return static_cast<int64_t>(a.batch) * a.heads * a.s_q; }
 
 // Which kernel: the tile kernel works on 128 rows of one head whether they
-// exist or not; the row kernel on 32 rows of the heads that share a key head.
-bool by_tiles(const XAttn& a) { return a.s_q >= 64; }
+// exist or not, the row kernel on 16 or 32 rows of the heads that share a key
+// head.  GPU us, tiles / rows, at 32 and 48 tokens: 24 heads x 512 keys 10.7 /
+// 14.9 and 11.1 / 14.9; 4 samples, 24 heads on 6, 2000 keys 33.8 / 26.1 and
+// 34.0 / 32.7; 32768 int8 tokens x 24 heads 136 / 86 and 136 / 142; 4 x 4096, 32
+// heads on 8 79 / 61 and 79 / 104.  Over at most 128 keys the row kernel's
+// shorter start wins up to 128 tokens (2 samples, 8 heads of 64, 77 keys: 7.5 / 6.0).
+bool by_tiles(const XAttn& a) { return a.s_q > 32 && (a.s_q > 128 || a.s_kv > 128); }
 
 // The last call's splits are kept by its sizes: a model's layers repeat them,
 // and the search is 2 us of divisions on calls of 10.
