@@ -5,6 +5,7 @@ from __future__ import annotations
 
 import ctypes
 
+import numpy as np
 import pytest
 import torch
 from torch._subclasses.fake_tensor import FakeTensorMode
@@ -177,3 +178,47 @@ def test_custom_operator_shapes():
         assert torch.ops.h3b.kv8_attention(q, codes, codes, scale, scale, table, lens, False, None).shape == q.shape
     with pytest.raises(NotImplementedError):
         torch.ops.h3b.cross_attention(t(1, 4, 2, 64), t(1, 5, 2, 64), t(1, 5, 2, 64), None, None, None)
+
+
+def fma32(a, b, c):
+    """The product is exact in 64 bits; the sum rounds twice, which moves no
+    code (a second rounding is off by 2^-53 of the value)."""
+    return (a.astype(np.float64) * b.astype(np.float64) + c.astype(np.float64)).astype(np.float32)
+
+
+@pytest.mark.parametrize("top", [127.0, 448.0])
+def test_codes_by_corrected_quotient(top):
+    """The append kernel's x / s (r = 1 / s; q = x r; q + (x - q s) r) gives
+    the codes of a true division over the whole range of scales: s from 1e-12
+    / 448 to the largest float / 127, |x| up to s * top, rows of 16-bit types
+    and rescaled ones (any 32-bit value), ties included."""
+    rng = np.random.default_rng(7)
+    n = 1 << 20
+    f = np.float32
+    e = rng.uniform(-48.9, 120.9, n)
+    s = np.exp2(e).astype(f)
+    s[:4] = [f(1e-12) / f(448), f(1e-12) / f(127), f(3.4028235e38) / f(127), 1]
+    with np.errstate(over="ignore"):  # (products past the largest float are dropped below)
+        x = (s * rng.uniform(-top, top, n).astype(f)).astype(f)
+    half = rng.integers(0, 2 * int(top), n // 4)   # near and on the borders between codes
+    with np.errstate(over="ignore"):
+        x[: n // 4] = ((half + 0.5).astype(f) * s[: n // 4]).astype(f)
+    tiny = rng.integers(0, 1 << 31, n // 8).astype(np.uint32).view(f)
+    small = np.isfinite(tiny) & (np.abs(tiny) < 2.0 ** -80)
+    x[-(n // 8):][small] = tiny[small]
+    x[::3] = (x[::3].view(np.uint32) & 0xffff0000).view(f)  # bf16 values
+    keep = np.isfinite(x) & (np.abs(x) <= s.astype(np.float64) * top)
+    x, s = x[keep], s[keep]
+    assert x.size > n // 2
+    with np.errstate(under="ignore"):
+        r = (f(1) / s).astype(f)
+        q = (x * r).astype(f)
+        got = fma32(fma32(-q, s, x), r, q)
+        want = (x / s).astype(f)
+    assert r.min() >= np.finfo(f).tiny
+    if top == 127.0:
+        codes = [np.clip(np.rint(y), -127, 127) for y in (got, want)]
+    else:
+        codes = [torch.from_numpy(y).clamp(-448, 448).to(torch.float8_e4m3fn).view(torch.uint8).numpy() & 0x7f
+                 for y in (got, want)]
+    assert (codes[0] == codes[1]).all()
