@@ -11,16 +11,18 @@
 // into the matrix instructions, exactly (|int8| <= 128 and every e4m3 value
 // are f16 numbers), so nothing is rounded between the cache and the product.
 //
-// The work is bound by the bytes of K and V.  A CTA is one range of keys x one
+// The work has to move the bytes of K and V.  A CTA is one range of keys x one
 // key head x 16 or 32 query rows (tokens x the heads that share the key
 // head).  Its 4 warps take the range's tiles in turn and never meet before
-// the end: each has its own ring of TMA tiles (24 KB) and its own running
-// softmax, and the four join through shared memory at the end.  A tile is 32
-// keys of the cache or 16 keys of a dense tensor.  m16n8k16 matrix
-// instructions do both products: 16 rows fill one, the conversion of the
-// codes is shared by all rows of the CTA, and the 4096 codes of 16 keys cost
-// ~250 warp instructions, a third of the SM's issue slots at full memory rate.
+// the end: each has its own ring of TMA tiles (16 KB at 16 rows, so that three
+// CTAs fit an SM; 24 KB at 32) and its own running softmax, and the four join
+// through shared memory at the end.  A tile is 32 keys of the cache or 16 keys
+// of a dense tensor.  m16n8k16 matrix instructions do both products: 16 rows
+// fill one, and the conversion of the codes is shared by all rows of the CTA.
 // (tcgen05 needs 128 rows per instruction; few-row calls have 1 to 32.)
+// What bounds it over a long cache is issue slots, about half of them taken in
+// every cycle by the conversion and the softmax: 131072 tokens x 24 heads of
+// 128 e4m3 145 us (5.6 TB/s), int8, whose conversion is longer, 161 (5.0 TB/s).
 //
 // Lane layout of the codes.  The contraction order of a product is free as
 // long as both operands use it, so K is read 16 bytes at a time: lane (g, t)
@@ -30,6 +32,8 @@
 // keys of its k slots and interleaves them by byte permutes.  perm() maps the
 // column n of a score tile to the key row so that both reads touch each bank
 // once under the TMA swizzle.
+#include <type_traits>
+
 #include "h3b_common.cuh"
 #include "h3b_host.hpp"
 #include "xattn.hpp"
@@ -576,50 +580,67 @@ __global__ void __launch_bounds__(WARPS * 32, MT == 1 ? 3 : 2)
 
 // Joins the split ranges of each row: o = sum_i 2^(M_i - M) o_i / sum_i
 // 2^(M_i - M) l_i.  One warp per row, D/32 values per lane; the sums run in
-// the order of the ranges.
+// the order of the ranges.  Eight ranges' values are under way at a time, the
+// first eight before the maxima arrive (1560 x 24 rows of 6 ranges: 36 us with
+// the maxima first, 28 so; 4.5 TB/s, much of it from L2).  (Row numbers have 32 bits: 2^31 rows
+// of two ranges would be a workspace of 1 TB.)
 template <int D>
 __global__ void __launch_bounds__(128) xattn_combine_kernel(const __grid_constant__ XAttn a) {
-  const int64_t total = static_cast<int64_t>(a.batch) * a.heads * a.s_q;
-  const int64_t row = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 5);
+  constexpr int E = D / 32, DEEP = 8;
+  using Vec = typename std::conditional<E == 4, float4, float2>::type;
+  const uint32_t total = static_cast<uint32_t>(a.batch) * a.heads * a.s_q;
+  const uint32_t row = blockIdx.x * 4 + (threadIdx.x >> 5);
   if (row >= total) return;
   const int lane = threadIdx.x & 31;
-  float mx = -INFINITY;
-  for (int i = lane; i < a.splits; i += 32) mx = fmaxf(mx, a.part_ml[i * total + row].x);
+  const Vec* src = reinterpret_cast<const Vec*>(a.part_o + static_cast<int64_t>(row) * D) + lane;
+  const int64_t step = static_cast<int64_t>(total) * 32;  // (Vecs from range to range)
+  Vec v[DEEP];
+#pragma unroll
+  for (int k = 0; k < DEEP; ++k)
+    if (k < a.splits) v[k] = src[k * step];
+  float2 ml = lane < a.splits ? a.part_ml[static_cast<int64_t>(lane) * total + row] : make_float2(-INFINITY, 0.0f);
+  float mx = ml.x;
+  for (int i = lane + 32; i < a.splits; i += 32) mx = fmaxf(mx, a.part_ml[static_cast<int64_t>(i) * total + row].x);
   mx = warp_max(mx);
   const float base = mx == -INFINITY ? 0.0f : mx;
   float l = 0.0f;
-  float o[D / 32];
+  float o[E];
 #pragma unroll
-  for (int e = 0; e < D / 32; ++e) o[e] = 0.0f;
-#pragma unroll 4
-  for (int i = 0; i < a.splits; ++i) {
-    const float2 ml = a.part_ml[i * total + row];
-    const float f = ex2(ml.x - base);
-    l = fmaf(ml.y, f, l);
-    const float* p = a.part_o + (i * total + row) * D + lane * (D / 32);
-    if constexpr (D == 128) {
-      const float4 v = *reinterpret_cast<const float4*>(p);
-      o[0] = fmaf(v.x, f, o[0]);
-      o[1] = fmaf(v.y, f, o[1]);
-      o[2] = fmaf(v.z, f, o[2]);
-      o[3] = fmaf(v.w, f, o[3]);
-    } else {
-      const float2 v = *reinterpret_cast<const float2*>(p);
-      o[0] = fmaf(v.x, f, o[0]);
-      o[1] = fmaf(v.y, f, o[1]);
+  for (int e = 0; e < E; ++e) o[e] = 0.0f;
+  for (int i = 0; i < a.splits; i += DEEP) {
+    if (i > 0) {
+#pragma unroll
+      for (int k = 0; k < DEEP; ++k)
+        if (i + k < a.splits) v[k] = src[(i + k) * step];
+      if ((i & 31) == 0)
+        ml = i + lane < a.splits ? a.part_ml[static_cast<int64_t>(i + lane) * total + row] : make_float2(-INFINITY, 0.0f);
+    }
+    const float w = ex2(ml.x - base);
+#pragma unroll
+    for (int k = 0; k < DEEP; ++k) {
+      if (i + k < a.splits) {
+        const float f = __shfl_sync(0xffffffffu, w, (i + k) & 31);
+        l = fmaf(__shfl_sync(0xffffffffu, ml.y, (i + k) & 31), f, l);
+        const float x[4] = {v[k].x, v[k].y, E == 4 ? reinterpret_cast<const float*>(&v[k])[E - 2] : 0.0f,
+                            E == 4 ? reinterpret_cast<const float*>(&v[k])[E - 1] : 0.0f};
+#pragma unroll
+        for (int e = 0; e < E; ++e) o[e] = fmaf(x[e], f, o[e]);
+      }
     }
   }
   const float inv = l > 0.0f ? 1.0f / l : 0.0f;
-  const int tok = static_cast<int>(row % a.s_q);
-  const int64_t bh = row / a.s_q;
-  const int head = static_cast<int>(bh % a.heads);
-  uint16_t* dst = static_cast<uint16_t*>(a.o) + (bh / a.heads) * a.o_stride[0] + tok * a.o_stride[1] +
-                  head * a.o_stride[2] + lane * (D / 32);
+  const uint32_t bh = row / static_cast<uint32_t>(a.s_q);
+  const int64_t tok = row - bh * a.s_q, b = bh / static_cast<uint32_t>(a.heads);
+  const int64_t head = bh - static_cast<uint32_t>(b) * a.heads;
+  uint16_t* dst = static_cast<uint16_t*>(a.o) + b * a.o_stride[0] + tok * a.o_stride[1] + head * a.o_stride[2] + lane * E;
+  uint32_t w[E / 2];
 #pragma unroll
-  for (int e = 0; e < D / 32; e += 2) {
-    const uint32_t w = a.dtype == H3B_F16 ? pack_f16x2(o[e] * inv, o[e + 1] * inv)
-                                          : pack_bf16x2(o[e] * inv, o[e + 1] * inv);
-    *reinterpret_cast<uint32_t*>(dst + e) = w;
+  for (int e = 0; e < E; e += 2)
+    w[e / 2] = a.dtype == H3B_F16 ? pack_f16x2(o[e] * inv, o[e + 1] * inv) : pack_bf16x2(o[e] * inv, o[e + 1] * inv);
+  if constexpr (E == 4) {
+    *reinterpret_cast<uint2*>(dst) = make_uint2(w[0], w[1]);
+  } else {
+    *reinterpret_cast<uint32_t*>(dst) = w[0];
   }
   if (lane == 0 && a.lse != nullptr) a.lse[row] = l > 0.0f ? (mx + __log2f(l)) * LN2 : -INFINITY;
 }
@@ -721,8 +742,9 @@ int xattn_rows_launch(const XAttn& a, cudaStream_t stream) {
 }
 
 int xattn_combine_launch(const XAttn& a, cudaStream_t stream) {
-  const int64_t grid = (static_cast<int64_t>(a.batch) * a.heads * a.s_q + 3) / 4;
-  if (grid > 0x7fffffff) return H3B_ERR_SHAPE;
+  const int64_t rows = static_cast<int64_t>(a.batch) * a.heads * a.s_q;
+  if (rows > 0x7fffffff) return H3B_ERR_SHAPE;
+  const int64_t grid = (rows + 3) / 4;
   if (a.head_dim == 128) {
     xattn_combine_kernel<128><<<static_cast<unsigned>(grid), 128, 0, stream>>>(a);
   } else {
