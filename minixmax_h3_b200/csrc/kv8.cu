@@ -339,13 +339,15 @@ extern "C" int h3b_kv8_append(const void* k, const void* v, int x_dtype, int64_t
   if (code_type != H3B_KV_INT8 && code_type != H3B_KV_E4M3) return H3B_ERR_DTYPE;
   if (batch == 0 || n == 0) return H3B_OK;
   if (!k || !v || !k_codes || !v_codes || !k_scale || !v_scale || !table || !start) return H3B_ERR_ARG;
-  for (int64_t st : {batch_stride, seq_stride, head_stride})
+  // (an axis of extent 1 may carry any stride)
+  const int64_t strides[3] = {batch > 1 ? batch_stride : 0, n > 1 ? seq_stride : 0, kv_heads > 1 ? head_stride : 0};
+  for (int64_t st : strides)
     if (st < 0 || st % 8 != 0) return H3B_ERR_ALIGN;
   for (const void* p : {k, v, static_cast<const void*>(k_codes), static_cast<const void*>(v_codes)})
     if (!h3b::aligned16(p)) return H3B_ERR_ALIGN;
   AppendArgs a{};
   a.src[0] = k, a.src[1] = v;
-  a.src_stride[0] = batch_stride, a.src_stride[1] = seq_stride, a.src_stride[2] = head_stride;
+  for (int i = 0; i < 3; ++i) a.src_stride[i] = strides[i];
   a.codes[0] = k_codes, a.codes[1] = v_codes;
   a.scale[0] = k_scale, a.scale[1] = v_scale;
   a.table = table, a.start = start, a.count = count;

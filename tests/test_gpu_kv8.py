@@ -256,3 +256,45 @@ def test_custom_operators(cuda):
     q = torch.randn(2, 1, 4, 64, device=cuda).to(torch.bfloat16)
     o = torch.ops.h3b.kv8_attention(q, *args, ints([9, 9], cuda), False, None)
     assert torch.equal(o, ops.kv8_attention(q, c, table, ints([9, 9], cuda)))
+
+
+@pytest.mark.parametrize("axis", [0, 1, 2])
+def test_append_any_stride_along_an_axis_of_one(cuda, axis):
+    """The stride of an axis of extent 1 is never used, whatever it is."""
+    from minixmax_h3_b200 import ops
+
+    shape = [2, 5, 3, 64]
+    shape[axis] = 1
+    b, n, hkv, d = shape
+    src = torch.randn(2, *shape, device=cuda).to(torch.bfloat16)
+    odd = [list(t.stride()) for t in src]
+    for st in odd:
+        st[axis] = 517
+    views = [torch.as_strided(src, shape, st, i * src[0].numel()) for i, st in enumerate(odd)]
+    table, lens = ints([[i] for i in range(b)], cuda), ints([0] * b, cuda)
+    got = []
+    for k, v in ((src[0], src[1]), views):
+        c = ops.KV8Cache.empty(2, hkv, d, device=cuda)
+        ops.kv8_append(c, k, v, table, lens)
+        got.append((c.k, c.v, c.k_scale, c.v_scale))
+    assert all(torch.equal(x, y) for x, y in zip(*got))
+    assert got[0][0].any() and got[0][1].any()
+
+
+def test_nothing_to_do(cuda):
+    """Appends of no rows, reads of no tokens and calls of no sequences or
+    queries return empty results and leave the cache alone."""
+    from minixmax_h3_b200 import ops
+
+    c = ops.KV8Cache.empty(2, 2, 64, device=cuda)
+    c.k.fill_(3)
+    table, lens = ints([[0, 1]], cuda), ints([7], cuda)
+    x = torch.zeros(1, 0, 2, 64, dtype=torch.bfloat16, device=cuda)
+    ops.kv8_append(c, x, x, table, lens)
+    assert [t.shape for t in ops.kv8_read(c, table, lens, 0)] == [(1, 0, 2, 64)] * 2
+    assert ops.kv8_attention(x, c, table, lens).shape == (1, 0, 2, 64)
+    x, table, lens = x[:0], table[:0], lens[:0]
+    ops.kv8_append(c, x, x, table, lens)
+    assert [t.shape for t in ops.kv8_read(c, table, lens, 9)] == [(0, 9, 2, 64)] * 2
+    assert ops.kv8_attention(torch.zeros(0, 3, 4, 64, dtype=torch.bfloat16, device=cuda), c, table, lens).shape == (0, 3, 4, 64)
+    assert bool((c.k == 3).all())
