@@ -58,9 +58,23 @@ class _CrossAttention(torch.autograd.Function):
     @staticmethod
     def backward(ctx, do):
         q, k, v, o, lse, kv_lens, key_mask = ctx.saved_tensors
-        dq, dk, dv = ops.cross_attention_bwd(do, q, k, v, o, lse, kv_lens=kv_lens, key_mask=key_mask,
-                                             scale=ctx.scale)
-        return dq, dk, dv, None, None, None
+        if torch.is_grad_enabled():  # create_graph
+            return (*_CrossAttentionGrad.apply(do, q, k, v, o, lse, kv_lens, key_mask, ctx.scale), None, None, None)
+        return (*ops.cross_attention_bwd(do, q, k, v, o, lse, kv_lens=kv_lens, key_mask=key_mask, scale=ctx.scale),
+                None, None, None)
+
+
+class _CrossAttentionGrad(torch.autograd.Function):
+    """The gradients as a node of a graph, so that a second derivative raises
+    where it reaches them (without a node it would silently lack their part)."""
+
+    @staticmethod
+    def forward(ctx, do, q, k, v, o, lse, kv_lens, key_mask, scale):
+        return ops.cross_attention_bwd(do, q, k, v, o, lse, kv_lens=kv_lens, key_mask=key_mask, scale=scale)
+
+    @staticmethod
+    def backward(ctx, *grads):
+        raise RuntimeError("cross_attention has no second derivatives")
 
 
 def cross_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, kv_lens: Optional[torch.Tensor] = None,
@@ -68,7 +82,8 @@ def cross_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, kv_len
     """ops.cross_attention (q [B, Sq, H, D], k and v [B, Skv, Hkv, D]; see
     there for kv_lens and key_mask), differentiable by autograd in q, k and v.
     The backward pass is one call of ops.cross_attention_bwd; it keeps q, k,
-    v, the result and a log-sum-exp per row, and is bit-reproducible."""
+    v, the result and a log-sum-exp per row, and is bit-reproducible.  There
+    are no second derivatives: asking for them raises."""
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
         return _CrossAttention.apply(q, k, v, kv_lens, key_mask, scale)
     return ops.cross_attention(q, k, v, kv_lens=kv_lens, key_mask=key_mask, scale=scale)

@@ -293,3 +293,14 @@ def test_cross_attention_layer(cuda):
     assert (got - want).float().norm() <= 0.02 * want.float().norm()
     with pytest.raises(ValueError):
         layer(x)
+
+
+def test_no_second_derivatives(cuda):
+    """A gradient penalty must not silently lose this operator's part."""
+    from minixmax_h3_b200.attention import cross_attention
+
+    q, k, v, do = make(cuda, 1, 9, 12, 2, 2, 64, torch.bfloat16)
+    q = q.requires_grad_()
+    (dq,) = torch.autograd.grad(cross_attention(q, k, v), q, do, create_graph=True)
+    with pytest.raises(RuntimeError):
+        (dq.float().square().sum() + q.float().sum()).backward()
