@@ -57,10 +57,6 @@ constexpr int KVST = 4;  // K/V ring (K_s in slots 0, 2, V_s in 1, 3)
 constexpr int THREADS = 512;
 constexpr int REGS_LAUNCH = 128;
 constexpr int REGS_CONTROL = 64;
-constexpr int REGS_STORE = 112;
-constexpr int REGS_SOFTMAX = 168;
-static_assert(128 * (REGS_CONTROL + REGS_STORE + 2 * REGS_SOFTMAX) <= THREADS * REGS_LAUNCH,
-              "register split exceeds launch");
 constexpr float RESCALE_THRESHOLD = 8.0f;
 constexpr float LOG2E = 1.4426950408889634f;
 constexpr float LN2 = 0.69314718055994531f;
@@ -72,6 +68,12 @@ template <int D, KvKind KIND, bool PRE>
 struct Cfg {
   static constexpr bool SCALED = KIND != KV_DENSE;
   static constexpr bool CODES = SCALED && !PRE;  // converted here
+  // Registers of the storing and the softmax warps.  (Where no codes are
+  // converted the storing warps leave enough that no score is spilled: masked 2
+  // x 2049 x 1025, 24 heads of 128 95 -> 89 us, 32768 x 512 of 64 191 -> 187.)
+  static constexpr int REGS_STORE = CODES ? 112 : 80;
+  static constexpr int REGS_SOFTMAX = CODES ? 168 : 184;
+  static_assert(128 * (REGS_CONTROL + REGS_STORE + 2 * REGS_SOFTMAX) <= THREADS * REGS_LAUNCH, "register split exceeds launch");
   // Q ring (128-row tiles).  Over a cache a unit is long, and the codes' own
   // two tiles take the room of the third slot.
   static constexpr int QST = CODES ? 2 : (D == 128 ? 3 : 6);
@@ -252,6 +254,18 @@ H3B_DEV void tmem_st8(uint32_t taddr, const uint32_t (&r)[8]) {
                : "memory");
 }
 
+H3B_DEV float4 lds4(const volatile void* p) {
+  float4 v;
+  asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
+               : "r"(smem_u32(const_cast<const void*>(p))));
+  return v;
+}
+H3B_DEV float2 lds2(const volatile void* p) {
+  float2 v;
+  asm volatile("ld.shared.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(smem_u32(const_cast<const void*>(p))));
+  return v;
+}
+
 H3B_DEV float row_max32(const uint32_t* r) {
   float mx[4];
 #pragma unroll
@@ -430,7 +444,7 @@ H3B_DEV void zero_row(uint32_t dst, int row) {
 
 // The cache's block of a key, -1 if there is none.
 H3B_DEV int block_of(const XAttn& a, int b, int key) {
-  const int j = key >> (a.block_tokens == 32 ? 5 : (a.block_tokens == 64 ? 6 : 7));
+  const int j = key >> (31 - __clz(a.block_tokens));  // (a power of two)
   if (j >= a.max_blocks) return -1;
   const int id = __ldg(a.table + static_cast<int64_t>(b) * a.max_blocks + j);
   return id >= 0 && id < a.num_blocks ? id : -1;
@@ -690,6 +704,7 @@ __global__ void __launch_bounds__(THREADS, 1)
       uint32_t ic[2] = {0, 0};          // infos written, per row tile
       int id_here = 0, id_ahead = 0;    // cache: blocks of this tile and the next, scales of this
       float k_here = 1.0f, v_here = 1.0f;
+      int kvh = 0;                      // the unit's key head
       bool ok = true;
       while (u.x < args.units && u.n == 0) u.next(args);
       int j = 0;
@@ -707,11 +722,13 @@ __global__ void __launch_bounds__(THREADS, 1)
                ((((qc + 1) / QST) & 1) ? R_Q1_PHASE : 0u);
           if constexpr (SCALED) {
             if (lane < 4) {
-              if (j == 0) id_ahead = block_of(a, u.b, key0 + 32 * lane);
+              if (j == 0) {
+                id_ahead = block_of(a, u.b, key0 + 32 * lane);
+                kvh = args.group == 1 ? u.head : u.head / args.group;
+              }
               id_here = id_ahead;
               if (j + 1 < u.n) id_ahead = block_of(a, u.b, key0 + BKV + 32 * lane);
-              const int64_t at = static_cast<int64_t>(max(id_here, 0)) * a.kv_heads +
-                                 (args.group == 1 ? u.head : u.head / args.group);
+              const int at = max(id_here, 0) * a.kv_heads + kvh;  // (below 2^31: checked on the host)
               k_here = __ldg(a.k_scale + at);
               v_here = __ldg(a.v_scale + at);
             }
@@ -771,7 +788,7 @@ __global__ void __launch_bounds__(THREADS, 1)
               volatile TileInfo* info = &bars->info[i][ic[i] % INFOS];
               info->k_factor[lane] = kf;
               info->v_log2[lane] = __log2f(vs);
-              info->v_inv[lane] = 1.0f / vs;
+              info->v_inv[lane] = __fdividef(1.0f, vs);  // (a call of the IEEE division is fetched anew each tile)
             }
           }
         }
@@ -793,7 +810,7 @@ __global__ void __launch_bounds__(THREADS, 1)
     }
   } else if (warp < 8) {
     // ------------------------------------------------------------ softmax
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(REGS_SOFTMAX));
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(C::REGS_SOFTMAX));
     const int wg = warp >> 2;
     const int row = (warp & 3) * 32 + lane;
     const uint32_t lane_off = static_cast<uint32_t>((warp & 3) * 32) << 16;
@@ -863,11 +880,9 @@ __global__ void __launch_bounds__(THREADS, 1)
           }
           float fx[4], ox[4];
           if constexpr (SCALED) {
-#pragma unroll
-            for (int g = 0; g < 4; ++g) {
-              fx[g] = info->k_factor[g];
-              ox[g] = info->v_log2[g];
-            }
+            const float4 f = lds4(info->k_factor), o = lds4(info->v_log2);
+            fx[0] = f.x, fx[1] = f.y, fx[2] = f.z, fx[3] = f.w;
+            ox[0] = o.x, ox[1] = o.y, ox[2] = o.z, ox[3] = o.w;
           }
           if (slow) {
             float m_tile;
@@ -904,7 +919,7 @@ __global__ void __launch_bounds__(THREADS, 1)
           float2 sm;
           if constexpr (SCALED) {
             sm = exp_codes64<F16, true>(r, r, make_float2(fx[0], fx[1]), make_float2(ox[0] + neg_m, ox[1] + neg_m),
-                                        make_float2(info->v_inv[0], info->v_inv[1]), fx, ox);
+                                        lds2(info->v_inv), fx, ox);
           } else {
             sm = exp_pack64<F16, true>(r, r, args.scale_log2, neg_m);
             sm.y *= args.scale_log2;
@@ -920,9 +935,9 @@ __global__ void __launch_bounds__(THREADS, 1)
             const float neg_m = m_use == -INFINITY ? 0.0f : -m_use;
             if constexpr (SCALED) {
               const float f[4] = {0.f, 0.f, 0.f, 0.f};
-              sum += exp_codes64<F16, false>(r + 64, r + 32, make_float2(info->k_factor[2], info->k_factor[3]),
-                                             make_float2(info->v_log2[2] + neg_m, info->v_log2[3] + neg_m),
-                                             make_float2(info->v_inv[2], info->v_inv[3]), f, f).x;
+              const float2 o = lds2(info->v_log2 + 2);
+              sum += exp_codes64<F16, false>(r + 64, r + 32, lds2(info->k_factor + 2),
+                                             make_float2(o.x + neg_m, o.y + neg_m), lds2(info->v_inv + 2), f, f).x;
             } else {
               sum += exp_pack64<F16, false>(r + 64, r + 32, args.scale_log2, neg_m).x;
             }
@@ -946,7 +961,7 @@ __global__ void __launch_bounds__(THREADS, 1)
     }
   } else {
     // ------------------------------------------------------------ stores
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(REGS_STORE));
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(C::REGS_STORE));
     const int row = (warp & 3) * 32 + lane;
     const uint32_t lane_off = static_cast<uint32_t>((warp & 3) * 32) << 16;
     const int64_t total_rows = static_cast<int64_t>(a.batch) * a.heads * a.s_q;
