@@ -67,8 +67,8 @@ void plan(XAttn& a) {
 
 // Whether a cache's codes are written out as 16-bit operands first; else each
 // 256-row tile of each query head converts them anew.  32768 int8 tokens x 24
-// heads, bf16, us with and without: 256 rows 229 / 177, 512 rows 314 / 329, 768
-// rows 404 / 475, 1560 rows 853 / 1279.  At most 8 GB of workspace.
+// heads, bf16, us with and without: 256 rows 212 / 167, 512 rows 294 / 306, 768
+// rows 380 / 450, 1560 rows 798 / 1222.  At most 8 GB of workspace.
 int64_t expand_bytes(const XAttn& a) {
   const int64_t times = static_cast<int64_t>(a.heads / a.kv_heads) * ((a.s_q + 255) / 256);
   if (a.kind == h3b::KV_DENSE || !by_tiles(a) || times < 2) return 0;

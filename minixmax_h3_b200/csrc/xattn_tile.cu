@@ -35,8 +35,8 @@
 // row of V is zeroed in shared memory before P V reads it (0 * NaN is NaN).
 // What bounds it is the chain softmax -> P V -> S -> softmax of a row tile and
 // its hand-offs, of which two are interleaved: 24 heads of 128, bf16, 16384 x
-// 4096 686 us (1200 TFLOP/s), 32768 x 512 216 us (950; the border counts for
-// a fourth), x 128 102 us (500).
+// 4096 673 us (1230 TFLOP/s), 32768 x 512 218 us (950; the border counts for
+// a fourth), x 128 102 us (500); of 64, 32768 x 512 185 us.
 #include "h3b_common.cuh"
 #include "h3b_host.hpp"
 #include "xattn.hpp"
@@ -70,7 +70,7 @@ struct Cfg {
   static constexpr bool CODES = SCALED && !PRE;  // converted here
   // Registers of the storing and the softmax warps.  (Where no codes are
   // converted the storing warps leave enough that no score is spilled: masked 2
-  // x 2049 x 1025, 24 heads of 128 95 -> 89 us, 32768 x 512 of 64 191 -> 187.)
+  // x 2049 x 1025, 24 heads of 128 95 -> 89 us, 32768 x 512 of 64 191 -> 186.)
   static constexpr int REGS_STORE = CODES ? 112 : 80;
   static constexpr int REGS_SOFTMAX = CODES ? 168 : 184;
   static_assert(128 * (REGS_CONTROL + REGS_STORE + 2 * REGS_SOFTMAX) <= THREADS * REGS_LAUNCH, "register split exceeds launch");
