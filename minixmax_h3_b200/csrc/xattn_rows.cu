@@ -392,7 +392,6 @@ __global__ void __launch_bounds__(WARPS * 32, MT == 1 ? 3 : 2)
     // ---- running softmax; x = score * mult * sk + log2 sv
     const float lsv = CODES ? __log2f(fmaxf(sv, 1e-37f)) : 0.0f;
     const float inv_sv = CODES ? 1.0f / fmaxf(sv, 1e-37f) : 1.0f;
-    const float ksk = CODES ? fmaxf(sk, 1e-37f) : 1.0f;  // (a factor of 0 would make NaN of -inf)
     if (keep != all || key0 + T::KEYS > full_to) {
 #pragma unroll
       for (int m = 0; m < MT; ++m)
@@ -415,7 +414,8 @@ __global__ void __launch_bounds__(WARPS * 32, MT == 1 ? 3 : 2)
         for (int n = 1; n < NT; ++n) top = fmax3(top, sc[m][n][2 * hf], sc[m][n][2 * hf + 1]);
         top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
         top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-        f[hf] = mult[m][hf] * ksk;
+        // (a factor of 0 would make NaN of -inf: a row of zeros has e = 2^-126, zero keys sk = 1e-14)
+        f[hf] = CODES ? fmaxf(mult[m][hf] * sk, 1e-37f) : mult[m][hf];
         const float mn = fmaxf(M[m][hf], fmaf(top, f[hf], lsv));
         const float base = mn == -INFINITY ? 0.0f : mn;  // nothing kept so far: every weight is 2^-inf = 0
         corr[hf] = ex2(M[m][hf] - base);
