@@ -162,12 +162,16 @@ extern "C" int h3b_cross_attention_fwd(const void* q, const void* k, const void*
 
 namespace {
 
-// Workspace of a backward call: the ranges' sums (16-byte pieces), then delta.
+// Workspace of a backward call: the ranges' sums (16-byte pieces), then delta,
+// and the norms that f16 calls scale dS by (the query of the size does not say
+// which type it is for).
 int64_t grad_part_floats(const h3b::XAttnGrad& a) {
   return a.splits > 1 ? 2ll * a.splits * a.batch * a.s_kv * a.kv_heads * a.head_dim : 0;
 }
+int64_t grad_rows(const h3b::XAttnGrad& a) { return static_cast<int64_t>(a.batch) * a.heads * a.s_q; }
 int64_t grad_workspace(const h3b::XAttnGrad& a) {
-  return (grad_part_floats(a) + static_cast<int64_t>(a.batch) * a.heads * a.s_q) * static_cast<int64_t>(sizeof(float));
+  return (grad_part_floats(a) + 2 * grad_rows(a) + static_cast<int64_t>(a.batch) * a.kv_heads) *
+         static_cast<int64_t>(sizeof(float));
 }
 h3b::XAttnGrad grad_sizes(int dtype, int64_t batch, int64_t heads, int64_t kv_heads, int64_t head_dim, int64_t s_q,
                           int64_t s_kv) {
@@ -245,6 +249,8 @@ extern "C" int h3b_cross_attention_bwd(const void* d_o, const void* q, const voi
   if (workspace_bytes < grad_workspace(a)) return H3B_ERR_SHAPE;
   a.part = static_cast<float*>(workspace);
   a.delta = a.part + grad_part_floats(a);
+  a.do_sq = a.delta + grad_rows(a);
+  a.v_sq = a.do_sq + grad_rows(a);
   a.kv_lens = kv_lens;
   a.key_mask = s_kv > 0 ? key_mask : nullptr;
   a.mask_stride = mask_stride;

@@ -66,6 +66,8 @@ struct XAttnGrad {
   int64_t mask_stride;
   float scale;
   float* delta;  // workspace [batch, heads, s_q]
+  float* do_sq;  // f16: workspace [batch, heads, s_q], |do|^2 of a row
+  float* v_sq;   // f16: workspace [batch, kv_heads], largest |v|^2 of a kept key
   int splits;
   float* part;   // workspace [dv | dk][splits, batch, s_kv, kv_heads, D], if splits > 1
 };

@@ -28,7 +28,14 @@
 // 3500 cycles in the second, 2048 are products, because TMEM holds one S^T and
 // one dP^T beside the sums (128 x 512 columns are full).
 // In f16, P is held times 2^8 (P <= 1), which lowers the point where small
-// weights lose bits; dS is not scaled (its size is the caller's loss scale).
+// weights lose bits.  dS has the size of the caller's gradients, which may be
+// anything, so in dq it is held times a power of two of its row, which the fp32
+// result is divided by: |dP - delta| <= 2 |do| |v|, and the factor brings that
+// bound to 2^14 .. 2^15.  Without it do ~ 1e-4 lost 1 % of dq over 1024 keys in
+// f16's smallest numbers, and left-out keys (dS = -delta P there, see warp 10)
+// made infinities, so NaN, of delta above 65504.  The norms cost a pass over
+// do, with delta's where that is taken, and one over v (2 x 2049 x 1025, 24
+// heads on 6 of 128: 5 us and a launch, 330 -> 340 with the forward).
 #include "h3b_common.cuh"
 #include "h3b_host.hpp"
 #include "xattn.hpp"
@@ -98,6 +105,15 @@ H3B_DEV void issue_ts_half(uint32_t d, uint32_t a_tmem, uint32_t b_s, int half, 
     mma_f16_ts(d, a_tmem + kk * 8, desc_add_lo(bd, static_cast<uint32_t>((4 * half + kk) * (2048 >> 4))), idesc,
                (fresh && kk == 0) ? 0u : 1u);
 }
+
+// The power of two that f16 dS is held times, from |do|^2 |v|^2 (see the top of
+// the file): 2^14 / (|do| |v|), rounded down by at most 2.  (0 gives 2^77, and
+// dS is 0 then; infinities and NaN give 2^-51 and stay.)
+H3B_DEV float ds_factor(float sq) {
+  const int e = static_cast<int>((__float_as_uint(sq) >> 23) & 0xffu) - 127;  // sq < 2^(e + 1)
+  return __uint_as_float(static_cast<uint32_t>(127 + 14 - ((e + 2) >> 1)) << 23);
+}
+H3B_DEV float inverse_of_power(float p) { return __uint_as_float((254u << 23) - __float_as_uint(p)); }
 
 struct GradArgs {
   XAttnGrad a;
@@ -414,7 +430,8 @@ __global__ void __launch_bounds__(THREADS, 1)
           keep_words(masked, mb, u.len - key0, w);
           if ((w[0] & w[1] & w[2] & w[3]) != ~0u) {
             // Left-out rows of K and V are zeroed: S and dP are 0 there, so P
-            // (held to 1) and dS are finite, and dS K adds nothing.
+            // is held to 1, dS to delta (f16: and its factor), both finite,
+            // and dS K adds nothing.
             zero_left_out<C::HALVES>(smem_u32(sK + (t % KST) * C::TILE_BYTES), w, lane);
             zero_left_out<C::HALVES>(smem_u32(sV + (t % VST) * C::TILE_BYTES), w, lane);
             fence_proxy_async_smem();
@@ -443,15 +460,17 @@ __global__ void __launch_bounds__(THREADS, 1)
     const uint32_t lane_off = static_cast<uint32_t>((warp & 3) * 32) << 16;
     uint32_t step = 0, dc = 0, qc = 0;
     bool ok = true;
-    float lse_next = -INFINITY, delta_next = 0.0f;
+    float lse_next = -INFINITY, delta_next = 0.0f, sq_next = 0.0f;
     auto fetch = [&](const DqUnit& v) {
       const int r = v.q0 + row;
       lse_next = -INFINITY;
-      delta_next = 0.0f;
+      delta_next = sq_next = 0.0f;
       if (v.x < args.units && r < a.s_q) {
         const int64_t at = (static_cast<int64_t>(v.b) * a.heads + v.head) * a.s_q + r;
         lse_next = __ldg(a.lse + at);
         if (args.k_tiles > 1) delta_next = a.delta[at];
+        if (F16 && args.k_tiles > 0)
+          sq_next = a.do_sq[at] * a.v_sq[v.b * a.kv_heads + (args.group == 1 ? v.head : v.head / args.group)];
       }
     };
     fetch(u);
@@ -462,6 +481,7 @@ __global__ void __launch_bounds__(THREADS, 1)
       // The rows' statistics, fetched a unit ahead.
       const float neg_lse2 = -lse2_of(lse_next);
       float delta = delta_next;
+      const float factor = F16 ? ds_factor(sq_next) : 1.0f;
       {
         DqUnit v = u;
         v.next(args);
@@ -522,10 +542,11 @@ __global__ void __launch_bounds__(THREADS, 1)
           delta = part[row] + part[128 + row];
           if (wg == 0 && q_row < a.s_q) a.delta[stat + q_row] = delta;
         }
-        const float2 nd = make_float2(-delta, -delta);
+        const float2 nd = make_float2(-delta * factor, -delta * factor);
 #pragma unroll
         for (int e = 0; e < 64; e += 2) {
-          float2 t = add2(make_float2(__uint_as_float(d[e]), __uint_as_float(d[e + 1])), nd);
+          float2 t = make_float2(__uint_as_float(d[e]), __uint_as_float(d[e + 1]));
+          t = F16 ? fma2(t, make_float2(factor, factor), nd) : add2(t, nd);
           t = mul2(t, make_float2(__uint_as_float(s[e]), __uint_as_float(s[e + 1])));
           d[e] = __float_as_uint(t.x);
           d[e + 1] = __float_as_uint(t.y);
@@ -549,6 +570,7 @@ __global__ void __launch_bounds__(THREADS, 1)
         ++qc;
         tc_fence_after();
       }
+      const float out_scale = F16 ? a.scale * inverse_of_power(factor) : a.scale;
       uint16_t* out = static_cast<uint16_t*>(a.dq) +
                       ((static_cast<int64_t>(u.b) * a.s_q + q_row) * a.heads + u.head) * D + wg * (D / 2);
 #pragma unroll
@@ -567,7 +589,7 @@ __global__ void __launch_bounds__(THREADS, 1)
             uint32_t v[8];
 #pragma unroll
             for (int t = 0; t < 8; ++t)
-              v[t] = pack16x2<F16>(__uint_as_float(r[e + 2 * t]) * a.scale, __uint_as_float(r[e + 2 * t + 1]) * a.scale);
+              v[t] = pack16x2<F16>(__uint_as_float(r[e + 2 * t]) * out_scale, __uint_as_float(r[e + 2 * t + 1]) * out_scale);
             st_global_v8(out + c * 32 + e, v);
           }
         }
@@ -585,11 +607,12 @@ __global__ void __launch_bounds__(THREADS, 1)
   }
 }
 
-// delta = do . o of every row, where the keys take more than one tile: one
-// pass over o and do at memory rate.  (In the dq kernel, at the start of each
-// unit, its loads were waited for: 7 us a unit of 128 rows x 512 keys, whose
-// tiles take 8.)  D / 8 lanes a row.
-template <int D, bool F16>
+// delta = do . o of every row, where the keys take more than one tile (DELTA):
+// one pass over o and do at memory rate.  (In the dq kernel, at the start of
+// each unit, its loads were waited for: 7 us a unit of 128 rows x 512 keys,
+// whose tiles take 8.)  In f16 |do|^2 too, and v_sq set to 0 for the kernel
+// below.  D / 8 lanes a row.
+template <int D, bool F16, bool DELTA>
 __global__ void __launch_bounds__(256) xattn_delta_kernel(const __grid_constant__ XAttnGrad a) {
   constexpr int LPR = D / 8;
   constexpr int ROWS = 4;  // a thread's loads in flight
@@ -597,6 +620,8 @@ __global__ void __launch_bounds__(256) xattn_delta_kernel(const __grid_constant_
   const uint32_t first = blockIdx.x * (256 / LPR) * ROWS + threadIdx.x / LPR;
   const int col = (threadIdx.x % LPR) * 8;
   const uint32_t rows = static_cast<uint32_t>(a.batch) * a.s_q * a.heads;
+  if (F16 && blockIdx.x == 0)
+    for (int i = threadIdx.x; i < a.batch * a.kv_heads; i += 256) a.v_sq[i] = 0.0f;
   uint4 ov[ROWS], gv[ROWS];
   int64_t at[ROWS];
 #pragma unroll
@@ -609,8 +634,9 @@ __global__ void __launch_bounds__(256) xattn_delta_kernel(const __grid_constant_
       const int64_t head = i - bt * a.heads;
       const uint32_t b32 = bt / static_cast<uint32_t>(a.s_q);
       const int64_t b = b32, tok = bt - b32 * a.s_q;
-      ov[k] = __ldg(reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(a.o) + b * a.o_stride[0] +
-                                                   tok * a.o_stride[1] + head * a.o_stride[2] + col));
+      if constexpr (DELTA)
+        ov[k] = __ldg(reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(a.o) + b * a.o_stride[0] +
+                                                     tok * a.o_stride[1] + head * a.o_stride[2] + col));
       gv[k] = __ldg(reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(a.d_o) + b * a.do_stride[0] +
                                                    tok * a.do_stride[1] + head * a.do_stride[2] + col));
       at[k] = (b * a.heads + head) * a.s_q + tok;
@@ -619,21 +645,68 @@ __global__ void __launch_bounds__(256) xattn_delta_kernel(const __grid_constant_
 #pragma unroll
   for (int k = 0; k < ROWS; ++k) {
     const uint32_t ow[4] = {ov[k].x, ov[k].y, ov[k].z, ov[k].w}, gw[4] = {gv[k].x, gv[k].y, gv[k].z, gv[k].w};
-    float s = 0.0f;
+    float s = 0.0f, sq = 0.0f;
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
       if constexpr (F16) {
         const float2 of = __half22float2(*reinterpret_cast<const __half2*>(&ow[e]));
         const float2 gf = __half22float2(*reinterpret_cast<const __half2*>(&gw[e]));
         s = fmaf(of.x, gf.x, fmaf(of.y, gf.y, s));
+        sq = fmaf(gf.x, gf.x, fmaf(gf.y, gf.y, sq));
       } else {
         s = fmaf(bf16lo_to_f32(ow[e]), bf16lo_to_f32(gw[e]), s);
         s = fmaf(bf16hi_to_f32(ow[e]), bf16hi_to_f32(gw[e]), s);
       }
     }
 #pragma unroll
-    for (int o = LPR / 2; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-    if (at[k] >= 0 && threadIdx.x % LPR == 0) a.delta[at[k]] = s;
+    for (int o = LPR / 2; o > 0; o >>= 1) {
+      if constexpr (DELTA) s += __shfl_xor_sync(0xffffffffu, s, o);
+      if constexpr (F16) sq += __shfl_xor_sync(0xffffffffu, sq, o);
+    }
+    if (at[k] >= 0 && threadIdx.x % LPR == 0) {
+      if constexpr (DELTA) a.delta[at[k]] = s;
+      if constexpr (F16) a.do_sq[at[k]] = sq;
+    }
+  }
+}
+
+// f16: the largest |v|^2 of a sample's kept keys; one block for NORM_KEYS keys of
+// a key head.  (As unsigned numbers: a NaN is the largest.  The maximum
+// does not depend on the order of the blocks.)
+constexpr int NORM_KEYS = 64;
+template <int D>
+__global__ void __launch_bounds__(256) xattn_value_norm_kernel(const __grid_constant__ XAttnGrad a) {
+  constexpr int LPR = D / 8;
+  __shared__ uint32_t s_top[8];
+  const int chunks = (a.s_kv + NORM_KEYS - 1) / NORM_KEYS;
+  const int chunk = blockIdx.x % chunks, slab = blockIdx.x / chunks;  // slab: (sample, key head)
+  const int kvh = slab % a.kv_heads, b = slab / a.kv_heads;
+  const int len = len_of(a, b);
+  const uint16_t* v = static_cast<const uint16_t*>(a.v) + b * a.kv_stride[0] + kvh * a.kv_stride[2] + (threadIdx.x % LPR) * 8;
+  uint32_t top = 0;
+#pragma unroll
+  for (int i = 0; i < NORM_KEYS * LPR / 256; ++i) {
+    const int key = chunk * NORM_KEYS + i * (256 / LPR) + static_cast<int>(threadIdx.x) / LPR;
+    float sq = 0.0f;
+    if (key < len && (a.key_mask == nullptr || __ldg(a.key_mask + b * a.mask_stride + key) != 0)) {
+      const uint4 x = __ldg(reinterpret_cast<const uint4*>(v + key * a.kv_stride[1]));
+      const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[e]));
+        sq = fmaf(f.x, f.x, fmaf(f.y, f.y, sq));
+      }
+    }
+#pragma unroll
+    for (int o = LPR / 2; o > 0; o >>= 1) sq += __shfl_xor_sync(0xffffffffu, sq, o);
+    top = max(top, __float_as_uint(sq) & 0x7fffffffu);
+  }
+  top = __reduce_max_sync(0xffffffffu, top);
+  if ((threadIdx.x & 31) == 0) s_top[threadIdx.x >> 5] = top;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    for (int i = 1; i < 8; ++i) top = max(top, s_top[i]);
+    if (top != 0) atomicMax(reinterpret_cast<uint32_t*>(a.v_sq) + slab, top);
   }
 }
 
@@ -1078,11 +1151,22 @@ int launch(const XAttnGrad& a, cudaStream_t stream) {
   const int64_t qu = static_cast<int64_t>(a.batch) * a.heads * args.q_tiles;
   const int64_t ku = static_cast<int64_t>(a.batch) * a.kv_heads * args.k_tiles * a.splits;
   if (qu > 0x3fffffff || ku > 0x3fffffff) return H3B_ERR_SHAPE;
-  if (args.k_tiles > 1) {
+  if (args.k_tiles > 1 || (F16 && args.k_tiles > 0)) {
     const int64_t per = 4 * 256 / (D / 8);  // rows of a block
     const int64_t blocks = (static_cast<int64_t>(a.batch) * a.s_q * a.heads + per - 1) / per;
     if (blocks > 0x7fffffff) return H3B_ERR_SHAPE;
-    xattn_delta_kernel<D, F16><<<static_cast<unsigned>(blocks), 256, 0, stream>>>(a);
+    if (args.k_tiles > 1) {
+      xattn_delta_kernel<D, F16, true><<<static_cast<unsigned>(blocks), 256, 0, stream>>>(a);
+    } else {
+      xattn_delta_kernel<D, true, false><<<static_cast<unsigned>(blocks), 256, 0, stream>>>(a);
+    }
+    rc = h3b::launch_status();
+    if (rc != H3B_OK) return rc;
+  }
+  if (F16 && args.k_tiles > 0) {
+    const int64_t blocks = static_cast<int64_t>(a.batch) * a.kv_heads * ((a.s_kv + NORM_KEYS - 1) / NORM_KEYS);
+    if (blocks > 0x7fffffff) return H3B_ERR_SHAPE;
+    xattn_value_norm_kernel<D><<<static_cast<unsigned>(blocks), 256, 0, stream>>>(a);
     rc = h3b::launch_status();
     if (rc != H3B_OK) return rc;
   }
