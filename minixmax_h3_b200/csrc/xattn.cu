@@ -170,7 +170,7 @@ int64_t grad_part_floats(const h3b::XAttnGrad& a) {
 }
 int64_t grad_rows(const h3b::XAttnGrad& a) { return static_cast<int64_t>(a.batch) * a.heads * a.s_q; }
 int64_t grad_workspace(const h3b::XAttnGrad& a) {
-  return (grad_part_floats(a) + 2 * grad_rows(a) + static_cast<int64_t>(a.batch) * a.kv_heads) *
+  return (grad_part_floats(a) + 2 * grad_rows(a) + 2ll * a.batch * a.kv_heads) *
          static_cast<int64_t>(sizeof(float));
 }
 h3b::XAttnGrad grad_sizes(int dtype, int64_t batch, int64_t heads, int64_t kv_heads, int64_t head_dim, int64_t s_q,
@@ -251,6 +251,7 @@ extern "C" int h3b_cross_attention_bwd(const void* d_o, const void* q, const voi
   a.delta = a.part + grad_part_floats(a);
   a.do_sq = a.delta + grad_rows(a);
   a.v_sq = a.do_sq + grad_rows(a);
+  a.do_top = a.v_sq + batch * kv_heads;
   a.kv_lens = kv_lens;
   a.key_mask = s_kv > 0 ? key_mask : nullptr;
   a.mask_stride = mask_stride;

@@ -68,6 +68,7 @@ struct XAttnGrad {
   float* delta;  // workspace [batch, heads, s_q]
   float* do_sq;  // f16: workspace [batch, heads, s_q], |do|^2 of a row
   float* v_sq;   // f16: workspace [batch, kv_heads], largest |v|^2 of a kept key
+  float* do_top; // f16: behind it, [batch, kv_heads], largest |do|^2 of the rows that share a key head
   int splits;
   float* part;   // workspace [dv | dk][splits, batch, s_kv, kv_heads, D], if splits > 1
 };

@@ -29,13 +29,15 @@
 // one dP^T beside the sums (128 x 512 columns are full).
 // In f16, P is held times 2^8 (P <= 1), which lowers the point where small
 // weights lose bits.  dS has the size of the caller's gradients, which may be
-// anything, so in dq it is held times a power of two of its row, which the fp32
-// result is divided by: |dP - delta| <= 2 |do| |v|, and the factor brings that
-// bound to 2^14 .. 2^15.  Without it do ~ 1e-4 lost 1 % of dq over 1024 keys in
-// f16's smallest numbers, and left-out keys (dS = -delta P there, see warp 10)
-// made infinities, so NaN, of delta above 65504.  The norms cost a pass over
-// do, with delta's where that is taken, and one over v (2 x 2049 x 1025, 24
-// heads on 6 of 128: 5 us and a launch, 330 -> 340 with the forward).
+// anything, so it is held times a power of two, of its row in dq, of its sample
+// and key head in dk (whose sums run over the rows), which the fp32 result is
+// divided by: |dP - delta| <= 2 |do| |v|, and the factor brings that bound to
+// 2^14 .. 2^15.  Without it do ~ 1e-4 lost 1 % of dq and dk over 1024 keys in
+// f16's smallest numbers, several thousands passed its largest, and left-out
+// keys (dS = -delta P in dq, see warp 10) made infinities, so NaN, of delta
+// above 65504.  The norms cost a pass over do (delta's, where that is
+// taken) and one over v: 2 x 2049 x 1025, 24 heads on 6 of 128, 5 us and a launch
+// (330 -> 341 with the forward); 16384 x 77, 24 heads of 128, 32 us of 226.
 #include "h3b_common.cuh"
 #include "h3b_host.hpp"
 #include "xattn.hpp"
@@ -610,8 +612,8 @@ __global__ void __launch_bounds__(THREADS, 1)
 // delta = do . o of every row, where the keys take more than one tile (DELTA):
 // one pass over o and do at memory rate.  (In the dq kernel, at the start of
 // each unit, its loads were waited for: 7 us a unit of 128 rows x 512 keys,
-// whose tiles take 8.)  In f16 |do|^2 too, and v_sq set to 0 for the kernel
-// below.  D / 8 lanes a row.
+// whose tiles take 8.)  In f16 |do|^2 too, and the maxima set to 0 for the
+// kernel below.  D / 8 lanes a row.
 template <int D, bool F16, bool DELTA>
 __global__ void __launch_bounds__(256) xattn_delta_kernel(const __grid_constant__ XAttnGrad a) {
   constexpr int LPR = D / 8;
@@ -621,7 +623,7 @@ __global__ void __launch_bounds__(256) xattn_delta_kernel(const __grid_constant_
   const int col = (threadIdx.x % LPR) * 8;
   const uint32_t rows = static_cast<uint32_t>(a.batch) * a.s_q * a.heads;
   if (F16 && blockIdx.x == 0)
-    for (int i = threadIdx.x; i < a.batch * a.kv_heads; i += 256) a.v_sq[i] = 0.0f;
+    for (int64_t i = threadIdx.x; i < 2ll * a.batch * a.kv_heads; i += 256) a.v_sq[i] = 0.0f;  // (and do_top)
   uint4 ov[ROWS], gv[ROWS];
   int64_t at[ROWS];
 #pragma unroll
@@ -670,22 +672,32 @@ __global__ void __launch_bounds__(256) xattn_delta_kernel(const __grid_constant_
   }
 }
 
-// f16: the largest |v|^2 of a sample's kept keys; one block for NORM_KEYS keys of
-// a key head.  (As unsigned numbers: a NaN is the largest.  The maximum
-// does not depend on the order of the blocks.)
-constexpr int NORM_KEYS = 64;
+// f16: the largest |v|^2 of a sample's kept keys (the first blocks, NORM_KEYS
+// keys of a key head each) and the largest |do|^2 of the rows that share the key
+// head (the others, NORM_ROWS rows each).  (As unsigned numbers: a NaN is the
+// largest.  The maximum does not depend on the order of the blocks.)
+constexpr int NORM_KEYS = 64, NORM_ROWS = 2048;
 template <int D>
-__global__ void __launch_bounds__(256) xattn_value_norm_kernel(const __grid_constant__ XAttnGrad a) {
+__global__ void __launch_bounds__(256) xattn_norms_kernel(const __grid_constant__ XAttnGrad a, int key_blocks) {
   constexpr int LPR = D / 8;
   __shared__ uint32_t s_top[8];
-  const int chunks = (a.s_kv + NORM_KEYS - 1) / NORM_KEYS;
-  const int chunk = blockIdx.x % chunks, slab = blockIdx.x / chunks;  // slab: (sample, key head)
+  const bool keys = static_cast<int>(blockIdx.x) < key_blocks;
+  const int x = keys ? blockIdx.x : blockIdx.x - key_blocks;
+  const int rows = a.heads / a.kv_heads * a.s_q;  // the group's heads lie one behind the other
+  const int chunks = keys ? (a.s_kv + NORM_KEYS - 1) / NORM_KEYS : (rows + NORM_ROWS - 1) / NORM_ROWS;
+  const int chunk = x % chunks, slab = x / chunks;  // slab: (sample, key head)
   const int kvh = slab % a.kv_heads, b = slab / a.kv_heads;
   const int len = len_of(a, b);
   const uint16_t* v = static_cast<const uint16_t*>(a.v) + b * a.kv_stride[0] + kvh * a.kv_stride[2] + (threadIdx.x % LPR) * 8;
   uint32_t top = 0;
 #pragma unroll
-  for (int i = 0; i < NORM_KEYS * LPR / 256; ++i) {
+  for (int i = 0; i < NORM_ROWS / 256; ++i) {
+    const int row = chunk * NORM_ROWS + i * 256 + static_cast<int>(threadIdx.x);
+    if (!keys && row < rows)
+      top = max(top, __float_as_uint(a.do_sq[static_cast<int64_t>(slab) * rows + row]) & 0x7fffffffu);
+  }
+#pragma unroll
+  for (int i = 0; i < NORM_KEYS * LPR / 256 && keys; ++i) {
     const int key = chunk * NORM_KEYS + i * (256 / LPR) + static_cast<int>(threadIdx.x) / LPR;
     float sq = 0.0f;
     if (key < len && (a.key_mask == nullptr || __ldg(a.key_mask + b * a.mask_stride + key) != 0)) {
@@ -706,7 +718,7 @@ __global__ void __launch_bounds__(256) xattn_value_norm_kernel(const __grid_cons
   __syncthreads();
   if (threadIdx.x == 0) {
     for (int i = 1; i < 8; ++i) top = max(top, s_top[i]);
-    if (top != 0) atomicMax(reinterpret_cast<uint32_t*>(a.v_sq) + slab, top);
+    if (top != 0) atomicMax(reinterpret_cast<uint32_t*>(keys ? a.v_sq : a.do_top) + slab, top);
   }
 }
 
@@ -734,6 +746,14 @@ constexpr size_t dkv_smem() {
 }
 
 static_assert(dkv_smem<128>() <= 232448, "shared memory of a CTA");
+
+// What dP - delta is multiplied by: f16, dS's factor without P's 2^P_SHIFT.
+template <bool F16>
+H3B_DEV float dp_factor(const XAttnGrad& a, int b, int kvh) {
+  if constexpr (!F16) return 1.0f;
+  const int64_t at = static_cast<int64_t>(b) * a.kv_heads + kvh;
+  return ds_factor(a.v_sq[at] * a.do_top[at]) * 0.00390625f;
+}
 
 struct DkvUnit {
   int b, kvh, key0, split, len;
@@ -771,7 +791,7 @@ __global__ void __launch_bounds__(THREADS, 1)
   uint8_t* sR = smem;
   uint8_t* sK = sR + RST * C::TILE_BYTES;
   uint8_t* sV = sK + C::TILE_BYTES;
-  float* s_stat = reinterpret_cast<float*>(sV + C::TILE_BYTES);  // [STATS][shift - lse2 | delta scaled][128]
+  float* s_stat = reinterpret_cast<float*>(sV + C::TILE_BYTES);  // [STATS][shift - lse2 | -delta scaled][128]
   DkvBars* bars = reinterpret_cast<DkvBars*>(s_stat + STATS * 2 * 128);
   const XAttnGrad& a = args.a;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -928,6 +948,7 @@ __global__ void __launch_bounds__(THREADS, 1)
       bool ok = true;
       for (int x = blockIdx.x; x < args.units && ok; x += gridDim.x) {
         const DkvUnit u = dkv_unit(args, x);
+        const float factor = dp_factor<F16>(a, u.b, u.kvh);
         for (int i = 0; i < u.n; ++i, ++step) {
           const int head = u.kvh * args.group + (u.t0 + i) / args.q_tiles;
           const int q0 = ((u.t0 + i) % args.q_tiles) * 128;
@@ -938,7 +959,7 @@ __global__ void __launch_bounds__(THREADS, 1)
             const int r = q0 + c * 32 + lane;
             const bool in = r < a.s_q;
             lse[c] = in ? P_SHIFT - lse2_of(__ldg(a.lse + at + r)) : -INFINITY;
-            del[c] = in ? -a.delta[at + r] * P_UNIT : 0.0f;
+            del[c] = in ? -a.delta[at + r] * factor : 0.0f;
           }
           const int s = step % STATS;
           if (step >= STATS && !warp_wait(&bars->stat_free[s], (step / STATS - 1) & 1, 14, abort_flag)) {
@@ -968,6 +989,7 @@ __global__ void __launch_bounds__(THREADS, 1)
     for (int x = blockIdx.x; x < args.units && ok; x += gridDim.x) {
       const DkvUnit u = dkv_unit(args, x);
       const int key = u.key0 + row;
+      const float factor = dp_factor<F16>(a, u.b, u.kvh);
       const bool kept = key < u.len && (a.key_mask == nullptr || __ldg(a.key_mask + u.b * a.mask_stride + key) != 0);
       for (int i = 0; i < u.n; ++i, ++step) {
         const int slot = step % STATS;
@@ -1009,7 +1031,7 @@ __global__ void __launch_bounds__(THREADS, 1)
         tmem_ld32p(dp_tmem, d);
         tmem_ld32p(dp_tmem + 32, d + 32);
         tmem_wait_fence<2>(d);
-        const float2 pu = make_float2(P_UNIT, P_UNIT);
+        const float2 pu = make_float2(factor, factor);
 #pragma unroll
         for (int e = 0; e < 64; e += 4) {
           const float4 l = del[e / 4];
@@ -1046,7 +1068,7 @@ __global__ void __launch_bounds__(THREADS, 1)
         ++oc;
         tc_fence_after();
       }
-      const float f = wg ? a.scale : P_UNIT;
+      const float f = wg ? (F16 ? a.scale * inverse_of_power(factor) * P_UNIT : a.scale) : P_UNIT;
       const int64_t key_row = (static_cast<int64_t>(u.b) * a.s_kv + key) * a.kv_heads + u.kvh;
       const int64_t per_split = static_cast<int64_t>(a.batch) * a.s_kv * a.kv_heads;
 #pragma unroll
@@ -1164,9 +1186,11 @@ int launch(const XAttnGrad& a, cudaStream_t stream) {
     if (rc != H3B_OK) return rc;
   }
   if (F16 && args.k_tiles > 0) {
-    const int64_t blocks = static_cast<int64_t>(a.batch) * a.kv_heads * ((a.s_kv + NORM_KEYS - 1) / NORM_KEYS);
+    const int64_t slabs = static_cast<int64_t>(a.batch) * a.kv_heads, rows = static_cast<int64_t>(args.group) * a.s_q;
+    const int64_t key_blocks = slabs * ((a.s_kv + NORM_KEYS - 1) / NORM_KEYS);
+    const int64_t blocks = key_blocks + slabs * ((rows + NORM_ROWS - 1) / NORM_ROWS);
     if (blocks > 0x7fffffff) return H3B_ERR_SHAPE;
-    xattn_value_norm_kernel<D><<<static_cast<unsigned>(blocks), 256, 0, stream>>>(a);
+    xattn_norms_kernel<D><<<static_cast<unsigned>(blocks), 256, 0, stream>>>(a, static_cast<int>(key_blocks));
     rc = h3b::launch_status();
     if (rc != H3B_OK) return rc;
   }

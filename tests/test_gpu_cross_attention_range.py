@@ -105,6 +105,35 @@ def test_f16_dq_of_any_size(cuda, d, size, s_kv):
     check(gradients(q, k, v, do)[2][0], formula(q, k, v, None, None, do)[2], F16, "dq", small=True)
 
 
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("size", [1e-5, 1e-4, 1e-3, 1e3])
+@pytest.mark.parametrize("s_kv", [100, 1024])
+def test_f16_dk_and_dv_of_any_size(cuda, d, size, s_kv):
+    """The same for dk, with large queries; samples and heads of different
+    size do not share what their gradients are scaled by."""
+    q, k, v, do = make(cuda, 2, 512, s_kv, 4, 2, d, F16, seed=d + s_kv + 1)
+    q, k, do = q * 32, k / 32, (do.float() * size).to(F16)
+    do[1] = (do[1].float() * 0.01).to(F16)
+    want = formula(q, k, v, None, None, do)
+    _, dk, dv = gradients(q, k, v, do)[2]
+    for b in range(2):
+        check(dk[b], want[3][b], F16, "dk", small=True)
+        check(dv[b], want[4][b], F16, "dv", small=True)
+
+
+@pytest.mark.parametrize("d", [64, 128])
+def test_f16_dk_of_large_gradients(cuda, d):
+    """Two keys and gradients of several thousands: dS passes f16's largest
+    number, dq, dk and dv do not."""
+    q, k, v, do = make(cuda, 2, 4, 2, 2, 2, d, F16, seed=d)
+    q, k, do = q / 4, k / 4, (do.float() * 8e3 * (128 / d) ** 0.5).to(F16)
+    want = formula(q, k, v, None, None, do)
+    s = torch.einsum("bihd,bjhd->bhij", do.double().cpu(), v.double().cpu())
+    assert d == 64 or (s[..., 0] - s[..., 1]).abs().max() * 0.25 > 65504  # (at 64 the largest dS is just below)
+    for got, w, name in zip(gradients(q, k, v, do)[2], want[2:], ("dq", "dk", "dv")):
+        check(got, w, F16, name)
+
+
 def test_f16_gradients_of_nothing(cuda):
     """do of zero, values of zero, rows without a key beside others: zeros,
     not 0 times the largest power of two."""
