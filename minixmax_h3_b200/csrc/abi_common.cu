@@ -47,49 +47,53 @@ static PFN_cuTensorMapEncodeTiled_v12000 encode_fn() {
   return fn;
 }
 
-int encode_2d(CUtensorMap* map, CUtensorMapDataType dtype, const void* base, uint64_t inner, uint64_t outer,
-              uint64_t row_stride_bytes, uint32_t box_inner, uint32_t box_outer, CUtensorMapSwizzle swizzle) {
+// The driver's encoder wants a current context.  A thread has none before its
+// first call of the runtime that needs one (autograd's thread, a server's
+// worker whose tensors come from the allocator's cache): it gets the current
+// device's then, as a launch would give it.
+static int encode(CUtensorMap* map, CUtensorMapDataType dtype, uint32_t rank, const void* base, const cuuint64_t* dims,
+                  const cuuint64_t* strides, const cuuint32_t* box, CUtensorMapSwizzle swizzle) {
   auto fn = encode_fn();
   if (fn == nullptr) return H3B_ERR_LAUNCH;
+  const cuuint32_t estr[4] = {1, 1, 1, 1};
+  auto run = [&] {
+    return fn(map, dtype, rank, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle,
+              CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  };
+  CUresult r = run();
+  int dev = 0;
+  if (r == CUDA_ERROR_INVALID_CONTEXT && cudaGetDevice(&dev) == cudaSuccess && cudaSetDevice(dev) == cudaSuccess) r = run();
+  return r == CUDA_SUCCESS ? H3B_OK : H3B_ERR_TMAP;
+}
+
+int encode_2d(CUtensorMap* map, CUtensorMapDataType dtype, const void* base, uint64_t inner, uint64_t outer,
+              uint64_t row_stride_bytes, uint32_t box_inner, uint32_t box_outer, CUtensorMapSwizzle swizzle) {
   cuuint64_t dims[2] = {inner, outer};
   cuuint64_t strides[1] = {row_stride_bytes};
   cuuint32_t box[2] = {box_inner, box_outer};
-  cuuint32_t estr[2] = {1, 1};
-  CUresult r = fn(map, dtype, 2, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                  swizzle, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-  return r == CUDA_SUCCESS ? H3B_OK : H3B_ERR_TMAP;
+  return encode(map, dtype, 2, base, dims, strides, box, swizzle);
 }
 
 int encode_3d(CUtensorMap* map, CUtensorMapDataType dtype, const void* base, uint64_t inner, uint64_t d1,
               uint64_t d2, uint64_t s1_bytes, uint64_t s2_bytes, uint32_t box_inner, uint32_t box_d1,
               uint32_t box_d2, CUtensorMapSwizzle swizzle) {
-  auto fn = encode_fn();
-  if (fn == nullptr) return H3B_ERR_LAUNCH;
   cuuint64_t dims[3] = {inner, d1, d2};
   cuuint64_t strides[2] = {s1_bytes, s2_bytes};
   cuuint32_t box[3] = {box_inner, box_d1, box_d2};
-  cuuint32_t estr[3] = {1, 1, 1};
-  CUresult r = fn(map, dtype, 3, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                  swizzle, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-  return r == CUDA_SUCCESS ? H3B_OK : H3B_ERR_TMAP;
+  return encode(map, dtype, 3, base, dims, strides, box, swizzle);
 }
 
 int encode_4d(CUtensorMap* map, CUtensorMapDataType dtype, const void* base, const uint64_t (&dims)[4],
               const uint64_t (&strides_bytes)[3], const uint32_t (&box)[4], CUtensorMapSwizzle swizzle) {
-  auto fn = encode_fn();
-  if (fn == nullptr) return H3B_ERR_LAUNCH;
   cuuint64_t d[4];
   cuuint64_t st[3];
   cuuint32_t b[4];
-  cuuint32_t estr[4] = {1, 1, 1, 1};
   for (int i = 0; i < 4; ++i) {
     d[i] = dims[i];
     b[i] = box[i];
     if (i > 0) st[i - 1] = strides_bytes[i - 1];
   }
-  CUresult r = fn(map, dtype, 4, const_cast<void*>(base), d, st, b, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle,
-                  CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-  return r == CUDA_SUCCESS ? H3B_OK : H3B_ERR_TMAP;
+  return encode(map, dtype, 4, base, d, st, b, swizzle);
 }
 
 }  // namespace h3b
