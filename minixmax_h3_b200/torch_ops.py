@@ -19,6 +19,7 @@ kernel of the path:
         -> (q int8 [m, hidden], scale fp32 [m])
     h3b::cross_attention(q, k, v, kv_lens, key_mask, scale)
         -> (o [B, Sq, H, D], lse fp32 [B, H, Sq]); differentiable in q, k, v
+           through o (a loss that uses lse raises)
     h3b::cross_attention_bwd(dout, q, k, v, out, lse, kv_lens, key_mask, scale) -> (dq, dk, dv)
     h3b::kv8_append(k, v, codes and scales of K and V, block_table, lens, new_lens) -> None  (updates the cache)
     h3b::kv8_attention(q, codes and scales, block_table, lens, causal, scale) -> o [B, Sq, H, D]
@@ -244,10 +245,12 @@ def _cross_attention_setup(ctx, inputs, output):
     q, k, v, kv_lens, key_mask, scale = inputs
     ctx.save_for_backward(q, k, v, *output, kv_lens, key_mask)
     ctx.scale = scale
+    ctx.set_materialize_grads(False)  # (a gradient of lse is None unless something has used it)
 
 
 def _cross_attention_grad(ctx, dout, dlse):
-    del dlse  # the log-sum-exps are for the backward pass only
+    if dlse is not None:
+        raise RuntimeError("h3b::cross_attention has no gradient through lse (it is for the backward pass): detach it")
     q, k, v, out, lse, kv_lens, key_mask = ctx.saved_tensors
     grads = torch.ops.h3b.cross_attention_bwd(dout, q, k, v, out, lse, kv_lens, key_mask, ctx.scale)
     return (*grads, None, None, None)

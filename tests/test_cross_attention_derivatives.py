@@ -1,0 +1,65 @@
+"""CPU: derivatives that cross attention does not have raise, none is silently
+left out (the library is replaced by a stub; no kernel runs)."""
+from __future__ import annotations
+
+import pytest
+import torch
+import torch.autograd.forward_ad as fwd
+
+from minixmax_h3_b200 import attention, ops
+from minixmax_h3_b200 import torch_ops as T
+
+BF16 = torch.bfloat16
+
+
+def qkv(**kw):
+    return [torch.randn(1, n, 2, 64, **kw).to(BF16) for n in (4, 5, 5)]
+
+
+@pytest.fixture
+def stub(monkeypatch):
+    """The entry points' results without their work."""
+    monkeypatch.setattr(ops, "_cuda", lambda *a: None)
+    monkeypatch.setattr(ops, "call", lambda *a: None)
+    monkeypatch.setattr(ops, "_stream", lambda t: 0)
+    monkeypatch.setattr(ops, "_workspace", lambda *a: None)
+
+
+@pytest.fixture
+def cpu_operator(stub):
+    """h3b::cross_attention with its own formula for gradients, for CPU
+    tensors under another name."""
+    lib = torch.library.custom_op("h3b_test::cross_attention", mutates_args=())(T._cross_attention)
+    lib.register_autograd(T._cross_attention_grad, setup_context=T._cross_attention_setup)
+    return lib
+
+
+def test_gradient_through_the_log_sum_exps_raises(cpu_operator, monkeypatch):
+    """lse is for the backward pass: a loss that uses it has no gradient here,
+    alone or beside one that uses o."""
+    def no_bwd(*a):
+        pytest.fail("gradients without the part of lse")
+
+    q, k, v = (t.requires_grad_() for t in qkv())
+    for loss in (lambda o, lse: lse.sum(), lambda o, lse: lse.sum() + o.float().sum()):
+        out = cpu_operator(q, k, v, None, None, None)
+        with monkeypatch.context() as m:
+            m.setattr(T.torch.ops.h3b, "cross_attention_bwd", no_bwd, raising=False)
+            with pytest.raises(RuntimeError, match="lse"):
+                loss(*out).backward()
+
+
+def test_gradient_of_the_result_alone(cpu_operator, monkeypatch):
+    q, k, v = (t.requires_grad_() for t in qkv())
+    o, _ = cpu_operator(q, k, v, None, None, None)
+    do = torch.randn_like(o)
+    seen = []
+
+    def bwd(dout, q, k, v, *rest):
+        seen.append(dout)
+        return torch.ones_like(q), 2 * torch.ones_like(k), 3 * torch.ones_like(v)
+
+    monkeypatch.setattr(T.torch.ops.h3b, "cross_attention_bwd", bwd, raising=False)
+    got = torch.autograd.grad(o, (q, k, v), do)
+    assert len(seen) == 1 and torch.equal(seen[0], do)
+    assert [g.flatten()[0].item() for g in got] == [1, 2, 3]
