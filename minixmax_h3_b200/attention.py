@@ -16,6 +16,7 @@ from __future__ import annotations
 from typing import Optional
 
 import torch
+from torch.autograd import forward_ad
 
 from . import ops
 
@@ -77,15 +78,24 @@ class _CrossAttentionGrad(torch.autograd.Function):
         raise RuntimeError("cross_attention has no second derivatives")
 
 
+def refuse_tangents(*ts: torch.Tensor) -> None:
+    """Raises if a tensor carries a forward-mode tangent: the kernels' results
+    would come back without one.  (Where reverse mode is recorded too, the
+    autograd function raises by itself.)"""
+    if any(forward_ad.unpack_dual(t).tangent is not None for t in ts):
+        raise NotImplementedError("cross_attention has no forward-mode derivatives")
+
+
 def cross_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, kv_lens: Optional[torch.Tensor] = None,
                     key_mask: Optional[torch.Tensor] = None, scale: Optional[float] = None) -> torch.Tensor:
     """ops.cross_attention (q [B, Sq, H, D], k and v [B, Skv, Hkv, D]; see
     there for kv_lens and key_mask), differentiable by autograd in q, k and v.
     The backward pass is one call of ops.cross_attention_bwd; it keeps q, k,
     v, the result and a log-sum-exp per row, and is bit-reproducible.  There
-    are no second derivatives: asking for them raises."""
+    are no second derivatives and no forward-mode ones: asking for them raises."""
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
         return _CrossAttention.apply(q, k, v, kv_lens, key_mask, scale)
+    refuse_tangents(q, k, v)
     return ops.cross_attention(q, k, v, kv_lens=kv_lens, key_mask=key_mask, scale=scale)
 
 

@@ -19,7 +19,7 @@ kernel of the path:
         -> (q int8 [m, hidden], scale fp32 [m])
     h3b::cross_attention(q, k, v, kv_lens, key_mask, scale)
         -> (o [B, Sq, H, D], lse fp32 [B, H, Sq]); differentiable in q, k, v
-           through o (a loss that uses lse raises)
+           through o (a loss that uses lse raises, and so does forward mode)
     h3b::cross_attention_bwd(dout, q, k, v, out, lse, kv_lens, key_mask, scale) -> (dq, dk, dv)
     h3b::kv8_append(k, v, codes and scales of K and V, block_table, lens, new_lens) -> None  (updates the cache)
     h3b::kv8_attention(q, codes and scales, block_table, lens, causal, scale) -> o [B, Sq, H, D]
@@ -41,7 +41,7 @@ from typing import Optional
 import torch
 
 from . import ops
-from .attention import h3_attention_bnsd
+from .attention import h3_attention_bnsd, refuse_tangents
 
 _GEMM_EPILOGUES = (ops.EPI_STORE, ops.EPI_GELU, ops.EPI_SWIGLU)
 
@@ -123,6 +123,7 @@ def _rmsnorm_modulate_quant_i8(x: torch.Tensor, weight: torch.Tensor, shift: tor
 def _cross_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, kv_lens: Optional[torch.Tensor] = None,
                      key_mask: Optional[torch.Tensor] = None,
                      scale: Optional[float] = None) -> tuple[torch.Tensor, torch.Tensor]:
+    refuse_tangents(q, k, v)
     lse = torch.empty((q.shape[0], q.shape[2], q.shape[1]), dtype=torch.float32, device=q.device)
     return ops.cross_attention(q, k, v, kv_lens=kv_lens, key_mask=key_mask, scale=scale, lse=lse), lse
 

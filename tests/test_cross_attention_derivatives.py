@@ -63,3 +63,28 @@ def test_gradient_of_the_result_alone(cpu_operator, monkeypatch):
     got = torch.autograd.grad(o, (q, k, v), do)
     assert len(seen) == 1 and torch.equal(seen[0], do)
     assert [g.flatten()[0].item() for g in got] == [1, 2, 3]
+
+
+@pytest.mark.parametrize("which", [0, 1, 2])
+@pytest.mark.parametrize("grad", [False, True])
+def test_forward_mode_raises(stub, which, grad):
+    """A tangent of q, k or v must not be dropped."""
+    with fwd.dual_level():
+        args = qkv()
+        args[which] = fwd.make_dual(args[which], torch.ones_like(args[which]))
+        if grad:
+            args[(which + 1) % 3].requires_grad_()
+        with pytest.raises(NotImplementedError):
+            attention.cross_attention(*args)
+        attention.cross_attention(*qkv())
+    attention.cross_attention(*qkv())
+
+
+@pytest.mark.parametrize("which", [0, 1, 2])
+def test_forward_mode_of_the_operator_raises(cpu_operator, which):
+    with fwd.dual_level():
+        args = qkv()
+        args[which] = fwd.make_dual(args[which], torch.ones_like(args[which]))
+        with pytest.raises(NotImplementedError):
+            cpu_operator(*args, None, None, None)
+        cpu_operator(*qkv(), None, None, None)
