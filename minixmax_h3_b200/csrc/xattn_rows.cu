@@ -6,8 +6,11 @@
 // with the running max M and sum l of a softmax per row, in fp32.  For the
 // 8-bit cache k_j = sk K_j and v_j = sv V_j with one sk, sv per block of
 // tokens and head: sk goes into the factor of the score, and sv into its
-// exponent: w_j = 2^(x_j + log2 sv - M) is what multiplies the codes V_j (at
-// most 1, so it stays inside f16), and l += w_j / sv.  The codes themselves go
+// exponent: w_j = 2^(x_j + log2 sv - M) is what multiplies the codes V_j, and l
+// += w_j / sv.  M lies 14 below the running maximum where the weights are f16 (any
+// call over the cache, bf16 queries too): w is at most 2^14, and a weight keeps
+// its bits down to 2^-28 of the largest.  (At most 1, those below 2^-25 were 0 in
+// the product but not in l, which a long tail beside one large key makes visible.)  The codes themselves go
 // into the matrix instructions, exactly (|int8| <= 128 and every e4m3 value
 // are f16 numbers), so nothing is rounded between the cache and the product.
 //
@@ -164,6 +167,7 @@ __global__ void __launch_bounds__(WARPS * 32, MT == 1 ? 3 : 2)
   using T = Tile<D, KIND, MT>;
   constexpr bool CODES = KIND != KV_DENSE;
   constexpr bool F16 = CODES || QF16;  // operand type of the matrix instructions
+  constexpr float UP = F16 ? 14.0f : 0.0f;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + WARPS * T::RING_BYTES);
@@ -416,7 +420,7 @@ __global__ void __launch_bounds__(WARPS * 32, MT == 1 ? 3 : 2)
         top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
         // (a factor of 0 would make NaN of -inf: a row of zeros has e = 2^-126, zero keys sk = 1e-14)
         f[hf] = CODES ? fmaxf(mult[m][hf] * sk, 1e-37f) : mult[m][hf];
-        const float mn = fmaxf(M[m][hf], fmaf(top, f[hf], lsv));
+        const float mn = fmaxf(M[m][hf], fmaf(top, f[hf], lsv - UP));
         const float base = mn == -INFINITY ? 0.0f : mn;  // nothing kept so far: every weight is 2^-inf = 0
         corr[hf] = ex2(M[m][hf] - base);
         off[hf] = lsv - base;

@@ -30,7 +30,9 @@
 // P V_i has read it, and the commit behind S_i(t) says that O_i is settled as
 // well.
 // The running maximum is raised lazily, by steps of more than 2^8, so P <=
-// 2^8: exact in fp32 sums, inside f16's range.
+// 2^8: exact in fp32 sums.  f16 weights are held times 2^7 (UP), so that they
+// fill f16's range up to 2^15 and down to 2^-31 of the largest (a long tail of
+// small ones is in l, and has to be in the products).
 // Left-out keys: a score column is replaced (-inf) whatever it holds, and the
 // row of V is zeroed in shared memory before P V reads it (0 * NaN is NaN).
 // What bounds it is the chain softmax -> P V -> S -> softmax of a row tile and
@@ -58,6 +60,8 @@ constexpr int THREADS = 512;
 constexpr int REGS_LAUNCH = 128;
 constexpr int REGS_CONTROL = 64;
 constexpr float RESCALE_THRESHOLD = 8.0f;
+template <bool F16>
+constexpr float UP = F16 ? 7.0f : 0.0f;
 constexpr float LOG2E = 1.4426950408889634f;
 constexpr float LN2 = 0.69314718055994531f;
 
@@ -915,7 +919,7 @@ __global__ void __launch_bounds__(THREADS, 1)
               if (rescale) m_run = m_use;
             }
           }
-          const float neg_m = m_use == -INFINITY ? 0.0f : -m_use;
+          const float neg_m = m_use == -INFINITY ? 0.0f : UP<F16> - m_use;
           float2 sm;
           if constexpr (SCALED) {
             sm = exp_codes64<F16, true>(r, r, make_float2(fx[0], fx[1]), make_float2(ox[0] + neg_m, ox[1] + neg_m),
@@ -932,7 +936,7 @@ __global__ void __launch_bounds__(THREADS, 1)
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
           if (h == 1) {
-            const float neg_m = m_use == -INFINITY ? 0.0f : -m_use;
+            const float neg_m = m_use == -INFINITY ? 0.0f : UP<F16> - m_use;
             if constexpr (SCALED) {
               const float f[4] = {0.f, 0.f, 0.f, 0.f};
               const float2 o = lds2(info->v_log2 + 2);
@@ -953,7 +957,7 @@ __global__ void __launch_bounds__(THREADS, 1)
           // ---- the row statistics, to the storing warps
           if (oc > 0 && !warp_wait<true>(&bars->ml_free[wg], (oc - 1) & 1, 22, abort_flag)) break;
           ++oc;
-          s_ml[wg * 128 + row] = make_float2(m_run, l_run);
+          s_ml[wg * 128 + row] = make_float2(m_run - UP<F16>, l_run);
           __syncwarp();
           if (lane == 0) mbar_arrive(&bars->ml_full[wg]);
         }

@@ -153,6 +153,28 @@ def test_f16_gradients_of_nothing(cuda):
 # ----------------------------------------------------------------------------- weights far apart
 
 
+@pytest.mark.parametrize("s_q", [1, 200])
+@pytest.mark.parametrize("dtype", [F16, BF16])
+def test_long_tail_beside_a_dominant_key(cuda, s_q, dtype):
+    """One key 17 to 18 nats above many equal ones: each of their weights is
+    about 2^-25 of the first, their sum is not.  The dominant value is small
+    (absent where the rows' kernel has normal f16 weights), so that the sum
+    shows."""
+    from minixmax_h3_b200 import ops
+
+    n, h, d = 65536, 4, 64
+    gap = torch.tensor([17.0, 17.5, 18.0, 17.25], dtype=torch.float64)
+    q = (gap / 8)[None, None, :, None].expand(1, s_q, h, d).to(cuda, dtype).contiguous()  # (exact in 8 bits)
+    k, v = torch.zeros(1, n, h, d, dtype=dtype, device=cuda), torch.ones(1, n, h, d, dtype=dtype, device=cuda)
+    k[:, 0], v[:, 0] = 1.0, 0.0 if s_q == 1 else 1 / 64
+    lse = torch.empty(1, h, s_q, device=cuda)
+    o = ops.cross_attention(q, k, v, lse=lse)
+    top = torch.exp(gap)
+    want = (top * v[0, 0, 0, 0].item() + n - 1) / (top + n - 1)
+    check(o, want[None, None, :, None].expand(1, s_q, h, d), dtype)
+    assert torch.allclose(lse.double().cpu(), torch.log(top + n - 1)[None, :, None].expand(1, h, s_q), atol=2e-5, rtol=2e-6)
+
+
 # ----------------------------------------------------------------------------- NaN in kept places
 
 

@@ -34,3 +34,34 @@ def test_zero_queries_and_keys(cuda, qdt, dtype, s_q, causal):
     check(o, exact(q, c, table.cpu(), [n], causal, 64), qdt)
     seen = (n - s_q + 1 + torch.arange(s_q)).clamp(min=0) if causal else torch.full((s_q,), n)
     assert torch.allclose(lse.double().cpu(), torch.log(seen.double())[None, None].expand(1, 4, s_q), atol=2e-5, rtol=2e-6)
+
+
+@pytest.mark.parametrize("qdt", [BF16, F16])
+@pytest.mark.parametrize("dtype", CODES)
+@pytest.mark.parametrize("s_q,b,hkv", [(1, 110, 4), (130, 1, 4), (513, 1, 4)])
+def test_long_tail_beside_a_dominant_token(cuda, qdt, dtype, s_q, b, hkv):
+    """One token 17 to 18 nats above half a million equal ones: each of their
+    weights is about 2^-25 of the first, their sum is not.  The dominant value
+    is small (0 where a single row is asked for), so that the sum shows.  (The
+    tail's blocks are one block, named again and again.)"""
+    from minixmax_h3_b200 import ops
+
+    blocks, bt, d = 8192, 64, 64
+    n = blocks * bt
+    c = ops.KV8Cache.empty(2, hkv, d, block_tokens=bt, dtype=dtype, device=cuda)
+    one = torch.ones((), device=cuda)
+    c.v.copy_((64 * one).to(dtype).expand(c.v.shape))
+    c.k[0, :, 0], c.v[0, :, 0] = one.to(dtype), ((0 if s_q == 1 else 1) * one).to(dtype)
+    c.k_scale.fill_(1.0), c.v_scale.fill_(1 / 64)
+    table = torch.ones(b, blocks, dtype=torch.int32, device=cuda)
+    table[:, 0] = 0
+    gap = torch.tensor([17.0, 17.5, 18.0, 17.25], dtype=torch.float64)
+    q = (gap / 8)[None, None, :, None].expand(b, s_q, hkv, d).to(cuda, qdt).contiguous()  # (exact in 8 bits)
+    lse = torch.empty(b, hkv, s_q, device=cuda)
+    o = ops.kv8_attention(q, c, table, ints([n] * b, cuda), lse=lse)
+    top = torch.exp(gap)
+    want = (top * (0 if s_q == 1 else 1 / 64) + n - 1) / (top + n - 1)
+    check(o, want[None, None, :, None].expand(b, s_q, hkv, d), qdt)
+    # (a running fp32 sum is off by 2^-24 a step at most: a warp may take every fourth tile of 32 keys)
+    want = torch.log(top + n - 1)[None, :, None].expand(b, hkv, s_q)
+    assert torch.allclose(lse.double().cpu(), want, atol=2e-5 + n / 128 * 2.0 ** -24, rtol=2e-6)
