@@ -356,7 +356,8 @@ H3B_API int h3b_kv8_read(const uint8_t* k_codes, const uint8_t* v_codes, const f
  * causal != 0: the queries are the sequence's last s_q tokens (their keys
  * already appended), query i sees keys j <= lens[b] - s_q + i.  A row that
  * sees no key gives o = 0, lse = -inf.  The codes enter the products exactly;
- * the scales are applied to scores and weights in fp32.  workspace:
+ * the scales are applied to scores and weights in fp32 (a value scale below
+ * 7e-28, 0 among them, counts as 7e-28).  workspace:
  * h3b_kv8_attention_workspace() bytes (may be 0); where many query rows share
  * the keys it holds the codes as 16-bit operands, up to 8 GB.
  */

@@ -13,6 +13,13 @@ namespace h3b {
 // 8-bit cache (codes int8 or e4m3, one scale per block of tokens and head).
 enum KvKind { KV_DENSE = 0, KV_INT8 = 1, KV_E4M3 = 2 };
 
+// The smallest scale that a cache's block counts with: a scale of 0 (a block of
+// zeros; an empty cache) has no logarithm.  Its values are then off by 4e-25 at
+// most, and its tokens keep their share of the weights: an exponent lowered by
+// log2 of this (90) does not vanish beside blocks of scale 2^10 and scores 15 nats
+// above, and l = sum w / sv of 2^14 a token stays finite over 1.4e7 tokens.
+constexpr float KV8_SCALE_MIN = 7e-28f;
+
 // One attention call.  Strides are in elements, in the order (batch, token,
 // head); o_* as q_*.  Element (b, s, h, d) of q lies at q + b*q_stride[0] +
 // s*q_stride[1] + h*q_stride[2] + d.

@@ -49,6 +49,7 @@ namespace {
 using h3b::KV_DENSE;
 using h3b::KV_E4M3;
 using h3b::KV_INT8;
+using h3b::KV8_SCALE_MIN;
 using h3b::KvKind;
 using h3b::XAttn;
 
@@ -394,8 +395,8 @@ __global__ void __launch_bounds__(WARPS * 32, MT == 1 ? 3 : 2)
     }
 
     // ---- running softmax; x = score * mult * sk + log2 sv
-    const float lsv = CODES ? __log2f(fmaxf(sv, 1e-37f)) : 0.0f;
-    const float inv_sv = CODES ? 1.0f / fmaxf(sv, 1e-37f) : 1.0f;
+    const float lsv = CODES ? __log2f(fmaxf(sv, KV8_SCALE_MIN)) : 0.0f;
+    const float inv_sv = CODES ? 1.0f / fmaxf(sv, KV8_SCALE_MIN) : 1.0f;
     if (keep != all || key0 + T::KEYS > full_to) {
 #pragma unroll
       for (int m = 0; m < MT; ++m)

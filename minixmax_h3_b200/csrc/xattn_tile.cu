@@ -51,6 +51,7 @@ namespace {
 using h3b::KV_DENSE;
 using h3b::KV_E4M3;
 using h3b::KV_INT8;
+using h3b::KV8_SCALE_MIN;
 using h3b::KvKind;
 using h3b::XAttn;
 
@@ -756,7 +757,7 @@ __global__ void __launch_bounds__(THREADS, 1)
           for (int c = 0; c < 4; ++c)
             if (((there >> c) & 1u) == 0) w[c] = 0u;
           kf = fmaxf(kf * args.scale_log2, 1e-37f);  // (a factor of 0 would make NaN of -inf)
-          vs = fmaxf(vs, 1e-37f);
+          vs = fmaxf(vs, KV8_SCALE_MIN);
         }
         if (pv != 0) {
           ok = ok && warp_wait(&bars->kv_full[2 * ((t + 1) & 1) + 1], ((t - 1) >> 1) & 1, 7, abort_flag);

@@ -37,6 +37,31 @@ def test_zero_queries_and_keys(cuda, qdt, dtype, s_q, causal):
 
 
 @pytest.mark.parametrize("qdt", [BF16, F16])
+@pytest.mark.parametrize("s_q", [1, 20, 100, 513])
+def test_blocks_with_scales_of_zero(cuda, qdt, s_q):
+    """A block whose scales are 0 (an empty cache's) holds keys and values of
+    0: its tokens take their share of the weights like others."""
+    from minixmax_h3_b200 import ops
+
+    hkv, d = 2, 128
+    g = torch.Generator(device=cuda).manual_seed(s_q)
+    c, table = ops.KV8Cache.empty(3, hkv, d, device=cuda), ints([[0, 2, 1], [1, 0, 0]], cuda)
+    c.k.copy_(torch.randint(-127, 128, c.k.shape, generator=g, device=cuda))
+    c.v.copy_(torch.randint(-127, 128, c.v.shape, generator=g, device=cuda))
+    c.k_scale[2], c.v_scale[2] = 0.01, 3.0
+    lens = [150, 100]
+    q, lse = torch.randn(2, s_q, 4, d, generator=g, device=cuda).to(qdt), torch.empty(2, 4, s_q, device=cuda)
+    o = ops.kv8_attention(q, c, table, ints(lens, cuda), lse=lse)
+    assert torch.allclose(lse[1], torch.full_like(lse[1], math.log(100)), atol=2e-5, rtol=2e-6)
+    assert o[1].float().abs().max() < 1e-25
+    check(o[:1], exact(q, c, table.cpu(), lens, False, 64)[:1], qdt)
+    k = c.k[2].double() * 0.01
+    s = torch.einsum("ihd,hjd->hij", q[0].double(), k.repeat_interleave(2, 0)) * d ** -0.5
+    want = torch.logsumexp(torch.cat([s, torch.zeros(4, s_q, 86, dtype=s.dtype, device=cuda)], -1), -1)
+    assert torch.allclose(lse[0].double(), want, atol=2e-5, rtol=2e-6)
+
+
+@pytest.mark.parametrize("qdt", [BF16, F16])
 @pytest.mark.parametrize("dtype", CODES)
 @pytest.mark.parametrize("s_q,b,hkv", [(1, 110, 4), (130, 1, 4), (513, 1, 4)])
 def test_long_tail_beside_a_dominant_token(cuda, qdt, dtype, s_q, b, hkv):
