@@ -69,6 +69,13 @@ H3B_DEV float ex2(float x) {
   return y;
 }
 
+// The smaller of two, NaN if one is.
+H3B_DEV float min_nan(float a, float b) {
+  float y;
+  asm("min.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(a), "f"(b));
+  return y;
+}
+
 template <bool SPIN = false>
 H3B_DEV bool warp_wait(uint64_t* bar, uint32_t parity, int site, volatile int* abort_flag) {
   const bool ok = mbar_wait<SPIN, false, true>(bar, parity, &g_status, site, abort_flag);
@@ -506,9 +513,9 @@ __global__ void __launch_bounds__(THREADS, 1)
         for (int e = 0; e < 64; e += 2) {
           const float2 t = fma2(make_float2(__uint_as_float(s[e]), __uint_as_float(s[e + 1])),
                                 make_float2(args.scale_log2, args.scale_log2), make_float2(neg_lse2, neg_lse2));
-          // (P <= 1 but for rounding; a left-out key's score of 0 may be far above lse)
-          s[e] = __float_as_uint(ex2(fminf(t.x, 0.0f)));
-          s[e + 1] = __float_as_uint(ex2(fminf(t.y, 0.0f)));
+          // (P <= 1 but for rounding; a left-out key's score of 0 may be far above lse; a NaN stays one)
+          s[e] = __float_as_uint(ex2(min_nan(t.x, 0.0f)));
+          s[e + 1] = __float_as_uint(ex2(min_nan(t.y, 0.0f)));
         }
         if (!warp_wait<true>(&bars->dp_full, step & 1, 22, abort_flag)) {
           ok = false;

@@ -569,7 +569,7 @@ __global__ void __launch_bounds__(WARPS * 32, MT == 1 ? 3 : 2)
       *reinterpret_cast<float4*>(a.part_o + (split * total_rows + row) * D + d) = o;
       if (d == 0) a.part_ml[split * total_rows + row] = make_float2(mx, l);
     } else {
-      const float inv = l > 0.0f ? 1.0f / l : 0.0f;
+      const float inv = l == 0.0f ? 0.0f : 1.0f / l;  // (0: no key; a NaN stays one)
       uint2 w;
       if (a.dtype == H3B_F16) {
         w = make_uint2(pack_f16x2(o.x * inv, o.y * inv), pack_f16x2(o.z * inv, o.w * inv));
@@ -578,7 +578,7 @@ __global__ void __launch_bounds__(WARPS * 32, MT == 1 ? 3 : 2)
       }
       *reinterpret_cast<uint2*>(static_cast<uint16_t*>(a.o) + b * a.o_stride[0] + tok * a.o_stride[1] +
                                 head * a.o_stride[2] + d) = w;
-      if (d == 0 && a.lse != nullptr) a.lse[row] = l > 0.0f ? (mx + __log2f(l)) * LN2 : -INFINITY;
+      if (d == 0 && a.lse != nullptr) a.lse[row] = l == 0.0f ? -INFINITY : (mx + __log2f(l)) * LN2;
     }
   }
 }
@@ -633,7 +633,7 @@ __global__ void __launch_bounds__(128) xattn_combine_kernel(const __grid_constan
       }
     }
   }
-  const float inv = l > 0.0f ? 1.0f / l : 0.0f;
+  const float inv = l == 0.0f ? 0.0f : 1.0f / l;  // (0: no key; a NaN stays one)
   const uint32_t bh = row / static_cast<uint32_t>(a.s_q);
   const int64_t tok = row - bh * a.s_q, b = bh / static_cast<uint32_t>(a.heads);
   const int64_t head = bh - static_cast<uint32_t>(b) * a.heads;
@@ -647,7 +647,7 @@ __global__ void __launch_bounds__(128) xattn_combine_kernel(const __grid_constan
   } else {
     *reinterpret_cast<uint32_t*>(dst) = w[0];
   }
-  if (lane == 0 && a.lse != nullptr) a.lse[row] = l > 0.0f ? (mx + __log2f(l)) * LN2 : -INFINITY;
+  if (lane == 0 && a.lse != nullptr) a.lse[row] = l == 0.0f ? -INFINITY : (mx + __log2f(l)) * LN2;
 }
 
 template <int D, KvKind KIND, bool QF16, int MT>

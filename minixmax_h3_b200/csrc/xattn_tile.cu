@@ -990,7 +990,7 @@ __global__ void __launch_bounds__(THREADS, 1)
         const int q_row = u.q0 + i * BQ + row;
         const bool in = q_row < a.s_q;
         const int64_t lse_row = (static_cast<int64_t>(u.b) * a.heads + u.head) * a.s_q + q_row;
-        const float inv_l = ml.y > 0.0f ? 1.0f / ml.y : 0.0f;
+        const float inv_l = ml.y == 0.0f ? 0.0f : 1.0f / ml.y;  // (0: no key; a NaN stays one)
         // 32 columns at a time in a rolled loop: this code runs once a unit, so
         // it is fetched anew each time (unrolled, a 128-row tile took 4500
         // cycles).  O is given back before its last columns are stored.
@@ -1052,7 +1052,7 @@ __global__ void __launch_bounds__(THREADS, 1)
           if (a.splits > 1) {
             a.part_ml[u.split * total_rows + lse_row] = ml;
           } else if (a.lse != nullptr) {
-            a.lse[lse_row] = ml.y > 0.0f ? (ml.x + __log2f(ml.y)) * LN2 : -INFINITY;
+            a.lse[lse_row] = ml.y == 0.0f ? -INFINITY : (ml.x + __log2f(ml.y)) * LN2;
           }
         }
       }

@@ -178,6 +178,29 @@ def test_long_tail_beside_a_dominant_key(cuda, s_q, dtype):
 # ----------------------------------------------------------------------------- NaN in kept places
 
 
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("s_q,s_kv", [(3, 40), (3, 300), (200, 40), (200, 300)])
+def test_nan_is_not_hidden(cuda, dtype, s_q, s_kv):
+    """A query row with a NaN gives NaN in o, lse and dq, and changes no other
+    row of them; a kept key with one gives NaN everywhere."""
+    q, k, v, do = make(cuda, 1, s_q, s_kv, 2, 2, 64, dtype)
+    want_o, want_lse, want = gradients(q, k, v, do)
+    q[0, 1, 0, 5] = math.nan
+    o, lse, grads = gradients(q, k, v, do)
+    bad = torch.zeros(1, s_q, 2, dtype=torch.bool, device=cuda)
+    bad[0, 1, 0] = True
+    for got, clean in ((o, want_o), (lse.transpose(1, 2)[..., None], want_lse.transpose(1, 2)[..., None])):
+        assert torch.isnan(got[bad]).all() and torch.equal(got[~bad], clean[~bad])
+    assert torch.isnan(grads[0][bad]).all()
+    assert torch.isfinite(grads[0][~bad]).all()
+    assert torch.isnan(grads[1][:, :, 0]).all() and torch.equal(grads[1][:, :, 1], want[1][:, :, 1])
+    q[0, 1, 0, 5] = 1.0
+    k[0, s_kv - 1, 1, 0] = math.nan
+    o, lse, grads = gradients(q, k, v, do)
+    assert torch.isnan(o[:, :, 1]).all() and torch.isnan(lse[:, 1]).all() and torch.isnan(grads[0][:, :, 1]).all()
+    assert torch.isfinite(o[:, :, 0]).all() and torch.isfinite(lse[:, 0]).all()
+
+
 # ----------------------------------------------------------------------------- layouts
 
 

@@ -90,3 +90,20 @@ def test_long_tail_beside_a_dominant_token(cuda, qdt, dtype, s_q, b, hkv):
     # (a running fp32 sum is off by 2^-24 a step at most: a warp may take every fourth tile of 32 keys)
     want = torch.log(top + n - 1)[None, :, None].expand(b, hkv, s_q)
     assert torch.allclose(lse.double().cpu(), want, atol=2e-5 + n / 128 * 2.0 ** -24, rtol=2e-6)
+
+
+@pytest.mark.parametrize("qdt", [BF16, F16])
+def test_nan_query_is_not_hidden(cuda, qdt):
+    from minixmax_h3_b200 import ops
+
+    lens = [90]
+    c, table = filled(cuda, lens, 2, 64, 64, torch.int8)
+    for s_q in (1, 40, 513):
+        q = torch.randn(1, s_q, 4, 64, generator=torch.Generator(device=cuda).manual_seed(0), device=cuda).to(qdt)
+        q[0, s_q - 1, 2, 7] = math.nan
+        lse = torch.empty(1, 4, s_q, device=cuda)
+        o = ops.kv8_attention(q, c, table, ints(lens, cuda), lse=lse)
+        bad = torch.zeros(1, s_q, 4, dtype=torch.bool, device=cuda)
+        bad[0, s_q - 1, 2] = True
+        assert torch.isnan(o[bad]).all() and torch.isfinite(o[~bad]).all()
+        assert torch.equal(torch.isnan(lse.transpose(1, 2)), bad)
