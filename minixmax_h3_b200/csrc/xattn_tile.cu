@@ -756,6 +756,9 @@ __global__ void __launch_bounds__(THREADS, 1)
 #pragma unroll
           for (int c = 0; c < 4; ++c)
             if (((there >> c) & 1u) == 0) w[c] = 0u;
+          // (columns that are all left out: their scales may be anything, and an
+          // infinity would make NaN of -inf)
+          if (((lane & 2) ? (lane & 1) ? w[3] : w[2] : (lane & 1) ? w[1] : w[0]) == 0) kf = vs = 1.0f;
           kf = fmaxf(kf * args.scale_log2, 1e-37f);  // (a factor of 0 would make NaN of -inf)
           vs = fmaxf(vs, KV8_SCALE_MIN);
         }

@@ -107,3 +107,28 @@ def test_nan_query_is_not_hidden(cuda, qdt):
         bad[0, s_q - 1, 2] = True
         assert torch.isnan(o[bad]).all() and torch.isfinite(o[~bad]).all()
         assert torch.equal(torch.isnan(lse.transpose(1, 2)), bad)
+
+
+@pytest.mark.parametrize("bad", [math.inf, math.nan])
+@pytest.mark.parametrize("dtype", CODES)
+@pytest.mark.parametrize("s_q", [1, 130, 513])
+def test_scales_of_left_out_blocks(cuda, dtype, bad, s_q):
+    """Scales of blocks that hold no attended token (absent ones, ones behind
+    the length) may be anything, like their codes."""
+    from minixmax_h3_b200 import ops
+
+    lens, bt = [300, 70], 32
+    c, table = filled(cuda, [320, 96], 2, 64, bt, dtype, max_blocks=12)
+    table[0, 3], table[1, 5] = -1, 10 ** 6
+    used = torch.cat([table[0, :10], table[1, :3]])
+    spare = torch.tensor([i for i in range(c.k.shape[0]) if i not in used.tolist()], device=cuda)
+    assert len(spare) == 1  # block table[0, 3] was
+    table[0, 10:], table[1, 3] = spare[0].int(), spare[0].int()
+    pool = ops.KV8Cache(*(torch.cat([t[spare], t]) for t in (c.k, c.v, c.k_scale, c.v_scale)))  # block 0 is spare too
+    table = torch.where((table >= 0) & (table < 10 ** 6), table + 1, table)
+    for t in (pool.k_scale, pool.v_scale):
+        t[0], t[spare + 1] = bad, bad
+    q = torch.randn(2, s_q, 4, 64, generator=torch.Generator(device=cuda).manual_seed(0), device=cuda).to(BF16)
+    for causal in (False, True):
+        o = ops.kv8_attention(q, pool, table, ints(lens, cuda), causal=causal)
+        check(o, exact(q, pool, table.cpu(), lens, causal, bt), BF16)
