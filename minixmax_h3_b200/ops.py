@@ -416,9 +416,15 @@ def _check_qkv(name: str, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor) -> 
     return b, heads, kv_heads, d, s_q, s_kv
 
 
+def _dense(t: torch.Tensor) -> torch.Tensor:
+    """A copy that _fits (contiguous() keeps a contiguous tensor whose first
+    element is not 16-byte aligned)."""
+    return t.clone(memory_format=torch.contiguous_format)
+
+
 def _kv_in_place(k: torch.Tensor, v: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
     if k.stride() != v.stride() or v.data_ptr() & 15 or not _fits(k):
-        k, v = k.contiguous(), v.contiguous()
+        k, v = _dense(k), _dense(v)
     return k, v
 
 
@@ -491,7 +497,7 @@ def cross_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, kv_len
     _check_lse("cross_attention", lse, q)
     out = _check_out("cross_attention", out, q)
     if not _fits(q):
-        q = q.contiguous()
+        q = _dense(q)
     k, v = _kv_in_place(k, v)
     ws = _workspace("h3b_cross_attention_workspace", q, *sizes)
     call("h3b_cross_attention_fwd", q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), _ptr(lse),
@@ -515,7 +521,7 @@ def cross_attention_bwd(dout: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v:
         raise ValueError("cross_attention_bwd: out and dout have q's shape and type")
     key_mask = _kept_keys("cross_attention_bwd", k, kv_lens, key_mask)
     _check_lse("cross_attention_bwd", lse, q)
-    q, out, dout = (t if _fits(t) else t.contiguous() for t in (q, out, dout))
+    q, out, dout = (t if _fits(t) else _dense(t) for t in (q, out, dout))
     k, v = _kv_in_place(k, v)
     dq, dk, dv = (torch.empty_like(t, memory_format=torch.contiguous_format) for t in (q, k, v))
     ws = _workspace("h3b_cross_attention_bwd_workspace", q, *sizes)
@@ -644,7 +650,7 @@ def kv8_attention(q: torch.Tensor, cache: KV8Cache, block_table: torch.Tensor, l
     _check_lse("kv8_attention", lse, q)
     out = _check_out("kv8_attention", out, q)
     if not _fits(q):
-        q = q.contiguous()
+        q = _dense(q)
     ws = _workspace("h3b_kv8_attention_workspace", q, b, heads, kv_heads, d, s_q, bt, max_blocks)
     call("h3b_kv8_attention", q.data_ptr(), out.data_ptr(), _ptr(lse), _FLOAT16[dtype], b, heads, kv_heads, d, s_q,
          *q.stride()[:3], *out.stride()[:3], cache.k.data_ptr(), cache.v.data_ptr(), cache.k_scale.data_ptr(),

@@ -211,3 +211,26 @@ def shifted(t):
     out.copy_(t)
     assert out.is_contiguous() and out.data_ptr() % 16
     return out
+
+
+@pytest.mark.parametrize("s_q", [3, 150])
+def test_contiguous_tensors_between_16_byte_borders(cuda, s_q):
+    """Layouts that cannot be read in place are copied, a contiguous tensor at
+    an odd address too."""
+    from minixmax_h3_b200 import ops
+
+    q, k, v, do = make(cuda, 2, s_q, 50, 4, 2, 64, BF16)
+    o, lse, grads = gradients(q, k.contiguous(), v.contiguous(), do)
+    got = torch.empty_like(lse)
+    assert torch.equal(ops.cross_attention(shifted(q), shifted(k), shifted(v), lse=got), o) and torch.equal(got, lse)
+    assert torch.equal(ops.cross_attention(q, k.contiguous(), shifted(v)), o)
+    for odd in ((0,), (1, 2), (3,), (4,), (0, 1, 2, 3, 4)):
+        args = [shifted(t) if i in odd else t for i, t in enumerate((do, q, k, v, o))]
+        assert all(torch.equal(a, b) for a, b in zip(ops.cross_attention_bwd(*args, lse), grads)), odd
+    c = ops.KV8Cache.empty(2, 2, 64, device=cuda)
+    c2 = ops.KV8Cache.empty(2, 2, 64, device=cuda)
+    table, lens = (torch.tensor(x, dtype=torch.int32, device=cuda) for x in ([[0], [1]], [0, 0]))
+    ops.kv8_append(c, k, v, table, lens)
+    ops.kv8_append(c2, shifted(k), shifted(v), table, lens)
+    assert torch.equal(c.k, c2.k) and torch.equal(c.v, c2.v) and c.k.any()
+    assert torch.equal(ops.kv8_attention(shifted(q), c, table, lens + 50), ops.kv8_attention(q, c, table, lens + 50))
