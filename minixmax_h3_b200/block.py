@@ -246,7 +246,11 @@ class CrossAttention(nn.Module):
     A prompt's states are the same at every denoising step, so their keys and
     values can be projected once: ``encode`` gives them as tensors for the
     ``kv`` argument, ``fill`` writes them into an 8-bit cache (half the bytes),
-    which ``forward`` then attends through ``cache``."""
+    which ``forward`` then attends through ``cache``.
+
+    The projections are quantised and have no gradients, so the layer has none:
+    an input that requires one raises.  Training uses
+    ``attention.cross_attention`` between projections of its own."""
 
     def __init__(self, hidden, heads, head_dim, cond_dim, kv_heads: Optional[int] = None, dtype=None, device=None,
                  operations=None):
@@ -261,9 +265,15 @@ class CrossAttention(nn.Module):
                                               device=device)
         self.out_proj = operations.QuantLinear(heads * head_dim, hidden, bias=False, dtype=dtype, device=device)
 
+    @staticmethod
+    def _without_gradients(*ts: Optional[torch.Tensor]) -> None:
+        if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in ts):
+            raise RuntimeError("CrossAttention has no gradients: detach its inputs, or use attention.cross_attention")
+
     def encode(self, cond: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
         """cond [B, n, cond_dim] -> k, v [B, n, kv_heads, head_dim], the two
         halves of one projection (read in place by the attention)."""
+        self._without_gradients(cond)
         b, n, _ = cond.shape
         kv = self.kv_proj(cond.reshape(b * n, -1)).view(b, n, 2, self.kv_heads, self.head_dim)
         return kv[:, :, 0], kv[:, :, 1]
@@ -285,6 +295,7 @@ class CrossAttention(nn.Module):
         a sample without any token gets zeros from the attention."""
         if sum(a is not None for a in (cond, kv, cache)) != 1:
             raise ValueError("CrossAttention.forward takes one of cond, kv and cache")
+        self._without_gradients(x, cond, *(kv or ()))
         b, s, _ = x.shape
         q = self.q_proj(x.reshape(b * s, -1)).view(b, s, self.heads, self.head_dim)
         if cache is not None:

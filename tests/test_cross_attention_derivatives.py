@@ -88,3 +88,24 @@ def test_forward_mode_of_the_operator_raises(cpu_operator, which):
         with pytest.raises(NotImplementedError):
             cpu_operator(*args, None, None, None)
         cpu_operator(*qkv(), None, None, None)
+
+
+def test_layer_refuses_what_needs_a_gradient(stub, monkeypatch):
+    """The layer's projections are quantised and have no gradients: inputs
+    that need one raise, and do not come back detached."""
+    from minixmax_h3_b200.block import CrossAttention
+
+    layer = CrossAttention(128, 2, 64, 256)
+    for name in ("q_proj", "kv_proj", "out_proj"):
+        p = getattr(layer, name)
+        monkeypatch.setattr(p, "forward", lambda x, n=p.out_features: x.new_zeros(x.shape[0], n))
+    x, cond = torch.randn(1, 4, 128).to(BF16), torch.randn(1, 5, 256).to(BF16)
+    kv = layer.encode(cond)
+    layer(x, cond), layer(x, kv=kv)
+    need = lambda t: t.detach().clone().requires_grad_()  # noqa: E731
+    for call in (lambda: layer(need(x), cond), lambda: layer(x, need(cond)), lambda: layer.encode(need(cond)),
+                 lambda: layer(x, kv=(kv[0], need(kv[1]))), lambda: layer(need(x), kv=kv)):
+        with pytest.raises(RuntimeError, match="gradient"):
+            call()
+        with torch.no_grad():
+            call()
