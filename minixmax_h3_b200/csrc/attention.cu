@@ -600,13 +600,9 @@ int launch_attention(const void* q, const void* k, const void* v, AttnArgs a, in
     rc = h3b::encode_3d(&tv, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, v, D, s_kv, heads, kv_seq_stride * 2,
                         kv_head_stride * 2, 64, BKV, 1, CU_TENSOR_MAP_SWIZZLE_128B);
   if (rc != H3B_OK) return rc;
-  static bool attr = false;
-  if (!attr) {
-    if (cudaFuncSetAttribute(attention_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                             static_cast<int>(SMEM_BYTES)) != cudaSuccess)
-      return H3B_ERR_LAUNCH;
-    attr = true;
-  }
+  static h3b::OncePerDevice attr;
+  rc = attr.run(h3b::device(), [] { return h3b::allow_smem(attention_kernel, SMEM_BYTES); });
+  if (rc != H3B_OK) return rc;
   a.s_q = static_cast<int>(s_q);
   a.s_kv = static_cast<int>(s_kv);
   a.scale_log2 = scale * 1.4426950408889634f;

@@ -875,11 +875,8 @@ int launch_gemm_t(const void* a, const void* b, int64_t a_row_bytes, int64_t b_r
     ty = ta;  // the int32 and scatter paths never use this map
   }
   const size_t smem = smem_bytes<KIND, PAIR, EM>();
-  static bool attr_set = false;
-  if (!attr_set) {
-    if (cudaFuncSetAttribute(gemm_kernel<KIND, PAIR, EM>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                             static_cast<int>(smem)) != cudaSuccess)
-      return H3B_ERR_LAUNCH;
+  static h3b::OncePerDevice attr;
+  rc = attr.run(h3b::device(), [smem]() -> int {
     if constexpr (C::NVF4_PAIR) {
       // setmaxnreg.inc waits for registers the launch must have provided:
       // refuse to launch a build whose kernel got fewer than the split needs.
@@ -887,8 +884,9 @@ int launch_gemm_t(const void* a, const void* b, int64_t a_row_bytes, int64_t b_r
       if (cudaFuncGetAttributes(&fa, gemm_kernel<KIND, PAIR, EM>) != cudaSuccess || fa.numRegs < PAIR_LAUNCH_REGS)
         return H3B_ERR_LAUNCH;
     }
-    attr_set = true;
-  }
+    return h3b::allow_smem(gemm_kernel<KIND, PAIR, EM>, smem);
+  });
+  if (rc != H3B_OK) return rc;
   const int m_tiles = static_cast<int>((args.m + BM * PAIR - 1) / (BM * PAIR));
   const int n_tiles = static_cast<int>((args.n + C::BN - 1) / C::BN);
   const int tiles = m_tiles * n_tiles;

@@ -8,6 +8,7 @@
 #include <stdint.h>
 
 #include "../../include/h3b.h"
+#include "per_device.hpp"
 
 namespace h3b {
 
@@ -17,6 +18,21 @@ int register_status_reader(StatusReader fn);
 
 // Current device's SM count (cached per device ordinal).
 int num_sms();
+
+// Current device's ordinal.
+inline int device() {
+  int dev = 0;
+  return cudaGetDevice(&dev) == cudaSuccess ? dev : 64;
+}
+
+// Lets a kernel take `bytes` of dynamic shared memory (an attribute of the
+// current device).
+template <class Kernel>
+int allow_smem(Kernel* kernel, size_t bytes) {
+  return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(bytes)) == cudaSuccess
+             ? H3B_OK
+             : H3B_ERR_LAUNCH;
+}
 
 // Encodes a row-major 2D tensor map: `inner` contiguous elements per row,
 // `outer` rows `row_stride_bytes` apart; box = box_inner x box_outer.

@@ -1161,15 +1161,12 @@ int launch(const XAttnGrad& a, cudaStream_t stream) {
   if (rc != H3B_OK) return rc;
   auto dq = xattn_dq_kernel<D, F16>;
   auto dkv = xattn_dkv_kernel<D, F16>;
-  static bool attr = false;
-  if (!attr) {
-    if (cudaFuncSetAttribute(dq, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(dq_smem<D>())) !=
-            cudaSuccess ||
-        cudaFuncSetAttribute(dkv, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(dkv_smem<D>())) !=
-            cudaSuccess)
-      return H3B_ERR_LAUNCH;
-    attr = true;
-  }
+  static h3b::OncePerDevice attr;
+  rc = attr.run(h3b::device(), [=] {
+    const int e = h3b::allow_smem(dq, dq_smem<D>());
+    return e == H3B_OK ? h3b::allow_smem(dkv, dkv_smem<D>()) : e;
+  });
+  if (rc != H3B_OK) return rc;
   GradArgs args{};
   args.a = a;
   args.group = a.heads / a.kv_heads;

@@ -675,13 +675,9 @@ int launch(const XAttn& a, cudaStream_t stream) {
   if (rc != H3B_OK) return rc;
   constexpr size_t smem = 1024 + WARPS * T::RING_BYTES + (WARPS * T::STAGES + 2) * 8 + WARPS * 16 * MT * sizeof(float2);
   auto kernel = xattn_rows_kernel<D, KIND, QF16, MT>;
-  static bool attr = false;
-  if (!attr) {
-    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem)) !=
-        cudaSuccess)
-      return H3B_ERR_LAUNCH;
-    attr = true;
-  }
+  static h3b::OncePerDevice attr;
+  rc = attr.run(h3b::device(), [=] { return h3b::allow_smem(kernel, smem); });
+  if (rc != H3B_OK) return rc;
   RowsArgs args{};
   args.a = a;
   args.group = a.heads / a.kv_heads;

@@ -1152,13 +1152,9 @@ int launch(const XAttn& a, cudaStream_t stream) {
   }
   if (rc != H3B_OK) return rc;
   auto kernel = xattn_tile_kernel<D, F16, KIND, MASKED, PRE>;
-  static bool attr = false;
-  if (!attr) {
-    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem_bytes<D, KIND, PRE>())) !=
-        cudaSuccess)
-      return H3B_ERR_LAUNCH;
-    attr = true;
-  }
+  static h3b::OncePerDevice attr;
+  rc = attr.run(h3b::device(), [=] { return h3b::allow_smem(kernel, smem_bytes<D, KIND, PRE>()); });
+  if (rc != H3B_OK) return rc;
   TileArgs args{};
   args.a = a;
   args.group = a.heads / a.kv_heads;
