@@ -597,7 +597,9 @@ def kv8_append(cache: KV8Cache, k: torch.Tensor, v: torch.Tensor, block_table: t
     lens[b] tokens that each sequence holds (int32 [B], device; not updated
     here).  new_lens (int32 [B]) appends the first new_lens[b] rows of a
     ragged batch.  A block that held tokens keeps the larger of its scale and
-    the new rows' one, and its codes are rounded again if it grew."""
+    the new rows' one, and its codes are rounded again if it grew.  Rows are
+    expected finite: a scale ignores NaN, which int8 stores as code -127 (e4m3
+    has a NaN), and an infinity makes the block's scale infinite."""
     nb, kv_heads, bt, d, b, max_blocks = _check_cache("kv8_append", cache, block_table, lens)
     _cuda(k, v, new_lens)
     dtype, rows = k.dtype, k.shape

@@ -109,6 +109,91 @@ def test_nan_query_is_not_hidden(cuda, qdt):
         assert torch.equal(torch.isnan(lse.transpose(1, 2)), bad)
 
 
+@pytest.mark.parametrize("s_q", [1, 130, 513])
+def test_lengths_beyond_the_table(cuda, s_q):
+    """Lengths beyond the table are cut to it: every row is as with the
+    table's own length, absent blocks among them."""
+    from minixmax_h3_b200 import ops
+
+    lens = [500, 320, 200]
+    c, table = filled(cuda, lens, 2, 128, 64, torch.int8, max_blocks=8)
+    table[0, 1], table[0, 4] = -1, 10 ** 6
+    table[1] = -5
+    q = torch.randn(3, s_q, 4, 128, generator=torch.Generator(device=cuda).manual_seed(0), device=cuda).to(BF16)
+    o = ops.kv8_attention(q, c, table, ints([10 ** 9, 10 ** 9, 200], cuda))
+    check(o, exact(q, c, table.cpu(), [512, 512, 200], False, 64), BF16)
+    assert (o[1] == 0).all()
+    assert torch.equal(o, ops.kv8_attention(q, c, table, ints([512, 512, 200], cuda)))
+
+
+@pytest.mark.parametrize("s_q", [1, 300])
+def test_step_in_a_cuda_graph(cuda, s_q):
+    """Append, attention and read of a step, and a training step, captured
+    once and replayed on other inputs: the same bits as the calls."""
+    from minixmax_h3_b200 import ops
+
+    hkv, d, lens = 2, 128, ints([100, 40], cuda)
+    g = torch.Generator(device=cuda).manual_seed(0)
+
+    def inputs():
+        return [torch.randn(2, s_q, n, d, generator=g, device=cuda).to(F16) for n in (4, hkv, hkv, 4)]
+
+    c0, table = filled(cuda, [100 + s_q, 40 + s_q], hkv, d, 64, torch.int8)
+
+    def step(cache, q, k, v, do):
+        ops.kv8_append(cache, k, v, table, lens)
+        o = ops.kv8_attention(q, cache, table, lens + s_q, causal=True)
+        lse = torch.empty(2, 4, s_q, device=cuda)
+        p = ops.cross_attention(q, k, v, lse=lse)
+        return (o, *ops.kv8_read(cache, table, lens + s_q, 100 + s_q), p, lse,
+                *ops.cross_attention_bwd(do, q, k, v, p, lse))
+
+    def fresh():
+        return ops.KV8Cache(*(t.clone() for t in (c0.k, c0.v, c0.k_scale, c0.v_scale)))
+
+    held, cache = inputs(), fresh()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step(fresh(), *held)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = step(cache, *held)
+    for _ in range(2):
+        new = inputs()
+        for a, b in zip(held, new):
+            a.copy_(b)
+        for a, b in zip((cache.k, cache.v, cache.k_scale, cache.v_scale), (c0.k, c0.v, c0.k_scale, c0.v_scale)):
+            a.copy_(b)
+        graph.replay()
+        for a, b in zip(got, step(fresh(), *new)):
+            assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("s_q", [1, 300])
+def test_other_stream_of_the_cache(cuda, s_q):
+    from minixmax_h3_b200 import ops
+
+    lens = ints([100], cuda)
+    c, table = filled(cuda, [100 + s_q], 2, 64, 64, torch.float8_e4m3fn)
+    g = torch.Generator(device=cuda).manual_seed(0)
+    q, k, v = (torch.randn(1, s_q, n, 64, generator=g, device=cuda).to(BF16) for n in (4, 2, 2))
+
+    def step(cache):
+        ops.kv8_append(cache, k, v, table, lens)
+        return (ops.kv8_attention(q, cache, table, lens + s_q), *ops.kv8_read(cache, table, lens + s_q, 100 + s_q))
+
+    caches = [ops.KV8Cache(*(t.clone() for t in (c.k, c.v, c.k_scale, c.v_scale))) for _ in range(2)]
+    want = step(caches[0])
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        got = step(caches[1])
+    torch.cuda.current_stream().wait_stream(s)
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
 @pytest.mark.parametrize("bad", [math.inf, math.nan])
 @pytest.mark.parametrize("dtype", CODES)
 @pytest.mark.parametrize("s_q", [1, 130, 513])
