@@ -38,7 +38,8 @@
 // What bounds it is the chain softmax -> P V -> S -> softmax of a row tile and
 // its hand-offs, of which two are interleaved: 24 heads of 128, bf16, 16384 x
 // 4096 673 us (1230 TFLOP/s), 32768 x 512 218 us (950; the border counts for
-// a fourth), x 128 102 us (500); of 64, 32768 x 512 185 us.
+// a fourth), x 128 102 us (500); of 64, 32768 x 512 185 us.  These are short
+// runs: under sustained load, at the power limit, 32768 x 512 of 128 takes 246 us.
 #include "h3b_common.cuh"
 #include "h3b_host.hpp"
 #include "xattn.hpp"

@@ -595,7 +595,8 @@ def kv8_append(cache: KV8Cache, k: torch.Tensor, v: torch.Tensor, block_table: t
                new_lens: Optional[torch.Tensor] = None) -> None:
     """Quantises k, v [B, T, Hkv, D] (bf16 or fp16) into the cache behind the
     lens[b] tokens that each sequence holds (int32 [B], device; not updated
-    here).  new_lens (int32 [B]) appends the first new_lens[b] rows of a
+    here); rows behind the table's last block are dropped.  new_lens (int32
+    [B]) appends the first new_lens[b] rows of a
     ragged batch.  A block that held tokens keeps the larger of its scale and
     the new rows' one, and its codes are rounded again if it grew.  Rows are
     expected finite: a scale ignores NaN, which int8 stores as code -127 (e4m3
@@ -640,7 +641,11 @@ def kv8_attention(q: torch.Tensor, cache: KV8Cache, block_table: torch.Tensor, l
     o [B, Sq, H, D].  causal: the queries are the sequence's last Sq tokens
     (already appended), each sees the tokens up to its own.  Tokens of a block
     that the table does not name (an entry outside the pool) are left out.  A
-    row that sees no token gives zeros (lse, fp32 [B, H, Sq] if given: -inf)."""
+    row that sees no token gives zeros (lse, fp32 [B, H, Sq] if given: -inf).
+    Where a key head serves more than one tile of 256 query rows (of 33 tokens
+    or more), the codes are written out as 16-bit numbers first, into a
+    workspace of the table's width and twice the codes' bytes, unless that is
+    more than 8 GB."""
     nb, kv_heads, bt, d, b, max_blocks = _check_cache("kv8_attention", cache, block_table, lens)
     _cuda(q, out, lse)
     dtype, rows = q.dtype, q.shape
