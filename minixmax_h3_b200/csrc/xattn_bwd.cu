@@ -36,9 +36,10 @@
 // f16's smallest numbers, several thousands passed its largest, and left-out
 // keys (dS = -delta P in dq, see warp 10) made infinities, so NaN, of delta
 // above 65504.  (In dk, rows whose |do| is below some 1e-4 of the largest of
-// their key head still lose bits, in sums that the others mostly make.)  The norms cost a pass over do (delta's, where that is
-// taken) and one over v: 2 x 2049 x 1025, 24 heads on 6 of 128, 5 us and a launch
-// (330 -> 341 with the forward); 16384 x 77, 24 heads of 128, 32 us of 226.
+// their key head still lose bits, in sums that the others mostly make.)  The
+// norms cost a pass over do (delta's, where that is taken) and one over v: 2 x
+// 2049 x 1025, 24 heads on 6 of 128, 5 us and a launch (330 -> 341 with the
+// forward); 16384 x 77, 24 heads of 128, 32 us of 226.
 #include "h3b_common.cuh"
 #include "h3b_host.hpp"
 #include "xattn.hpp"
