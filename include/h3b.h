@@ -53,7 +53,7 @@ enum {
 };
 
 /* Element type codes for activation inputs. */
-enum { H3B_BF16 = 0, H3B_F16 = 1, H3B_F32 = 2 /* h3b_kv8_read's output only */ };
+enum { H3B_BF16 = 0, H3B_F16 = 1, H3B_F32 = 2 /* h3b_kv8_read's output, rotary, layer norm */ };
 
 /* Code types of the 8-bit key/value cache. */
 enum { H3B_KV_INT8 = 0, H3B_KV_E4M3 = 1 };
@@ -371,6 +371,65 @@ H3B_API int h3b_kv8_attention(const void* q, void* o, float* lse, int dtype, int
                               int64_t num_blocks, int64_t block_tokens, const int32_t* table, int64_t max_blocks,
                               const int32_t* lens, int causal, float scale, void* workspace,
                               int64_t workspace_bytes, h3b_stream_t stream);
+
+/* -------------------------------------------------------- rotary positions */
+
+/*
+ * Turns the first `rot` channels of every head of q [b, s, heads, d] and k
+ * [b, s, kv_heads, d] by their token's position:
+ *   (x1, x2) -> factor * (x1 cos a - x2 sin a, x2 cos a + x1 sin a)
+ * with a = position * turns[pair] / 2^64 turns (one turn = 2 pi; whole turns
+ * drop out of the 64-bit product, so any position is exact to 2^-33 turns),
+ * pairs (i, i + rot/2), or (2i, 2i + 1) with interleaved != 0.  The other
+ * channels are copied.  inverse != 0 turns by -a (the transpose).  The
+ * product and sum are fp32, rounded once to the type.
+ * dtype H3B_BF16, H3B_F16 or H3B_F32 (inputs and outputs); strides in
+ * elements, the last one 1, nothing else asked of them; d even; rot even, at
+ * most d; heads + kv_heads at most 65535.  k and k_out may be NULL with
+ * kv_heads 0.  An output may be its input (with its strides); it must overlap
+ * nothing else.
+ * positions: int32, or int64 with positions64 != 0; token (i, j)'s position
+ * on axis x at i*pos_batch + j*pos_seq + x*pos_axis.  Pairs below axis0_pairs
+ * use axis 0, the next axis1_pairs axis 1, the rest axis 2; an axis without
+ * pairs is not read.  turns: [rot / 2], device.
+ */
+H3B_API int h3b_rotary(const void* q, const void* k, void* q_out, void* k_out, int dtype, int64_t b, int64_t s,
+                       int64_t heads, int64_t kv_heads, int64_t d, int64_t rot, int interleaved, int64_t q_batch,
+                       int64_t q_seq, int64_t q_head, int64_t k_batch, int64_t k_seq, int64_t k_head,
+                       int64_t qo_batch, int64_t qo_seq, int64_t qo_head, int64_t ko_batch, int64_t ko_seq,
+                       int64_t ko_head, const void* positions, int positions64, int64_t pos_batch, int64_t pos_seq,
+                       int64_t pos_axis, const uint64_t* turns, int64_t axis0_pairs, int64_t axis1_pairs,
+                       float factor, int inverse, h3b_stream_t stream);
+
+/* -------------------------------------------------------------- layer norm */
+
+/*
+ * y[r,:] = (x[r,:] - mean) * rstd * w + b, rstd = 1 / sqrt(var + eps), mean
+ * and var (of n, not n - 1) over the row, fp32, rounded once.  x, y: [m, n]
+ * of dtype (H3B_BF16, H3B_F16 or H3B_F32), rows ldx / ldy apart, unit column
+ * stride; w, b: [n] of wdtype (dtype or H3B_F32), each may be NULL; mean,
+ * rstd: fp32 [m], both or neither.  m below 2^31, n at most 2^30; any
+ * alignment (16-byte words where n, the strides and the pointers allow).
+ */
+H3B_API int h3b_layer_norm_fwd(const void* x, const void* w, const void* b, void* y, float* mean, float* rstd,
+                               int dtype, int wdtype, int64_t m, int64_t n, int64_t ldx, int64_t ldy, float eps,
+                               h3b_stream_t stream);
+
+/* Bytes of h3b_layer_norm_bwd's workspace on the current device. */
+H3B_API int h3b_layer_norm_bwd_workspace(int64_t m, int64_t n, int64_t* bytes);
+
+/*
+ * Gradients of h3b_layer_norm_fwd: with g = dy * w,
+ * dx = rstd * (g - mean(g) - xhat * mean(g * xhat)), dw = sum over rows of
+ * dy * xhat, db = sum over rows of dy (dw, db: [n] of wdtype, each may be
+ * NULL).  Sums are fp32 in a fixed order.  The workspace (16-byte aligned) is
+ * needed only with dw or db; calls that overlap need one each.  m = 0 does
+ * nothing (dw and db are not written).
+ */
+H3B_API int h3b_layer_norm_bwd(const void* dy, const void* x, const void* w, const float* mean, const float* rstd,
+                               void* dx, void* dw, void* db, int dtype, int wdtype, int64_t m, int64_t n,
+                               int64_t lddy, int64_t ldx, int64_t lddx, void* workspace, int64_t workspace_bytes,
+                               h3b_stream_t stream);
 
 /* ------------------------------------------------------- block elementwise */
 

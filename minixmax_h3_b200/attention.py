@@ -9,7 +9,8 @@ inputs raise.  The reference's sequence-parallel entries are here too:
 ``ring_attention_bnsd`` (the K/V ring with log-sum-exp merges).
 
 ``cross_attention`` (no reference counterpart) is the differentiable form of
-``ops.cross_attention``: a batch of query tokens against an encoder's states.
+``ops.cross_attention``: a batch of query tokens against an encoder's states,
+and ``rotary`` that of ``ops.rotary``, their positions.
 """
 from __future__ import annotations
 
@@ -78,12 +79,12 @@ class _CrossAttentionGrad(torch.autograd.Function):
         raise RuntimeError("cross_attention has no second derivatives")
 
 
-def refuse_tangents(*ts: torch.Tensor) -> None:
+def refuse_tangents(*ts: Optional[torch.Tensor], name: str = "cross_attention") -> None:
     """Raises if a tensor carries a forward-mode tangent: the kernels' results
     would come back without one.  (Where reverse mode is recorded too, the
     autograd function raises by itself.)"""
-    if any(forward_ad.unpack_dual(t).tangent is not None for t in ts):
-        raise NotImplementedError("cross_attention has no forward-mode derivatives")
+    if any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in ts):
+        raise NotImplementedError(f"{name} has no forward-mode derivatives")
 
 
 def cross_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, kv_lens: Optional[torch.Tensor] = None,
@@ -97,6 +98,32 @@ def cross_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, kv_len
         return _CrossAttention.apply(q, k, v, kv_lens, key_mask, scale)
     refuse_tangents(q, k, v)
     return ops.cross_attention(q, k, v, kv_lens=kv_lens, key_mask=key_mask, scale=scale)
+
+
+class _Rotary(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, positions, rope, inverse):
+        ctx.save_for_backward(positions)
+        ctx.rope, ctx.inverse = rope, inverse
+        return ops.rotary(q, k, positions, rope, inverse=inverse)
+
+    @staticmethod
+    def backward(ctx, dq, dk):
+        # linear, so its gradient is the other rotation, which has one in turn
+        dq, dk = rotary(dq, dk, ctx.saved_tensors[0], ctx.rope, inverse=not ctx.inverse)
+        return dq, dk, None, None, None
+
+
+def rotary(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Tensor, rope: "ops.Rotary", *,
+           inverse: bool = False) -> tuple[torch.Tensor, Optional[torch.Tensor]]:
+    """ops.rotary (q [B, S, H, D], k [B, S, Hkv, D] or None; see there for
+    positions and rope), differentiable by autograd in q and k, any number of
+    times; nothing but the positions is kept for the backward pass.  There are
+    no forward-mode derivatives: asking for them raises."""
+    if torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad)):
+        return _Rotary.apply(q, k, positions, rope, inverse)
+    refuse_tangents(q, k, name="rotary")
+    return ops.rotary(q, k, positions, rope, inverse=inverse)
 
 
 def _tokens(t: torch.Tensor) -> torch.Tensor:

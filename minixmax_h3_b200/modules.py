@@ -18,6 +18,7 @@ import torch.nn as nn
 import torch.nn.functional as F
 
 from . import ops
+from .attention import refuse_tangents
 from .ops import EPI_STORE, NVFP4Tensor
 from .timing import TIMER
 
@@ -41,6 +42,68 @@ class RMSNorm(nn.Module):
         sel = torch.full((x.numel() // hidden,), -1, dtype=torch.int32, device=x.device)
         out = ops.rmsnorm_modulate(x, self.weight.to(x.device), self._no_mod, self._no_mod, self.eps, row_sel=sel)
         return out.view_as(x)
+
+
+class _LayerNorm(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, bias, eps):
+        stats = torch.empty(2, x.numel() // x.shape[-1], dtype=torch.float32, device=x.device)
+        y = ops.layer_norm(x, weight, bias, eps, stats=stats)
+        ctx.save_for_backward(x, weight, stats)
+        return y
+
+    @staticmethod
+    def backward(ctx, dy):
+        x, weight, stats = ctx.saved_tensors
+        wanted = ctx.needs_input_grad[1:3]
+        if torch.is_grad_enabled():  # create_graph
+            return (*_LayerNormGrad.apply(dy, x, weight, stats, *wanted), None)
+        return (*ops.layer_norm_bwd(dy, x, stats, weight, weight_grad=wanted[0], bias_grad=wanted[1]), None)
+
+
+class _LayerNormGrad(torch.autograd.Function):
+    """The gradients as a node of a graph, so that a second derivative raises
+    where it reaches them (without a node it would silently lack their part)."""
+
+    @staticmethod
+    def forward(ctx, dy, x, weight, stats, weight_grad, bias_grad):
+        return ops.layer_norm_bwd(dy, x, stats, weight, weight_grad=weight_grad, bias_grad=bias_grad)
+
+    @staticmethod
+    def backward(ctx, *grads):
+        raise RuntimeError("layer_norm has no second derivatives")
+
+
+def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Optional[torch.Tensor] = None,
+               eps: float = 1e-5) -> torch.Tensor:
+    """ops.layer_norm (see there), differentiable by autograd in x, weight and
+    bias.  It keeps x, weight and two fp32 numbers a row for the backward pass,
+    which is bit-reproducible.  There are no second derivatives and no
+    forward-mode ones: asking for them raises."""
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, bias)):
+        if x.dim() == 0 or x.shape[-1] == 0:
+            raise ValueError("layer_norm: an axis of at least one element is normalised")
+        return _LayerNorm.apply(x, weight, bias, eps)
+    refuse_tangents(x, weight, bias, name="layer_norm")
+    return ops.layer_norm(x, weight, bias, eps)
+
+
+class LayerNorm(nn.Module):
+    """Layer norm over the last axis, trainable: the norm before a trained
+    layer's projections.  Weight and bias are fp32 unless ``dtype`` says
+    otherwise (they are read in their own type), and absent without
+    ``elementwise_affine`` (the bias without ``bias``)."""
+
+    def __init__(self, dim: int, eps: float = 1e-5, elementwise_affine: bool = True, bias: bool = True,
+                 dtype=None, device=None, **_):
+        super().__init__()
+        self.eps = eps
+        for name, there, value in (("weight", elementwise_affine, 1.0), ("bias", elementwise_affine and bias, 0.0)):
+            p = nn.Parameter(torch.full((dim,), value, dtype=dtype or torch.float32, device=device)) if there else None
+            self.register_parameter(name, p)
+
+    def forward(self, x: torch.Tensor) -> torch.Tensor:
+        return layer_norm(x, self.weight, self.bias, self.eps)
 
 
 class Linear(nn.Module):
@@ -339,4 +402,5 @@ class Ops:
 
     Linear = Linear
     RMSNorm = RMSNorm
+    LayerNorm = LayerNorm
     QuantLinear = QuantLinear

@@ -8,6 +8,7 @@ from __future__ import annotations
 
 import ctypes
 import functools
+import math
 from dataclasses import dataclass
 from typing import Optional, Sequence
 
@@ -664,6 +665,275 @@ def kv8_attention(q: torch.Tensor, cache: KV8Cache, block_table: torch.Tensor, l
          cache.v_scale.data_ptr(), _KV8_CODES[cache.k.dtype], nb, bt, block_table.data_ptr(), max_blocks,
          lens.data_ptr(), 1 if causal else 0, _scale(scale, d), _ptr(ws), 0 if ws is None else ws.numel(), _stream(q))
     return out
+
+
+# ----------------------------------------------------------------------------- rotary positions
+
+_FLOATS = {**_FLOAT16, torch.float32: 2}
+
+
+def _call_on(t: torch.Tensor, name: str, *args) -> None:
+    """call() with t's device current (its streams and kernels belong to it)."""
+    if t.get_device() == torch._C._cuda_getDevice():
+        call(name, *args)
+    else:
+        with torch.cuda.device(t.device):
+            call(name, *args)
+
+
+def _workspace_on(fn: str, t: torch.Tensor, *sizes: int) -> torch.Tensor:
+    """A workspace on t's device (its size may follow the SM count)."""
+    with torch.cuda.device(t.device):
+        return t.new_empty(_workspace_bytes(fn, t.get_device(), *sizes), dtype=torch.uint8)
+
+
+def _one_device(name: str, *ts: Optional[torch.Tensor]) -> None:
+    _cuda(*ts)
+    devices = {t.get_device() for t in ts if t is not None}
+    if len(devices) > 1:
+        raise ValueError(f"{name}: tensors on different devices")
+
+
+# 2^190 / 2 pi: a frequency's product with it keeps 64 bits of a turn and more
+_TURN = 249757942369376157889070878929404173453413734678272424196
+
+
+def _turns(radians: float) -> int:
+    """radians / 2 pi as a multiple of 2^-64, modulo one turn, as an int64."""
+    n, d = radians.as_integer_ratio()  # d is a power of two
+    shift = 190 - 64 + d.bit_length() - 1
+    t = ((n * _TURN + (1 << (shift - 1))) >> shift) & ((1 << 64) - 1)
+    return t - (1 << 64) if t >> 63 else t
+
+
+@dataclass
+class Rotary:
+    """The rotations of ``rotary``: how far a pair of channels turns at each
+    position.  turns [pairs] (int64) holds radians / 2 pi as multiples of
+    2^-64 (modulo one turn), so that angles of far positions are exact;
+    sections are the pairs that each axis of the positions turns, in order;
+    factor multiplies the turned channels.  Pairs are channels (i, i + R/2) of
+    the first R = 2 * pairs of a head, or (2i, 2i + 1) if interleaved."""
+
+    turns: torch.Tensor
+    sections: tuple[int, ...]
+    interleaved: bool = False
+    factor: float = 1.0
+
+    @classmethod
+    def from_frequencies(cls, frequencies: Sequence[float] | torch.Tensor, *, sections: Optional[Sequence[int]] = None,
+                         interleaved: bool = False, factor: float = 1.0, device="cuda") -> "Rotary":
+        """frequencies: radians a position of each pair (64-bit floats are
+        used as they are)."""
+        if isinstance(frequencies, torch.Tensor):
+            frequencies = frequencies.detach().double().cpu().tolist()
+        w = [float(f) for f in frequencies]
+        if not all(math.isfinite(f) for f in w) or not math.isfinite(factor):
+            raise ValueError("Rotary: frequencies and factor are finite")
+        sections = (len(w),) if sections is None else tuple(int(n) for n in sections)
+        if not 1 <= len(sections) <= 3 or min(sections) < 0 or sum(sections) != len(w):
+            raise ValueError(f"Rotary: sections {sections} of {len(w)} pairs (one to three axes)")
+        return cls(torch.tensor([_turns(f) for f in w], dtype=torch.int64, device=device), sections, bool(interleaved), float(factor))
+
+    @classmethod
+    def build(cls, dims: int | Sequence[int], *, theta: float = 10000.0, interleaved: bool = False,
+              scaling: Optional[str] = None, scale: float = 1.0, trained_len: int = 0, fast: float = 32.0,
+              slow: float = 1.0, factor: Optional[float] = None, device="cuda") -> "Rotary":
+        """dims: the turned channels of a head (even), or those of each axis
+        of the positions (up to three).  Pair i of an axis with d channels
+        turns by theta^(-2i/d) radians a position, and for contexts ``scale``
+        times longer than trained:
+
+        * "linear": every frequency divided by scale;
+        * "base": theta multiplied by scale^(d/(d-2)), which leaves the fastest
+          pair as it is and divides the slowest one by scale;
+        * "by_parts": pairs that make at least ``fast`` turns over trained_len
+          positions stay, those of at most ``slow`` are divided by scale, those
+          between by a share linear in the turns; the turned channels are
+          multiplied by factor, 0.1 ln(scale) + 1 if None.
+
+        Without a factor the others leave the channels' size as it is."""
+        dims = (dims,) if isinstance(dims, int) else tuple(dims)
+        if any(d < 0 or d & 1 for d in dims) or not dims:
+            raise ValueError(f"Rotary: turned channels {dims} are even numbers")
+        if scaling not in (None, "linear", "base", "by_parts"):
+            raise ValueError(f"Rotary: scaling {scaling!r}")
+        if not (theta > 0 and scale > 0 and math.isfinite(theta) and math.isfinite(scale)):
+            raise ValueError("Rotary: theta and scale are positive and finite")
+        if scaling == "by_parts" and not (trained_len > 0 and fast > slow):
+            raise ValueError("Rotary: by_parts needs trained_len and fast > slow")
+        if factor is None:
+            factor = 0.1 * math.log(scale) + 1 if scaling == "by_parts" and scale > 1 else 1.0
+        w = []
+        for d in dims:
+            base = theta * scale ** (d / (d - 2)) if scaling == "base" and d > 2 else theta
+            for i in range(d // 2):
+                f = base ** (-2 * i / d)
+                if scaling == "linear":
+                    f /= scale
+                elif scaling == "by_parts":
+                    turns = trained_len * f / (2 * math.pi)
+                    keep = min(1.0, max(0.0, (turns - slow) / (fast - slow)))
+                    f = f / scale * (1 - keep) + f * keep
+                w.append(f)
+        return cls.from_frequencies(w, sections=[d // 2 for d in dims], interleaved=interleaved, factor=factor,
+                                    device=device)
+
+
+def _check_heads(name: str, x: torch.Tensor, like: torch.Tensor) -> None:
+    if x.dtype not in _FLOATS or x.dtype != like.dtype:
+        raise TypeError(f"{name} expects q and k of one type, bf16, fp16 or fp32")
+    if x.dim() != 4 or x.shape[:2] != like.shape[:2] or x.shape[3] != like.shape[3]:
+        raise ValueError(f"{name} expects q [B, S, H, D] and k [B, S, Hkv, D]")
+
+
+def _rotary_out(out: Optional[torch.Tensor], x: torch.Tensor) -> torch.Tensor:
+    if out is None:
+        return torch.empty_like(x, memory_format=torch.contiguous_format)
+    if out.shape != x.shape or out.dtype != x.dtype or (out.shape[3] > 1 and out.stride(3) != 1):
+        raise ValueError("rotary: an output has its input's shape and type and unit last stride")
+    return out
+
+
+def rotary(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Tensor, rope: Rotary, *,
+           inverse: bool = False, q_out: Optional[torch.Tensor] = None,
+           k_out: Optional[torch.Tensor] = None) -> tuple[torch.Tensor, Optional[torch.Tensor]]:
+    """q [B, S, H, D] and k [B, S, Hkv, D] (bf16, fp16 or fp32; k may be None)
+    with the channels that ``rope`` pairs turned by the tokens' positions, the
+    others as they are: (q, k), new tensors or q_out / k_out, which may be the
+    inputs themselves and else overlap nothing.
+
+    positions: int32 or int64, any value, [S] or [B, S] (any strides), with a
+    last axis of one position per section where rope has several.  inverse
+    turns the other way: with the same factor this is the transpose, which
+    takes the gradients of the results to those of q and k
+    (``attention.rotary`` does so under autograd).  Strided inputs are read in
+    place (unit last stride; other layouts are copied).  Angles are exact to
+    2^-33 of a turn at any position, results are rounded once."""
+    _one_device("rotary", q, k, positions, rope.turns, q_out, k_out)
+    _check_heads("rotary", q, q)
+    if k is not None:
+        _check_heads("rotary", k, q)
+    b, s, heads, d = q.shape
+    pairs = rope.turns.numel()
+    if 2 * pairs > d or d & 1:
+        raise ValueError(f"rotary: {2 * pairs} turned channels of a head of {d} (an even number)")
+    axes = len(rope.sections)
+    if positions.dtype not in (torch.int32, torch.int64):
+        raise TypeError("rotary: positions are int32 or int64")
+    if positions.shape not in ((s,), (b, s)) if axes == 1 else positions.shape not in ((s, axes), (b, s, axes)):
+        raise ValueError(f"rotary: positions [S] or [B, S]{f', each with {axes} axes' if axes > 1 else ''}")
+    p = positions.stride()
+    if axes == 1:
+        p = (*p, 0)
+    if len(p) == 2:
+        p = (0, *p)
+    q_out = _rotary_out(q_out, q)
+    if q.shape[3] > 1 and q.stride(3) != 1:
+        q = q.contiguous()
+    if k is not None:
+        k_out = _rotary_out(k_out, k)
+        if k.shape[3] > 1 and k.stride(3) != 1:
+            k = k.contiguous()
+    turns = rope.turns if rope.turns.is_contiguous() else rope.turns.contiguous()
+    sections = (*rope.sections, 0)
+    no_k = (0, 0, 0)
+    _call_on(q, "h3b_rotary", q.data_ptr(), _ptr(k), q_out.data_ptr(), None if k is None else k_out.data_ptr(),
+             _FLOATS[q.dtype], b, s, heads, 0 if k is None else k.shape[2], d, 2 * pairs, 1 if rope.interleaved else 0,
+             *q.stride()[:3], *(no_k if k is None else k.stride()[:3]), *q_out.stride()[:3],
+             *(no_k if k is None else k_out.stride()[:3]), positions.data_ptr(),
+             1 if positions.dtype == torch.int64 else 0, *p, turns.data_ptr(), sections[0], sections[1],
+             rope.factor, 1 if inverse else 0, _stream(q))
+    return q_out, None if k is None else k_out
+
+
+# ----------------------------------------------------------------------------- layer norm
+
+
+def _check_norm(name: str, x: torch.Tensor, weight: Optional[torch.Tensor], bias: Optional[torch.Tensor]) -> int:
+    """Checks types and shapes; returns the code of the weights' type."""
+    if x.dtype not in _FLOATS:
+        raise TypeError(f"{name} expects bf16, fp16 or fp32 input")
+    if x.dim() == 0 or x.shape[-1] == 0:
+        raise ValueError(f"{name}: an axis of at least one element is normalised")
+    if bias is not None and (weight is None or bias.dtype != weight.dtype):
+        raise ValueError(f"{name}: a bias comes with a weight of its type")
+    for w in (weight, bias):
+        if w is not None and (w.shape != x.shape[-1:] or w.dtype not in (x.dtype, torch.float32)):
+            raise ValueError(f"{name}: weight and bias are [{x.shape[-1]}] tensors of x's type or fp32")
+    return _FLOATS[x.dtype if weight is None else weight.dtype]
+
+
+def _check_stats(name: str, stats: Optional[torch.Tensor], m: int) -> None:
+    if stats is not None and (stats.dtype != torch.float32 or stats.shape != (2, m) or not stats.is_contiguous()):
+        raise ValueError(f"{name}: stats is a contiguous fp32 [2, rows] tensor")
+
+
+def _packed(w: Optional[torch.Tensor]) -> Optional[torch.Tensor]:
+    return w if w is None or w.is_contiguous() else w.contiguous()
+
+
+def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Optional[torch.Tensor] = None,
+               eps: float = 1e-5, *, out: Optional[torch.Tensor] = None,
+               stats: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """(x - mean) / sqrt(var + eps) * weight + bias over the last axis of x
+    (bf16, fp16 or fp32; weight and bias of x's type or fp32): x's shape and
+    type, contiguous, or ``out`` (contiguous).  stats, if given (fp32
+    [2, rows]), receives each row's mean and 1 / sqrt(var + eps), which
+    layer_norm_bwd needs.  Rows with a unit last stride and one row stride are
+    read in place, other layouts copied first.  A row that holds NaN or an
+    infinity gives NaN.  For gradients by autograd see ``modules.layer_norm``."""
+    _one_device("layer_norm", x, weight, bias, out, stats)
+    wdtype = _check_norm("layer_norm", x, weight, bias)
+    if not 0.0 <= eps < float("inf"):
+        raise ValueError("layer_norm: eps is not negative and finite")
+    if out is None:
+        out = torch.empty_like(x, memory_format=torch.contiguous_format)
+    elif out.shape != x.shape or out.dtype != x.dtype or not out.is_contiguous():
+        raise ValueError("layer_norm: out is a contiguous tensor of x's shape and type")
+    n = x.shape[-1]
+    m = x.numel() // n
+    _check_stats("layer_norm", stats, m)
+    if m == 0:
+        return out
+    x2, _, _, ld = _rows(x)
+    weight, bias = _packed(weight), _packed(bias)
+    at = None if stats is None else stats.data_ptr()
+    _call_on(x, "h3b_layer_norm_fwd", x2.data_ptr(), _ptr(weight), _ptr(bias), out.data_ptr(), at,
+             None if at is None else at + 4 * m, _FLOATS[x.dtype], wdtype, m, n, ld, n, float(eps), _stream(x))
+    return out
+
+
+def layer_norm_bwd(dout: torch.Tensor, x: torch.Tensor, stats: torch.Tensor, weight: Optional[torch.Tensor] = None, *,
+                   weight_grad: bool = True, bias_grad: bool = True
+                   ) -> tuple[torch.Tensor, Optional[torch.Tensor], Optional[torch.Tensor]]:
+    """Gradients (dx, dweight, dbias) of layer_norm for the gradient dout of
+    its result; x, stats and weight as the forward call had them.  dweight and
+    dbias have the weight's type, and are None without a weight or where they
+    are not asked for.  Sums are fp32 in a fixed order (bit-reproducible)."""
+    _one_device("layer_norm_bwd", dout, x, stats, weight)
+    wdtype = _check_norm("layer_norm_bwd", x, weight, None)
+    if dout.shape != x.shape or dout.dtype != x.dtype:
+        raise ValueError("layer_norm_bwd: dout has x's shape and type")
+    n = x.shape[-1]
+    m = x.numel() // n
+    _check_stats("layer_norm_bwd", stats, m)
+    dx = torch.empty_like(x, memory_format=torch.contiguous_format)
+    new = torch.zeros if m == 0 else torch.empty
+    dw, db = (new(n, dtype=weight.dtype, device=x.device) if weight is not None and wanted else None
+              for wanted in (weight_grad, bias_grad))
+    if m == 0:
+        return dx, dw, db
+    x2, _, _, ldx = _rows(x)
+    dout2, _, _, lddy = _rows(dout)
+    weight = _packed(weight)
+    ws = None
+    if dw is not None or db is not None:
+        ws = _workspace_on("h3b_layer_norm_bwd_workspace", x, m, n)
+    _call_on(x, "h3b_layer_norm_bwd", dout2.data_ptr(), x2.data_ptr(), _ptr(weight), stats.data_ptr(),
+             stats.data_ptr() + 4 * m, dx.data_ptr(), _ptr(dw), _ptr(db), _FLOATS[x.dtype], wdtype, m, n, lddy, ldx, n,
+             _ptr(ws), 0 if ws is None else ws.numel(), _stream(x))
+    return dx, dw, db
 
 
 # ----------------------------------------------------------------------------- block elementwise
