@@ -431,6 +431,26 @@ H3B_API int h3b_layer_norm_bwd(const void* dy, const void* x, const void* w, con
                                int64_t lddy, int64_t ldx, int64_t lddx, void* workspace, int64_t workspace_bytes,
                                h3b_stream_t stream);
 
+/* --------------------------------------------------- orthogonalised updates */
+
+/* Bytes of h3b_orthogonalize's workspace. */
+H3B_API int h3b_orthogonalize_workspace(int64_t batch, int64_t m, int64_t n, int64_t* bytes);
+
+/*
+ * Newton-Schulz steps toward the orthogonal factor of `batch` matrices x
+ * [m, n] (rows ld apart, matrices batch_stride, unit column stride): from
+ * X = x / (|x| + eps), Frobenius norm, `steps` times
+ * X <- a X + (b G + c G G) X, G = X X^T (for m > n the same on X^T).  out:
+ * [batch, m, n] contiguous, may be x where that is contiguous.  dtype
+ * H3B_BF16, H3B_F16 or H3B_F32 for both.  Products of f16 planes in pairs,
+ * fp32 sums; elements of the iterates must stay below 64.  m, n at most
+ * 65536, batch at most 65535, batch * max(m, n) at most 2^29, steps at most
+ * 1000.  The workspace is 16-byte aligned; calls that overlap need one each.
+ */
+H3B_API int h3b_orthogonalize(const void* x, void* out, int dtype, int64_t batch, int64_t m, int64_t n,
+                              int64_t batch_stride, int64_t ld, int64_t steps, float a, float b, float c, float eps,
+                              void* workspace, int64_t workspace_bytes, h3b_stream_t stream);
+
 /* ------------------------------------------------------- block elementwise */
 
 /*

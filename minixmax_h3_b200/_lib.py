@@ -64,6 +64,8 @@ SIGNATURES: dict[str, list] = {
     "h3b_layer_norm_fwd": [c_ptr] * 6 + [c_int, c_int] + [c_i64] * 4 + [c_f32, c_ptr],
     "h3b_layer_norm_bwd_workspace": [c_i64, c_i64, c_ptr],
     "h3b_layer_norm_bwd": [c_ptr] * 8 + [c_int, c_int] + [c_i64] * 5 + [c_ptr, c_i64, c_ptr],
+    "h3b_orthogonalize_workspace": [c_i64] * 3 + [c_ptr],
+    "h3b_orthogonalize": [c_ptr, c_ptr, c_int] + [c_i64] * 6 + [c_f32] * 4 + [c_ptr, c_i64, c_ptr],
     "h3b_selftest_wait_timeout": [c_ptr] * 7 + [c_i64] * 3 + [c_ptr],
     "h3b_attention_merge_lse": [c_ptr, c_ptr, c_ptr, c_ptr, c_i64, c_i64, c_int, c_ptr, c_ptr, c_ptr],
 }
@@ -114,7 +116,7 @@ def lib() -> ctypes.CDLL:
 # Entry points that launch no kernel of this library.
 _NO_LAUNCH = {"h3b_version", "h3b_device_status", "h3b_cross_attention_workspace",
               "h3b_cross_attention_bwd_workspace", "h3b_kv8_attention_workspace",
-              "h3b_layer_norm_bwd_workspace"}
+              "h3b_layer_norm_bwd_workspace", "h3b_orthogonalize_workspace"}
 LAUNCHES = [0]  # kernels this process has launched through the ABI
 
 
