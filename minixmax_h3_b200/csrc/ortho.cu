@@ -4,10 +4,15 @@
 // given back so).
 //
 // A step is three matrix products on tcgen05 (kind::f16, fp32 accumulators in
-// TMEM), each with its arithmetic in the epilogue:
-//   GRAM  G = X X^T            symmetric: only tiles on or below the diagonal,
-//   POLY  B = b G + c G G      stored to both sides
-//   MUL   X' = a X + B X       (X is read K-major by GRAM, N-major by MUL)
+// TMEM), arranged so that none has a second matrix to add where it stores.
+// Results in 16 bits complete the polynomial's square:
+//   GRAM  H = X X^T + (b / 2c) 1         symmetric: only tiles on or below the
+//   POLY  B = c H H + (a - b^2 / 4c) 1   diagonal, stored to both sides
+//   MUL   X' = B X    (X is read K-major by GRAM, N-major by MUL)
+// Results in 32 bits, whose first steps the constants would cost a bit or two
+// (G is small there), and coefficients with |b / 2c| above 4 take a second
+// factor instead, K = c G + b 1, for B = G K + a 1 (at 4096 GRAM takes 180 us
+// with it and 156 without).
 //
 // Precision.  A step multiplies small singular values by a, five steps by
 // 480: what a rounding spills from the large directions into the small ones
@@ -18,11 +23,13 @@
 // is 2^-22).  That is as near as 32-bit arithmetic comes at a fifth of its
 // time on CUDA cores.  Two products are exact or late enough to save on:
 // x in 16 bits is one plane as it is (its 8 or 11 bits are kept by a scale of
-// a power of two; the norm's fraction goes into the first epilogues), and the
-// last step of a bf16 result, after which nothing grows, takes one plane.
-// That step is written about G = 1, where X is by then: with H = G - 1,
-// X' = (a + b + c) X + ((b + 2c) H + c H H) X, so that what is rounded to 11
-// bits is small beside what it is added to.
+// a power of two; the norm's fraction goes into the first epilogues).  And of
+// a bf16 result, after whose last step nothing grows, that step takes one
+// plane, and the one before it makes H and B of one: X is near an orthogonal
+// factor by then, H near -0.2 and B near 1 (with K, both steps are written
+// about H = G - 1), so that what is rounded to 11 bits is no larger than what
+// it makes.  That leaves 0.0004 to 0.001 of the root mean square beside the
+// result's own rounding of 0.0017.
 //
 // Planes hold SCALE * value: f16 has its full precision between 2^-24 and 64
 // of the value then.  Elements are below the largest singular value, 1.2 for
@@ -41,8 +48,13 @@
 // CTA (its operand reads and copies share the shared-memory port: a tile
 // costs 0.8 of the pair's time for half the work).  Warp 0 loads (TMA, zero
 // beyond the matrix), warp 1 issues the products, eight warps add and store;
-// two accumulators in turn, so that products go on meanwhile.  Every wait is
-// bounded.
+// two accumulators in turn, so that products go on meanwhile.  Stores go
+// through shared memory as TMA blocks of 32 x 32 (lanes that stored their
+// rows' 16-byte pieces themselves took 20 us a tile, a third of a product's
+// time at 4096), the other side's from registers.  Every wait is bounded.
+//
+// A launch's setup overlaps the end of the one before it (programmatic
+// dependent launch); every kernel waits for it before it touches memory.
 #include "h3b_common.cuh"
 #include "h3b_host.hpp"
 
@@ -55,6 +67,8 @@ constexpr float SCALE = 1024.0f;
 constexpr int BM = 128;            // accumulator rows of a CTA
 constexpr int KB = 64;             // elements of K a stage (128 bytes a row)
 constexpr int PLANE_BYTES = BM * 128;
+constexpr int BLOCK_BYTES = 32 * 64;  // a block on its way out: 32 rows of 64 bytes
+constexpr int BLOCKS = 2;             // of each storing warp
 constexpr int EPI_WARPS = 8;
 constexpr int THREADS = 128 + 32 * EPI_WARPS;  // a warpgroup to load and issue (two of its warps idle), two to store
 
@@ -87,15 +101,13 @@ struct Args {
   int rows, cols, k;       // of the product, per matrix
   int batch;
   int b_lo;                // SPLIT: the B operand has a second plane
-  Planes add;              // POLY: G, MUL: X (rows x cols, row stride add_ld), lo may be null
-  int64_t add_ld, add_batch;
-  Planes out;              // rows x cols planes; lo may be null (nothing reads it)
-  int64_t out_ld, out_batch;
+  int out_lo;              // second planes are stored (something reads them)
+  int with_k;              // GRAM: K is stored beside G
   const float* factor;     // [batch], x's scale: value = factor * plane (the first step), or null
-  float alpha, beta;       // result = alpha * add + beta * product
-  float diagonal;          // GRAM: added to the planes' diagonal
+  float beta, diagonal;    // beta * product + diagonal * 1
+  float k_beta, k_diagonal;  // GRAM's K: of the former
   void* result;            // MUL's last: the caller's matrix instead of planes
-  int result_dtype, result_t, result_wide;  // transposed; rows in 16-byte words
+  int result_dtype, result_t, result_tma;  // transposed; out_hi is its map
   int64_t result_batch, result_ld;
 };
 
@@ -113,7 +125,7 @@ struct __align__(8) Barriers {
 template <int PAIR, int OP, int SPLIT>
 constexpr size_t smem_bytes() {
   using C = Cfg<PAIR, OP, SPLIT>;
-  return 1024 + static_cast<size_t>(C::STAGES) * C::STAGE_BYTES + sizeof(Barriers);
+  return 1024 + static_cast<size_t>(C::STAGES) * C::STAGE_BYTES + EPI_WARPS * BLOCKS * BLOCK_BYTES + sizeof(Barriers);
 }
 
 template <bool SPIN = false, bool CLUSTER = false>
@@ -161,70 +173,116 @@ H3B_DEV Tile tile_at(int t, int per_matrix, int col_tiles) {
   return r;
 }
 
-H3B_DEV void unpack8(const uint4& w, float* v) {
-  const uint32_t u[4] = {w.x, w.y, w.z, w.w};
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&u[i]));
-    v[2 * i] = f.x;
-    v[2 * i + 1] = f.y;
-  }
+H3B_DEV void tma_store_3d(const CUtensorMap* map, const void* smem_src, int32_t x, int32_t y, int32_t z) {
+  asm volatile("cp.async.bulk.tensor.3d.global.shared::cta.tile.bulk_group [%0, {%1, %2, %3}], [%4];" ::"l"(
+                   reinterpret_cast<uint64_t>(map)),
+               "r"(x), "r"(y), "r"(z), "r"(smem_u32(smem_src))
+               : "memory");
 }
 
-template <class T>
-H3B_DEV T from_f32(float v);
-template <>
-H3B_DEV float from_f32<float>(float v) { return v; }
-template <>
-H3B_DEV __half from_f32<__half>(float v) { return __float2half_rn(v); }
-template <>
-H3B_DEV __nv_bfloat16 from_f32<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
+// A storing warp's blocks.  Lane l holds row y0 + l, columns x0 .. x0 + 31 (16
+// bits) or x0 .. x0 + 15 (32 bits); `turned` stores the block transposed.
+struct Blocks {
+  uint8_t* smem;
+  int lane, at;
 
-// Sixteen columns of a row of the caller's matrix.
-template <class T>
-H3B_DEV void store_row(const Args& args, int batch, int row, int col0, const float (&v)[16]) {
-  T* base = static_cast<T*>(args.result) + batch * args.result_batch;
-  constexpr int N = 16 / sizeof(T);
-  if (args.result_t) {  // consecutive lanes, consecutive columns
-#pragma unroll
-    for (int j = 0; j < 16; ++j)
-      if (col0 + j < args.cols) base[(col0 + j) * args.result_ld + row] = from_f32<T>(v[j]);
-    return;
+  // 16-byte piece c of row r in the 64-byte swizzle
+  H3B_DEV static uint32_t swz(int r, int c) { return static_cast<uint32_t>(r * 64 + ((c ^ ((r >> 1) & 3)) << 4)); }
+  H3B_DEV uint8_t* next() {
+    uint8_t* p = smem + (at++ % BLOCKS) * BLOCK_BYTES;
+    if (lane == 0) bulk_wait_group_read<BLOCKS - 1>();  // the store from here has read it
+    __syncwarp();
+    return p;
   }
-  T* dst = base + row * args.result_ld + col0;
-  if (args.result_wide && col0 + 16 <= args.cols) {
-#pragma unroll
-    for (int j = 0; j < 16; j += N) {
-      T w[N];
-#pragma unroll
-      for (int e = 0; e < N; ++e) w[e] = from_f32<T>(v[j + e]);
-      *reinterpret_cast<uint4*>(dst + j) = *reinterpret_cast<const uint4*>(w);
+  H3B_DEV void send(const CUtensorMap* map, const uint8_t* p, int x, int y, int z) {
+    fence_proxy_async_smem();
+    __syncwarp();
+    if (lane == 0) {
+      tma_store_3d(map, p, x, y, z);
+      bulk_commit_group();
     }
-    return;
   }
+  // w: 32 columns of 16 bits
+  H3B_DEV void put(const CUtensorMap* map, const uint32_t (&w)[16], bool turned, int x0, int y0, int z) {
+    uint8_t* p = next();
+    if (!turned) {
 #pragma unroll
-  for (int j = 0; j < 16; ++j)
-    if (col0 + j < args.cols) dst[j] = from_f32<T>(v[j]);
+      for (int c = 0; c < 4; ++c)
+        *reinterpret_cast<uint4*>(p + swz(lane, c)) = make_uint4(w[4 * c], w[4 * c + 1], w[4 * c + 2], w[4 * c + 3]);
+      send(map, p, x0, y0, z);
+      return;
+    }
+    // A pair of lanes trades halves: the even one takes the even column of
+    // both rows, the odd one the odd column; a row of the block is a column.
+    const uint32_t pick = lane & 1 ? 0x3276 : 0x5410;
+#pragma unroll
+    for (int j = 0; j < 16; ++j) {
+      const uint32_t other = __shfl_xor_sync(0xffffffffu, w[j], 1);
+      *reinterpret_cast<uint32_t*>(p + swz(2 * j + (lane & 1), lane >> 3) + ((lane >> 1) & 3) * 4) =
+          __byte_perm(w[j], other, pick);
+    }
+    send(map, p, y0, x0, z);
+  }
+  // v: 32 columns of 32 bits, as two blocks of 16 (columns, or, turned, lanes)
+  H3B_DEV void put(const CUtensorMap* map, const float (&v)[32], bool turned, int x0, int y0, int z) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      uint8_t* p = next();
+      if (!turned) {
+#pragma unroll
+        for (int c = 0; c < 4; ++c)
+          *reinterpret_cast<float4*>(p + swz(lane, c)) =
+              make_float4(v[16 * h + 4 * c], v[16 * h + 4 * c + 1], v[16 * h + 4 * c + 2], v[16 * h + 4 * c + 3]);
+        send(map, p, x0 + 16 * h, y0, z);
+      } else {
+        if ((lane >> 4) == h) {
+#pragma unroll
+          for (int j = 0; j < 32; ++j)
+            *reinterpret_cast<float*>(p + swz(j, (lane & 15) >> 2) + (lane & 3) * 4) = v[j];
+        }
+        send(map, p, y0 + 16 * h, x0, z);
+      }
+    }
+  }
+};
+
+// 32 columns of a row of the caller's matrix, element by element (rows that
+// are no multiple of 16 bytes).
+H3B_DEV void store_elements(const Args& args, int batch, int row, int col0, const float (&v)[32]) {
+  const int64_t base = batch * args.result_batch + (args.result_t ? col0 * args.result_ld + row : row * args.result_ld + col0);
+  const int64_t step = args.result_t ? args.result_ld : 1;
+#pragma unroll
+  for (int j = 0; j < 32; ++j) {
+    if (col0 + j < args.cols) {
+      const int64_t at = base + j * step;
+      if (args.result_dtype == H3B_F32)
+        static_cast<float*>(args.result)[at] = v[j];
+      else if (args.result_dtype == H3B_F16)
+        static_cast<__half*>(args.result)[at] = __float2half_rn(v[j]);
+      else
+        static_cast<__nv_bfloat16*>(args.result)[at] = __float2bfloat16_rn(v[j]);
+    }
+  }
 }
-H3B_DEV void store_result(const Args& args, int batch, int row, int col0, const float (&v)[16]) {
-  if (args.result_dtype == H3B_F32)
-    store_row<float>(args, batch, row, col0, v);
-  else if (args.result_dtype == H3B_F16)
-    store_row<__half>(args, batch, row, col0, v);
-  else
-    store_row<__nv_bfloat16>(args, batch, row, col0, v);
-}
+
+// Lets the next launch set itself up; waits for the one before to end.
+H3B_DEV void launch_next() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+H3B_DEV void wait_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 
 template <int PAIR, int OP, int SPLIT>
 __global__ void __launch_bounds__(THREADS, 1)
     ortho_product(const __grid_constant__ CUtensorMap a_hi, const __grid_constant__ CUtensorMap a_lo,
-                  const __grid_constant__ CUtensorMap b_hi, const __grid_constant__ CUtensorMap b_lo, const Args args) {
+                  const __grid_constant__ CUtensorMap b_hi, const __grid_constant__ CUtensorMap b_lo,
+                  const __grid_constant__ CUtensorMap out_hi, const __grid_constant__ CUtensorMap out_lo,
+                  const __grid_constant__ CUtensorMap k_hi, const __grid_constant__ CUtensorMap k_lo,
+                  const Args args) {
   using C = Cfg<PAIR, OP, SPLIT>;
   constexpr int STAGES = C::STAGES, BN = C::BN;
   constexpr bool SYMMETRIC = OP != MUL;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  Barriers* bars = reinterpret_cast<Barriers*>(smem + STAGES * C::STAGE_BYTES);
+  uint8_t* blocks = smem + STAGES * C::STAGE_BYTES;
+  Barriers* bars = reinterpret_cast<Barriers*>(blocks + EPI_WARPS * BLOCKS * BLOCK_BYTES);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t rank = PAIR == 2 ? cluster_ctarank() : 0u;
   const bool leader = rank == 0;
@@ -250,6 +308,7 @@ __global__ void __launch_bounds__(THREADS, 1)
     fence_barrier_init();
     prefetch_tmap(&a_hi);
     prefetch_tmap(&b_hi);
+    prefetch_tmap(&out_hi);
   }
   if (warp == 1) {
     if constexpr (PAIR == 2) {
@@ -267,6 +326,8 @@ __global__ void __launch_bounds__(THREADS, 1)
     __syncthreads();
   tc_fence_after();
   const uint32_t tmem_base = bars->tmem_base;
+  launch_next();
+  wait_previous();
 
   if (warp < 4) {
    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(REGS_CTL));
@@ -404,6 +465,7 @@ __global__ void __launch_bounds__(THREADS, 1)
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(REGS_EPI));
     const int quad = warp & 3, half = (warp - 4) >> 2;  // TMEM lane quadrant; alternate 32-column chunks
     constexpr int MINE = BN / 64;                         // this warp's chunks of 32 columns
+    Blocks out{blocks + (warp - 4) * BLOCKS * BLOCK_BYTES, lane, 0};
     int local = 0;
     bool ok = true;
     for (int t = cluster; t < num_tiles && ok; t += n_clusters) {
@@ -438,76 +500,74 @@ __global__ void __launch_bounds__(THREADS, 1)
       }
       if (!ok) break;
       const Tile tile = tile_at<SYMMETRIC>(t, per_matrix, col_tiles);
-      const int row = tile.i * BN + static_cast<int>(rank) * BM + quad * 32 + lane;
-      const bool row_ok = row < args.rows;
+      const int row0 = tile.i * BN + static_cast<int>(rank) * BM + quad * 32, row = row0 + lane;
+      if (row0 >= args.rows) continue;  // warp-uniform, as all that follows
       const float f = args.factor != nullptr ? args.factor[tile.batch] : 1.0f;
       const float beta = (OP == GRAM ? f * f : OP == MUL ? f : 1.0f) * args.beta;
-      const float alpha = (OP == MUL ? f : 1.0f) * args.alpha;
-      const int64_t add_at = tile.batch * args.add_batch + row * args.add_ld;
-      const int64_t out_at = tile.batch * args.out_batch;
-      if (row_ok) {
-        // Sixteen columns at a time.  Rows of the planes are multiples of 32
-        // elements apart, so whole pieces are read and written; what lies
-        // behind the last column is never used.
 #pragma unroll
-        for (int i = 0; i < 2 * MINE; ++i) {
-          const int col0 = tile.j * BN + (half + 2 * (i >> 1)) * 32 + (i & 1) * 16;
-          if (col0 >= args.cols) continue;
-          float v[16];
+      for (int i = 0; i < MINE; ++i) {
+        const int col0 = tile.j * BN + (half + 2 * i) * 32;
+        if (col0 >= args.cols) continue;
+        float v[32];
 #pragma unroll
-          for (int j = 0; j < 16; ++j) v[j] = acc[i][j] * beta;
-          if (OP == GRAM && tile.i == tile.j) {
+        for (int j = 0; j < 32; ++j) v[j] = acc[2 * i + (j >> 4)][j & 15] * beta;
+        if (SYMMETRIC && tile.i == tile.j) {
+#pragma unroll
+          for (int j = 0; j < 32; ++j)
+            if (col0 + j == row) v[j] += args.diagonal;
+        }
+        __syncwarp();
+        uint32_t w[16];
+        if (OP == MUL && args.result != nullptr) {
+          if (!args.result_tma) {
+            if (row < args.rows) store_elements(args, tile.batch, row, col0, v);
+            __syncwarp();
+          } else if (args.result_dtype == H3B_F32) {
+            out.put(&out_hi, v, args.result_t, col0, row0, tile.batch);
+          } else {
 #pragma unroll
             for (int j = 0; j < 16; ++j)
-              if (col0 + j == row) v[j] += args.diagonal;
+              w[j] = args.result_dtype == H3B_F16 ? pack_f16x2(v[2 * j], v[2 * j + 1]) : pack_bf16x2(v[2 * j], v[2 * j + 1]);
+            out.put(&out_hi, w, args.result_t, col0, row0, tile.batch);
           }
-          if (OP != GRAM) {
+          continue;
+        }
+        const bool mirror = SYMMETRIC && tile.i != tile.j;
 #pragma unroll
-            for (int j = 0; j < 16; j += 8) {
-              float h[8];
-              unpack8(*reinterpret_cast<const uint4*>(args.add.hi + add_at + col0 + j), h);
+        for (int m = 0; m < (OP == GRAM ? 2 : 1); ++m) {
+          if (m == 1 && !args.with_k) break;
+          const CUtensorMap *hi = m == 0 ? &out_hi : &k_hi, *lo = m == 0 ? &out_lo : &k_lo;
+          if (m == 1) {  // K, from the sums once more (fewer registers than keeping G)
 #pragma unroll
-              for (int e = 0; e < 8; ++e) v[j + e] = fmaf(alpha, h[e], v[j + e]);
-              if (args.add.lo != nullptr) {
-                unpack8(*reinterpret_cast<const uint4*>(args.add.lo + add_at + col0 + j), h);
+            for (int j = 0; j < 32; ++j) v[j] = acc[2 * i + (j >> 4)][j & 15] * beta;
+            if (!mirror) {
 #pragma unroll
-                for (int e = 0; e < 8; ++e) v[j + e] = fmaf(alpha, h[e], v[j + e]);
-              }
+              for (int j = 0; j < 32; ++j)
+                if (col0 + j == row) v[j] += args.diagonal;
             }
-          }
-          if (OP == MUL && args.result != nullptr) {
-            store_result(args, tile.batch, row, col0, v);
-            continue;
-          }
-          uint32_t hi[8], lo[8];
 #pragma unroll
-          for (int j = 0; j < 8; ++j) {
-            hi[j] = pack_f16x2(v[2 * j], v[2 * j + 1]);
-            const float2 h = __half22float2(*reinterpret_cast<const __half2*>(&hi[j]));
-            lo[j] = pack_f16x2(v[2 * j] - h.x, v[2 * j + 1] - h.y);
+            for (int j = 0; j < 32; ++j) v[j] = v[j] * args.k_beta + (col0 + j == row ? args.k_diagonal : 0.0f);
           }
 #pragma unroll
-          for (int p = 0; p < 2; ++p) {
-            __half* plane = p == 0 ? args.out.hi : args.out.lo;
-            if (plane == nullptr) continue;
-            const uint32_t* w = p == 0 ? hi : lo;
-            uint4* dst = reinterpret_cast<uint4*>(plane + out_at + row * args.out_ld + col0);
-            dst[0] = make_uint4(w[0], w[1], w[2], w[3]);
-            dst[1] = make_uint4(w[4], w[5], w[6], w[7]);
-            if (SYMMETRIC && tile.i != tile.j) {  // the other side: consecutive lanes, consecutive columns
-              __half* mirror = plane + out_at + col0 * args.out_ld + row;
+          for (int j = 0; j < 16; ++j) {
+            w[j] = pack_f16x2(v[2 * j], v[2 * j + 1]);
+            const float2 h = __half22float2(*reinterpret_cast<const __half2*>(&w[j]));
+            v[2 * j] -= h.x;
+            v[2 * j + 1] -= h.y;
+          }
+          out.put(hi, w, false, col0, row0, tile.batch);
+          if (mirror) out.put(hi, w, true, col0, row0, tile.batch);
+          if (args.out_lo) {
 #pragma unroll
-              for (int j = 0; j < 16; ++j) {
-                if (col0 + j < args.cols)
-                  *mirror = __ushort_as_half(static_cast<unsigned short>(w[j >> 1] >> (16 * (j & 1))));
-                mirror += args.out_ld;
-              }
-            }
+            for (int j = 0; j < 16; ++j) w[j] = pack_f16x2(v[2 * j], v[2 * j + 1]);
+            out.put(lo, w, false, col0, row0, tile.batch);
+            if (mirror) out.put(lo, w, true, col0, row0, tile.batch);
           }
         }
       }
-      __syncwarp();  // before the next tile's TMEM loads
     }
+    if (lane == 0) bulk_wait_group<0>();  // the blocks are in place before the CTA leaves
+    __syncwarp();
   }
 
   tc_fence_before();
@@ -530,109 +590,185 @@ H3B_DEV float to_f32(float v) { return v; }
 H3B_DEV float to_f32(__half v) { return __half2float(v); }
 H3B_DEV float to_f32(__nv_bfloat16 v) { return __bfloat162float(v); }
 
-constexpr int MAX_PARTS = 256;
+constexpr int MAX_PARTS = 256;  // of a matrix's sum of squares; the threads of a CTA
 
-// Sums of squares in 64 bits (a 32-bit square of a gradient of 10^-20 is
-// nothing); part p of matrix b: rows p, p + parts, ...
+// Eight elements, from 16-byte words where `wide`; those at and behind `n` are 0.
 template <class T>
-__global__ void __launch_bounds__(256) ortho_squares(const T* x, int64_t batch_stride, int64_t ld, int m, int n,
-                                                     double* parts) {
-  const T* base = x + blockIdx.y * batch_stride;
-  double s = 0.0;
-  for (int r = blockIdx.x; r < m; r += gridDim.x) {
-    const T* row = base + r * ld;
-    for (int c = threadIdx.x; c < n; c += 256) {
-      const double v = to_f32(row[c]);
-      s = fma(v, v, s);
-    }
+H3B_DEV void load8(const T* p, int n, bool wide, float (&v)[8]) {
+  if (wide) {  // n is a multiple of 8 then
+    T e[8];
+#pragma unroll
+    for (int i = 0; i < static_cast<int>(sizeof(T)) / 2; ++i)
+      reinterpret_cast<uint4*>(e)[i] = reinterpret_cast<const uint4*>(p)[i];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = to_f32(e[i]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = i < n ? to_f32(p[i]) : 0.0f;
   }
-  __shared__ double warp_sums[8];
+}
+
+// CTA-wide sum of 256 threads' values, in a fixed order.
+H3B_DEV double block_sum(double s) {
+  __shared__ double sums[8];
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-  if ((threadIdx.x & 31) == 0) warp_sums[threadIdx.x >> 5] = s;
+  if ((threadIdx.x & 31) == 0) sums[threadIdx.x >> 5] = s;
   __syncthreads();
-  if (threadIdx.x == 0) {
-    for (int i = 1; i < 8; ++i) s += warp_sums[i];
-    parts[blockIdx.y * gridDim.x + blockIdx.x] = s;
+  s = 0.0;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) s += sums[i];
+  return s;
+}
+
+struct Input {
+  const void* x;
+  int64_t batch_stride, ld;
+  int m, n;
+  int wide;       // rows in 16-byte words
+  double* parts;  // [batch][n_parts]
+  int n_parts;
+};
+
+// Sums of squares, in 64 bits: a 32-bit square of a gradient of 10^-20 is
+// nothing.
+template <class T>
+__global__ void __launch_bounds__(MAX_PARTS) ortho_squares(const Input in) {
+  launch_next();
+  const T* base = static_cast<const T*>(in.x) + blockIdx.y * in.batch_stride;
+  const unsigned vectors = (in.n + 7) / 8;
+  const int64_t items = static_cast<int64_t>(vectors) * in.m, step = static_cast<int64_t>(gridDim.x) * MAX_PARTS;
+  double s = 0.0;
+#pragma unroll 4
+  for (int64_t i = static_cast<int64_t>(blockIdx.x) * MAX_PARTS + threadIdx.x; i < items; i += step) {
+    const unsigned r = static_cast<unsigned>(i / vectors), c = static_cast<unsigned>(i - r * static_cast<int64_t>(vectors)) * 8;
+    float v[8];
+    load8(base + r * in.ld + c, in.n - static_cast<int>(c), in.wide, v);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) s = fma(static_cast<double>(v[e]), static_cast<double>(v[e]), s);
   }
+  s = block_sum(s);
+  if (threadIdx.x == 0) in.parts[blockIdx.y * gridDim.x + blockIdx.x] = s;
 }
 
 // Planes of SCALE * x / 2^e, 2^e <= |x| < 2^(e+1), and the factor
-// 2^e / (|x| + eps) that is left; 32 x 32 elements a CTA, transposed if asked.
+// 2^e / (|x| + eps) that is left.
+struct Output {
+  float eps;
+  float* factor;
+  __half *hi, *lo;  // lo null: one plane holds x
+  int64_t batch, ld;
+};
+
+struct Scales {
+  float s1, s2;  // x * s1 * s2
+};
 template <class T>
-__global__ void __launch_bounds__(256) ortho_planes(const T* x, int64_t batch_stride, int64_t ld, int m, int n,
-                                                    int transposed, const double* parts, int n_parts, float eps,
-                                                    float* factor, __half* hi, __half* lo, int64_t out_batch,
-                                                    int64_t out_ld) {
-  __shared__ float tile[32][33];
-  __shared__ double total;
-  const int b = blockIdx.z;
-  if (threadIdx.x == 0) {
-    double s = 0.0;
-    for (int i = 0; i < n_parts; ++i) s += parts[b * n_parts + i];
-    total = s;
-  }
-  __syncthreads();
+H3B_DEV Scales scales(const Input& in, const Output& out, bool first) {
+  const double total = block_sum(threadIdx.x < static_cast<unsigned>(in.n_parts)
+                                     ? in.parts[blockIdx.z * in.n_parts + threadIdx.x] : 0.0);
   const double norm = sqrt(total);
   const int e = norm > 0.0 && norm < 1e300 ? ilogb(norm) : 0;
-  const int up = 10 - e;  // 2^10 = SCALE
-  const float s1 = ldexpf(1.0f, up / 2), s2 = ldexpf(1.0f, up - up / 2);
-  if (blockIdx.x == 0 && blockIdx.y == 0 && threadIdx.x == 0)
-    factor[b] = static_cast<float>(scalbn(1.0, e) / (norm + static_cast<double>(eps)));
-  const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
-  const int r0 = blockIdx.y * 32, c0 = blockIdx.x * 32;
-  const T* base = x + b * batch_stride;
-  auto put = [&](int r, int c, float v) {
-    const int64_t at = b * out_batch + r * out_ld + c;
-    const __half h = __float2half_rn(v);
-    hi[at] = h;
-    if (lo != nullptr) lo[at] = __float2half_rn(v - __half2float(h));
-  };
+  const int up = 10 - e;  // 2^10 = SCALE; two factors, as one would leave the range of 32 bits
+  if (first && threadIdx.x == 0)
+    out.factor[blockIdx.z] = static_cast<float>(scalbn(1.0, e) / (norm + static_cast<double>(out.eps)));
+  return {ldexpf(1.0f, up / 2), ldexpf(1.0f, up - up / 2)};
+}
+
+template <class T>
+__global__ void __launch_bounds__(MAX_PARTS) ortho_planes(const Input in, const Output out) {
+  launch_next();
+  wait_previous();
+  const Scales k = scales<T>(in, out, blockIdx.x == 0);
+  const T* base = static_cast<const T*>(in.x) + blockIdx.z * in.batch_stride;
+  const unsigned vectors = (in.n + 7) / 8;
+  const int64_t items = static_cast<int64_t>(vectors) * in.m, step = static_cast<int64_t>(gridDim.x) * MAX_PARTS;
+#pragma unroll 2
+  for (int64_t i = static_cast<int64_t>(blockIdx.x) * MAX_PARTS + threadIdx.x; i < items; i += step) {
+    const unsigned r = static_cast<unsigned>(i / vectors), c = static_cast<unsigned>(i - r * static_cast<int64_t>(vectors)) * 8;
+    float v[8];
+    load8(base + r * in.ld + c, in.n - static_cast<int>(c), in.wide, v);
+    uint32_t hi[4], lo[4];
 #pragma unroll
-  for (int i = 0; i < 32; i += 8) {
-    const int r = r0 + ty + i, c = c0 + tx;
-    if (r < m && c < n) {
-      const float v = to_f32(base[r * ld + c]) * s1 * s2;
-      if (transposed)
-        tile[ty + i][tx] = v;
-      else
-        put(r, c, v);
+    for (int e = 0; e < 4; ++e) {
+      const float x = v[2 * e] * k.s1 * k.s2, y = v[2 * e + 1] * k.s1 * k.s2;
+      hi[e] = pack_f16x2(x, y);
+      const float2 h = __half22float2(*reinterpret_cast<const __half2*>(&hi[e]));
+      lo[e] = pack_f16x2(x - h.x, y - h.y);
     }
-  }
-  if (!transposed) return;
-  __syncthreads();
-#pragma unroll
-  for (int i = 0; i < 32; i += 8) {
-    const int r = c0 + ty + i, c = r0 + tx;
-    if (r < n && c < m) put(r, c, tile[tx][ty + i]);
+    // the planes' rows are multiples of 32 elements apart
+    const int64_t at = blockIdx.z * out.batch + r * out.ld + c;
+    *reinterpret_cast<uint4*>(out.hi + at) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+    if (out.lo != nullptr) *reinterpret_cast<uint4*>(out.lo + at) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
   }
 }
 
+// The same of x transposed, 64 x 64 elements a CTA.
+template <class T>
+__global__ void __launch_bounds__(MAX_PARTS) ortho_planes_t(const Input in, const Output out) {
+  __shared__ float tile[64][65];
+  launch_next();
+  wait_previous();
+  const Scales k = scales<T>(in, out, blockIdx.x == 0 && blockIdx.y == 0);
+  const T* base = static_cast<const T*>(in.x) + blockIdx.z * in.batch_stride;
+  const int r0 = blockIdx.y * 64, c0 = blockIdx.x * 64, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+#pragma unroll
+  for (int i = warp; i < 64; i += 8)
+#pragma unroll
+    for (int h = 0; h < 64; h += 32) {
+      const int r = r0 + i, c = c0 + h + lane;
+      tile[i][h + lane] = r < in.m && c < in.n ? to_f32(base[r * in.ld + c]) * k.s1 * k.s2 : 0.0f;
+    }
+  __syncthreads();
+#pragma unroll
+  for (int i = warp; i < 64; i += 8) {
+    const int r = c0 + i, c = r0 + 2 * lane;  // of the transposed
+    if (r < in.n && c < in.m) {  // a pair may reach into the padding of the plane's row
+      const float x = tile[2 * lane][i], y = tile[2 * lane + 1][i];
+      const uint32_t hi = pack_f16x2(x, y);
+      const int64_t at = blockIdx.z * out.batch + r * out.ld + c;
+      *reinterpret_cast<uint32_t*>(out.hi + at) = hi;
+      const float2 h = __half22float2(*reinterpret_cast<const __half2*>(&hi));
+      if (out.lo != nullptr) *reinterpret_cast<uint32_t*>(out.lo + at) = pack_f16x2(x - h.x, y - h.y);
+    }
+  }
+}
+
+template <class T>
+H3B_DEV T from_f32(float v);
+template <>
+H3B_DEV float from_f32<float>(float v) { return v; }
+template <>
+H3B_DEV __half from_f32<__half>(float v) { return __float2half_rn(v); }
+template <>
+H3B_DEV __nv_bfloat16 from_f32<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
+
 // No steps: x / (|x| + eps).
 template <class T>
-__global__ void __launch_bounds__(256) ortho_scale(const T* x, int64_t batch_stride, int64_t ld, int m, int n,
-                                                   const double* parts, int n_parts, float eps, T* out) {
-  double s = 0.0;
-  for (int i = 0; i < n_parts; ++i) s += parts[blockIdx.y * n_parts + i];
-  const double inv = 1.0 / (sqrt(s) + static_cast<double>(eps));
-  for (int r = blockIdx.x; r < m; r += gridDim.x)
-    for (int c = threadIdx.x; c < n; c += 256)
-      out[(static_cast<int64_t>(blockIdx.y) * m + r) * n + c] =
-          static_cast<T>(static_cast<float>(to_f32(x[blockIdx.y * batch_stride + r * ld + c]) * inv));
+__global__ void __launch_bounds__(MAX_PARTS) ortho_scale(const Input in, float eps, T* out) {
+  wait_previous();
+  const double norm = sqrt(block_sum(threadIdx.x < static_cast<unsigned>(in.n_parts)
+                                         ? in.parts[blockIdx.z * in.n_parts + threadIdx.x] : 0.0));
+  const double inv = 1.0 / (norm + static_cast<double>(eps));
+  const T* base = static_cast<const T*>(in.x) + blockIdx.z * in.batch_stride;
+  for (int r = blockIdx.x; r < in.m; r += gridDim.x)
+    for (int c = threadIdx.x; c < in.n; c += MAX_PARTS)
+      out[(static_cast<int64_t>(blockIdx.z) * in.m + r) * in.n + c] =
+          from_f32<T>(static_cast<float>(to_f32(base[r * in.ld + c]) * inv));
 }
 
 // ---------------------------------------------------------------- hosts
 
 struct Layout {
   int64_t small, large;      // sides of X
-  int64_t x_ld, g_ld;        // row strides of the planes of X and of G, B
+  int64_t x_ld, g_ld;        // row strides of the planes of X and of G, K, B
   int64_t x_plane, g_plane;  // elements of a plane, all matrices
   int64_t bytes;
 };
 
 int64_t up(int64_t v, int64_t to) { return (v + to - 1) / to * to; }
 
-// Planes of X (two, in turn), G and B, two each; sums of squares; factors.
+// Planes of X (two, in turn), G, K and B, two each; sums of squares; factors.
 Layout layout(int64_t batch, int64_t m, int64_t n) {
   Layout l;
   l.small = m < n ? m : n;
@@ -641,7 +777,7 @@ Layout layout(int64_t batch, int64_t m, int64_t n) {
   l.g_ld = up(l.small, 32);
   l.x_plane = up(batch * l.small * l.x_ld, 128);
   l.g_plane = up(batch * l.small * l.g_ld, 128);
-  l.bytes = (4 * l.x_plane + 4 * l.g_plane) * 2 + batch * (MAX_PARTS * 8) + up(batch * 4, 256);
+  l.bytes = (4 * l.x_plane + 6 * l.g_plane) * 2 + batch * (MAX_PARTS * 8) + up(batch * 4, 256);
   return l;
 }
 
@@ -655,21 +791,23 @@ struct Maps {
   CUtensorMap hi, lo;
 };
 
-// rows x cols planes for tiles of 128 rows by 64 columns, or (by_rows) for
-// boxes of 64 columns by 64 rows.
-int encode(Maps* maps, const Planes& p, int64_t batch, int64_t rows, int64_t cols, int64_t ld, bool boxes) {
-  const uint32_t high = boxes ? 64 : 128;
+// Boxes of a map of planes: an operand whose rows are K (128 rows by 64
+// elements of K), one whose columns are K (64 rows of K by 64), stores.
+enum Boxes { BY_ROWS, BY_COLUMNS, STORES };
+
+int encode(Maps* maps, const Planes& p, int64_t batch, int64_t rows, int64_t cols, int64_t ld, Boxes boxes) {
+  const uint32_t high = boxes == BY_ROWS ? 128 : boxes == BY_COLUMNS ? 64 : 32;
   for (int i = 0; i < 2; ++i) {
-    const __half* base = i == 0 || p.lo == nullptr ? p.hi : p.lo;
-    const int rc = h3b::encode_3d(i == 0 ? &maps->hi : &maps->lo, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, base, cols, rows,
-                                  batch, ld * 2, rows * ld * 2, 64, high, 1, CU_TENSOR_MAP_SWIZZLE_128B);
+    const int rc = h3b::encode_3d(i == 0 ? &maps->hi : &maps->lo, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, i == 0 ? p.hi : p.lo,
+                                  cols, rows, batch, ld * 2, rows * ld * 2, boxes == STORES ? 32 : 64, high, 1,
+                                  boxes == STORES ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B);
     if (rc != H3B_OK) return rc;
   }
   return H3B_OK;
 }
 
 template <int PAIR, int OP, int SPLIT>
-int launch(const Maps& a, const Maps& b, const Args& args, int64_t tiles, cudaStream_t stream) {
+int launch(const Maps& a, const Maps& b, const Maps& out, const Maps& k, const Args& args, int64_t tiles, cudaStream_t stream) {
   constexpr size_t smem = smem_bytes<PAIR, OP, SPLIT>();
   static_assert(smem <= 227 * 1024, "shared memory budget");
   static h3b::OncePerDevice once;
@@ -687,13 +825,15 @@ int launch(const Maps& a, const Maps& b, const Args& args, int64_t tiles, cudaSt
   cfg.blockDim = dim3(THREADS);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = stream;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = PAIR;
-  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = PAIR;
+  attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
   cfg.attrs = attr;
-  cfg.numAttrs = PAIR == 2 ? 1 : 0;
-  return cudaLaunchKernelEx(&cfg, kernel, a.hi, a.lo, b.hi, b.lo, args) == cudaSuccess ? H3B_OK : H3B_ERR_LAUNCH;
+  cfg.numAttrs = PAIR == 2 ? 2 : 1;
+  return cudaLaunchKernelEx(&cfg, kernel, a.hi, a.lo, b.hi, b.lo, out.hi, out.lo, k.hi, k.lo, args) == cudaSuccess ? H3B_OK : H3B_ERR_LAUNCH;
 }
 
 // Tiles of side `t`, all matrices.
@@ -703,18 +843,34 @@ int64_t tiles_of(int64_t rows, int64_t cols, int64_t batch, int64_t t, bool symm
 }
 
 template <int OP, int SPLIT>
-int product(const Maps& a, const Maps& b, const Args& args, cudaStream_t stream) {
+int product(const Maps& a, const Maps& b, const Maps& out, const Maps& k, const Args& args, cudaStream_t stream) {
   const int64_t sms = h3b::num_sms();
   const int64_t t1 = tiles_of(args.rows, args.cols, args.batch, 128, OP != MUL);
   const int64_t t2 = tiles_of(args.rows, args.cols, args.batch, 256, OP != MUL);
   // Rounds of tiles, a 128 x 128 tile counted 0.8 of a pair's 256 x 256 one.
   const int64_t single = (t1 + sms - 1) / sms * 4, pair = (t2 + sms / 2 - 1) / (sms / 2) * 5;
-  return single <= pair ? launch<1, OP, SPLIT>(a, b, args, t1, stream) : launch<2, OP, SPLIT>(a, b, args, t2, stream);
+  return single <= pair ? launch<1, OP, SPLIT>(a, b, out, k, args, t1, stream)
+                        : launch<2, OP, SPLIT>(a, b, out, k, args, t2, stream);
 }
 
 template <int OP>
-int product(bool split, const Maps& a, const Maps& b, const Args& args, cudaStream_t stream) {
-  return split ? product<OP, 1>(a, b, args, stream) : product<OP, 0>(a, b, args, stream);
+int product(bool split, const Maps& a, const Maps& b, const Maps& out, const Maps& k, const Args& args, cudaStream_t stream) {
+  return split ? product<OP, 1>(a, b, out, k, args, stream) : product<OP, 0>(a, b, out, k, args, stream);
+}
+
+// A small kernel that starts while the one before it ends.
+template <class... Params, class... Values>
+int launch_after(void (*kernel)(Params...), dim3 grid, cudaStream_t stream, Values... values) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(MAX_PARTS);
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kernel, values...) == cudaSuccess ? H3B_OK : H3B_ERR_LAUNCH;
 }
 
 template <class T>
@@ -728,88 +884,105 @@ int run(const T* x, T* out, int dtype, int64_t batch, int64_t m, int64_t n, int6
     return p;
   };
   Planes xs[2] = {take(l.x_plane), take(l.x_plane)};
-  const Planes g = take(l.g_plane), b = take(l.g_plane);
+  const Planes g = take(l.g_plane), k = take(l.g_plane), b = take(l.g_plane);
   double* parts = reinterpret_cast<double*>(at);
   float* factor = reinterpret_cast<float*>(parts + batch * MAX_PARTS);
-  const int n_parts = static_cast<int>(m < MAX_PARTS ? m : MAX_PARTS);
-  const int mi = static_cast<int>(m), ni = static_cast<int>(n);
-  ortho_squares<T><<<dim3(n_parts, static_cast<unsigned>(batch)), 256, 0, stream>>>(x, batch_stride, ld, mi, ni, parts);
-  if (steps == 0) {
-    ortho_scale<T><<<dim3(n_parts, static_cast<unsigned>(batch)), 256, 0, stream>>>(x, batch_stride, ld, mi, ni, parts,
-                                                                                 n_parts, eps, out);
-    return h3b::launch_status();
-  }
+  const int64_t row_bytes = n * static_cast<int64_t>(sizeof(T));
+  const bool wide = n % 8 == 0 && h3b::aligned16(x) && ld * static_cast<int64_t>(sizeof(T)) % 16 == 0 &&
+                    (batch == 1 || batch_stride * static_cast<int64_t>(sizeof(T)) % 16 == 0);
+  // 2048 elements a CTA at least, and CTAs for two an SM together
+  const int64_t pieces = ((n + 7) / 8 * m + MAX_PARTS - 1) / MAX_PARTS;
+  const int64_t share = (2 * h3b::num_sms() + batch - 1) / batch;
+  const int64_t most = pieces < share ? pieces : share;
+  const int n_parts = static_cast<int>(most < MAX_PARTS ? most : MAX_PARTS);
+  const unsigned nb = static_cast<unsigned>(batch);
+  const Input in{x, batch_stride, ld, static_cast<int>(m), static_cast<int>(n), wide ? 1 : 0, parts, n_parts};
+  ortho_squares<T><<<dim3(n_parts, nb), MAX_PARTS, 0, stream>>>(in);
+  if (steps == 0) return launch_after(ortho_scale<T>, dim3(n_parts, 1, nb), stream, in, eps, out);
   const bool tall = m > n;
   const bool exact = dtype != H3B_F32;  // one plane holds x
-  const dim3 grid(static_cast<unsigned>((n + 31) / 32), static_cast<unsigned>((m + 31) / 32), static_cast<unsigned>(batch));
-  ortho_planes<T><<<grid, 256, 0, stream>>>(x, batch_stride, ld, mi, ni, tall ? 1 : 0, parts, n_parts, eps, factor,
-                                            xs[0].hi, exact ? nullptr : xs[0].lo, l.small * l.x_ld, l.x_ld);
-  int rc = h3b::launch_status();
+  const Output planes{eps, factor, xs[0].hi, exact ? nullptr : xs[0].lo, l.small * l.x_ld, l.x_ld};
+  int rc = tall ? launch_after(ortho_planes_t<T>, dim3(static_cast<unsigned>((n + 63) / 64), static_cast<unsigned>((m + 63) / 64), nb),
+                               stream, in, planes)
+                : launch_after(ortho_planes<T>, dim3(static_cast<unsigned>(pieces < 4 * share ? pieces : 4 * share), 1, nb), stream,
+                               in, planes);
   if (rc != H3B_OK) return rc;
 
-  Maps x_k[2], x_n[2], gm, bm;  // X by rows (K-major) and by boxes (N-major)
-  for (int i = 0; i < 2 && rc == H3B_OK; ++i) {
-    rc = encode(&x_k[i], xs[i], batch, l.small, l.large, l.x_ld, false);
-    if (rc == H3B_OK) rc = encode(&x_n[i], xs[i], batch, l.small, l.large, l.x_ld, true);
+  // X by rows and by columns, both sets of planes; G, K and B by rows; all as stores
+  Maps x_k[2], x_n[2], x_out[2], g_k, g_out, k_k, k_out, b_k, b_out, result;
+  const auto enc = [&](Maps* maps, const Planes& p, int64_t cols, int64_t pitch, Boxes boxes) {
+    if (rc == H3B_OK) rc = encode(maps, p, batch, l.small, cols, pitch, boxes);
+  };
+  for (int i = 0; i < (steps > 1 ? 2 : 1); ++i) {
+    enc(&x_k[i], xs[i], l.large, l.x_ld, BY_ROWS);
+    enc(&x_n[i], xs[i], l.large, l.x_ld, BY_COLUMNS);
+    if (steps > 1) enc(&x_out[i], xs[i], l.large, l.x_ld, STORES);
   }
-  if (rc == H3B_OK) rc = encode(&gm, g, batch, l.small, l.small, l.g_ld, false);
-  if (rc == H3B_OK) rc = encode(&bm, b, batch, l.small, l.small, l.g_ld, false);
+  enc(&g_k, g, l.small, l.g_ld, BY_ROWS);
+  enc(&g_out, g, l.small, l.g_ld, STORES);
+  enc(&k_k, k, l.small, l.g_ld, BY_ROWS);
+  enc(&k_out, k, l.small, l.g_ld, STORES);
+  enc(&b_k, b, l.small, l.g_ld, BY_ROWS);
+  enc(&b_out, b, l.small, l.g_ld, STORES);
+  const bool result_tma = row_bytes % 16 == 0 && h3b::aligned16(out);
+  if (rc == H3B_OK && result_tma) {
+    rc = h3b::encode_3d(&result.hi,
+                        dtype == H3B_F32   ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
+                        : dtype == H3B_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16
+                                           : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16,
+                        out, n, m, batch, row_bytes, m * row_bytes, 64 / sizeof(T), 32, 1, CU_TENSOR_MAP_SWIZZLE_64B);
+    result.lo = result.hi;
+  } else {
+    result = g_out;  // not used
+  }
 
+  const double ca = coefficients[0], cb = coefficients[1], cc = coefficients[2];
+  const bool square = dtype != H3B_F32 && cc != 0.0 && cb * cb <= 64.0 * cc * cc;
   for (int s = 0; s < steps && rc == H3B_OK; ++s) {
-    const bool first = s == 0, last = s == steps - 1;
-    const bool pairs = !(last && dtype == H3B_BF16);  // planes in pairs: all steps but a bf16 result's last
-    const bool x_lo = pairs && !(first && exact);
+    const bool first = s == 0, last = s == steps - 1, bf16 = dtype == H3B_BF16;
+    // planes in pairs: the products with X, and those that make B
+    const bool x_pairs = !(bf16 && last), b_pairs = !(bf16 && s >= steps - 2);
+    const bool x_exact = first && exact;
     const int cur = s & 1;
-    Args a{};
-    a.batch = static_cast<int>(batch);
-    a.rows = a.cols = static_cast<int>(l.small);
-    a.k = static_cast<int>(l.large);
-    a.factor = first ? factor : nullptr;
-    a.b_lo = x_lo;
-    a.beta = 1.0f / SCALE;
-    a.diagonal = pairs ? 0.0f : -SCALE;
-    a.out = {g.hi, pairs ? g.lo : nullptr};
-    a.out_ld = l.g_ld;
-    a.out_batch = l.small * l.g_ld;
-    rc = product<GRAM>(x_lo, x_k[cur], x_k[cur], a, stream);
+    Args p{};
+    p.batch = static_cast<int>(batch);
+    p.rows = p.cols = static_cast<int>(l.small);
+    p.k = static_cast<int>(l.large);
+    p.factor = first ? factor : nullptr;
+    p.b_lo = 1;
+    p.out_lo = b_pairs;
+    p.beta = 1.0f / SCALE;
+    p.diagonal = square ? static_cast<float>(SCALE * cb / (2.0 * cc)) : b_pairs ? 0.0f : -SCALE;
+    p.k_beta = coefficients[2];
+    p.k_diagonal = static_cast<float>(SCALE * (b_pairs ? cb : cb + 2.0 * cc));
+    p.with_k = !square;
+    rc = product<GRAM>(b_pairs && !x_exact, x_k[cur], x_k[cur], g_out, k_out, p, stream);
     if (rc != H3B_OK) break;
 
-    a.factor = nullptr;
-    a.k = a.rows;
-    a.b_lo = pairs;
-    a.add = a.out;
-    a.add_ld = l.g_ld;
-    a.add_batch = a.out_batch;
-    a.out = b;
-    if (!pairs) a.out.lo = nullptr;
-    a.alpha = pairs ? coefficients[1] : coefficients[1] + 2.0f * coefficients[2];
-    a.beta = coefficients[2] / SCALE;
-    rc = product<POLY>(pairs, gm, gm, a, stream);
+    p.factor = nullptr;
+    p.k = p.rows;
+    p.out_lo = x_pairs;
+    if (square) p.beta *= coefficients[2];
+    p.diagonal = static_cast<float>(SCALE * (square ? ca - cb * cb / (4.0 * cc) : b_pairs ? ca : ca + cb + cc));
+    rc = product<POLY>(b_pairs, g_k, square ? g_k : k_k, b_out, b_out, p, stream);
     if (rc != H3B_OK) break;
 
-    a.factor = first ? factor : nullptr;
-    a.cols = static_cast<int>(l.large);
-    a.b_lo = x_lo;
-    a.add = xs[cur];
-    if (first && exact) a.add.lo = nullptr;
-    a.add_ld = l.x_ld;
-    a.add_batch = l.small * l.x_ld;
-    a.out = xs[cur ^ 1];
-    a.out_ld = l.x_ld;
-    a.out_batch = a.add_batch;
-    a.alpha = pairs ? coefficients[0] : coefficients[0] + coefficients[1] + coefficients[2];
-    a.beta = 1.0f / SCALE;
+    p.factor = first ? factor : nullptr;
+    p.beta = 1.0f / SCALE;
+    p.cols = static_cast<int>(l.large);
+    p.b_lo = !x_exact;
     if (last) {
-      a.alpha /= SCALE;
-      a.beta /= SCALE;
-      a.result = out;
-      a.result_dtype = dtype;
-      a.result_t = tall;
-      a.result_batch = m * n;
-      a.result_ld = n;
-      a.result_wide = !tall && h3b::aligned16(out) && n * static_cast<int64_t>(sizeof(T)) % 16 == 0;
+      p.beta /= SCALE;
+      p.result = out;
+      p.result_dtype = dtype;
+      p.result_t = tall;
+      p.result_tma = result_tma;
+      p.result_batch = m * n;
+      p.result_ld = n;
     }
-    rc = product<MUL>(pairs, bm, x_n[cur], a, stream);
+    p.out_lo = 1;
+    const Maps& to = last ? result : x_out[cur ^ 1];
+    rc = product<MUL>(x_pairs, b_k, x_n[cur], to, to, p, stream);
   }
   return rc;
 }
