@@ -57,6 +57,7 @@
 // dependent launch); every kernel waits for it before it touches memory.
 #include "h3b_common.cuh"
 #include "h3b_host.hpp"
+#include "ortho.hpp"
 
 H3B_DECLARE_STATUS();
 H3B_REGISTER_STATUS_READER(ortho);
@@ -763,12 +764,13 @@ struct Layout {
   int64_t small, large;      // sides of X
   int64_t x_ld, g_ld;        // row strides of the planes of X and of G, K, B
   int64_t x_plane, g_plane;  // elements of a plane, all matrices
-  int64_t bytes;
+  int64_t planes, bytes;     // where the planes begin; all
 };
 
 int64_t up(int64_t v, int64_t to) { return (v + to - 1) / to * to; }
 
-// Planes of X (two, in turn), G, K and B, two each; sums of squares; factors.
+// Sums of squares, factors; planes of X (two, in turn), G, K and B, two each
+// (none for matrices that ortho_small takes).
 Layout layout(int64_t batch, int64_t m, int64_t n) {
   Layout l;
   l.small = m < n ? m : n;
@@ -777,7 +779,8 @@ Layout layout(int64_t batch, int64_t m, int64_t n) {
   l.g_ld = up(l.small, 32);
   l.x_plane = up(batch * l.small * l.x_ld, 128);
   l.g_plane = up(batch * l.small * l.g_ld, 128);
-  l.bytes = (4 * l.x_plane + 6 * l.g_plane) * 2 + batch * (MAX_PARTS * 8) + up(batch * 4, 256);
+  l.planes = batch * (MAX_PARTS * 8) + up(batch * 4, 256);
+  l.bytes = l.planes + (h3b::ortho_small_fits(m, n) ? 0 : (4 * l.x_plane + 6 * l.g_plane) * 2);
   return l;
 }
 
@@ -874,10 +877,16 @@ int launch_after(void (*kernel)(Params...), dim3 grid, cudaStream_t stream, Valu
 }
 
 template <class T>
-int run(const T* x, T* out, int dtype, int64_t batch, int64_t m, int64_t n, int64_t batch_stride, int64_t ld, int steps,
-        const float* coefficients, float eps, uint8_t* ws, cudaStream_t stream) {
+int run(const h3b::OrthoCall& call, uint8_t* ws, cudaStream_t stream) {
+  const T* x = static_cast<const T*>(call.x);
+  T* out = static_cast<T*>(call.out);
+  const int dtype = call.dtype, steps = call.steps;
+  const int64_t batch = call.batch, m = call.m, n = call.n, batch_stride = call.batch_stride, ld = call.ld;
+  const float eps = call.eps;
   const Layout l = layout(batch, m, n);
-  __half* at = reinterpret_cast<__half*>(ws);
+  double* parts = reinterpret_cast<double*>(ws);
+  float* factor = reinterpret_cast<float*>(parts + batch * MAX_PARTS);
+  __half* at = reinterpret_cast<__half*>(ws + l.planes);
   auto take = [&](int64_t plane) {
     Planes p{at, at + plane};
     at += 2 * plane;
@@ -885,8 +894,6 @@ int run(const T* x, T* out, int dtype, int64_t batch, int64_t m, int64_t n, int6
   };
   Planes xs[2] = {take(l.x_plane), take(l.x_plane)};
   const Planes g = take(l.g_plane), k = take(l.g_plane), b = take(l.g_plane);
-  double* parts = reinterpret_cast<double*>(at);
-  float* factor = reinterpret_cast<float*>(parts + batch * MAX_PARTS);
   const int64_t row_bytes = n * static_cast<int64_t>(sizeof(T));
   const bool wide = n % 8 == 0 && h3b::aligned16(x) && ld * static_cast<int64_t>(sizeof(T)) % 16 == 0 &&
                     (batch == 1 || batch_stride * static_cast<int64_t>(sizeof(T)) % 16 == 0);
@@ -936,7 +943,7 @@ int run(const T* x, T* out, int dtype, int64_t batch, int64_t m, int64_t n, int6
     result = g_out;  // not used
   }
 
-  const double ca = coefficients[0], cb = coefficients[1], cc = coefficients[2];
+  const double ca = call.a, cb = call.b, cc = call.c;
   const bool square = dtype != H3B_F32 && cc != 0.0 && cb * cb <= 64.0 * cc * cc;
   for (int s = 0; s < steps && rc == H3B_OK; ++s) {
     const bool first = s == 0, last = s == steps - 1, bf16 = dtype == H3B_BF16;
@@ -953,7 +960,7 @@ int run(const T* x, T* out, int dtype, int64_t batch, int64_t m, int64_t n, int6
     p.out_lo = b_pairs;
     p.beta = 1.0f / SCALE;
     p.diagonal = square ? static_cast<float>(SCALE * cb / (2.0 * cc)) : b_pairs ? 0.0f : -SCALE;
-    p.k_beta = coefficients[2];
+    p.k_beta = call.c;
     p.k_diagonal = static_cast<float>(SCALE * (b_pairs ? cb : cb + 2.0 * cc));
     p.with_k = !square;
     rc = product<GRAM>(b_pairs && !x_exact, x_k[cur], x_k[cur], g_out, k_out, p, stream);
@@ -962,7 +969,7 @@ int run(const T* x, T* out, int dtype, int64_t batch, int64_t m, int64_t n, int6
     p.factor = nullptr;
     p.k = p.rows;
     p.out_lo = x_pairs;
-    if (square) p.beta *= coefficients[2];
+    if (square) p.beta *= call.c;
     p.diagonal = static_cast<float>(SCALE * (square ? ca - cb * cb / (4.0 * cc) : b_pairs ? ca : ca + cb + cc));
     rc = product<POLY>(b_pairs, g_k, square ? g_k : k_k, b_out, b_out, p, stream);
     if (rc != H3B_OK) break;
@@ -1008,16 +1015,11 @@ extern "C" int h3b_orthogonalize(const void* x, void* out, int dtype, int64_t ba
     return H3B_ERR_ARG;
   if (!h3b::aligned16(workspace)) return H3B_ERR_ALIGN;
   if (workspace_bytes < layout(batch, m, n).bytes) return H3B_ERR_ARG;
-  const float coefficients[3] = {a, b, c};
+  const h3b::OrthoCall call{x, out, dtype, batch, m, n, batch_stride, ld, static_cast<int>(steps), a, b, c, eps};
   const auto st = reinterpret_cast<cudaStream_t>(stream);
+  if (steps > 0 && h3b::ortho_small_fits(m, n)) return h3b::ortho_small(call, st);
   auto* ws = static_cast<uint8_t*>(workspace);
-  const int k = static_cast<int>(steps);
-  if (dtype == H3B_F32)
-    return run(static_cast<const float*>(x), static_cast<float*>(out), dtype, batch, m, n, batch_stride, ld, k,
-               coefficients, eps, ws, st);
-  if (dtype == H3B_F16)
-    return run(static_cast<const __half*>(x), static_cast<__half*>(out), dtype, batch, m, n, batch_stride, ld, k,
-               coefficients, eps, ws, st);
-  return run(static_cast<const __nv_bfloat16*>(x), static_cast<__nv_bfloat16*>(out), dtype, batch, m, n, batch_stride,
-             ld, k, coefficients, eps, ws, st);
+  if (dtype == H3B_F32) return run<float>(call, ws, st);
+  if (dtype == H3B_F16) return run<__half>(call, ws, st);
+  return run<__nv_bfloat16>(call, ws, st);
 }
