@@ -489,10 +489,11 @@ __global__ void __launch_bounds__(THREADS, 1)
             tc_fence_before();
             __syncwarp();
             if (lane == 0) {
-              if constexpr (PAIR == 2)
-                mbar_arrive_cluster(mapa_shared(smem_u32(&bars->acc_empty[buf]), 0));
-              else
+              // (a release of cluster scope would hold this warp for 1000 cycles)
+              if (leader)
                 mbar_arrive(&bars->acc_empty[buf]);
+              else
+                mbar_arrive_remote(mapa_shared(smem_u32(&bars->acc_empty[buf]), 0));
             }
           }
 #pragma unroll
