@@ -44,17 +44,19 @@
 // accumulators in registers, rounding to nearest.
 //
 // Tiles: 256 x 256 by CTA pairs (cta_group::2, each CTA stages 128 rows of
-// both operands) or, where those are too few for the SMs, 128 x 128 by one
-// CTA (its operand reads and copies share the shared-memory port: a tile
-// costs 0.8 of the pair's time for half the work).  Warp 0 loads (TMA, zero
-// beyond the matrix), warp 1 issues the products, eight warps add and store;
-// two accumulators in turn, so that products go on meanwhile.  Stores go
-// through shared memory as TMA blocks of 32 x 32 (lanes that stored their
-// rows' 16-byte pieces themselves took 20 us a tile, a third of a product's
-// time at 4096), the other side's from registers.  Every wait is bounded.
+// both operands); where those are too few for the SMs, 128 x 128 by one CTA;
+// where those are, too, by a cluster of two or four, each with a part of K, that
+// hand each other their sums through distributed shared memory.
+// Warp 0 loads (TMA, zero beyond the matrix), warp 1 issues the products,
+// eight warps add and store; two accumulators in turn, so that products go on
+// meanwhile.  Stores go through shared memory as TMA blocks of 32 x 32 (lanes
+// that stored their rows' 16-byte pieces themselves took 20 us a tile, a third
+// of a product's time at 4096).  Every wait is bounded.
 //
 // A launch's setup overlaps the end of the one before it (programmatic
 // dependent launch); every kernel waits for it before it touches memory.
+#include <algorithm>
+
 #include "h3b_common.cuh"
 #include "h3b_host.hpp"
 #include "ortho.hpp"
@@ -82,8 +84,11 @@ static_assert(4 * REGS_CTL + 8 * REGS_EPI <= 12 * LAUNCH_REGS, "register split e
 
 enum Op { GRAM = 0, POLY = 1, MUL = 2 };
 
-template <int PAIR, int OP, int SPLIT>
+// PAIR: CTAs of a 256 x 256 tile.  PARTS: CTAs that share the K of a 128 x 128
+// tile (PAIR = 1).
+template <int PAIR, int PARTS, int OP, int SPLIT>
 struct Cfg {
+  static_assert(PAIR == 1 || PARTS == 1, "pairs take all of K");
   static constexpr int BN = 128 * PAIR;
   static constexpr int PLANES = SPLIT ? 2 : 1;
   static constexpr int STAGE_BYTES = 2 * PLANES * PLANE_BYTES;  // A planes, then B planes
@@ -123,9 +128,9 @@ struct __align__(8) Barriers {
   int consumed;
 };
 
-template <int PAIR, int OP, int SPLIT>
+template <int PAIR, int PARTS, int OP, int SPLIT>
 constexpr size_t smem_bytes() {
-  using C = Cfg<PAIR, OP, SPLIT>;
+  using C = Cfg<PAIR, PARTS, OP, SPLIT>;
   return 1024 + static_cast<size_t>(C::STAGES) * C::STAGE_BYTES + EPI_WARPS * BLOCKS * BLOCK_BYTES + sizeof(Barriers);
 }
 
@@ -270,14 +275,14 @@ H3B_DEV void store_elements(const Args& args, int batch, int row, int col0, cons
 H3B_DEV void launch_next() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 H3B_DEV void wait_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 
-template <int PAIR, int OP, int SPLIT>
+template <int PAIR, int PARTS, int OP, int SPLIT>
 __global__ void __launch_bounds__(THREADS, 1)
     ortho_product(const __grid_constant__ CUtensorMap a_hi, const __grid_constant__ CUtensorMap a_lo,
                   const __grid_constant__ CUtensorMap b_hi, const __grid_constant__ CUtensorMap b_lo,
                   const __grid_constant__ CUtensorMap out_hi, const __grid_constant__ CUtensorMap out_lo,
                   const __grid_constant__ CUtensorMap k_hi, const __grid_constant__ CUtensorMap k_lo,
                   const Args args) {
-  using C = Cfg<PAIR, OP, SPLIT>;
+  using C = Cfg<PAIR, PARTS, OP, SPLIT>;
   constexpr int STAGES = C::STAGES, BN = C::BN;
   constexpr bool SYMMETRIC = OP != MUL;
   extern __shared__ uint8_t smem_raw[];
@@ -287,11 +292,14 @@ __global__ void __launch_bounds__(THREADS, 1)
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t rank = PAIR == 2 ? cluster_ctarank() : 0u;
   const bool leader = rank == 0;
-  const int cluster = static_cast<int>(blockIdx.x) / PAIR, n_clusters = static_cast<int>(gridDim.x) / PAIR;
+  const int part = PARTS > 1 ? static_cast<int>(cluster_ctarank()) : 0;
+  const int cluster = static_cast<int>(blockIdx.x) / (PAIR * PARTS), n_clusters = static_cast<int>(gridDim.x) / (PAIR * PARTS);
   const int row_tiles = (args.rows + BN - 1) / BN, col_tiles = (args.cols + BN - 1) / BN;  // tiles are square
   const int per_matrix = SYMMETRIC ? row_tiles * (row_tiles + 1) / 2 : row_tiles * col_tiles;
   const int num_tiles = per_matrix * args.batch;
-  const int nk = (args.k + KB - 1) / KB;
+  // stages of K: this CTA's (PARTS > 1: a launch has a cluster for each tile)
+  const int all_k = (args.k + KB - 1) / KB, share_k = (all_k + PARTS - 1) / PARTS;
+  const int first_k = part * share_k, nk = max(0, min(share_k, all_k - first_k));
   volatile int* abort_flag = &bars->abort_flag;
 
   if (threadIdx.x == 0) {
@@ -321,7 +329,7 @@ __global__ void __launch_bounds__(THREADS, 1)
     }
   }
   tc_fence_before();
-  if constexpr (PAIR == 2)
+  if constexpr (PAIR * PARTS > 1)
     cluster_sync();
   else
     __syncthreads();
@@ -359,14 +367,14 @@ __global__ void __launch_bounds__(THREADS, 1)
             else
               tma_load_3d(dst, map, x, y, tile.batch, &bars->full[s]);
           };
-          load(stage, &a_hi, kb * KB, m0);
-          if constexpr (SPLIT != 0) load(stage + PLANE_BYTES, &a_lo, kb * KB, m0);
+          load(stage, &a_hi, (first_k + kb) * KB, m0);
+          if constexpr (SPLIT != 0) load(stage + PLANE_BYTES, &a_lo, (first_k + kb) * KB, m0);
           auto load_b = [&](uint8_t* dst, const CUtensorMap* map) {
             if constexpr (OP == MUL) {  // boxes of 64 columns x 64 rows of K
-              load(dst, map, n0, kb * KB);
-              load(dst + PLANE_BYTES / 2, map, n0 + 64, kb * KB);
+              load(dst, map, n0, (first_k + kb) * KB);
+              load(dst + PLANE_BYTES / 2, map, n0 + 64, (first_k + kb) * KB);
             } else {
-              load(dst, map, kb * KB, n0);
+              load(dst, map, (first_k + kb) * KB, n0);
             }
           };
           load_b(stage + C::PLANES * PLANE_BYTES, &b_hi);
@@ -461,6 +469,11 @@ __global__ void __launch_bounds__(THREADS, 1)
       warp_wait(&bars->drain, 0, 8, nullptr);
     }
   }
+  if constexpr (PARTS > 1) {  // the storing warps' hand-over
+    __syncwarp();
+    cluster_sync();
+    cluster_sync();
+  }
   } else {
     // --------------------------------------------------------- stores
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(REGS_EPI));
@@ -471,6 +484,12 @@ __global__ void __launch_bounds__(THREADS, 1)
     bool ok = true;
     for (int t = cluster; t < num_tiles && ok; t += n_clusters) {
       float acc[2 * MINE][16];
+      if (PARTS > 1 && nk == 0) {  // a part without any of K
+#pragma unroll
+        for (int i = 0; i < 2 * MINE; ++i)
+#pragma unroll
+          for (int j = 0; j < 16; ++j) acc[i][j] = 0.0f;
+      }
       for (int kb = 0; kb < nk; kb += C::CHUNK, ++local) {
         const int buf = local & 1, use = local >> 1;
         if (!warp_wait<true>(&bars->acc_full[buf], use & 1, 4, abort_flag)) {
@@ -500,27 +519,28 @@ __global__ void __launch_bounds__(THREADS, 1)
           for (int j = 0; j < 16; ++j) acc[i][j] = kb == 0 ? __uint_as_float(r[j]) : acc[i][j] + __uint_as_float(r[j]);
         }
       }
-      if (!ok) break;
+      if constexpr (PARTS == 1) {
+        if (!ok) break;
+      }
       const Tile tile = tile_at<SYMMETRIC>(t, per_matrix, col_tiles);
       const int row0 = tile.i * BN + static_cast<int>(rank) * BM + quad * 32, row = row0 + lane;
-      if (row0 >= args.rows) continue;  // warp-uniform, as all that follows
       const float f = args.factor != nullptr ? args.factor[tile.batch] : 1.0f;
       const float beta = (OP == GRAM ? f * f : OP == MUL ? f : 1.0f) * args.beta;
-#pragma unroll
-      for (int i = 0; i < MINE; ++i) {
-        const int col0 = tile.j * BN + (half + 2 * i) * 32;
-        if (col0 >= args.cols) continue;
+      // Stores 32 columns from col0 of the sums that sums(v) puts into v; of
+      // the planes (G's, then K's two) those in `planes`.
+      auto store = [&](auto sums, int col0, int planes) {
         float v[32];
+        sums(v);
 #pragma unroll
-        for (int j = 0; j < 32; ++j) v[j] = acc[2 * i + (j >> 4)][j & 15] * beta;
+        for (int j = 0; j < 32; ++j) v[j] *= beta;
         if (SYMMETRIC && tile.i == tile.j) {
 #pragma unroll
           for (int j = 0; j < 32; ++j)
             if (col0 + j == row) v[j] += args.diagonal;
         }
-        __syncwarp();
         uint32_t w[16];
         if (OP == MUL && args.result != nullptr) {
+          if ((planes & 1) == 0) return;
           if (!args.result_tma) {
             if (row < args.rows) store_elements(args, tile.batch, row, col0, v);
             __syncwarp();
@@ -532,24 +552,22 @@ __global__ void __launch_bounds__(THREADS, 1)
               w[j] = args.result_dtype == H3B_F16 ? pack_f16x2(v[2 * j], v[2 * j + 1]) : pack_bf16x2(v[2 * j], v[2 * j + 1]);
             out.put(&out_hi, w, args.result_t, col0, row0, tile.batch);
           }
-          continue;
+          return;
         }
         const bool mirror = SYMMETRIC && tile.i != tile.j;
 #pragma unroll
         for (int m = 0; m < (OP == GRAM ? 2 : 1); ++m) {
-          if (m == 1 && !args.with_k) break;
-          const CUtensorMap *hi = m == 0 ? &out_hi : &k_hi, *lo = m == 0 ? &out_lo : &k_lo;
           if (m == 1) {  // K, from the sums once more (fewer registers than keeping G)
+            if (!args.with_k) break;
+            sums(v);
 #pragma unroll
-            for (int j = 0; j < 32; ++j) v[j] = acc[2 * i + (j >> 4)][j & 15] * beta;
-            if (!mirror) {
-#pragma unroll
-              for (int j = 0; j < 32; ++j)
-                if (col0 + j == row) v[j] += args.diagonal;
+            for (int j = 0; j < 32; ++j) {
+              v[j] *= beta;
+              if (!mirror && col0 + j == row) v[j] += args.diagonal;
+              v[j] = v[j] * args.k_beta + (col0 + j == row ? args.k_diagonal : 0.0f);
             }
-#pragma unroll
-            for (int j = 0; j < 32; ++j) v[j] = v[j] * args.k_beta + (col0 + j == row ? args.k_diagonal : 0.0f);
           }
+          const CUtensorMap *hi = m == 0 ? &out_hi : &k_hi, *lo = m == 0 ? &out_lo : &k_lo;
 #pragma unroll
           for (int j = 0; j < 16; ++j) {
             w[j] = pack_f16x2(v[2 * j], v[2 * j + 1]);
@@ -557,15 +575,75 @@ __global__ void __launch_bounds__(THREADS, 1)
             v[2 * j] -= h.x;
             v[2 * j + 1] -= h.y;
           }
-          out.put(hi, w, false, col0, row0, tile.batch);
-          if (mirror) out.put(hi, w, true, col0, row0, tile.batch);
-          if (args.out_lo) {
+          if (planes & (1 << (2 * m))) {
+            out.put(hi, w, false, col0, row0, tile.batch);
+            if (mirror) out.put(hi, w, true, col0, row0, tile.batch);
+          }
+          if (args.out_lo && (planes & (2 << (2 * m)))) {
 #pragma unroll
             for (int j = 0; j < 16; ++j) w[j] = pack_f16x2(v[2 * j], v[2 * j + 1]);
             out.put(lo, w, false, col0, row0, tile.batch);
             if (mirror) out.put(lo, w, true, col0, row0, tile.batch);
           }
         }
+      };
+      if constexpr (PARTS == 1) {
+        if (row0 >= args.rows) continue;  // warp-uniform, as all that follows
+#pragma unroll
+        for (int i = 0; i < MINE; ++i) {
+          const int col0 = tile.j * BN + (half + 2 * i) * 32;
+          if (col0 < args.cols)
+            store([&](float(&v)[32]) {
+#pragma unroll
+              for (int j = 0; j < 32; ++j) v[j] = acc[2 * i + (j >> 4)][j & 15];
+            }, col0, 15);
+        }
+      } else {
+        // Part q gets the parts' sums of its 128 / PARTS columns, in blocks
+        // of 32 columns, four columns of all rows after the other (a warp
+        // writes 512 bytes at once), where the operands' stages were.
+        static_assert(PARTS == 1 || PARTS == 2 || PARTS == 4, "whole blocks for each part");
+        constexpr int OWN = 4 / PARTS;  // blocks of a part
+        auto share = [&](int from, int block, int p) {
+          return static_cast<uint32_t>((((from * OWN + block) * 8 + p) * BM + quad * 32 + lane) * 16);
+        };
+        __syncwarp();
+        cluster_sync();  // every part's products have read their stages
+#pragma unroll
+        for (int i = 0; i < MINE; ++i) {
+          const int block = half + 2 * i;
+          const uint32_t to = mapa_shared(smem_u32(smem), static_cast<uint32_t>(block / OWN));
+#pragma unroll
+          for (int p = 0; p < 8; ++p) {
+            const float* x = &acc[2 * i + (p >> 2)][4 * (p & 3)];
+            asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(to + share(part, block % OWN, p)), "f"(x[0]), "f"(x[1]),
+                         "f"(x[2]), "f"(x[3])
+                         : "memory");
+          }
+        }
+        cluster_sync();
+        const int block = OWN == 2 ? half : 0, col0 = tile.j * BN + (part * OWN + block) * 32;
+        // with one block for both halves' warps they share its planes: G's and K's, or first and second
+        const int planes = OWN == 2 ? 15 : OP == GRAM && args.with_k ? (half ? 12 : 3) : (half ? 2 : 1);
+        if (row0 < args.rows && col0 < args.cols)
+          store([&](float(&v)[32]) {
+#pragma unroll
+            for (int p = 0; p < 8; ++p) {
+              float4 s = *reinterpret_cast<const float4*>(smem + share(0, block, p));
+#pragma unroll
+              for (int q = 1; q < PARTS; ++q) {
+                const float4 x = *reinterpret_cast<const float4*>(smem + share(q, block, p));
+                s.x += x.x;
+                s.y += x.y;
+                s.z += x.z;
+                s.w += x.w;
+              }
+              v[4 * p] = s.x;
+              v[4 * p + 1] = s.y;
+              v[4 * p + 2] = s.z;
+              v[4 * p + 3] = s.w;
+            }
+          }, col0, planes);
       }
     }
     if (lane == 0) bulk_wait_group<0>();  // the blocks are in place before the CTA leaves
@@ -810,12 +888,12 @@ int encode(Maps* maps, const Planes& p, int64_t batch, int64_t rows, int64_t col
   return H3B_OK;
 }
 
-template <int PAIR, int OP, int SPLIT>
+template <int PAIR, int PARTS, int OP, int SPLIT>
 int launch(const Maps& a, const Maps& b, const Maps& out, const Maps& k, const Args& args, int64_t tiles, cudaStream_t stream) {
-  constexpr size_t smem = smem_bytes<PAIR, OP, SPLIT>();
+  constexpr size_t smem = smem_bytes<PAIR, PARTS, OP, SPLIT>();
   static_assert(smem <= 227 * 1024, "shared memory budget");
   static h3b::OncePerDevice once;
-  const auto kernel = ortho_product<PAIR, OP, SPLIT>;
+  const auto kernel = ortho_product<PAIR, PARTS, OP, SPLIT>;
   const int rc = once.run(h3b::device(), [&] {
     // the register split waits for good in a launch with fewer registers than it adds up to
     cudaFuncAttributes attr;
@@ -823,9 +901,10 @@ int launch(const Maps& a, const Maps& b, const Maps& out, const Maps& k, const A
     return h3b::allow_smem(kernel, smem);
   });
   if (rc != H3B_OK) return rc;
-  const int64_t most = h3b::num_sms() / PAIR;
+  // every tile has a cluster of its own where parts share it
+  const int64_t most = PARTS > 1 ? tiles : h3b::num_sms() / PAIR;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(static_cast<unsigned>((tiles < most ? tiles : most) * PAIR));
+  cfg.gridDim = dim3(static_cast<unsigned>((tiles < most ? tiles : most) * PAIR * PARTS));
   cfg.blockDim = dim3(THREADS);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = stream;
@@ -833,10 +912,10 @@ int launch(const Maps& a, const Maps& b, const Maps& out, const Maps& k, const A
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   attr[1].id = cudaLaunchAttributeClusterDimension;
-  attr[1].val.clusterDim.x = PAIR;
+  attr[1].val.clusterDim.x = PAIR * PARTS;
   attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
   cfg.attrs = attr;
-  cfg.numAttrs = PAIR == 2 ? 2 : 1;
+  cfg.numAttrs = PAIR * PARTS > 1 ? 2 : 1;
   return cudaLaunchKernelEx(&cfg, kernel, a.hi, a.lo, b.hi, b.lo, out.hi, out.lo, k.hi, k.lo, args) == cudaSuccess ? H3B_OK : H3B_ERR_LAUNCH;
 }
 
@@ -851,10 +930,23 @@ int product(const Maps& a, const Maps& b, const Maps& out, const Maps& k, const 
   const int64_t sms = h3b::num_sms();
   const int64_t t1 = tiles_of(args.rows, args.cols, args.batch, 128, OP != MUL);
   const int64_t t2 = tiles_of(args.rows, args.cols, args.batch, 256, OP != MUL);
-  // Rounds of tiles, a 128 x 128 tile counted 0.8 of a pair's 256 x 256 one.
-  const int64_t single = (t1 + sms - 1) / sms * 4, pair = (t2 + sms / 2 - 1) / (sms / 2) * 5;
-  return single <= pair ? launch<1, OP, SPLIT>(a, b, out, k, args, t1, stream)
-                        : launch<2, OP, SPLIT>(a, b, out, k, args, t2, stream);
+  // Rounds of tiles times what one takes, in cycles: a stage of K in three
+  // products 1280 (one CTA; its operand reads and copies share the
+  // shared-memory port) or 1540 (a pair's tile of four times the size), a
+  // third of it in one; the beginning and the stores 8000, 14000, and 10000
+  // where CTAs hand their sums over.  Of clusters of four with a whole SM
+  // each, 33 run at once on 148 SMs.
+  const int64_t stages = (args.k + KB - 1) / KB, stage = SPLIT ? 1281 : 427;
+  const auto rounds = [](int64_t n, int64_t at_once) { return (n + at_once - 1) / at_once; };
+  const int64_t single = rounds(t1, sms) * (stages * stage + 8000);
+  const int64_t pair = rounds(t2, sms / 2) * (stages * stage * 6 / 5 + 14000);
+  const int64_t halves = rounds(t1, sms / 2) * ((stages + 1) / 2 * stage + 10000);
+  const int64_t quarters = rounds(t1, sms * 9 / 40) * ((stages + 3) / 4 * stage + 10000);
+  const int64_t best = std::min(std::min(single, pair), std::min(halves, quarters));
+  if (single == best) return launch<1, 1, OP, SPLIT>(a, b, out, k, args, t1, stream);
+  if (pair == best) return launch<2, 1, OP, SPLIT>(a, b, out, k, args, t2, stream);
+  if (halves == best) return launch<1, 2, OP, SPLIT>(a, b, out, k, args, t1, stream);
+  return launch<1, 4, OP, SPLIT>(a, b, out, k, args, t1, stream);
 }
 
 template <int OP>
