@@ -153,10 +153,13 @@ __global__ void __launch_bounds__(THREADS, 1) ortho_small_kernel(const Args args
   };
 
   // ------------------------------------------------- norm, planes of X
-  // Items of eight elements that are consecutive in memory, all of a thread's
-  // loaded before any is used.  Neighbouring threads take neighbouring items
-  // of a row of X, or of a column of it where x is its transpose (the rows of
-  // x they read are short, the planes' rows are what they write).
+  // First x as it is: the upper 16 bits of an element (as 32 bits) where its
+  // first plane will be, the lower ones where the second; 32 elements of a
+  // thread in flight, in loops (code that runs once comes from L2: unrolled
+  // whole it took longer than the loads).  Then the norm, and each piece in
+  // its place.  Where rows of x are whole 16-byte words an item is eight
+  // elements, neighbouring threads taking neighbouring items of a row of X, or
+  // of a column of it where x is its transpose; else a warp takes rows of x.
   const T* x = static_cast<const T*>(args.x) + matrix * args.batch_stride;
   const int cols = max(0, min(args.width, args.cols - col0));
   const int lines = args.tall ? cols : args.rows, length = args.tall ? args.rows : cols;
@@ -170,76 +173,99 @@ __global__ void __launch_bounds__(THREADS, 1) ortho_small_kernel(const Args args
       *at = (i - *line * per_line) * 8;
     }
   };
-  constexpr int ITEMS = ROWS * MAX_W / 8 / THREADS;
-  {
-    const int64_t first = args.tall ? col0 * args.ld : col0;
-    T e[ITEMS][8];
+  auto put_raw = [&](int line, int at, T v) {
+    const uint32_t to = args.tall ? piece(at, line >> 3) + (line & 7) * 2 : piece(line, at >> 3) + (at & 7) * 2;
+    const uint32_t bits = __float_as_uint(to_f32(v));
+    *reinterpret_cast<uint16_t*>(x_hi + to) = static_cast<uint16_t>(bits >> 16);
+    *reinterpret_cast<uint16_t*>(x_lo + to) = static_cast<uint16_t>(bits);
+  };
+  // zero planes: rows and columns behind the matrix stay so
+  for (int i = tid; i < tiles * TILE * 2 / 16; i += THREADS) reinterpret_cast<uint4*>(x_hi)[i] = make_uint4(0, 0, 0, 0);
+  __syncthreads();
+  double s = 0.0;
+  auto square_of = [&](T v) { s = fma(static_cast<double>(to_f32(v)), static_cast<double>(to_f32(v)), s); };
+  x += args.tall ? col0 * args.ld : col0;
+  if (args.wide) {
+    for (int i0 = tid; i0 < items; i0 += 4 * THREADS) {
+      T e[4][8];
+      int line[4], at[4];
 #pragma unroll
-    for (int k = 0; k < ITEMS; ++k) {
-      const int i = tid + k * THREADS;
-      if (i < items) {
-        int line, at;
-        item(i, &line, &at);
-        const T* p = x + first + line * args.ld + at;
-        if (args.wide) {
+      for (int k = 0; k < 4; ++k) {
+        const int i = i0 + k * THREADS;
+        if (i < items) {
+          item(i, &line[k], &at[k]);
+          const T* p = x + line[k] * args.ld + at[k];
 #pragma unroll
           for (int j = 0; j < static_cast<int>(sizeof(T)) / 2; ++j)
             reinterpret_cast<uint4*>(e[k])[j] = reinterpret_cast<const uint4*>(p)[j];
-        } else {
-#pragma unroll
-          for (int j = 0; j < 8; ++j) e[k][j] = at + j < length ? p[j] : from_f32<T>(0.0f);
         }
       }
-    }
-    double s = 0.0;
 #pragma unroll
-    for (int k = 0; k < ITEMS; ++k)
-      if (tid + k * THREADS < items)
+      for (int k = 0; k < 4; ++k)
+        if (i0 + k * THREADS < items) {
 #pragma unroll
-        for (int j = 0; j < 8; ++j) s = fma(static_cast<double>(to_f32(e[k][j])), static_cast<double>(to_f32(e[k][j])), s);
+          for (int j = 0; j < 8; ++j) square_of(e[k][j]);
+          if (args.tall) {
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-    if (lane == 0) sh->warp_sums[warp] = s;
-    // zero planes: rows and columns behind the matrix stay so
-    for (int i = tid; i < tiles * TILE * 2 / 16; i += THREADS) reinterpret_cast<uint4*>(x_hi)[i] = make_uint4(0, 0, 0, 0);
-    __syncthreads();
-    if (CTAS > 1) cluster_sync();  // every CTA runs: its shared memory can be written
-    if (tid < CTAS) {
-      s = 0.0;
-      for (int i = 0; i < THREADS / 32; ++i) s += sh->warp_sums[i];
-      asm volatile("st.shared::cluster.f64 [%0], %1;" ::"r"(mapa_shared(smem_u32(&sh->squares[rank]), tid)), "d"(s) : "memory");
-    }
-    all_sync();
-    s = 0.0;
-    for (int i = 0; i < CTAS; ++i) s += sh->squares[i];
-    const double scale = static_cast<double>(SCALE) / (sqrt(s) + static_cast<double>(args.eps));
+            for (int j = 0; j < 8; ++j) put_raw(line[k], at[k] + j, e[k][j]);
+          } else {
+            uint32_t h[4], l[4];
 #pragma unroll
-    for (int k = 0; k < ITEMS; ++k) {
-      const int i = tid + k * THREADS;
-      if (i < items) {
-        int line, at;
-        item(i, &line, &at);
-        float v[8];
-#pragma unroll
-        for (int j = 0; j < 8; ++j) v[j] = static_cast<float>(to_f32(e[k][j]) * scale);
-        if (!args.tall) {  // what is behind the last column is 0
-          uint4 h, l;
-          split8(v, &h, &l);
-          *reinterpret_cast<uint4*>(x_hi + piece(line, at >> 3)) = h;
-          *reinterpret_cast<uint4*>(x_lo + piece(line, at >> 3)) = l;
-        } else {
-#pragma unroll
-          for (int j = 0; j < 8; ++j) {
-            if (at + j < length) {
-              const __half h = __float2half_rn(v[j]);
-              const uint32_t to = piece(at + j, line >> 3) + (line & 7) * 2;
-              *reinterpret_cast<__half*>(x_hi + to) = h;
-              *reinterpret_cast<__half*>(x_lo + to) = __float2half_rn(v[j] - __half2float(h));
+            for (int j = 0; j < 4; ++j) {
+              const uint32_t u = __float_as_uint(to_f32(e[k][2 * j])), v = __float_as_uint(to_f32(e[k][2 * j + 1]));
+              h[j] = __byte_perm(u, v, 0x7632);
+              l[j] = __byte_perm(u, v, 0x5410);
             }
+            *reinterpret_cast<uint4*>(x_hi + piece(line[k], at[k] >> 3)) = make_uint4(h[0], h[1], h[2], h[3]);
+            *reinterpret_cast<uint4*>(x_lo + piece(line[k], at[k] >> 3)) = make_uint4(l[0], l[1], l[2], l[3]);
           }
         }
+    }
+  } else {
+    // a warp's elements: 16 lines of 256, or (x transposed) 32 of 128
+    const int shift = args.tall ? 2 : 3;
+    for (int q0 = 0; warp + 8 * (q0 >> shift) < lines; q0 += 32) {
+      T e[32];
+#pragma unroll
+      for (int q = 0; q < 32; ++q) {
+        const int line = warp + 8 * ((q0 + q) >> shift), at = lane + 32 * ((q0 + q) & ((1 << shift) - 1));
+        e[q] = line < lines && at < length ? x[line * args.ld + at] : from_f32<T>(0.0f);
+      }
+#pragma unroll
+      for (int q = 0; q < 32; ++q) {
+        const int line = warp + 8 * ((q0 + q) >> shift), at = lane + 32 * ((q0 + q) & ((1 << shift) - 1));
+        square_of(e[q]);
+        if (line < lines && at < length) put_raw(line, at, e[q]);
       }
     }
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+  if (lane == 0) sh->warp_sums[warp] = s;
+  __syncthreads();
+  if (CTAS > 1) cluster_sync();  // every CTA runs: its shared memory can be written
+  if (tid < CTAS) {
+    s = 0.0;
+    for (int i = 0; i < THREADS / 32; ++i) s += sh->warp_sums[i];
+    asm volatile("st.shared::cluster.f64 [%0], %1;" ::"r"(mapa_shared(smem_u32(&sh->squares[rank]), tid)), "d"(s) : "memory");
+  }
+  all_sync();
+  s = 0.0;
+  for (int i = 0; i < CTAS; ++i) s += sh->squares[i];
+  const double scale = static_cast<double>(SCALE) / (sqrt(s) + static_cast<double>(args.eps));
+  const int pieces = tiles * 8;
+  for (int i = tid; i < args.rows * pieces; i += THREADS) {
+    const uint32_t at = piece(i / pieces, i % pieces);
+    uint4* hi = reinterpret_cast<uint4*>(x_hi + at);
+    uint4* lo = reinterpret_cast<uint4*>(x_lo + at);
+    const uint32_t h[4] = {hi->x, hi->y, hi->z, hi->w}, l[4] = {lo->x, lo->y, lo->z, lo->w};
+    float v[8];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      v[2 * j] = static_cast<float>(__uint_as_float(__byte_perm(l[j], h[j], 0x5410)) * scale);
+      v[2 * j + 1] = static_cast<float>(__uint_as_float(__byte_perm(l[j], h[j], 0x7632)) * scale);
+    }
+    split8(v, hi, lo);
   }
   local_sync();
 
@@ -251,18 +277,19 @@ __global__ void __launch_bounds__(THREADS, 1) ortho_small_kernel(const Args args
     ++phase;
     tc_fence_after();
   };
-  constexpr uint32_t SQUARE = idesc_f16_f32(ROWS, ROWS, 0, 0);
-  const uint32_t wide = idesc_f16_f32(ROWS, static_cast<uint32_t>(args.width), 0, 1);
-  // A B^T (planes with K along the rows, `n` tiles): the small products first
+  // Products stop at the last 16 rows and columns that hold anything; what the
+  // planes get behind those is never read.
+  const int k_rows = (args.rows + 15) / 16, k_cols = max(1, (cols + 15) / 16);  // of 16
+  const uint32_t square_d = idesc_f16_f32(ROWS, 16 * static_cast<uint32_t>(k_rows), 0, 0);
+  const uint32_t wide_d = idesc_f16_f32(ROWS, 16 * static_cast<uint32_t>(k_cols), 0, 1);
+  // A A^T (K along the planes' rows, `n` times 16): the small products first
   auto square = [&](const uint8_t* hi, const uint8_t* lo, int n) {
     if (warp == 0 && elect_one()) {
       const uint64_t h = sdesc_kmajor_sw128(smem_u32(hi)), l = sdesc_kmajor_sw128(smem_u32(lo));
       for (int p = 0; p < 3; ++p)
-        for (int t = 0; t < n; ++t) {
-          const uint32_t at = t * (TILE >> 4);
-#pragma unroll
-          for (int j = 0; j < 4; ++j)
-            mma_f16_ss(tmem, (p == 0 ? l : h) + at + 2 * j, (p == 1 ? l : h) + at + 2 * j, SQUARE, (p | t | j) != 0);
+        for (int k = 0; k < n; ++k) {
+          const uint32_t at = (k >> 2) * (TILE >> 4) + 2 * (k & 3);
+          mma_f16_ss(tmem, (p == 0 ? l : h) + at, (p == 1 ? l : h) + at, square_d, (p | k) != 0);
         }
       tc_commit(&sh->done);
     }
@@ -271,12 +298,13 @@ __global__ void __launch_bounds__(THREADS, 1) ortho_small_kernel(const Args args
 
   if constexpr (CTAS > 1) cluster_arrive();
   for (int step = 0; step < args.steps; ++step) {
-    square(x_hi, x_lo, tiles);
+    square(x_hi, x_lo, k_cols);
     wait_products();
     if constexpr (CTAS == 1) {
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
         const int c = half * 64 + i * 32;
+        if (c >= 16 * k_rows) break;
         uint32_t r[32];
         tmem_ld32p(t_row + c, r);
         tmem_wait_fence<1>(r);
@@ -302,6 +330,7 @@ __global__ void __launch_bounds__(THREADS, 1) ortho_small_kernel(const Args args
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
         const int c = half * 64 + i * 32;
+        if (c >= 16 * k_rows) break;
         uint32_t r[32];
         tmem_ld32p(t_row + c, r);
         tmem_wait_fence<1>(r);
@@ -354,11 +383,12 @@ __global__ void __launch_bounds__(THREADS, 1) ortho_small_kernel(const Args args
       tc_fence_after();
     }
 
-    square(g_hi, g_lo, 2);
+    square(g_hi, g_lo, k_rows);
     wait_products();
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
       const int c = half * 64 + i * 32;
+      if (c >= 16 * k_rows) break;
       uint32_t r[32];
       tmem_ld32p(t_row + c, r);
       tmem_wait_fence<1>(r);
@@ -375,21 +405,20 @@ __global__ void __launch_bounds__(THREADS, 1) ortho_small_kernel(const Args args
     }
     local_sync();
 
-    if (warp == 0 && elect_one()) {  // B X: K = 128 rows of X
+    if (warp == 0 && elect_one()) {  // B X: K down the rows of X
       const uint64_t bh = sdesc_kmajor_sw128(smem_u32(g_hi)), bl = sdesc_kmajor_sw128(smem_u32(g_lo));
       const uint64_t xh = sdesc_mnmajor_sw128(smem_u32(x_hi), TILE, 1024);
       const uint64_t xl = sdesc_mnmajor_sw128(smem_u32(x_lo), TILE, 1024);
       for (int p = 0; p < 3; ++p)
-#pragma unroll
-        for (int k = 0; k < 8; ++k)
+        for (int k = 0; k < k_rows; ++k)
           mma_f16_ss(tmem, (p == 0 ? bl : bh) + (k >> 2) * (TILE >> 4) + 2 * (k & 3), (p == 1 ? xl : xh) + k * (2048 >> 4),
-                     wide, (p | k) != 0);
+                     wide_d, (p | k) != 0);
       tc_commit(&sh->done);
     }
     __syncwarp();
     wait_products();
     if (CTAS > 1 && step + 1 < args.steps) cluster_arrive();
-    for (int c = half * 32; c < args.width; c += 64) {
+    for (int c = half * 32; c < 16 * k_cols; c += 64) {
       uint32_t r[32];
       tmem_ld32p(t_row + c, r);
       tmem_wait_fence<1>(r);
@@ -410,34 +439,38 @@ __global__ void __launch_bounds__(THREADS, 1) ortho_small_kernel(const Args args
   // ------------------------------------------------------------ result
   T* out = static_cast<T*>(args.out) + static_cast<int64_t>(matrix) * args.m * args.n +
            (args.tall ? static_cast<int64_t>(col0) * args.n : col0);
+  auto get = [&](int r, int c) {
+    const uint32_t from = piece(r, c >> 3) + (c & 7) * 2;
+    return (__half2float(*reinterpret_cast<const __half*>(x_hi + from)) +
+            __half2float(*reinterpret_cast<const __half*>(x_lo + from))) * (1.0f / SCALE);
+  };
+  if (!args.out_wide) {
+    for (int line = warp; line < lines; line += THREADS / 32)
+#pragma unroll 4
+      for (int at = lane; at < length; at += 32)
+        out[static_cast<int64_t>(line) * args.n + at] = from_f32<T>(args.tall ? get(at, line) : get(line, at));
+  } else {
 #pragma unroll 2
-  for (int i = tid; i < items; i += THREADS) {
-    int line, at;
-    item(i, &line, &at);
-    float v[8];
-    if (!args.tall) {
-      join8(*reinterpret_cast<const uint4*>(x_hi + piece(line, at >> 3)),
-            *reinterpret_cast<const uint4*>(x_lo + piece(line, at >> 3)), v);
-    } else {
+    for (int i = tid; i < items; i += THREADS) {
+      int line, at;
+      item(i, &line, &at);
+      float v[8];
+      if (!args.tall) {
+        join8(*reinterpret_cast<const uint4*>(x_hi + piece(line, at >> 3)),
+              *reinterpret_cast<const uint4*>(x_lo + piece(line, at >> 3)), v);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const uint32_t from = piece(at + j, line >> 3) + (line & 7) * 2;  // row below 128 in any case
-        v[j] = __half2float(*reinterpret_cast<const __half*>(x_hi + from)) +
-               __half2float(*reinterpret_cast<const __half*>(x_lo + from));
+        for (int j = 0; j < 8; ++j) v[j] *= 1.0f / SCALE;
+      } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] = get(at + j, line);
       }
-    }
-    T e[8];
+      T e[8];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) e[j] = from_f32<T>(v[j] * (1.0f / SCALE));
-    T* p = out + static_cast<int64_t>(line) * args.n + at;
-    if (args.out_wide) {
+      for (int j = 0; j < 8; ++j) e[j] = from_f32<T>(v[j]);
+      T* p = out + static_cast<int64_t>(line) * args.n + at;
 #pragma unroll
       for (int j = 0; j < static_cast<int>(sizeof(T)) / 2; ++j)
         reinterpret_cast<uint4*>(p)[j] = reinterpret_cast<const uint4*>(e)[j];
-    } else {
-#pragma unroll
-      for (int j = 0; j < 8; ++j)
-        if (at + j < length) p[j] = e[j];
     }
   }
   // (the last writes between CTAs were G, before the step's last barrier)
