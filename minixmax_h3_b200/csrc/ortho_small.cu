@@ -17,6 +17,8 @@
 //
 // Planes hold SCALE times the value, as in ortho.cu; the result is read back
 // from them (22 bits) so that it leaves in whole rows.
+#include <type_traits>
+
 #include "h3b_common.cuh"
 #include "h3b_host.hpp"
 #include "ortho.hpp"
@@ -173,8 +175,8 @@ __global__ void __launch_bounds__(THREADS, 1) ortho_small_kernel(const Args args
       *at = (i - *line * per_line) * 8;
     }
   };
-  auto put_raw = [&](int line, int at, T v) {
-    const uint32_t to = args.tall ? piece(at, line >> 3) + (line & 7) * 2 : piece(line, at >> 3) + (at & 7) * 2;
+  auto put_raw = [&](int r, int c, T v) {
+    const uint32_t to = piece(r, c >> 3) + (c & 7) * 2;
     const uint32_t bits = __float_as_uint(to_f32(v));
     *reinterpret_cast<uint16_t*>(x_hi + to) = static_cast<uint16_t>(bits >> 16);
     *reinterpret_cast<uint16_t*>(x_lo + to) = static_cast<uint16_t>(bits);
@@ -182,8 +184,8 @@ __global__ void __launch_bounds__(THREADS, 1) ortho_small_kernel(const Args args
   // zero planes: rows and columns behind the matrix stay so
   for (int i = tid; i < tiles * TILE * 2 / 16; i += THREADS) reinterpret_cast<uint4*>(x_hi)[i] = make_uint4(0, 0, 0, 0);
   __syncthreads();
-  double s = 0.0;
-  auto square_of = [&](T v) { s = fma(static_cast<double>(to_f32(v)), static_cast<double>(to_f32(v)), s); };
+  double sums[2] = {0.0, 0.0};  // 64 bits: a 32-bit square of 10^-20 is nothing
+  auto square_of = [&](T v, int i) { sums[i] = fma(static_cast<double>(to_f32(v)), static_cast<double>(to_f32(v)), sums[i]); };
   x += args.tall ? col0 * args.ld : col0;
   if (args.wide) {
     for (int i0 = tid; i0 < items; i0 += 4 * THREADS) {
@@ -204,10 +206,10 @@ __global__ void __launch_bounds__(THREADS, 1) ortho_small_kernel(const Args args
       for (int k = 0; k < 4; ++k)
         if (i0 + k * THREADS < items) {
 #pragma unroll
-          for (int j = 0; j < 8; ++j) square_of(e[k][j]);
+          for (int j = 0; j < 8; ++j) square_of(e[k][j], j & 1);
           if (args.tall) {
 #pragma unroll
-            for (int j = 0; j < 8; ++j) put_raw(line[k], at[k] + j, e[k][j]);
+            for (int j = 0; j < 8; ++j) put_raw(at[k] + j, line[k], e[k][j]);
           } else {
             uint32_t h[4], l[4];
 #pragma unroll
@@ -222,23 +224,38 @@ __global__ void __launch_bounds__(THREADS, 1) ortho_small_kernel(const Args args
         }
     }
   } else {
-    // a warp's elements: 16 lines of 256, or (x transposed) 32 of 128
-    const int shift = args.tall ? 2 : 3;
-    for (int q0 = 0; warp + 8 * (q0 >> shift) < lines; q0 += 32) {
-      T e[32];
+    auto rows_of_x = [&](auto transposed, auto across) {  // rows of 32 * across elements at most
+      constexpr bool T_ = decltype(transposed)::value;
+      constexpr int N = decltype(across)::value, L = 32 / N;
+      for (int line0 = warp; line0 < lines; line0 += 8 * L) {
+        T e[L][N];
 #pragma unroll
-      for (int q = 0; q < 32; ++q) {
-        const int line = warp + 8 * ((q0 + q) >> shift), at = lane + 32 * ((q0 + q) & ((1 << shift) - 1));
-        e[q] = line < lines && at < length ? x[line * args.ld + at] : from_f32<T>(0.0f);
-      }
+        for (int l = 0; l < L; ++l) {
+          const int line = line0 + 8 * l;
+          const T* p = x + line * args.ld + lane;
 #pragma unroll
-      for (int q = 0; q < 32; ++q) {
-        const int line = warp + 8 * ((q0 + q) >> shift), at = lane + 32 * ((q0 + q) & ((1 << shift) - 1));
-        square_of(e[q]);
-        if (line < lines && at < length) put_raw(line, at, e[q]);
+          for (int j = 0; j < N; ++j) e[l][j] = line < lines && lane + 32 * j < length ? p[32 * j] : from_f32<T>(0.0f);
+        }
+#pragma unroll
+        for (int l = 0; l < L; ++l)
+#pragma unroll
+          for (int j = 0; j < N; ++j) square_of(e[l][j], j & 1);
+#pragma unroll
+        for (int l = 0; l < L; ++l) {
+          const int line = line0 + 8 * l;
+#pragma unroll
+          for (int j = 0; j < N; ++j)
+            if (line < lines && lane + 32 * j < length)
+              put_raw(T_ ? lane + 32 * j : line, T_ ? line : lane + 32 * j, e[l][j]);
+        }
       }
-    }
+    };
+    if (args.tall)
+      rows_of_x(std::true_type{}, std::integral_constant<int, ROWS / 32>{});
+    else
+      rows_of_x(std::false_type{}, std::integral_constant<int, MAX_W / 32>{});
   }
+  double s = sums[0] + sums[1];
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
   if (lane == 0) sh->warp_sums[warp] = s;
@@ -252,7 +269,12 @@ __global__ void __launch_bounds__(THREADS, 1) ortho_small_kernel(const Args args
   all_sync();
   s = 0.0;
   for (int i = 0; i < CTAS; ++i) s += sh->squares[i];
-  const double scale = static_cast<double>(SCALE) / (sqrt(s) + static_cast<double>(args.eps));
+  // x * SCALE / (norm + eps), as a factor below 2 and two powers of two (one
+  // would leave the range of 32 bits)
+  const double divisor = sqrt(s) + static_cast<double>(args.eps);
+  const int e = divisor > 0.0 && divisor < 1e300 ? ilogb(divisor) : 0;
+  const float f = static_cast<float>(static_cast<double>(SCALE) * scalbn(1.0, e) / divisor);
+  const float s1 = ldexpf(1.0f, -e / 2), s2 = ldexpf(1.0f, -e + e / 2);
   const int pieces = tiles * 8;
   for (int i = tid; i < args.rows * pieces; i += THREADS) {
     const uint32_t at = piece(i / pieces, i % pieces);
@@ -262,8 +284,8 @@ __global__ void __launch_bounds__(THREADS, 1) ortho_small_kernel(const Args args
     float v[8];
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      v[2 * j] = static_cast<float>(__uint_as_float(__byte_perm(l[j], h[j], 0x5410)) * scale);
-      v[2 * j + 1] = static_cast<float>(__uint_as_float(__byte_perm(l[j], h[j], 0x7632)) * scale);
+      v[2 * j] = __uint_as_float(__byte_perm(l[j], h[j], 0x5410)) * s1 * s2 * f;
+      v[2 * j + 1] = __uint_as_float(__byte_perm(l[j], h[j], 0x7632)) * s1 * s2 * f;
     }
     split8(v, hi, lo);
   }
@@ -445,10 +467,20 @@ __global__ void __launch_bounds__(THREADS, 1) ortho_small_kernel(const Args args
             __half2float(*reinterpret_cast<const __half*>(x_lo + from))) * (1.0f / SCALE);
   };
   if (!args.out_wide) {
-    for (int line = warp; line < lines; line += THREADS / 32)
-#pragma unroll 4
-      for (int at = lane; at < length; at += 32)
-        out[static_cast<int64_t>(line) * args.n + at] = from_f32<T>(args.tall ? get(at, line) : get(line, at));
+    auto rows_of_x = [&](auto transposed, auto across) {
+      constexpr bool T_ = decltype(transposed)::value;
+#pragma unroll 2
+      for (int line = warp; line < lines; line += THREADS / 32) {
+        T* p = out + static_cast<int64_t>(line) * args.n + lane;
+#pragma unroll
+        for (int j = 0; j < decltype(across)::value; ++j)
+          if (lane + 32 * j < length) p[32 * j] = from_f32<T>(T_ ? get(lane + 32 * j, line) : get(line, lane + 32 * j));
+      }
+    };
+    if (args.tall)
+      rows_of_x(std::true_type{}, std::integral_constant<int, ROWS / 32>{});
+    else
+      rows_of_x(std::false_type{}, std::integral_constant<int, MAX_W / 32>{});
   } else {
 #pragma unroll 2
     for (int i = tid; i < items; i += THREADS) {
