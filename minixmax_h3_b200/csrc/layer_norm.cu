@@ -5,9 +5,9 @@
 //   dw = sum_rows dy xhat,   db = sum_rows dy
 //
 // Both directions are bound by HBM: x is read and y written once; backward, x
-// and dy are read and dx written once.  A group of threads holds a row in
-// registers (forward 32 elements a thread at most, backward 16), so the
-// variance is taken about the mean in a second pass over registers, and what
+// and dy are read and dx written once.  Arithmetic is packed, two elements an
+// instruction, or it would bind first.  A group of threads holds a row in
+// registers, so the variance is taken about the mean in a second pass over registers, and what
 // rounding the mean left over is taken off with it: var = mean(d^2) -
 // mean(d)^2, d = x - mean, with mean(d) of the size of a rounding.
 //
@@ -16,6 +16,8 @@
 // adds its groups' sums in order through shared memory and writes one partial
 // row; a second launch adds the partial rows of a column in order.  No
 // atomics: results do not depend on scheduling.
+#include <type_traits>
+
 #include "h3b_common.cuh"
 #include "h3b_host.hpp"
 
@@ -56,20 +58,68 @@ H3B_DEV void store_pack(T* p, const Pack<T, VEC>& r) {
   else
     *reinterpret_cast<uint4*>(p) = *reinterpret_cast<const uint4*>(r.e);
 }
-// VEC values of the weight's type WT (float beside a 16-bit T takes two words).
-template <class WT, int VEC>
-H3B_DEV void load_weights(const WT* p, float (&v)[VEC]) {
-  if constexpr (VEC == 1) {
-    v[0] = to_f32(*p);
+// Pairs of elements, for packed fp32 arithmetic.
+H3B_DEV float2 pair_of(uint32_t w, __nv_bfloat16) { return make_float2(bf16lo_to_f32(w), bf16hi_to_f32(w)); }
+H3B_DEV float2 pair_of(uint32_t w, __half) { return __half22float2(*reinterpret_cast<const __half2*>(&w)); }
+template <class T, int VEC>
+H3B_DEV float2 get2(const Pack<T, VEC>& p, int i) {  // elements 2 i, 2 i + 1
+  if constexpr (sizeof(T) == 4)
+    return make_float2(p.e[2 * i], p.e[2 * i + 1]);
+  else
+    return pair_of(reinterpret_cast<const uint32_t*>(p.e)[i], T());
+}
+template <class T, int VEC>
+H3B_DEV void set2(Pack<T, VEC>& p, int i, float2 v) {
+  if constexpr (sizeof(T) == 4) {
+    p.e[2 * i] = v.x;
+    p.e[2 * i + 1] = v.y;
+  } else if constexpr (std::is_same<T, __half>::value) {
+    reinterpret_cast<uint32_t*>(p.e)[i] = pack_f16x2(v.x, v.y);
   } else {
-    constexpr int N = 16 / sizeof(WT);
-#pragma unroll
-    for (int i = 0; i < VEC; i += N) {
-      const Pack<WT, N> r = load_pack<WT, N>(p + i);
-#pragma unroll
-      for (int j = 0; j < N; ++j) v[i + j] = to_f32(r.e[j]);
-    }
+    reinterpret_cast<uint32_t*>(p.e)[i] = pack_bf16x2(v.x, v.y);
   }
+}
+H3B_DEV float2 both(float v) { return make_float2(v, v); }
+// Pair q of a thread's elements: of a vector, or of two vectors of one.
+template <class T, int VEC, int N>
+H3B_DEV float2 pair_at(const Pack<T, VEC> (&v)[N], int q) {
+  if constexpr (VEC == 1)
+    return make_float2(to_f32(v[2 * q].e[0]), to_f32(v[2 * q + 1].e[0]));
+  else
+    return get2(v[2 * q / VEC], 2 * q % VEC / 2);
+}
+template <class T, int VEC, int N>
+H3B_DEV void set_pair(Pack<T, VEC> (&v)[N], int q, float2 x) {
+  if constexpr (VEC == 1) {
+    v[2 * q].e[0] = from_f32<T>(x.x);
+    v[2 * q + 1].e[0] = from_f32<T>(x.y);
+  } else {
+    set2(v[2 * q / VEC], 2 * q % VEC / 2, x);
+  }
+}
+
+// VEC weights of type WT (float beside a 16-bit T takes two words).
+template <class WT, int VEC>
+struct Weights {
+  static constexpr int N = VEC == 1 ? 1 : 16 / sizeof(WT);
+  Pack<WT, N> p[VEC / N];
+  H3B_DEV void load(const WT* at) {
+#pragma unroll
+    for (int i = 0; i < VEC / N; ++i) p[i] = load_pack<WT, N>(at + i * N);
+  }
+  H3B_DEV void fill(float v) {
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) p[i / N].e[i % N] = from_f32<WT>(v);
+  }
+  H3B_DEV float operator[](int i) const { return to_f32(p[i / N].e[i % N]); }
+  H3B_DEV float2 pair(int i) const { return get2(p[2 * i / N], 2 * i % N / 2); }
+};
+template <class WT, int VEC, int N>
+H3B_DEV float2 pair_at(const Weights<WT, VEC> (&w)[N], int q) {
+  if constexpr (VEC == 1)
+    return make_float2(w[2 * q][0], w[2 * q + 1][0]);
+  else
+    return w[2 * q / VEC].pair(2 * q % VEC / 2);
 }
 
 // Sums of two values over a group of TPR threads (a row), the same in all of
@@ -104,7 +154,42 @@ struct RowSum {
   }
 };
 
+// Both sums of each of N rows over their group of TPR threads, behind one
+// barrier; `slots` are used by every other call.
+template <int TPR, int N>
+H3B_DEV void row_sums(float (&a)[N], float (&b)[N], float2 (*slots)[32]) {
+  constexpr int W = TPR < 32 ? TPR : 32;
+#pragma unroll
+  for (int o = W / 2; o > 0; o >>= 1)
+#pragma unroll
+    for (int k = 0; k < N; ++k) {
+      a[k] += __shfl_xor_sync(0xffffffffu, a[k], o);
+      b[k] += __shfl_xor_sync(0xffffffffu, b[k], o);
+    }
+  if constexpr (TPR > 32) {
+    if ((threadIdx.x & 31) == 0)
+#pragma unroll
+      for (int k = 0; k < N; ++k) slots[k][threadIdx.x >> 5] = make_float2(a[k], b[k]);
+    __syncthreads();
+    const int first = threadIdx.x / TPR * (TPR / 32);
+#pragma unroll
+    for (int k = 0; k < N; ++k) {
+      a[k] = b[k] = 0.0f;
+#pragma unroll
+      for (int i = 0; i < TPR / 32; ++i) {
+        const float2 t = slots[k][first + i];
+        a[k] += t.x;
+        b[k] += t.y;
+      }
+    }
+  }
+}
+
+template <int N>
+H3B_DEV float half_of(const float2 (&p)[N], int j) { return j & 1 ? p[j / 2].y : p[j / 2].x; }
+
 // Rows of a warp or less share a CTA; larger groups are a CTA (RowSum).
+constexpr int EPT = 16;  // elements of a row that a thread holds, backward
 constexpr int block_threads(int tpr) { return tpr <= 32 ? 128 : tpr; }
 
 // From mean(d^2) and mean(d).  A rounding must not leave less than nothing; a
@@ -124,9 +209,10 @@ struct FwdArgs {
   float eps;
 };
 
-template <class T, class WT, int VEC, int TPR>
+// TPR threads a row, HELD elements a thread at most.
+template <class T, class WT, int VEC, int TPR, int HELD>
 __global__ void __launch_bounds__(block_threads(TPR)) ln_fwd_kernel(const FwdArgs a) {
-  constexpr int MAXV = 32 / VEC;
+  constexpr int MAXV = HELD / VEC;
   constexpr int GROUPS = block_threads(TPR) / TPR;
   __shared__ float2 slots[2][32];
   RowSum<TPR> sum{slots};
@@ -139,29 +225,41 @@ __global__ void __launch_bounds__(block_threads(TPR)) ln_fwd_kernel(const FwdArg
   const float inv_n = 1.0f / static_cast<float>(n);
 
   Pack<T, VEC> v[MAXV];
-  float s = 0.0f;
 #pragma unroll
   for (int i = 0; i < MAXV; ++i) {
     const int c = t + i * TPR;
     if (c < nv) v[i] = load_pack<T, VEC>(x + static_cast<int64_t>(c) * VEC);
   }
+  float2 s = both(0.0f);
 #pragma unroll
   for (int i = 0; i < MAXV; ++i)
-    if (t + i * TPR < nv)
+    if (t + i * TPR < nv) {
+      if constexpr (VEC == 1) {
+        s.x += to_f32(v[i].e[0]);
+      } else {
 #pragma unroll
-      for (int j = 0; j < VEC; ++j) s += to_f32(v[i].e[j]);
-  const float m0 = sum(s, 0.0f).x * inv_n;
-  float s1 = 0.0f, s2 = 0.0f;
-#pragma unroll
-  for (int i = 0; i < MAXV; ++i)
-    if (t + i * TPR < nv)
-#pragma unroll
-      for (int j = 0; j < VEC; ++j) {
-        const float d = to_f32(v[i].e[j]) - m0;
-        s1 += d;
-        s2 = fmaf(d, d, s2);
+        for (int j = 0; j < VEC / 2; ++j) s = add2(s, get2(v[i], j));
       }
-  const float2 r = sum(s1, s2);
+    }
+  const float m0 = sum(s.x + s.y, 0.0f).x * inv_n;
+  float2 s1 = both(0.0f), s2 = both(0.0f);
+#pragma unroll
+  for (int i = 0; i < MAXV; ++i)
+    if (t + i * TPR < nv) {
+      if constexpr (VEC == 1) {
+        const float d = to_f32(v[i].e[0]) - m0;
+        s1.x += d;
+        s2.x = fmaf(d, d, s2.x);
+      } else {
+#pragma unroll
+        for (int j = 0; j < VEC / 2; ++j) {
+          const float2 d = add2(get2(v[i], j), both(-m0));
+          s1 = add2(s1, d);
+          s2 = fma2(d, d, s2);
+        }
+      }
+    }
+  const float2 r = sum(s1.x + s1.y, s2.x + s2.y);
   const float dm = r.x * inv_n;
   const float rstd = inverse_std(r.y * inv_n, dm, a.eps);
   if (!live) return;
@@ -172,19 +270,29 @@ __global__ void __launch_bounds__(block_threads(TPR)) ln_fwd_kernel(const FwdArg
   T* y = static_cast<T*>(a.y) + row * a.ldy;
   const WT* w = static_cast<const WT*>(a.w);
   const WT* b = static_cast<const WT*>(a.b);
+  const float shift = -dm * rstd;
 #pragma unroll
   for (int i = 0; i < MAXV; ++i) {
     const int c = t + i * TPR;
     if (c < nv) {
-      float wv[VEC], bv[VEC];
-      if (w != nullptr) load_weights<WT, VEC>(w + c * VEC, wv);
-      if (b != nullptr) load_weights<WT, VEC>(b + c * VEC, bv);
+      Weights<WT, VEC> wv, bv;
+      if (w != nullptr) wv.load(w + c * VEC);
+      if (b != nullptr) bv.load(b + c * VEC);
+      if constexpr (VEC == 1) {
+        float h = fmaf(to_f32(v[i].e[0]) - m0, rstd, shift);
+        if (w != nullptr) h *= wv[0];
+        if (b != nullptr) h += bv[0];
+        v[i].e[0] = from_f32<T>(h);
+      } else {
 #pragma unroll
-      for (int j = 0; j < VEC; ++j) {
-        float h = ((to_f32(v[i].e[j]) - m0) - dm) * rstd;
-        if (w != nullptr) h *= wv[j];
-        if (b != nullptr) h += bv[j];
-        v[i].e[j] = from_f32<T>(h);
+        for (int j = 0; j < VEC / 2; ++j) {
+          float2 h = fma2(add2(get2(v[i], j), both(-m0)), both(rstd), both(shift));
+          if (b != nullptr)  // comes with a weight
+            h = fma2(h, wv.pair(j), bv.pair(j));
+          else if (w != nullptr)
+            h = mul2(h, wv.pair(j));
+          set2(v[i], j, h);
+        }
       }
       store_pack<T, VEC>(y + static_cast<int64_t>(c) * VEC, v[i]);
     }
@@ -236,82 +344,111 @@ struct BwdArgs {
   int sums;        // write partials
 };
 
+// Backward, groups of any size share a CTA of 256 threads: their sums of the
+// columns are joined before they are written.  Two such CTAs an SM (three and
+// four, with fewer registers each, are slower).
+constexpr int bwd_threads(int tpr) { return tpr < 256 ? 256 : tpr; }
+constexpr int bwd_ctas_per_sm(int tpr) { return bwd_threads(tpr) == 256 ? 2 : 1; }
+
 template <class T, class WT, int VEC, int TPR>
-__global__ void __launch_bounds__(block_threads(TPR)) ln_bwd_kernel(const BwdArgs a) {
-  constexpr int MAXV = 16 / VEC;
-  constexpr int THREADS = block_threads(TPR);
+__global__ void __launch_bounds__(bwd_threads(TPR), VEC > 1 ? bwd_ctas_per_sm(TPR) : 1) ln_bwd_kernel(const BwdArgs a) {
+  constexpr int MAXV = EPT / VEC;
+  constexpr int THREADS = bwd_threads(TPR);
   constexpr int GROUPS = THREADS / TPR;
-  __shared__ float2 slots[2][32];
+  // Rows that a group works on together, their loads in flight and their sums
+  // behind one barrier: two of 16 bits (16384 x 4096 in 96 us, one 111), one
+  // of 32 (8192 x 4096 in 82 us, two 96).  CTAs of 1024 threads have 64
+  // registers a thread: one row, and the weights again for each (from L1).
+  constexpr bool SMALL = THREADS == 1024;
+  constexpr int ROWS = SMALL || sizeof(T) == 4 || VEC == 1 ? 1 : 2;
+  __shared__ float2 slots[2][ROWS][32];
   // groups' sums meet here (only groups of less than a CTA)
-  __shared__ float2 joined[GROUPS > 1 ? TPR * 16 : 1];
-  RowSum<TPR> sum{slots};
+  __shared__ float2 joined[GROUPS > 1 ? TPR * EPT : 1];
   const int t = threadIdx.x % TPR, group = threadIdx.x / TPR;
   const int n = static_cast<int>(a.n);
   const int nv = (n + VEC - 1) / VEC;
   const float inv_n = 1.0f / static_cast<float>(n);
   const WT* w = static_cast<const WT*>(a.w);
 
-  float wv[MAXV][VEC];
-  float sw[MAXV][VEC], sb[MAXV][VEC];
+  Weights<WT, VEC> wv[MAXV];
+  auto load_weights = [&] {
 #pragma unroll
-  for (int i = 0; i < MAXV; ++i) {
+    for (int i = 0; i < MAXV; ++i) {
+      const int c = t + i * TPR;
+      wv[i].fill(c < nv ? 1.0f : 0.0f);  // beyond the row there is nothing
+      if (w != nullptr && c < nv) wv[i].load(w + c * VEC);
+    }
+  };
+  if (!SMALL) load_weights();
+  constexpr int PAIRS = EPT / 2;
+  float2 sw[PAIRS], sb[PAIRS];
 #pragma unroll
-    for (int j = 0; j < VEC; ++j) wv[i][j] = 1.0f, sw[i][j] = sb[i][j] = 0.0f;
-    const int c = t + i * TPR;
-    if (w != nullptr && c < nv) load_weights<WT, VEC>(w + c * VEC, wv[i]);
-  }
+  for (int q = 0; q < PAIRS; ++q) sw[q] = sb[q] = both(0.0f);
+  int set = 0;
   // Every group of the CTA makes the same number of rounds (the row sums need
   // whole warps); one without a row adds zeros and writes nothing.
   const int64_t step = static_cast<int64_t>(gridDim.x) * GROUPS;
-  for (int64_t base = static_cast<int64_t>(blockIdx.x) * GROUPS; base < a.m; base += step) {
-    const int64_t row = base + group;
-    const bool live = row < a.m;
-    Pack<T, VEC> vx[MAXV], vg[MAXV];
-    float mean = 0.0f, rstd = 0.0f;
-    if (live) {
+  for (int64_t base = static_cast<int64_t>(blockIdx.x) * GROUPS; base < a.m; base += ROWS * step) {
+    Pack<T, VEC> vx[ROWS][MAXV], vg[ROWS][MAXV];
+    float rstd[ROWS], shift[ROWS];
+    bool live[ROWS];
+#pragma unroll
+    for (int k = 0; k < ROWS; ++k) {
+      const int64_t row = base + k * step + group;
+      live[k] = row < a.m;
+      rstd[k] = shift[k] = 0.0f;
       const T* x = static_cast<const T*>(a.x) + row * a.ldx;
       const T* dy = static_cast<const T*>(a.dy) + row * a.lddy;
 #pragma unroll
       for (int i = 0; i < MAXV; ++i) {
         const int c = t + i * TPR;
-        if (c < nv) {
-          vx[i] = load_pack<T, VEC>(x + static_cast<int64_t>(c) * VEC);
-          vg[i] = load_pack<T, VEC>(dy + static_cast<int64_t>(c) * VEC);
+        if (live[k] && c < nv) {
+          vx[k][i] = load_pack<T, VEC>(x + static_cast<int64_t>(c) * VEC);
+          vg[k][i] = load_pack<T, VEC>(dy + static_cast<int64_t>(c) * VEC);
+        } else {
+#pragma unroll
+          for (int j = 0; j < VEC; ++j) vx[k][i].e[j] = vg[k][i].e[j] = from_f32<T>(0.0f);
         }
       }
-      mean = a.mean[row];
-      rstd = a.rstd[row];
+      if (live[k]) {
+        shift[k] = -a.mean[row];
+        rstd[k] = a.rstd[row];
+      }
     }
-    float s1 = 0.0f, s2 = 0.0f;
+    if (SMALL) load_weights();
+    float s1[ROWS], s2[ROWS];
 #pragma unroll
-    for (int i = 0; i < MAXV; ++i)
-      if (live && t + i * TPR < nv)
+    for (int k = 0; k < ROWS; ++k) {
+      float2 p1 = both(0.0f), p2 = both(0.0f);
 #pragma unroll
-        for (int j = 0; j < VEC; ++j) {
-          const float xhat = (to_f32(vx[i].e[j]) - mean) * rstd;
-          const float d = to_f32(vg[i].e[j]);
-          const float g = d * wv[i][j];
-          s1 += g;
-          s2 = fmaf(g, xhat, s2);
-          sw[i][j] = fmaf(d, xhat, sw[i][j]);
-          sb[i][j] += d;
-        }
-    const float2 r = sum(s1, s2);
-    if (live) {
-      const float c1 = r.x * inv_n, c2 = r.y * inv_n;
-      T* dx = static_cast<T*>(a.dx) + row * a.lddx;
+      for (int q = 0; q < PAIRS; ++q) {
+        const float2 xhat = mul2(add2(pair_at(vx[k], q), both(shift[k])), both(rstd[k]));
+        const float2 d = pair_at(vg[k], q);
+        const float2 g = mul2(d, pair_at(wv, q));
+        p1 = add2(p1, g);
+        p2 = fma2(g, xhat, p2);
+        sw[q] = fma2(d, xhat, sw[q]);
+        sb[q] = add2(sb[q], d);
+      }
+      s1[k] = p1.x + p1.y;
+      s2[k] = p2.x + p2.y;
+    }
+    row_sums<TPR, ROWS>(s1, s2, slots[set]);
+    set ^= 1;
+#pragma unroll
+    for (int k = 0; k < ROWS; ++k) {
+      const float c1 = s1[k] * inv_n, c2 = s2[k] * inv_n;
+#pragma unroll
+      for (int q = 0; q < PAIRS; ++q) {
+        const float2 xhat = mul2(add2(pair_at(vx[k], q), both(shift[k])), both(rstd[k]));
+        const float2 g = mul2(pair_at(vg[k], q), pair_at(wv, q));
+        set_pair(vx[k], q, mul2(add2(fma2(xhat, both(-c2), g), both(-c1)), both(rstd[k])));
+      }
+      T* dx = static_cast<T*>(a.dx) + (base + k * step + group) * a.lddx;
 #pragma unroll
       for (int i = 0; i < MAXV; ++i) {
         const int c = t + i * TPR;
-        if (c < nv) {
-#pragma unroll
-          for (int j = 0; j < VEC; ++j) {
-            const float xhat = (to_f32(vx[i].e[j]) - mean) * rstd;
-            const float g = to_f32(vg[i].e[j]) * wv[i][j];
-            vx[i].e[j] = from_f32<T>(rstd * (fmaf(-xhat, c2, g) - c1));
-          }
-          store_pack<T, VEC>(dx + static_cast<int64_t>(c) * VEC, vx[i]);
-        }
+        if (live[k] && c < nv) store_pack<T, VEC>(dx + static_cast<int64_t>(c) * VEC, vx[k][i]);
       }
     }
   }
@@ -327,7 +464,7 @@ __global__ void __launch_bounds__(block_threads(TPR)) ln_bwd_kernel(const BwdArg
           for (int j = 0; j < VEC; ++j) {
             const int at = c * VEC + j;
             const float2 before = g == 0 ? make_float2(0.0f, 0.0f) : joined[at];
-            joined[at] = make_float2(before.x + sw[i][j], before.y + sb[i][j]);
+            joined[at] = make_float2(before.x + half_of(sw, i * VEC + j), before.y + half_of(sb, i * VEC + j));
           }
         }
       }
@@ -344,8 +481,8 @@ __global__ void __launch_bounds__(block_threads(TPR)) ln_bwd_kernel(const BwdArg
       if (c < nv)
 #pragma unroll
         for (int j = 0; j < VEC; ++j) {
-          out[c * VEC + j] = sw[i][j];
-          out[n + c * VEC + j] = sb[i][j];
+          out[c * VEC + j] = half_of(sw, i * VEC + j);
+          out[n + c * VEC + j] = half_of(sb, i * VEC + j);
         }
     }
   }
@@ -393,85 +530,87 @@ __global__ void __launch_bounds__(256) ln_bwd_long_sums_kernel(const BwdArgs a) 
   out[a.n + c] = sb;
 }
 
-// dw and db from the partial rows, in order: a warp reads 32 columns of every
-// eighth partial row, the CTA's eight warps' sums are added in order.
+// dw and db from the partial rows, in order: each of a CTA's 32 warps reads 32
+// columns of every 32nd partial row, the first one adds the warps' sums.
 template <class WT>
-__global__ void __launch_bounds__(256) ln_bwd_join_kernel(const float* partial, int ctas, int64_t n, WT* dw, WT* db) {
-  __shared__ float part[8][32];
+__global__ void __launch_bounds__(1024) ln_bwd_join_kernel(const float* partial, int ctas, int64_t n, WT* dw, WT* db) {
+  __shared__ float part[32][32];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int64_t c = static_cast<int64_t>(blockIdx.x) * 32 + lane;
-  const int64_t which = blockIdx.y;
+  const int64_t which = dw == nullptr ? 1 : blockIdx.y;
   float s = 0.0f;
   if (c < n)
-#pragma unroll 4
-    for (int p = warp; p < ctas; p += 8) s += partial[(static_cast<int64_t>(p) * 2 + which) * n + c];
+#pragma unroll 5
+    for (int p = warp; p < ctas; p += 32) s += partial[(static_cast<int64_t>(p) * 2 + which) * n + c];
   part[warp][lane] = s;
   __syncthreads();
-  WT* out = which == 0 ? dw : db;
-  if (warp == 0 && c < n && out != nullptr) {
+  if (warp == 0 && c < n) {
 #pragma unroll
-    for (int i = 1; i < 8; ++i) s += part[i][lane];
-    out[c] = from_f32<WT>(s);
+    for (int i = 1; i < 32; ++i) s += part[i][lane];
+    (which == 0 ? dw : db)[c] = from_f32<WT>(s);
   }
 }
 
 // ------------------------------------------------------------------- hosts
 
-// Threads a row of n elements takes at `ept` elements a thread.
-int row_threads(int64_t n, int ept) {
+// Threads that a row of n elements takes, backward.
+int row_threads(int64_t n) {
   for (int tpr : {8, 32, 64, 128, 256, 512, 1024})
-    if (n <= static_cast<int64_t>(tpr) * ept) return tpr;
+    if (n <= static_cast<int64_t>(tpr) * EPT) return tpr;
   return 0;  // longer
 }
 
 int element_bytes(int dtype) { return dtype == H3B_F32 ? 4 : 2; }
 
-// CTAs of a backward pass: two waves of 1024 threads an SM at most, so that a
-// CTA's partial row stands for many rows.
+// CTAs of a backward pass, each of which leaves a partial row.
 int64_t bwd_ctas(int64_t m, int64_t n) {
-  const int tpr = row_threads(n, 16);
+  const int tpr = row_threads(n);
   if (tpr == 0) {
     const int64_t most = 64;
     return m < most ? m : most;
   }
-  const int threads = block_threads(tpr);
-  const int64_t groups = threads / tpr;
-  const int64_t ctas = static_cast<int64_t>(h3b::num_sms()) * (threads >= 512 ? 1 : 512 / threads);
+  const int64_t groups = bwd_threads(tpr) / tpr;
+  const int64_t ctas = static_cast<int64_t>(h3b::num_sms()) * bwd_ctas_per_sm(tpr);
   const int64_t need = (m + groups - 1) / groups;
   return need < ctas ? need : ctas;
 }
 
 template <class T, class WT, int VEC>
 int run_fwd(const FwdArgs& a, cudaStream_t st) {
-  const int tpr = row_threads(a.n, 32);
-#define H3B_LN_FWD(TPR)                                                                              \
-  case TPR: {                                                                                        \
-    const int64_t groups = block_threads(TPR) / TPR, blocks = (a.m + groups - 1) / groups;           \
-    ln_fwd_kernel<T, WT, VEC, TPR><<<static_cast<unsigned>(blocks), block_threads(TPR), 0, st>>>(a); \
-    break;                                                                                           \
+#define H3B_LN_FWD(TPR, HELD)                                                                             \
+  if (a.n <= static_cast<int64_t>(TPR) * HELD) {                                                          \
+    constexpr int64_t groups = block_threads(TPR) / TPR;                                                  \
+    const unsigned blocks = static_cast<unsigned>((a.m + groups - 1) / groups);                           \
+    ln_fwd_kernel<T, WT, VEC, TPR, HELD><<<blocks, block_threads(TPR), 0, st>>>(a);                         \
+    return h3b::launch_status();                                                                          \
   }
-  switch (tpr) {
-    H3B_LN_FWD(8)
-    H3B_LN_FWD(32)
-    H3B_LN_FWD(64)
-    H3B_LN_FWD(128)
-    H3B_LN_FWD(256)
-    H3B_LN_FWD(512)
-    H3B_LN_FWD(1024)
-    default:
-      ln_fwd_long_kernel<T, WT><<<static_cast<unsigned>(a.m), 1024, 0, st>>>(a);
+  H3B_LN_FWD(8, 32)
+  H3B_LN_FWD(32, 32)
+  if constexpr (VEC > 1) {
+    // A warp a row needs no barriers, and its 8 or 16 KB are loads enough for
+    // its share of an SM (32768 x 4096 in 96 us, with four warps a row 119).
+    // Few rows would be a little quicker with more threads; a row's result
+    // does not depend on how many others there are.
+    H3B_LN_FWD(32, 64)
+    H3B_LN_FWD(32, 128)
   }
+  H3B_LN_FWD(64, 32)
+  H3B_LN_FWD(128, 32)
+  H3B_LN_FWD(256, 32)
+  H3B_LN_FWD(512, 32)
+  H3B_LN_FWD(1024, 32)
 #undef H3B_LN_FWD
+  ln_fwd_long_kernel<T, WT><<<static_cast<unsigned>(a.m), 1024, 0, st>>>(a);
   return h3b::launch_status();
 }
 
 template <class T, class WT, int VEC>
 int run_bwd(const BwdArgs& a, cudaStream_t st) {
-  const int tpr = row_threads(a.n, 16);
+  const int tpr = row_threads(a.n);
   const unsigned ctas = static_cast<unsigned>(bwd_ctas(a.m, a.n));
 #define H3B_LN_BWD(TPR)                                                        \
   case TPR:                                                                    \
-    ln_bwd_kernel<T, WT, VEC, TPR><<<ctas, block_threads(TPR), 0, st>>>(a);    \
+    ln_bwd_kernel<T, WT, VEC, TPR><<<ctas, bwd_threads(TPR), 0, st>>>(a);      \
     break;
   switch (tpr) {
     H3B_LN_BWD(8)
@@ -490,8 +629,8 @@ int run_bwd(const BwdArgs& a, cudaStream_t st) {
   }
 #undef H3B_LN_BWD
   if (a.sums) {
-    const dim3 grid(static_cast<unsigned>((a.n + 31) / 32), a.db != nullptr ? 2 : 1);
-    ln_bwd_join_kernel<WT><<<grid, 256, 0, st>>>(a.partial, static_cast<int>(ctas), a.n, static_cast<WT*>(a.dw),
+    const dim3 grid(static_cast<unsigned>((a.n + 31) / 32), a.dw != nullptr && a.db != nullptr ? 2 : 1);
+    ln_bwd_join_kernel<WT><<<grid, 1024, 0, st>>>(a.partial, static_cast<int>(ctas), a.n, static_cast<WT*>(a.dw),
                                                  static_cast<WT*>(a.db));
   }
   return h3b::launch_status();

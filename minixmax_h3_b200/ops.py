@@ -683,15 +683,21 @@ def _call_on(t: torch.Tensor, name: str, *args) -> None:
 
 def _workspace_on(fn: str, t: torch.Tensor, *sizes: int) -> torch.Tensor:
     """A workspace on t's device (its size may follow the SM count)."""
-    with torch.cuda.device(t.device):
-        return t.new_empty(_workspace_bytes(fn, t.get_device(), *sizes), dtype=torch.uint8)
+    device = t.get_device()
+    if device == torch._C._cuda_getDevice():
+        return t.new_empty(_workspace_bytes(fn, device, *sizes), dtype=torch.uint8)
+    with torch.cuda.device(device):
+        return t.new_empty(_workspace_bytes(fn, device, *sizes), dtype=torch.uint8)
 
 
-def _one_device(name: str, *ts: Optional[torch.Tensor]) -> None:
-    _cuda(*ts)
-    devices = {t.get_device() for t in ts if t is not None}
-    if len(devices) > 1:
-        raise ValueError(f"{name}: tensors on different devices")
+def _one_device(name: str, t: torch.Tensor, *others: Optional[torch.Tensor]) -> None:
+    device = t.get_device()
+    for o in others:
+        if o is not None and o.get_device() != device:
+            _cuda(t, *others)
+            raise ValueError(f"{name}: tensors on different devices")
+    if device < 0 or not t.is_cuda:
+        _cuda(t)
 
 
 # 2^190 / 2 pi: a frequency's product with it keeps 64 bits of a turn and more
@@ -810,40 +816,48 @@ def rotary(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Tensor, 
     (``attention.rotary`` does so under autograd).  Strided inputs are read in
     place (unit last stride; other layouts are copied).  Angles are exact to
     2^-33 of a turn at any position, results are rounded once."""
-    _one_device("rotary", q, k, positions, rope.turns, q_out, k_out)
+    turns, sections = rope.turns, rope.sections
+    _one_device("rotary", q, k, positions, turns, q_out, k_out)
     _check_heads("rotary", q, q)
-    if k is not None:
-        _check_heads("rotary", k, q)
     b, s, heads, d = q.shape
-    pairs = rope.turns.numel()
+    pairs, axes = turns.shape[0], len(sections)
     if 2 * pairs > d or d & 1:
         raise ValueError(f"rotary: {2 * pairs} turned channels of a head of {d} (an even number)")
-    axes = len(rope.sections)
-    if positions.dtype not in (torch.int32, torch.int64):
+    if positions.dtype is not torch.int32 and positions.dtype is not torch.int64:
         raise TypeError("rotary: positions are int32 or int64")
-    if positions.shape not in ((s,), (b, s)) if axes == 1 else positions.shape not in ((s, axes), (b, s, axes)):
-        raise ValueError(f"rotary: positions [S] or [B, S]{f', each with {axes} axes' if axes > 1 else ''}")
-    p = positions.stride()
+    shape, p = positions.shape, positions.stride()
     if axes == 1:
         p = (*p, 0)
-    if len(p) == 2:
+    elif shape[-1:] == (axes,):
+        shape = shape[:-1]
+    else:
+        shape = ()
+    if shape == (s,):
         p = (0, *p)
+    elif shape != (b, s):
+        raise ValueError(f"rotary: positions [S] or [B, S]{f', each with {axes} axes' if axes > 1 else ''}")
     q_out = _rotary_out(q_out, q)
-    if q.shape[3] > 1 and q.stride(3) != 1:
+    qs = q.stride()
+    if d > 1 and qs[3] != 1:
         q = q.contiguous()
-    if k is not None:
-        k_out = _rotary_out(k_out, k)
-        if k.shape[3] > 1 and k.stride(3) != 1:
+        qs = q.stride()
+    if k is None:
+        kv_heads, ks, kos = 0, (0, 0, 0, 0), (0, 0, 0, 0)
+    else:
+        _check_heads("rotary", k, q)
+        kv_heads, k_out = k.shape[2], _rotary_out(k_out, k)
+        ks, kos = k.stride(), k_out.stride()
+        if d > 1 and ks[3] != 1:
             k = k.contiguous()
-    turns = rope.turns if rope.turns.is_contiguous() else rope.turns.contiguous()
-    sections = (*rope.sections, 0)
-    no_k = (0, 0, 0)
+            ks = k.stride()
+    if not turns.is_contiguous():
+        turns = turns.contiguous()
+    qos = q_out.stride()
     _call_on(q, "h3b_rotary", q.data_ptr(), _ptr(k), q_out.data_ptr(), None if k is None else k_out.data_ptr(),
-             _FLOATS[q.dtype], b, s, heads, 0 if k is None else k.shape[2], d, 2 * pairs, 1 if rope.interleaved else 0,
-             *q.stride()[:3], *(no_k if k is None else k.stride()[:3]), *q_out.stride()[:3],
-             *(no_k if k is None else k_out.stride()[:3]), positions.data_ptr(),
-             1 if positions.dtype == torch.int64 else 0, *p, turns.data_ptr(), sections[0], sections[1],
-             rope.factor, 1 if inverse else 0, _stream(q))
+             _FLOATS[q.dtype], b, s, heads, kv_heads, d, 2 * pairs, 1 if rope.interleaved else 0, qs[0], qs[1], qs[2],
+             ks[0], ks[1], ks[2], qos[0], qos[1], qos[2], kos[0], kos[1], kos[2], positions.data_ptr(),
+             1 if positions.dtype is torch.int64 else 0, *p, turns.data_ptr(), sections[0],
+             sections[1] if axes > 1 else 0, rope.factor, 1 if inverse else 0, _stream(q))
     return q_out, None if k is None else k_out
 
 
@@ -852,21 +866,35 @@ def rotary(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Tensor, 
 
 def _check_norm(name: str, x: torch.Tensor, weight: Optional[torch.Tensor], bias: Optional[torch.Tensor]) -> int:
     """Checks types and shapes; returns the code of the weights' type."""
-    if x.dtype not in _FLOATS:
+    dtype = x.dtype
+    if dtype not in _FLOATS:
         raise TypeError(f"{name} expects bf16, fp16 or fp32 input")
-    if x.dim() == 0 or x.shape[-1] == 0:
+    last = x.shape[-1:]
+    if not last or last[0] == 0:
         raise ValueError(f"{name}: an axis of at least one element is normalised")
-    if bias is not None and (weight is None or bias.dtype != weight.dtype):
-        raise ValueError(f"{name}: a bias comes with a weight of its type")
-    for w in (weight, bias):
-        if w is not None and (w.shape != x.shape[-1:] or w.dtype not in (x.dtype, torch.float32)):
-            raise ValueError(f"{name}: weight and bias are [{x.shape[-1]}] tensors of x's type or fp32")
-    return _FLOATS[x.dtype if weight is None else weight.dtype]
+    if weight is None:
+        if bias is not None:
+            raise ValueError(f"{name}: a bias comes with a weight")
+        return _FLOATS[dtype]
+    wdtype = weight.dtype
+    if weight.shape != last or (wdtype is not dtype and wdtype is not torch.float32):
+        raise ValueError(f"{name}: weight and bias are [{last[0]}] tensors of x's type or fp32")
+    if bias is not None and (bias.shape != last or bias.dtype is not wdtype):
+        raise ValueError(f"{name}: a bias has its weight's shape and type")
+    return _FLOATS[wdtype]
 
 
 def _check_stats(name: str, stats: Optional[torch.Tensor], m: int) -> None:
     if stats is not None and (stats.dtype != torch.float32 or stats.shape != (2, m) or not stats.is_contiguous()):
         raise ValueError(f"{name}: stats is a contiguous fp32 [2, rows] tensor")
+
+
+def _flat_rows(x: torch.Tensor) -> tuple[torch.Tensor, int]:
+    """x as rows of its last axis with unit column stride, and their stride."""
+    if x.is_contiguous():
+        return x, x.shape[-1]
+    x2, _, _, ld = _rows(x)
+    return x2, ld
 
 
 def _packed(w: Optional[torch.Tensor]) -> Optional[torch.Tensor]:
@@ -896,7 +924,7 @@ def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Opt
     _check_stats("layer_norm", stats, m)
     if m == 0:
         return out
-    x2, _, _, ld = _rows(x)
+    x2, ld = _flat_rows(x)
     weight, bias = _packed(weight), _packed(bias)
     at = None if stats is None else stats.data_ptr()
     _call_on(x, "h3b_layer_norm_fwd", x2.data_ptr(), _ptr(weight), _ptr(bias), out.data_ptr(), at,
@@ -920,12 +948,12 @@ def layer_norm_bwd(dout: torch.Tensor, x: torch.Tensor, stats: torch.Tensor, wei
     _check_stats("layer_norm_bwd", stats, m)
     dx = torch.empty_like(x, memory_format=torch.contiguous_format)
     new = torch.zeros if m == 0 else torch.empty
-    dw, db = (new(n, dtype=weight.dtype, device=x.device) if weight is not None and wanted else None
-              for wanted in (weight_grad, bias_grad))
+    dw = new(n, dtype=weight.dtype, device=x.device) if weight is not None and weight_grad else None
+    db = new(n, dtype=weight.dtype, device=x.device) if weight is not None and bias_grad else None
     if m == 0:
         return dx, dw, db
-    x2, _, _, ldx = _rows(x)
-    dout2, _, _, lddy = _rows(dout)
+    x2, ldx = _flat_rows(x)
+    dout2, lddy = _flat_rows(dout)
     weight = _packed(weight)
     ws = None
     if dw is not None or db is not None:
