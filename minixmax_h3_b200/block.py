@@ -27,8 +27,9 @@ import torch.nn as nn
 import torch.nn.functional as F
 
 from . import ops
+from .attention import cross_attention, rotary
 from .dist import is_distributed, state
-from .modules import Linear, Ops, QuantizedRows, QuantLinear, RMSNorm
+from .modules import LayerNorm, Linear, Ops, QuantizedRows, QuantLinear, RMSNorm
 from .ops import EPI_GATE_RES, EPI_GELU, EPI_STORE_POSMAX, EPI_SWIGLU
 from .timing import TIMER
 from .ulysses import (all_gather_kv, all_to_all_heads, all_to_all_qkv, check_scheme, clip_mod_segments,
@@ -248,18 +249,29 @@ class CrossAttention(nn.Module):
     ``kv`` argument, ``fill`` writes them into an 8-bit cache (half the bytes),
     which ``forward`` then attends through ``cache``.
 
+    With ``norm`` the tokens go through a layer norm before the query
+    projection; with ``rope`` queries and keys are turned by their positions
+    (``positions``, ``cond_positions``: see ops.rotary), keys before they are
+    handed out or written into a cache.
+
     The projections are quantised and have no gradients, so the layer has none:
     an input that requires one raises.  Training uses
-    ``attention.cross_attention`` between projections of its own."""
+    ``TrainableCrossAttention``, whose ``quantized`` gives a layer of this
+    class, or ``attention.cross_attention`` between projections of its own."""
 
     def __init__(self, hidden, heads, head_dim, cond_dim, kv_heads: Optional[int] = None, dtype=None, device=None,
-                 operations=None):
+                 operations=None, norm: bool = False, norm_eps: float = 1e-5, rope: Optional["ops.Rotary"] = None):
         super().__init__()
         operations = operations or Ops
         self.heads, self.head_dim = heads, head_dim
         self.kv_heads = heads if kv_heads is None else kv_heads
         if head_dim not in (64, 128) or heads % self.kv_heads:
             raise ValueError("CrossAttention: head_dim 64 or 128, heads a multiple of kv_heads")
+        self.rope = rope
+        self.norm = None
+        if norm:
+            self.norm = getattr(operations, "LayerNorm", LayerNorm)(hidden, eps=norm_eps, device=device)
+            self.norm.requires_grad_(False)
         self.q_proj = operations.QuantLinear(hidden, heads * head_dim, bias=False, dtype=dtype, device=device)
         self.kv_proj = operations.QuantLinear(cond_dim, 2 * self.kv_heads * head_dim, bias=False, dtype=dtype,
                                               device=device)
@@ -270,44 +282,122 @@ class CrossAttention(nn.Module):
         if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in ts):
             raise RuntimeError("CrossAttention has no gradients: detach its inputs, or use attention.cross_attention")
 
-    def encode(self, cond: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
+    def _turned(self, x: torch.Tensor, positions: Optional[torch.Tensor], name: str, in_place: bool) -> torch.Tensor:
+        if (self.rope is None) != (positions is None):
+            raise ValueError(f"CrossAttention: {name} come with rope, and rope with them")
+        return x if self.rope is None else ops.rotary(x, None, positions, self.rope, q_out=x if in_place else None)[0]
+
+    def encode(self, cond: torch.Tensor, *, cond_positions: Optional[torch.Tensor] = None
+               ) -> tuple[torch.Tensor, torch.Tensor]:
         """cond [B, n, cond_dim] -> k, v [B, n, kv_heads, head_dim], the two
         halves of one projection (read in place by the attention)."""
         self._without_gradients(cond)
         b, n, _ = cond.shape
         kv = self.kv_proj(cond.reshape(b * n, -1)).view(b, n, 2, self.kv_heads, self.head_dim)
-        return kv[:, :, 0], kv[:, :, 1]
+        return self._turned(kv[:, :, 0], cond_positions, "cond_positions", True), kv[:, :, 1]
 
     def fill(self, cache: "ops.KV8Cache", cond: torch.Tensor, block_table: torch.Tensor, lens: torch.Tensor, *,
-             new_lens: Optional[torch.Tensor] = None) -> None:
+             new_lens: Optional[torch.Tensor] = None, cond_positions: Optional[torch.Tensor] = None) -> None:
         """Appends the keys and values of cond [B, n, cond_dim] to the
         sequences' blocks behind lens[b] tokens (ops.kv8_append)."""
-        k, v = self.encode(cond)
+        k, v = self.encode(cond, cond_positions=cond_positions)
         ops.kv8_append(cache, k, v, block_table, lens, new_lens=new_lens)
 
     def forward(self, x: torch.Tensor, cond: Optional[torch.Tensor] = None, *,
                 kv: Optional[tuple[torch.Tensor, torch.Tensor]] = None, cond_lens: Optional[torch.Tensor] = None,
                 key_mask: Optional[torch.Tensor] = None, cache: Optional["ops.KV8Cache"] = None,
-                block_table: Optional[torch.Tensor] = None) -> torch.Tensor:
+                block_table: Optional[torch.Tensor] = None, positions: Optional[torch.Tensor] = None,
+                cond_positions: Optional[torch.Tensor] = None) -> torch.Tensor:
         """x [B, S, hidden] bf16 attends to cond (or to kv, or to the
         cond_lens[b] tokens of a cache): [B, S, hidden].  cond_lens (int32
         [B]) and key_mask (bool [B, n]) leave padding and dropped tokens out;
         a sample without any token gets zeros from the attention."""
         if sum(a is not None for a in (cond, kv, cache)) != 1:
             raise ValueError("CrossAttention.forward takes one of cond, kv and cache")
+        if cond is None and cond_positions is not None:
+            raise ValueError("CrossAttention: cond_positions come with cond")
         self._without_gradients(x, cond, *(kv or ()))
         b, s, _ = x.shape
-        q = self.q_proj(x.reshape(b * s, -1)).view(b, s, self.heads, self.head_dim)
+        h = x if self.norm is None else self.norm(x)
+        q = self.q_proj(h.reshape(b * s, -1)).view(b, s, self.heads, self.head_dim)
+        q = self._turned(q, positions, "positions", True)
         if cache is not None:
             if block_table is None or cond_lens is None or key_mask is not None:
                 raise ValueError("a cache is attended through block_table and cond_lens, without key_mask")
             with TIMER.span("cross_attention"):
                 o = ops.kv8_attention(q, cache, block_table, cond_lens)
         else:
-            k, v = self.encode(cond) if kv is None else kv
+            k, v = self.encode(cond, cond_positions=cond_positions) if kv is None else kv
             with TIMER.span("cross_attention"):
                 o = ops.cross_attention(q, k, v, kv_lens=cond_lens, key_mask=key_mask)
         return self.out_proj(o.view(b * s, self.heads * self.head_dim)).view(b, s, -1)
+
+
+class TrainableCrossAttention(nn.Module):
+    """``CrossAttention`` as it is trained, with dense projections: layer norm
+    -> query projection, key and value projection of the encoder's states,
+    rotary positions (with ``rope``), cross attention, output projection.
+
+    Weights are fp32 parameters, used in ``compute_dtype`` (bf16 or fp16), which
+    is also the type of the result.  ``matrices()`` are what ``optim.Muon``
+    updates, the norm's weight and bias what remains; ``quantized`` gives the
+    layer for inference."""
+
+    def __init__(self, hidden, heads, head_dim, cond_dim, kv_heads: Optional[int] = None, norm_eps: float = 1e-5,
+                 rope: Optional["ops.Rotary"] = None, compute_dtype: torch.dtype = torch.bfloat16, device=None):
+        super().__init__()
+        self.hidden, self.heads, self.head_dim, self.cond_dim = hidden, heads, head_dim, cond_dim
+        self.kv_heads = heads if kv_heads is None else kv_heads
+        if head_dim not in (64, 128) or heads % self.kv_heads:
+            raise ValueError("TrainableCrossAttention: head_dim 64 or 128, heads a multiple of kv_heads")
+        if compute_dtype not in (torch.bfloat16, torch.float16):
+            raise ValueError("TrainableCrossAttention computes in bf16 or fp16")
+        self.rope, self.compute_dtype = rope, compute_dtype
+        self.norm = LayerNorm(hidden, eps=norm_eps, device=device)
+
+        def matrix(rows: int, columns: int) -> nn.Parameter:
+            return nn.Parameter(torch.randn(rows, columns, device=device) * columns ** -0.5)
+
+        self.q_proj = matrix(heads * head_dim, hidden)
+        self.k_proj = matrix(self.kv_heads * head_dim, cond_dim)
+        self.v_proj = matrix(self.kv_heads * head_dim, cond_dim)
+        self.out_proj = matrix(hidden, heads * head_dim)
+
+    def matrices(self) -> list[nn.Parameter]:
+        return [self.q_proj, self.k_proj, self.v_proj, self.out_proj]
+
+    def forward(self, x: torch.Tensor, cond: torch.Tensor, *, cond_lens: Optional[torch.Tensor] = None,
+                key_mask: Optional[torch.Tensor] = None, positions: Optional[torch.Tensor] = None,
+                cond_positions: Optional[torch.Tensor] = None) -> torch.Tensor:
+        """x [B, S, hidden] attends to cond [B, n, cond_dim]: [B, S, hidden];
+        the other arguments as in ``CrossAttention.forward``."""
+        if (self.rope is None) != (positions is None) or (self.rope is None) != (cond_positions is None):
+            raise ValueError("TrainableCrossAttention: positions and cond_positions come with rope, and rope with them")
+        dt = self.compute_dtype
+
+        def project(t: torch.Tensor, w: torch.Tensor, heads: int) -> torch.Tensor:
+            return F.linear(t, w.to(dt)).unflatten(-1, (heads, self.head_dim))
+
+        cond = cond.to(dt)
+        q = project(self.norm(x.to(dt)), self.q_proj, self.heads)
+        k, v = project(cond, self.k_proj, self.kv_heads), project(cond, self.v_proj, self.kv_heads)
+        if self.rope is not None:
+            q, k = rotary(q, None, positions, self.rope)[0], rotary(k, None, cond_positions, self.rope)[0]
+        o = cross_attention(q, k, v, kv_lens=cond_lens, key_mask=key_mask)
+        return F.linear(o.flatten(2), self.out_proj.to(dt))
+
+    @torch.no_grad()
+    def quantized(self, fmt: str = "int8_tensorwise", operations=None) -> CrossAttention:
+        """The layer for inference, its projections quantised to ``fmt``."""
+        layer = CrossAttention(self.hidden, self.heads, self.head_dim, self.cond_dim, kv_heads=self.kv_heads,
+                               device=self.q_proj.device, operations=operations, norm=True, norm_eps=self.norm.eps,
+                               rope=self.rope)
+        layer.norm.weight.copy_(self.norm.weight)
+        layer.norm.bias.copy_(self.norm.bias)
+        for ql, w in ((layer.q_proj, self.q_proj), (layer.kv_proj, torch.cat([self.k_proj, self.v_proj])),
+                      (layer.out_proj, self.out_proj)):
+            load_quant_linear(ql, w.detach(), fmt)
+        return layer
 
 
 class MLP(nn.Module):

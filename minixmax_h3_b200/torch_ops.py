@@ -23,6 +23,12 @@ kernel of the path:
     h3b::cross_attention_bwd(dout, q, k, v, out, lse, kv_lens, key_mask, scale) -> (dq, dk, dv)
     h3b::kv8_append(k, v, codes and scales of K and V, block_table, lens, new_lens) -> None  (updates the cache)
     h3b::kv8_attention(q, codes and scales, block_table, lens, causal, scale) -> o [B, Sq, H, D]
+    h3b::rotary(x, positions, turns, sections, interleaved, factor, inverse) -> x turned (the fields of
+        ops.Rotary); differentiable in x, any number of times
+    h3b::layer_norm(x, weight, bias, eps) -> (y, stats fp32 [2, rows]); differentiable in x, weight and
+        bias through y
+    h3b::layer_norm_bwd(dout, x, stats, weight) -> (dx, dweight, dbias), empty without a weight
+    h3b::orthogonalize(x, steps, a, b, c, eps) -> x's shape and type (no gradient)
 
 Each is registered for CUDA tensors only, so tensors on any other device raise
 (there is no CPU fallback).  Each forwards to the ``ops`` function of the same
@@ -148,6 +154,32 @@ def _kv8_attention(q: torch.Tensor, k_codes: torch.Tensor, v_codes: torch.Tensor
                              scale=scale)
 
 
+def _rotary(x: torch.Tensor, positions: torch.Tensor, turns: torch.Tensor, sections: list[int],
+            interleaved: bool = False, factor: float = 1.0, inverse: bool = False) -> torch.Tensor:
+    refuse_tangents(x, name="rotary")
+    return ops.rotary(x, None, positions, ops.Rotary(turns, tuple(sections), interleaved, factor), inverse=inverse)[0]
+
+
+def _layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Optional[torch.Tensor] = None,
+                eps: float = 1e-5) -> tuple[torch.Tensor, torch.Tensor]:
+    refuse_tangents(x, weight, bias, name="layer_norm")
+    if x.dim() == 0 or x.shape[-1] == 0:
+        raise ValueError("layer_norm: an axis of at least one element is normalised")
+    stats = torch.empty((2, x.numel() // x.shape[-1]), dtype=torch.float32, device=x.device)
+    return ops.layer_norm(x, weight, bias, eps, stats=stats), stats
+
+
+def _layer_norm_bwd(dout: torch.Tensor, x: torch.Tensor, stats: torch.Tensor, weight: Optional[torch.Tensor] = None
+                    ) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    dx, dw, db = ops.layer_norm_bwd(dout, x, stats, weight)
+    return dx, x.new_empty(0) if dw is None else dw, x.new_empty(0) if db is None else db
+
+
+def _orthogonalize(x: torch.Tensor, steps: int = 5, a: float = 3.4445, b: float = -4.7750, c: float = 2.0315,
+                   eps: float = 1e-7) -> torch.Tensor:
+    return ops.orthogonalize(x, steps=steps, coefficients=(a, b, c), eps=eps)
+
+
 # ----------------------------------------------------------------------------- registration
 
 quant_i8_rows = torch.library.custom_op("h3b::quant_i8_rows", mutates_args=(), device_types="cuda")(_quant_i8_rows)
@@ -173,6 +205,10 @@ cross_attention_bwd = torch.library.custom_op("h3b::cross_attention_bwd", mutate
 kv8_append = torch.library.custom_op("h3b::kv8_append", mutates_args=("k_codes", "v_codes", "k_scale", "v_scale"),
                                      device_types="cuda")(_kv8_append)
 kv8_attention = torch.library.custom_op("h3b::kv8_attention", mutates_args=(), device_types="cuda")(_kv8_attention)
+rotary = torch.library.custom_op("h3b::rotary", mutates_args=(), device_types="cuda")(_rotary)
+layer_norm = torch.library.custom_op("h3b::layer_norm", mutates_args=(), device_types="cuda")(_layer_norm)
+layer_norm_bwd = torch.library.custom_op("h3b::layer_norm_bwd", mutates_args=(), device_types="cuda")(_layer_norm_bwd)
+orthogonalize = torch.library.custom_op("h3b::orthogonalize", mutates_args=(), device_types="cuda")(_orthogonalize)
 
 
 @quant_i8_rows.register_fake
@@ -268,3 +304,57 @@ def _(k, v, k_codes, v_codes, k_scale, v_scale, block_table, lens, new_lens=None
 @kv8_attention.register_fake
 def _(q, k_codes, v_codes, k_scale, v_scale, block_table, lens, causal=False, scale=None):
     return q.new_empty(tuple(q.shape))
+
+
+@rotary.register_fake
+def _(x, positions, turns, sections, interleaved=False, factor=1.0, inverse=False):
+    return x.new_empty(tuple(x.shape))
+
+
+@layer_norm.register_fake
+def _(x, weight=None, bias=None, eps=1e-5):
+    return x.new_empty(tuple(x.shape)), x.new_empty((2, _rows_of(x)), dtype=torch.float32)
+
+
+@layer_norm_bwd.register_fake
+def _(dout, x, stats, weight=None):
+    if weight is None:
+        return x.new_empty(tuple(x.shape)), x.new_empty(0), x.new_empty(0)
+    return (x.new_empty(tuple(x.shape)), *(weight.new_empty(tuple(weight.shape)) for _ in range(2)))
+
+
+@orthogonalize.register_fake
+def _(x, steps=5, a=3.4445, b=-4.7750, c=2.0315, eps=1e-7):
+    return x.new_empty(tuple(x.shape))
+
+
+def _rotary_setup(ctx, inputs, output):
+    _, positions, turns, *ctx.rest = inputs
+    ctx.save_for_backward(positions, turns)
+
+
+def _rotary_grad(ctx, dout):
+    sections, interleaved, factor, inverse = ctx.rest
+    dx = torch.ops.h3b.rotary(dout, *ctx.saved_tensors, sections, interleaved, factor, not inverse)
+    return dx, None, None, None, None, None, None
+
+
+rotary.register_autograd(_rotary_grad, setup_context=_rotary_setup)
+
+
+def _layer_norm_setup(ctx, inputs, output):
+    x, weight, bias, _ = inputs
+    ctx.save_for_backward(x, weight, output[1])
+    ctx.with_bias = bias is not None
+    ctx.set_materialize_grads(False)
+
+
+def _layer_norm_grad(ctx, dout, dstats):
+    if dstats is not None:
+        raise RuntimeError("h3b::layer_norm has no gradient through stats (they are for the backward pass): detach them")
+    x, weight, stats = ctx.saved_tensors
+    dx, dw, db = torch.ops.h3b.layer_norm_bwd(dout, x, stats, weight)
+    return dx, None if weight is None else dw, db if ctx.with_bias else None, None
+
+
+layer_norm.register_autograd(_layer_norm_grad, setup_context=_layer_norm_setup)
