@@ -362,8 +362,7 @@ __global__ void __launch_bounds__(bwd_threads(TPR), VEC > 1 ? bwd_ctas_per_sm(TP
   constexpr bool SMALL = THREADS == 1024;
   constexpr int ROWS = SMALL || sizeof(T) == 4 || VEC == 1 ? 1 : 2;
   __shared__ float2 slots[2][ROWS][32];
-  // groups' sums meet here (only groups of less than a CTA)
-  __shared__ float2 joined[GROUPS > 1 ? TPR * EPT : 1];
+  extern __shared__ float2 joined[];  // groups' sums, where there are several: [GROUPS][TPR * EPT]
   const int t = threadIdx.x % TPR, group = threadIdx.x / TPR;
   const int n = static_cast<int>(a.n);
   const int nv = (n + VEC - 1) / VEC;
@@ -422,12 +421,12 @@ __global__ void __launch_bounds__(bwd_threads(TPR), VEC > 1 ? bwd_ctas_per_sm(TP
       float2 p1 = both(0.0f), p2 = both(0.0f);
 #pragma unroll
       for (int q = 0; q < PAIRS; ++q) {
-        const float2 xhat = mul2(add2(pair_at(vx[k], q), both(shift[k])), both(rstd[k]));
-        const float2 d = pair_at(vg[k], q);
-        const float2 g = mul2(d, pair_at(wv, q));
-        p1 = add2(p1, g);
-        p2 = fma2(g, xhat, p2);
-        sw[q] = fma2(d, xhat, sw[q]);
+        const float2 xm = add2(pair_at(vx[k], q), both(shift[k]));  // x - mean = xhat / rstd
+        const float2 d = pair_at(vg[k], q), w = pair_at(wv, q);
+        const float2 e = mul2(d, xm);
+        p1 = fma2(d, w, p1);
+        p2 = fma2(e, w, p2);
+        sw[q] = fma2(e, both(rstd[k]), sw[q]);
         sb[q] = add2(sb[q], d);
       }
       s1[k] = p1.x + p1.y;
@@ -437,12 +436,13 @@ __global__ void __launch_bounds__(bwd_threads(TPR), VEC > 1 ? bwd_ctas_per_sm(TP
     set ^= 1;
 #pragma unroll
     for (int k = 0; k < ROWS; ++k) {
-      const float c1 = s1[k] * inv_n, c2 = s2[k] * inv_n;
+      // dx = rstd (g - c1) - rstd^2 c2 (x - mean), with c2 = rstd mean(g (x - mean))
+      const float c1 = -s1[k] * inv_n * rstd[k], c2 = -s2[k] * inv_n * rstd[k] * rstd[k] * rstd[k];
 #pragma unroll
       for (int q = 0; q < PAIRS; ++q) {
-        const float2 xhat = mul2(add2(pair_at(vx[k], q), both(shift[k])), both(rstd[k]));
+        const float2 xm = add2(pair_at(vx[k], q), both(shift[k]));
         const float2 g = mul2(pair_at(vg[k], q), pair_at(wv, q));
-        set_pair(vx[k], q, mul2(add2(fma2(xhat, both(-c2), g), both(-c1)), both(rstd[k])));
+        set_pair(vx[k], q, fma2(g, both(rstd[k]), fma2(xm, both(c2), both(c1))));
       }
       T* dx = static_cast<T*>(a.dx) + (base + k * step + group) * a.lddx;
 #pragma unroll
@@ -452,27 +452,21 @@ __global__ void __launch_bounds__(bwd_threads(TPR), VEC > 1 ? bwd_ctas_per_sm(TP
       }
     }
   }
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   if (!a.sums) return;
   float* out = a.partial + static_cast<int64_t>(blockIdx.x) * 2 * a.n;
   if constexpr (GROUPS > 1) {
-    for (int g = 0; g < GROUPS; ++g) {
-      if (group == g) {
 #pragma unroll
-        for (int i = 0; i < MAXV; ++i) {
-          const int c = t + i * TPR;
+    for (int i = 0; i < MAXV; ++i)
 #pragma unroll
-          for (int j = 0; j < VEC; ++j) {
-            const int at = c * VEC + j;
-            const float2 before = g == 0 ? make_float2(0.0f, 0.0f) : joined[at];
-            joined[at] = make_float2(before.x + half_of(sw, i * VEC + j), before.y + half_of(sb, i * VEC + j));
-          }
-        }
-      }
-      __syncthreads();
-    }
+      for (int j = 0; j < VEC; ++j)
+        joined[group * TPR * EPT + (t + i * TPR) * VEC + j] = make_float2(half_of(sw, i * VEC + j), half_of(sb, i * VEC + j));
+    __syncthreads();
     for (int c = threadIdx.x; c < n; c += THREADS) {
-      out[c] = joined[c].x;
-      out[n + c] = joined[c].y;
+      float2 s = joined[c];
+      for (int g = 1; g < GROUPS; ++g) s = add2(s, joined[g * TPR * EPT + c]);
+      out[c] = s.x;
+      out[n + c] = s.y;
     }
   } else {
 #pragma unroll
@@ -535,6 +529,7 @@ __global__ void __launch_bounds__(256) ln_bwd_long_sums_kernel(const BwdArgs a) 
 template <class WT>
 __global__ void __launch_bounds__(1024) ln_bwd_join_kernel(const float* partial, int ctas, int64_t n, WT* dw, WT* db) {
   __shared__ float part[32][32];
+  asm volatile("griddepcontrol.wait;" ::: "memory");  // for the partial rows
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int64_t c = static_cast<int64_t>(blockIdx.x) * 32 + lane;
   const int64_t which = dw == nullptr ? 1 : blockIdx.y;
@@ -608,10 +603,15 @@ template <class T, class WT, int VEC>
 int run_bwd(const BwdArgs& a, cudaStream_t st) {
   const int tpr = row_threads(a.n);
   const unsigned ctas = static_cast<unsigned>(bwd_ctas(a.m, a.n));
-#define H3B_LN_BWD(TPR)                                                        \
-  case TPR:                                                                    \
-    ln_bwd_kernel<T, WT, VEC, TPR><<<ctas, bwd_threads(TPR), 0, st>>>(a);      \
-    break;
+#define H3B_LN_BWD(TPR)                                                                                            \
+  case TPR: {                                                                                                      \
+    constexpr int threads = bwd_threads(TPR), bytes = threads > TPR ? threads * EPT * 8 : 0;                       \
+    static h3b::OncePerDevice once;                                                                                \
+    const int rc = once.run(h3b::device(), [] { return h3b::allow_smem(ln_bwd_kernel<T, WT, VEC, TPR>, bytes); }); \
+    if (rc != H3B_OK) return rc;                                                                                   \
+    ln_bwd_kernel<T, WT, VEC, TPR><<<ctas, threads, bytes, st>>>(a);                                               \
+    break;                                                                                                         \
+  }
   switch (tpr) {
     H3B_LN_BWD(8)
     H3B_LN_BWD(32)
@@ -630,8 +630,19 @@ int run_bwd(const BwdArgs& a, cudaStream_t st) {
 #undef H3B_LN_BWD
   if (a.sums) {
     const dim3 grid(static_cast<unsigned>((a.n + 31) / 32), a.dw != nullptr && a.db != nullptr ? 2 : 1);
-    ln_bwd_join_kernel<WT><<<grid, 1024, 0, st>>>(a.partial, static_cast<int>(ctas), a.n, static_cast<WT*>(a.dw),
-                                                 static_cast<WT*>(a.db));
+    // (set up while the kernel before it ends, and waiting for it)
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = grid;
+    cfg.blockDim = dim3(1024);
+    cfg.stream = st;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    if (cudaLaunchKernelEx(&cfg, ln_bwd_join_kernel<WT>, static_cast<const float*>(a.partial), static_cast<int>(ctas), a.n,
+                           static_cast<WT*>(a.dw), static_cast<WT*>(a.db)) != cudaSuccess)
+      return H3B_ERR_LAUNCH;
   }
   return h3b::launch_status();
 }
