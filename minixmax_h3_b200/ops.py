@@ -798,6 +798,8 @@ def _rotary_out(out: Optional[torch.Tensor], x: torch.Tensor) -> torch.Tensor:
         return torch.empty_like(x, memory_format=torch.contiguous_format)
     if out.shape != x.shape or out.dtype != x.dtype or (out.shape[3] > 1 and out.stride(3) != 1):
         raise ValueError("rotary: an output has its input's shape and type and unit last stride")
+    if any(n > 1 and s == 0 for n, s in zip(out.shape, out.stride())):
+        raise ValueError("rotary: an output has elements of its own")
     return out
 
 

@@ -20,7 +20,7 @@ class Muon(torch.optim.Optimizer):
     orthogonalised by itself.  Those of one shape are orthogonalised in one
     call.  Averages are fp32; ``dtype`` is the type in which an update is
     orthogonalised (bf16: the result is within its rounding; fp32 costs
-    about a quarter more).  Gradients and parameters may be of any floating
+    about half more).  Gradients and parameters may be of any floating
     type: a parameter is updated in its own, so what is below its rounding is
     lost there.  State and steps follow the parameters' devices; a step can be
     captured into a CUDA graph once the averages exist."""

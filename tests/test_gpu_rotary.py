@@ -247,7 +247,8 @@ def test_refusals(cuda):
             (ValueError, (torch.zeros(2, 3, 4, 65, device=cuda), None, p, rope), {}),
             (ValueError, (x, None, p, rope), {"q_out": x[..., :32]}),
             (ValueError, (x, None, p, rope), {"q_out": torch.zeros(2, 3, 64, 4, device=cuda).transpose(2, 3)}),
-            (ValueError, (x, x, p, rope), {"k_out": x.half()})):
+            (ValueError, (x, x, p, rope), {"k_out": x.half()}),
+            (ValueError, (x, None, p, rope), {"q_out": x[:, :, :1].expand(2, 3, 4, 64)})):
         with pytest.raises(error):
             ops.rotary(*args, **kw)
     with torch.autograd.forward_ad.dual_level():

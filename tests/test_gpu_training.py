@@ -134,6 +134,28 @@ def test_muon_moves_the_layer(cuda, dtype):
             g.mul_(-0.5)
 
 
+def test_captured_training_step(cuda):
+    """Forward and backward through autograd, captured and replayed on other inputs."""
+    layer, x, cond, where = layer_and_inputs(cuda)
+    params, dy = list(layer.parameters()), torch.randn(2, 70, 192, device=cuda).to(BF16)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        torch.autograd.grad(layer(x, cond, **where), params, dy)  # its results are gone before the capture
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        y = layer(x, cond, **where)
+        grads = torch.autograd.grad(y, params, dy)
+    for _ in range(2):
+        x.normal_()
+        cond.normal_()
+        graph.replay()
+        want = layer(x, cond, **where)
+        wanted = torch.autograd.grad(want, params, dy)
+        assert torch.equal(y, want) and all(torch.equal(g, w) for g, w in zip(grads, wanted))
+
+
 def test_quantized_layer(cuda):
     """The layer for inference is its parts: norm, quantised projections, rotations, attention - dense, with keys
     encoded once, and through the 8-bit cache, chunk and single token."""
