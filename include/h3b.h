@@ -383,23 +383,29 @@ H3B_API int h3b_kv8_attention(const void* q, void* o, float* lse, int dtype, int
  * pairs (i, i + rot/2), or (2i, 2i + 1) with interleaved != 0.  The other
  * channels are copied.  inverse != 0 turns by -a (the transpose).  The
  * product and sum are fp32, rounded once to the type.
- * dtype H3B_BF16, H3B_F16 or H3B_F32 (inputs and outputs); strides in
- * elements, the last one 1, nothing else asked of them; d even; rot even, at
- * most d; heads + kv_heads at most 65535.  k and k_out may be NULL with
- * kv_heads 0.  An output may be its input (with its strides); it must overlap
- * nothing else.
- * positions: int32, or int64 with positions64 != 0; token (i, j)'s position
- * on axis x at i*pos_batch + j*pos_seq + x*pos_axis.  Pairs below axis0_pairs
- * use axis 0, the next axis1_pairs axis 1, the rest axis 2; an axis without
- * pairs is not read.  turns: [rot / 2], device.
+ * dtype H3B_BF16, H3B_F16 or H3B_F32 (inputs and outputs); strides (batch,
+ * sequence, head) in elements, that of a head's channels 1, nothing else asked
+ * of them; d even; rot even, at most d; heads + kv_heads at most 65535.  k and
+ * k_out may be NULL with kv_heads 0.  An output may be its input (with its
+ * strides); it must overlap nothing else.
+ * positions: int32, or int64 with positions64 != 0; token (i, j)'s position on
+ * axis x at i*pos_stride[0] + j*pos_stride[1] + x*pos_stride[2].  Pairs below
+ * axis0_pairs use axis 0, the next axis1_pairs axis 1, the rest axis 2; an axis
+ * without pairs is not read.  turns: [rot / 2], device.
  */
-H3B_API int h3b_rotary(const void* q, const void* k, void* q_out, void* k_out, int dtype, int64_t b, int64_t s,
-                       int64_t heads, int64_t kv_heads, int64_t d, int64_t rot, int interleaved, int64_t q_batch,
-                       int64_t q_seq, int64_t q_head, int64_t k_batch, int64_t k_seq, int64_t k_head,
-                       int64_t qo_batch, int64_t qo_seq, int64_t qo_head, int64_t ko_batch, int64_t ko_seq,
-                       int64_t ko_head, const void* positions, int positions64, int64_t pos_batch, int64_t pos_seq,
-                       int64_t pos_axis, const uint64_t* turns, int64_t axis0_pairs, int64_t axis1_pairs,
-                       float factor, int inverse, h3b_stream_t stream);
+typedef struct {
+  const void *q, *k;
+  void *q_out, *k_out;
+  const void* positions;
+  const uint64_t* turns;
+  int64_t b, s, heads, kv_heads, d, rot;
+  int64_t q_stride[3], k_stride[3], q_out_stride[3], k_out_stride[3];
+  int64_t pos_stride[3];
+  int64_t axis0_pairs, axis1_pairs;
+  double factor;
+  int32_t dtype, interleaved, positions64, inverse;
+} h3b_rotary_args;
+H3B_API int h3b_rotary(const h3b_rotary_args* args, h3b_stream_t stream);
 
 /* -------------------------------------------------------------- layer norm */
 

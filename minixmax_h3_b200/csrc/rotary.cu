@@ -212,42 +212,42 @@ bool fits(const Operand& o, int64_t b, int64_t s, int64_t h, int64_t vec, int64_
 
 }  // namespace
 
-extern "C" int h3b_rotary(const void* q, const void* k, void* q_out, void* k_out, int dtype, int64_t b, int64_t s,
-                          int64_t heads, int64_t kv_heads, int64_t d, int64_t rot, int interleaved, int64_t q_batch,
-                          int64_t q_seq, int64_t q_head, int64_t k_batch, int64_t k_seq, int64_t k_head,
-                          int64_t qo_batch, int64_t qo_seq, int64_t qo_head, int64_t ko_batch, int64_t ko_seq,
-                          int64_t ko_head, const void* positions, int positions64, int64_t pos_batch, int64_t pos_seq,
-                          int64_t pos_axis, const uint64_t* turns, int64_t axis0_pairs, int64_t axis1_pairs,
-                          float factor, int inverse, h3b_stream_t stream) {
+extern "C" int h3b_rotary(const h3b_rotary_args* r, h3b_stream_t stream) {
+  if (r == nullptr) return H3B_ERR_ARG;
+  const int dtype = r->dtype;
+  const int64_t b = r->b, s = r->s, heads = r->heads, kv_heads = r->kv_heads, d = r->d, rot = r->rot;
   if (dtype != H3B_BF16 && dtype != H3B_F16 && dtype != H3B_F32) return H3B_ERR_DTYPE;
   if (b < 0 || s < 0 || heads < 0 || kv_heads < 0 || heads + kv_heads > 65535) return H3B_ERR_SHAPE;
   if (d < 1 || d > 65536 || rot < 0 || rot > d || (rot & 1)) return H3B_ERR_SHAPE;
-  if (axis0_pairs < 0 || axis1_pairs < 0 || axis0_pairs + axis1_pairs > rot / 2) return H3B_ERR_SHAPE;
+  if (r->axis0_pairs < 0 || r->axis1_pairs < 0 || r->axis0_pairs + r->axis1_pairs > rot / 2) return H3B_ERR_SHAPE;
   if (b == 0 || s == 0 || heads + kv_heads == 0) return H3B_OK;
-  if ((heads > 0 && (q == nullptr || q_out == nullptr)) || (kv_heads > 0 && (k == nullptr || k_out == nullptr)))
+  if ((heads > 0 && (r->q == nullptr || r->q_out == nullptr)) || (kv_heads > 0 && (r->k == nullptr || r->k_out == nullptr)))
     return H3B_ERR_ARG;
-  if (rot > 0 && (positions == nullptr || turns == nullptr)) return H3B_ERR_ARG;
+  if (rot > 0 && (r->positions == nullptr || r->turns == nullptr)) return H3B_ERR_ARG;
   if (s > 0x7FFFFFFF || b > 0x7FFFFFFF || b * s > (1ll << 40)) return H3B_ERR_SHAPE;
+  const auto operand = [](const void* in, void* out, const int64_t (&i)[3], const int64_t (&o)[3]) {
+    return Operand{in, out, i[0], i[1], i[2], o[0], o[1], o[2]};
+  };
   RotaryArgs a{};
-  a.q = {q, q_out, q_batch, q_seq, q_head, qo_batch, qo_seq, qo_head};
-  a.k = {k, k_out, k_batch, k_seq, k_head, ko_batch, ko_seq, ko_head};
+  a.q = operand(r->q, r->q_out, r->q_stride, r->q_out_stride);
+  a.k = operand(r->k, r->k_out, r->k_stride, r->k_out_stride);
   if (heads == 0) a.q = a.k;
   if (kv_heads == 0) a.k = a.q;
-  a.pos = positions;
-  a.pos_b = pos_batch;
-  a.pos_s = pos_seq;
-  a.pos_a = pos_axis;
-  a.turns = turns;
+  a.pos = r->positions;
+  a.pos_b = r->pos_stride[0];
+  a.pos_s = r->pos_stride[1];
+  a.pos_a = r->pos_stride[2];
+  a.turns = r->turns;
   a.tokens = b * s;
   a.s = static_cast<int>(s);
   a.heads = static_cast<int>(heads);
   a.all_heads = static_cast<int>(heads + kv_heads);
   a.half = static_cast<int>(rot / 2);
-  a.end0 = static_cast<int>(axis0_pairs);
-  a.end1 = static_cast<int>(axis0_pairs + axis1_pairs);
-  a.pos64 = positions64;
-  a.factor = factor;
-  a.sign = inverse ? -1.0f : 1.0f;
+  a.end0 = static_cast<int>(r->axis0_pairs);
+  a.end1 = static_cast<int>(r->axis0_pairs + r->axis1_pairs);
+  a.pos64 = r->positions64;
+  a.factor = static_cast<float>(r->factor);
+  a.sign = r->inverse ? -1.0f : 1.0f;
   const int64_t bytes = dtype == H3B_F32 ? 4 : 2;
   int64_t vec = 16 / bytes;
   while (vec > 1 && (rot % (2 * vec) != 0 || d % (2 * vec) != 0 ||
@@ -256,7 +256,7 @@ extern "C" int h3b_rotary(const void* q, const void* k, void* q_out, void* k_out
     vec /= 2;
   if (vec == 1 && (d & 1)) return H3B_ERR_SHAPE;
   const auto st = reinterpret_cast<cudaStream_t>(stream);
-#define H3B_ROTARY(T, V) return launch<T, V>(a, d, rot, interleaved, st)
+#define H3B_ROTARY(T, V) return launch<T, V>(a, d, rot, r->interleaved, st)
 #define H3B_ROTARY16(T)      \
   if (vec == 8) H3B_ROTARY(T, 8); \
   if (vec == 4) H3B_ROTARY(T, 4); \
