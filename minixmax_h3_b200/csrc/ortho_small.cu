@@ -9,7 +9,8 @@
 //     gets columns q of the others' sums through distributed shared memory,
 //     adds them in order and gives the result to all.
 //   B = b G + c G G in every CTA (128^3 products cost less than a hand-over)
-//   X = a X + B X over this CTA's columns
+//   X = a X + B X over this CTA's columns, in two halves: one is stored while
+//     the other's product runs, and the next G begins while that is stored.
 // a X and b G are added in fp32 from the planes, which a thread reads and
 // overwrites at its own elements.  A launch a product takes 17 launches of 8
 // to 18 us here, bound by their beginnings and ends: 24 matrices of
@@ -33,8 +34,10 @@ constexpr int ROWS = 128;
 constexpr int MAX_W = 256;               // columns of a CTA
 constexpr int MAX_CTAS = 8;
 constexpr int TILE = ROWS * 128;         // bytes of a tile of 64 columns
-constexpr int THREADS = 256;
-constexpr uint32_t TMEM_COLS = 256;
+constexpr int THREADS = 512, WARPS = THREADS / 32;
+constexpr uint32_t TMEM_COLS = 512;      // B X (columns 0 .. 255), G and G G
+constexpr uint32_t G_COL = 256, GG_COL = 384;
+enum { GRAM = 0, POLY = 1, MUL = 2, MUL_2 = 3 };  // products, each once a step
 
 struct Args {
   const void* x;
@@ -50,8 +53,8 @@ struct Args {
 
 struct Shared {
   double squares[MAX_CTAS];
-  double warp_sums[THREADS / 32];
-  uint64_t done;
+  double warp_sums[WARPS];
+  uint64_t done[4];
   uint32_t tmem;
   int abort_flag;
 };
@@ -119,11 +122,11 @@ __global__ void __launch_bounds__(THREADS, 1) ortho_small_kernel(const Args args
   const int rank = CTAS > 1 ? static_cast<int>(cluster_ctarank()) : 0;
   const int matrix = static_cast<int>(blockIdx.x) / CTAS;
   const int col0 = rank * args.width;
-  const int quad = warp & 3, half = warp >> 2, row = quad * 32 + lane;  // this thread's row of an accumulator
+  const int quad = warp & 3, part = warp >> 2, row = quad * 32 + lane;  // this thread's row and columns of an accumulator
   volatile int* abort_flag = &sh->abort_flag;
 
   if (tid == 0) {
-    mbar_init(&sh->done, 1);
+    for (int i = 0; i < 4; ++i) mbar_init(&sh->done[i], 1);
     sh->abort_flag = 0;
     fence_barrier_init();
   }
@@ -227,11 +230,11 @@ __global__ void __launch_bounds__(THREADS, 1) ortho_small_kernel(const Args args
     auto rows_of_x = [&](auto transposed, auto across) {  // rows of 32 * across elements at most
       constexpr bool T_ = decltype(transposed)::value;
       constexpr int N = decltype(across)::value, L = 32 / N;
-      for (int line0 = warp; line0 < lines; line0 += 8 * L) {
+      for (int line0 = warp; line0 < lines; line0 += WARPS * L) {
         T e[L][N];
 #pragma unroll
         for (int l = 0; l < L; ++l) {
-          const int line = line0 + 8 * l;
+          const int line = line0 + WARPS * l;
           const T* p = x + line * args.ld + lane;
 #pragma unroll
           for (int j = 0; j < N; ++j) e[l][j] = line < lines && lane + 32 * j < length ? p[32 * j] : from_f32<T>(0.0f);
@@ -242,7 +245,7 @@ __global__ void __launch_bounds__(THREADS, 1) ortho_small_kernel(const Args args
           for (int j = 0; j < N; ++j) square_of(e[l][j], j & 1);
 #pragma unroll
         for (int l = 0; l < L; ++l) {
-          const int line = line0 + 8 * l;
+          const int line = line0 + WARPS * l;
 #pragma unroll
           for (int j = 0; j < N; ++j)
             if (line < lines && lane + 32 * j < length)
@@ -263,7 +266,7 @@ __global__ void __launch_bounds__(THREADS, 1) ortho_small_kernel(const Args args
   if (CTAS > 1) cluster_sync();  // every CTA runs: its shared memory can be written
   if (tid < CTAS) {
     s = 0.0;
-    for (int i = 0; i < THREADS / 32; ++i) s += sh->warp_sums[i];
+    for (int i = 0; i < WARPS; ++i) s += sh->warp_sums[i];
     asm volatile("st.shared::cluster.f64 [%0], %1;" ::"r"(mapa_shared(smem_u32(&sh->squares[rank]), tid)), "d"(s) : "memory");
   }
   all_sync();
@@ -292,43 +295,74 @@ __global__ void __launch_bounds__(THREADS, 1) ortho_small_kernel(const Args args
   local_sync();
 
   // ------------------------------------------------------------- steps
-  uint32_t phase = 0;
-  auto wait_products = [&] {
-    mbar_wait(&sh->done, phase & 1, &g_status, 1, abort_flag);  // out of time: noted, and on to the barriers
+  // Products stop at the last 16 rows and columns that hold anything; what the
+  // planes get behind those is never read.  X is worked on in halves of 128
+  // columns: while the second one's product runs the first one is stored, and
+  // while the second one is stored the next G takes the first.
+  const int k_rows = (args.rows + 15) / 16, k_cols = max(1, (cols + 15) / 16);  // of 16
+  const int k_first = min(k_cols, 8), k_second = k_cols - k_first;
+  const uint32_t square_d = idesc_f16_f32(ROWS, 16 * static_cast<uint32_t>(k_rows), 0, 0);
+  uint32_t parity = 0;
+  auto wait_for = [&](int product) {
+    mbar_wait<false, false, true>(&sh->done[product], parity, &g_status, 1 + product, abort_flag);  // out of time: noted, and on to the barriers
     __syncwarp();
-    ++phase;
     tc_fence_after();
   };
-  // Products stop at the last 16 rows and columns that hold anything; what the
-  // planes get behind those is never read.
-  const int k_rows = (args.rows + 15) / 16, k_cols = max(1, (cols + 15) / 16);  // of 16
-  const uint32_t square_d = idesc_f16_f32(ROWS, 16 * static_cast<uint32_t>(k_rows), 0, 0);
-  const uint32_t wide_d = idesc_f16_f32(ROWS, 16 * static_cast<uint32_t>(k_cols), 0, 1);
-  // A A^T (K along the planes' rows, `n` times 16): the small products first
-  auto square = [&](const uint8_t* hi, const uint8_t* lo, int n) {
-    if (warp == 0 && elect_one()) {
-      const uint64_t h = sdesc_kmajor_sw128(smem_u32(hi)), l = sdesc_kmajor_sw128(smem_u32(lo));
-      for (int p = 0; p < 3; ++p)
-        for (int k = 0; k < n; ++k) {
-          const uint32_t at = (k >> 2) * (TILE >> 4) + 2 * (k & 3);
-          mma_f16_ss(tmem, (p == 0 ? l : h) + at, (p == 1 ? l : h) + at, square_d, (p | k) != 0);
-        }
-      tc_commit(&sh->done);
-    }
-    __syncwarp();
+  // A A^T over K from 16 `from` to 16 `to` along the planes' rows, the small products first
+  auto square = [&](uint32_t d, const uint8_t* hi, const uint8_t* lo, int from, int to, bool add) {
+    const uint64_t h = sdesc_kmajor_sw128(smem_u32(hi)), l = sdesc_kmajor_sw128(smem_u32(lo));
+    for (int p = 0; p < 3; ++p)
+      for (int k = from; k < to; ++k) {
+        const uint32_t at = (k >> 2) * (TILE >> 4) + 2 * (k & 3);
+        mma_f16_ss(d, (p == 0 ? l : h) + at, (p == 1 ? l : h) + at, square_d, add || p != 0 || k != from);
+      }
   };
+  // columns 128 i .. of B X, K down the rows of X
+  auto product = [&](int i, int n) {
+    const uint32_t wide_d = idesc_f16_f32(ROWS, 16 * static_cast<uint32_t>(n), 0, 1);
+    const uint64_t bh = sdesc_kmajor_sw128(smem_u32(g_hi)), bl = sdesc_kmajor_sw128(smem_u32(g_lo));
+    const uint64_t xh = sdesc_mnmajor_sw128(smem_u32(x_hi + i * 2 * TILE), TILE, 1024);
+    const uint64_t xl = sdesc_mnmajor_sw128(smem_u32(x_lo + i * 2 * TILE), TILE, 1024);
+    for (int p = 0; p < 3; ++p)
+      for (int k = 0; k < k_rows; ++k)
+        mma_f16_ss(tmem + 128 * i, (p == 0 ? bl : bh) + (k >> 2) * (TILE >> 4) + 2 * (k & 3),
+                   (p == 1 ? xl : xh) + k * (2048 >> 4), wide_d, (p | k) != 0);
+    tc_commit(&sh->done[MUL + i]);
+  };
+  // 32 of its columns: X = a X + B X
+  auto store_half = [&](int i, int n) {
+    const int c = i * 128 + part * 32;
+    if (part * 32 >= 16 * n) return;
+    uint32_t r[32];
+    tmem_ld32p(t_row + c, r);
+    tmem_wait_fence<1>(r);
+#pragma unroll
+    for (int j = 0; j < 32; j += 8) {
+      uint4* hi = reinterpret_cast<uint4*>(x_hi + piece(row, (c + j) >> 3));
+      uint4* lo = reinterpret_cast<uint4*>(x_lo + piece(row, (c + j) >> 3));
+      float v[8];
+      join8(*hi, *lo, v);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[e] = fmaf(args.a, v[e], __uint_as_float(r[j + e]) * (1.0f / SCALE));
+      split8(v, hi, lo);
+    }
+  };
+  const bool mine = part * 32 < 16 * k_rows;  // columns of G and B
 
   if constexpr (CTAS > 1) cluster_arrive();
-  for (int step = 0; step < args.steps; ++step) {
-    square(x_hi, x_lo, k_cols);
-    wait_products();
+  if (warp == 0 && elect_one()) square(tmem + G_COL, x_hi, x_lo, 0, k_first, false);
+  __syncwarp();
+  for (int step = 0; step < args.steps; ++step, parity ^= 1) {
+    if (warp == 0 && elect_one()) {
+      square(tmem + G_COL, x_hi, x_lo, k_first, k_cols, true);
+      tc_commit(&sh->done[GRAM]);
+    }
+    __syncwarp();
+    wait_for(GRAM);
+    uint32_t r[32];
     if constexpr (CTAS == 1) {
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const int c = half * 64 + i * 32;
-        if (c >= 16 * k_rows) break;
-        uint32_t r[32];
-        tmem_ld32p(t_row + c, r);
+      if (mine) {
+        tmem_ld32p(t_row + G_COL + part * 32, r);
         tmem_wait_fence<1>(r);
         float v[32];
 #pragma unroll
@@ -337,8 +371,8 @@ __global__ void __launch_bounds__(THREADS, 1) ortho_small_kernel(const Args args
         for (int j = 0; j < 32; j += 8) {
           uint4 h, l;
           split8(v + j, &h, &l);
-          *reinterpret_cast<uint4*>(g_hi + piece(row, (c + j) >> 3)) = h;
-          *reinterpret_cast<uint4*>(g_lo + piece(row, (c + j) >> 3)) = l;
+          *reinterpret_cast<uint4*>(g_hi + piece(row, part * 4 + (j >> 3))) = h;
+          *reinterpret_cast<uint4*>(g_lo + piece(row, part * 4 + (j >> 3))) = l;
         }
       }
       local_sync();
@@ -349,28 +383,25 @@ __global__ void __launch_bounds__(THREADS, 1) ortho_small_kernel(const Args args
       // 512 bytes at once (rows 128 bytes apart crossed at a third of that).
       auto share = [](int r, int p) { return static_cast<uint32_t>((p * ROWS + r) * 16); };
       cluster_wait();  // every CTA is done with B
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const int c = half * 64 + i * 32;
-        if (c >= 16 * k_rows) break;
-        uint32_t r[32];
-        tmem_ld32p(t_row + c, r);
+      if (mine) {
+        tmem_ld32p(t_row + G_COL + part * 32, r);
         tmem_wait_fence<1>(r);
 #pragma unroll
         for (int j = 0; j < 32; j += 4) {
-          const int owner = (c + j) / OWN, p = (c + j) % OWN / 4;
+          const int c = part * 32 + j, owner = c / OWN, p = c % OWN / 4;
           st_cluster(mapa_shared(smem_u32(g_hi) + rank * PART + share(row, p), owner),
                      make_uint4(r[j], r[j + 1], r[j + 2], r[j + 3]));
         }
       }
+      __syncwarp();
       tc_fence_before();
       cluster_sync();
       // a thread adds eight columns of a row, its neighbours the next eight
-      constexpr int SUMS = OWN / 16;
+      constexpr int ITEMS = ROWS * OWN / 8, SUMS = (ITEMS + THREADS - 1) / THREADS;
       float v[SUMS][8];
 #pragma unroll
       for (int k = 0; k < SUMS; ++k) {
-        const int r = (tid + k * THREADS) / (OWN / 8), p = (tid + k * THREADS) % (OWN / 8) * 2;
+        const int i = (tid + k * THREADS) % ITEMS, r = i / (OWN / 8), p = i % (OWN / 8) * 2;
 #pragma unroll
         for (int j = 0; j < 8; ++j) v[k][j] = 0.0f;
 #pragma unroll
@@ -389,35 +420,37 @@ __global__ void __launch_bounds__(THREADS, 1) ortho_small_kernel(const Args args
       cluster_wait();
 #pragma unroll
       for (int k = 0; k < SUMS; ++k) {
-        const int r = (tid + k * THREADS) / (OWN / 8), p = (tid + k * THREADS) % (OWN / 8);
+        const int i = tid + k * THREADS, r = i / (OWN / 8), p = i % (OWN / 8);
+        if (i < ITEMS) {
 #pragma unroll
-        for (int j = 0; j < 8; ++j) v[k][j] *= 1.0f / SCALE;
-        uint4 h, l;
-        split8(v[k], &h, &l);
-        const uint32_t at = piece(r, rank * (OWN / 8) + p);
+          for (int j = 0; j < 8; ++j) v[k][j] *= 1.0f / SCALE;
+          uint4 h, l;
+          split8(v[k], &h, &l);
+          const uint32_t at = piece(r, rank * (OWN / 8) + p);
 #pragma unroll
-        for (int q = 0; q < CTAS; ++q) {
-          st_cluster(mapa_shared(smem_u32(g_hi) + at, q), h);
-          st_cluster(mapa_shared(smem_u32(g_lo) + at, q), l);
+          for (int q = 0; q < CTAS; ++q) {
+            st_cluster(mapa_shared(smem_u32(g_hi) + at, q), h);
+            st_cluster(mapa_shared(smem_u32(g_lo) + at, q), l);
+          }
         }
       }
       all_sync();
       tc_fence_after();
     }
 
-    square(g_hi, g_lo, k_rows);
-    wait_products();
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const int c = half * 64 + i * 32;
-      if (c >= 16 * k_rows) break;
-      uint32_t r[32];
-      tmem_ld32p(t_row + c, r);
+    if (warp == 0 && elect_one()) {
+      square(tmem + GG_COL, g_hi, g_lo, 0, k_rows, false);
+      tc_commit(&sh->done[POLY]);
+    }
+    __syncwarp();
+    wait_for(POLY);
+    if (mine) {
+      tmem_ld32p(t_row + GG_COL + part * 32, r);
       tmem_wait_fence<1>(r);
 #pragma unroll
       for (int j = 0; j < 32; j += 8) {
-        uint4* hi = reinterpret_cast<uint4*>(g_hi + piece(row, (c + j) >> 3));
-        uint4* lo = reinterpret_cast<uint4*>(g_lo + piece(row, (c + j) >> 3));
+        uint4* hi = reinterpret_cast<uint4*>(g_hi + piece(row, part * 4 + (j >> 3)));
+        uint4* lo = reinterpret_cast<uint4*>(g_lo + piece(row, part * 4 + (j >> 3)));
         float v[8];
         join8(*hi, *lo, v);
 #pragma unroll
@@ -427,35 +460,22 @@ __global__ void __launch_bounds__(THREADS, 1) ortho_small_kernel(const Args args
     }
     local_sync();
 
-    if (warp == 0 && elect_one()) {  // B X: K down the rows of X
-      const uint64_t bh = sdesc_kmajor_sw128(smem_u32(g_hi)), bl = sdesc_kmajor_sw128(smem_u32(g_lo));
-      const uint64_t xh = sdesc_mnmajor_sw128(smem_u32(x_hi), TILE, 1024);
-      const uint64_t xl = sdesc_mnmajor_sw128(smem_u32(x_lo), TILE, 1024);
-      for (int p = 0; p < 3; ++p)
-        for (int k = 0; k < k_rows; ++k)
-          mma_f16_ss(tmem, (p == 0 ? bl : bh) + (k >> 2) * (TILE >> 4) + 2 * (k & 3), (p == 1 ? xl : xh) + k * (2048 >> 4),
-                     wide_d, (p | k) != 0);
-      tc_commit(&sh->done);
+    if (warp == 0 && elect_one()) {
+      product(0, k_first);
+      if (k_second > 0) product(1, k_second);
     }
     __syncwarp();
-    wait_products();
-    if (CTAS > 1 && step + 1 < args.steps) cluster_arrive();
-    for (int c = half * 32; c < 16 * k_cols; c += 64) {
-      uint32_t r[32];
-      tmem_ld32p(t_row + c, r);
-      tmem_wait_fence<1>(r);
-#pragma unroll
-      for (int j = 0; j < 32; j += 8) {
-        uint4* hi = reinterpret_cast<uint4*>(x_hi + piece(row, (c + j) >> 3));
-        uint4* lo = reinterpret_cast<uint4*>(x_lo + piece(row, (c + j) >> 3));
-        float v[8];
-        join8(*hi, *lo, v);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) v[e] = fmaf(args.a, v[e], __uint_as_float(r[j + e]) * (1.0f / SCALE));
-        split8(v, hi, lo);
-      }
-    }
+    wait_for(MUL);
+    store_half(0, k_first);
     local_sync();
+    if (step + 1 < args.steps && warp == 0 && elect_one()) square(tmem + G_COL, x_hi, x_lo, 0, k_first, false);
+    __syncwarp();
+    if (k_second > 0) {
+      wait_for(MUL_2);
+      store_half(1, k_second);
+      local_sync();
+    }
+    if (CTAS > 1 && step + 1 < args.steps) cluster_arrive();
   }
 
   // ------------------------------------------------------------ result
@@ -470,7 +490,7 @@ __global__ void __launch_bounds__(THREADS, 1) ortho_small_kernel(const Args args
     auto rows_of_x = [&](auto transposed, auto across) {
       constexpr bool T_ = decltype(transposed)::value;
 #pragma unroll 2
-      for (int line = warp; line < lines; line += THREADS / 32) {
+      for (int line = warp; line < lines; line += WARPS) {
         T* p = out + static_cast<int64_t>(line) * args.n + lane;
 #pragma unroll
         for (int j = 0; j < decltype(across)::value; ++j)
@@ -509,7 +529,13 @@ __global__ void __launch_bounds__(THREADS, 1) ortho_small_kernel(const Args args
   if (warp == 0) tmem_dealloc(tmem, TMEM_COLS);
 }
 
-size_t smem_bytes(int width) { return 1024 + static_cast<size_t>(width / 64) * TILE * 2 + 4 * TILE + sizeof(Shared); }
+// More than half of an SM's at least: a CTA takes all of TMEM, and of two
+// clusters that share SMs each could hold what the other waits for.
+size_t smem_bytes(int width) {
+  const size_t need = 1024 + static_cast<size_t>(width / 64) * TILE * 2 + 4 * TILE + sizeof(Shared);
+  const size_t alone = 116 * 1024;
+  return need > alone ? need : alone;
+}
 static_assert(1024 + MAX_W / 64 * TILE * 2 + 4 * TILE + sizeof(Shared) <= 227 * 1024, "shared memory budget");
 
 template <class T, int CTAS>
