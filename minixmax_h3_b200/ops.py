@@ -727,6 +727,12 @@ class Rotary:
     interleaved: bool = False
     factor: float = 1.0
 
+    def __post_init__(self) -> None:
+        if self.turns.dtype is not torch.int64 or self.turns.dim() != 1:
+            raise TypeError("Rotary: turns is an int64 tensor [pairs]")
+        if not 1 <= len(self.sections) <= 3 or min(self.sections) < 0 or sum(self.sections) != self.turns.shape[0]:
+            raise ValueError(f"Rotary: sections {self.sections} of {self.turns.shape[0]} pairs (one to three axes)")
+
     @classmethod
     def from_frequencies(cls, frequencies: Sequence[float] | torch.Tensor, *, sections: Optional[Sequence[int]] = None,
                          interleaved: bool = False, factor: float = 1.0, device="cuda") -> "Rotary":
@@ -738,9 +744,8 @@ class Rotary:
         if not all(math.isfinite(f) for f in w) or not math.isfinite(factor):
             raise ValueError("Rotary: frequencies and factor are finite")
         sections = (len(w),) if sections is None else tuple(int(n) for n in sections)
-        if not 1 <= len(sections) <= 3 or min(sections) < 0 or sum(sections) != len(w):
-            raise ValueError(f"Rotary: sections {sections} of {len(w)} pairs (one to three axes)")
-        return cls(torch.tensor([_turns(f) for f in w], dtype=torch.int64, device=device), sections, bool(interleaved), float(factor))
+        return cls(torch.tensor([_turns(f) for f in w], dtype=torch.int64, device=device), sections, bool(interleaved),
+                   float(factor))
 
     @classmethod
     def build(cls, dims: int | Sequence[int], *, theta: float = 10000.0, interleaved: bool = False,
@@ -913,7 +918,7 @@ def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Opt
     (bf16, fp16 or fp32; weight and bias of x's type or fp32): x's shape and
     type, contiguous, or ``out`` (contiguous).  stats, if given (fp32
     [2, rows]), receives each row's mean and 1 / sqrt(var + eps), which
-    layer_norm_bwd needs.  Rows with a unit last stride and one row stride are
+    layer_norm_bwd needs.  out may be x itself and else overlaps nothing.  Rows with a unit last stride and one row stride are
     read in place, other layouts copied first.  A row that holds NaN or an
     infinity gives NaN.  For gradients by autograd see ``modules.layer_norm``."""
     _one_device("layer_norm", x, weight, bias, out, stats)

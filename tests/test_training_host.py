@@ -73,6 +73,15 @@ def test_from_frequencies_refusals():
             ops.Rotary.from_frequencies(w, device="cpu", **kw)
 
 
+def test_fields_are_checked():
+    """Sections that are not the pairs would read positions that are not there."""
+    turns = torch.zeros(4, dtype=torch.int64)
+    for error, args in ((TypeError, (turns.int(), (4,))), (TypeError, (turns.view(2, 2), (2,))), (ValueError, (turns, (1, 1))),
+                        (ValueError, (turns, ())), (ValueError, (turns, (5, -1))), (ValueError, (turns, (1, 1, 1, 1)))):
+        with pytest.raises(error):
+            ops.Rotary(*args)
+
+
 # ----------------------------------------------------------------------------- Muon
 
 
