@@ -287,10 +287,10 @@ __global__ void __launch_bounds__(block_threads(TPR)) ln_fwd_kernel(const FwdArg
 #pragma unroll
         for (int j = 0; j < VEC / 2; ++j) {
           float2 h = fma2(add2(get2(v[i], j), both(-m0)), both(rstd), both(shift));
-          if (b != nullptr)  // comes with a weight
-            h = fma2(h, wv.pair(j), bv.pair(j));
-          else if (w != nullptr)
-            h = mul2(h, wv.pair(j));
+          if (w != nullptr)
+            h = b != nullptr ? fma2(h, wv.pair(j), bv.pair(j)) : mul2(h, wv.pair(j));
+          else if (b != nullptr)
+            h = add2(h, bv.pair(j));
           set2(v[i], j, h);
         }
       }
@@ -702,6 +702,7 @@ extern "C" int h3b_layer_norm_bwd(const void* dy, const void* x, const void* w, 
   const bool sums = dw != nullptr || db != nullptr;
   if (sums && (workspace == nullptr || workspace_bytes < bwd_ctas(m, n) * 2 * n * static_cast<int64_t>(sizeof(float))))
     return H3B_ERR_ARG;
+  if (sums && !h3b::aligned16(workspace)) return H3B_ERR_ALIGN;
   const BwdArgs a{dy, x, w, mean, rstd, dx, dw, db, static_cast<float*>(workspace), m, n, lddy, ldx, lddx, sums ? 1 : 0};
   const int64_t vec = 16 / element_bytes(dtype);
   const bool wide = n % vec == 0 && (m == 1 || (ldx % vec == 0 && lddy % vec == 0 && lddx % vec == 0)) &&

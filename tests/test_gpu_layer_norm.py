@@ -293,3 +293,20 @@ def test_refusals(cuda):
                         (ValueError, (x, x, stats, w.half()))):
         with pytest.raises(error):
             ops.layer_norm_bwd(*args)
+
+
+@pytest.mark.parametrize("n", [256, 100, 40000])
+@pytest.mark.parametrize("dt", [F32, BF16])
+def test_c_entries_arguments(cuda, n, dt):
+    """A bias without a weight (the Python call refuses it); a workspace off its alignment."""
+    x, b = torch.randn(5, n, device=cuda).to(dt), torch.randn(n, device=cuda).to(dt)
+    y, stats = torch.empty_like(x), torch.empty(2, 5, device=cuda)
+    code, stream = {BF16: 0, F32: 2}[dt], torch.cuda.current_stream().cuda_stream
+    assert code == ops._FLOATS[dt]
+    _lib.call("h3b_layer_norm_fwd", x.data_ptr(), None, b.data_ptr(), y.data_ptr(), stats.data_ptr(),
+              stats.data_ptr() + 20, code, code, 5, n, n, n, 1e-5, stream)
+    close(y, *formulas(x, None, b, 1e-5)["y"], "y")
+    ws = torch.empty(1 << 24, dtype=torch.uint8, device=cuda)
+    with pytest.raises(RuntimeError):
+        _lib.call("h3b_layer_norm_bwd", x.data_ptr(), x.data_ptr(), None, stats.data_ptr(), stats.data_ptr() + 20,
+                  y.data_ptr(), b.data_ptr(), None, code, code, 5, n, n, n, n, ws.data_ptr() + 2, ws.numel() - 2, stream)
