@@ -34,6 +34,19 @@ int allow_smem(Kernel* kernel, size_t bytes) {
              : H3B_ERR_LAUNCH;
 }
 
+// The same for a kernel that is launched with attributes (clusters, an early
+// start), once on each device.  `registers`: what its launch has to come with,
+// 0 for any number (a register split waits for good in one with fewer).
+template <class Kernel>
+int prepare(OncePerDevice& once, Kernel* kernel, size_t bytes, int registers = 0) {
+  return once.run(device(), [&]() -> int {
+    cudaFuncAttributes attr;
+    if (registers > 0 && (cudaFuncGetAttributes(&attr, kernel) != cudaSuccess || attr.numRegs < registers))
+      return H3B_ERR_LAUNCH;
+    return allow_smem(kernel, bytes);
+  });
+}
+
 // Encodes a row-major 2D tensor map: `inner` contiguous elements per row,
 // `outer` rows `row_stride_bytes` apart; box = box_inner x box_outer.
 int encode_2d(CUtensorMap* map, CUtensorMapDataType dtype, const void* base, uint64_t inner, uint64_t outer,

@@ -606,9 +606,7 @@ int run_bwd(const BwdArgs& a, cudaStream_t st) {
 #define H3B_LN_BWD(TPR)                                                                                            \
   case TPR: {                                                                                                      \
     constexpr int threads = bwd_threads(TPR), bytes = threads > TPR ? threads * EPT * 8 : 0;                       \
-    static h3b::OncePerDevice once;                                                                                \
-    const int rc = once.run(h3b::device(), [] { return h3b::allow_smem(ln_bwd_kernel<T, WT, VEC, TPR>, bytes); }); \
-    if (rc != H3B_OK) return rc;                                                                                   \
+    static_assert(bytes <= 40 * 1024, "dynamic shared memory without an attribute");                               \
     ln_bwd_kernel<T, WT, VEC, TPR><<<ctas, threads, bytes, st>>>(a);                                               \
     break;                                                                                                         \
   }

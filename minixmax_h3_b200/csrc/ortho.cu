@@ -894,12 +894,7 @@ int launch(const Maps& a, const Maps& b, const Maps& out, const Maps& k, const A
   static_assert(smem <= 227 * 1024, "shared memory budget");
   static h3b::OncePerDevice once;
   const auto kernel = ortho_product<PAIR, PARTS, OP, SPLIT>;
-  const int rc = once.run(h3b::device(), [&] {
-    // the register split waits for good in a launch with fewer registers than it adds up to
-    cudaFuncAttributes attr;
-    if (cudaFuncGetAttributes(&attr, kernel) != cudaSuccess || attr.numRegs < LAUNCH_REGS) return static_cast<int>(H3B_ERR_LAUNCH);
-    return h3b::allow_smem(kernel, smem);
-  });
+  const int rc = h3b::prepare(once, kernel, smem, LAUNCH_REGS);
   if (rc != H3B_OK) return rc;
   // every tile has a cluster of its own where parts share it
   const int64_t most = PARTS > 1 ? tiles : h3b::num_sms() / PAIR;

@@ -542,7 +542,7 @@ template <class T, int CTAS>
 int launch(const Args& args, int64_t batch, cudaStream_t stream) {
   const auto kernel = ortho_small_kernel<T, CTAS>;
   static h3b::OncePerDevice once;
-  const int rc = once.run(h3b::device(), [&] { return h3b::allow_smem(kernel, smem_bytes(MAX_W)); });
+  const int rc = h3b::prepare(once, kernel, smem_bytes(MAX_W));
   if (rc != H3B_OK) return rc;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>(batch * CTAS));
