@@ -53,7 +53,7 @@ enum {
 };
 
 /* Element type codes for activation inputs. */
-enum { H3B_BF16 = 0, H3B_F16 = 1, H3B_F32 = 2 /* h3b_kv8_read's output, rotary, layer norm */ };
+enum { H3B_BF16 = 0, H3B_F16 = 1, H3B_F32 = 2 /* h3b_kv8_read's output, rotary, layer norm, orthogonalize */ };
 
 /* Code types of the 8-bit key/value cache. */
 enum { H3B_KV_INT8 = 0, H3B_KV_E4M3 = 1 };

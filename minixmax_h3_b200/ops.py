@@ -713,7 +713,7 @@ def _turns(radians: float) -> int:
     return t - (1 << 64) if t >> 63 else t
 
 
-@dataclass
+@dataclass(frozen=True, eq=False)
 class Rotary:
     """The rotations of ``rotary``: how far a pair of channels turns at each
     position.  turns [pairs] (int64) holds radians / 2 pi as multiples of
@@ -730,6 +730,7 @@ class Rotary:
     def __post_init__(self) -> None:
         if self.turns.dtype is not torch.int64 or self.turns.dim() != 1:
             raise TypeError("Rotary: turns is an int64 tensor [pairs]")
+        object.__setattr__(self, "sections", tuple(self.sections))
         if not 1 <= len(self.sections) <= 3 or min(self.sections) < 0 or sum(self.sections) != self.turns.shape[0]:
             raise ValueError(f"Rotary: sections {self.sections} of {self.turns.shape[0]} pairs (one to three axes)")
 

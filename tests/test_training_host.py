@@ -82,6 +82,16 @@ def test_fields_are_checked():
             ops.Rotary(*args)
 
 
+def test_fields_stay_as_checked():
+    sections = [2, 2]
+    rope = ops.Rotary(torch.zeros(4, dtype=torch.int64), sections)
+    sections[1] = 1
+    assert rope.sections == (2, 2)
+    for name, value in (("sections", (1, 1)), ("turns", torch.zeros(2, dtype=torch.int64)), ("factor", 2.0)):
+        with pytest.raises(AttributeError):
+            setattr(rope, name, value)
+
+
 # ----------------------------------------------------------------------------- Muon
 
 
