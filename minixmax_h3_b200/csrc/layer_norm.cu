@@ -299,6 +299,132 @@ __global__ void __launch_bounds__(block_threads(TPR)) ln_fwd_kernel(const FwdArg
   }
 }
 
+// N values of every lane, summed over the warp: lane l gets the sum of value
+// l N / 32 in v[0].  Halves of the values change sides while there are several.
+template <int N>
+H3B_DEV void fold(float (&v)[N]) {
+  int have = N;
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    if (have > 1) {
+      have /= 2;
+      const bool upper = threadIdx.x & o;
+#pragma unroll
+      for (int i = 0; i < N / 2; ++i)
+        if (i < have) {
+          const float other = __shfl_xor_sync(0xffffffffu, upper ? v[i] : v[i + have], o);
+          v[i] = (upper ? v[i + have] : v[i]) + other;
+        }
+    } else {
+      v[0] += __shfl_xor_sync(0xffffffffu, v[0], o);
+    }
+  }
+}
+
+// WARPS warps hold R rows together, PACKS 16-byte words of each a thread: the
+// weights of its columns are loaded once for the R.
+template <class T, class WT, int VEC, int WARPS, int R, int PACKS>
+__global__ void __launch_bounds__(32 * WARPS) ln_fwd_rows_kernel(const FwdArgs a) {
+  constexpr int THREADS = 32 * WARPS;
+  __shared__ float means[R][WARPS], squares[2 * R][WARPS];
+  auto total = [](const float (&of_warps)[WARPS]) {
+    float s = of_warps[0];
+#pragma unroll
+    for (int i = 1; i < WARPS; ++i) s += of_warps[i];
+    return s;
+  };
+  const int t = threadIdx.x, lane = t & 31, warp = t >> 5;
+  const int64_t row0 = static_cast<int64_t>(blockIdx.x) * R;
+  const int rows = static_cast<int>(a.m - row0 < R ? a.m - row0 : R);
+  const T* x = static_cast<const T*>(a.x) + row0 * a.ldx;
+  const int n = static_cast<int>(a.n), nv = n / VEC;
+  const float inv_n = 1.0f / static_cast<float>(n);
+  Pack<T, VEC> v[R][PACKS];
+#pragma unroll
+  for (int r = 0; r < R; ++r)
+#pragma unroll
+    for (int i = 0; i < PACKS; ++i) {
+      const int c = t + i * THREADS;
+      if (c < nv && r < rows) {
+        v[r][i] = load_pack<T, VEC>(x + r * a.ldx + c * VEC);
+      } else {
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) v[r][i].e[j] = from_f32<T>(0.0f);
+      }
+    }
+  float m0[R];
+#pragma unroll
+  for (int r = 0; r < R; ++r) {
+    float2 s = both(0.0f);
+#pragma unroll
+    for (int i = 0; i < PACKS; ++i)
+#pragma unroll
+      for (int j = 0; j < VEC / 2; ++j) s = add2(s, get2(v[r][i], j));
+    m0[r] = s.x + s.y;
+  }
+  fold(m0);
+  if (lane % (32 / R) == 0) means[lane / (32 / R)][warp] = m0[0];
+  __syncthreads();
+#pragma unroll
+  for (int r = 0; r < R; ++r) m0[r] = total(means[r]) * inv_n;
+  float s[2 * R];
+#pragma unroll
+  for (int r = 0; r < R; ++r) {
+    float2 s1 = both(0.0f), s2 = both(0.0f);
+#pragma unroll
+    for (int i = 0; i < PACKS; ++i)
+      if (t + i * THREADS < nv) {
+#pragma unroll
+        for (int j = 0; j < VEC / 2; ++j) {
+          const float2 d = add2(get2(v[r][i], j), both(-m0[r]));
+          s1 = add2(s1, d);
+          s2 = fma2(d, d, s2);
+        }
+      }
+    s[r] = s1.x + s1.y;
+    s[R + r] = s2.x + s2.y;
+  }
+  fold(s);
+  if (lane % (16 / R) == 0) squares[lane / (16 / R)][warp] = s[0];
+  __syncthreads();
+  float rstd[R], shift[R];
+#pragma unroll
+  for (int r = 0; r < R; ++r) {
+    const float dm = total(squares[r]) * inv_n;
+    rstd[r] = inverse_std(total(squares[R + r]) * inv_n, dm, a.eps);
+    shift[r] = -dm * rstd[r];
+    if (a.mean != nullptr && t == r && r < rows) {
+      a.mean[row0 + r] = m0[r] + dm;
+      a.rstd[row0 + r] = rstd[r];
+    }
+  }
+  T* y = static_cast<T*>(a.y) + row0 * a.ldy;
+  const WT* w = static_cast<const WT*>(a.w);
+  const WT* b = static_cast<const WT*>(a.b);
+#pragma unroll
+  for (int i = 0; i < PACKS; ++i) {
+    const int c = t + i * THREADS;
+    if (c < nv) {
+      Weights<WT, VEC> wv, bv;
+      if (w != nullptr) wv.load(w + c * VEC);
+      if (b != nullptr) bv.load(b + c * VEC);
+#pragma unroll
+      for (int r = 0; r < R; ++r) {
+#pragma unroll
+        for (int j = 0; j < VEC / 2; ++j) {
+          float2 h = fma2(add2(get2(v[r][i], j), both(-m0[r])), both(rstd[r]), both(shift[r]));
+          if (w != nullptr)
+            h = b != nullptr ? fma2(h, wv.pair(j), bv.pair(j)) : mul2(h, wv.pair(j));
+          else if (b != nullptr)
+            h = add2(h, bv.pair(j));
+          set2(v[r][i], j, h);
+        }
+        if (r < rows) store_pack<T, VEC>(y + r * a.ldy + c * VEC, v[r][i]);
+      }
+    }
+  }
+}
+
 // Rows longer than 32 x 1024 elements: a CTA a row, read three times (from L2
 // after the first), element by element.
 template <class T, class WT>
@@ -580,18 +706,36 @@ int run_fwd(const FwdArgs& a, cudaStream_t st) {
     return h3b::launch_status();                                                                          \
   }
   H3B_LN_FWD(8, 32)
-  H3B_LN_FWD(32, 32)
-  if constexpr (VEC > 1) {
-    // A warp a row needs no barriers, and its 8 or 16 KB are loads enough for
-    // its share of an SM (32768 x 4096 in 96 us, with four warps a row 119).
-    // Few rows would be a little quicker with more threads; a row's result
-    // does not depend on how many others there are.
-    H3B_LN_FWD(32, 64)
-    H3B_LN_FWD(32, 128)
+  if constexpr (VEC == 1) {
+    H3B_LN_FWD(32, 32)
+    H3B_LN_FWD(64, 32)
+    H3B_LN_FWD(128, 32)
+  } else {
+    // Weights in fp32 are twice the bytes of a 16-bit row, and L1 would bind:
+    // as many warps as hold four rows (two longer ones) in 64 registers of
+    // each thread.  16384 x 4096 bf16 takes 48.7 us, with a warp a row 57.4;
+    // 131072 x 512 47, 62; 8192 x 8192 54, a CTA a row 60; fp32 within 2 us of
+    // those.  Few rows would be a little quicker with more threads; a row's
+    // result does not depend on how many others there are.
+#define H3B_LN_FWD_ROWS(WARPS, R, PACKS)                                                                                    \
+  if (a.n <= 32 * WARPS * PACKS * VEC) {                                                                                   \
+    ln_fwd_rows_kernel<T, WT, VEC, WARPS, R, PACKS><<<static_cast<unsigned>((a.m + R - 1) / R), 32 * WARPS, 0, st>>>(a);    \
+    return h3b::launch_status();                                                                                           \
   }
-  H3B_LN_FWD(64, 32)
-  H3B_LN_FWD(128, 32)
-  H3B_LN_FWD(256, 32)
+    H3B_LN_FWD_ROWS(1, 4, 2)
+    H3B_LN_FWD_ROWS(1, 4, 3)
+    H3B_LN_FWD_ROWS(1, 4, 4)
+    H3B_LN_FWD_ROWS(2, 4, 3)
+    H3B_LN_FWD_ROWS(2, 4, 4)
+    H3B_LN_FWD_ROWS(4, 4, 3)
+    H3B_LN_FWD_ROWS(4, 4, 4)
+    H3B_LN_FWD_ROWS(4, 2, 5)
+    H3B_LN_FWD_ROWS(4, 2, 6)
+    H3B_LN_FWD_ROWS(4, 2, 8)
+    H3B_LN_FWD_ROWS(8, 2, 6)
+#undef H3B_LN_FWD_ROWS
+  }
+  if constexpr (VEC < 8) H3B_LN_FWD(256, 32)
   H3B_LN_FWD(512, 32)
   H3B_LN_FWD(1024, 32)
 #undef H3B_LN_FWD

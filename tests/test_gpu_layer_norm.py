@@ -310,3 +310,20 @@ def test_c_entries_arguments(cuda, n, dt):
     with pytest.raises(RuntimeError):
         _lib.call("h3b_layer_norm_bwd", x.data_ptr(), x.data_ptr(), None, stats.data_ptr(), stats.data_ptr() + 20,
                   y.data_ptr(), b.data_ptr(), None, code, code, 5, n, n, n, n, ws.data_ptr() + 2, ws.numel() - 2, stream)
+
+
+@pytest.mark.parametrize("dt", [F32, BF16])
+@pytest.mark.parametrize("n", [264, 600, 768, 1152, 1536, 2056, 2560, 4104, 5120, 5128, 6144, 7000, 12288, 12296])
+def test_rows_share_warps(cuda, n, dt):
+    """Rows by fours and twos, and what is left of them: the same bits in any company."""
+    g = torch.Generator(device=cuda).manual_seed(n)
+    x = (torch.randn(11, n, generator=g, device=cuda) * 3 - 1).to(dt)
+    w, b = torch.randn(n, generator=g, device=cuda), torch.randn(n, generator=g, device=cuda)
+    want, stats = ops.layer_norm(x, w, b), torch.empty(2, 11, device=cuda)
+    ops.layer_norm(x, w, b, stats=stats)
+    for rows in (1, 2, 3, 5):
+        wide, own = torch.full((rows + 1, n), 7.0, dtype=dt, device=cuda), torch.full((2, rows), 7.0, device=cuda)
+        ops.layer_norm(x[4:4 + rows], w, b, out=wide[:rows], stats=own)
+        assert torch.equal(wide[:rows], want[4:4 + rows]) and torch.equal(own, stats[:, 4:4 + rows])
+        assert (wide[rows] == 7).all()
+        check(x[:rows], w, b)
