@@ -21,6 +21,9 @@
 #include "h3b_common.cuh"
 #include "h3b_host.hpp"
 
+H3B_DECLARE_STATUS();
+H3B_REGISTER_STATUS_READER(layer_norm);
+
 namespace {
 
 H3B_DEV float to_f32(float v) { return v; }
@@ -476,6 +479,12 @@ struct BwdArgs {
 constexpr int bwd_threads(int tpr) { return tpr < 256 ? 256 : tpr; }
 constexpr int bwd_ctas_per_sm(int tpr) { return bwd_threads(tpr) == 256 ? 2 : 1; }
 
+// 16-bit rows come through a ring of RING rounds in shared memory, fetched by
+// bulk copies while earlier ones are worked on (32-bit rows have twice the
+// bytes for the same arithmetic, and two CTAs' loads in turn are enough).
+constexpr int RING = 6;
+constexpr bool bwd_ring(int element, int vec, int tpr) { return element == 2 && vec > 1 && tpr >= 64 && tpr <= 512; }
+
 template <class T, class WT, int VEC, int TPR>
 __global__ void __launch_bounds__(bwd_threads(TPR), VEC > 1 ? bwd_ctas_per_sm(TPR) : 1) ln_bwd_kernel(const BwdArgs a) {
   constexpr int MAXV = EPT / VEC;
@@ -487,8 +496,12 @@ __global__ void __launch_bounds__(bwd_threads(TPR), VEC > 1 ? bwd_ctas_per_sm(TP
   // registers a thread: one row, and the weights again for each (from L1).
   constexpr bool SMALL = THREADS == 1024;
   constexpr int ROWS = SMALL || sizeof(T) == 4 || VEC == 1 ? 1 : 2;
+  constexpr bool FETCHED = bwd_ring(sizeof(T), VEC, TPR);
   __shared__ float2 slots[2][ROWS][32];
-  extern __shared__ float2 joined[];  // groups' sums, where there are several: [GROUPS][TPR * EPT]
+  __shared__ uint64_t full[RING];
+  // the ring, [RING][x, dy][GROUPS][n]; then groups' sums, where there are several, [GROUPS][TPR * EPT]
+  extern __shared__ __align__(128) uint8_t smem[];
+  float2* joined = reinterpret_cast<float2*>(smem);
   const int t = threadIdx.x % TPR, group = threadIdx.x / TPR;
   const int n = static_cast<int>(a.n);
   const int nv = (n + VEC - 1) / VEC;
@@ -513,6 +526,33 @@ __global__ void __launch_bounds__(bwd_threads(TPR), VEC > 1 ? bwd_ctas_per_sm(TP
   // Every group of the CTA makes the same number of rounds (the row sums need
   // whole warps); one without a row adds zeros and writes nothing.
   const int64_t step = static_cast<int64_t>(gridDim.x) * GROUPS;
+  const uint32_t row_bytes = static_cast<uint32_t>(n * sizeof(T)), tensor_bytes = GROUPS * row_bytes;
+  auto fetch = [&](int64_t first, int slot) {  // a round's rows; warp 0
+    const int rows = static_cast<int>(a.m - first < GROUPS ? a.m - first : GROUPS);
+    if (threadIdx.x == 0) mbar_arrive_expect_tx(&full[slot], 2 * static_cast<uint32_t>(rows) * row_bytes);
+    __syncwarp();
+    const int r = static_cast<int>(threadIdx.x);
+    if (r < rows) {
+      uint8_t* to = smem + 2 * slot * tensor_bytes + r * row_bytes;
+      bulk_load(to, static_cast<const T*>(a.x) + (first + r) * a.ldx, row_bytes, &full[slot]);
+      bulk_load(to + tensor_bytes, static_cast<const T*>(a.dy) + (first + r) * a.lddy, row_bytes, &full[slot]);
+    }
+  };
+  int slot = 0;
+  uint32_t parity = 0;
+  if constexpr (FETCHED) {
+    static_assert(RING % ROWS == 0, "whole iterations");
+    if (threadIdx.x == 0) {
+      for (int i = 0; i < RING; ++i) mbar_init(&full[i], 1);
+      fence_barrier_init();
+    }
+    __syncthreads();
+    if (threadIdx.x < 32)
+      for (int i = 0; i < RING; ++i) {
+        const int64_t first = static_cast<int64_t>(blockIdx.x) * GROUPS + i * step;
+        if (first < a.m) fetch(first, i);
+      }
+  }
   for (int64_t base = static_cast<int64_t>(blockIdx.x) * GROUPS; base < a.m; base += ROWS * step) {
     Pack<T, VEC> vx[ROWS][MAXV], vg[ROWS][MAXV];
     float rstd[ROWS], shift[ROWS];
@@ -522,8 +562,19 @@ __global__ void __launch_bounds__(bwd_threads(TPR), VEC > 1 ? bwd_ctas_per_sm(TP
       const int64_t row = base + k * step + group;
       live[k] = row < a.m;
       rstd[k] = shift[k] = 0.0f;
+      if (FETCHED && live[k]) {
+        shift[k] = -a.mean[row];
+        rstd[k] = a.rstd[row];
+      }
+    }
+    auto load_row = [&](int k) {
+      const int64_t row = base + k * step + group;
       const T* x = static_cast<const T*>(a.x) + row * a.ldx;
       const T* dy = static_cast<const T*>(a.dy) + row * a.lddy;
+      if constexpr (FETCHED) {
+        x = reinterpret_cast<const T*>(smem + 2 * (slot + k) * tensor_bytes + group * row_bytes);
+        dy = reinterpret_cast<const T*>(smem + (2 * (slot + k) + 1) * tensor_bytes + group * row_bytes);
+      }
 #pragma unroll
       for (int i = 0; i < MAXV; ++i) {
         const int c = t + i * TPR;
@@ -535,9 +586,14 @@ __global__ void __launch_bounds__(bwd_threads(TPR), VEC > 1 ? bwd_ctas_per_sm(TP
           for (int j = 0; j < VEC; ++j) vx[k][i].e[j] = vg[k][i].e[j] = from_f32<T>(0.0f);
         }
       }
-      if (live[k]) {
-        shift[k] = -a.mean[row];
-        rstd[k] = a.rstd[row];
+    };
+#pragma unroll
+    for (int k = 0; k < ROWS; ++k) {
+      if (FETCHED && base + k * step < a.m) mbar_wait(&full[slot + k], parity, &g_status, 1, nullptr);  // out of time: noted
+      load_row(k);
+      if (!FETCHED && live[k]) {
+        shift[k] = -a.mean[base + k * step + group];
+        rstd[k] = a.rstd[base + k * step + group];
       }
     }
     if (SMALL) load_weights();
@@ -560,10 +616,20 @@ __global__ void __launch_bounds__(bwd_threads(TPR), VEC > 1 ? bwd_ctas_per_sm(TP
     }
     row_sums<TPR, ROWS>(s1, s2, slots[set]);
     set ^= 1;
+    if constexpr (FETCHED) {
+      // a barrier was among the sums: all threads are done with the rounds before these
+      if (threadIdx.x < 32 && base >= ROWS * step)
+#pragma unroll
+        for (int k = 0; k < ROWS; ++k) {
+          const int64_t next = base + (RING - ROWS + k) * step;
+          if (next < a.m) fetch(next, (slot == 0 ? RING : slot) - ROWS + k);
+        }
+    }
 #pragma unroll
     for (int k = 0; k < ROWS; ++k) {
       // dx = rstd (g - c1) - rstd^2 c2 (x - mean), with c2 = rstd mean(g (x - mean))
       const float c1 = -s1[k] * inv_n * rstd[k], c2 = -s2[k] * inv_n * rstd[k] * rstd[k] * rstd[k];
+      if (FETCHED) load_row(k);  // once more: both rows' would not fit in registers beside the sums
 #pragma unroll
       for (int q = 0; q < PAIRS; ++q) {
         const float2 xm = add2(pair_at(vx[k], q), both(shift[k]));
@@ -577,11 +643,19 @@ __global__ void __launch_bounds__(bwd_threads(TPR), VEC > 1 ? bwd_ctas_per_sm(TP
         if (live[k] && c < nv) store_pack<T, VEC>(dx + static_cast<int64_t>(c) * VEC, vx[k][i]);
       }
     }
+    if constexpr (FETCHED) {
+      slot += ROWS;
+      if (slot == RING) {
+        slot = 0;
+        parity ^= 1;
+      }
+    }
   }
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   if (!a.sums) return;
   float* out = a.partial + static_cast<int64_t>(blockIdx.x) * 2 * a.n;
   if constexpr (GROUPS > 1) {
+    if constexpr (FETCHED) __syncthreads();  // the ring's last rows have been read
 #pragma unroll
     for (int i = 0; i < MAXV; ++i)
 #pragma unroll
@@ -598,12 +672,19 @@ __global__ void __launch_bounds__(bwd_threads(TPR), VEC > 1 ? bwd_ctas_per_sm(TP
 #pragma unroll
     for (int i = 0; i < MAXV; ++i) {
       const int c = t + i * TPR;
-      if (c < nv)
+      if (c < nv) {
+        if constexpr (VEC == 1) {
+          out[c] = half_of(sw, i);
+          out[n + c] = half_of(sb, i);
+        } else {
 #pragma unroll
-        for (int j = 0; j < VEC; ++j) {
-          out[c * VEC + j] = half_of(sw, i * VEC + j);
-          out[n + c * VEC + j] = half_of(sb, i * VEC + j);
+          for (int j = 0; j < VEC; j += 4) {
+            const int q = (i * VEC + j) / 2;
+            *reinterpret_cast<float4*>(out + c * VEC + j) = make_float4(sw[q].x, sw[q].y, sw[q + 1].x, sw[q + 1].y);
+            *reinterpret_cast<float4*>(out + n + c * VEC + j) = make_float4(sb[q].x, sb[q].y, sb[q + 1].x, sb[q + 1].y);
+          }
         }
+      }
     }
   }
 }
@@ -661,8 +742,16 @@ __global__ void __launch_bounds__(1024) ln_bwd_join_kernel(const float* partial,
   const int64_t which = dw == nullptr ? 1 : blockIdx.y;
   float s = 0.0f;
   if (c < n)
-#pragma unroll 5
-    for (int p = warp; p < ctas; p += 32) s += partial[(static_cast<int64_t>(p) * 2 + which) * n + c];
+    for (int p0 = warp; p0 < ctas; p0 += 32 * 10) {  // (two CTAs an SM: once, all loads in flight)
+      float v[10];
+#pragma unroll
+      for (int i = 0; i < 10; ++i) {
+        const int p = p0 + 32 * i;
+        v[i] = p < ctas ? partial[(static_cast<int64_t>(p) * 2 + which) * n + c] : 0.0f;
+      }
+#pragma unroll
+      for (int i = 0; i < 10; ++i) s += v[i];
+    }
   part[warp][lane] = s;
   __syncthreads();
   if (warp == 0 && c < n) {
@@ -747,12 +836,20 @@ template <class T, class WT, int VEC>
 int run_bwd(const BwdArgs& a, cudaStream_t st) {
   const int tpr = row_threads(a.n);
   const unsigned ctas = static_cast<unsigned>(bwd_ctas(a.m, a.n));
-#define H3B_LN_BWD(TPR)                                                                                            \
-  case TPR: {                                                                                                      \
-    constexpr int threads = bwd_threads(TPR), bytes = threads > TPR ? threads * EPT * 8 : 0;                       \
-    static_assert(bytes <= 40 * 1024, "dynamic shared memory without an attribute");                               \
-    ln_bwd_kernel<T, WT, VEC, TPR><<<ctas, threads, bytes, st>>>(a);                                               \
-    break;                                                                                                         \
+#define H3B_LN_BWD(TPR)                                                                                             \
+  case TPR: {                                                                                                       \
+    constexpr int threads = bwd_threads(TPR), joined = threads > TPR ? threads * EPT * 8 : 0;                       \
+    constexpr int ring = bwd_ring(sizeof(T), VEC, TPR) ? RING * 2 * threads * EPT * static_cast<int>(sizeof(T)) : 0; \
+    constexpr int most = ring > joined ? ring : joined;                                                             \
+    static_assert(bwd_ctas_per_sm(TPR) * (most + 3 * 1024) <= 227 * 1024, "shared memory of the CTAs of an SM");    \
+    if constexpr (most > 40 * 1024) {                                                                               \
+      static h3b::OncePerDevice once;                                                                               \
+      const int rc = h3b::prepare(once, ln_bwd_kernel<T, WT, VEC, TPR>, most);                                      \
+      if (rc != H3B_OK) return rc;                                                                                  \
+    }                                                                                                               \
+    const int used = ring > 0 ? static_cast<int>(RING * 2 * (threads / TPR) * a.n * sizeof(T)) : 0;                 \
+    ln_bwd_kernel<T, WT, VEC, TPR><<<ctas, threads, used > joined ? used : joined, st>>>(a);                        \
+    break;                                                                                                          \
   }
   switch (tpr) {
     H3B_LN_BWD(8)
