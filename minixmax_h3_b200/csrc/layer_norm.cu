@@ -480,8 +480,11 @@ constexpr int bwd_threads(int tpr) { return tpr < 256 ? 256 : tpr; }
 constexpr int bwd_ctas_per_sm(int tpr) { return bwd_threads(tpr) == 256 ? 2 : 1; }
 
 // 16-bit rows come through a ring of RING rounds in shared memory, fetched by
-// bulk copies while earlier ones are worked on (32-bit rows have twice the
-// bytes for the same arithmetic, and two CTAs' loads in turn are enough).
+// bulk copies while earlier ones are worked on: 16384 x 4096 without the sums
+// takes 70 us, with four rounds 77, with loads into registers 78.  Rows of a
+// warp would wait for each other (131072 x 512: 84, without the ring 71).
+// 32-bit rows have twice the bytes for the same arithmetic, and two CTAs'
+// loads in turn are enough.
 constexpr int RING = 6;
 constexpr bool bwd_ring(int element, int vec, int tpr) { return element == 2 && vec > 1 && tpr >= 64 && tpr <= 512; }
 
@@ -490,10 +493,10 @@ __global__ void __launch_bounds__(bwd_threads(TPR), VEC > 1 ? bwd_ctas_per_sm(TP
   constexpr int MAXV = EPT / VEC;
   constexpr int THREADS = bwd_threads(TPR);
   constexpr int GROUPS = THREADS / TPR;
-  // Rows that a group works on together, their loads in flight and their sums
-  // behind one barrier: two of 16 bits (16384 x 4096 in 96 us, one 111), one
-  // of 32 (8192 x 4096 in 82 us, two 96).  CTAs of 1024 threads have 64
-  // registers a thread: one row, and the weights again for each (from L1).
+  // Rows that a group works on together, their sums behind one barrier: two
+  // of 16 bits (32768 x 2048 in 77 us, one 86), one of 32 (8192 x 4096 in 70
+  // us, two are a sixth slower).  CTAs of 1024 threads have 64 registers a
+  // thread: one row, and the weights again for each (from L1).
   constexpr bool SMALL = THREADS == 1024;
   constexpr int ROWS = SMALL || sizeof(T) == 4 || VEC == 1 ? 1 : 2;
   constexpr bool FETCHED = bwd_ring(sizeof(T), VEC, TPR);
