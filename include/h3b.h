@@ -417,9 +417,15 @@ H3B_API int h3b_rotary(const h3b_rotary_args* args, h3b_stream_t stream);
  * rstd: fp32 [m], both or neither.  m below 2^31, n at most 2^30; any
  * alignment (16-byte words where n, the strides and the pointers allow).
  */
-H3B_API int h3b_layer_norm_fwd(const void* x, const void* w, const void* b, void* y, float* mean, float* rstd,
-                               int dtype, int wdtype, int64_t m, int64_t n, int64_t ldx, int64_t ldy, float eps,
-                               h3b_stream_t stream);
+typedef struct {
+  const void *x, *w, *b;
+  void* y;
+  float *mean, *rstd;
+  int64_t m, n, ldx, ldy;
+  double eps;
+  int32_t dtype, wdtype;
+} h3b_layer_norm_args;
+H3B_API int h3b_layer_norm_fwd(const h3b_layer_norm_args* args, h3b_stream_t stream);
 
 /* Bytes of h3b_layer_norm_bwd's workspace on the current device. */
 H3B_API int h3b_layer_norm_bwd_workspace(int64_t m, int64_t n, int64_t* bytes);
@@ -432,10 +438,14 @@ H3B_API int h3b_layer_norm_bwd_workspace(int64_t m, int64_t n, int64_t* bytes);
  * needed only with dw or db; calls that overlap need one each.  m = 0 does
  * nothing (dw and db are not written).
  */
-H3B_API int h3b_layer_norm_bwd(const void* dy, const void* x, const void* w, const float* mean, const float* rstd,
-                               void* dx, void* dw, void* db, int dtype, int wdtype, int64_t m, int64_t n,
-                               int64_t lddy, int64_t ldx, int64_t lddx, void* workspace, int64_t workspace_bytes,
-                               h3b_stream_t stream);
+typedef struct {
+  const void *dy, *x, *w;
+  const float *mean, *rstd;
+  void *dx, *dw, *db, *workspace;
+  int64_t m, n, lddy, ldx, lddx, workspace_bytes;
+  int32_t dtype, wdtype;
+} h3b_layer_norm_bwd_args;
+H3B_API int h3b_layer_norm_bwd(const h3b_layer_norm_bwd_args* args, h3b_stream_t stream);
 
 /* --------------------------------------------------- orthogonalised updates */
 

@@ -60,9 +60,9 @@ SIGNATURES: dict[str, list] = {
     "h3b_kv8_attention": [c_ptr] * 3 + [c_int] + [c_i64] * 11 + [c_ptr] * 4 + [c_int, c_i64, c_i64, c_ptr, c_i64, c_ptr,
                                                                                c_int, c_f32, c_ptr, c_i64, c_ptr],
     "h3b_rotary": [c_ptr, c_ptr],
-    "h3b_layer_norm_fwd": [c_ptr] * 6 + [c_int, c_int] + [c_i64] * 4 + [c_f32, c_ptr],
+    "h3b_layer_norm_fwd": [c_ptr, c_ptr],
     "h3b_layer_norm_bwd_workspace": [c_i64, c_i64, c_ptr],
-    "h3b_layer_norm_bwd": [c_ptr] * 8 + [c_int, c_int] + [c_i64] * 5 + [c_ptr, c_i64, c_ptr],
+    "h3b_layer_norm_bwd": [c_ptr, c_ptr],
     "h3b_orthogonalize_workspace": [c_i64] * 3 + [c_ptr],
     "h3b_orthogonalize": [c_ptr, c_ptr, c_int] + [c_i64] * 6 + [c_f32] * 4 + [c_ptr, c_i64, c_ptr],
     "h3b_selftest_wait_timeout": [c_ptr] * 7 + [c_i64] * 3 + [c_ptr],

@@ -911,17 +911,19 @@ int check(int dtype, int wdtype, int64_t m, int64_t n) {
 
 }  // namespace
 
-extern "C" int h3b_layer_norm_fwd(const void* x, const void* w, const void* b, void* y, float* mean, float* rstd,
-                                  int dtype, int wdtype, int64_t m, int64_t n, int64_t ldx, int64_t ldy, float eps,
-                                  h3b_stream_t stream) {
+extern "C" int h3b_layer_norm_fwd(const h3b_layer_norm_args* p, h3b_stream_t stream) {
+  if (p == nullptr) return H3B_ERR_ARG;
+  const int dtype = p->dtype, wdtype = p->wdtype;
+  const int64_t m = p->m, n = p->n;
   const int rc = check(dtype, wdtype, m, n);
   if (rc != H3B_OK) return rc;
   if (m == 0) return H3B_OK;
-  if (x == nullptr || y == nullptr || (mean == nullptr) != (rstd == nullptr) || !(eps >= 0.0f)) return H3B_ERR_ARG;
-  const FwdArgs a{x, w, b, y, mean, rstd, m, n, ldx, ldy, eps};
+  if (p->x == nullptr || p->y == nullptr || (p->mean == nullptr) != (p->rstd == nullptr) || !(p->eps >= 0.0))
+    return H3B_ERR_ARG;
+  const FwdArgs a{p->x, p->w, p->b, p->y, p->mean, p->rstd, m, n, p->ldx, p->ldy, static_cast<float>(p->eps)};
   const int64_t vec = 16 / element_bytes(dtype);
-  const bool wide = n % vec == 0 && (m == 1 || (ldx % vec == 0 && ldy % vec == 0)) && h3b::aligned16(x) &&
-                    h3b::aligned16(y) && h3b::aligned16(w) && h3b::aligned16(b);
+  const bool wide = n % vec == 0 && (m == 1 || (a.ldx % vec == 0 && a.ldy % vec == 0)) && h3b::aligned16(a.x) &&
+                    h3b::aligned16(a.y) && h3b::aligned16(a.w) && h3b::aligned16(a.b);
   const auto st = reinterpret_cast<cudaStream_t>(stream);
   H3B_LN_TYPES(run_fwd, a, st);
 }
@@ -933,22 +935,24 @@ extern "C" int h3b_layer_norm_bwd_workspace(int64_t m, int64_t n, int64_t* bytes
   return H3B_OK;
 }
 
-extern "C" int h3b_layer_norm_bwd(const void* dy, const void* x, const void* w, const float* mean, const float* rstd,
-                                  void* dx, void* dw, void* db, int dtype, int wdtype, int64_t m, int64_t n,
-                                  int64_t lddy, int64_t ldx, int64_t lddx, void* workspace, int64_t workspace_bytes,
-                                  h3b_stream_t stream) {
+extern "C" int h3b_layer_norm_bwd(const h3b_layer_norm_bwd_args* p, h3b_stream_t stream) {
+  if (p == nullptr) return H3B_ERR_ARG;
+  const int dtype = p->dtype, wdtype = p->wdtype;
+  const int64_t m = p->m, n = p->n;
   const int rc = check(dtype, wdtype, m, n);
   if (rc != H3B_OK) return rc;
   if (m == 0) return H3B_OK;
-  if (dy == nullptr || x == nullptr || mean == nullptr || rstd == nullptr || dx == nullptr) return H3B_ERR_ARG;
-  const bool sums = dw != nullptr || db != nullptr;
-  if (sums && (workspace == nullptr || workspace_bytes < bwd_ctas(m, n) * 2 * n * static_cast<int64_t>(sizeof(float))))
+  if (p->dy == nullptr || p->x == nullptr || p->mean == nullptr || p->rstd == nullptr || p->dx == nullptr)
     return H3B_ERR_ARG;
-  if (sums && !h3b::aligned16(workspace)) return H3B_ERR_ALIGN;
-  const BwdArgs a{dy, x, w, mean, rstd, dx, dw, db, static_cast<float*>(workspace), m, n, lddy, ldx, lddx, sums ? 1 : 0};
+  const bool sums = p->dw != nullptr || p->db != nullptr;
+  if (sums && (p->workspace == nullptr || p->workspace_bytes < bwd_ctas(m, n) * 2 * n * static_cast<int64_t>(sizeof(float))))
+    return H3B_ERR_ARG;
+  if (sums && !h3b::aligned16(p->workspace)) return H3B_ERR_ALIGN;
+  const BwdArgs a{p->dy,   p->x, p->w,    p->mean, p->rstd, p->dx,        p->dw, p->db, static_cast<float*>(p->workspace),
+                  m,       n,    p->lddy, p->ldx,  p->lddx, sums ? 1 : 0};
   const int64_t vec = 16 / element_bytes(dtype);
-  const bool wide = n % vec == 0 && (m == 1 || (ldx % vec == 0 && lddy % vec == 0 && lddx % vec == 0)) &&
-                    h3b::aligned16(x) && h3b::aligned16(dy) && h3b::aligned16(dx) && h3b::aligned16(w);
+  const bool wide = n % vec == 0 && (m == 1 || (a.ldx % vec == 0 && a.lddy % vec == 0 && a.lddx % vec == 0)) &&
+                    h3b::aligned16(a.x) && h3b::aligned16(a.dy) && h3b::aligned16(a.dx) && h3b::aligned16(a.w);
   const auto st = reinterpret_cast<cudaStream_t>(stream);
   H3B_LN_TYPES(run_bwd, a, st);
 }

@@ -900,6 +900,10 @@ def _check_stats(name: str, stats: Optional[torch.Tensor], m: int) -> None:
         raise ValueError(f"{name}: stats is a contiguous fp32 [2, rows] tensor")
 
 
+# h3b_layer_norm_args, h3b_layer_norm_bwd_args
+_NORM_ARGS, _NORM_BWD_ARGS = struct.Struct("@6P4qd2i"), struct.Struct("@9P6q2i")
+
+
 def _flat_rows(x: torch.Tensor) -> tuple[torch.Tensor, int]:
     """x as rows of its last axis with unit column stride, and their stride."""
     if x.is_contiguous():
@@ -919,9 +923,10 @@ def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Opt
     (bf16, fp16 or fp32; weight and bias of x's type or fp32): x's shape and
     type, contiguous, or ``out`` (contiguous).  stats, if given (fp32
     [2, rows]), receives each row's mean and 1 / sqrt(var + eps), which
-    layer_norm_bwd needs.  out may be x itself and else overlaps nothing.  Rows with a unit last stride and one row stride are
-    read in place, other layouts copied first.  A row that holds NaN or an
-    infinity gives NaN.  For gradients by autograd see ``modules.layer_norm``."""
+    layer_norm_bwd needs.  out may be x itself and else overlaps nothing.  Rows
+    with a unit last stride and one row stride are read in place, other layouts
+    copied first.  A row that holds NaN or an infinity gives NaN.  For gradients
+    by autograd see ``modules.layer_norm``."""
     _one_device("layer_norm", x, weight, bias, out, stats)
     wdtype = _check_norm("layer_norm", x, weight, bias)
     if not 0.0 <= eps < float("inf"):
@@ -937,9 +942,10 @@ def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Opt
         return out
     x2, ld = _flat_rows(x)
     weight, bias = _packed(weight), _packed(bias)
-    at = None if stats is None else stats.data_ptr()
-    _call_on(x, "h3b_layer_norm_fwd", x2.data_ptr(), _ptr(weight), _ptr(bias), out.data_ptr(), at,
-             None if at is None else at + 4 * m, _FLOATS[x.dtype], wdtype, m, n, ld, n, float(eps), _stream(x))
+    at = 0 if stats is None else stats.data_ptr()
+    args = _NORM_ARGS.pack(x2.data_ptr(), 0 if weight is None else weight.data_ptr(), 0 if bias is None else bias.data_ptr(),
+                           out.data_ptr(), at, at and at + 4 * m, m, n, ld, n, eps, _FLOATS[x.dtype], wdtype)
+    _call_on(x, "h3b_layer_norm_fwd", args, _stream(x))
     return out
 
 
@@ -958,20 +964,23 @@ def layer_norm_bwd(dout: torch.Tensor, x: torch.Tensor, stats: torch.Tensor, wei
     m = x.numel() // n
     _check_stats("layer_norm_bwd", stats, m)
     dx = torch.empty_like(x, memory_format=torch.contiguous_format)
-    new = torch.zeros if m == 0 else torch.empty
-    dw = new(n, dtype=weight.dtype, device=x.device) if weight is not None and weight_grad else None
-    db = new(n, dtype=weight.dtype, device=x.device) if weight is not None and bias_grad else None
+    weight = _packed(weight)
+    new = torch.zeros_like if m == 0 else torch.empty_like
+    dw = new(weight) if weight is not None and weight_grad else None
+    db = new(weight) if weight is not None and bias_grad else None
     if m == 0:
         return dx, dw, db
     x2, ldx = _flat_rows(x)
     dout2, lddy = _flat_rows(dout)
-    weight = _packed(weight)
     ws = None
     if dw is not None or db is not None:
         ws = _workspace_on("h3b_layer_norm_bwd_workspace", x, m, n)
-    _call_on(x, "h3b_layer_norm_bwd", dout2.data_ptr(), x2.data_ptr(), _ptr(weight), stats.data_ptr(),
-             stats.data_ptr() + 4 * m, dx.data_ptr(), _ptr(dw), _ptr(db), _FLOATS[x.dtype], wdtype, m, n, lddy, ldx, n,
-             _ptr(ws), 0 if ws is None else ws.numel(), _stream(x))
+    at = stats.data_ptr()
+    args = _NORM_BWD_ARGS.pack(
+        dout2.data_ptr(), x2.data_ptr(), 0 if weight is None else weight.data_ptr(), at, at + 4 * m, dx.data_ptr(),
+        0 if dw is None else dw.data_ptr(), 0 if db is None else db.data_ptr(), 0 if ws is None else ws.data_ptr(), m, n,
+        lddy, ldx, n, 0 if ws is None else ws.numel(), _FLOATS[x.dtype], wdtype)
+    _call_on(x, "h3b_layer_norm_bwd", args, _stream(x))
     return dx, dw, db
 
 

@@ -303,13 +303,15 @@ def test_c_entries_arguments(cuda, n, dt):
     y, stats = torch.empty_like(x), torch.empty(2, 5, device=cuda)
     code, stream = {BF16: 0, F32: 2}[dt], torch.cuda.current_stream().cuda_stream
     assert code == ops._FLOATS[dt]
-    _lib.call("h3b_layer_norm_fwd", x.data_ptr(), None, b.data_ptr(), y.data_ptr(), stats.data_ptr(),
-              stats.data_ptr() + 20, code, code, 5, n, n, n, 1e-5, stream)
+    at = stats.data_ptr()
+    _lib.call("h3b_layer_norm_fwd", ops._NORM_ARGS.pack(x.data_ptr(), 0, b.data_ptr(), y.data_ptr(), at, at + 20, 5, n, n, n,
+                                                        1e-5, code, code), stream)
     close(y, *formulas(x, None, b, 1e-5)["y"], "y")
     ws = torch.empty(1 << 24, dtype=torch.uint8, device=cuda)
     with pytest.raises(RuntimeError):
-        _lib.call("h3b_layer_norm_bwd", x.data_ptr(), x.data_ptr(), None, stats.data_ptr(), stats.data_ptr() + 20,
-                  y.data_ptr(), b.data_ptr(), None, code, code, 5, n, n, n, n, ws.data_ptr() + 2, ws.numel() - 2, stream)
+        _lib.call("h3b_layer_norm_bwd", ops._NORM_BWD_ARGS.pack(
+            x.data_ptr(), x.data_ptr(), 0, at, at + 20, y.data_ptr(), b.data_ptr(), 0, ws.data_ptr() + 2, 5, n, n, n, n,
+            ws.numel() - 2, code, code), stream)
 
 
 @pytest.mark.parametrize("dt", [F32, BF16])
