@@ -45,7 +45,7 @@
 //
 // Tiles: 256 x 256 by CTA pairs (cta_group::2, each CTA stages 128 rows of
 // both operands); where those are too few for the SMs, 128 x 128 by one CTA;
-// where those are, too, by a cluster of two or four, each with a part of K, that
+// where those are, too, by a cluster of two to four, each with a part of K, that
 // hand each other their sums through distributed shared memory.
 // Warp 0 loads (TMA, zero beyond the matrix), warp 1 issues the products,
 // eight warps add and store; two accumulators in turn, so that products go on
@@ -599,11 +599,15 @@ __global__ void __launch_bounds__(THREADS, 1)
             }, col0, 15);
         }
       } else {
-        // Part q gets the parts' sums of its 128 / PARTS columns, in blocks
-        // of 32 columns, four columns of all rows after the other (a warp
-        // writes 512 bytes at once), where the operands' stages were.
-        static_assert(PARTS == 1 || PARTS == 2 || PARTS == 4, "whole blocks for each part");
-        constexpr int OWN = 4 / PARTS;  // blocks of a part
+        // Each part gets the parts' sums of one or two of the four blocks of
+        // 32 columns (of three parts the first gets two), four columns of
+        // all rows after the other (a warp writes 512 bytes at once), where
+        // the operands' stages were.
+        static_assert(PARTS >= 1 && PARTS <= 4, "a block for each part");
+        constexpr int OWN = PARTS == 4 ? 1 : 2;  // blocks of a part, at most
+        const auto owner = [](int block) { return PARTS == 3 ? max(block - 1, 0) : block / OWN; };
+        const int first = PARTS == 3 ? (part == 0 ? 0 : part + 1) : part * OWN;
+        const bool two = OWN == 2 && (PARTS != 3 || part == 0);
         auto share = [&](int from, int block, int p) {
           return static_cast<uint32_t>((((from * OWN + block) * 8 + p) * BM + quad * 32 + lane) * 16);
         };
@@ -612,19 +616,20 @@ __global__ void __launch_bounds__(THREADS, 1)
 #pragma unroll
         for (int i = 0; i < MINE; ++i) {
           const int block = half + 2 * i;
-          const uint32_t to = mapa_shared(smem_u32(smem), static_cast<uint32_t>(block / OWN));
+          const int to_part = owner(block), at = block == 0 ? 0 : owner(block - 1) == to_part ? 1 : 0;
+          const uint32_t to = mapa_shared(smem_u32(smem), static_cast<uint32_t>(to_part));
 #pragma unroll
           for (int p = 0; p < 8; ++p) {
             const float* x = &acc[2 * i + (p >> 2)][4 * (p & 3)];
-            asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(to + share(part, block % OWN, p)), "f"(x[0]), "f"(x[1]),
+            asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(to + share(part, at, p)), "f"(x[0]), "f"(x[1]),
                          "f"(x[2]), "f"(x[3])
                          : "memory");
           }
         }
         cluster_sync();
-        const int block = OWN == 2 ? half : 0, col0 = tile.j * BN + (part * OWN + block) * 32;
+        const int block = two ? half : 0, col0 = tile.j * BN + (first + block) * 32;
         // with one block for both halves' warps they share its planes: G's and K's, or first and second
-        const int planes = OWN == 2 ? 15 : OP == GRAM && args.with_k ? (half ? 12 : 3) : (half ? 2 : 1);
+        const int planes = two ? 15 : OP == GRAM && args.with_k ? (half ? 12 : 3) : (half ? 2 : 1);
         if (row0 < args.rows && col0 < args.cols)
           store([&](float(&v)[32]) {
 #pragma unroll
@@ -925,22 +930,24 @@ int product(const Maps& a, const Maps& b, const Maps& out, const Maps& k, const 
   const int64_t sms = h3b::num_sms();
   const int64_t t1 = tiles_of(args.rows, args.cols, args.batch, 128, OP != MUL);
   const int64_t t2 = tiles_of(args.rows, args.cols, args.batch, 256, OP != MUL);
-  // Rounds of tiles times what one takes, in cycles: a stage of K in three
+  // (Ties go to the fewer CTAs.)  Rounds of tiles times what one takes, in cycles: a stage of K in three
   // products 1280 (one CTA; its operand reads and copies share the
   // shared-memory port) or 1540 (a pair's tile of four times the size), a
   // third of it in one; the beginning and the stores 8000, 14000, and 10000
-  // where CTAs hand their sums over.  Of clusters of four with a whole SM
-  // each, 33 run at once on 148 SMs.
+  // where CTAs hand their sums over.  Of clusters of three with a whole SM
+  // for each CTA 45 run at once on 148 SMs, of four 33.
   const int64_t stages = (args.k + KB - 1) / KB, stage = SPLIT ? 1281 : 427;
   const auto rounds = [](int64_t n, int64_t at_once) { return (n + at_once - 1) / at_once; };
   const int64_t single = rounds(t1, sms) * (stages * stage + 8000);
   const int64_t pair = rounds(t2, sms / 2) * (stages * stage * 6 / 5 + 14000);
   const int64_t halves = rounds(t1, sms / 2) * ((stages + 1) / 2 * stage + 10000);
+  const int64_t thirds = rounds(t1, sms * 45 / 148) * ((stages + 2) / 3 * stage + 10000);
   const int64_t quarters = rounds(t1, sms * 9 / 40) * ((stages + 3) / 4 * stage + 10000);
-  const int64_t best = std::min(std::min(single, pair), std::min(halves, quarters));
+  const int64_t best = std::min({single, pair, halves, thirds, quarters});
   if (single == best) return launch<1, 1, OP, SPLIT>(a, b, out, k, args, t1, stream);
   if (pair == best) return launch<2, 1, OP, SPLIT>(a, b, out, k, args, t2, stream);
   if (halves == best) return launch<1, 2, OP, SPLIT>(a, b, out, k, args, t1, stream);
+  if (thirds == best) return launch<1, 3, OP, SPLIT>(a, b, out, k, args, t1, stream);
   return launch<1, 4, OP, SPLIT>(a, b, out, k, args, t1, stream);
 }
 
