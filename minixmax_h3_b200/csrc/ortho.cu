@@ -45,8 +45,11 @@
 //
 // Tiles: 256 x 256 by CTA pairs (cta_group::2, each CTA stages 128 rows of
 // both operands); where those are too few for the SMs, 128 x 128 by one CTA;
-// where those are, too, by a cluster of two to four, each with a part of K, that
-// hand each other their sums through distributed shared memory.
+// where those are, too, 128 x 64 or 128 x 32 (a launch takes 1 us by itself and
+// the stores of 128 columns 3.4: five steps of 200 x 200 bf16 in 91 us, with
+// 128 columns 121), or, over a long K, 128 x 128 by a cluster of two to four,
+// each with a part of K, that hand each other their sums through distributed
+// shared memory.
 // Warp 0 loads (TMA, zero beyond the matrix), warp 1 issues the products,
 // eight warps add and store; two accumulators in turn, so that products go on
 // meanwhile.  Stores go through shared memory as TMA blocks of 32 x 32 (lanes
@@ -85,14 +88,19 @@ static_assert(4 * REGS_CTL + 8 * REGS_EPI <= 12 * LAUNCH_REGS, "register split e
 enum Op { GRAM = 0, POLY = 1, MUL = 2 };
 
 // PAIR: CTAs of a 256 x 256 tile.  PARTS: CTAs that share the K of a 128 x 128
-// tile (PAIR = 1).
-template <int PAIR, int PARTS, int OP, int SPLIT>
+// tile (PAIR = 1).  COLS: columns of a CTA's part of a 128 x 128 tile (where
+// all three are 1, 1 and less than 128).
+template <int PAIR, int PARTS, int OP, int SPLIT, int COLS>
 struct Cfg {
   static_assert(PAIR == 1 || PARTS == 1, "pairs take all of K");
-  static constexpr int BN = 128 * PAIR;
+  static_assert(COLS == 128 || (PAIR * PARTS == 1 && (COLS == 64 || (COLS == 32 && OP != MUL))), "narrow tiles");
+  static constexpr int SIDE = 128 * PAIR;      // of a tile
+  static constexpr int SLICES = 128 / COLS;    // of a tile, a CTA's work each
+  static constexpr int BN = COLS * PAIR;
+  static constexpr int B_BYTES = COLS * 128;   // a plane of B
   static constexpr int PLANES = SPLIT ? 2 : 1;
-  static constexpr int STAGE_BYTES = 2 * PLANES * PLANE_BYTES;  // A planes, then B planes
-  static constexpr int STAGES = SPLIT ? 3 : 6;
+  static constexpr int STAGE_BYTES = PLANES * (PLANE_BYTES + B_BYTES);  // A planes, then B planes
+  static constexpr int STAGES = SPLIT ? (COLS == 128 ? 3 : 4) : 6;
   static constexpr int TMEM_COLS = 2 * BN;  // two accumulators
   static constexpr int CHUNK = SPLIT ? 2 : 8;  // stages of K an accumulator takes
   static constexpr uint32_t IDESC = idesc_f16_f32(BM * PAIR, BN, 0, OP == MUL ? 1 : 0);
@@ -128,9 +136,9 @@ struct __align__(8) Barriers {
   int consumed;
 };
 
-template <int PAIR, int PARTS, int OP, int SPLIT>
+template <int PAIR, int PARTS, int OP, int SPLIT, int COLS>
 constexpr size_t smem_bytes() {
-  using C = Cfg<PAIR, PARTS, OP, SPLIT>;
+  using C = Cfg<PAIR, PARTS, OP, SPLIT, COLS>;
   return 1024 + static_cast<size_t>(C::STAGES) * C::STAGE_BYTES + EPI_WARPS * BLOCKS * BLOCK_BYTES + sizeof(Barriers);
 }
 
@@ -275,15 +283,15 @@ H3B_DEV void store_elements(const Args& args, int batch, int row, int col0, cons
 H3B_DEV void launch_next() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 H3B_DEV void wait_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 
-template <int PAIR, int PARTS, int OP, int SPLIT>
+template <int PAIR, int PARTS, int OP, int SPLIT, int COLS>
 __global__ void __launch_bounds__(THREADS, 1)
     ortho_product(const __grid_constant__ CUtensorMap a_hi, const __grid_constant__ CUtensorMap a_lo,
                   const __grid_constant__ CUtensorMap b_hi, const __grid_constant__ CUtensorMap b_lo,
                   const __grid_constant__ CUtensorMap out_hi, const __grid_constant__ CUtensorMap out_lo,
                   const __grid_constant__ CUtensorMap k_hi, const __grid_constant__ CUtensorMap k_lo,
                   const Args args) {
-  using C = Cfg<PAIR, PARTS, OP, SPLIT>;
-  constexpr int STAGES = C::STAGES, BN = C::BN;
+  using C = Cfg<PAIR, PARTS, OP, SPLIT, COLS>;
+  constexpr int STAGES = C::STAGES, BN = C::BN, SIDE = C::SIDE, SLICES = C::SLICES;
   constexpr bool SYMMETRIC = OP != MUL;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -294,9 +302,9 @@ __global__ void __launch_bounds__(THREADS, 1)
   const bool leader = rank == 0;
   const int part = PARTS > 1 ? static_cast<int>(cluster_ctarank()) : 0;
   const int cluster = static_cast<int>(blockIdx.x) / (PAIR * PARTS), n_clusters = static_cast<int>(gridDim.x) / (PAIR * PARTS);
-  const int row_tiles = (args.rows + BN - 1) / BN, col_tiles = (args.cols + BN - 1) / BN;  // tiles are square
+  const int row_tiles = (args.rows + SIDE - 1) / SIDE, col_tiles = (args.cols + SIDE - 1) / SIDE;  // tiles are square
   const int per_matrix = SYMMETRIC ? row_tiles * (row_tiles + 1) / 2 : row_tiles * col_tiles;
-  const int num_tiles = per_matrix * args.batch;
+  const int num_tiles = per_matrix * args.batch * SLICES;  // or slices
   // stages of K: this CTA's (PARTS > 1: a launch has a cluster for each tile)
   const int all_k = (args.k + KB - 1) / KB, share_k = (all_k + PARTS - 1) / PARTS;
   const int first_k = part * share_k, nk = max(0, min(share_k, all_k - first_k));
@@ -346,11 +354,11 @@ __global__ void __launch_bounds__(THREADS, 1)
       int it = 0;
       bool ok = true;
       const bool two_b = SPLIT && args.b_lo;
-      const uint32_t bytes = PAIR * PLANE_BYTES * (C::PLANES + (two_b ? 2 : 1));
+      const uint32_t bytes = PAIR * (PLANE_BYTES * C::PLANES + C::B_BYTES * (two_b ? 2 : 1));
       for (int t = cluster; t < num_tiles && ok; t += n_clusters) {
-        const Tile tile = tile_at<SYMMETRIC>(t, per_matrix, col_tiles);
-        const int m0 = tile.i * BN + static_cast<int>(rank) * BM;
-        const int n0 = tile.j * BN + static_cast<int>(rank) * BM;  // this CTA's 128 of the tile's columns
+        const Tile tile = tile_at<SYMMETRIC>(t / SLICES, per_matrix, col_tiles);
+        const int m0 = tile.i * SIDE + static_cast<int>(rank) * BM;
+        const int n0 = tile.j * SIDE + static_cast<int>(rank) * BM + t % SLICES * COLS;  // this CTA's of the tile's columns
         for (int kb = 0; kb < nk; ++kb, ++it) {
           const int s = it % STAGES, round = it / STAGES;
           if (round > 0 && !mbar_wait(&bars->empty[s], (round - 1) & 1, &g_status, 1, abort_flag)) {
@@ -372,13 +380,13 @@ __global__ void __launch_bounds__(THREADS, 1)
           auto load_b = [&](uint8_t* dst, const CUtensorMap* map) {
             if constexpr (OP == MUL) {  // boxes of 64 columns x 64 rows of K
               load(dst, map, n0, (first_k + kb) * KB);
-              load(dst + PLANE_BYTES / 2, map, n0 + 64, (first_k + kb) * KB);
+              if constexpr (COLS == 128) load(dst + PLANE_BYTES / 2, map, n0 + 64, (first_k + kb) * KB);
             } else {
               load(dst, map, (first_k + kb) * KB, n0);
             }
           };
           load_b(stage + C::PLANES * PLANE_BYTES, &b_hi);
-          if (two_b) load_b(stage + (C::PLANES + 1) * PLANE_BYTES, &b_lo);
+          if (two_b) load_b(stage + C::PLANES * PLANE_BYTES + C::B_BYTES, &b_lo);
         }
       }
       if (!ok || *abort_flag) {
@@ -423,7 +431,7 @@ __global__ void __launch_bounds__(THREADS, 1)
           const uint32_t sb = stage + C::PLANES * PLANE_BYTES;
           const uint64_t bd = OP == MUL ? sdesc_mnmajor_sw128(sb, PLANE_BYTES / 2, 1024) : sdesc_kmajor_sw128(sb);
           constexpr uint32_t B_STEP = OP == MUL ? 2048 >> 4 : 2;  // 16 elements of K
-          constexpr uint32_t NEXT = PLANE_BYTES >> 4;             // the second plane
+          constexpr uint32_t NEXT = PLANE_BYTES >> 4, NEXT_B = C::B_BYTES >> 4;  // the second planes
           const bool last = kb % C::CHUNK == C::CHUNK - 1 || kb == nk - 1;
           if (elect_one()) {
             auto mma = [&](uint64_t x, uint64_t y, bool add) {
@@ -438,7 +446,7 @@ __global__ void __launch_bounds__(THREADS, 1)
               for (int j = 0; j < 4; ++j) mma(ad + NEXT + 2 * j, bd + B_STEP * j, add || j != 0);
               if (two_b) {
 #pragma unroll
-                for (int j = 0; j < 4; ++j) mma(ad + 2 * j, bd + NEXT + B_STEP * j, true);
+                for (int j = 0; j < 4; ++j) mma(ad + 2 * j, bd + NEXT_B + B_STEP * j, true);
               }
             }
 #pragma unroll
@@ -478,7 +486,9 @@ __global__ void __launch_bounds__(THREADS, 1)
     // --------------------------------------------------------- stores
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(REGS_EPI));
     const int quad = warp & 3, half = (warp - 4) >> 2;  // TMEM lane quadrant; alternate 32-column chunks
-    constexpr int MINE = BN / 64;                         // this warp's chunks of 32 columns
+    constexpr int MINE = BN > 32 ? BN / 64 : 1;           // this warp's chunks of 32 columns
+    // (both halves take a single chunk, and share its planes)
+    const auto chunk = [&](int i) { return COLS == 32 ? 0 : half + 2 * i; };
     Blocks out{blocks + (warp - 4) * BLOCKS * BLOCK_BYTES, lane, 0};
     int local = 0;
     bool ok = true;
@@ -501,7 +511,7 @@ __global__ void __launch_bounds__(THREADS, 1)
 #pragma unroll
         for (int i = 0; i < 2 * MINE; ++i) {
           uint32_t r[16];
-          tmem_ld16(t_row + (half + 2 * (i >> 1)) * 32 + (i & 1) * 16, r);
+          tmem_ld16(t_row + chunk(i >> 1) * 32 + (i & 1) * 16, r);
           tc_wait_ld();
           reg_fence16(r);
           if (i == 2 * MINE - 1) {
@@ -522,8 +532,8 @@ __global__ void __launch_bounds__(THREADS, 1)
       if constexpr (PARTS == 1) {
         if (!ok) break;
       }
-      const Tile tile = tile_at<SYMMETRIC>(t, per_matrix, col_tiles);
-      const int row0 = tile.i * BN + static_cast<int>(rank) * BM + quad * 32, row = row0 + lane;
+      const Tile tile = tile_at<SYMMETRIC>(t / SLICES, per_matrix, col_tiles);
+      const int row0 = tile.i * SIDE + static_cast<int>(rank) * BM + quad * 32, row = row0 + lane;
       const float f = args.factor != nullptr ? args.factor[tile.batch] : 1.0f;
       const float beta = (OP == GRAM ? f * f : OP == MUL ? f : 1.0f) * args.beta;
       // Stores 32 columns from col0 of the sums that sums(v) puts into v; of
@@ -587,16 +597,18 @@ __global__ void __launch_bounds__(THREADS, 1)
           }
         }
       };
+      // where both halves' warps store a chunk: G's planes and K's, or first and second
+      const int shared_planes = OP == GRAM && args.with_k ? (half ? 12 : 3) : (half ? 2 : 1);
       if constexpr (PARTS == 1) {
         if (row0 >= args.rows) continue;  // warp-uniform, as all that follows
 #pragma unroll
         for (int i = 0; i < MINE; ++i) {
-          const int col0 = tile.j * BN + (half + 2 * i) * 32;
+          const int col0 = tile.j * SIDE + t % SLICES * COLS + chunk(i) * 32;
           if (col0 < args.cols)
             store([&](float(&v)[32]) {
 #pragma unroll
               for (int j = 0; j < 32; ++j) v[j] = acc[2 * i + (j >> 4)][j & 15];
-            }, col0, 15);
+            }, col0, COLS > 32 ? 15 : shared_planes);
         }
       } else {
         // Each part gets the parts' sums of one or two of the four blocks of
@@ -627,9 +639,8 @@ __global__ void __launch_bounds__(THREADS, 1)
           }
         }
         cluster_sync();
-        const int block = two ? half : 0, col0 = tile.j * BN + (first + block) * 32;
-        // with one block for both halves' warps they share its planes: G's and K's, or first and second
-        const int planes = two ? 15 : OP == GRAM && args.with_k ? (half ? 12 : 3) : (half ? 2 : 1);
+        const int block = two ? half : 0, col0 = tile.j * SIDE + (first + block) * 32;
+        const int planes = two ? 15 : shared_planes;
         if (row0 < args.rows && col0 < args.cols)
           store([&](float(&v)[32]) {
 #pragma unroll
@@ -879,11 +890,12 @@ struct Maps {
 };
 
 // Boxes of a map of planes: an operand whose rows are K (128 rows by 64
-// elements of K), one whose columns are K (64 rows of K by 64), stores.
-enum Boxes { BY_ROWS, BY_COLUMNS, STORES };
+// elements of K; 64 and 32 for narrow tiles), one whose columns are K (64 rows
+// of K by 64), stores.
+enum Boxes { BY_ROWS, BY_ROWS_64, BY_ROWS_32, BY_COLUMNS, STORES };
 
 int encode(Maps* maps, const Planes& p, int64_t batch, int64_t rows, int64_t cols, int64_t ld, Boxes boxes) {
-  const uint32_t high = boxes == BY_ROWS ? 128 : boxes == BY_COLUMNS ? 64 : 32;
+  const uint32_t high = boxes == BY_ROWS ? 128 : boxes == BY_COLUMNS || boxes == BY_ROWS_64 ? 64 : 32;
   for (int i = 0; i < 2; ++i) {
     const int rc = h3b::encode_3d(i == 0 ? &maps->hi : &maps->lo, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, i == 0 ? p.hi : p.lo,
                                   cols, rows, batch, ld * 2, rows * ld * 2, boxes == STORES ? 32 : 64, high, 1,
@@ -893,12 +905,12 @@ int encode(Maps* maps, const Planes& p, int64_t batch, int64_t rows, int64_t col
   return H3B_OK;
 }
 
-template <int PAIR, int PARTS, int OP, int SPLIT>
+template <int PAIR, int PARTS, int OP, int SPLIT, int COLS = 128>
 int launch(const Maps& a, const Maps& b, const Maps& out, const Maps& k, const Args& args, int64_t tiles, cudaStream_t stream) {
-  constexpr size_t smem = smem_bytes<PAIR, PARTS, OP, SPLIT>();
+  constexpr size_t smem = smem_bytes<PAIR, PARTS, OP, SPLIT, COLS>();
   static_assert(smem <= 227 * 1024, "shared memory budget");
   static h3b::OncePerDevice once;
-  const auto kernel = ortho_product<PAIR, PARTS, OP, SPLIT>;
+  const auto kernel = ortho_product<PAIR, PARTS, OP, SPLIT, COLS>;
   const int rc = h3b::prepare(once, kernel, smem, LAUNCH_REGS);
   if (rc != H3B_OK) return rc;
   // every tile has a cluster of its own where parts share it
@@ -925,15 +937,25 @@ int64_t tiles_of(int64_t rows, int64_t cols, int64_t batch, int64_t t, bool symm
   return batch * (symmetric ? r * (r + 1) / 2 : r * c);
 }
 
+// The second operand of a product, for tiles of 128 columns and narrow ones.
+struct Operand {
+  Maps all, narrow;
+};
+
+// Columns of narrow tiles, if they are taken (one round of them): as few as
+// there are SMs for.
+int narrow_columns(int64_t tiles, bool symmetric) { return symmetric && 4 * tiles <= h3b::num_sms() ? 32 : 64; }
+
 template <int OP, int SPLIT>
-int product(const Maps& a, const Maps& b, const Maps& out, const Maps& k, const Args& args, cudaStream_t stream) {
+int product(const Maps& a, const Operand& b, const Maps& out, const Maps& k, const Args& args, cudaStream_t stream) {
   const int64_t sms = h3b::num_sms();
   const int64_t t1 = tiles_of(args.rows, args.cols, args.batch, 128, OP != MUL);
   const int64_t t2 = tiles_of(args.rows, args.cols, args.batch, 256, OP != MUL);
-  // (Ties go to the fewer CTAs.)  Rounds of tiles times what one takes, in cycles: a stage of K in three
-  // products 1280 (one CTA; its operand reads and copies share the
-  // shared-memory port) or 1540 (a pair's tile of four times the size), a
-  // third of it in one; the beginning and the stores 8000, 14000, and 10000
+  // Rounds of tiles times what one takes, in cycles (fitted to 200 x 200 up to
+  // 4096 x 4096): a stage of K in three products 1280 (one CTA; its operand
+  // reads and copies share the shared-memory port), 1540 (a pair's tile of
+  // four times the size), 1100 and 900 (64 and 32 columns), a third of it in
+  // one; the beginning and the stores 8000, 14000, 4500 and 3800, and 10000
   // where CTAs hand their sums over.  Of clusters of three with a whole SM
   // for each CTA 45 run at once on 148 SMs, of four 33.
   const int64_t stages = (args.k + KB - 1) / KB, stage = SPLIT ? 1281 : 427;
@@ -943,16 +965,25 @@ int product(const Maps& a, const Maps& b, const Maps& out, const Maps& k, const 
   const int64_t halves = rounds(t1, sms / 2) * ((stages + 1) / 2 * stage + 10000);
   const int64_t thirds = rounds(t1, sms * 45 / 148) * ((stages + 2) / 3 * stage + 10000);
   const int64_t quarters = rounds(t1, sms * 9 / 40) * ((stages + 3) / 4 * stage + 10000);
-  const int64_t best = std::min({single, pair, halves, thirds, quarters});
-  if (single == best) return launch<1, 1, OP, SPLIT>(a, b, out, k, args, t1, stream);
-  if (pair == best) return launch<2, 1, OP, SPLIT>(a, b, out, k, args, t2, stream);
-  if (halves == best) return launch<1, 2, OP, SPLIT>(a, b, out, k, args, t1, stream);
-  if (thirds == best) return launch<1, 3, OP, SPLIT>(a, b, out, k, args, t1, stream);
-  return launch<1, 4, OP, SPLIT>(a, b, out, k, args, t1, stream);
+  const int narrow = narrow_columns(t1, OP != MUL);
+  const int64_t slices = 128 / narrow * t1 > sms ? INT64_MAX
+                         : narrow == 64          ? stages * stage * 6 / 7 + 4500
+                                                 : stages * stage * 7 / 10 + 3800;
+  const int64_t best = std::min({single, pair, halves, thirds, quarters, slices});
+  if (single == best) return launch<1, 1, OP, SPLIT>(a, b.all, out, k, args, t1, stream);
+  if (pair == best) return launch<2, 1, OP, SPLIT>(a, b.all, out, k, args, t2, stream);
+  if (slices == best) {
+    if constexpr (OP != MUL)
+      if (narrow == 32) return launch<1, 1, OP, SPLIT, 32>(a, b.narrow, out, k, args, 4 * t1, stream);
+    return launch<1, 1, OP, SPLIT, 64>(a, b.narrow, out, k, args, 2 * t1, stream);
+  }
+  if (halves == best) return launch<1, 2, OP, SPLIT>(a, b.all, out, k, args, t1, stream);
+  if (thirds == best) return launch<1, 3, OP, SPLIT>(a, b.all, out, k, args, t1, stream);
+  return launch<1, 4, OP, SPLIT>(a, b.all, out, k, args, t1, stream);
 }
 
 template <int OP>
-int product(bool split, const Maps& a, const Maps& b, const Maps& out, const Maps& k, const Args& args, cudaStream_t stream) {
+int product(bool split, const Maps& a, const Operand& b, const Maps& out, const Maps& k, const Args& args, cudaStream_t stream) {
   return split ? product<OP, 1>(a, b, out, k, args, stream) : product<OP, 0>(a, b, out, k, args, stream);
 }
 
@@ -1010,20 +1041,35 @@ int run(const h3b::OrthoCall& call, uint8_t* ws, cudaStream_t stream) {
                                in, planes);
   if (rc != H3B_OK) return rc;
 
-  // X by rows and by columns, both sets of planes; G, K and B by rows; all as stores
-  Maps x_k[2], x_n[2], x_out[2], g_k, g_out, k_k, k_out, b_k, b_out, result;
+  // X by rows and by columns, both sets of planes; G, K (where the square is
+  // not completed) and B by rows; all as stores
+  const double ca = call.a, cb = call.b, cc = call.c;
+  Maps x_out[2], g_out, k_out, b_k, b_out, result;
+  Operand x_k[2], x_n[2], g_k, k_k;
   const auto enc = [&](Maps* maps, const Planes& p, int64_t cols, int64_t pitch, Boxes boxes) {
     if (rc == H3B_OK) rc = encode(maps, p, batch, l.small, cols, pitch, boxes);
   };
+  const bool square = dtype != H3B_F32 && cc != 0.0 && cb * cb <= 64.0 * cc * cc;
+  const int64_t tiles = tiles_of(l.small, l.small, batch, 128, true);  // of the symmetric products
+  const Boxes narrow = narrow_columns(tiles, true) == 32 ? BY_ROWS_32 : BY_ROWS_64;
+  const auto enc_second = [&](Operand* o, const Planes& p, int64_t cols, int64_t pitch) {
+    enc(&o->all, p, cols, pitch, BY_ROWS);
+    if (2 * tiles <= h3b::num_sms()) enc(&o->narrow, p, cols, pitch, narrow);
+  };
   for (int i = 0; i < (steps > 1 ? 2 : 1); ++i) {
-    enc(&x_k[i], xs[i], l.large, l.x_ld, BY_ROWS);
-    enc(&x_n[i], xs[i], l.large, l.x_ld, BY_COLUMNS);
+    enc_second(&x_k[i], xs[i], l.large, l.x_ld);
+    enc(&x_n[i].all, xs[i], l.large, l.x_ld, BY_COLUMNS);
+    x_n[i].narrow = x_n[i].all;
     if (steps > 1) enc(&x_out[i], xs[i], l.large, l.x_ld, STORES);
   }
-  enc(&g_k, g, l.small, l.g_ld, BY_ROWS);
+  enc_second(&g_k, g, l.small, l.g_ld);
   enc(&g_out, g, l.small, l.g_ld, STORES);
-  enc(&k_k, k, l.small, l.g_ld, BY_ROWS);
-  enc(&k_out, k, l.small, l.g_ld, STORES);
+  k_k = g_k;
+  k_out = g_out;
+  if (!square) {
+    enc_second(&k_k, k, l.small, l.g_ld);
+    enc(&k_out, k, l.small, l.g_ld, STORES);
+  }
   enc(&b_k, b, l.small, l.g_ld, BY_ROWS);
   enc(&b_out, b, l.small, l.g_ld, STORES);
   const bool result_tma = row_bytes % 16 == 0 && h3b::aligned16(out);
@@ -1038,8 +1084,6 @@ int run(const h3b::OrthoCall& call, uint8_t* ws, cudaStream_t stream) {
     result = g_out;  // not used
   }
 
-  const double ca = call.a, cb = call.b, cc = call.c;
-  const bool square = dtype != H3B_F32 && cc != 0.0 && cb * cb <= 64.0 * cc * cc;
   for (int s = 0; s < steps && rc == H3B_OK; ++s) {
     const bool first = s == 0, last = s == steps - 1, bf16 = dtype == H3B_BF16;
     // planes in pairs: the products with X, and those that make B
@@ -1058,7 +1102,7 @@ int run(const h3b::OrthoCall& call, uint8_t* ws, cudaStream_t stream) {
     p.k_beta = call.c;
     p.k_diagonal = static_cast<float>(SCALE * (b_pairs ? cb : cb + 2.0 * cc));
     p.with_k = !square;
-    rc = product<GRAM>(b_pairs && !x_exact, x_k[cur], x_k[cur], g_out, k_out, p, stream);
+    rc = product<GRAM>(b_pairs && !x_exact, x_k[cur].all, x_k[cur], g_out, k_out, p, stream);
     if (rc != H3B_OK) break;
 
     p.factor = nullptr;
@@ -1066,7 +1110,7 @@ int run(const h3b::OrthoCall& call, uint8_t* ws, cudaStream_t stream) {
     p.out_lo = x_pairs;
     if (square) p.beta *= call.c;
     p.diagonal = static_cast<float>(SCALE * (square ? ca - cb * cb / (4.0 * cc) : b_pairs ? ca : ca + cb + cc));
-    rc = product<POLY>(b_pairs, g_k, square ? g_k : k_k, b_out, b_out, p, stream);
+    rc = product<POLY>(b_pairs, g_k.all, k_k, b_out, b_out, p, stream);
     if (rc != H3B_OK) break;
 
     p.factor = first ? factor : nullptr;

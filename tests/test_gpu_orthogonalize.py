@@ -215,3 +215,10 @@ def test_refusals(cuda):
             (ValueError, (x,), {"out": torch.empty(9, 8, device=cuda).T})):
         with pytest.raises(error):
             ops.orthogonalize(*args, **kw)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("b,m,n", [(4, 512, 520), (20, 130, 200), (1, 161, 161), (1, 225, 1000), (2, 350, 290), (1, 900, 1100)])
+def test_narrow_tiles(cuda, b, m, n, dtype):
+    """Tiles of 64 and 32 columns, some of them wholly beyond the matrix."""
+    check(gradient(cuda, b, m, n, dtype=dtype, seed=n), 5)
