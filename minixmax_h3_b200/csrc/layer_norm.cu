@@ -6,8 +6,9 @@
 //
 // Both directions are bound by HBM: x is read and y written once; backward, x
 // and dy are read and dx written once.  Arithmetic is packed, two elements an
-// instruction, or it would bind first.  A group of threads holds a row in
-// registers, so the variance is taken about the mean in a second pass over registers, and what
+// instruction, or it would bind first.  Rows are held in registers, each by a
+// group of threads (forward mostly four rows by a few warps together), so the
+// variance is taken about the mean in a second pass over registers, and what
 // rounding the mean left over is taken off with it: var = mean(d^2) -
 // mean(d)^2, d = x - mean, with mean(d) of the size of a rounding.
 //
