@@ -329,3 +329,18 @@ def test_rows_share_warps(cuda, n, dt):
         assert torch.equal(wide[:rows], want[4:4 + rows]) and torch.equal(own, stats[:, 4:4 + rows])
         assert (wide[rows] == 7).all()
         check(x[:rows], w, b)
+
+
+@pytest.mark.parametrize("dt", [F16, BF16])
+@pytest.mark.parametrize("m,n", [(9001, 520), (5003, 1048), (2777, 2056), (1201, 4104), (1999, 8192)])
+def test_many_rounds(cuda, m, n, dt):
+    """Several turns of the backward pass's ring, groups that end within a round, rows apart in memory."""
+    g = torch.Generator(device=cuda).manual_seed(m)
+    x = torch.randn(m, n + 24, generator=g, device=cuda).to(dt)[:, 8:n + 8]
+    w, b = torch.randn(n, generator=g, device=cuda), torch.randn(n, generator=g, device=cuda)
+    check(x, w, b)
+    stats = torch.empty(2, m, device=cuda)
+    ops.layer_norm(x, w, b, stats=stats)
+    one = torch.randn(1, n, generator=g, device=cuda).to(dt)  # a gradient that is one row for all
+    got, want = (ops.layer_norm_bwd(dy, x, stats, w) for dy in (one.expand(m, n), one.expand(m, n).contiguous()))
+    assert all(torch.equal(s, t) for s, t in zip(got, want))
