@@ -458,8 +458,8 @@ H3B_API int h3b_orthogonalize_workspace(int64_t batch, int64_t m, int64_t n, int
  * X = x / (|x| + eps), Frobenius norm, `steps` times
  * X <- a X + (b G + c G G) X, G = X X^T (for m > n the same on X^T).  out:
  * [batch, m, n] contiguous, may be x where that is contiguous.  dtype
- * H3B_BF16, H3B_F16 or H3B_F32 for both.  Products of f16 planes in pairs,
- * fp32 sums; elements of the iterates must stay below 64.  m, n at most
+ * H3B_BF16, H3B_F16 or H3B_F32 for both.  Products of f16 planes in pairs
+ * (22 bits) with fp32 sums for every type, one rounding of the result; elements of the iterates must stay below 64.  m, n at most
  * 65536, batch at most 65535, batch * max(m, n) at most 2^29, steps at most
  * 1000.  The workspace is 16-byte aligned; calls that overlap need one each.
  */

@@ -21,15 +21,12 @@
 // operands 13 %.  So operands are pairs of f16 planes, v = hi + lo (22 bits),
 // and a product is hi hi + lo hi + hi lo in one accumulator (what is left out
 // is 2^-22).  That is as near as 32-bit arithmetic comes at a fifth of its
-// time on CUDA cores.  Two products are exact or late enough to save on:
-// x in 16 bits is one plane as it is (its 8 or 11 bits are kept by a scale of
-// a power of two; the norm's fraction goes into the first epilogues).  And of
-// a bf16 result, after whose last step nothing grows, that step takes one
-// plane, and the one before it makes H and B of one: X is near an orthogonal
-// factor by then, H near -0.2 and B near 1 (with K, both steps are written
-// about H = G - 1), so that what is rounded to 11 bits is no larger than what
-// it makes.  That leaves 0.0004 to 0.001 of the root mean square beside the
-// result's own rounding of 0.0017.
+// time on CUDA cores, for every step of every type: a bf16 result's last steps
+// in one plane were a fifth faster (4096 x 4096 in 2.73 ms, so 3.40), but off
+// by 0.0006 to 0.0015, up to what the result's own rounding is (0.0017).  One product saves a plane without a loss: x in 16 bits is one as it
+// is, by a scale of a power of two (the norm's fraction goes into the first
+// epilogues; its 8 or 11 bits are whole down to 2^-24 of the norm, smaller
+// elements are off by 2^-35 of the norm at most, as any element of a pair is).
 //
 // Planes hold SCALE * value: f16 has its full precision between 2^-24 and 64
 // of the value then.  Elements are below the largest singular value, 1.2 for
@@ -40,8 +37,8 @@
 // elements of K; over a long row that is a bias (2^-25 for each of 768 sums
 // at K = 4096: 1e-5 of G's diagonal, 3e-5 of the result).  An accumulator
 // therefore takes 128 elements of K, the small products before the large
-// ones (512 where a plane of 11 bits decides), and the storing warps add
-// accumulators in registers, rounding to nearest.
+// ones, and the storing warps add accumulators in registers, rounding to
+// nearest.
 //
 // Tiles: 256 x 256 by CTA pairs (cta_group::2, each CTA stages 128 rows of
 // both operands); where those are too few for the SMs, 128 x 128 by one CTA;
@@ -72,6 +69,7 @@ namespace {
 constexpr float SCALE = 1024.0f;
 constexpr int BM = 128;            // accumulator rows of a CTA
 constexpr int KB = 64;             // elements of K a stage (128 bytes a row)
+constexpr int CHUNK = 2;           // stages of K an accumulator takes
 constexpr int PLANE_BYTES = BM * 128;
 constexpr int BLOCK_BYTES = 32 * 64;  // a block on its way out: 32 rows of 64 bytes
 constexpr int BLOCKS = 2;             // of each storing warp
@@ -102,7 +100,6 @@ struct Cfg {
   static constexpr int STAGE_BYTES = PLANES * (PLANE_BYTES + B_BYTES);  // A planes, then B planes
   static constexpr int STAGES = SPLIT ? (COLS == 128 ? 3 : 4) : 6;
   static constexpr int TMEM_COLS = 2 * BN;  // two accumulators
-  static constexpr int CHUNK = SPLIT ? 2 : 8;  // stages of K an accumulator takes
   static constexpr uint32_t IDESC = idesc_f16_f32(BM * PAIR, BN, 0, OP == MUL ? 1 : 0);
 };
 
@@ -115,7 +112,6 @@ struct Args {
   int rows, cols, k;       // of the product, per matrix
   int batch;
   int b_lo;                // SPLIT: the B operand has a second plane
-  int out_lo;              // second planes are stored (something reads them)
   int with_k;              // GRAM: K is stored beside G
   const float* factor;     // [batch], x's scale: value = factor * plane (the first step), or null
   float beta, diagonal;    // beta * product + diagonal * 1
@@ -412,7 +408,7 @@ __global__ void __launch_bounds__(THREADS, 1)
       for (int t = cluster; t < num_tiles && ok; t += n_clusters) {
         for (int kb = 0; kb < nk; ++kb, ++it) {
           const int buf = local & 1;
-          if (kb % C::CHUNK == 0) {
+          if (kb % CHUNK == 0) {
             const int use = local >> 1;
             if (use > 0 && !warp_wait<false, PAIR == 2>(&bars->acc_empty[buf], (use - 1) & 1, 2, abort_flag)) {
               ok = false;
@@ -432,7 +428,7 @@ __global__ void __launch_bounds__(THREADS, 1)
           const uint64_t bd = OP == MUL ? sdesc_mnmajor_sw128(sb, PLANE_BYTES / 2, 1024) : sdesc_kmajor_sw128(sb);
           constexpr uint32_t B_STEP = OP == MUL ? 2048 >> 4 : 2;  // 16 elements of K
           constexpr uint32_t NEXT = PLANE_BYTES >> 4, NEXT_B = C::B_BYTES >> 4;  // the second planes
-          const bool last = kb % C::CHUNK == C::CHUNK - 1 || kb == nk - 1;
+          const bool last = kb % CHUNK == CHUNK - 1 || kb == nk - 1;
           if (elect_one()) {
             auto mma = [&](uint64_t x, uint64_t y, bool add) {
               if constexpr (PAIR == 2)
@@ -440,7 +436,7 @@ __global__ void __launch_bounds__(THREADS, 1)
               else
                 mma_f16_ss(d_tmem, x, y, C::IDESC, add);
             };
-            const bool add = kb % C::CHUNK != 0;
+            const bool add = kb % CHUNK != 0;
             if constexpr (SPLIT != 0) {
 #pragma unroll
               for (int j = 0; j < 4; ++j) mma(ad + NEXT + 2 * j, bd + B_STEP * j, add || j != 0);
@@ -500,7 +496,7 @@ __global__ void __launch_bounds__(THREADS, 1)
 #pragma unroll
           for (int j = 0; j < 16; ++j) acc[i][j] = 0.0f;
       }
-      for (int kb = 0; kb < nk; kb += C::CHUNK, ++local) {
+      for (int kb = 0; kb < nk; kb += CHUNK, ++local) {
         const int buf = local & 1, use = local >> 1;
         if (!warp_wait<true>(&bars->acc_full[buf], use & 1, 4, abort_flag)) {
           ok = false;
@@ -589,7 +585,7 @@ __global__ void __launch_bounds__(THREADS, 1)
             out.put(hi, w, false, col0, row0, tile.batch);
             if (mirror) out.put(hi, w, true, col0, row0, tile.batch);
           }
-          if (args.out_lo && (planes & (2 << (2 * m)))) {
+          if (planes & (2 << (2 * m))) {
 #pragma unroll
             for (int j = 0; j < 16; ++j) w[j] = pack_f16x2(v[2 * j], v[2 * j + 1]);
             out.put(lo, w, false, col0, row0, tile.batch);
@@ -982,11 +978,6 @@ int product(const Maps& a, const Operand& b, const Maps& out, const Maps& k, con
   return launch<1, 4, OP, SPLIT>(a, b.all, out, k, args, t1, stream);
 }
 
-template <int OP>
-int product(bool split, const Maps& a, const Operand& b, const Maps& out, const Maps& k, const Args& args, cudaStream_t stream) {
-  return split ? product<OP, 1>(a, b, out, k, args, stream) : product<OP, 0>(a, b, out, k, args, stream);
-}
-
 // A small kernel that starts while the one before it ends.
 template <class... Params, class... Values>
 int launch_after(void (*kernel)(Params...), dim3 grid, cudaStream_t stream, Values... values) {
@@ -1085,9 +1076,7 @@ int run(const h3b::OrthoCall& call, uint8_t* ws, cudaStream_t stream) {
   }
 
   for (int s = 0; s < steps && rc == H3B_OK; ++s) {
-    const bool first = s == 0, last = s == steps - 1, bf16 = dtype == H3B_BF16;
-    // planes in pairs: the products with X, and those that make B
-    const bool x_pairs = !(bf16 && last), b_pairs = !(bf16 && s >= steps - 2);
+    const bool first = s == 0, last = s == steps - 1;
     const bool x_exact = first && exact;
     const int cur = s & 1;
     Args p{};
@@ -1096,21 +1085,20 @@ int run(const h3b::OrthoCall& call, uint8_t* ws, cudaStream_t stream) {
     p.k = static_cast<int>(l.large);
     p.factor = first ? factor : nullptr;
     p.b_lo = 1;
-    p.out_lo = b_pairs;
     p.beta = 1.0f / SCALE;
-    p.diagonal = square ? static_cast<float>(SCALE * cb / (2.0 * cc)) : b_pairs ? 0.0f : -SCALE;
+    p.diagonal = square ? static_cast<float>(SCALE * cb / (2.0 * cc)) : 0.0f;
     p.k_beta = call.c;
-    p.k_diagonal = static_cast<float>(SCALE * (b_pairs ? cb : cb + 2.0 * cc));
+    p.k_diagonal = static_cast<float>(SCALE * cb);
     p.with_k = !square;
-    rc = product<GRAM>(b_pairs && !x_exact, x_k[cur].all, x_k[cur], g_out, k_out, p, stream);
+    rc = x_exact ? product<GRAM, 0>(x_k[cur].all, x_k[cur], g_out, k_out, p, stream)
+                 : product<GRAM, 1>(x_k[cur].all, x_k[cur], g_out, k_out, p, stream);
     if (rc != H3B_OK) break;
 
     p.factor = nullptr;
     p.k = p.rows;
-    p.out_lo = x_pairs;
     if (square) p.beta *= call.c;
-    p.diagonal = static_cast<float>(SCALE * (square ? ca - cb * cb / (4.0 * cc) : b_pairs ? ca : ca + cb + cc));
-    rc = product<POLY>(b_pairs, g_k.all, k_k, b_out, b_out, p, stream);
+    p.diagonal = static_cast<float>(SCALE * (square ? ca - cb * cb / (4.0 * cc) : ca));
+    rc = product<POLY, 1>(g_k.all, k_k, b_out, b_out, p, stream);
     if (rc != H3B_OK) break;
 
     p.factor = first ? factor : nullptr;
@@ -1126,9 +1114,8 @@ int run(const h3b::OrthoCall& call, uint8_t* ws, cudaStream_t stream) {
       p.result_batch = m * n;
       p.result_ld = n;
     }
-    p.out_lo = 1;
     const Maps& to = last ? result : x_out[cur ^ 1];
-    rc = product<MUL>(x_pairs, b_k, x_n[cur], to, to, p, stream);
+    rc = product<MUL, 1>(b_k, x_n[cur], to, to, p, stream);
   }
   return rc;
 }

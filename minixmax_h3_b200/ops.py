@@ -998,11 +998,13 @@ def orthogonalize(x: torch.Tensor, *, steps: int = 5,
     Returns a contiguous tensor of x's shape and type, or ``out`` (contiguous;
     x itself may be given).
 
-    Products run in pairs of f16 planes (22 bits) with fp32 sums; the last
-    step of a bf16 result in one.  Elements of the iterates must stay below
-    64, which any coefficients that converge keep.  A zero matrix gives zeros
-    (eps > 0); NaN or an infinity makes its matrix NaN.  The result is
-    bit-reproducible.  Matrices with a unit last stride are read in place."""
+    Products run in pairs of f16 planes (22 bits) with fp32 sums whatever the
+    type, and the result is rounded once: it is as near as 32-bit arithmetic
+    comes.  Elements of the iterates must stay below 64, which any coefficients
+    that converge keep.  A zero matrix gives zeros (eps > 0); NaN or an
+    infinity makes its matrix NaN (with no steps an infinity leaves zeros
+    beside it).  The result is bit-reproducible.  Matrices with a unit last
+    stride are read in place."""
     _one_device("orthogonalize", x, out)
     if x.dtype not in _FLOATS:
         raise TypeError("orthogonalize expects bf16, fp16 or fp32 matrices")
