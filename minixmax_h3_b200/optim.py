@@ -18,9 +18,10 @@ class Muon(torch.optim.Optimizer):
 
     Parameters are matrices, or stacks [..., m, n] of them, each
     orthogonalised by itself.  Those of one shape are orthogonalised in one
-    call.  Averages are fp32; ``dtype`` is the type in which an update is
-    orthogonalised (bf16: the result is within its rounding; fp32 costs
-    about half more).  Gradients and parameters may be of any floating
+    call.  Averages are fp32; ``dtype`` is the type that an update is rounded
+    to and orthogonalised in.  bf16's rounding is felt by what is small beside
+    an update's large directions, fp32 costs little more; fp16 does not hold
+    the range of averaged gradients and is taken as fp32.  Gradients and parameters may be of any floating
     type: a parameter is updated in its own, so what is below its rounding is
     lost there.  State and steps follow the parameters' devices; a step can be
     captured into a CUDA graph once the averages exist."""
@@ -81,7 +82,9 @@ class Muon(torch.optim.Optimizer):
             averages.append(state["average"])
         torch._foreach_lerp_(averages, grads, 1.0 - momentum)
         updates = torch._foreach_lerp(grads, averages, momentum) if group["nesterov"] else averages
-        u = torch.stack(list(updates)).to(group["dtype"])
+        u = torch.stack(list(updates))
+        if group["dtype"] != torch.float16:  # (1e-8 would be nothing, 1e5 infinite)
+            u = u.to(group["dtype"])
         u = ops.orthogonalize(u, steps=group["steps"], coefficients=group["coefficients"], eps=group["eps"], out=u)
         rows, columns = shape[-2:]
         if group["weight_decay"]:
