@@ -255,7 +255,8 @@ class CrossAttention(nn.Module):
     handed out or written into a cache.
 
     The projections are quantised and have no gradients, so the layer has none:
-    an input that requires one raises.  Training uses
+    an input that requires one raises, and so does a norm whose weight or bias
+    was made to (they are not, as the layer is built).  Training uses
     ``TrainableCrossAttention``, whose ``quantized`` gives a layer of this
     class, or ``attention.cross_attention`` between projections of its own."""
 
@@ -280,7 +281,8 @@ class CrossAttention(nn.Module):
     @staticmethod
     def _without_gradients(*ts: Optional[torch.Tensor]) -> None:
         if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in ts):
-            raise RuntimeError("CrossAttention has no gradients: detach its inputs, or use attention.cross_attention")
+            raise RuntimeError("CrossAttention has no gradients: detach its inputs and its norm's parameters, or use "
+                               "TrainableCrossAttention or attention.cross_attention")
 
     def _turned(self, x: torch.Tensor, positions: Optional[torch.Tensor], name: str, in_place: bool) -> torch.Tensor:
         if (self.rope is None) != (positions is None):
@@ -316,7 +318,7 @@ class CrossAttention(nn.Module):
             raise ValueError("CrossAttention.forward takes one of cond, kv and cache")
         if cond is None and cond_positions is not None:
             raise ValueError("CrossAttention: cond_positions come with cond")
-        self._without_gradients(x, cond, *(kv or ()))
+        self._without_gradients(x, cond, *(kv or ()), *(() if self.norm is None else self.norm.parameters()))
         b, s, _ = x.shape
         h = x if self.norm is None else self.norm(x)
         q = self.q_proj(h.reshape(b * s, -1)).view(b, s, self.heads, self.head_dim)
