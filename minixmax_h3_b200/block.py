@@ -238,7 +238,21 @@ class Attention(nn.Module):
         return self.out_proj.forward_fused(o, amax=amax_o)
 
 
-class CrossAttention(nn.Module):
+class _WithRope(nn.Module):
+    """A layer whose rotations (``rope``) follow its parameters to another device."""
+
+    rope: Optional["ops.Rotary"] = None
+
+    def _apply(self, fn, *args, **kwargs):
+        super()._apply(fn, *args, **kwargs)
+        if self.rope is not None and not self.rope.turns.is_meta:
+            device = fn(torch.empty(0, device=self.rope.turns.device)).device
+            if device.type != "meta":  # (their values are nowhere else)
+                self.rope = self.rope.to(device)
+        return self
+
+
+class CrossAttention(_WithRope):
     """Cross attention of video tokens to a text encoder's states, beside the
     joint-sequence ``Attention``: quantised query, key/value and output
     projections around ops.cross_attention, with ``kv_heads`` shared key heads
@@ -335,7 +349,7 @@ class CrossAttention(nn.Module):
         return self.out_proj(o.view(b * s, self.heads * self.head_dim)).view(b, s, -1)
 
 
-class TrainableCrossAttention(nn.Module):
+class TrainableCrossAttention(_WithRope):
     """``CrossAttention`` as it is trained, with dense projections: layer norm
     -> query projection, key and value projection of the encoder's states,
     rotary positions (with ``rope``), cross attention, output projection.

@@ -10,7 +10,7 @@ import ctypes
 import functools
 import math
 import struct
-from dataclasses import dataclass
+from dataclasses import dataclass, replace
 from typing import Optional, Sequence
 
 import torch
@@ -733,6 +733,11 @@ class Rotary:
         object.__setattr__(self, "sections", tuple(self.sections))
         if not 1 <= len(self.sections) <= 3 or min(self.sections) < 0 or sum(self.sections) != self.turns.shape[0]:
             raise ValueError(f"Rotary: sections {self.sections} of {self.turns.shape[0]} pairs (one to three axes)")
+
+    def to(self, device) -> "Rotary":
+        """The same rotations on ``device`` (themselves, if they are there)."""
+        turns = self.turns.to(device)
+        return self if turns is self.turns else replace(self, turns=turns)
 
     @classmethod
     def from_frequencies(cls, frequencies: Sequence[float] | torch.Tensor, *, sections: Optional[Sequence[int]] = None,

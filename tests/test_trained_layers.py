@@ -39,3 +39,43 @@ def test_a_norm_that_wants_gradients_raises(monkeypatch):
         layer(x, cond)
     bare = block.CrossAttention(64, 1, 64, 32, operations=Layers).requires_grad_(True)
     assert bare(x, cond).shape == x.shape
+
+
+# ----------------------------------------------------------------------------- rotations move with their layer
+
+
+def test_rotations_move(monkeypatch):
+    rope = ops.Rotary.build(32, factor=1.5, interleaved=True, device="cpu")
+    assert rope.to("cpu") is rope
+    far = rope.to("meta")
+    assert far.turns.is_meta and (far.sections, far.interleaved, far.factor) == (rope.sections, True, 1.5)
+    layers = [block.CrossAttention(64, 1, 64, 32, rope=rope), block.TrainableCrossAttention(64, 1, 64, 32, rope=rope)]
+    moves = []
+    monkeypatch.setattr(ops.Rotary, "to", lambda self, device: moves.append(torch.device(device)) or self)
+    for layer in layers:
+        outer = torch.nn.Sequential(torch.nn.Sequential(layer))
+        outer.to("cpu", torch.float64)
+        assert moves.pop() == torch.device("cpu") and layer.rope is rope and rope.turns.dtype == torch.int64
+        outer.half().share_memory()
+        assert len(moves) == 2 and rope.turns.dtype == torch.int64
+        moves.clear()
+        outer.to("meta")  # values would be lost
+        assert not moves and not layer.rope.turns.is_meta
+        outer.to_empty(device="cpu")
+        assert moves.pop() == torch.device("cpu") and torch.equal(layer.rope.turns, rope.turns)
+        moves.clear()
+    block.CrossAttention(64, 1, 64, 32).to("cpu")
+    assert not moves
+
+
+@pytest.mark.gpu
+def test_layer_built_elsewhere(cuda):
+    """Built on the CPU, moved and called: the same bits as built in its place."""
+    torch.manual_seed(0)
+    here = block.TrainableCrossAttention(128, 2, 64, 128, rope=ops.Rotary.build(64, device="cpu"))
+    there = block.TrainableCrossAttention(128, 2, 64, 128, rope=ops.Rotary.build(64, device=cuda), device=cuda)
+    there.load_state_dict(here.state_dict())
+    here = here.to(cuda)
+    x, cond = torch.randn(2, 9, 128, device=cuda), torch.randn(2, 5, 128, device=cuda)
+    where = {"positions": torch.arange(9, device=cuda), "cond_positions": torch.arange(5, device=cuda)}
+    assert torch.equal(here(x, cond, **where), there(x, cond, **where))
