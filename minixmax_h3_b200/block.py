@@ -404,7 +404,16 @@ class TrainableCrossAttention(_WithRope):
 
     @torch.no_grad()
     def quantized(self, fmt: str = "int8_tensorwise", operations=None) -> CrossAttention:
-        """The layer for inference, its projections quantised to ``fmt``."""
+        """The layer for inference, its projections quantised to ``fmt``.  Their
+        products take hidden, cond_dim and heads * head_dim in multiples of
+        128 ("int8_tensorwise") or 256 ("nvfp4"); other sizes raise."""
+        step = {"int8_tensorwise": 128, "nvfp4": 256}.get(fmt)
+        if step is None:
+            raise ValueError(f"TrainableCrossAttention.quantized: format {fmt!r}")
+        sizes = (self.hidden, self.cond_dim, self.heads * self.head_dim)
+        if any(k % step for k in sizes):
+            raise ValueError(f"TrainableCrossAttention.quantized: hidden, cond_dim and heads * head_dim {sizes} "
+                             f"are not multiples of {step} ({fmt})")
         layer = CrossAttention(self.hidden, self.heads, self.head_dim, self.cond_dim, kv_heads=self.kv_heads,
                                device=self.q_proj.device, operations=operations, norm=True, norm_eps=self.norm.eps,
                                rope=self.rope)

@@ -79,3 +79,57 @@ def test_layer_built_elsewhere(cuda):
     x, cond = torch.randn(2, 9, 128, device=cuda), torch.randn(2, 5, 128, device=cuda)
     where = {"positions": torch.arange(9, device=cuda), "cond_positions": torch.arange(5, device=cuda)}
     assert torch.equal(here(x, cond, **where), there(x, cond, **where))
+
+
+# ----------------------------------------------------------------------------- quantised forms
+
+
+def test_sizes_that_cannot_be_quantised(monkeypatch):
+    """The products take K in multiples of 128 (int8) or 256 (nvfp4): said where the layer is made, not at its first call."""
+    made = []
+    monkeypatch.setattr(block, "load_quant_linear", lambda ql, w, fmt: made.append((tuple(w.shape), fmt)))
+    good = {"hidden": 256, "heads": 4, "head_dim": 64, "cond_dim": 512}
+    for fmt in ("int8_tensorwise", "nvfp4"):
+        block.TrainableCrossAttention(**good).quantized(fmt)
+    assert made == [(s, f) for f in ("int8_tensorwise", "nvfp4") for s in ((256, 256), (512, 512), (256, 256))]
+    made.clear()
+    for name, value, fmts in (("hidden", 192, ("int8_tensorwise", "nvfp4")), ("cond_dim", 160, ("int8_tensorwise", "nvfp4")),
+                              ("heads", 3, ("int8_tensorwise", "nvfp4")), ("hidden", 384, ("nvfp4",)),
+                              ("cond_dim", 128, ("nvfp4",)), ("heads", 2, ("nvfp4",))):
+        layer = block.TrainableCrossAttention(**{**good, name: value})
+        for fmt in fmts:
+            with pytest.raises(ValueError, match="multiples of"):
+                layer.quantized(fmt)
+    with pytest.raises(ValueError):
+        block.TrainableCrossAttention(**good).quantized("other")
+    assert not made
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("fmt,dtype", [("int8_tensorwise", BF16), ("int8_tensorwise", F16), ("nvfp4", BF16), ("nvfp4", F16)])
+def test_quantised_layer_is_its_parts(cuda, fmt, dtype):
+    """Of bf16 and fp16 layers, in both formats: dense, with keys encoded once, and through the 8-bit cache."""
+    torch.manual_seed(1)
+    rope = ops.Rotary.build(32, interleaved=True, device=cuda)
+    layer = block.TrainableCrossAttention(256, 4, 128, 512, kv_heads=2, rope=rope, compute_dtype=dtype, device=cuda)
+    layer.norm.weight.data.normal_(1.0, 0.1)
+    layer.norm.bias.data.normal_(0.0, 0.1)
+    q8 = layer.quantized(fmt)
+    x, cond = torch.randn(2, 37, 256, device=cuda, dtype=dtype), torch.randn(2, 21, 512, device=cuda, dtype=dtype)
+    at, cond_at = torch.arange(37, device=cuda), torch.arange(21, device=cuda) + 4
+    lens = torch.tensor([21, 9], dtype=torch.int32, device=cuda)
+    h = ops.layer_norm(x, layer.norm.weight, layer.norm.bias, layer.norm.eps)
+    q = ops.rotary(q8.q_proj(h.view(74, 256)).view(2, 37, 4, 128), None, at, rope)[0]
+    kv = q8.kv_proj(cond.view(42, 512)).view(2, 21, 2, 2, 128)
+    k, v = ops.rotary(kv[:, :, 0], None, cond_at, rope)[0], kv[:, :, 1]
+    want = q8.out_proj(ops.cross_attention(q, k, v, kv_lens=lens).view(74, 512)).view(2, 37, 256)
+    got = q8(x, cond, cond_lens=lens, positions=at, cond_positions=cond_at)
+    assert got.dtype == dtype and torch.equal(got, want)
+    kept = q8.encode(cond, cond_positions=cond_at)
+    assert torch.equal(q8(x, kv=kept, cond_lens=lens, positions=at), want)
+    cache = ops.KV8Cache.empty(2, 2, 128, device=cuda)
+    table = torch.tensor([[1], [0]], dtype=torch.int32, device=cuda)
+    q8.fill(cache, cond, table, torch.zeros(2, dtype=torch.int32, device=cuda), new_lens=lens, cond_positions=cond_at)
+    o = ops.kv8_attention(q, cache, table, lens)
+    got = q8(x, cache=cache, block_table=table, cond_lens=lens, positions=at)
+    assert torch.equal(got, q8.out_proj(o.view(74, 512)).view(2, 37, 256))
