@@ -105,13 +105,22 @@ class _Rotary(torch.autograd.Function):
     def forward(ctx, q, k, positions, rope, inverse):
         ctx.save_for_backward(positions)
         ctx.rope, ctx.inverse = rope, inverse
+        ctx.shapes = q.shape, None if k is None else k.shape
+        ctx.set_materialize_grads(False)  # zeros, for a result that nothing used, need not be turned
         return ops.rotary(q, k, positions, rope, inverse=inverse)
 
     @staticmethod
     def backward(ctx, dq, dk):
         # linear, so its gradient is the other rotation, which has one in turn
-        dq, dk = rotary(dq, dk, ctx.saved_tensors[0], ctx.rope, inverse=not ctx.inverse)
-        return dq, dk, None, None, None
+        given, wanted = (dq, dk), ctx.needs_input_grad[:2]
+        turn = [i for i in (0, 1) if wanted[i] and given[i] is not None]
+        if turn:
+            turned = rotary(given[turn[0]], given[1] if len(turn) == 2 else None, ctx.saved_tensors[0], ctx.rope,
+                            inverse=not ctx.inverse)
+        like = dk if dq is None else dq
+        grads = [turned[turn.index(i)] if i in turn else like.new_zeros(ctx.shapes[i]) if wanted[i] and like is not None
+                 else None for i in (0, 1)]
+        return *grads, None, None, None
 
 
 def rotary(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Tensor, rope: "ops.Rotary", *,

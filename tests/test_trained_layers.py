@@ -5,7 +5,7 @@ from __future__ import annotations
 import pytest
 import torch
 
-from minixmax_h3_b200 import block, modules, ops
+from minixmax_h3_b200 import attention, block, modules, ops
 
 BF16, F16 = torch.bfloat16, torch.float16
 
@@ -133,3 +133,39 @@ def test_quantised_layer_is_its_parts(cuda, fmt, dtype):
     o = ops.kv8_attention(q, cache, table, lens)
     got = q8(x, cache=cache, block_table=table, cond_lens=lens, positions=at)
     assert torch.equal(got, q8.out_proj(o.view(74, 512)).view(2, 37, 256))
+
+
+# ----------------------------------------------------------------------------- rotary's gradients
+
+
+def test_rotary_turns_only_gradients_that_are_there(monkeypatch):
+    """One of two results used, or one of two inputs that requires a gradient: the other's is not turned."""
+    turned = []
+
+    def plain(q, k, positions, rope, *, inverse=False):
+        turned.append((tuple(q.shape), None if k is None else tuple(k.shape), inverse))
+        return (-q if inverse else 2 * q), None if k is None else (-k if inverse else 2 * k)
+
+    monkeypatch.setattr(ops, "rotary", plain)
+    rope, p = ops.Rotary.build(4, device="cpu"), torch.zeros(2, dtype=torch.int32)
+    q, k = torch.randn(1, 2, 3, 8), torch.randn(1, 2, 1, 8)
+    for wanted in ("q", "k", "qk"):
+        for used in ("q", "k", "qk"):
+            a, b = q.clone().requires_grad_("q" in wanted), k.clone().requires_grad_("k" in wanted)
+            out = attention.rotary(a, b, p, rope)
+            turned.clear()
+            sum((o ** 2).sum() for o, n in zip(out, "qk") if n in used).backward()
+            there = [n for n in "qk" if n in wanted and n in used]
+            want = {0: [], 1: [(tuple((q if there == ["q"] else k).shape), None, True)],
+                    2: [(tuple(q.shape), tuple(k.shape), True)]}[len(there)]
+            assert turned == want
+            for t, n in ((a, "q"), (b, "k")):
+                if n not in wanted:
+                    assert t.grad is None
+                else:
+                    assert torch.equal(t.grad, -4 * t.detach() if n in there else torch.zeros_like(t))
+    # and their own gradients
+    a = q.clone().requires_grad_()
+    g = torch.randn_like(q).requires_grad_()
+    da, = torch.autograd.grad(attention.rotary(a, k, p, rope)[0], a, g, create_graph=True)
+    assert torch.equal(torch.autograd.grad(da, g, torch.ones_like(da))[0], 2 * torch.ones_like(q))
