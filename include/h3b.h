@@ -379,7 +379,9 @@ H3B_API int h3b_kv8_attention(const void* q, void* o, float* lse, int dtype, int
  * [b, s, kv_heads, d] by their token's position:
  *   (x1, x2) -> factor * (x1 cos a - x2 sin a, x2 cos a + x1 sin a)
  * with a = position * turns[pair] / 2^64 turns (one turn = 2 pi; whole turns
- * drop out of the 64-bit product, so any position is exact to 2^-33 turns),
+ * drop out of the 64-bit product, so with turns rounded to nearest an angle is
+ * off by |position| 2^-65 turns, 2^-34 at 2^31; its part beside the nearest
+ * quarter turn is rounded to 32 bits, 2^-28 turns at most),
  * pairs (i, i + rot/2), or (2i, 2i + 1) with interleaved != 0.  The other
  * channels are copied.  inverse != 0 turns by -a (the transpose).  The
  * product and sum are fp32, rounded once to the type.
@@ -390,8 +392,8 @@ H3B_API int h3b_kv8_attention(const void* q, void* o, float* lse, int dtype, int
  * strides); it must overlap nothing else.
  * positions: int32, or int64 with positions64 != 0; token (i, j)'s position on
  * axis x at i*pos_stride[0] + j*pos_stride[1] + x*pos_stride[2].  Pairs below
- * axis0_pairs use axis 0, the next axis1_pairs axis 1, the rest axis 2; an axis
- * without pairs is not read.  turns: [rot / 2], device.
+ * axis0_pairs use axis 0, the next axis1_pairs axis 1, the rest axis 2; axes
+ * behind the last one with pairs are not read.  turns: [rot / 2], device.
  */
 typedef struct {
   const void *q, *k;
@@ -434,9 +436,10 @@ H3B_API int h3b_layer_norm_bwd_workspace(int64_t m, int64_t n, int64_t* bytes);
  * Gradients of h3b_layer_norm_fwd: with g = dy * w,
  * dx = rstd * (g - mean(g) - xhat * mean(g * xhat)), dw = sum over rows of
  * dy * xhat, db = sum over rows of dy (dw, db: [n] of wdtype, each may be
- * NULL).  Sums are fp32 in a fixed order.  The workspace (16-byte aligned) is
- * needed only with dw or db; calls that overlap need one each.  m = 0 does
- * nothing (dw and db are not written).
+ * NULL).  Sums are fp32 in a fixed order; xhat comes from the mean as it is
+ * stored in 32 bits, so it is off by up to 2^-24 |mean| * rstd.  The workspace
+ * (16-byte aligned) is needed only with dw or db; calls that overlap need one
+ * each.  m = 0 does nothing (dw and db are not written).
  */
 typedef struct {
   const void *dy, *x, *w;

@@ -10,7 +10,11 @@
 // group of threads (forward mostly four rows by a few warps together), so the
 // variance is taken about the mean in a second pass over registers, and what
 // rounding the mean left over is taken off with it: var = mean(d^2) -
-// mean(d)^2, d = x - mean, with mean(d) of the size of a rounding.
+// mean(d)^2, d = x - mean, with mean(d) of the size of a rounding.  Forward
+// that keeps the accuracy of 32 bits for any mean.  Backward x - mean comes
+// from the mean as it is stored, one 32-bit number: xhat is off by 2^-24 |mean|
+// rstd in the whole row (5e-4 where the mean is 10^4 deviations away, as in
+// plain 32-bit arithmetic).
 //
 // The weights' gradients are sums over all rows.  Each CTA walks rows with a
 // stride and keeps its threads' columns of both sums in registers (32-bit),

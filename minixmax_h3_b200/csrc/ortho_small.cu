@@ -17,7 +17,10 @@
 // 128 x 1024 took 165 us.
 //
 // Planes hold SCALE times the value, as in ortho.cu; the result is read back
-// from them (22 bits) so that it leaves in whole rows.
+// from them (22 bits) so that it leaves in whole rows.  A sum over K stays in
+// one accumulator, up to 256 elements long (128 in ortho.cu), which the tensor
+// core cuts as often: 96 x 250 in 32 bits is off by 1.4e-6, plain 32-bit
+// products by 1.2e-6.
 #include <type_traits>
 
 #include "h3b_common.cuh"

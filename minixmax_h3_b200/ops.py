@@ -717,7 +717,7 @@ def _turns(radians: float) -> int:
 class Rotary:
     """The rotations of ``rotary``: how far a pair of channels turns at each
     position.  turns [pairs] (int64) holds radians / 2 pi as multiples of
-    2^-64 (modulo one turn), so that angles of far positions are exact;
+    2^-64 (modulo one turn), so that whole turns of far positions drop out;
     sections are the pairs that each axis of the positions turns, in order;
     factor multiplies the turned channels.  Pairs are channels (i, i + R/2) of
     the first R = 2 * pairs of a head, or (2i, 2i + 1) if interleaved."""
@@ -767,8 +767,9 @@ class Rotary:
           pair as it is and divides the slowest one by scale;
         * "by_parts": pairs that make at least ``fast`` turns over trained_len
           positions stay, those of at most ``slow`` are divided by scale, those
-          between by a share linear in the turns; the turned channels are
-          multiplied by factor, 0.1 ln(scale) + 1 if None.
+          between by a share linear in the turns (a checkpoint made with a
+          share linear in the pair's index takes ``from_frequencies``); the
+          turned channels are multiplied by factor, 0.1 ln(scale) + 1 if None.
 
         Without a factor the others leave the channels' size as it is."""
         dims = (dims,) if isinstance(dims, int) else tuple(dims)
@@ -825,8 +826,11 @@ def rotary(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Tensor, 
     turns the other way: with the same factor this is the transpose, which
     takes the gradients of the results to those of q and k
     (``attention.rotary`` does so under autograd).  Strided inputs are read in
-    place (unit last stride; other layouts are copied).  Angles are exact to
-    2^-33 of a turn at any position, results are rounded once."""
+    place (unit last stride; other layouts are copied).  Angles are off by
+    |position| 2^-65 turns at most (2^-34 at 2^31, an eighth of a turn at
+    2^62: frequencies are multiples of 2^-64), and what is left of them beside
+    the nearest quarter turn is rounded to 32 bits (2^-28 of a turn at most);
+    results are rounded once."""
     turns, sections, dtype = rope.turns, rope.sections, q.dtype
     _one_device("rotary", q, k, positions, turns, q_out, k_out)
     if dtype not in _FLOATS or (k is not None and k.dtype is not dtype):
