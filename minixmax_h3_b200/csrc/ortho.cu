@@ -762,8 +762,9 @@ H3B_DEV Scales scales(const Input& in, const Output& out, bool first) {
   const double norm = sqrt(total);
   const int e = norm > 0.0 && norm < 1e300 ? ilogb(norm) : 0;
   const int up = 10 - e;  // 2^10 = SCALE; two factors, as one would leave the range of 32 bits
-  if (first && threadIdx.x == 0)
-    out.factor[blockIdx.z] = static_cast<float>(scalbn(1.0, e) / (norm + static_cast<double>(out.eps)));
+  // (a zero matrix times 1 / eps would be NaN where that, or its square, is infinite)
+  const double all = norm > 0.0 || out.eps == 0.0f ? norm + static_cast<double>(out.eps) : 1.0;
+  if (first && threadIdx.x == 0) out.factor[blockIdx.z] = static_cast<float>(scalbn(1.0, e) / all);
   return {ldexpf(1.0f, up / 2), ldexpf(1.0f, up - up / 2)};
 }
 

@@ -233,3 +233,18 @@ def test_batches(cuda):
     for dtype in (BF16, F32):
         check(cuda, gradient(96, 700, dtype, 0.5, batch=3))
         check(cuda, gradient(200, 150, dtype, 0.5, batch=5))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [BF16, F16, F32])
+def test_zeros(cuda, dtype):
+    """Zeros for any eps above zero, beside a matrix that has values; 0 / 0 without one."""
+    for shape in ((3, 50, 90), (3, 150, 190), (3, 190, 150), (3, 700, 600)):
+        x = gradient(*shape[1:], dtype, 0.5, batch=3).to(cuda)
+        x[1] = 0
+        for eps in (1.0, 1e-7, 1e-19, 1e-30, 1e-38, 1e-44):
+            y = ops.orthogonalize(x, eps=eps)
+            assert not y[1].any() and y[0].isfinite().all() and outside(y[2], x[2], eps=eps) is None
+            assert not ops.orthogonalize(x, eps=eps, steps=0)[1].any()
+        y = ops.orthogonalize(x, eps=0.0)
+        assert y[1].isnan().all() and y[0].isfinite().all()
