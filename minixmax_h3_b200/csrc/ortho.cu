@@ -43,7 +43,7 @@
 // Tiles: 256 x 256 by CTA pairs (cta_group::2, each CTA stages 128 rows of
 // both operands); where those are too few for the SMs, 128 x 128 by one CTA;
 // where those are, too, 128 x 64 or 128 x 32 (a launch takes 1 us by itself and
-// the stores of 128 columns 3.4: five steps of 200 x 200 bf16 in 91 us, with
+// the stores of 128 columns 3.4: five steps of 200 x 200 bf16 in 92 us, with
 // 128 columns 121), or, over a long K, 128 x 128 by a cluster of two to four,
 // each with a part of K, that hand each other their sums through distributed
 // shared memory.
